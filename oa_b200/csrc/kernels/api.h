@@ -271,6 +271,30 @@ int oa_decode_attn_stream(const void* q, long long q_stride, const void* k_cache
                           int batch, int heads, int head_dim, int len, int max_seq, float scale, const int* pos_dev, void* partial,
                           int splits, int* status, void* stream);
 
+// ---- serving unequal requests (paged.cu, paged_attn.cu, sampling.cu): a cache in pages [pages, kv_heads, page_size, head_dim] of 16 to 128 tokens
+// Page tables and slot maps from request lengths.  Requests hold `cached` tokens and get `fresh` more: pages for them are taken from the
+// stack (free_pages[taken..]) into tables [batch, width], and every token t of `tokens` gets its request (rows), position and slot (-1
+// without one).  starts [batch + 1], lens [batch] = cached + fresh; `missing`: tokens that got no slot or are beyond `tokens`.
+int oa_paged_plan(const int* cached, const int* fresh, int* tables, long long table_stride, const int* free_pages, const int* taken,
+                  int* starts, int* lens, int* slots, int* positions, int* rows, int* taken_out, int* missing, int batch, int width,
+                  int n_free, int page_size, int tokens, int position0, void* stream);
+// Pages of the requests marked in done (bytes) go back on the stack; their lengths become 0.
+int oa_paged_release(const void* done, int* lens, int* tables, long long table_stride, int* free_pages, int n_free, const int* taken,
+                     int* taken_out, int batch, int width, int page_size, void* stream);
+// Packed rows x (q | k | v heads): q rotated by its position into q_out, k rotated and v into their slots.  turns: head_dim / 2 doubles in
+// HOST memory, the turns a position of each pair of dimensions, or null for no rotation.  Strides in elements.
+int oa_paged_append(int dtype, const void* x, long long row_stride, void* q_out, void* k_pages, void* v_pages, long long k_page_stride,
+                    long long v_page_stride, const int* positions, const int* slots, const void* turns, int tokens, int q_heads, int kv_heads,
+                    int head_dim, int page_size, int pages, void* stream);
+// Attention of every request's new tokens (starts, at most max_fresh each) over the shared prompt's pages and the request's own.
+int oa_paged_attn(int dtype, const void* q, long long q_stride, const void* k_pages, const void* v_pages, long long k_page_stride,
+                  long long v_page_stride, const int* tables, long long table_stride, const int* lens, const int* starts, const int* prefix_table,
+                  int prefix_len, void* out, float* lse, int tokens, int batch, int max_fresh, int q_heads, int kv_heads, int head_dim,
+                  int page_size, int pages, int width, float scale, void* stream);
+// The next token of each row of logits from its random number u in [0, 1).  temperature, top_k, top_p, min_p: [rows] or null (off).
+int oa_sample(int dtype, const void* logits, long long stride, const float* u, const float* temperature, const int* top_k, const float* top_p,
+              const float* min_p, int* tokens, float* logprobs, int rows, int vocab, void* stream);
+
 // ---- reinforcement learning (rl.cu): vector CartPole, GAE, rollout / replay storage, loss targets, categorical sampling
 int oa_rl_cartpole_reset(void* state, void* done, void* steps, void* episode, int envs, unsigned seed_lo, unsigned seed_hi,
                          int only_done, void* stream);

@@ -290,7 +290,9 @@ int oa_paged_append(int dtype, const void* x, long long row_stride, void* q_out,
 int oa_paged_attn(int dtype, const void* q, long long q_stride, const void* k_pages, const void* v_pages, long long k_page_stride,
                   long long v_page_stride, const int* tables, long long table_stride, const int* lens, const int* starts, const int* prefix_table,
                   int prefix_len, void* out, float* lse, int tokens, int batch, int max_fresh, int q_heads, int kv_heads, int head_dim,
-                  int page_size, int pages, int width, float scale, void* stream);
+                  int page_size, int pages, int width, float scale, void* scratch, int* status, void* stream);
+size_t oa_paged_attn_scratch_bytes(int dtype, int tokens, int batch, int max_fresh, int q_heads, int kv_heads, int head_dim, int pages,
+                                   int prefix_len, float scale);
 // The next token of each row of logits from its random number u in [0, 1).  temperature, top_k, top_p, min_p: [rows] or null (off).
 int oa_sample(int dtype, const void* logits, long long stride, const float* u, const float* temperature, const int* top_k, const float* top_p,
               const float* min_p, int* tokens, float* logprobs, int rows, int vocab, void* stream);

@@ -1256,6 +1256,18 @@ int make_tmap_3d_bf16(CUtensorMap* out, const void* ptr, uint64_t inner, uint64_
   return r == CUDA_SUCCESS ? OA_OK : OA_ERR_DRIVER;
 }
 
+// 3-D bf16 tensor map with a box of any three extents; strides of the two outer dimensions in bytes.
+int make_tmap_box3_bf16(CUtensorMap* out, const void* ptr, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+  PFN_encodeTiled enc = get_encode();
+  if (!enc) return OA_ERR_DRIVER;
+  if ((reinterpret_cast<uintptr_t>(ptr) & 15) || (strides[0] & 15) || (strides[1] & 15)) return OA_ERR_ALIGN;
+  const cuuint64_t d[3] = {dims[0], dims[1], dims[2]}, s[2] = {strides[0], strides[1]};
+  const cuuint32_t b[3] = {box[0], box[1], box[2]}, estr[3] = {1, 1, 1};
+  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? OA_OK : OA_ERR_DRIVER;
+}
+
 #ifdef OA_GEMM_PROBE
 extern "C" int gemm_pair_probe_read(long long* host, int n) {
   return cudaMemcpyFromSymbol(host, g_pair_probe, sizeof(long long) * (n < 512 ? n : 512)) == cudaSuccess ? OA_OK : OA_ERR_DRIVER;

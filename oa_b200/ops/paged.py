@@ -223,10 +223,14 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tab
     q = _aligned_rows(q)
     out = torch.empty((tokens, qh * hd), dtype=q.dtype, device=q.device)
     lse = torch.empty((tokens, qh), dtype=torch.float32, device=q.device) if return_lse else None
-    K._launch(N.require().oa_paged_attn(K.dt(q), q.data_ptr(), _row_stride(q), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), v_pages.stride(0),
+    lib, code = N.require(), K.dt(q)
+    # scratch of the call's own: calls on several streams do not meet in it
+    need = lib.oa_paged_attn_scratch_bytes(code, tokens, batch, max_fresh, qh, kvh, hd, pages, prefix_len, scale)
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    K._launch(lib.oa_paged_attn(code, q.data_ptr(), _row_stride(q), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), v_pages.stride(0),
                                         tables.data_ptr(), _row_stride(tables), lens.data_ptr(), starts.data_ptr(), N.ptr(prefix_table), prefix_len,
-                                        out.data_ptr(), N.ptr(lse), tokens, batch, max_fresh, qh, kvh, hd, ps, pages, tables.shape[1], scale, N.stream()),
-              "oa_paged_attn", outputs=(out,))
+                                        out.data_ptr(), N.ptr(lse), tokens, batch, max_fresh, qh, kvh, hd, ps, pages, tables.shape[1], scale, N.ptr(scratch),
+                                K.status_word(q.device).data_ptr(), N.stream()), "oa_paged_attn", 2 if need else 1, outputs=(out,))
     return (out, lse) if return_lse else out
 
 

@@ -295,7 +295,7 @@ size_t oa_paged_attn_scratch_bytes(int dtype, int tokens, int batch, int max_fre
                                    int prefix_len, float scale);
 // The next token of each row of logits from its random number u in [0, 1).  temperature, top_k, top_p, min_p: [rows] or null (off).
 int oa_sample(int dtype, const void* logits, long long stride, const float* u, const float* temperature, const int* top_k, const float* top_p,
-              const float* min_p, int* tokens, float* logprobs, int rows, int vocab, void* stream);
+              const float* min_p, int* tokens, float* logprobs, int rows, int vocab, int* status, void* stream);
 
 // ---- reinforcement learning (rl.cu): vector CartPole, GAE, rollout / replay storage, loss targets, categorical sampling
 int oa_rl_cartpole_reset(void* state, void* done, void* steps, void* episode, int envs, unsigned seed_lo, unsigned seed_hi,

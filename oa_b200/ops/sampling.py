@@ -37,7 +37,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
     tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
     logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
     K._launch(N.require().oa_sample(K.dt(logits), logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, u.data_ptr(), N.ptr(temperature), N.ptr(top_k),
-                                    N.ptr(top_p), N.ptr(min_p), tokens.data_ptr(), logprobs.data_ptr(), rows, vocab, N.stream()), "oa_sample")
+                                    N.ptr(top_p), N.ptr(min_p), tokens.data_ptr(), logprobs.data_ptr(), rows, vocab,
+                                    K.status_word(logits.device).data_ptr(), N.stream()), "oa_sample")
     return tokens, logprobs
 
 

@@ -31,13 +31,14 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return x != x ? 0x007fffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 constexpr uint32_t KEY_NONE = 0x007fffffu;   // of -inf
+constexpr float LOWEST = -3.402823466e38f;   // the lowest logit that counts
 
 __device__ __forceinline__ float load_logit(const float* p) { return *p; }
 __device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
 struct Weigh {
   float max, inv_t;
-  __device__ __forceinline__ float scaled(float x) const { return x == max ? 0.f : (x - max) * inv_t; }
+  __device__ __forceinline__ float scaled(float x) const { return x == max ? 0.f : __fmul_rn(x - max, inv_t); }
   __device__ __forceinline__ float weight(float x) const { return x != x || x == -INFINITY ? 0.f : expf(scaled(x)); }
 };
 // floor(w * 2^40) for w in [0, 1] as two numbers of 20 bits: sums of up to 4096 of either fit 32 bits.  Adding 2^23 rounded down leaves a
@@ -175,16 +176,19 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SamplePara
 
 // ------------------------------------------------------------------------------------------------ a cluster of CTAs for a row
 // A row is read once, by up to eight CTAs of a cluster that keep it in shared memory; every later pass is over those copies.  A warp owns
-// neighbouring tokens, fetched by a bulk copy of its own, and a lane 16 bytes of them at a time.
-//   1  maximum of each thread, warp, CTA, cluster.  A greedy row ends here.
-//   2  top-k up to 512: the k-th largest of the threads' maxima is no larger than the k-th largest logit, so that what lies in its bin of
-//      (max - x) or above holds the top k, and little more; those tokens meet in the leading CTA, which sorts them.
-//   3  top-p (and larger top-k): masses in 1024 bins of y; the bin in which the wanted mass is reached goes to the leading CTA, which sorts it.
-//      A token of weight below (1 - p) / (2 V) is never kept: all such ones together have less than the mass to be cut off, as the
-//      maximum's weight is 1.  Those take no part.
-//      Bins too full for the list (equal logits, above all) are left to a search over keys and indices, 50 passes in shared memory.
-//   4  mass of what is kept for each warp, prefix sums over warps and CTAs, and the warp in whose stretch u falls looks again.
-constexpr int ROW_BINS = 1024, ROW_LIST = 1024, ROW_BRIEF_K = 512;
+// neighbouring tokens, fetched by a bulk copy of its own, a lane 16 bytes of them at a time; warps in the order of their CTAs own the
+// vocabulary in order, so that a number from each warp (a maximum, a mass), sent to every CTA, says who has the first of something.
+//   1  maximum of each thread, of all warps.  A greedy row ends here.
+//   2  top-k up to 256: the k-th largest of the threads' maxima is no larger than the k-th largest logit, so that what is not below its bin of
+//      (max - x) contains the top k, and little more.  Those tokens go to the first CTA, which sorts them, makes all cuts and samples; the
+//      other CTAs are done.
+//   3  top-p (and larger top-k): masses (counts) in 512 bins of t, which falls with x; the bin in which the wanted sum is reached is cut into 512
+//      again while it holds more than a list does; its tokens go to the first CTA, which sorts them and says where the cut is.
+//      A token of weight below (1 - p) / (2 V) is never kept: all such ones together have less than the mass that is cut off, as the
+//      maximum's weight is 1.  Those take no part.  Equal logits that no bins separate are left to a search over keys and indices, 50 passes.
+//   4  mass of what is kept for each warp, and the warp in whose stretch u falls looks again.
+constexpr int ROW_LIST = 512, ROW_BRIEF_K = 256, ROW_WARPS = SAMPLE_THREADS / 32;
+static_assert(ROW_LIST == SAMPLE_THREADS, "an entry of the list, and a bin, to a thread");
 
 template <typename T> struct Lane16;
 template <> struct Lane16<float> {
@@ -203,35 +207,49 @@ template <> struct Lane16<__nv_bfloat16> {
     for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
   }
 };
-
-__device__ __forceinline__ uint32_t cluster_add(uint32_t addr, uint32_t v) {
-  uint32_t r;
-  asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(r) : "r"(addr), "r"(v) : "memory");
-  return r;
+template <int N> __device__ __forceinline__ float highest(const float* v) {
+  float m = v[0];
+#pragma unroll
+  for (int k = 1; k < N; ++k) m = fmaxf(m, v[k]);
+  return m;
 }
+
 __device__ __forceinline__ void cluster_st(uint32_t addr, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory"); }
+__device__ __forceinline__ void cluster_st32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ u64 cluster_ld(uint32_t addr) {
   u64 v;
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ u64 warp_scan(u64 v, int lane) {      // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const u64 u = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += u; }
+  return v;
+}
+__device__ __forceinline__ u64 warp_total(u64 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key); }
 
 struct RowShared {
-  u64 exchange[2][8];                      // a number of each CTA of the cluster, in two sets used in turn
-  u64 red[SAMPLE_THREADS / 32];
-  u64 cut;                                 // from the leader: key and index, or a bin and what lies before it
-  u64 base;
-  uint64_t bars[SAMPLE_THREADS / 32];
-  uint32_t listed;
+  u64 slots[2][8 * ROW_WARPS];             // a number of each warp of the cluster, in two sets used in turn
+  u64 red[ROW_WARPS];
+  u64 cut, base;                           // where a cut is; a bin and the sum before it
+  u64 far_cut;                             // the first CTA's word to the others
+  uint64_t bars[ROW_WARPS];
+  int listed, bin;
 };
 
 template <typename T>
 __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const SampleParams p, int span, int* status) {
-  constexpr int N16 = Lane16<T>::N, WARPS = SAMPLE_THREADS / 32;
+  constexpr int N16 = Lane16<T>::N;
   extern __shared__ __align__(16) uint8_t row_smem[];
   __shared__ RowShared sh;
-  u64* bins = reinterpret_cast<u64*>(row_smem);                  // [ROW_BINS], and later, in the leader, the list [ROW_LIST]
-  uint8_t* data = row_smem + ROW_BINS * sizeof(u64);
+  u64* bins = reinterpret_cast<u64*>(row_smem);                  // [512]; later, in the first CTA, the list of all
+  u64* own_list = bins + ROW_LIST;                               // tokens of this CTA
+  uint8_t* data = row_smem + 2 * ROW_LIST * sizeof(u64);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t ctas;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
@@ -239,6 +257,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
   const int row = blockIdx.x / ctas, V = p.vocab;
   pdl_launch_dependents();
   if (lane == 0) { mbar_init(&sh.bars[warp], 1); mbar_fence_init(); }
+  bins[tid] = 0;
+  for (int i = tid; i < 2 * 8 * ROW_WARPS; i += SAMPLE_THREADS) sh.slots[0][i] = 0;
+  if (tid == 0) sh.listed = 0;
   __syncwarp();
   pdl_wait();
 
@@ -248,340 +269,380 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
   const int skew = (int)((reinterpret_cast<uintptr_t>(x + lo) & 15) / sizeof(T));
   const int first = lo - skew;                                   // token at place 0
   const int s0 = warp * span, s1 = s0 + span;                    // this warp's places
-  const int a = min(max(s0, skew), s1), b = max(min(s1, hi - first), a);          // of them [a, b) hold tokens
-  const int a16 = min((a + N16 - 1) / N16 * N16, b), b16 = max(b / N16 * N16, a16);
   T* places = reinterpret_cast<T*>(data);
-  if (b16 > a16 && lane == 0) {
-    mbar_expect_tx(&sh.bars[warp], (uint32_t)(b16 - a16) * sizeof(T));
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(places + a16)), "l"(x + first + a16),
-                 "r"((uint32_t)(b16 - a16) * (uint32_t)sizeof(T)), "r"(smem_u32(&sh.bars[warp])) : "memory");
+  {
+    const int a = min(max(s0, skew), s1), b = max(min(s1, hi - first), a);        // of them [a, b) hold tokens
+    const int a16 = min((a + N16 - 1) / N16 * N16, b), b16 = max(b / N16 * N16, a16);
+    if (b16 > a16 && lane == 0) {
+      mbar_expect_tx(&sh.bars[warp], (uint32_t)(b16 - a16) * sizeof(T));
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(places + a16)), "l"(x + first + a16),
+                   "r"((uint32_t)(b16 - a16) * (uint32_t)sizeof(T)), "r"(smem_u32(&sh.bars[warp])) : "memory");
+    }
+    const auto by_hand = [&](int i) { if (i >= a && i < b) places[i] = x[first + i]; else places[i] = T(-INFINITY); };
+    for (int i = s0 + lane; i < a16; i += 32) by_hand(i);        // ends off 16 bytes, and places without a token
+    for (int i = b16 + lane; i < s1; i += 32) by_hand(i);
+    if (ctas > 1) cluster_sync_all(); else __syncthreads();      // every CTA of the cluster is there before anything is written to it
+    if (b16 > a16 && !warp_wait(&sh.bars[warp], 0) && lane == 0) report_error(status, OA_KERR_WAIT_FULL);
   }
-  const auto by_hand = [&](int i) { if (i >= a && i < b) places[i] = x[first + i]; else places[i] = T(-INFINITY); };
-  for (int i = s0 + lane; i < a16; i += 32) by_hand(i);          // ends off 16 bytes, and places without a token
-  for (int i = b16 + lane; i < s1; i += 32) by_hand(i);
-  if (ctas > 1) cluster_sync_all();                              // every CTA of the cluster is there before anything is written to it
-  __syncwarp();
-  bool fine = true;
-  if (b16 > a16) fine = warp_wait(&sh.bars[warp], 0);
-  if (!fine && lane == 0) report_error(status, OA_KERR_WAIT_FULL);
-  // every pass: f(token, logit) for the tokens of this lane, 16 bytes at a time
+  const auto meet = [&] { if (ctas > 1) cluster_sync_all(); else __syncthreads(); };
+  // a pass: f(place, N16 logits) for 16 bytes of this lane at a time
   const auto each = [&](auto f) {
     for (int c = s0 + lane * N16; c < s1; c += 32 * N16) {
       float v[N16];
       Lane16<T>::get(data + c * sizeof(T), v);
-#pragma unroll
-      for (int k = 0; k < N16; ++k) f(first + c + k, v[k]);
+      f(c, v);
     }
   };
-  const auto sum = [](u64 u, u64 v) { return u + v; };
-  const auto top = [](u64 u, u64 v) { return u > v ? u : v; };
-  int turn = 0;
-  // op over the whole cluster, the result to all
-  const auto cluster_all = [&](u64 v, auto op) {
-    v = block_all(v, sh.red, op);
-    if (ctas == 1) return v;
-    turn ^= 1;
-    if (tid < (int)ctas) cluster_st(map_to_cta(smem_u32(&sh.exchange[turn][rank]), tid), v);
-    cluster_sync_all();
-    v = sh.exchange[turn][0];
-    for (uint32_t r = 1; r < ctas; ++r) v = op(v, sh.exchange[turn][r]);
-    return v;
+  // a pass for which most of 16 bytes is nothing: f(token, logit) where the logit is not below `floor`
+  const auto each_from = [&](float floor, auto f) {
+    each([&](int c, const float* v) {
+      if (!(highest<N16>(v) >= floor)) return;
+#pragma unroll
+      for (int k = 0; k < N16; ++k)
+        if (v[k] >= floor && v[k] > -INFINITY) f(first + c + k, v[k]);
+    });
   };
-  const auto meet = [&] { if (ctas > 1) cluster_sync_all(); else __syncthreads(); };
+  int turn = 0;
+  // Every warp's number to every CTA; then, to each warp, the sum of the numbers before its own and of all.
+  const auto share_sums = [&](u64 mine, u64& before, u64& all) {
+    turn ^= 1;
+    if (lane < (int)ctas) cluster_st(map_to_cta(smem_u32(&sh.slots[turn][rank * ROW_WARPS + warp]), lane), mine);
+    meet();
+    u64 v[4], sum = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { v[k] = lane * 4 + k < (int)ctas * ROW_WARPS ? sh.slots[turn][lane * 4 + k] : 0; sum += v[k]; }
+    u64 at = warp_scan(sum, lane);
+    all = __shfl_sync(0xffffffffu, at, 31);
+    at -= sum;
+    const int me = rank * ROW_WARPS + warp;
+    u64 upto = at;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) if (k < (me & 3)) upto += v[k];
+    before = __shfl_sync(0xffffffffu, upto, me >> 2);
+  };
 
   // ---- 1
   float high = -INFINITY;                                        // of this thread; NaN is passed over
-  each([&](int, float v) { high = fmaxf(high, v); });
-  const uint32_t top_key = (uint32_t)cluster_all(key_of(high), top);
+  each([&](int, const float* v) { high = fmaxf(high, highest<N16>(v)); });
+  uint32_t top_key;
+  int first_warp;                                                // the first that has the maximum
+  {
+    const uint32_t mine = __reduce_max_sync(0xffffffffu, key_of(high));
+    turn ^= 1;
+    if (lane < (int)ctas) cluster_st(map_to_cta(smem_u32(&sh.slots[turn][rank * ROW_WARPS + warp]), lane), mine);
+    meet();
+    uint32_t k[4], best = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { k[i] = lane * 4 + i < (int)ctas * ROW_WARPS ? (uint32_t)sh.slots[turn][lane * 4 + i] : 0; best = max(best, k[i]); }
+    top_key = __reduce_max_sync(0xffffffffu, best);
+    int w = 8 * ROW_WARPS;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) if (k[i] == top_key) w = lane * 4 + i;
+    first_warp = (int)__reduce_min_sync(0xffffffffu, (unsigned)w);
+  }
   const float t = p.temperature ? p.temperature[row] : 1.f;
-  const bool none = top_key <= KEY_NONE;
-  if (none || !(t > 0.f)) {
-    u64 best = 0;
-    if (!none) {
-      each([&](int i, float v) { if (key_of(v) == top_key) best = top(best, (uint32_t)~i); });
-      best = cluster_all(best, top);
-    }
-    if (rank == 0 && tid == 0) {
-      p.tokens[row] = none ? -1 : (int)~(uint32_t)best;
-      p.logprobs[row] = none ? -INFINITY : 0.f;
-    }
+  float peak = logit_of(top_key);
+  if (top_key <= KEY_NONE) {
+    if (rank == 0 && tid == 0) { p.tokens[row] = -1; p.logprobs[row] = -INFINITY; }
     return;
   }
-  const float peak = __uint_as_float((top_key & 0x80000000u) ? top_key & 0x7fffffffu : ~top_key);
-  const Weigh wt{peak, peak == INFINITY ? 1.f : 1.f / t};
-  uint32_t key = KEY_NONE + 1;                                   // kept: keys above, and of those equal the indices up to idx
-  int idx = V - 1;
-  const auto in = [&](uint32_t k, int i) { return k > key || (k == key && i <= idx); };
-  const uint32_t list_at = map_to_cta(smem_u32(bins), 0), listed_at = map_to_cta(smem_u32(&sh.listed), 0);
-  // Tokens for which pred holds go to the leader's list, in any order; returns how many there were (more than ROW_LIST: not all are there).
-  const auto collect = [&](auto pred) {
-    if (rank == 0 && tid == 0) sh.listed = 0;
-    meet();
-    each([&](int i, float v) {
-      const uint32_t k = key_of(v);
-      const bool yes = k > KEY_NONE && in(k, i) && pred(v);
-      const unsigned who = __ballot_sync(0xffffffffu, yes);
-      if (who) {
-        uint32_t at = 0;
-        if (lane == 0) at = cluster_add(listed_at, __popc(who));
-        at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
-        if (yes && at < ROW_LIST) cluster_st(list_at + at * 8, ((u64)k << 32) | (uint32_t)~i);
-      }
+  if (!(t > 0.f)) {
+    if (first_warp != (int)rank * ROW_WARPS + warp) return;
+    unsigned at = 0xffffffffu;
+    each([&](int c, const float* v) {
+#pragma unroll
+      for (int k = N16 - 1; k >= 0; --k) if (v[k] == peak) at = min(at, (unsigned)(first + c + k));
     });
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0) { p.tokens[row] = (int)at; p.logprobs[row] = 0.f; }
+    return;
+  }
+  const float inv_t = fminf(1.f / t, -LOWEST);
+  if (peak == INFINITY) {                                        // only those that are infinite count: 0 for them, nothing for the others
+    for (int i = s0 + lane; i < s1; i += 32) places[i] = load_logit(places + i) == INFINITY ? T(0.f) : T(-INFINITY);
+    __syncwarp();
+    high = high == INFINITY ? 0.f : -INFINITY;
+    peak = 0.f;
+    top_key = key_of(0.f);
+  }
+  // products that are never joined with an addition behind them: bins, and the rule itself, are of the rounded numbers
+  const auto scaled = [&](float v) { return __fmul_rn(v - peak, inv_t); };
+  const auto weight = [&](float v) { return expf(scaled(v)); };
+  float from = -INFINITY;                                        // kept: logits above, and of those equal the indices up to idx
+  int idx = V - 1;
+  const auto in = [&](int i, float v) { return v > from || (v == from && i <= idx); };
+  const auto cut_at = [&](u64 entry) { from = logit_of((uint32_t)(entry >> 32)); idx = (int)~(uint32_t)entry; };
+  // Tokens with logits from `floor` on for which pred holds go to the first CTA's list, in any order; returns how many there are.  With more than
+  // ROW_LIST the list is of no use.
+  const auto collect = [&](float floor, auto pred) {
+    each_from(floor, [&](int i, float v) {
+      if (!in(i, v) || !pred(v)) return;
+      const int at = atomicAdd(&sh.listed, 1);
+      if (at < ROW_LIST) own_list[at] = ((u64)key_of(v) << 32) | (uint32_t)~i;
+    });
+    __syncthreads();
+    const int mine = sh.listed;
+    u64 before, all;
+    share_sums(warp == 0 ? (u64)mine : 0, before, all);          // a CTA's number stands with its first warp
+    if (tid == 0) { sh.base = before; sh.listed = 0; }
+    __syncthreads();
+    if (all <= ROW_LIST && tid < mine) cluster_st(map_to_cta(smem_u32(bins + sh.base + tid), 0), own_list[tid]);
     meet();
-    return rank == 0 ? (int)sh.listed : 0;
+    return (int)min(all, (u64)ROW_LIST + 1);
   };
-  // The leader's list into the ranking's order.
+  // The first n entries of bins into falling order.
   const auto sort_list = [&](int n) {
     int size = 64;
     while (size < n) size <<= 1;
-    for (int i = n + tid; i < size; i += SAMPLE_THREADS) bins[i] = 0;
+    if (tid >= n && tid < size) bins[tid] = 0;
     __syncthreads();
-    for (int k = 2; k <= size; k <<= 1) {
-      for (int j = k >> 1; j > 0; j >>= 1) {
+    for (int lk = 1; 1 << lk <= size; ++lk) {
+      for (int lj = lk - 1; lj >= 0; --lj) {
         if (tid < size / 2) {
-          const int i = 2 * j * (tid / j) + tid % j;
-          const u64 u = bins[i], v = bins[i + j];
-          if ((u < v) == ((i & k) == 0)) { bins[i] = v; bins[i + j] = u; }
+          const int i = ((tid >> lj) << (lj + 1)) | (tid & ((1 << lj) - 1)), o = i + (1 << lj);
+          const u64 u = bins[i], v = bins[o];
+          if ((u < v) == (((i >> lk) & 1) == 0)) { bins[i] = v; bins[o] = u; }
         }
-        if (j > 32) __syncthreads(); else __syncwarp();          // up to a distance of 32 a warp's pairs lie in 64 entries of its own
+        if (lj > 5) __syncthreads(); else __syncwarp();          // up to a distance of 32 a warp's pairs lie in 64 entries of its own
       }
-      __syncthreads();
+      if (lk >= 6) __syncthreads();
     }
+    __syncthreads();
   };
-  // Of the sorted list's first n: the mass before entry `tid` and before entry `tid + SAMPLE_THREADS`.
-  const auto list_masses = [&](int n, u64* before, u64& total) {
-    u64 m[2], run = 0;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int i = tid + r * SAMPLE_THREADS;
-      const uint32_t k = i < n ? (uint32_t)(bins[i] >> 32) : 0;
-      m[r] = i < n ? mass_of(wt.weight(__uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k))) : 0;
-      u64 inc = m[r];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const u64 u = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += u; }
-      __syncthreads();
-      if (lane == 31) sh.red[warp] = inc;
-      __syncthreads();
-      u64 all = 0, prior = 0;
-      for (int w = 0; w < WARPS; ++w) { if (w < warp) prior += sh.red[w]; all += sh.red[w]; }
-      before[r] = run + prior + inc - m[r];
-      run += all;
-    }
-    total = run;
+  // Sums over a block in thread order: what is before this thread, and all.
+  const auto block_scan = [&](u64 v, u64& all) {
+    const u64 inc = warp_scan(v, lane);
+    __syncthreads();
+    if (lane == 31) sh.red[warp] = inc;
+    __syncthreads();
+    const u64 r = lane < ROW_WARPS ? sh.red[lane] : 0, up = warp_scan(r, lane);
+    all = __shfl_sync(0xffffffffu, up, ROW_WARPS - 1);
+    return __shfl_sync(0xffffffffu, up - r, warp) + inc - v;
   };
-  // The leader tells where the list's first n end.
-  const auto cut_after = [&](int n) {
-    if (rank == 0) {
-      __syncthreads();
-      if (tid < (int)ctas) cluster_st(map_to_cta(smem_u32(&sh.cut), tid), bins[n - 1]);
-    }
-    meet();
-    key = (uint32_t)(sh.cut >> 32);
-    idx = (int)~(uint32_t)sh.cut;
+  // The sums of all CTAs' bins, a bin to a thread; then the first bin in which the running sum is enough, and the sum before it.  Returns
+  // false when no bin is.
+  const auto find_bin = [&](u64 base, auto enough, int& bin, u64& before, u64& all) {
+    if (tid == 0) sh.bin = -1;
+    meet();                                                      // all bins are filled
+    const uint32_t at = smem_u32(bins + tid);
+    u64 v = 0;
+    for (uint32_t c = 0; c < ctas; ++c) { const u64 pair = cluster_ld(map_to_cta(at, c)); v += ((pair >> 32) << 20) + (uint32_t)pair; }
+    const u64 run = base + block_scan(v, all);
+    if (enough(run + v) && !enough(run)) { sh.bin = tid; sh.base = run; }
+    __syncthreads();
+    bin = sh.bin;
+    before = sh.base;
+    return bin >= 0;
+  };
+  // What a bin holds are two sums of 32 bits, in units of 1 and 2^20.  A bin of very many large weights overflows, which shows in the sum of all.
+  const auto add_to_bin = [&](int bin, Mass20 m) {
+    uint32_t* at = reinterpret_cast<uint32_t*>(bins + bin);
+    atomicAdd(at, m.lo);
+    if (m.hi) atomicAdd(at + 1, m.hi);
   };
   // Slow and sure: the largest key, and of the tokens with it the lowest index, for which enough(f over what is up to there) holds.
   const auto search = [&](auto f, auto enough) {
-    const auto measure = [&](auto part) {
-      u64 s = 0;
-      each([&](int i, float v) { const uint32_t k = key_of(v); if (k > KEY_NONE && in(k, i) && part(k, i)) s += f(v); });
-      return cluster_all(s, sum);
+    const auto measure = [&](float floor, auto part) {
+      u64 s = 0, before, all;
+      each_from(floor, [&](int i, float v) { if (in(i, v) && part(i, v)) s += f(v); });
+      share_sums(warp_total(s), before, all);
+      return all;
     };
-    uint32_t low = key;
+    uint32_t low = key_of(from) > KEY_NONE ? key_of(from) : KEY_NONE + 1;
+    const uint32_t start = low;
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t c = low + (1u << bit);
       if (c < low || c > top_key) continue;
-      if (enough(measure([&](uint32_t k, int) { return k >= c; }))) low = c;
+      if (enough(measure(logit_of(c), [](int, float) { return true; }))) low = c;
     }
-    int up = low == key ? idx : V - 1, down = 0;
+    const float at = logit_of(low);
+    int up = low == start ? idx : V - 1, down = 0;
     while (down < up) {
       const int mid = (down + up) >> 1;
-      if (enough(measure([&](uint32_t k, int i) { return k > low || (k == low && i <= mid); }))) up = mid;
+      if (enough(measure(at, [&](int i, float v) { return v > at || i <= mid; }))) up = mid;
       else down = mid + 1;
     }
-    key = low;
+    from = at;
     idx = up;
   };
-  // From the leader to all: the list's length was too large
-  const auto agreed = [&](int n) { return (int)cluster_all(rank == 0 && tid == 0 ? (u64)n : 0, sum); };
-  // First bin in which a running sum over the cluster's bins meets enough(); ROW_BINS if there is none.  `base`: the sum before it.
-  const auto find_bin = [&](auto enough, u64& base) {
-    meet();                                                      // all bins are filled
-    if (rank == 0) {
-      u64 v[2], run = 0;
-      if (tid == 0) { sh.cut = ROW_BINS; sh.base = 0; }
-      __syncthreads();
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t at = smem_u32(bins + tid + r * SAMPLE_THREADS);
-        v[r] = 0;
-        for (uint32_t c = 0; c < ctas; ++c) v[r] += cluster_ld(map_to_cta(at, c));
-        u64 inc = v[r];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const u64 u = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += u; }
-        __syncthreads();
-        if (lane == 31) sh.red[warp] = inc;
-        __syncthreads();
-        u64 all = 0, prior = 0;
-        for (int w = 0; w < WARPS; ++w) { if (w < warp) prior += sh.red[w]; all += sh.red[w]; }
-        const u64 upto = run + prior + inc;
-        if (enough(upto) && !enough(upto - v[r])) { sh.cut = tid + r * SAMPLE_THREADS; sh.base = upto - v[r]; }
-        run += all;
+  // Cuts what is kept to the shortest head of the ranking whose sum of f is enough.  place(v) falls with v from 0 on in steps of bins; tokens at
+  // ROW_LIST or more of it take no part in the first pass of bins, which the caller has made (their sum: `binned`), and are not reached.
+  const auto cut_by_bins = [&](u64 binned, auto place, auto f, auto enough) {
+    u64 base = 0, all;
+    float origin = 0.f, zoom = 1.f;                              // bins of this pass: (place - origin) * zoom
+    for (int pass = 0; pass < 3; ++pass) {
+      int bin;
+      u64 before;
+      const bool there = find_bin(base, enough, bin, before, all);
+      if (!there || all != binned) break;                        // a bin has overflowed, or all was cut off
+      base = before;
+      const float o = origin, z = zoom;
+      const auto mine = [&](float v) { const float s = (place(v) - o) * z; return s >= 0.f && s < (float)ROW_LIST && (int)s == bin; };
+      const int n = collect(LOWEST, mine);
+      if (n > 0 && n <= ROW_LIST) {
+        if (rank == 0) {
+          sort_list(n);
+          u64 m = tid < n ? (u64)f(logit_of((uint32_t)(bins[tid] >> 32))) : 0, total;
+          const u64 run = base + block_scan(m, total);
+          if (tid < n && !enough(run) && (enough(run + m) || tid == n - 1)) sh.cut = bins[tid];
+          __syncthreads();
+          if (tid < (int)ctas) cluster_st(map_to_cta(smem_u32(&sh.far_cut), tid), sh.cut);
+        }
+        meet();
+        cut_at(sh.far_cut);
+        return;
       }
+      if (pass == 2 || n == 0) break;
+      // the bin again, in as many: the next bits of place
+      origin = o + (float)bin / z;
+      zoom = z * (float)ROW_LIST;
+      bins[tid] = 0;
       __syncthreads();
-      const u64 bin = sh.cut, before = sh.base;
-      if (tid > 0 && tid < (int)ctas) { cluster_st(map_to_cta(smem_u32(&sh.cut), tid), bin); cluster_st(map_to_cta(smem_u32(&sh.base), tid), before); }
+      u64 sum = 0, prior;
+      each_from(LOWEST, [&](int i, float v) {
+        if (!in(i, v) || !mine(v)) return;
+        const u64 m = f(v);
+        sum += m;
+        add_to_bin((int)fminf((place(v) - origin) * zoom, (float)(ROW_LIST - 1)), {(uint32_t)(m >> 20), (uint32_t)m & 0xfffffu});
+      });
+      share_sums(warp_total(sum), prior, binned);
     }
-    meet();
-    base = sh.base;
-    return (int)sh.cut;
+    search(f, enough);
   };
-  const auto clear_bins = [&] {
-    for (int i = tid; i < ROW_BINS; i += SAMPLE_THREADS) bins[i] = 0;
-    __syncthreads();
+  const float least = p.min_p ? fminf(p.min_p[row], 1.f) : 0.f;
+  const float u01 = p.u[row];
+  const auto target = [&](u64 S) -> u64 {
+    const double at = floor((double)u01 * (double)S);
+    return !(at > 0.0) ? 0 : at >= (double)S ? S - 1 : min((u64)at, S - 1);
+  };
+  const auto answer = [&](int token, float v, u64 S) {
+    p.tokens[row] = token;
+    p.logprobs[row] = scaled(v) - (float)log((double)S / 1099511627776.0);
   };
 
   // ---- 2
   const int want = p.top_k ? p.top_k[row] : 0;
   const float top_p = p.top_p ? p.top_p[row] : 1.f;
   const double dp = (double)top_p;
-  bool cut_p = !(top_p >= 1.f);
-  if (want > 0 && want < V) {
-    const auto by_gap = [&](float v) { return v == peak ? 0 : (int)fminf((peak - v) * 32.f, (float)(ROW_BINS - 1)); };
-    const auto enough = [&](u64 n) { return n >= (u64)want; };
-    int n = ROW_LIST + 1;
-    if (want <= ROW_BRIEF_K) {
-      clear_bins();
-      if (key_of(high) > KEY_NONE) atomicAdd(&bins[by_gap(high)], 1ull);
-      u64 base;
-      const int bin = min(find_bin(enough, base), ROW_BINS - 1);
-      n = agreed(collect([&](float v) { return by_gap(v) <= bin; }));
+  const bool cut_p = !(top_p >= 1.f);
+  const auto place_of_gap = [&](float v) { return fminf(__fmul_rn(peak - v, 16.f), (float)ROW_LIST - 0.5f); };      // 32 of logits, all beyond in the last
+  bool brief = V <= ROW_LIST && ((want > 0 && want < V) || cut_p);
+  float floor = LOWEST;
+  if (!brief && want > 0 && want <= ROW_BRIEF_K && want < V) {
+    brief = true;
+    if (high > -INFINITY) atomicAdd(reinterpret_cast<uint32_t*>(bins + (int)place_of_gap(high)), 1u);
+    int bin;
+    u64 before, all;
+    if (find_bin(0, [&](u64 n) { return n >= (u64)want; }, bin, before, all) && bin < ROW_LIST - 1) {
+      const float gap = (float)(bin + 1) * (1.f / 16.f);
+      floor = fmaxf(peak - gap - (fabsf(peak) + gap) * 0x1p-20f, floor);                    // below the bin, whatever was rounded
     }
+  }
+  if (brief) {
+    const int n = collect(floor, [](float) { return true; });
     if (n <= ROW_LIST) {
-      int keep = min(want, n);                                   // fewer than wanted: the others are -inf
-      if (rank == 0) {
-        sort_list(n);
-        if (cut_p) {
-          u64 before[2], total;
-          list_masses(keep, before, total);
-          const double part = dp * (double)total;
-          const u64 inside = (tid < keep && (double)before[0] < part) + (tid + SAMPLE_THREADS < keep && (double)before[1] < part);
-          const int fewer = (int)block_all(inside, sh.red, sum);
-          keep = fewer > 1 ? fewer : 1;
-        }
-      }
-      cut_after(keep);
-      cut_p = false;
-    } else {
-      u64 have = 0;
-      each([&](int i, float v) { have += key_of(v) > KEY_NONE; });
-      if (cluster_all(have, sum) > (u64)want) {
-        clear_bins();
-        each([&](int i, float v) { if (key_of(v) > KEY_NONE) atomicAdd(&bins[by_gap(v)], 1ull); });
-        u64 base;
-        const int bin = find_bin(enough, base);
-        n = agreed(collect([&](float v) { return by_gap(v) == bin; }));
-        if (n <= ROW_LIST) {
-          if (rank == 0) sort_list(n);
-          cut_after(want - (int)base);
-        } else {
-          search([](float) { return 1ull; }, enough);
-        }
-      }
+      if (rank != 0) return;
+      sort_list(n);
+      int keep = want > 0 ? min(want, n) : n;
+      const float w = tid < keep ? weight(logit_of((uint32_t)(bins[tid] >> 32))) : 0.f;
+      const u64 m = mass_of(w);
+      u64 S;
+      const u64 run = block_scan(m, S);
+      const double part = dp * (double)S;
+      const bool stays = tid < keep && (tid == 0 || ((!cut_p || (double)run < part) && w >= least));      // both cuts leave a head of the ranking
+      keep = __syncthreads_count(stays);
+      const u64 entry = tid < keep ? bins[tid] : 0;
+      __syncthreads();
+      if (tid < keep) bins[tid] = (entry << 32) | (entry >> 32);                             // the lowest index first
+      sort_list(keep);
+      const u64 e = tid < keep ? bins[tid] : 0;
+      const float v = logit_of((uint32_t)e);
+      const u64 mine = tid < keep ? mass_of(weight(v)) : 0, at = block_scan(mine, S), r = target(S);
+      if (r >= at && r < at + mine) answer((int)~(uint32_t)(e >> 32), v, S);
+      return;
     }
+  }
+  if (want > 0 && want < V) {
+    u64 have = 0, before, all;
+    bins[tid] = 0;
+    __syncthreads();
+    each_from(LOWEST, [&](int, float v) {
+      ++have;
+      atomicAdd(reinterpret_cast<uint32_t*>(bins + (int)place_of_gap(v)), 1u);
+    });
+    share_sums(warp_total(have), before, all);
+    if (all > (u64)want) cut_by_bins(all, place_of_gap, [](float) { return 1ull; }, [&](u64 n) { return n >= (u64)want; });
   }
   // ---- 3
   if (cut_p) {
-    const float floor_w = fminf(fmaxf((float)(0.5 * (1.0 - dp) / V), 5e-13f), 0.5f), deep = logf(floor_w), scale = (float)ROW_BINS / -deep;
-    const auto by_y = [&](float y) { return (int)fminf(-y * scale, (float)(ROW_BINS - 1)); };
-    clear_bins();
-    u64 mine = 0;
-    each([&](int i, float v) {
-      const uint32_t k = key_of(v);
-      if (!(k > KEY_NONE && in(k, i))) return;
-      const float y = wt.scaled(v);
-      const u64 m = mass_of(expf(y));
-      mine += m;
-      if (y > deep) atomicAdd(&bins[by_y(y)], m);
-    });
-    const double part = dp * (double)cluster_all(mine, sum);
-    const auto enough = [&](u64 m) { return m > 0 && !((double)m < part); };
-    u64 base;
-    const int bin = find_bin(enough, base);
-    const int n = agreed(collect([&](float v) { const float y = wt.scaled(v); return y > deep && by_y(y) == bin; }));
-    if (n > 0 && n <= ROW_LIST) {
-      int keep = 1;
-      if (rank == 0) {
-        sort_list(n);
-        u64 before[2], total;
-        list_masses(n, before, total);
-        const u64 inside = (tid < n && (double)(base + before[0]) < part) + (tid + SAMPLE_THREADS < n && (double)(base + before[1]) < part);
-        keep = max((int)block_all(inside, sh.red, sum), 1);
+    const float never = fminf(fmaxf((float)(0.5 * (1.0 - dp) / V), 5e-13f), 0.5f), scale = (float)ROW_LIST / -logf(never);
+    const auto place = [&](float v) { return __fmul_rn(-scaled(v), scale); };
+    bins[tid] = 0;
+    __syncthreads();
+    uint32_t hi_in = 0, lo_in = 0, hi_out = 0, lo_out = 0;       // a lane has fewer than 4096 tokens
+    each([&](int c, const float* v) {
+#pragma unroll
+      for (int k = 0; k < N16; ++k) {
+        if (!(v[k] > -INFINITY) || !in(first + c + k, v[k])) continue;
+        const float s = place(v[k]);
+        const Mass20 m = mass20_of(weight(v[k]));
+        if (s < (float)ROW_LIST) { hi_in += m.hi; lo_in += m.lo; add_to_bin((int)s, m); }
+        else { hi_out += m.hi; lo_out += m.lo; }
       }
-      cut_after(keep);
-    } else {
-      search([&](float v) { return mass_of(wt.weight(v)); }, enough);
-    }
+    });
+    u64 before, binned, rest;
+    share_sums(warp_total(((u64)hi_in << 20) + lo_in), before, binned);
+    share_sums(warp_total(((u64)hi_out << 20) + lo_out), before, rest);
+    const double part = dp * (double)(binned + rest);
+    cut_by_bins(binned, place, [&](float v) -> u64 { return mass_of(weight(v)); }, [&](u64 m) { return m > 0 && !((double)m < part); });
   }
   // ---- 4
-  const float least = p.min_p ? fminf(p.min_p[row], 1.f) : 0.f;
+  const bool all_in = from == -INFINITY && !(least > 0.f);
+  const float start = fmaxf(from, least > 0.f ? peak + (logf(least) * 1.0001f - 1e-5f) * t - 1e-6f * (1.f + fabsf(peak)) : -INFINITY);    // below: weights below `least`
+  uint32_t hi20 = 0, lo20 = 0;
+  if (all_in) {
+    each([&](int, const float* v) {
+#pragma unroll
+      for (int k = 0; k < N16; ++k) {
+        const Mass20 m = mass20_of(fmaxf(weight(v[k]), 0.f));    // NaN: nothing
+        hi20 += m.hi;
+        lo20 += m.lo;
+      }
+    });
+  } else {
+    each_from(start, [&](int i, float v) {
+      const float w = weight(v);
+      if (!in(i, v) || !(w >= least)) return;
+      const Mass20 m = mass20_of(w);
+      hi20 += m.hi;
+      lo20 += m.lo;
+    });
+  }
+  const u64 mine = warp_total(((u64)hi20 << 20) + lo20);
+  u64 before, S;
+  share_sums(mine, before, S);
+  const u64 r = target(S);
+  if (r < before || r >= before + mine) return;                  // not in this warp's stretch
   const auto kept = [&](int i, float v) -> u64 {
-    const uint32_t k = key_of(v);
-    if (!(k > KEY_NONE && in(k, i))) return 0;
-    const float w = expf(wt.scaled(v));
+    if (!(v > -INFINITY) || !in(i, v)) return 0;
+    const float w = weight(v);
     return w >= least ? mass_of(w) : 0;
   };
-  uint32_t hi20 = 0, lo20 = 0;                                   // a lane has fewer than 4096 tokens
-  each([&](int i, float v) {
-    const uint32_t k = key_of(v);
-    if (!(k > KEY_NONE && in(k, i))) return;
-    const float w = expf(wt.scaled(v));
-    if (!(w >= least)) return;
-    const Mass20 m = mass20_of(w);
-    hi20 += m.hi;
-    lo20 += m.lo;
-  });
-  u64 mine = ((u64)hi20 << 20) + lo20;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  __syncthreads();
-  if (lane == 0) sh.red[warp] = mine;
-  __syncthreads();
-  u64 before = 0, all = 0;
-  for (int w = 0; w < WARPS; ++w) { if (w < warp) before += sh.red[w]; all += sh.red[w]; }
-  u64 S = all;
-  if (ctas > 1) {
-    turn ^= 1;
-    if (tid < (int)ctas) cluster_st(map_to_cta(smem_u32(&sh.exchange[turn][rank]), tid), all);
-    cluster_sync_all();
-    S = 0;
-    for (uint32_t r = 0; r < ctas; ++r) { if (r < rank) before += sh.exchange[turn][r]; S += sh.exchange[turn][r]; }
-  }
-  const double at = floor((double)p.u[row] * (double)S);
-  const u64 r = !(at > 0.0) ? 0 : at >= (double)S ? S - 1 : min((u64)at, S - 1);
-  if (r < before || r >= before + mine) return;                  // not in this warp's stretch
   // a lane takes neighbours, then the lane's stretch is looked at token by token
   const int piece = (span + 31) / 32, p0 = min(s0 + lane * piece, s1), p1 = min(p0 + piece, s1);
   u64 part = 0;
   for (int i = p0; i < p1; ++i) part += kept(first + i, load_logit(places + i));
-  u64 inc = part;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) { const u64 v = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += v; }
-  const int who = __ffs(__ballot_sync(0xffffffffu, before + inc > r)) - 1;
-  u64 run = before + __shfl_sync(0xffffffffu, inc - part, who);
+  const u64 upto = warp_scan(part, lane);
+  const int who = __ffs(__ballot_sync(0xffffffffu, before + upto > r)) - 1;
+  u64 run = before + __shfl_sync(0xffffffffu, upto - part, who);
   const int q0 = __shfl_sync(0xffffffffu, p0, who), q1 = __shfl_sync(0xffffffffu, p1, who);
   for (int c = q0; c < q1; c += 32) {
     const int i = c + lane;
     const float v = i < q1 ? load_logit(places + i) : -INFINITY;
-    inc = i < q1 ? kept(first + i, v) : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const u64 u = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += u; }
+    const u64 inc = warp_scan(kept(first + i, v), lane);
     const unsigned past = __ballot_sync(0xffffffffu, run + inc > r);
     if (past) {
-      if (lane == __ffs(past) - 1) {
-        p.tokens[row] = first + i;
-        p.logprobs[row] = wt.scaled(v) - (float)log((double)S / 1099511627776.0);
-      }
+      if (lane == __ffs(past) - 1) answer(first + i, v, S);
       return;
     }
     run += __shfl_sync(0xffffffffu, inc, 31);
@@ -601,7 +662,7 @@ static int launch_sample(const SampleParams& p, int* status, cudaStream_t st) {
   while (ctas < 8 && ((size_t)(p.vocab / ctas) * sizeof(T) > 104 * 1024 || (p.rows * (long long)ctas < 148 && p.vocab / ctas >= 2 * 4096))) ctas *= 2;
   const int share = (p.vocab + ctas - 1) / ctas + Lane16<T>::N;  // places: tokens, and what the first lacks to 16 bytes
   const int span = (share + WARPS * UNIT - 1) / (WARPS * UNIT) * UNIT;
-  const size_t smem = ROW_BINS * sizeof(u64) + (size_t)span * WARPS * sizeof(T);
+  const size_t smem = 2 * ROW_LIST * sizeof(u64) + (size_t)span * WARPS * sizeof(T);
   if (smem > MOST) {                                             // beyond what eight CTAs hold
     launch_short(sample_kernel<T>, dim3((unsigned)p.rows), dim3(SAMPLE_THREADS), 0, st, p);
     return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;

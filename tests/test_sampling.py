@@ -150,10 +150,14 @@ def test_large_vocabularies(dtype, vocab):
     x[2::4] *= 0.01                                               # rows that are nearly flat
     x[3::4, 1000:] = -math.inf
     u = torch.rand(n, generator=g, device="cuda")
-    f = lambda i, dtype=torch.float32: torch.tensor([r[i] for r in RULES], dtype=dtype, device="cuda")  # noqa: E731
+    _check_on_device(x, u, RULES)
+
+
+def _check_on_device(x, u, rules):
+    f = lambda i, dtype=torch.float32: torch.tensor([r[i] for r in rules], dtype=dtype, device="cuda")  # noqa: E731
     t, k, p, least = f(0), f(1, torch.int32), f(2), f(3)
     tokens, logprobs = S.sample(x, u, t, k, p, least)
-    for r, (tr, kr, pr, lr) in enumerate(RULES):                  # the rule again, with int64 sums along a sorted row
+    for r, (tr, kr, pr, lr) in enumerate(rules):                  # the rule again, with int64 sums along a sorted row
         xs, order = torch.sort(x[r].float(), descending=True, stable=True)
         if tr <= 0:
             assert int(tokens[r]) == int(order[0]) and float(logprobs[r]) == 0
@@ -174,6 +178,30 @@ def test_large_vocabularies(dtype, vocab):
         assert int(tokens[r]) == want, f"row {r}"
         lp = float(y[int((order == want).nonzero()[0, 0])]) - math.log(total / 2 ** 40)
         assert abs(float(logprobs[r]) - lp) <= 2 ** -22 * (1 + abs(lp) + 20), f"row {r}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [600, 9000, 77777, 201088])
+@pytest.mark.parametrize("spread", [1e-6, 0.05, 1.0, 40.0])
+def test_cuts_deep_in_a_row(dtype, vocab, spread):
+    """Cuts that leave thousands of tokens, from rows in which many are nearly or quite equal to rows that spread far."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    rules = [(1.0, 300, 1.0, 0.0), (3.0, 0, 0.9, 0.0), (1.0, 5000, 1.0, 0.0), (1.0, 5000, 0.7, 0.001), (100.0, 0, 0.5, 0.0), (1e4, 0, 0.97, 0.0), (0.5, 0, 0.999999, 0.0),
+             (1.0, 70000, 0.9, 0.0), (1.0, 0, 0.999, 0.9999), (2.0, 257, 0.01, 0.0), (1.0, 0, 1.0, 1e-6), (1.0, vocab - 1, 1.0, 0.0)]
+    x = (torch.randn(len(rules), vocab, generator=g, device="cuda") * spread).to(dtype)
+    u = torch.rand(len(rules), generator=g, device="cuda")
+    _check_on_device(x, u, rules)
+    _check_on_device((x * 4).round() / 4 + 100, u, rules)         # equal ones, away from zero
+    x[:, vocab // 3:] = torch.finfo(dtype).min
+    _check_on_device(x, u, rules)
+
+
+@pytest.mark.gpu
+def test_more_tokens_than_a_cluster_holds():
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(len(RULES), 500009, generator=g, device="cuda") * 2.5
+    _check_on_device(x, torch.rand(len(RULES), generator=g, device="cuda"), RULES)
 
 
 @pytest.mark.parametrize("device", DEVICES)

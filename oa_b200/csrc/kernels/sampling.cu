@@ -392,6 +392,18 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
   };
   // The first n entries of bins into falling order.
   const auto sort_list = [&](int n) {
+    __syncthreads();
+    if (n <= ROW_LIST / 4) {                                     // by counting, four threads to an entry (64 entries: 0.4 us, by exchanges 2.0)
+      const u64 e = (tid >> 2) < n ? bins[tid >> 2] : 0;
+      int above = 0;
+      for (int i = tid & 3; i < n; i += 4) above += bins[i] > e;
+      above += __shfl_xor_sync(0xffffffffu, above, 1);
+      above += __shfl_xor_sync(0xffffffffu, above, 2);
+      __syncthreads();
+      if ((tid & 3) == 0 && (tid >> 2) < n) bins[above] = e;
+      __syncthreads();
+      return;
+    }
     int size = 64;
     while (size < n) size <<= 1;
     if (tid >= n && tid < size) bins[tid] = 0;
@@ -426,7 +438,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     meet();                                                      // all bins are filled
     const uint32_t at = smem_u32(bins + tid);
     u64 v = 0;
-    for (uint32_t c = 0; c < ctas; ++c) { const u64 pair = cluster_ld(map_to_cta(at, c)); v += ((pair >> 32) << 20) + (uint32_t)pair; }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {                                // all under way together
+      const u64 pair = c < (int)ctas ? cluster_ld(map_to_cta(at, c)) : 0;
+      v += ((pair >> 32) << 20) + (uint32_t)pair;
+    }
     const u64 run = base + block_scan(v, all);
     if (enough(run + v) && !enough(run)) { sh.bin = tid; sh.base = run; }
     __syncthreads();
@@ -465,9 +481,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     from = at;
     idx = up;
   };
-  // Cuts what is kept to the shortest head of the ranking whose sum of f is enough.  place(v) falls with v from 0 on in steps of bins; tokens at
-  // ROW_LIST or more of it take no part in the first pass of bins, which the caller has made (their sum: `binned`), and are not reached.
-  const auto cut_by_bins = [&](u64 binned, auto place, auto f, auto enough) {
+  // A logit that is surely not above peak - gap, whatever was rounded on the way to the gap
+  const auto below_gap = [&](float gap, bool unbounded) { return unbounded ? LOWEST : fmaxf(peak - gap * 1.00001f - (fabsf(peak) + gap) * 0x1p-20f, LOWEST); };
+  // Cuts what is kept to the shortest head of the ranking whose sum of f is enough.  place(v) rises from 0 as v falls, by 1, a bin, for `step`;
+  // tokens at ROW_LIST or more of it take no part in the first pass of bins, which the caller has made (their sum: `binned`), and are not reached.
+  const auto cut_by_bins = [&](u64 binned, auto place, float step, auto f, auto enough) {
     u64 base = 0, all;
     float origin = 0.f, zoom = 1.f;                              // bins of this pass: (place - origin) * zoom
     for (int pass = 0; pass < 3; ++pass) {
@@ -478,7 +496,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
       base = before;
       const float o = origin, z = zoom;
       const auto mine = [&](float v) { const float s = (place(v) - o) * z; return s >= 0.f && s < (float)ROW_LIST && (int)s == bin; };
-      const int n = collect(LOWEST, mine);
+      const float below = below_gap((o + (float)(bin + 1) / z) * step, o == 0.f && bin == ROW_LIST - 1);
+      const int n = collect(below, mine);
       if (n > 0 && n <= ROW_LIST) {
         if (rank == 0) {
           sort_list(n);
@@ -499,7 +518,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
       bins[tid] = 0;
       __syncthreads();
       u64 sum = 0, prior;
-      each_from(LOWEST, [&](int i, float v) {
+      each_from(below, [&](int i, float v) {
         if (!in(i, v) || !mine(v)) return;
         const u64 m = f(v);
         sum += m;
@@ -533,10 +552,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     if (high > -INFINITY) atomicAdd(reinterpret_cast<uint32_t*>(bins + (int)place_of_gap(high)), 1u);
     int bin;
     u64 before, all;
-    if (find_bin(0, [&](u64 n) { return n >= (u64)want; }, bin, before, all) && bin < ROW_LIST - 1) {
-      const float gap = (float)(bin + 1) * (1.f / 16.f);
-      floor = fmaxf(peak - gap - (fabsf(peak) + gap) * 0x1p-20f, floor);                    // below the bin, whatever was rounded
-    }
+    if (find_bin(0, [&](u64 n) { return n >= (u64)want; }, bin, before, all)) floor = below_gap((float)(bin + 1) * (1.f / 16.f), bin == ROW_LIST - 1);
   }
   if (brief) {
     const int n = collect(floor, [](float) { return true; });
@@ -571,7 +587,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
       atomicAdd(reinterpret_cast<uint32_t*>(bins + (int)place_of_gap(v)), 1u);
     });
     share_sums(warp_total(have), before, all);
-    if (all > (u64)want) cut_by_bins(all, place_of_gap, [](float) { return 1ull; }, [&](u64 n) { return n >= (u64)want; });
+    if (all > (u64)want) cut_by_bins(all, place_of_gap, 1.f / 16.f, [](float) { return 1ull; }, [&](u64 n) { return n >= (u64)want; });
   }
   // ---- 3
   if (cut_p) {
@@ -594,7 +610,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     share_sums(warp_total(((u64)hi_in << 20) + lo_in), before, binned);
     share_sums(warp_total(((u64)hi_out << 20) + lo_out), before, rest);
     const double part = dp * (double)(binned + rest);
-    cut_by_bins(binned, place, [&](float v) -> u64 { return mass_of(weight(v)); }, [&](u64 m) { return m > 0 && !((double)m < part); });
+    cut_by_bins(binned, place, t / scale, [&](float v) -> u64 { return mass_of(weight(v)); }, [&](u64 m) { return m > 0 && !((double)m < part); });
   }
   // ---- 4
   const bool all_in = from == -INFINITY && !(least > 0.f);
@@ -657,7 +673,7 @@ template <typename T>
 static int launch_sample(const SampleParams& p, int* status, cudaStream_t st) {
   // As many CTAs to a row as keep its share within 104 KB (two CTAs on an SM); more, up to eight, while rows leave SMs idle and a share
   // has 4096 tokens or more.
-  constexpr int UNIT = 32 * Lane16<T>::N, WARPS = SAMPLE_THREADS / 32, MOST = 216 * 1024;
+  constexpr int UNIT = Lane16<T>::N, WARPS = SAMPLE_THREADS / 32, MOST = 216 * 1024;
   int ctas = 1;
   while (ctas < 8 && ((size_t)(p.vocab / ctas) * sizeof(T) > 104 * 1024 || (p.rows * (long long)ctas < 148 && p.vocab / ctas >= 2 * 4096))) ctas *= 2;
   const int share = (p.vocab + ctas - 1) / ctas + Lane16<T>::N;  // places: tokens, and what the first lacks to 16 bytes

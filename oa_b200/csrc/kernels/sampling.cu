@@ -179,16 +179,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SamplePara
 // neighbouring tokens, fetched by a bulk copy of its own, a lane 16 bytes of them at a time; warps in the order of their CTAs own the
 // vocabulary in order, so that a number from each warp (a maximum, a mass), sent to every CTA, says who has the first of something.
 //   1  maximum of each thread, of all warps.  A greedy row ends here.
-//   2  top-k up to 256: the k-th largest of the threads' maxima is no larger than the k-th largest logit, so that what is not below its bin of
-//      (max - x) contains the top k, and little more.  Those tokens go to the first CTA, which sorts them, makes all cuts and samples; the
-//      other CTAs are done.
-//   3  top-p (and larger top-k): masses (counts) in 512 bins of t, which falls with x; the bin in which the wanted sum is reached is cut into 512
-//      again while it holds more than a list does; its tokens go to the first CTA, which sorts them and says where the cut is.
+//   2  top-k up to 256: the k-th largest of the maxima of 512 groups of threads is no larger than the k-th largest logit, so that what is not
+//      below it (cut to 16 bits) contains the top k, and little more: of n tokens spread over the groups about 512 ln(512 / (512 - k)).  Those
+//      tokens go to the first CTA, which sorts them, makes all cuts and samples; the other CTAs are done.
+//   3  top-p (and larger top-k): masses (counts) in 1024 bins of a place that rises as x falls; the bin in which the wanted sum is reached is cut into
+//      1024 again while it holds more than a list does; its tokens go to the first CTA, which sorts them and says where the cut is.
 //      A token of weight below (1 - p) / (2 V) is never kept: all such ones together have less than the mass that is cut off, as the
 //      maximum's weight is 1.  Those take no part.  Equal logits that no bins separate are left to a search over keys and indices, 50 passes.
 //   4  mass of what is kept for each warp, and the warp in whose stretch u falls looks again.
-constexpr int ROW_LIST = 512, ROW_BRIEF_K = 256, ROW_WARPS = SAMPLE_THREADS / 32;
-static_assert(ROW_LIST == SAMPLE_THREADS, "an entry of the list, and a bin, to a thread");
+constexpr int ROW_LIST = 512, ROW_BINS = 1024, ROW_BRIEF_K = 256, ROW_WARPS = SAMPLE_THREADS / 32;
+static_assert(ROW_LIST == SAMPLE_THREADS && ROW_BINS == 2 * SAMPLE_THREADS, "an entry of the list to a thread, and two bins");
 
 template <typename T> struct Lane16;
 template <> struct Lane16<float> {
@@ -216,10 +216,8 @@ template <int N> __device__ __forceinline__ float highest(const float* v) {
 
 __device__ __forceinline__ void cluster_st(uint32_t addr, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory"); }
 __device__ __forceinline__ void cluster_st32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
-__device__ __forceinline__ u64 cluster_ld(uint32_t addr) {
-  u64 v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void cluster_ld2(uint32_t addr, u64& a, u64& b) {
+  asm volatile("ld.shared::cluster.v2.u64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {      // inclusive
 #pragma unroll
@@ -243,21 +241,21 @@ struct RowShared {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const SampleParams p, int span, int* status) {
+__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const SampleParams p, int span, int lg, int* status) {
   constexpr int N16 = Lane16<T>::N;
   extern __shared__ __align__(16) uint8_t row_smem[];
   __shared__ RowShared sh;
-  u64* bins = reinterpret_cast<u64*>(row_smem);                  // [512]; later, in the first CTA, the list of all
-  u64* own_list = bins + ROW_LIST;                               // tokens of this CTA
-  uint8_t* data = row_smem + 2 * ROW_LIST * sizeof(u64);
+  u64* bins = reinterpret_cast<u64*>(row_smem);                  // [ROW_BINS]; later, in the first CTA, the list of all
+  u64* own_list = bins + ROW_BINS;                               // tokens of this CTA
+  uint32_t* group_tops = reinterpret_cast<uint32_t*>(own_list);  // before that, maxima of groups of threads, in the vocabulary's order by warps
+  uint8_t* data = row_smem + (ROW_BINS + ROW_LIST) * sizeof(u64);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  uint32_t ctas;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
-  const uint32_t rank = cluster_ctarank();
-  const int row = blockIdx.x / ctas, V = p.vocab;
+  const uint32_t ctas = 1u << lg, rank = cluster_ctarank();
+  const int row = blockIdx.x >> lg, V = p.vocab;
   pdl_launch_dependents();
-  if (lane == 0) { mbar_init(&sh.bars[warp], 1); mbar_fence_init(); }
-  bins[tid] = 0;
+  if (lane == 0) { mbar_init(&sh.bars[warp], 1); fence_proxy_async_smem(); }
+  const auto clear_bins = [&] { reinterpret_cast<ulonglong2*>(bins)[tid] = make_ulonglong2(0, 0); };
+  clear_bins();
   for (int i = tid; i < 2 * 8 * ROW_WARPS; i += SAMPLE_THREADS) sh.slots[0][i] = 0;
   if (tid == 0) sh.listed = 0;
   __syncwarp();
@@ -265,7 +263,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
 
   // ---- the row's share of this CTA, [lo, hi), lies in shared memory as it does to 16 bytes in the row
   const T* x = static_cast<const T*>(p.logits) + row * p.stride;
-  const int share = (V + (int)ctas - 1) / (int)ctas, lo = min((int)rank * share, V), hi = min(lo + share, V);
+  const int share = (V + (int)ctas - 1) >> lg, lo = min((int)rank * share, V), hi = min(lo + share, V);
   const int skew = (int)((reinterpret_cast<uintptr_t>(x + lo) & 15) / sizeof(T));
   const int first = lo - skew;                                   // token at place 0
   const int s0 = warp * span, s1 = s0 + span;                    // this warp's places
@@ -281,7 +279,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     const auto by_hand = [&](int i) { if (i >= a && i < b) places[i] = x[first + i]; else places[i] = T(-INFINITY); };
     for (int i = s0 + lane; i < a16; i += 32) by_hand(i);        // ends off 16 bytes, and places without a token
     for (int i = b16 + lane; i < s1; i += 32) by_hand(i);
-    if (ctas > 1) cluster_sync_all(); else __syncthreads();      // every CTA of the cluster is there before anything is written to it
+    // every CTA of the cluster is there before anything is written to it
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
     if (b16 > a16 && !warp_wait(&sh.bars[warp], 0) && lane == 0) report_error(status, OA_KERR_WAIT_FULL);
   }
   const auto meet = [&] { if (ctas > 1) cluster_sync_all(); else __syncthreads(); };
@@ -293,52 +292,81 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
       f(c, v);
     }
   };
-  // a pass for which most of 16 bytes is nothing: f(token, logit) where the logit is not below `floor`
+  // a pass for which most of 16 bytes is nothing: f(token, logit) where the logit is not below `floor`.  Four pieces are fetched before the first
+  // is looked at.
   const auto each_from = [&](float floor, auto f) {
-    each([&](int c, const float* v) {
-      if (!(highest<N16>(v) >= floor)) return;
+    for (int c0 = s0 + lane * N16; c0 < s1; c0 += 4 * 32 * N16) {
+      float top4[4];
 #pragma unroll
-      for (int k = 0; k < N16; ++k)
-        if (v[k] >= floor && v[k] > -INFINITY) f(first + c + k, v[k]);
-    });
+      for (int q = 0; q < 4; ++q) {
+        const int c = c0 + q * 32 * N16;
+        float v[N16];
+        Lane16<T>::get(data + min(c, s1 - N16) * sizeof(T), v);
+        top4[q] = c < s1 ? highest<N16>(v) : -INFINITY;
+      }
+      if (!(highest<4>(top4) >= floor)) continue;
+#pragma unroll 1
+      for (int q = 0; q < 4; ++q) {
+        const int c = c0 + q * 32 * N16;
+        if (c >= s1) break;
+        float v[N16];
+        Lane16<T>::get(data + c * sizeof(T), v);
+#pragma unroll
+        for (int k = 0; k < N16; ++k)
+          if (v[k] >= floor && v[k] > -INFINITY) f(first + c + k, v[k]);
+      }
+    }
   };
   int turn = 0;
   // Every warp's number to every CTA; then, to each warp, the sum of the numbers before its own and of all.
-  const auto share_sums = [&](u64 mine, u64& before, u64& all) {
-    turn ^= 1;
-    if (lane < (int)ctas) cluster_st(map_to_cta(smem_u32(&sh.slots[turn][rank * ROW_WARPS + warp]), lane), mine);
-    meet();
+  const auto tell = [&](u64* slots, u64 mine) {
+    if (lane < (int)ctas) cluster_st(map_to_cta(smem_u32(&slots[rank * ROW_WARPS + warp]), lane), mine);
+  };
+  const auto hear = [&](const u64* slots, u64& before, u64& all) {
     u64 v[4], sum = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) { v[k] = lane * 4 + k < (int)ctas * ROW_WARPS ? sh.slots[turn][lane * 4 + k] : 0; sum += v[k]; }
+    for (int k = 0; k < 4; ++k) { v[k] = lane * 4 + k < (int)ctas * ROW_WARPS ? slots[lane * 4 + k] : 0; sum += v[k]; }
     u64 at = warp_scan(sum, lane);
     all = __shfl_sync(0xffffffffu, at, 31);
     at -= sum;
     const int me = rank * ROW_WARPS + warp;
-    u64 upto = at;
 #pragma unroll
-    for (int k = 0; k < 3; ++k) if (k < (me & 3)) upto += v[k];
-    before = __shfl_sync(0xffffffffu, upto, me >> 2);
+    for (int k = 0; k < 3; ++k) if (k < (me & 3)) at += v[k];
+    before = __shfl_sync(0xffffffffu, at, me >> 2);
+  };
+  const auto share_sums = [&](u64 mine, u64& before, u64& all) {
+    turn ^= 1;
+    tell(sh.slots[turn], mine);
+    meet();
+    hear(sh.slots[turn], before, all);
   };
 
   // ---- 1
-  float high = -INFINITY;                                        // of this thread; NaN is passed over
-  each([&](int, const float* v) { high = fmaxf(high, highest<N16>(v)); });
-  uint32_t top_key;
+  uint32_t top_key, tops;                                        // tops: of the maxima of 512 groups of threads, the one of group tid
   int first_warp;                                                // the first that has the maximum
   {
-    const uint32_t mine = __reduce_max_sync(0xffffffffu, key_of(high));
-    turn ^= 1;
-    if (lane < (int)ctas) cluster_st(map_to_cta(smem_u32(&sh.slots[turn][rank * ROW_WARPS + warp]), lane), mine);
+    float high = -INFINITY;                                      // NaN is passed over
+#pragma unroll 4
+    for (int c = s0 + lane * N16; c < s1; c += 32 * N16) {
+      float v[N16];
+      Lane16<T>::get(data + c * sizeof(T), v);
+      high = fmaxf(high, highest<N16>(v));
+    }
+    uint32_t mine = key_of(high);                                // groups of as many lanes as there are CTAs, so that every lane tells one CTA
+    for (int o = 1; o < (int)ctas; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+    cluster_st32(map_to_cta(smem_u32(&group_tops[((rank * ROW_WARPS + warp) << (5 - lg)) + (lane >> lg)]), lane & (ctas - 1)), mine);
     meet();
-    uint32_t k[4], best = 0;
+    tops = group_tops[tid];
+    uint32_t k[16], best = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { k[i] = lane * 4 + i < (int)ctas * ROW_WARPS ? (uint32_t)sh.slots[turn][lane * 4 + i] : 0; best = max(best, k[i]); }
+    for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(k)[i] = reinterpret_cast<const uint4*>(group_tops)[lane * 4 + i];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) best = max(best, k[i]);
     top_key = __reduce_max_sync(0xffffffffu, best);
-    int w = 8 * ROW_WARPS;
+    int at = SAMPLE_THREADS;
 #pragma unroll
-    for (int i = 3; i >= 0; --i) if (k[i] == top_key) w = lane * 4 + i;
-    first_warp = (int)__reduce_min_sync(0xffffffffu, (unsigned)w);
+    for (int i = 15; i >= 0; --i) if (k[i] == top_key) at = lane * 16 + i;
+    first_warp = (int)__reduce_min_sync(0xffffffffu, (unsigned)at) >> (5 - lg);
   }
   const float t = p.temperature ? p.temperature[row] : 1.f;
   float peak = logit_of(top_key);
@@ -361,7 +389,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
   if (peak == INFINITY) {                                        // only those that are infinite count: 0 for them, nothing for the others
     for (int i = s0 + lane; i < s1; i += 32) places[i] = load_logit(places + i) == INFINITY ? T(0.f) : T(-INFINITY);
     __syncwarp();
-    high = high == INFINITY ? 0.f : -INFINITY;
+    tops = logit_of(tops) == INFINITY ? key_of(0.f) : KEY_NONE;
     peak = 0.f;
     top_key = key_of(0.f);
   }
@@ -372,10 +400,22 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
   int idx = V - 1;
   const auto in = [&](int i, float v) { return v > from || (v == from && i <= idx); };
   const auto cut_at = [&](u64 entry) { from = logit_of((uint32_t)(entry >> 32)); idx = (int)~(uint32_t)entry; };
-  // Tokens with logits from `floor` on for which pred holds go to the first CTA's list, in any order; returns how many there are.  With more than
+  // the same for logits between two that lie close together
+  const auto each_between = [&](float below, float above, auto f) {
+    each([&](int c, const float* v) {
+      bool any = false;
+#pragma unroll
+      for (int k = 0; k < N16; ++k) any |= v[k] >= below && v[k] <= above;
+      if (!any) return;
+#pragma unroll
+      for (int k = 0; k < N16; ++k)
+        if (v[k] >= below && v[k] <= above) f(first + c + k, v[k]);
+    });
+  };
+  // Tokens of a pass for which pred holds go to the first CTA's list, in any order; returns how many there are.  With more than
   // ROW_LIST the list is of no use.
-  const auto collect = [&](float floor, auto pred) {
-    each_from(floor, [&](int i, float v) {
+  const auto collect = [&](auto pass, auto pred) {
+    pass([&](int i, float v) {
       if (!in(i, v) || !pred(v)) return;
       const int at = atomicAdd(&sh.listed, 1);
       if (at < ROW_LIST) own_list[at] = ((u64)key_of(v) << 32) | (uint32_t)~i;
@@ -406,7 +446,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     }
     int size = 64;
     while (size < n) size <<= 1;
-    if (tid >= n && tid < size) bins[tid] = 0;
+    if (tid >= n && tid < size) clear_bins();
     __syncthreads();
     for (int lk = 1; 1 << lk <= size; ++lk) {
       for (int lj = lk - 1; lj >= 0; --lj) {
@@ -431,30 +471,37 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     all = __shfl_sync(0xffffffffu, up, ROW_WARPS - 1);
     return __shfl_sync(0xffffffffu, up - r, warp) + inc - v;
   };
-  // The sums of all CTAs' bins, a bin to a thread; then the first bin in which the running sum is enough, and the sum before it.  Returns
+  // The sums of all CTAs' bins, two to a thread; then the first bin in which the running sum is enough, and the sum before it.  Returns
   // false when no bin is.
   const auto find_bin = [&](u64 base, auto enough, int& bin, u64& before, u64& all) {
     if (tid == 0) sh.bin = -1;
     meet();                                                      // all bins are filled
-    const uint32_t at = smem_u32(bins + tid);
-    u64 v = 0;
+    const uint32_t at = smem_u32(bins + 2 * tid);
+    u64 v0 = 0, v1 = 0;
 #pragma unroll
     for (int c = 0; c < 8; ++c) {                                // all under way together
-      const u64 pair = c < (int)ctas ? cluster_ld(map_to_cta(at, c)) : 0;
-      v += ((pair >> 32) << 20) + (uint32_t)pair;
+      u64 a = 0, b = 0;
+      if (c < (int)ctas) cluster_ld2(map_to_cta(at, c), a, b);
+      v0 += ((a >> 32) << 20) + (uint32_t)a;
+      v1 += ((b >> 32) << 20) + (uint32_t)b;
     }
-    const u64 run = base + block_scan(v, all);
-    if (enough(run + v) && !enough(run)) { sh.bin = tid; sh.base = run; }
+    const u64 run = base + block_scan(v0 + v1, all);
+    if (enough(run + v0 + v1) && !enough(run)) {
+      const bool second = !enough(run + v0);
+      sh.bin = 2 * tid + second;
+      sh.base = run + (second ? v0 : 0);
+    }
     __syncthreads();
     bin = sh.bin;
     before = sh.base;
     return bin >= 0;
   };
   // What a bin holds are two sums of 32 bits, in units of 1 and 2^20.  A bin of very many large weights overflows, which shows in the sum of all.
-  const auto add_to_bin = [&](int bin, Mass20 m) {
-    uint32_t* at = reinterpret_cast<uint32_t*>(bins + bin);
-    atomicAdd(at, m.lo);
-    if (m.hi) atomicAdd(at + 1, m.hi);
+  const uint32_t bins_at = smem_u32(bins) - (0x4b000000u << 3);
+  const auto add_to_bin = [&](float s, Mass20 m) {              // s in [0, ROW_BINS): the bin is its whole part
+    const uint32_t at = bins_at + (__float_as_uint(__fadd_rd(s, 8388608.f)) << 3);
+    asm volatile("red.shared.add.u32 [%0], %1;" ::"r"(at), "r"(m.lo) : "memory");
+    if (m.hi) asm volatile("red.shared.add.u32 [%0], %1;" ::"r"(at + 4), "r"(m.hi) : "memory");
   };
   // Slow and sure: the largest key, and of the tokens with it the lowest index, for which enough(f over what is up to there) holds.
   const auto search = [&](auto f, auto enough) {
@@ -483,6 +530,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
   };
   // A logit that is surely not above peak - gap, whatever was rounded on the way to the gap
   const auto below_gap = [&](float gap, bool unbounded) { return unbounded ? LOWEST : fmaxf(peak - gap * 1.00001f - (fabsf(peak) + gap) * 0x1p-20f, LOWEST); };
+  // and one that is surely not below it
+  const auto above_gap = [&](float gap) { return peak - gap * 0.99999f + (fabsf(peak) + gap) * 0x1p-20f; };
   // Cuts what is kept to the shortest head of the ranking whose sum of f is enough.  place(v) rises from 0 as v falls, by 1, a bin, for `step`;
   // tokens at ROW_LIST or more of it take no part in the first pass of bins, which the caller has made (their sum: `binned`), and are not reached.
   const auto cut_by_bins = [&](u64 binned, auto place, float step, auto f, auto enough) {
@@ -495,9 +544,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
       if (!there || all != binned) break;                        // a bin has overflowed, or all was cut off
       base = before;
       const float o = origin, z = zoom;
-      const auto mine = [&](float v) { const float s = (place(v) - o) * z; return s >= 0.f && s < (float)ROW_LIST && (int)s == bin; };
-      const float below = below_gap((o + (float)(bin + 1) / z) * step, o == 0.f && bin == ROW_LIST - 1);
-      const int n = collect(below, mine);
+      const auto mine = [&](float v) { const float s = (place(v) - o) * z; return s >= (float)bin && s < (float)(bin + 1); };
+      const float below = below_gap((o + (float)(bin + 1) / z) * step, o == 0.f && bin == ROW_BINS - 1), above = above_gap((o + (float)bin / z) * step);
+      const int n = collect([&](auto f) { each_between(below, above, f); }, mine);
       if (n > 0 && n <= ROW_LIST) {
         if (rank == 0) {
           sort_list(n);
@@ -514,15 +563,15 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
       if (pass == 2 || n == 0) break;
       // the bin again, in as many: the next bits of place
       origin = o + (float)bin / z;
-      zoom = z * (float)ROW_LIST;
-      bins[tid] = 0;
+      zoom = z * (float)ROW_BINS;
+      clear_bins();
       __syncthreads();
       u64 sum = 0, prior;
-      each_from(below, [&](int i, float v) {
+      each_between(below, above, [&](int i, float v) {
         if (!in(i, v) || !mine(v)) return;
         const u64 m = f(v);
         sum += m;
-        add_to_bin((int)fminf((place(v) - origin) * zoom, (float)(ROW_LIST - 1)), {(uint32_t)(m >> 20), (uint32_t)m & 0xfffffu});
+        add_to_bin((place(v) - origin) * zoom, {(uint32_t)(m >> 20), (uint32_t)m & 0xfffffu});
       });
       share_sums(warp_total(sum), prior, binned);
     }
@@ -544,18 +593,19 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
   const float top_p = p.top_p ? p.top_p[row] : 1.f;
   const double dp = (double)top_p;
   const bool cut_p = !(top_p >= 1.f);
-  const auto place_of_gap = [&](float v) { return fminf(__fmul_rn(peak - v, 16.f), (float)ROW_LIST - 0.5f); };      // 32 of logits, all beyond in the last
+  const auto place_of_gap = [&](float v) { return fminf(__fmul_rn(peak - v, 32.f), (float)ROW_BINS - 0.5f); };      // 32 of logits, all beyond in the last
   bool brief = V <= ROW_LIST && ((want > 0 && want < V) || cut_p);
   float floor = LOWEST;
   if (!brief && want > 0 && want <= ROW_BRIEF_K && want < V) {
     brief = true;
-    if (high > -INFINITY) atomicAdd(reinterpret_cast<uint32_t*>(bins + (int)place_of_gap(high)), 1u);
-    int bin;
-    u64 before, all;
-    if (find_bin(0, [&](u64 n) { return n >= (u64)want; }, bin, before, all)) floor = below_gap((float)(bin + 1) * (1.f / 16.f), bin == ROW_LIST - 1);
+    uint32_t low = 0;                                            // the largest number of 16 bits that `want` of the maxima reach
+    for (int bit = 31; bit >= 16; --bit)
+      if (__syncthreads_count(tops >= (low | 1u << bit)) >= want) low |= 1u << bit;
+    if (low > KEY_NONE) floor = logit_of(low);
   }
   if (brief) {
-    const int n = collect(floor, [](float) { return true; });
+    __syncthreads();                                             // the maxima have been read: the list may go over them
+    const int n = collect([&](auto f) { each_from(floor, f); }, [](float) { return true; });
     if (n <= ROW_LIST) {
       if (rank != 0) return;
       sort_list(n);
@@ -580,35 +630,42 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
   }
   if (want > 0 && want < V) {
     u64 have = 0, before, all;
-    bins[tid] = 0;
+    clear_bins();
     __syncthreads();
     each_from(LOWEST, [&](int, float v) {
       ++have;
-      atomicAdd(reinterpret_cast<uint32_t*>(bins + (int)place_of_gap(v)), 1u);
+      add_to_bin(place_of_gap(v), {0, 1});
     });
     share_sums(warp_total(have), before, all);
-    if (all > (u64)want) cut_by_bins(all, place_of_gap, 1.f / 16.f, [](float) { return 1ull; }, [&](u64 n) { return n >= (u64)want; });
+    if (all > (u64)want) cut_by_bins(all, place_of_gap, 1.f / 32.f, [](float) { return 1ull; }, [&](u64 n) { return n >= (u64)want; });
   }
   // ---- 3
   if (cut_p) {
-    const float never = fminf(fmaxf((float)(0.5 * (1.0 - dp) / V), 5e-13f), 0.5f), scale = (float)ROW_LIST / -logf(never);
+    const float never = fminf(fmaxf((float)(0.5 * (1.0 - dp) / V), 5e-13f), 0.5f), scale = (float)ROW_BINS / -logf(never);
     const auto place = [&](float v) { return __fmul_rn(-scaled(v), scale); };
-    bins[tid] = 0;
+    clear_bins();
     __syncthreads();
     uint32_t hi_in = 0, lo_in = 0, hi_out = 0, lo_out = 0;       // a lane has fewer than 4096 tokens
-    each([&](int c, const float* v) {
+    const auto put = [&](float v) {
+      const float s = place(v);
+      const Mass20 m = mass20_of(fmaxf(weight(v), 0.f));         // NaN: nothing
+      if (s < (float)ROW_BINS) { hi_in += m.hi; lo_in += m.lo; add_to_bin(s, m); }
+      else { hi_out += m.hi; lo_out += m.lo; }
+    };
+    if (from == -INFINITY) {
+      each([&](int, const float* v) {
 #pragma unroll
-      for (int k = 0; k < N16; ++k) {
-        if (!(v[k] > -INFINITY) || !in(first + c + k, v[k])) continue;
-        const float s = place(v[k]);
-        const Mass20 m = mass20_of(weight(v[k]));
-        if (s < (float)ROW_LIST) { hi_in += m.hi; lo_in += m.lo; add_to_bin((int)s, m); }
-        else { hi_out += m.hi; lo_out += m.lo; }
-      }
-    });
+        for (int k = 0; k < N16; ++k) put(v[k]);
+      });
+    } else {
+      each_from(from, [&](int i, float v) { if (in(i, v)) put(v); });
+    }
     u64 before, binned, rest;
-    share_sums(warp_total(((u64)hi_in << 20) + lo_in), before, binned);
-    share_sums(warp_total(((u64)hi_out << 20) + lo_out), before, rest);
+    tell(sh.slots[0], warp_total(((u64)hi_in << 20) + lo_in));   // both sets: since either was read last, all have met
+    tell(sh.slots[1], warp_total(((u64)hi_out << 20) + lo_out));
+    meet();
+    hear(sh.slots[0], before, binned);
+    hear(sh.slots[1], before, rest);
     const double part = dp * (double)(binned + rest);
     cut_by_bins(binned, place, t / scale, [&](float v) -> u64 { return mass_of(weight(v)); }, [&](u64 m) { return m > 0 && !((double)m < part); });
   }
@@ -626,12 +683,15 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
       }
     });
   } else {
-    each_from(start, [&](int i, float v) {
-      const float w = weight(v);
-      if (!in(i, v) || !(w >= least)) return;
-      const Mass20 m = mass20_of(w);
-      hi20 += m.hi;
-      lo20 += m.lo;
+    each([&](int c, const float* v) {
+      if (!(highest<N16>(v) >= start)) return;
+#pragma unroll
+      for (int k = 0; k < N16; ++k) {
+        const float w = weight(v[k]);
+        const Mass20 m = mass20_of(v[k] > -INFINITY && in(first + c + k, v[k]) && w >= least ? w : 0.f);
+        hi20 += m.hi;
+        lo20 += m.lo;
+      }
     });
   }
   const u64 mine = warp_total(((u64)hi20 << 20) + lo20);
@@ -674,11 +734,12 @@ static int launch_sample(const SampleParams& p, int* status, cudaStream_t st) {
   // As many CTAs to a row as keep its share within 104 KB (two CTAs on an SM); more, up to eight, while rows leave SMs idle and a share
   // has 4096 tokens or more.
   constexpr int UNIT = Lane16<T>::N, WARPS = SAMPLE_THREADS / 32, MOST = 216 * 1024;
-  int ctas = 1;
-  while (ctas < 8 && ((size_t)(p.vocab / ctas) * sizeof(T) > 104 * 1024 || (p.rows * (long long)ctas < 148 && p.vocab / ctas >= 2 * 4096))) ctas *= 2;
+  int lg = 0;
+  while (lg < 3 && ((size_t)(p.vocab >> lg) * sizeof(T) > 104 * 1024 || ((long long)p.rows << lg < 148 && p.vocab >> lg >= 2 * 4096))) ++lg;
+  const int ctas = 1 << lg;
   const int share = (p.vocab + ctas - 1) / ctas + Lane16<T>::N;  // places: tokens, and what the first lacks to 16 bytes
   const int span = (share + WARPS * UNIT - 1) / (WARPS * UNIT) * UNIT;
-  const size_t smem = 2 * ROW_LIST * sizeof(u64) + (size_t)span * WARPS * sizeof(T);
+  const size_t smem = (ROW_BINS + ROW_LIST) * sizeof(u64) + (size_t)span * WARPS * sizeof(T);
   if (smem > MOST) {                                             // beyond what eight CTAs hold
     launch_short(sample_kernel<T>, dim3((unsigned)p.rows), dim3(SAMPLE_THREADS), 0, st, p);
     return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
@@ -700,7 +761,7 @@ static int launch_sample(const SampleParams& p, int* status, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_on((long long)p.rows * ctas <= PDL_SHORT_BLOCKS) ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, sample_row_kernel<T>, p, span, status) == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, sample_row_kernel<T>, p, span, lg, status) == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }
 
 extern "C" int oa_sample(int dtype, const void* logits, long long stride, const float* u, const float* temperature, const int* top_k, const float* top_p,

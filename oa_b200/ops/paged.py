@@ -34,34 +34,41 @@ class PagedStep(NamedTuple):
     missing: torch.Tensor       # [1] tokens without a slot (no page left, or the table's row full), plus those beyond `tokens`
 
 
+_I32 = torch.int32
+
+
 def _int32(what: str, *tensors: torch.Tensor) -> None:
     for t in tensors:
-        if t.dtype != torch.int32 or not t.is_contiguous():
+        if t.dtype is not _I32 or not t.is_contiguous():
             raise ValueError(f"{what}: contiguous int32 tensors expected")
 
 
-def _tables(what: str, tables: torch.Tensor, batch: int) -> None:
-    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != batch or (tables.shape[1] > 1 and tables.stride(1) != 1) \
-            or (batch > 1 and tables.stride(0) < tables.shape[1]):
+def _table(what: str, tables: torch.Tensor, batch: int):
+    """(width, elements between rows) of a table of `batch` rows."""
+    if tables.dtype is not _I32 or tables.dim() != 2:
+        raise ValueError(f"{what}: tables must be int32 [{batch}, width]")
+    rows, width = tables.shape
+    step, unit = tables.stride()
+    if rows != batch or (width > 1 and unit != 1) or (batch > 1 and step < width):
         raise ValueError(f"{what}: tables must be int32 [{batch}, width] with rows side by side")
+    return width, step if batch > 1 else width
 
 
-def _same_device(what: str, first: torch.Tensor, *tensors: Optional[torch.Tensor]) -> None:
+def _same_device(what: str, first: torch.Tensor, *tensors: torch.Tensor) -> None:
+    at = first.get_device()
     for t in tensors:
-        if t is not None and t.device != first.device:
+        if t.get_device() != at:
             raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
 
 
-def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    """The rows as the kernels read them: elements side by side, every row on 16 bytes.  A copy where they are not."""
-    if t.stride(1) == 1 and _row_stride(t) * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format) if t.is_contiguous() else K.contiguous(t)
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements between rows; of a single row, whose stride says nothing, its own length."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _aligned_rows(t: torch.Tensor, rows: int, cols: int):
+    """(the rows as the kernels read them, elements between rows): elements side by side, every row on 16 bytes.  A copy where they are not."""
+    step, unit = t.stride()
+    if rows <= 1:
+        step = cols                                  # the stride of a single row says nothing
+    if unit == 1 and step * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
+        return t, step
+    return (t.clone(memory_format=torch.contiguous_format) if t.is_contiguous() else K.contiguous(t)), cols
 
 
 def plan(cached: torch.Tensor, fresh: torch.Tensor, tables: torch.Tensor, free_pages: torch.Tensor, taken: torch.Tensor, page_size: int,
@@ -70,24 +77,23 @@ def plan(cached: torch.Tensor, fresh: torch.Tensor, tables: torch.Tensor, free_p
     one request after the other.  `tokens` is the number of token rows the caller has (rows beyond the step's are marked -1); `position0` the
     length of what all requests share.  Nothing is read back to the host; `taken` is not changed, the step holds the new one.  Lengths
     are not negative and sum up below 2^31."""
-    batch, width = cached.numel(), tables.shape[1] if tables.dim() == 2 else 0
+    batch = cached.numel()
     if page_size not in PAGE_SIZES:
         raise ValueError(f"plan: a page holds one of {PAGE_SIZES} tokens, not {page_size}")
     if fresh.numel() != batch or taken.numel() != 1 or tokens < 0:
         raise ValueError("plan: cached and fresh of one batch, taken of one number, tokens not negative")
     _int32("plan", cached, fresh, free_pages, taken)
-    _tables("plan", tables, batch)
+    width, row_stride = _table("plan", tables, batch)
     _same_device("plan", cached, fresh, tables, free_pages, taken)
     if not cached.is_cuda:
         return _plan_cpu(cached, fresh, tables, free_pages, taken, page_size, tokens, position0)
     out = torch.empty(2 * batch + 3 * tokens + 3, dtype=torch.int32, device=cached.device)
-    starts, lens, slots, positions, rows, now, missing = out.split((batch + 1, batch, tokens, tokens, tokens, 1, 1))
     a = out.data_ptr()
     b = a + 4 * (2 * batch + 1)
-    K._launch(N.require().oa_paged_plan(cached.data_ptr(), fresh.data_ptr(), tables.data_ptr(), _row_stride(tables), free_pages.data_ptr(), taken.data_ptr(),
+    K._launch(N.require().oa_paged_plan(cached.data_ptr(), fresh.data_ptr(), tables.data_ptr(), row_stride, free_pages.data_ptr(), taken.data_ptr(),
                                         a, a + 4 * (batch + 1), b, b + 4 * tokens, b + 8 * tokens, b + 12 * tokens, b + 12 * tokens + 4, batch, width,
                                         free_pages.numel(), page_size, tokens, position0, N.stream()), "oa_paged_plan")
-    return PagedStep(starts, lens, slots, positions, rows, now, missing)
+    return PagedStep._make(torch.unsafe_split_with_sizes(out, (batch + 1, batch, tokens, tokens, tokens, 1, 1)))
 
 
 def _plan_cpu(cached, fresh, tables, free_pages, taken, ps, tokens, position0) -> PagedStep:
@@ -123,13 +129,13 @@ def release(done: torch.Tensor, lens: torch.Tensor, tables: torch.Tensor, free_p
     if done.dtype != torch.bool or done.numel() != batch or not done.is_contiguous() or taken.numel() != 1:
         raise ValueError("release: done must be a contiguous bool tensor with one entry for each request, taken one number")
     _int32("release", lens, free_pages, taken)
-    _tables("release", tables, batch)
+    width, row_stride = _table("release", tables, batch)
     _same_device("release", lens, done, tables, free_pages, taken)
     if not lens.is_cuda:
         top = min(max(int(taken), 0), free_pages.numel())
         for b in range(batch):
             if done[b]:
-                n = min(-(-max(int(lens[b]), 0) // page_size), tables.shape[1])
+                n = min(-(-max(int(lens[b]), 0) // page_size), width)
                 pages = [int(i) for i in tables[b, :n] if i >= 0]
                 back = top - len(pages)
                 for k, i in enumerate(pages):
@@ -140,22 +146,24 @@ def release(done: torch.Tensor, lens: torch.Tensor, tables: torch.Tensor, free_p
                 lens[b] = 0
         return torch.tensor([top], dtype=torch.int32)
     now = torch.empty(1, dtype=torch.int32, device=lens.device)
-    K._launch(N.require().oa_paged_release(done.data_ptr(), lens.data_ptr(), tables.data_ptr(), _row_stride(tables), free_pages.data_ptr(),
-                                           free_pages.numel(), taken.data_ptr(), now.data_ptr(), batch, tables.shape[1], page_size, N.stream()),
+    K._launch(N.require().oa_paged_release(done.data_ptr(), lens.data_ptr(), tables.data_ptr(), row_stride, free_pages.data_ptr(),
+                                           free_pages.numel(), taken.data_ptr(), now.data_ptr(), batch, width, page_size, N.stream()),
               "oa_paged_release")
     return now
 
 
 def _pool(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != dtype or v_pages.dtype != dtype:
+    """(pages, kv heads, page size, head dim, elements between pages of k, and of v)."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype is not dtype or v_pages.dtype is not dtype:
         raise ValueError(f"{what}: k_pages and v_pages must be [pages, kv_heads, page_size, head_dim] of {dtype}")
     pages, heads, ps, hd = k_pages.shape
     if ps not in PAGE_SIZES:
         raise ValueError(f"{what}: a page holds one of {PAGE_SIZES} tokens, not {ps}")
-    for t in (k_pages, v_pages):
-        if t.stride()[1:] != (ps * hd, hd, 1) or (pages > 1 and t.stride(0) < heads * ps * hd):
-            raise ValueError(f"{what}: a page must be contiguous and pages must not overlap")
-    return pages, heads, ps, hd
+    k0, *k_in = k_pages.stride()
+    v0, *v_in = v_pages.stride()
+    if k_in != [ps * hd, hd, 1] or v_in != k_in or (pages > 1 and min(k0, v0) < heads * ps * hd):
+        raise ValueError(f"{what}: a page must be contiguous and pages must not overlap")
+    return pages, heads, ps, hd, k0, v0
 
 
 @functools.lru_cache(maxsize=16)
@@ -167,9 +175,8 @@ def append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, k_pa
     """New tokens' packed rows [tokens, (q_heads + 2 kv_heads) * head_dim] (row stride allowed): returns q [tokens, q_heads * head_dim], rotated by
     each token's own position (pairs j, j + head_dim / 2; theta <= 0: not rotated), and writes rotated k and v to their slots.  A slot that is
     not in the pool (-1) is left out."""
-    pages, kvh, ps, hd = _pool("append", k_pages, v_pages, qkv.dtype)
-    tokens = qkv.shape[0] if qkv.dim() == 2 else -1
-    width = qkv.shape[1] if tokens >= 0 else 0
+    pages, kvh, ps, hd, k_step, v_step = _pool("append", k_pages, v_pages, qkv.dtype)
+    tokens, width = qkv.shape if qkv.dim() == 2 else (-1, 0)
     qh = width // hd - 2 * kvh
     if tokens < 0 or width % hd or qh < 1:
         raise ValueError(f"append: rows of q, k and v heads of {hd} expected, with {kvh} k and v heads")
@@ -190,11 +197,11 @@ def append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, k_pa
         k_pages[at // ps, :, at % ps] = x[there, qh:qh + kvh]
         v_pages[at // ps, :, at % ps] = x[there, qh + kvh:]
         return x[:, :qh].reshape(tokens, qh * hd)
-    qkv = _aligned_rows(qkv)
-    q = torch.empty((tokens, qh * hd), dtype=qkv.dtype, device=qkv.device)
+    qkv, row_stride = _aligned_rows(qkv, tokens, width)
+    q = qkv.new_empty_strided((tokens, qh * hd), (qh * hd, 1))
     turns = ctypes.addressof(_turns(float(theta), hd // 2)) if theta > 0 else None
-    K._launch(N.require().oa_paged_append(K.dt(qkv), qkv.data_ptr(), _row_stride(qkv), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                                          k_pages.stride(0), v_pages.stride(0), positions.data_ptr(), slots.data_ptr(), turns, tokens, qh, kvh, hd, ps,
+    K._launch(N.require().oa_paged_append(K.dt(qkv), qkv.data_ptr(), row_stride, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                          k_step, v_step, positions.data_ptr(), slots.data_ptr(), turns, tokens, qh, kvh, hd, ps,
                                           pages, N.stream()), "oa_paged_append")
     return q
 
@@ -206,32 +213,42 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tab
     starts[b] .. starts[b + 1], at most `max_fresh`) sees the whole shared prompt, `prefix_len` keys in the pages of `prefix_table`, and the
     first lens[b] - n + i + 1 keys of its own pages.  q_heads is a multiple of kv_heads.  Returns [tokens, q_heads * head_dim] and, with
     return_lse, also the natural log-sum-exp [tokens, q_heads] fp32.  Rows that see nothing, and rows of no request, are 0 (-inf)."""
-    pages, kvh, ps, hd = _pool("attention", k_pages, v_pages, q.dtype)
-    if q.dim() != 2 or q.shape[1] % (hd * kvh) or q.shape[1] == 0:
+    pages, kvh, ps, hd, k_step, v_step = _pool("attention", k_pages, v_pages, q.dtype)
+    tokens, cols = q.shape if q.dim() == 2 else (0, 0)
+    if cols == 0 or cols % (hd * kvh):
         raise ValueError(f"attention: q must be [tokens, q_heads * {hd}] with q_heads a multiple of {kvh}")
-    tokens, qh, batch = q.shape[0], q.shape[1] // hd, lens.numel()
+    qh, batch = cols // hd, lens.numel()
     if starts.numel() != batch + 1 or max_fresh < 0 or prefix_len < 0:
         raise ValueError("attention: starts has one entry more than lens; max_fresh and prefix_len are not negative")
-    if prefix_len > 0 and (prefix_table is None or prefix_table.numel() * ps < prefix_len):
-        raise ValueError(f"attention: prefix_table holds fewer than {prefix_len} tokens")
-    _int32("attention", lens, starts, *([prefix_table] if prefix_len else []))
-    _tables("attention", tables, batch)
-    _same_device("attention", q, k_pages, v_pages, tables, lens, starts, prefix_table)
-    scale = 1.0 / math.sqrt(hd) if scale is None else scale
+    if prefix_len > 0:
+        if prefix_table is None or prefix_table.numel() * ps < prefix_len:
+            raise ValueError(f"attention: prefix_table holds fewer than {prefix_len} tokens")
+        _int32("attention", lens, starts, prefix_table)
+        _same_device("attention", q, k_pages, v_pages, tables, lens, starts, prefix_table)
+    else:
+        _int32("attention", lens, starts)
+        _same_device("attention", q, k_pages, v_pages, tables, lens, starts)
+    width, table_stride = _table("attention", tables, batch)
+    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
     if not q.is_cuda:
         return _attention_cpu(q, k_pages, v_pages, tables, lens, starts, max_fresh, prefix_table, prefix_len, scale, return_lse)
-    q = _aligned_rows(q)
-    out = torch.empty((tokens, qh * hd), dtype=q.dtype, device=q.device)
-    lse = torch.empty((tokens, qh), dtype=torch.float32, device=q.device) if return_lse else None
-    lib, code = N.require(), K.dt(q)
+    q, q_step = _aligned_rows(q, tokens, cols)
+    out = q.new_empty_strided((tokens, cols), (cols, 1))
+    lse = torch.empty_strided((tokens, qh), (qh, 1), dtype=torch.float32, device=q.device) if return_lse else None
+    code = K.dt(q)
     # scratch of the call's own: calls on several streams do not meet in it
-    need = lib.oa_paged_attn_scratch_bytes(code, tokens, batch, max_fresh, qh, kvh, hd, pages, prefix_len, scale)
+    need = _scratch_bytes(code, tokens, batch, max_fresh, qh, kvh, hd, pages, prefix_len, scale)
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    K._launch(lib.oa_paged_attn(code, q.data_ptr(), _row_stride(q), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), v_pages.stride(0),
-                                        tables.data_ptr(), _row_stride(tables), lens.data_ptr(), starts.data_ptr(), N.ptr(prefix_table), prefix_len,
-                                        out.data_ptr(), N.ptr(lse), tokens, batch, max_fresh, qh, kvh, hd, ps, pages, tables.shape[1], scale, N.ptr(scratch),
-                                K.status_word(q.device).data_ptr(), N.stream()), "oa_paged_attn", 2 if need else 1, outputs=(out,))
+    K._launch(N.require().oa_paged_attn(code, q.data_ptr(), q_step, k_pages.data_ptr(), v_pages.data_ptr(), k_step, v_step, tables.data_ptr(), table_stride,
+                                        lens.data_ptr(), starts.data_ptr(), N.ptr(prefix_table), prefix_len, out.data_ptr(), N.ptr(lse), tokens, batch,
+                                        max_fresh, qh, kvh, hd, ps, pages, width, scale, N.ptr(scratch), K.status_word(q.device).data_ptr(), N.stream()),
+              "oa_paged_attn", 2 if need else 1, outputs=(out,))
     return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(*sizes) -> int:
+    return N.require().oa_paged_attn_scratch_bytes(*sizes)
 
 
 def _attention_cpu(q, k_pages, v_pages, tables, lens, starts, max_fresh, prefix_table, prefix_len, scale, return_lse):

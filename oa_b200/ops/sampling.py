@@ -23,20 +23,22 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
     least `min_p` of the likeliest one's probability.  The token is where u falls in what is kept, in the vocabulary's order.  Equal logits
     rank by index; the same inputs always give the same token.  Returns (tokens int32 [rows], log-probabilities fp32 [rows] among what
     was kept); (-1, -inf) for a row without a logit above -inf (NaN counts as -inf)."""
-    if logits.dim() != 2 or u.numel() != logits.shape[0]:
+    if logits.dim() != 2 or u.dim() != 1 or u.numel() != logits.shape[0]:
         raise ValueError("sample: logits [rows, vocab] and one random number for each row")
     rows, vocab = logits.shape
+    at = logits.get_device()
     for name, t, dtype in (("u", u, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
                            ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if t is not None and (t.dtype != dtype or t.numel() != rows or not t.is_contiguous() or t.device != logits.device):
+        if t is not None and (t.dtype is not dtype or t.numel() != rows or not t.is_contiguous() or t.get_device() != at):
             raise ValueError(f"sample: {name} must be a contiguous {dtype} tensor [{rows}] on {logits.device}")
     if not logits.is_cuda:
         return _sample_cpu(logits, u, temperature, top_k, top_p, min_p)
-    if vocab > 1 and logits.stride(1) != 1:
-        logits = K.contiguous(logits)
+    step, unit = logits.stride()
+    if vocab > 1 and unit != 1:
+        logits, step = K.contiguous(logits), vocab
     tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
-    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    K._launch(N.require().oa_sample(K.dt(logits), logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, u.data_ptr(), N.ptr(temperature), N.ptr(top_k),
+    logprobs = torch.empty_like(u)
+    K._launch(N.require().oa_sample(K.dt(logits), logits.data_ptr(), step if rows > 1 else vocab, u.data_ptr(), N.ptr(temperature), N.ptr(top_k),
                                     N.ptr(top_p), N.ptr(min_p), tokens.data_ptr(), logprobs.data_ptr(), rows, vocab,
                                     K.status_word(logits.device).data_ptr(), N.stream()), "oa_sample")
     return tokens, logprobs

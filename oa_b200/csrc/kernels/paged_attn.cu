@@ -2,6 +2,7 @@
 // request sees all `prefix_len` keys of the prompt and the first len - n + i + 1 keys of the request's own pages:
 //   o = sum_s softmax_s(scale q . k_s) v_s,   lse = log sum_s exp(scale q . k_s);   a row that sees nothing gives o = 0, lse = -inf.
 // A table entry that names no page counts as keys and values of zeros.  Nothing beyond a request's length is read into a result.
+#include <type_traits>
 #include "common.cuh"
 #include "api.h"
 
@@ -132,46 +133,60 @@ __global__ void __launch_bounds__(128) paged_attn_rows_kernel(const PagedAttnPar
 
 
 // ------------------------------------------------------------------------------------------------ bf16 on the tensor cores
-// A tile of queries is 128 rows, the group of query heads that share a key-value head times `tpt` tokens (row = token * group + head), and
-// a tile of keys is 128 keys, one to eight pages.  An item is the work of one query tile on one key-value head:
+// A tile of queries is up to 128 rows, the group of query heads that share a key-value head times `tpt` tokens (row = token * group +
+// head), and a tile of keys is 128 keys, one to eight pages.  An item is the work of one query tile on one key-value head:
 //   shared form   the prompt is read once for the whole batch: its items take tokens of the batch as they come, whatever request they
 //                 belong to, and each request's own keys make items of their own; every row then has two partial results or more;
 //   joint form    where a request's new tokens fill a tile themselves (or there is no prompt) an item sees the prompt's keys and then its own.
-// The key tiles of all items, one after the other, are cut into as many equal stretches as there are CTAs, so that a long prompt for few
-// requests and short histories for many fill the chip alike.  The part of an item in one stretch is a segment.  Segments that are not a
-// whole result leave (o, m, l) in fp32 in scratch, a second launch joins them.  Where everything goes follows from prefix sums over the
-// batch that each CTA makes for itself; CTA 0 leaves them for the second launch.
+// The key tiles of all items, one after the other, are cut into as many equal stretches as there are CTAs for them (in the shared form some
+// CTAs have the prompt's items and the others the requests'), so that a long prompt for few requests and short histories for many fill the chip
+// alike.  The part of an item in one stretch is a segment.  Segments that are not a whole result leave (o, m, l) in fp32 in scratch, and a
+// second launch joins them.  Where everything goes follows from prefix sums over the batch that each CTA makes for itself; CTA 0 leaves them
+// for the second launch.
 //
-// Inside a CTA, segments run through one pipeline of tiles, g = 0, 1, ..:  warp 9 loads Q (two buffers), K and V by TMA, a box for each
-// page;  warp 8 issues S[g & 1] = Q K_g^T two tiles ahead of O[segment & 1] += P_g V_g, P taken from TMEM;  warps 0-7 are the softmax, two
-// threads to a row.  Warps all of whose rows are empty only keep step: a request's single token fills 8 of 128 rows with 8 heads to a group,
-// and its key tiles then cost what they take to arrive.
+// Inside a CTA, segments run through one pipeline of tiles, g = 0, 1, ..:  warps 13 and 14 load Q (two buffers) and K, and V, by TMA, a box
+// for each page;  warp 12 issues S[g & 1] = Q K_g^T two tiles ahead of O[segment & 1] += P_g V_g, P taken from TMEM;  warps 0-7 are the
+// softmax, two threads to a row;  warps 8-11 write a segment's result out while the next one runs.
+//
+// Few rows: a warp reaches only its own quarter of the TMEM lanes, and the two warps of a quarter share a scheduler, so that 32 rows alone
+// would take as long as 128 (0.9 us a tile, where the products need 0.55).  Up to 32 (64) rows therefore lie in the tile four (two) times, and
+// copy c takes a quarter (half) of a tile's keys, its other weights being zeros; the copies' results are joined on the way out.
+//
 // Keys beyond a length are cut off from the scores by a select, and their values are overwritten by zeros before the product: what lies there
 // (the rest of a page, or of the ring) may be anything, NaN included.
 // The product P_g V_g has a barrier for even and one for odd tiles: the scores of tile g + 1 do not wait for it, so that a reader may be two
 // products ahead of one barrier's phase.
-constexpr int PA_M = 128, PA_N = 128, PA_THREADS = 320, PA_MAX_BATCH = 2048;
+constexpr int PA_M = 128, PA_N = 128, PA_THREADS = 480, PA_MAX_BATCH = 1024;
 constexpr float PA_RESCALE = 8.f;          // log2: the running maximum is let be while rows grow by less
 
 template <int HD> struct PaCfg {
   static constexpr int NK = HD == 64 ? 4 : 2, NV = HD == 64 ? 4 : 2;
   static constexpr int Q_BYTES = PA_M * HD * 2, T_BYTES = PA_N * HD * 2;
-  static constexpr int OFF_Q = 0, OFF_K = 2 * Q_BYTES, OFF_V = OFF_K + NK * T_BYTES, OFF_X = OFF_V + NV * T_BYTES;
-  static constexpr int OFF_BAR = OFF_X + 3 * 2 * PA_M * 4, OFF_SCAN = OFF_BAR + 512;
+  static constexpr int OFF_Q = 0, OFF_K = 2 * Q_BYTES, OFF_V = OFF_K + NK * T_BYTES;
+  static constexpr int OFF_X = OFF_V + NV * T_BYTES;             // float[2 parities][2 halves][128]: maxima of a tile's halves
+  static constexpr int OFF_ML = OFF_X + 2 * 2 * PA_M * 4;        // float[2 segments][3][128]: m, and l of either half
+  static constexpr int OFF_STAGE = OFF_ML + 2 * 3 * PA_M * 4;    // float[128][36] (or [32][HD + 8]): results of copies on the way out
+  static constexpr int OFF_BAR = OFF_STAGE + PA_M * 36 * 4, OFF_SCAN = OFF_BAR + 512;
   static constexpr int SMEM_BYTES = OFF_SCAN + 2 * (PA_MAX_BATCH + 1) * 4;
   static constexpr int TM_S = 0, TM_O = 256;
 };
 
 struct PagedTcParams {
   PagedAttnParams a;
-  int group, tpt, ts;                      // query heads to a key-value head, tokens in a tile, tokens in an own item's box
+  int group, group_mul, tpt;               // query heads to a key-value head (and 65536 / group + 1: see token_of), tokens in a tile
+  int ts, tb;                              // tokens in a box of an own item, of a prompt's item
+  int copies, copies_prompt;
   int joint, prefix_tiles, prefix_row_tiles, prefix_work;   // prefix_work: key tiles of all prompt items (shared form)
-  float* part;                             // partial o: [prompt slots][128][HD], then [own slots][ts * group][HD]
+  float* part;                             // partial o: [prompt slots][tb * group][HD], then [own slots][ts * group][HD]
   float2* ml;                              // their (m, l), m in units of log2
-  int* sums;                               // per, tiles before a request [batch + 1], query tiles before a request [batch + 1]
+  int* sums;                               // Stretches, tiles before a request [batch + 1], query tiles before a request [batch + 1]
   long long own_slot0, part_rows;          // rows of the prompt's slots, rows in all
   int* status;
 };
+constexpr int PA_SUMS = 4;                 // ints in front of the prefix sums
+
+// row / group for rows of a tile
+__device__ __forceinline__ int token_of(const PagedTcParams& p, int row) { return row * p.group_mul >> 16; }
 
 struct Request {
   int t0, n, fresh, own, row_tiles;        // first token, new tokens, those of them that count, own keys, query tiles
@@ -202,20 +217,38 @@ struct Segment {
   int t0, tokens, n, own, seen, i0;        // first token and how many; own items: see Request, i0 = index of the first token in the request
 };
 
-// The segments of a stretch [pos, end) of all key tiles, in order.
+// How the tiles are dealt: CTAs [0, prompt_ctas) have stretches of `per_prompt` of the prompt's, the others of `per` of the requests'.  With
+// both there, in proportion to what they cost: tiles and items of a request's own, tiles of the prompt's by the rows in them.
+// Relative: a full tile waits for its exponentials, one of few rows for its products or its bytes, and an item for its first bytes.
+constexpr float PA_COST_FULL = 1.f, PA_COST_FEW = 0.6f, PA_COST_ITEM = 0.3f;
+struct Stretches { int prompt_ctas, per_prompt, per, own_work; };
+__device__ __forceinline__ Stretches stretches_of(const PagedTcParams& p, int own_work, int own_items, int ctas) {
+  Stretches d;
+  d.own_work = own_work;
+  d.prompt_ctas = 0;
+  if (p.prefix_work > 0) {
+    const float prompt = (float)p.prefix_work * (p.copies_prompt == 1 ? PA_COST_FULL : PA_COST_FEW);
+    const float own = (float)own_work * (p.copies == 1 ? PA_COST_FULL : PA_COST_FEW) + (float)own_items * PA_COST_ITEM;
+    d.prompt_ctas = own_work > 0 ? min(max((int)((float)ctas * prompt / (prompt + own) + 0.5f), 1), ctas - 1) : ctas;
+  }
+  d.per_prompt = max((p.prefix_work + max(d.prompt_ctas, 1) - 1) / max(d.prompt_ctas, 1), 1);
+  d.per = max((own_work + max(ctas - d.prompt_ctas, 1) - 1) / max(ctas - d.prompt_ctas, 1), 1);
+  return d;
+}
+
+// The segments of a stretch [pos, end) of the prompt's or the requests' key tiles, in order.
 struct Walk {
   const PagedTcParams& p;
   const int *tiles_before, *items_before;
   int pos, end;
   int b, h, rt, tile;                      // own items: the next one and the tile in it
   Request r;
-  bool placed;
-  __device__ __forceinline__ Walk(const PagedTcParams& p_, const int* tb, const int* ib, int pos_, int end_)
-      : p(p_), tiles_before(tb), items_before(ib), pos(pos_), end(end_), b(0), h(0), rt(0), tile(0), placed(false) {}
+  bool prompt, placed;
+  __device__ __forceinline__ Walk(const PagedTcParams& p_, const int* tb, const int* ib, bool prompt_, int pos_, int end_)
+      : p(p_), tiles_before(tb), items_before(ib), pos(pos_), end(end_), b(0), h(0), rt(0), tile(0), prompt(prompt_), placed(false) {}
   __device__ __forceinline__ void place() {
-    const int u = pos - p.prefix_work;
-    int lo = 0, n = p.a.batch;             // the last request whose tiles begin at or before u
-    const int per_head = u / p.a.kv_heads;
+    int lo = 0, n = p.a.batch;             // the last request whose tiles begin at or before pos
+    const int per_head = pos / p.a.kv_heads;
     while (n > 1) {
       const int half = n >> 1;
       if (tiles_before[lo + half] <= per_head) { lo += half; n -= half; } else n = half;
@@ -223,7 +256,7 @@ struct Walk {
     b = lo;
     r = request_of(p, b);
     const int all = max(tiles_before[b + 1] - tiles_before[b], 1);
-    int off = u - tiles_before[b] * p.a.kv_heads;
+    int off = pos - tiles_before[b] * p.a.kv_heads;
     h = off / all;
     off -= h * all;
     rt = 0;
@@ -233,7 +266,7 @@ struct Walk {
   }
   __device__ __forceinline__ bool next(Segment& s) {
     if (pos >= end) return false;
-    if (pos < p.prefix_work) {
+    if (prompt) {
       s.prompt = 1;
       s.item = pos / p.prefix_tiles;
       s.tile = pos - s.item * p.prefix_tiles;
@@ -245,7 +278,7 @@ struct Walk {
       s.b = s.n = s.own = s.seen = s.i0 = 0;
     } else {
       if (!placed) place();
-      while (tiles_of(p, r, rt) <= tile || rt >= r.row_tiles) {      // on to the next item that has tiles; there is one before `end`
+      while (rt >= r.row_tiles || tiles_of(p, r, rt) <= tile) {      // on to the next item that has tiles; there is one before `end`
         tile = 0;
         if (++rt >= r.row_tiles) {
           rt = 0;
@@ -286,12 +319,20 @@ __device__ __forceinline__ KeyTile key_tile(const PagedTcParams& p, const Segmen
   k.count = max(min(PA_N, (k.prompt ? p.a.prefix_len : s.seen) - k.first), 0);
   return k;
 }
+// The page, for lane i, that holds the tile's keys from i * page_size on; -1 for lanes without one.  `boxes`: how many there are.
+__device__ __forceinline__ int page_for(const PagedTcParams& p, const Segment& s, int j, int lane, int& boxes) {
+  const KeyTile k = key_tile(p, s, j);
+  boxes = (k.count + (1 << p.a.page_log2) - 1) >> p.a.page_log2;
+  if (lane >= boxes) return -1;
+  const int at = (k.first >> p.a.page_log2) + lane;
+  return k.prompt ? p.a.prefix_table[at] : p.a.tables[s.b * p.a.table_stride + at];
+}
 
-// Prefix sums over the batch (a block of `threads`): key tiles for one key-value head, and query tiles, before each request.  Returns the tiles
-// of all.
-__device__ __forceinline__ int scan_batch(const PagedTcParams& p, int* tiles_before, int* items_before, int* warp_sums, int threads) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
-  const int per = (p.a.batch + threads - 1) / threads, b0 = min(tid * per, p.a.batch), b1 = min(b0 + per, p.a.batch);
+// Prefix sums over the batch (a block of PA_THREADS): key tiles for one key-value head, and query tiles, before each request.
+__device__ __forceinline__ void scan_batch(const PagedTcParams& p, int* tiles_before, int* items_before, int* warp_sums, int& all_tiles, int& all_items) {
+  constexpr int WARPS = PA_THREADS / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.a.batch + PA_THREADS - 1) / PA_THREADS, b0 = min(tid * per, p.a.batch), b1 = min(b0 + per, p.a.batch);
   int tiles = 0, items = 0;
   for (int b = b0; b < b1; ++b) {
     const Request r = request_of(p, b);
@@ -309,26 +350,47 @@ __device__ __forceinline__ int scan_batch(const PagedTcParams& p, int* tiles_bef
   if (lane == 31) { warp_sums[2 * warp] = it; warp_sums[2 * warp + 1] = ii; }
   __syncthreads();
   int bt = it - tiles, bi = ii - items, all_t = 0, all_i = 0;
-  for (int w = 0; w < warps; ++w) {
-    if (w < warp) { bt += warp_sums[2 * w]; bi += warp_sums[2 * w + 1]; }
-    all_t += warp_sums[2 * w];
-    all_i += warp_sums[2 * w + 1];
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    const int x = warp_sums[2 * w], y = warp_sums[2 * w + 1];
+    if (w < warp) { bt += x; bi += y; }
+    all_t += x;
+    all_i += y;
   }
   for (int b = b0; b < b1; ++b) { tiles_before[b] += bt; items_before[b] += bi; }
   if (tid == 0) { tiles_before[p.a.batch] = all_t; items_before[p.a.batch] = all_i; }
-  return all_t;
+  all_tiles = all_t;
+  all_items = all_i;
 }
 
 // Where a partial result goes.  Shared form: every segment of every item, numbered by item + CTA (a segment begins where an item or a
 // stretch does).  Joint form: only items that a stretch's end cuts, of which a CTA has its first and its last segment.
-__device__ __forceinline__ long long partial_row(const PagedTcParams& p, const Segment& s, int cta, bool first) {
-  if (s.prompt) return (long long)(s.item + cta) * PA_M;
-  return p.own_slot0 + (p.joint ? 2ll * cta + (first ? 0 : 1) : (long long)s.item + cta) * (p.ts * p.group);
-}
+__device__ __forceinline__ long long own_row(const PagedTcParams& p, long long slot) { return p.own_slot0 + slot * (p.ts * p.group); }
+__device__ __forceinline__ long long prompt_row(const PagedTcParams& p, long long slot) { return slot * (p.tb * p.group); }
 // Starts that do not rise would make more items than there is room for: their rows stay out of the scratch.
 __device__ __forceinline__ bool has_room(const PagedTcParams& p, long long row) { return row >= 0 && row < p.part_rows; }
 
 __device__ __forceinline__ void softmax_pair_sync(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
+__device__ __forceinline__ void out_sync() { asm volatile("bar.sync 5, 128;" ::: "memory"); }
+// Lanes 0-15 of the quarter, 64 columns: lane l of the warp receives columns 8 k + 2 (l % 4) and the next of row l / 4 in r[4 k], r[4 k + 1], of
+// row 8 + l / 4 in r[4 k + 2], r[4 k + 3].
+__device__ __forceinline__ void tmem_ld_16x256b_x8(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 
 template <int HD>
 __global__ void __launch_bounds__(PA_THREADS, 1)
@@ -338,12 +400,15 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   constexpr int NK = Cfg::NK, NV = Cfg::NV, CHUNKS = HD / 64;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int s_warp_sums[2 * PA_THREADS / 32];
+  __shared__ float s_inv[PA_M];
+  __shared__ int s_fail;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
   uint64_t *q_full = bars, *q_empty = bars + 2, *k_full = bars + 4, *k_empty = k_full + NK, *v_full = k_empty + NK, *v_empty = v_full + NV;
-  uint64_t *s_full = v_empty + NV, *p_full = s_full + 2, *o_done = s_full + 4, *o_free = s_full + 6;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 8);
+  uint64_t *s_full = v_empty + NV, *p_full = s_full + 2, *o_done = s_full + 4, *o_free = s_full + 6, *seg_done = s_full + 8, *o_full = s_full + 10;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 12);
   int* tiles_before = reinterpret_cast<int*>(smem + Cfg::OFF_SCAN);
   int* items_before = tiles_before + p.a.batch + 1;
+  float* s_ml = reinterpret_cast<float*>(smem + Cfg::OFF_ML);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -351,88 +416,100 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     return;
   }
   if (threadIdx.x == 0) {
-    tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmQown); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
-    for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 8); mbar_init(&o_done[i], 1); mbar_init(&o_free[i], 8); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 8);
+      mbar_init(&o_done[i], 1); mbar_init(&o_full[i], 1); mbar_init(&o_free[i], 4); mbar_init(&seg_done[i], 8);
+    }
     for (int i = 0; i < NK; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
     for (int i = 0; i < NV; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
     mbar_fence_init();
   }
-  if (warp == 8) { tmem_alloc<512>(tmem_slot); tmem_relinquish(); }
+  if (warp == 12) { tmem_alloc<512>(tmem_slot); tmem_relinquish(); }
+  if (threadIdx.x == 0) s_fail = 0;
+  if (warp == 13 && lane == 0) { tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmQown); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); }
+  __syncwarp();
   pdl_wait();
-  const int own_tiles = scan_batch(p, tiles_before, items_before, s_warp_sums, PA_THREADS);
+  {                                        // tables on their way to L2 while the lengths arrive: 128 bytes to a thread
+    const int lines = (p.a.width + 31) / 32, at = blockIdx.x * PA_THREADS + threadIdx.x;
+    for (int i = at; i < p.a.batch * lines; i += gridDim.x * PA_THREADS)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.a.tables + (long long)(i / lines) * p.a.table_stride + min(i % lines * 32, p.a.width - 1)));
+    if (at * 32 < p.a.prefix_len >> p.a.page_log2) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.a.prefix_table + at * 32));
+  }
+  int own_tiles, own_items;
+  scan_batch(p, tiles_before, items_before, s_warp_sums, own_tiles, own_items);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int work = p.prefix_work + own_tiles * p.a.kv_heads, per = max((work + (int)gridDim.x - 1) / (int)gridDim.x, 1);
+  const Stretches deal = stretches_of(p, own_tiles * p.a.kv_heads, own_items * p.a.kv_heads, gridDim.x);
   if (blockIdx.x == 0) {                   // for the second launch
-    if (threadIdx.x == 0) { p.sums[0] = per; p.sums[1] = work; }
-    for (int b = threadIdx.x; b <= p.a.batch; b += PA_THREADS) { p.sums[2 + b] = tiles_before[b]; p.sums[3 + p.a.batch + b] = items_before[b]; }
+    if (threadIdx.x == 0) { p.sums[0] = deal.prompt_ctas; p.sums[1] = deal.per_prompt; p.sums[2] = deal.per; p.sums[3] = deal.own_work; }
+    for (int b = threadIdx.x; b <= p.a.batch; b += PA_THREADS) { p.sums[PA_SUMS + b] = tiles_before[b]; p.sums[PA_SUMS + 1 + p.a.batch + b] = items_before[b]; }
   }
-  const long long begin = (long long)blockIdx.x * per;
-  const int lo = (int)min(begin, (long long)work), hi = (int)min(begin + per, (long long)work);
-  Walk walk(p, tiles_before, items_before, lo, hi);
+  const bool on_prompt = (int)blockIdx.x < deal.prompt_ctas;
+  const int cta = on_prompt ? blockIdx.x : blockIdx.x - deal.prompt_ctas, per = on_prompt ? deal.per_prompt : deal.per;
+  const int work = on_prompt ? p.prefix_work : deal.own_work;
+  const int lo = (int)min((long long)cta * per, (long long)work), hi = (int)min((long long)(cta + 1) * per, (long long)work);
+  Walk walk(p, tiles_before, items_before, on_prompt, lo, hi);
   Segment s;
+  const int copies = on_prompt ? p.copies_prompt : p.copies, copy_rows = PA_M / copies;
 
-  if (warp == 9) {
-    // ---------------------------------------------------------------- loads.  Lane i fetches the page that holds the tile's keys from i * page_size on.
-    const int ps = 1 << p.a.page_log2;
-    int g = 0, sq = 0;
-    bool ok = true;
-    int id1 = -1, h1 = 0, n1 = -1, id2 = -1, h2 = 0, n2 = -1;    // page, head and pages of the tiles one and two before (their values are still to come)
-    const auto load = [&](uint8_t* to, const CUtensorMap* m, uint64_t* bar, int id, int h, int boxes) {
-      if (elect_one()) mbar_expect_tx(bar, (uint32_t)(boxes * ps * HD * 2));
-      __syncwarp();
-      if (lane < boxes) {
-#pragma unroll
-        for (int x = 0; x < CHUNKS; ++x) tma_load_3d(to + x * (PA_N * 128) + lane * ps * 128, m, bar, x * 64, h << p.a.page_log2, id);
-      }
-      __syncwarp();
-    };
-    const auto load_v = [&](int gv, int id, int h, int boxes) {
-      const int st = gv % NV;
-      if (!warp_wait(&v_empty[st], ((gv / NV) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); return false; }
-      load(smem + Cfg::OFF_V + st * Cfg::T_BYTES, &tmV, &v_full[st], id, h, boxes);
-      return true;
-    };
-    while (ok && walk.next(s)) {
-      const int qb = sq & 1;
-      ok = warp_wait(&q_empty[qb], ((sq >> 1) & 1) ^ 1);
-      if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
-      if (elect_one()) {
-        const int tokens = s.prompt ? p.tpt : p.ts;
-        mbar_expect_tx(&q_full[qb], (uint32_t)(tokens * p.group * HD * 2));
-#pragma unroll
-        for (int x = 0; x < CHUNKS; ++x)
-          tma_load_3d(smem + Cfg::OFF_Q + qb * Cfg::Q_BYTES + x * (PA_M * 128), s.prompt ? &tmQ : &tmQown, &q_full[qb], x * 64, s.h * p.group, s.t0);
-      }
-      __syncwarp();
-      for (int j = 0; j < s.tiles && ok; ++j, ++g) {
-        const KeyTile kt = key_tile(p, s, s.tile + j);
-        const int boxes = (kt.count + ps - 1) >> p.a.page_log2;
-        int id = -1;
-        if (lane < boxes) {
-          const int at = (kt.first >> p.a.page_log2) + lane;
-          id = kt.prompt ? p.a.prefix_table[at] : p.a.tables[s.b * p.a.table_stride + at];
-        }
-        const int st = g % NK;
-        ok = warp_wait(&k_empty[st], ((g / NK) & 1) ^ 1);
+  if (warp == 13 || warp == 14) {
+    // ---------------------------------------------------------------- loads: warp 13 Q and K, warp 14 V
+    const bool is_k = warp == 13;
+    const int ps = 1 << p.a.page_log2, ring = is_k ? NK : NV;
+    uint64_t *full = is_k ? k_full : v_full, *empty = is_k ? k_empty : v_empty;
+    uint8_t* tiles = smem + (is_k ? Cfg::OFF_K : Cfg::OFF_V);
+    const CUtensorMap* map = is_k ? &tmK : &tmV;
+    int st = 0, sq = 0, boxes = 0, id = -1;
+    uint32_t phase = 1;                                           // of the slot to fill: free at first
+    bool ok = true, more = walk.next(s);
+    if (more) id = page_for(p, s, s.tile, lane, boxes);
+    while (ok && more) {
+      if (is_k) {
+        const int qb = sq & 1;
+        ok = warp_wait(&q_empty[qb], ((sq >> 1) & 1) ^ 1);
         if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
-        load(smem + Cfg::OFF_K + st * Cfg::T_BYTES, &tmK, &k_full[st], id, s.h, boxes);
-        if (n2 >= 0) ok = load_v(g - 2, id2, h2, n2);
-        id2 = id1; h2 = h1; n2 = n1;
-        id1 = id; h1 = s.h; n1 = boxes;
+        if (elect_one()) {
+          const int tokens = s.prompt ? p.tb : p.ts;
+          mbar_expect_tx(&q_full[qb], (uint32_t)(copies * tokens * p.group * HD * 2));
+          for (int c = 0; c < copies; ++c)
+#pragma unroll
+            for (int x = 0; x < CHUNKS; ++x)
+              tma_load_3d(smem + Cfg::OFF_Q + qb * Cfg::Q_BYTES + x * (PA_M * 128) + c * copy_rows * 128, s.prompt ? &tmQ : &tmQown, &q_full[qb], x * 64,
+                          s.h * p.group, s.t0);
+        }
+        __syncwarp();
+        ++sq;
       }
-      ++sq;
+      const int n = s.tiles, h = s.h;
+      for (int j = 0; j < n; ++j) {
+        const int now = id, now_boxes = boxes;                    // the next tile's page, of the next segment's first where this is the last
+        if (j + 1 < n) {
+          id = page_for(p, s, s.tile + j + 1, lane, boxes);
+        } else {
+          more = walk.next(s);
+          if (more) id = page_for(p, s, s.tile, lane, boxes);
+        }
+        ok = warp_wait(&empty[st], phase);
+        if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
+        if (elect_one()) mbar_expect_tx(&full[st], (uint32_t)(now_boxes * ps * HD * 2));
+        __syncwarp();
+        if (lane < now_boxes) {
+#pragma unroll
+          for (int x = 0; x < CHUNKS; ++x)
+            tma_load_3d(tiles + st * Cfg::T_BYTES + x * (PA_N * 128) + lane * ps * 128, map, &full[st], x * 64, h << p.a.page_log2, now);
+        }
+        __syncwarp();
+        if (++st == ring) { st = 0; phase ^= 1; }
+      }
     }
-    if (ok && n2 >= 0) ok = load_v(g - 2, id2, h2, n2);
-    if (ok && n1 >= 0) load_v(g - 1, id1, h1, n1);
-  } else if (warp == 8) {
+  } else if (warp == 12) {
     // ---------------------------------------------------------------- products
     constexpr uint32_t idesc_qk = umma_idesc_bf16(PA_M, PA_N, 0, 0), idesc_pv = umma_idesc_bf16(PA_M, HD, 0, 1);
     const uint64_t q_desc = umma_smem_desc_sw128(smem_u32(smem + Cfg::OFF_Q), 16, 1024), k_desc = umma_smem_desc_sw128(smem_u32(smem + Cfg::OFF_K), 16, 1024);
     const uint64_t v_desc = umma_smem_desc_sw128(smem_u32(smem + Cfg::OFF_V), PA_N * 128, 1024);
-    Walk ahead(p, tiles_before, items_before, lo, hi);           // of the score products, two tiles ahead
+    Walk ahead(p, tiles_before, items_before, on_prompt, lo, hi);         // of the score products, two tiles ahead
     Segment sa;
     int ja = 0, na = 0, sqa = -1, ga = 0;
     const auto issue_qk = [&]() -> bool {                         // the next score product, if there is one
@@ -480,6 +557,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         (j > 0 || ks > 0) ? 1u : 0u);
           umma_commit(&v_empty[st]);
           umma_commit(&o_done[g & 1]);
+          if (j + 1 == s.tiles) umma_commit(&o_full[sq & 1]);
         }
         __syncwarp();
         ok = issue_qk();                                          // over S[g & 1] = P_g: behind its product in the pipe
@@ -487,19 +565,20 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       ++sq;
     }
-  } else {
-    // ---------------------------------------------------------------- softmax: warp w has rows 32 (w % 4).., keys 64 (w / 4).. of a tile
+  } else if (warp < 8) {
+    // ---------------------------------------------------------------- softmax: warp w has TMEM lanes 32 (w % 4).. and the keys of half w / 4 of a tile
     constexpr int OC = HD / 2;
     const int quad = warp & 3, half = warp >> 2, r = quad * 32 + lane;
+    const int copy = r / copy_rows, row = r - copy * copy_rows, i_row = token_of(p, row);   // i_row: token of this row in the tile
     const uint32_t t_lane = (uint32_t)(quad * 32) << 16;
     const float sl2 = p.a.scale * 1.4426950408889634f;
+    const unsigned long long sl22 = f2_splat(sl2);
     float* xch = reinterpret_cast<float*>(smem + Cfg::OFF_X);
-    const int i_row = r / p.group;                                // token of this row in the tile
     int g = 0, sq = 0;
     bool ok = true;
     while (ok && walk.next(s)) {
       const int rows = s.tokens * p.group;
-      const bool live = quad * 32 < rows;                         // of this warp: some row is there
+      const bool live = quad * 32 - copy * copy_rows < rows;      // of this warp: some row is there
       float m_run = -INFINITY, l_run = 0.f;
       const uint32_t o_addr = tmem_base + t_lane + Cfg::TM_O + (sq & 1) * HD + half * OC;
       for (int j = 0; j < s.tiles; ++j, ++g) {
@@ -509,48 +588,70 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         tc_fence_after();
         if (live) {
           const uint32_t s_addr = tmem_base + t_lane + Cfg::TM_S + (g & 1) * PA_N;
-          uint32_t sv[64];
-          tmem_ld32(s_addr + half * 64, sv);
-          tmem_ld32(s_addr + half * 64 + 32, sv + 32);
-          tmem_ld_wait();
-          // columns up to lim are seen: the keys that there are, and of a request's own keys those up to the row's token
+          // columns up to `last` are seen: the keys that there are, and of a request's own keys those up to the row's token
           const int last = kt.prompt ? kt.count - 1 : min(kt.count - 1, s.own - s.n + s.i0 + i_row - kt.first);
-          const int first_last = kt.prompt ? kt.count - 1 : min(kt.count - 1, s.own - s.n + s.i0 - kt.first);
-          if (first_last < PA_N - 1) {
-            const int lim = last - half * 64;
+          const bool cut = (kt.prompt ? kt.count - 1 : min(kt.count - 1, s.own - s.n + s.i0 - kt.first)) < PA_N - 1;
+          float alpha = 1.f;
+          bool grow = false;
+          const auto tile = [&](auto copies_of) {                 // 64 / C keys of this thread: half * 64 + copy * W ..
+            constexpr int C = decltype(copies_of)::value, W = 64 / C;
+            uint32_t sv[W];
+            if constexpr (C == 1) { tmem_ld32(s_addr + half * 64, sv); tmem_ld32(s_addr + half * 64 + 32, sv + 32); }
+            else if constexpr (C == 2) tmem_ld32(s_addr + half * 64 + copy * 32, sv);
+            else tmem_ld16(s_addr + half * 64 + copy * 16, sv);
+            tmem_ld_wait();
+            if (cut) {
+              const int lim = last - half * 64 - copy * W;
 #pragma unroll
-            for (int i = 0; i < 64; ++i) sv[i] = i <= lim ? sv[i] : 0xff800000u;
-          }
-          float m0 = __uint_as_float(sv[0]), m1 = __uint_as_float(sv[1]), m2 = __uint_as_float(sv[2]), m3 = __uint_as_float(sv[3]);
+              for (int i = 0; i < W; ++i) sv[i] = i <= lim ? sv[i] : 0xff800000u;
+            }
+            float m0 = __uint_as_float(sv[0]), m1 = __uint_as_float(sv[1]);
 #pragma unroll
-          for (int i = 4; i < 64; i += 4) {
-            m0 = fmaxf(m0, __uint_as_float(sv[i])); m1 = fmaxf(m1, __uint_as_float(sv[i + 1]));
-            m2 = fmaxf(m2, __uint_as_float(sv[i + 2])); m3 = fmaxf(m3, __uint_as_float(sv[i + 3]));
-          }
-          float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-          float* slots = xch + (g & 1) * (2 * PA_M);
-          slots[(half ^ 1) * PA_M + r] = mx;
-          softmax_pair_sync(quad);                                // both halves are in registers: P may go over S
-          mx = fmaxf(mx, slots[half * PA_M + r]) * sl2;
-          const float m_new = fmaxf(m_run, mx);
-          const bool grow = (m_new - m_run) > PA_RESCALE;         // the first time: from -inf
-          const float m_cand = grow ? m_new : m_run;
-          const float m_use = m_cand == -INFINITY ? 0.f : m_cand; // a row that has seen nothing yet
-          const float alpha = grow ? fast_exp2(m_run - m_use) : 1.f;
-          const float neg_m = -m_use;
-          float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
-          uint32_t pk[32];
+            for (int i = 2; i < W - 2; i += 4) {
+              m0 = fmax3(m0, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+              m1 = fmax3(m1, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
+            }
+            float mx = fmax3(m0, m1, fmaxf(__uint_as_float(sv[W - 2]), __uint_as_float(sv[W - 1])));
+            float* slots = xch + (g & 1) * (2 * PA_M);
+            slots[(half ^ 1) * PA_M + r] = mx;
+            softmax_pair_sync(quad);                              // both halves are in registers: P may go over S
+            mx = fmaxf(mx, slots[half * PA_M + r]) * sl2;
+            const float m_new = fmaxf(m_run, mx);
+            grow = row < rows && (m_new - m_run) > PA_RESCALE;    // the first time: from -inf.  Not for rows that are not there, whose scores are anything
+            const float m_cand = grow ? m_new : m_run;
+            const float m_use = m_cand == -INFINITY ? 0.f : m_cand;       // a row that has seen nothing yet
+            alpha = grow ? fast_exp2(m_run - m_use) : 1.f;
+            m_run = m_cand;
+            const unsigned long long neg_m = f2_splat(-m_use);
+            unsigned long long l01 = 0, l23 = 0;
+            uint32_t pk[W / 2];
 #pragma unroll
-          for (int i = 0; i < 64; i += 4) {
-            const float e0 = fast_exp2(fmaf(__uint_as_float(sv[i]), sl2, neg_m)), e1 = fast_exp2(fmaf(__uint_as_float(sv[i + 1]), sl2, neg_m));
-            const float e2 = fast_exp2(fmaf(__uint_as_float(sv[i + 2]), sl2, neg_m)), e3 = fast_exp2(fmaf(__uint_as_float(sv[i + 3]), sl2, neg_m));
-            l0 += e0; l1 += e1; l2 += e2; l3 += e3;
-            pk[i >> 1] = pack_bf16x2(e0, e1);                     // weights to bf16, as the tensor cores take them; their sum stays fp32
-            pk[(i >> 1) + 1] = pack_bf16x2(e2, e3);
-          }
-          tmem_st32(s_addr + half * 32, pk);
-          l_run = l_run * alpha + ((l0 + l1) + (l2 + l3));
-          m_run = m_cand;
+            for (int i = 0; i < W; i += 4) {
+              const unsigned long long x01 = f2_fma(f2_of(sv[i], sv[i + 1]), sl22, neg_m), x23 = f2_fma(f2_of(sv[i + 2], sv[i + 3]), sl22, neg_m);
+              // one of eight pairs on the multiply-add pipe, where the special-function units are what a full tile waits for
+              const unsigned long long e01 = exp2_mufu2(x01), e23 = C == 1 && (i >> 2) % 4 == 0 ? exp2_fma2(x23) : exp2_mufu2(x23);
+              l01 = f2_add(l01, e01);
+              l23 = f2_add(l23, e23);
+              pk[i >> 1] = f2_bf16(e01);                          // weights to bf16, as the tensor cores take them; their sum stays fp32
+              pk[(i >> 1) + 1] = f2_bf16(e23);
+            }
+            uint32_t a, b;
+            f2_to(f2_add(l01, l23), a, b);
+            l_run = l_run * alpha + (__uint_as_float(a) + __uint_as_float(b));
+            const uint32_t p_addr = s_addr + half * 32;           // this half's 64 keys: the copy's own, zeros elsewhere
+            const uint32_t z[16] = {};
+            if constexpr (C == 1) tmem_st32(p_addr, pk);
+            else {
+#pragma unroll
+              for (int c = 0; c < C; ++c) {
+                if constexpr (C == 2) { if (c == copy) tmem_st16(p_addr + c * 16, pk); else tmem_st16(p_addr + c * 16, z); }
+                else { if (c == copy) tmem_st8(p_addr + c * 8, pk); else tmem_st8(p_addr + c * 8, z); }
+              }
+            }
+          };
+          if (copies == 4) tile(std::integral_constant<int, 4>());
+          else if (copies == 2) tile(std::integral_constant<int, 2>());
+          else tile(std::integral_constant<int, 1>());
           if (j > 0 && __any_sync(0xffffffffu, grow)) {           // O again to the new maximum, behind the product before
             ok = warp_wait(&o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
             if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
@@ -574,8 +675,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
           const uint32_t base = smem_u32(smem + Cfg::OFF_V + st * Cfg::T_BYTES);
           for (int i = threadIdx.x; i < (PA_N - kt.count) * CHUNKS * 8; i += 256) {
-            const int row = kt.count + i / (CHUNKS * 8), c = i % (CHUNKS * 8);
-            st_shared_v4(base + (c >> 3) * (PA_N * 128) + row * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
+            const int at = kt.count + i / (CHUNKS * 8), c = i % (CHUNKS * 8);
+            st_shared_v4(base + (c >> 3) * (PA_N * 128) + at * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
           }
           fence_proxy_async_smem();
         }
@@ -583,67 +684,171 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (lane == 0) mbar_arrive(&p_full[g & 1]);
       }
       if (!ok) break;
-      if (live) {                                                 // the two halves' sums, in slots of their own: the next tile's maxima may come at once
-        float* slots = xch + 2 * (2 * PA_M);
-        slots[(half ^ 1) * PA_M + r] = l_run;
-        softmax_pair_sync(quad);
-        l_run += slots[half * PA_M + r];
-      }
-      ok = warp_wait(&o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
-      if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
+      ok = warp_wait(&o_free[sq & 1], ((sq >> 1) & 1) ^ 1);       // m and l of the segment before the last have been read
+      if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); break; }
+      float* ml = s_ml + (sq & 1) * 3 * PA_M;
+      if (half == 0) ml[r] = m_run;
+      ml[(1 + half) * PA_M + r] = l_run;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_done[sq & 1]);
+      ++sq;
+    }
+  } else {
+    // ---------------------------------------------------------------- results: warp 8 + q has TMEM lanes 32 q..
+    const int quad = warp & 3, r = quad * 32 + lane, et = threadIdx.x - 256;
+    const int copy = r / copy_rows, row = r - copy * copy_rows;
+    const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16);
+    float* stage = reinterpret_cast<float*>(smem + Cfg::OFF_STAGE);
+    int sq = 0;
+    while (walk.next(s)) {
+      // barriers of segments, of which at most two are under way: this warp may be behind by many tiles
+      bool ok = warp_wait(&seg_done[sq & 1], (sq >> 1) & 1) && warp_wait(&o_full[sq & 1], (sq >> 1) & 1);
+      if (!ok && lane == 0) { report_error(p.status, OA_KERR_WAIT_TMEM_FULL); s_fail = 1; }
+      if (copies > 1) { out_sync(); ok = s_fail == 0; }           // what was staged before has been read; and the four warps leave together
+      if (!ok) break;
       tc_fence_after();
-      if (live) {
-        uint32_t o[OC];
+      const int rows = s.tokens * p.group;
+      const float* ml = s_ml + (sq & 1) * 3 * PA_M;
+      const uint32_t o_addr = t_lane + Cfg::TM_O + (sq & 1) * HD;
+      const bool whole = p.joint && s.tiles == s.item_tiles;      // nothing to be joined
+      const bool first = s.tile > 0 || walk.pos - s.tiles == lo;
+      const long long slot = p.joint ? 2ll * cta + (first ? 0 : 1) : (long long)s.item + cta;
+      const long long at = s.prompt ? prompt_row(p, slot) : own_row(p, slot);
+      // the row's m, l and the factor of this copy's part
+      float m = ml[r], l = ml[PA_M + r] + ml[2 * PA_M + r], f = 1.f;
+      if (copies > 1) {
+        const float mine = m;
+        float sum = 0.f;
+        for (int c = 0; c < copies; ++c) m = fmaxf(m, ml[c * copy_rows + row]);
+        for (int c = 0; c < copies; ++c) {
+          const int o = c * copy_rows + row;
+          const float mc = ml[o];
+          sum += (ml[PA_M + o] + ml[2 * PA_M + o]) * (mc == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : fast_exp2(mc - m));
+        }
+        f = mine == -INFINITY ? 0.f : fast_exp2(mine - m);
+        l = sum;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;                 // NaN stays NaN
+      if (copy == 0 && row < rows) {
+        const int i = token_of(p, row), t = s.t0 + i, hq = s.h * p.group + row - i * p.group;
+        if (!whole) { if (has_room(p, at + row)) p.ml[at + row] = make_float2(m, l); }
+        else if (p.a.lse && t >= 0 && t < p.a.tokens) p.a.lse[(long long)t * p.a.q_heads + hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      }
+      const auto out_at = [&](int rw) -> __nv_bfloat16* {         // of a row, or null
+        const int i = token_of(p, rw), t = s.t0 + i;
+        return rw < rows && t >= 0 && t < p.a.tokens ? static_cast<__nv_bfloat16*>(p.a.out) + ((long long)t * p.a.q_heads + s.h * p.group + rw - i * p.group) * HD : nullptr;
+      };
+      if (copies == 1) {
+        if (quad * 32 < rows) {
+          const int r0 = quad * 32 + (lane & ~3);                 // after an exchange among four lanes a lane has 16 bytes of four rows
 #pragma unroll
-        for (int c = 0; c < OC / 32; ++c) tmem_ld32(o_addr + c * 32, o + c * 32);
-        tmem_ld_wait();
-        const int r0 = quad * 32 + (lane & ~3);                   // after an exchange among four lanes a lane has 16 bytes of four rows
-        if (p.joint && s.tiles == s.item_tiles) {                 // the whole result
-          const float inv = l_run > 0.f ? 1.f / l_run : l_run == 0.f ? 0.f : l_run;      // NaN stays NaN
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + c * 32, o);
+            tmem_ld_wait();
+            if (whole) {
+              uint4 v[4];
 #pragma unroll
-          for (int c = 0; c < OC / 32; ++c) {
-            uint4 v[4];
+              for (int k = 0; k < 4; ++k) {
+                const float* x = reinterpret_cast<const float*>(o) + k * 8;
+                v[k] = make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv), pack_bf16x2(x[6] * inv, x[7] * inv));
+              }
+              exchange4(v, lane);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float* f = reinterpret_cast<const float*>(o) + c * 32 + k * 8;
-              v[k] = make_uint4(pack_bf16x2(f[0] * inv, f[1] * inv), pack_bf16x2(f[2] * inv, f[3] * inv), pack_bf16x2(f[4] * inv, f[5] * inv), pack_bf16x2(f[6] * inv, f[7] * inv));
-            }
-            exchange4(v, lane);
+              for (int k = 0; k < 4; ++k) {
+                __nv_bfloat16* to = out_at(r0 + k);
+                if (to) *reinterpret_cast<uint4*>(to + c * 32 + (lane & 3) * 8) = v[k];
+              }
+            } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int row = r0 + k, t = s.t0 + row / p.group;
-              if (row < rows && t >= 0 && t < p.a.tokens)
-                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.a.out) + ((long long)t * p.a.q_heads + s.h * p.group + row % p.group) * HD + half * OC +
-                                          c * 32 + (lane & 3) * 8) = v[k];
+              for (int e = 0; e < 2; ++e) {
+                uint4 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = make_uint4(o[e * 16 + k * 4], o[e * 16 + k * 4 + 1], o[e * 16 + k * 4 + 2], o[e * 16 + k * 4 + 3]);
+                exchange4(v, lane);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  if (r0 + k < rows && has_room(p, at + r0 + k)) *reinterpret_cast<uint4*>(p.part + (at + r0 + k) * HD + c * 32 + e * 16 + (lane & 3) * 4) = v[k];
+              }
             }
           }
-          const int t = s.t0 + i_row;
-          if (p.a.lse && half == 0 && r < rows && t >= 0 && t < p.a.tokens)
-            p.a.lse[(long long)t * p.a.q_heads + s.h * p.group + r % p.group] = l_run == 0.f ? -INFINITY : (m_run + log2f(l_run)) * 0.6931471805599453f;
-        } else {
-          const long long at = partial_row(p, s, blockIdx.x, s.tile > 0 || walk.pos - s.tiles == lo);
-#pragma unroll
-          for (int c = 0; c < OC / 16; ++c) {
-            uint4 v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = make_uint4(o[c * 16 + k * 4], o[c * 16 + k * 4 + 1], o[c * 16 + k * 4 + 2], o[c * 16 + k * 4 + 3]);
-            exchange4(v, lane);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (r0 + k < rows && has_room(p, at + r0 + k)) *reinterpret_cast<uint4*>(p.part + (at + r0 + k) * HD + half * OC + c * 16 + (lane & 3) * 4) = v[k];
-          }
-          if (half == 0 && r < rows && has_room(p, at + r)) p.ml[at + r] = make_float2(m_run, l_run);
         }
         tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[sq & 1]);
+      } else {
+        // copies meet in shared memory
+        if (copy == 0) s_inv[row] = inv;
+        const auto emit = [&](int rw, int c, float4 sum) {        // four columns of a row
+          if (!whole) {
+            if (has_room(p, at + rw)) *reinterpret_cast<float4*>(p.part + (at + rw) * HD + c) = sum;
+          } else if (__nv_bfloat16* to = out_at(rw)) {
+            const float q = s_inv[rw];
+            *reinterpret_cast<uint2*>(to + c) = make_uint2(pack_bf16x2(sum.x * q, sum.y * q), pack_bf16x2(sum.z * q, sum.w * q));
+          }
+        };
+        const auto release = [&] {                                // all has been read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_free[sq & 1]);
+        };
+        if (rows <= 8 && copies == 4) {
+          // Up to eight rows: a load that gives lane l two neighbouring columns of row l / 4, so that every lane has some of them.  A row to a
+          // lane left 24 lanes or more idle and made a request's single token 1.5 us of it.
+          const float fr = __shfl_sync(0xffffffffu, f, lane >> 2);
+          uint32_t o[HD / 2];
+#pragma unroll
+          for (int c = 0; c < HD / 64; ++c) tmem_ld_16x256b_x8(o_addr + c * 64, o + c * 32);
+          tmem_ld_wait();
+          release();
+          float* to = stage + (copy * 8 + (lane >> 2)) * (HD + 8) + (lane & 3) * 2;
+#pragma unroll
+          for (int c = 0; c < HD / 8; ++c)
+            *reinterpret_cast<float2*>(to + c * 8) = fr == 0.f ? make_float2(0.f, 0.f) : make_float2(__uint_as_float(o[c * 4]) * fr, __uint_as_float(o[c * 4 + 1]) * fr);
+          out_sync();
+          constexpr int PER_ROW = HD / 4;
+          for (int i = et; i < rows * PER_ROW; i += 128) {
+            const int rw = i / PER_ROW, c = (i - rw * PER_ROW) * 4;
+            float4 x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4*>(stage + (k * 8 + rw) * (HD + 8) + c);
+            emit(rw, c, make_float4((x[0].x + x[1].x) + (x[2].x + x[3].x), (x[0].y + x[1].y) + (x[2].y + x[3].y), (x[0].z + x[1].z) + (x[2].z + x[3].z),
+                                    (x[0].w + x[1].w) + (x[2].w + x[3].w)));
+          }
+        } else {
+          for (int c0 = 0; c0 < HD; c0 += 32) {                   // 32 columns at a time
+            if (c0 > 0) out_sync();                               // the columns before have been read
+            uint32_t o[32];
+            tmem_ld32(o_addr + c0, o);
+            tmem_ld_wait();
+            if (c0 + 32 == HD) release();
+            if (row < rows) {
+              float4* to = reinterpret_cast<float4*>(stage + r * 36);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float* x = reinterpret_cast<const float*>(o) + k * 4;
+                to[k] = f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+              }
+            }
+            out_sync();
+            for (int i = et; i < rows * 8; i += 128) {
+              const int rw = i >> 3, c = (i & 7) * 4;
+              float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+              for (int k = 0; k < copies; ++k) {
+                const float4 x = *reinterpret_cast<const float4*>(stage + (k * copy_rows + rw) * 36 + c);
+                sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+              }
+              emit(rw, c0 + c, sum);
+            }
+          }
+        }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&o_free[sq & 1]);
       ++sq;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) { tc_fence_after(); tmem_dealloc<512>(tmem_base); }
+  if (warp == 12) { tc_fence_after(); tmem_dealloc<512>(tmem_base); }
 }
 
 // Joins partial results (acc, m, l) of one row, a warp to a row, a lane to HD / 32 neighbouring columns.
@@ -651,19 +856,40 @@ template <int HD>
 struct RowJoin {
   static constexpr int PER = HD / 32;
   float m = -INFINITY, l = 0.f, acc[PER] = {};
-  __device__ __forceinline__ void add(const PagedTcParams& p, long long row, int lane) {
-    if (!has_room(p, row)) return;
-    const float2 ml = p.ml[row];
-    float v[PER];
-    if (PER == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p.part + row * HD + lane * PER);
-    else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(p.part + row * HD + lane * PER);
-    if (ml.y == 0.f) return;                                     // a piece of which this row saw nothing
-    const float m_new = fmaxf(m, ml.x);
-    const float a = m == -INFINITY ? 0.f : fast_exp2(m - m_new), b = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - m_new);
-    l = l * a + ml.y * b;
+  // `count` pieces, of which row_of(i) is the i-th: the weights of 32 at a time, one to a lane, then their rows, four under way at once
+  template <typename F>
+  __device__ __forceinline__ void add(const PagedTcParams& p, int count, F row_of, int lane) {
+    for (int i0 = 0; i0 < count; i0 += 32) {
+      const int i = i0 + lane;
+      const long long mine = i < count ? row_of(i) : -1;
+      const float2 ml = has_room(p, mine) ? p.ml[mine] : make_float2(-INFINITY, 0.f);
+      const bool some = ml.y != 0.f;                             // otherwise a piece of which this row saw nothing
+      const float m_new = fmaxf(m, warp_max(some ? ml.x : -INFINITY));
+      const float a = m == -INFINITY ? 0.f : fast_exp2(m - m_new), w = some ? (ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - m_new)) : 0.f;
+      l = l * a + warp_sum(ml.y * w);
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = acc[e] * a + v[e] * b;
-    m = m_new;
+      for (int e = 0; e < PER; ++e) acc[e] *= a;
+      m = m_new;
+      const int n = min(count - i0, 32);
+      for (int j0 = 0; j0 < n; j0 += 4) {
+        float v[4][PER], wj[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const long long row = __shfl_sync(0xffffffffu, mine, min(j0 + k, 31));
+          wj[k] = j0 + k < n ? __shfl_sync(0xffffffffu, w, min(j0 + k, 31)) : 0.f;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) v[k][e] = 0.f;
+          if (wj[k] != 0.f) {
+            if (PER == 4) *reinterpret_cast<float4*>(v[k]) = *reinterpret_cast<const float4*>(p.part + row * HD + lane * PER);
+            else *reinterpret_cast<float2*>(v[k]) = *reinterpret_cast<const float2*>(p.part + row * HD + lane * PER);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int e = 0; e < PER; ++e) acc[e] += v[k][e] * wj[k];
+      }
+    }
   }
   __device__ __forceinline__ void write(const PagedTcParams& p, int t, int hq, int lane) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -683,24 +909,27 @@ __global__ void __launch_bounds__(256) paged_join_rows_kernel(const __grid_const
   const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= (long long)p.a.tokens * p.a.q_heads) return;
   const int t = (int)(row / p.a.q_heads), hq = (int)(row - (long long)t * p.a.q_heads), h = hq / p.group, head = hq - h * p.group;
-  const int per = p.sums[0];
+  const int per_prompt = p.sums[1], per = p.sums[2];
   RowJoin<HD> join;
   int b = 0, i = 0;
   if (find_request(p.a.starts, p.a.batch, t, lane, b, i) && i < p.a.max_fresh) {
-    {
-      const int rt = t / p.tpt, item = h * p.prefix_row_tiles + rt, a = item * p.prefix_tiles;
-      for (int c = a / per; c <= (a + p.prefix_tiles - 1) / per; ++c) join.add(p, (long long)(item + c) * PA_M + (t - rt * p.tpt) * p.group + head, lane);
-    }
+    const int prt = t / p.tpt, p_item = h * p.prefix_row_tiles + prt, pa = p_item * p.prefix_tiles;
+    const int p_first = pa / per_prompt, p_count = (pa + p.prefix_tiles - 1) / per_prompt - p_first + 1;
     const Request r = request_of(p, b);
     const int rt = i / p.tpt, tiles = tiles_of(p, r, rt);
+    int first = 0, count = 0, item = 0;
     if (tiles > 0) {
-      const int before = p.sums[2 + b], all = p.sums[3 + b] - before;
-      int a = p.prefix_work + before * p.a.kv_heads + h * all;
+      const int before = p.sums[PA_SUMS + b], all = p.sums[PA_SUMS + b + 1] - before;
+      int a = before * p.a.kv_heads + h * all;
       for (int k = 0; k < rt; ++k) a += tiles_of(p, r, k);
-      const int item = p.sums[3 + p.a.batch + b] * p.a.kv_heads + h * r.row_tiles + rt;
-      for (int c = a / per; c <= (a + tiles - 1) / per; ++c)
-        join.add(p, p.own_slot0 + (long long)(item + c) * (p.ts * p.group) + (i - rt * p.tpt) * p.group + head, lane);
+      item = p.sums[PA_SUMS + 1 + p.a.batch + b] * p.a.kv_heads + h * r.row_tiles + rt;
+      first = a / per;
+      count = (a + tiles - 1) / per - first + 1;
     }
+    join.add(p, p_count + count, [&](int k) -> long long {
+      return k < p_count ? prompt_row(p, (long long)p_item + p_first + k) + (t - prt * p.tpt) * p.group + head
+                         : own_row(p, (long long)item + first + k - p_count) + (i - rt * p.tpt) * p.group + head;
+    }, lane);
   }
   join.write(p, t, hq, lane);
 }
@@ -711,19 +940,18 @@ template <int HD>
 __global__ void __launch_bounds__(256) paged_join_cuts_kernel(const __grid_constant__ PagedTcParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = p.sums[0], work = p.sums[1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = p.sums[2], work = p.sums[3];
   const long long cut = (long long)(blockIdx.x + 1) * per;       // the first tile of the next stretch
   if (cut < work) {
-    Walk walk(p, p.sums + 2, p.sums + 3 + p.a.batch, (int)cut, work);
+    Walk walk(p, p.sums + PA_SUMS, p.sums + PA_SUMS + 1 + p.a.batch, false, (int)cut, work);
     Segment s;
     if (walk.next(s) && s.tile > 0 && s.tile <= per) {           // begins in this stretch (at its very first tile at the earliest)
-      const int a = (int)cut - s.tile, last = (a + s.item_tiles - 1) / per;
+      const int a = (int)cut - s.tile, last = (a + s.item_tiles - 1) / per, c0 = blockIdx.x;
       for (int r = warp; r < s.tokens * p.group; r += 8) {
         RowJoin<HD> join;
-        for (int c = blockIdx.x; c <= last; ++c) {
-          const bool first = (long long)c * per >= a;             // the piece is the first of its CTA
-          join.add(p, p.own_slot0 + (2ll * c + (first ? 0 : 1)) * (p.ts * p.group) + r, lane);
-        }
+        join.add(p, last - c0 + 1, [&](int k) -> long long {      // the piece is the first of its CTA, but for an item that begins inside
+          return own_row(p, 2ll * (c0 + k) + ((long long)(c0 + k) * per >= a ? 0 : 1)) + r;
+        }, lane);
         const int t = s.t0 + r / p.group;
         if (t >= 0 && t < p.a.tokens) join.write(p, t, s.h * p.group + r % p.group, lane);
       }
@@ -745,7 +973,7 @@ using namespace oa;
 
 // The sizes that follow from a call's arguments: which form, how many items there can be, what they need in scratch.
 struct PagedTcPlan {
-  int group, tpt, ts, joint, prefix_tiles, prefix_row_tiles, grid;
+  int group, tpt, ts, tb, copies, copies_prompt, joint, prefix_tiles, prefix_row_tiles, grid;
   long long prompt_rows, own_rows, items;
   size_t o_bytes, ml_bytes, bytes;
 };
@@ -762,17 +990,20 @@ static PagedTcPlan plan_tc(int tokens, int batch, int max_fresh, int q_heads, in
   c.group = q_heads / kv_heads;
   c.tpt = PA_M / c.group;
   c.ts = max_fresh < c.tpt ? (max_fresh > 0 ? max_fresh : 1) : c.tpt;
+  c.tb = tokens < c.tpt ? tokens : c.tpt;
+  c.copies = c.ts * c.group <= 32 ? 4 : c.ts * c.group <= 64 ? 2 : 1;
+  c.copies_prompt = c.tb * c.group <= 32 ? 4 : c.tb * c.group <= 64 ? 2 : 1;
   c.prefix_tiles = (prefix_len + PA_N - 1) / PA_N;
   c.prefix_row_tiles = (tokens + c.tpt - 1) / c.tpt;
   // The prompt for the whole batch at once where that reads it at most half as often as request by request.
   c.joint = prefix_len == 0 || 2ll * c.prefix_row_tiles > batch;
   c.grid = sm_count();
   c.items = ((long long)batch + tokens / c.tpt) * kv_heads;                    // query tiles of single requests, at most
-  c.prompt_rows = c.joint ? 0 : ((long long)c.prefix_row_tiles * kv_heads + c.grid) * PA_M;
+  c.prompt_rows = c.joint ? 0 : ((long long)c.prefix_row_tiles * kv_heads + c.grid) * (c.tb * c.group);
   c.own_rows = (c.joint ? 2ll * c.grid : c.items + c.grid) * (c.ts * c.group);
   c.o_bytes = (size_t)(c.prompt_rows + c.own_rows) * head_dim * sizeof(float);
   c.ml_bytes = (size_t)(c.prompt_rows + c.own_rows) * sizeof(float2);
-  c.bytes = c.o_bytes + c.ml_bytes + (2 * ((size_t)batch + 1) + 2) * sizeof(int);
+  c.bytes = c.o_bytes + c.ml_bytes + (2 * ((size_t)batch + 1) + PA_SUMS) * sizeof(int);
   return c;
 }
 // Which calls the tensor-core kernel takes: bf16, head dims of whole 128-byte rows, a batch whose prefix sums fit in shared memory beside the
@@ -807,7 +1038,8 @@ static int launch_tc(const PagedAttnParams& a, void* scratch, int* status, cudaS
   if (work + c.items * (own_tiles + c.prefix_tiles + 1) > 0x7fffffffll) return OA_ERR_TOO_LARGE;
   PagedTcParams p;
   p.a = a;
-  p.group = c.group; p.tpt = c.tpt; p.ts = c.ts;
+  p.group = c.group; p.group_mul = 65536 / c.group + 1; p.tpt = c.tpt; p.ts = c.ts; p.tb = c.tb;
+  p.copies = c.copies; p.copies_prompt = c.copies_prompt;
   p.joint = c.joint; p.prefix_tiles = c.prefix_tiles; p.prefix_row_tiles = c.prefix_row_tiles; p.prefix_work = (int)work;
   p.part = static_cast<float*>(scratch);
   p.ml = reinterpret_cast<float2*>(static_cast<char*>(scratch) + c.o_bytes);
@@ -819,7 +1051,7 @@ static int launch_tc(const PagedAttnParams& a, void* scratch, int* status, cudaS
   int rc;
   {
     const uint64_t dims[3] = {HD, (uint64_t)a.q_heads, (uint64_t)a.tokens}, strides[2] = {HD * 2, (uint64_t)a.q_stride * 2};
-    const uint32_t box[3] = {64, (uint32_t)c.group, (uint32_t)c.tpt}, own[3] = {64, (uint32_t)c.group, (uint32_t)c.ts};
+    const uint32_t box[3] = {64, (uint32_t)c.group, (uint32_t)c.tb}, own[3] = {64, (uint32_t)c.group, (uint32_t)c.ts};
     if ((rc = make_tmap_box3_bf16(&tq, a.q, dims, strides, box)) || (rc = make_tmap_box3_bf16(&tqo, a.q, dims, strides, own))) return rc;
   }
   const uint64_t packed = (uint64_t)a.kv_heads * ps * HD;

@@ -144,19 +144,20 @@ __global__ void __launch_bounds__(128) paged_attn_rows_kernel(const PagedAttnPar
 // second launch joins them.  Where everything goes follows from prefix sums over the batch that each CTA makes for itself; CTA 0 leaves them
 // for the second launch.
 //
-// Inside a CTA, segments run through one pipeline of tiles, g = 0, 1, ..:  warps 13 and 14 load Q (two buffers) and K, and V, by TMA, a box
-// for each page;  warp 12 issues S[g & 1] = Q K_g^T two tiles ahead of O[segment & 1] += P_g V_g, P taken from TMEM;  warps 0-7 are the
+// Inside a CTA, warp 15 works out the segments, one after the other, and leaves them in a list of eight in shared memory (every warp on
+// its own needed so much code that the warps waited for instructions: 32 requests behind 2048 tokens 59 us).  They run through one pipeline of tiles,
+// g = 0, 1, ..:  warps 13 and 14 load Q (two buffers) and K, and V, by TMA, a box for each page;  warp 12 issues S[g & 1] = Q K_g^T two tiles ahead of O[segment & 1] += P_g V_g, P taken from TMEM;  warps 0-7 are the
 // softmax, two threads to a row;  warps 8-11 write a segment's result out while the next one runs.
 //
 // Few rows: a warp reaches only its own quarter of the TMEM lanes, and the two warps of a quarter share a scheduler, so that 32 rows alone
-// would take as long as 128 (0.9 us a tile, where the products need 0.55).  Up to 32 (64) rows therefore lie in the tile four (two) times, and
-// copy c takes a quarter (half) of a tile's keys, its other weights being zeros; the copies' results are joined on the way out.
+// would take as long as 128 (0.9 us a tile, where the products need 0.55).  Up to 32 rows therefore lie in the tile four times, and copy c
+// takes a quarter of a tile's keys, its other weights being zeros; the copies' results are joined on the way out.
 //
 // Keys beyond a length are cut off from the scores by a select, and their values are overwritten by zeros before the product: what lies there
 // (the rest of a page, or of the ring) may be anything, NaN included.
 // The product P_g V_g has a barrier for even and one for odd tiles: the scores of tile g + 1 do not wait for it, so that a reader may be two
 // products ahead of one barrier's phase.
-constexpr int PA_M = 128, PA_N = 128, PA_THREADS = 480, PA_MAX_BATCH = 1024;
+constexpr int PA_M = 128, PA_N = 128, PA_THREADS = 512, PA_MAX_BATCH = 1024, PA_LIST = 8;
 constexpr float PA_RESCALE = 8.f;          // log2: the running maximum is let be while rows grow by less
 
 template <int HD> struct PaCfg {
@@ -166,7 +167,7 @@ template <int HD> struct PaCfg {
   static constexpr int OFF_X = OFF_V + NV * T_BYTES;             // float[2 parities][2 halves][128]: maxima of a tile's halves
   static constexpr int OFF_ML = OFF_X + 2 * 2 * PA_M * 4;        // float[2 segments][3][128]: m, and l of either half
   static constexpr int OFF_STAGE = OFF_ML + 2 * 3 * PA_M * 4;    // float[128][36] (or [32][HD + 8]): results of copies on the way out
-  static constexpr int OFF_BAR = OFF_STAGE + PA_M * 36 * 4, OFF_SCAN = OFF_BAR + 512;
+  static constexpr int OFF_BAR = OFF_STAGE + PA_M * 36 * 4, OFF_LIST = OFF_BAR + 512, OFF_SCAN = OFF_LIST + PA_LIST * 48;
   static constexpr int SMEM_BYTES = OFF_SCAN + 2 * (PA_MAX_BATCH + 1) * 4;
   static constexpr int TM_S = 0, TM_O = 256;
 };
@@ -310,18 +311,29 @@ struct Walk {
   }
 };
 
+// What the warps have to know of a segment, as it lies in the list.
+struct __align__(16) Listed {
+  int tiles;                               // 0: no more
+  int tile, flags, h, b;                   // first key tile in the item; 1: of the prompt, 2: a whole result
+  int t0, rows;                            // first token, rows
+  int seen, shift;                         // own keys that some row sees; the row of token i sees own keys up to shift + i
+  int pad;
+  long long at;                            // where its partial rows go
+};
+static_assert(sizeof(Listed) == 48, "a list entry");
+
 // Keys of key tile j of a segment's item: how many there are and where in their table they begin.
 struct KeyTile { int prompt, first, count; };
-__device__ __forceinline__ KeyTile key_tile(const PagedTcParams& p, const Segment& s, int j) {
+__device__ __forceinline__ KeyTile key_tile(const PagedTcParams& p, int flags, int seen, int j) {
   KeyTile k;
-  k.prompt = s.prompt || (p.joint && j < p.prefix_tiles);
+  k.prompt = (flags & 1) || (p.joint && j < p.prefix_tiles);
   k.first = (k.prompt || !p.joint ? j : j - p.prefix_tiles) * PA_N;
-  k.count = max(min(PA_N, (k.prompt ? p.a.prefix_len : s.seen) - k.first), 0);
+  k.count = max(min(PA_N, (k.prompt ? p.a.prefix_len : seen) - k.first), 0);
   return k;
 }
 // The page, for lane i, that holds the tile's keys from i * page_size on; -1 for lanes without one.  `boxes`: how many there are.
-__device__ __forceinline__ int page_for(const PagedTcParams& p, const Segment& s, int j, int lane, int& boxes) {
-  const KeyTile k = key_tile(p, s, j);
+__device__ __forceinline__ int page_for(const PagedTcParams& p, const Listed& s, int j, int lane, int& boxes) {
+  const KeyTile k = key_tile(p, s.flags, s.seen, j);
   boxes = (k.count + (1 << p.a.page_log2) - 1) >> p.a.page_log2;
   if (lane >= boxes) return -1;
   const int at = (k.first >> p.a.page_log2) + lane;
@@ -405,7 +417,9 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
   uint64_t *q_full = bars, *q_empty = bars + 2, *k_full = bars + 4, *k_empty = k_full + NK, *v_full = k_empty + NK, *v_empty = v_full + NV;
   uint64_t *s_full = v_empty + NV, *p_full = s_full + 2, *o_done = s_full + 4, *o_free = s_full + 6, *seg_done = s_full + 8, *o_full = s_full + 10;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 12);
+  uint64_t *listed = s_full + 12, *list_free = listed + PA_LIST;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(list_free + PA_LIST);
+  const Listed* list = reinterpret_cast<const Listed*>(smem + Cfg::OFF_LIST);
   int* tiles_before = reinterpret_cast<int*>(smem + Cfg::OFF_SCAN);
   int* items_before = tiles_before + p.a.batch + 1;
   float* s_ml = reinterpret_cast<float*>(smem + Cfg::OFF_ML);
@@ -422,10 +436,11 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
     for (int i = 0; i < NK; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
     for (int i = 0; i < NV; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
+    for (int i = 0; i < PA_LIST; ++i) { mbar_init(&listed[i], 1); mbar_init(&list_free[i], 15); }
     mbar_fence_init();
+    s_fail = 0;
   }
   if (warp == 12) { tmem_alloc<512>(tmem_slot); tmem_relinquish(); }
-  if (threadIdx.x == 0) s_fail = 0;
   if (warp == 13 && lane == 0) { tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmQown); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); }
   __syncwarp();
   pdl_wait();
@@ -442,19 +457,62 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const Stretches deal = stretches_of(p, own_tiles * p.a.kv_heads, own_items * p.a.kv_heads, gridDim.x);
-  if (blockIdx.x == 0) {                   // for the second launch
-    if (threadIdx.x == 0) { p.sums[0] = deal.prompt_ctas; p.sums[1] = deal.per_prompt; p.sums[2] = deal.per; p.sums[3] = deal.own_work; }
-    for (int b = threadIdx.x; b <= p.a.batch; b += PA_THREADS) { p.sums[PA_SUMS + b] = tiles_before[b]; p.sums[PA_SUMS + 1 + p.a.batch + b] = items_before[b]; }
-  }
   const bool on_prompt = (int)blockIdx.x < deal.prompt_ctas;
-  const int cta = on_prompt ? blockIdx.x : blockIdx.x - deal.prompt_ctas, per = on_prompt ? deal.per_prompt : deal.per;
-  const int work = on_prompt ? p.prefix_work : deal.own_work;
-  const int lo = (int)min((long long)cta * per, (long long)work), hi = (int)min((long long)(cta + 1) * per, (long long)work);
-  Walk walk(p, tiles_before, items_before, on_prompt, lo, hi);
-  Segment s;
-  const int copies = on_prompt ? p.copies_prompt : p.copies, copy_rows = PA_M / copies;
+  const int copies = on_prompt ? p.copies_prompt : p.copies, copy_rows = PA_M / copies;     // 1 and 128, or 4 and 32
 
-  if (warp == 13 || warp == 14) {
+  // The next entry of the list.  Every warp reads each once, in order, and lets go of it when it has what it needs.
+  int li = 0;
+  uint32_t lphase = 0;
+  const auto take = [&](Listed& s, bool& ok) -> bool {
+    ok = warp_wait(&listed[li], lphase);
+    if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
+    s = list[li];
+    return s.tiles > 0;
+  };
+  const auto let_go = [&] {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&list_free[li]);
+    if (++li == PA_LIST) { li = 0; lphase ^= 1; }
+  };
+  Listed s;
+  bool ok = true;
+
+  if (warp == 15) {
+    // ---------------------------------------------------------------- segments
+    if (blockIdx.x == 0) {                 // for the second launch
+      if (lane == 0) { p.sums[0] = deal.prompt_ctas; p.sums[1] = deal.per_prompt; p.sums[2] = deal.per; p.sums[3] = deal.own_work; }
+      for (int b = lane; b <= p.a.batch; b += 32) { p.sums[PA_SUMS + b] = tiles_before[b]; p.sums[PA_SUMS + 1 + p.a.batch + b] = items_before[b]; }
+    }
+    if (lane == 0) {
+      const int cta = on_prompt ? blockIdx.x : blockIdx.x - deal.prompt_ctas, per = on_prompt ? deal.per_prompt : deal.per;
+      const int work = on_prompt ? p.prefix_work : deal.own_work;
+      const int lo = (int)min((long long)cta * per, (long long)work), hi = (int)min((long long)(cta + 1) * per, (long long)work);
+      Walk walk(p, tiles_before, items_before, on_prompt, lo, hi);
+      Segment g;
+      bool more = true;
+      while (more) {
+        more = walk.next(g);
+        if (!mbar_wait(&list_free[li], lphase ^ 1)) { report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
+        Listed e;
+        e.tiles = more ? g.tiles : 0;
+        e.tile = g.tile;
+        e.flags = (g.prompt ? 1 : 0) | (p.joint && g.tiles == g.item_tiles ? 2 : 0);
+        e.h = g.h;
+        e.b = g.b;
+        e.t0 = g.t0;
+        e.rows = g.tokens * p.group;
+        e.seen = g.seen;
+        e.shift = g.own - g.n + g.i0;
+        const bool first = g.tile > 0 || walk.pos - g.tiles == lo;
+        const long long slot = p.joint ? 2ll * cta + (first ? 0 : 1) : (long long)g.item + cta;
+        e.at = g.prompt ? prompt_row(p, slot) : own_row(p, slot);
+        reinterpret_cast<Listed*>(smem + Cfg::OFF_LIST)[li] = e;
+        mbar_arrive(&listed[li]);
+        if (++li == PA_LIST) { li = 0; lphase ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 13 || warp == 14) {
     // ---------------------------------------------------------------- loads: warp 13 Q and K, warp 14 V
     const bool is_k = warp == 13;
     const int ps = 1 << p.a.page_log2, ring = is_k ? NK : NV;
@@ -463,35 +521,37 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const CUtensorMap* map = is_k ? &tmK : &tmV;
     int st = 0, sq = 0, boxes = 0, id = -1;
     uint32_t phase = 1;                                           // of the slot to fill: free at first
-    bool ok = true, more = walk.next(s);
-    if (more) id = page_for(p, s, s.tile, lane, boxes);
+    bool more = take(s, ok);
+    if (more) { let_go(); id = page_for(p, s, s.tile, lane, boxes); }
     while (ok && more) {
+      const int n = s.tiles, h = s.h;
       if (is_k) {
         const int qb = sq & 1;
         ok = warp_wait(&q_empty[qb], ((sq >> 1) & 1) ^ 1);
         if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
         if (elect_one()) {
-          const int tokens = s.prompt ? p.tb : p.ts;
-          mbar_expect_tx(&q_full[qb], (uint32_t)(copies * tokens * p.group * HD * 2));
+          const CUtensorMap* mq = (s.flags & 1) ? &tmQ : &tmQown;
+          mbar_expect_tx(&q_full[qb], (uint32_t)(copies * ((s.flags & 1) ? p.tb : p.ts) * p.group * HD * 2));
+#pragma unroll 1
           for (int c = 0; c < copies; ++c)
 #pragma unroll
             for (int x = 0; x < CHUNKS; ++x)
-              tma_load_3d(smem + Cfg::OFF_Q + qb * Cfg::Q_BYTES + x * (PA_M * 128) + c * copy_rows * 128, s.prompt ? &tmQ : &tmQown, &q_full[qb], x * 64,
-                          s.h * p.group, s.t0);
+              tma_load_3d(smem + Cfg::OFF_Q + qb * Cfg::Q_BYTES + x * (PA_M * 128) + c * copy_rows * 128, mq, &q_full[qb], x * 64, h * p.group, s.t0);
         }
         __syncwarp();
         ++sq;
       }
-      const int n = s.tiles, h = s.h;
+#pragma unroll 1
       for (int j = 0; j < n; ++j) {
-        const int now = id, now_boxes = boxes;                    // the next tile's page, of the next segment's first where this is the last
-        if (j + 1 < n) {
-          id = page_for(p, s, s.tile + j + 1, lane, boxes);
-        } else {
-          more = walk.next(s);
-          if (more) id = page_for(p, s, s.tile, lane, boxes);
+        const int now = id, now_boxes = boxes;                    // and the next tile's page, of the next segment's first where this is the last
+        int next = s.tile + j + 1;
+        if (j + 1 == n) {
+          more = take(s, ok);
+          if (more) let_go();
+          next = s.tile;
         }
-        ok = warp_wait(&empty[st], phase);
+        if (more) id = page_for(p, s, next, lane, boxes);
+        if (ok) ok = warp_wait(&empty[st], phase);
         if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
         if (elect_one()) mbar_expect_tx(&full[st], (uint32_t)(now_boxes * ps * HD * 2));
         __syncwarp();
@@ -509,13 +569,15 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     constexpr uint32_t idesc_qk = umma_idesc_bf16(PA_M, PA_N, 0, 0), idesc_pv = umma_idesc_bf16(PA_M, HD, 0, 1);
     const uint64_t q_desc = umma_smem_desc_sw128(smem_u32(smem + Cfg::OFF_Q), 16, 1024), k_desc = umma_smem_desc_sw128(smem_u32(smem + Cfg::OFF_K), 16, 1024);
     const uint64_t v_desc = umma_smem_desc_sw128(smem_u32(smem + Cfg::OFF_V), PA_N * 128, 1024);
-    Walk ahead(p, tiles_before, items_before, on_prompt, lo, hi);         // of the score products, two tiles ahead
-    Segment sa;
-    int ja = 0, na = 0, sqa = -1, ga = 0;
+    int ja = 0, na = 0, sqa = -1, ga = 0, la = 0;                 // of the score products, two tiles ahead
+    uint32_t laphase = 0;
     const auto issue_qk = [&]() -> bool {                         // the next score product, if there is one
       if (ja == na) {
-        if (!ahead.next(sa)) return true;
-        ja = 0; na = sa.tiles; ++sqa;
+        if (!warp_wait(&listed[la], laphase)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
+        const int n = list[la].tiles;
+        if (n == 0) return true;
+        if (++la == PA_LIST) { la = 0; laphase ^= 1; }
+        ja = 0; na = n; ++sqa;
         if (!warp_wait(&q_full[sqa & 1], (sqa >> 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
       }
       const int st = ga % NK;
@@ -536,13 +598,18 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       ++ja; ++ga;
       return true;
     };
-    bool ok = issue_qk();
-    if (ok) ok = issue_qk();
-    int g = 0, sq = 0;
-    while (ok && walk.next(s)) {
-      ok = warp_wait(&o_free[sq & 1], ((sq >> 1) & 1) ^ 1);       // the result before the last has been read
-      if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); break; }
-      for (int j = 0; j < s.tiles; ++j, ++g) {
+    int g = -2, sq = 0, j = 0, n = 0;                             // g: the tile whose values come next, behind two score products
+#pragma unroll 1
+    while (ok) {
+      if (g >= 0) {
+        if (j == n) {
+          if (!take(s, ok)) break;
+          let_go();
+          n = s.tiles;
+          j = 0;
+          ok = warp_wait(&o_free[sq & 1], ((sq >> 1) & 1) ^ 1);   // the result before the last has been read
+          if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); break; }
+        }
         const int st = g % NV;
         ok = warp_wait(&v_full[st], (g / NV) & 1);
         if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
@@ -557,47 +624,47 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         (j > 0 || ks > 0) ? 1u : 0u);
           umma_commit(&v_empty[st]);
           umma_commit(&o_done[g & 1]);
-          if (j + 1 == s.tiles) umma_commit(&o_full[sq & 1]);
+          if (j + 1 == n) umma_commit(&o_full[sq & 1]);
         }
         __syncwarp();
-        ok = issue_qk();                                          // over S[g & 1] = P_g: behind its product in the pipe
-        if (!ok) break;
+        if (++j == n) ++sq;
       }
-      ++sq;
+      ok = issue_qk();                                            // over S[g & 1] = P_g: behind its product in the pipe
+      ++g;
     }
   } else if (warp < 8) {
     // ---------------------------------------------------------------- softmax: warp w has TMEM lanes 32 (w % 4).. and the keys of half w / 4 of a tile
     constexpr int OC = HD / 2;
     const int quad = warp & 3, half = warp >> 2, r = quad * 32 + lane;
-    const int copy = r / copy_rows, row = r - copy * copy_rows, i_row = token_of(p, row);   // i_row: token of this row in the tile
+    const int copy = copies == 1 ? 0 : quad, row = copies == 1 ? r : lane, i_row = token_of(p, row);      // i_row: token of this row in the tile
     const uint32_t t_lane = (uint32_t)(quad * 32) << 16;
     const float sl2 = p.a.scale * 1.4426950408889634f;
     const unsigned long long sl22 = f2_splat(sl2);
     float* xch = reinterpret_cast<float*>(smem + Cfg::OFF_X);
     int g = 0, sq = 0;
-    bool ok = true;
-    while (ok && walk.next(s)) {
-      const int rows = s.tokens * p.group;
-      const bool live = quad * 32 - copy * copy_rows < rows;      // of this warp: some row is there
+#pragma unroll 1
+    while (ok && take(s, ok)) {
+      let_go();
+      const bool live = copies > 1 || quad * 32 < s.rows;         // of this warp: some row is there
       float m_run = -INFINITY, l_run = 0.f;
       const uint32_t o_addr = tmem_base + t_lane + Cfg::TM_O + (sq & 1) * HD + half * OC;
+#pragma unroll 1
       for (int j = 0; j < s.tiles; ++j, ++g) {
-        const KeyTile kt = key_tile(p, s, s.tile + j);
+        const KeyTile kt = key_tile(p, s.flags, s.seen, s.tile + j);
         ok = warp_wait(&s_full[g & 1], (g >> 1) & 1);
         if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
         tc_fence_after();
         if (live) {
           const uint32_t s_addr = tmem_base + t_lane + Cfg::TM_S + (g & 1) * PA_N;
           // columns up to `last` are seen: the keys that there are, and of a request's own keys those up to the row's token
-          const int last = kt.prompt ? kt.count - 1 : min(kt.count - 1, s.own - s.n + s.i0 + i_row - kt.first);
-          const bool cut = (kt.prompt ? kt.count - 1 : min(kt.count - 1, s.own - s.n + s.i0 - kt.first)) < PA_N - 1;
+          const int last = kt.prompt ? kt.count - 1 : min(kt.count - 1, s.shift + i_row - kt.first);
+          const bool cut = (kt.prompt ? kt.count - 1 : min(kt.count - 1, s.shift - kt.first)) < PA_N - 1;
           float alpha = 1.f;
           bool grow = false;
           const auto tile = [&](auto copies_of) {                 // 64 / C keys of this thread: half * 64 + copy * W ..
             constexpr int C = decltype(copies_of)::value, W = 64 / C;
             uint32_t sv[W];
             if constexpr (C == 1) { tmem_ld32(s_addr + half * 64, sv); tmem_ld32(s_addr + half * 64 + 32, sv + 32); }
-            else if constexpr (C == 2) tmem_ld32(s_addr + half * 64 + copy * 32, sv);
             else tmem_ld16(s_addr + half * 64 + copy * 16, sv);
             tmem_ld_wait();
             if (cut) {
@@ -617,7 +684,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             softmax_pair_sync(quad);                              // both halves are in registers: P may go over S
             mx = fmaxf(mx, slots[half * PA_M + r]) * sl2;
             const float m_new = fmaxf(m_run, mx);
-            grow = row < rows && (m_new - m_run) > PA_RESCALE;    // the first time: from -inf.  Not for rows that are not there, whose scores are anything
+            grow = row < s.rows && (m_new - m_run) > PA_RESCALE;  // the first time: from -inf.  Not for rows that are not there, whose scores are anything
             const float m_cand = grow ? m_new : m_run;
             const float m_use = m_cand == -INFINITY ? 0.f : m_cand;       // a row that has seen nothing yet
             alpha = grow ? fast_exp2(m_run - m_use) : 1.f;
@@ -639,24 +706,21 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             f2_to(f2_add(l01, l23), a, b);
             l_run = l_run * alpha + (__uint_as_float(a) + __uint_as_float(b));
             const uint32_t p_addr = s_addr + half * 32;           // this half's 64 keys: the copy's own, zeros elsewhere
-            const uint32_t z[16] = {};
             if constexpr (C == 1) tmem_st32(p_addr, pk);
             else {
+              uint32_t all[32];
 #pragma unroll
-              for (int c = 0; c < C; ++c) {
-                if constexpr (C == 2) { if (c == copy) tmem_st16(p_addr + c * 16, pk); else tmem_st16(p_addr + c * 16, z); }
-                else { if (c == copy) tmem_st8(p_addr + c * 8, pk); else tmem_st8(p_addr + c * 8, z); }
-              }
+              for (int i = 0; i < 32; ++i) all[i] = (i >> 3) == copy ? pk[i & 7] : 0u;
+              tmem_st32(p_addr, all);
             }
           };
-          if (copies == 4) tile(std::integral_constant<int, 4>());
-          else if (copies == 2) tile(std::integral_constant<int, 2>());
+          if (copies > 1) tile(std::integral_constant<int, 4>());
           else tile(std::integral_constant<int, 1>());
           if (j > 0 && __any_sync(0xffffffffu, grow)) {           // O again to the new maximum, behind the product before
             ok = warp_wait(&o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
             if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < OC / 32; ++c) {
               uint32_t o[32];
               tmem_ld32(o_addr + c * 32, o);
@@ -674,6 +738,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           ok = warp_wait(&v_full[st], (g / NV) & 1);
           if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
           const uint32_t base = smem_u32(smem + Cfg::OFF_V + st * Cfg::T_BYTES);
+#pragma unroll 1
           for (int i = threadIdx.x; i < (PA_N - kt.count) * CHUNKS * 8; i += 256) {
             const int at = kt.count + i / (CHUNKS * 8), c = i % (CHUNKS * 8);
             st_shared_v4(base + (c >> 3) * (PA_N * 128) + at * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
@@ -696,119 +761,104 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   } else {
     // ---------------------------------------------------------------- results: warp 8 + q has TMEM lanes 32 q..
     const int quad = warp & 3, r = quad * 32 + lane, et = threadIdx.x - 256;
-    const int copy = r / copy_rows, row = r - copy * copy_rows;
+    const int copy = copies == 1 ? 0 : quad, row = copies == 1 ? r : lane, i_row = token_of(p, row);
     const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16);
     float* stage = reinterpret_cast<float*>(smem + Cfg::OFF_STAGE);
     int sq = 0;
-    while (walk.next(s)) {
+    bool met = false;
+#pragma unroll 1
+    while (take(s, ok)) {
+      let_go();
       // barriers of segments, of which at most two are under way: this warp may be behind by many tiles
-      bool ok = warp_wait(&seg_done[sq & 1], (sq >> 1) & 1) && warp_wait(&o_full[sq & 1], (sq >> 1) & 1);
+      ok = warp_wait(&seg_done[sq & 1], (sq >> 1) & 1) && warp_wait(&o_full[sq & 1], (sq >> 1) & 1);
       if (!ok && lane == 0) { report_error(p.status, OA_KERR_WAIT_TMEM_FULL); s_fail = 1; }
       if (copies > 1) { out_sync(); ok = s_fail == 0; }           // what was staged before has been read; and the four warps leave together
-      if (!ok) break;
+      if (!ok) { met = true; break; }
       tc_fence_after();
-      const int rows = s.tokens * p.group;
       const float* ml = s_ml + (sq & 1) * 3 * PA_M;
       const uint32_t o_addr = t_lane + Cfg::TM_O + (sq & 1) * HD;
-      const bool whole = p.joint && s.tiles == s.item_tiles;      // nothing to be joined
-      const bool first = s.tile > 0 || walk.pos - s.tiles == lo;
-      const long long slot = p.joint ? 2ll * cta + (first ? 0 : 1) : (long long)s.item + cta;
-      const long long at = s.prompt ? prompt_row(p, slot) : own_row(p, slot);
+      const bool whole = s.flags & 2;                             // nothing to be joined
       // the row's m, l and the factor of this copy's part
       float m = ml[r], l = ml[PA_M + r] + ml[2 * PA_M + r], f = 1.f;
       if (copies > 1) {
         const float mine = m;
-        float sum = 0.f;
-        for (int c = 0; c < copies; ++c) m = fmaxf(m, ml[c * copy_rows + row]);
-        for (int c = 0; c < copies; ++c) {
-          const int o = c * copy_rows + row;
-          const float mc = ml[o];
-          sum += (ml[PA_M + o] + ml[2 * PA_M + o]) * (mc == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : fast_exp2(mc - m));
-        }
+        float mc[4], sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) { mc[c] = ml[c * 32 + lane]; m = fmaxf(m, mc[c]); }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          sum += (ml[PA_M + c * 32 + lane] + ml[2 * PA_M + c * 32 + lane]) * (mc[c] == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : fast_exp2(mc[c] - m));
         f = mine == -INFINITY ? 0.f : fast_exp2(mine - m);
         l = sum;
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;                 // NaN stays NaN
-      if (copy == 0 && row < rows) {
-        const int i = token_of(p, row), t = s.t0 + i, hq = s.h * p.group + row - i * p.group;
-        if (!whole) { if (has_room(p, at + row)) p.ml[at + row] = make_float2(m, l); }
-        else if (p.a.lse && t >= 0 && t < p.a.tokens) p.a.lse[(long long)t * p.a.q_heads + hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      const int t = s.t0 + i_row;
+      const bool there = row < s.rows && (whole ? t >= 0 && t < p.a.tokens : has_room(p, s.at + row));
+      const long long out_row = (long long)t * p.a.q_heads + s.h * p.group + row - i_row * p.group;
+      if (copy == 0 && there) {
+        if (!whole) p.ml[s.at + row] = make_float2(m, l);
+        else if (p.a.lse) p.a.lse[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       }
-      const auto out_at = [&](int rw) -> __nv_bfloat16* {         // of a row, or null
-        const int i = token_of(p, rw), t = s.t0 + i;
-        return rw < rows && t >= 0 && t < p.a.tokens ? static_cast<__nv_bfloat16*>(p.a.out) + ((long long)t * p.a.q_heads + s.h * p.group + rw - i * p.group) * HD : nullptr;
-      };
-      if (copies == 1) {
-        if (quad * 32 < rows) {
-          const int r0 = quad * 32 + (lane & ~3);                 // after an exchange among four lanes a lane has 16 bytes of four rows
-#pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + c * 32, o);
-            tmem_ld_wait();
-            if (whole) {
-              uint4 v[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float* x = reinterpret_cast<const float*>(o) + k * 8;
-                v[k] = make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv), pack_bf16x2(x[6] * inv, x[7] * inv));
-              }
-              exchange4(v, lane);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                __nv_bfloat16* to = out_at(r0 + k);
-                if (to) *reinterpret_cast<uint4*>(to + c * 32 + (lane & 3) * 8) = v[k];
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                uint4 v[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = make_uint4(o[e * 16 + k * 4], o[e * 16 + k * 4 + 1], o[e * 16 + k * 4 + 2], o[e * 16 + k * 4 + 3]);
-                exchange4(v, lane);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  if (r0 + k < rows && has_room(p, at + r0 + k)) *reinterpret_cast<uint4*>(p.part + (at + r0 + k) * HD + c * 32 + e * 16 + (lane & 3) * 4) = v[k];
-              }
-            }
-          }
-        }
+      const auto release = [&] {                                  // all has been read
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_free[sq & 1]);
+      };
+      if (copies == 1) {                                          // a row to a lane
+        if (quad * 32 < s.rows) {
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + c, o);
+            tmem_ld_wait();
+            const float* x = reinterpret_cast<const float*>(o);
+            if (!there) {
+            } else if (whole) {
+              uint4* to = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.a.out) + out_row * HD + c);
+#pragma unroll
+              for (int k = 0; k < 4; ++k, x += 8)
+                to[k] = make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv), pack_bf16x2(x[6] * inv, x[7] * inv));
+            } else {
+              uint4* to = reinterpret_cast<uint4*>(p.part + (s.at + row) * HD + c);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) to[k] = make_uint4(o[k * 4], o[k * 4 + 1], o[k * 4 + 2], o[k * 4 + 3]);
+            }
+            __syncwarp();
+          }
+        }
+        release();
       } else {
         // copies meet in shared memory
         if (copy == 0) s_inv[row] = inv;
         const auto emit = [&](int rw, int c, float4 sum) {        // four columns of a row
           if (!whole) {
-            if (has_room(p, at + rw)) *reinterpret_cast<float4*>(p.part + (at + rw) * HD + c) = sum;
-          } else if (__nv_bfloat16* to = out_at(rw)) {
-            const float q = s_inv[rw];
-            *reinterpret_cast<uint2*>(to + c) = make_uint2(pack_bf16x2(sum.x * q, sum.y * q), pack_bf16x2(sum.z * q, sum.w * q));
+            if (has_room(p, s.at + rw)) *reinterpret_cast<float4*>(p.part + (s.at + rw) * HD + c) = sum;
+            return;
           }
+          const int i = token_of(p, rw), tr = s.t0 + i;
+          if (tr < 0 || tr >= p.a.tokens) return;
+          const float q = s_inv[rw];
+          *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.a.out) + ((long long)tr * p.a.q_heads + s.h * p.group + rw - i * p.group) * HD + c) =
+              make_uint2(pack_bf16x2(sum.x * q, sum.y * q), pack_bf16x2(sum.z * q, sum.w * q));
         };
-        const auto release = [&] {                                // all has been read
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&o_free[sq & 1]);
-        };
-        if (rows <= 8 && copies == 4) {
+        if (s.rows <= 8) {
           // Up to eight rows: a load that gives lane l two neighbouring columns of row l / 4, so that every lane has some of them.  A row to a
           // lane left 24 lanes or more idle and made a request's single token 1.5 us of it.
           const float fr = __shfl_sync(0xffffffffu, f, lane >> 2);
+          float* to = stage + (copy * 8 + (lane >> 2)) * (HD + 8) + (lane & 3) * 2;
           uint32_t o[HD / 2];
 #pragma unroll
           for (int c = 0; c < HD / 64; ++c) tmem_ld_16x256b_x8(o_addr + c * 64, o + c * 32);
           tmem_ld_wait();
           release();
-          float* to = stage + (copy * 8 + (lane >> 2)) * (HD + 8) + (lane & 3) * 2;
 #pragma unroll
           for (int c = 0; c < HD / 8; ++c)
             *reinterpret_cast<float2*>(to + c * 8) = fr == 0.f ? make_float2(0.f, 0.f) : make_float2(__uint_as_float(o[c * 4]) * fr, __uint_as_float(o[c * 4 + 1]) * fr);
           out_sync();
           constexpr int PER_ROW = HD / 4;
-          for (int i = et; i < rows * PER_ROW; i += 128) {
-            const int rw = i / PER_ROW, c = (i - rw * PER_ROW) * 4;
+#pragma unroll 1
+          for (int i = et; i < s.rows * PER_ROW; i += 128) {
+            const int rw = i / PER_ROW, c = (i % PER_ROW) * 4;
             float4 x[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4*>(stage + (k * 8 + rw) * (HD + 8) + c);
@@ -816,13 +866,14 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                                     (x[0].w + x[1].w) + (x[2].w + x[3].w)));
           }
         } else {
+#pragma unroll 1
           for (int c0 = 0; c0 < HD; c0 += 32) {                   // 32 columns at a time
             if (c0 > 0) out_sync();                               // the columns before have been read
             uint32_t o[32];
             tmem_ld32(o_addr + c0, o);
             tmem_ld_wait();
             if (c0 + 32 == HD) release();
-            if (row < rows) {
+            if (row < s.rows) {
               float4* to = reinterpret_cast<float4*>(stage + r * 36);
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
@@ -831,11 +882,13 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
               }
             }
             out_sync();
-            for (int i = et; i < rows * 8; i += 128) {
+#pragma unroll 1
+            for (int i = et; i < s.rows * 8; i += 128) {
               const int rw = i >> 3, c = (i & 7) * 4;
               float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-              for (int k = 0; k < copies; ++k) {
-                const float4 x = *reinterpret_cast<const float4*>(stage + (k * copy_rows + rw) * 36 + c);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float4 x = *reinterpret_cast<const float4*>(stage + (k * 32 + rw) * 36 + c);
                 sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
               }
               emit(rw, c0 + c, sum);
@@ -845,6 +898,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       ++sq;
     }
+    if (!ok && copies > 1 && !met) { s_fail = 1; out_sync(); }    // the entry never came: the others, who meet once more, do not wait for this warp
   }
   tc_fence_before();
   __syncthreads();
@@ -991,8 +1045,8 @@ static PagedTcPlan plan_tc(int tokens, int batch, int max_fresh, int q_heads, in
   c.tpt = PA_M / c.group;
   c.ts = max_fresh < c.tpt ? (max_fresh > 0 ? max_fresh : 1) : c.tpt;
   c.tb = tokens < c.tpt ? tokens : c.tpt;
-  c.copies = c.ts * c.group <= 32 ? 4 : c.ts * c.group <= 64 ? 2 : 1;
-  c.copies_prompt = c.tb * c.group <= 32 ? 4 : c.tb * c.group <= 64 ? 2 : 1;
+  c.copies = c.ts * c.group <= 32 ? 4 : 1;
+  c.copies_prompt = c.tb * c.group <= 32 ? 4 : 1;
   c.prefix_tiles = (prefix_len + PA_N - 1) / PA_N;
   c.prefix_row_tiles = (tokens + c.tpt - 1) / c.tpt;
   // The prompt for the whole batch at once where that reads it at most half as often as request by request.

@@ -247,15 +247,18 @@ struct Walk {
   bool prompt, placed;
   __device__ __forceinline__ Walk(const PagedTcParams& p_, const int* tb, const int* ib, bool prompt_, int pos_, int end_)
       : p(p_), tiles_before(tb), items_before(ib), pos(pos_), end(end_), b(0), h(0), rt(0), tile(0), prompt(prompt_), placed(false) {}
-  __device__ __forceinline__ void place() {
-    int lo = 0, n = p.a.batch;             // the last request whose tiles begin at or before pos
+  __device__ __forceinline__ int find() const {      // the last request whose tiles begin at or before pos
+    int lo = 0, n = p.a.batch;
     const int per_head = pos / p.a.kv_heads;
     while (n > 1) {
       const int half = n >> 1;
       if (tiles_before[lo + half] <= per_head) { lo += half; n -= half; } else n = half;
     }
-    b = lo;
-    r = request_of(p, b);
+    return lo;
+  }
+  __device__ __forceinline__ void place(int at, const Request& its) {
+    b = at;
+    r = its;
     const int all = max(tiles_before[b + 1] - tiles_before[b], 1);
     int off = pos - tiles_before[b] * p.a.kv_heads;
     h = off / all;
@@ -278,7 +281,7 @@ struct Walk {
       s.tokens = min(p.tpt, p.a.tokens - s.t0);
       s.b = s.n = s.own = s.seen = s.i0 = 0;
     } else {
-      if (!placed) place();
+      if (!placed) { const int at = find(); place(at, request_of(p, at)); }
       while (rt >= r.row_tiles || tiles_of(p, r, rt) <= tile) {      // on to the next item that has tiles; there is one before `end`
         tile = 0;
         if (++rt >= r.row_tiles) {
@@ -382,6 +385,17 @@ __device__ __forceinline__ long long prompt_row(const PagedTcParams& p, long lon
 // Starts that do not rise would make more items than there is room for: their rows stay out of the scratch.
 __device__ __forceinline__ bool has_room(const PagedTcParams& p, long long row) { return row >= 0 && row < p.part_rows; }
 
+// Whether the phase is complete, without waiting for it.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred P;\n\tmbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\tselp.b32 %0, 1, 0, P;\n\t}\n" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+// Out of the way until the phase completes, for at most about `ns`: a loop over several barriers that only tests them takes issue slots from
+// the warps beside it.
+__device__ __forceinline__ void mbar_nap(uint64_t* bar, uint32_t parity, uint32_t ns) {
+  asm volatile("{\n\t.reg .pred P;\n\tmbarrier.try_wait.parity.shared::cta.b64 P, [%0], %1, %2;\n\t}\n" ::"r"(smem_u32(bar)), "r"(parity), "r"(ns) : "memory");
+}
 __device__ __forceinline__ void softmax_pair_sync(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
 __device__ __forceinline__ void out_sync() { asm volatile("bar.sync 5, 128;" ::: "memory"); }
 // Lanes 0-15 of the quarter, 64 columns: lane l of the warp receives columns 8 k + 2 (l % 4) and the next of row l / 4 in r[4 k], r[4 k + 1], of
@@ -413,7 +427,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int s_warp_sums[2 * PA_THREADS / 32];
   __shared__ float s_inv[PA_M];
-  __shared__ int s_fail;
+  __shared__ int s_fail, s_first;
+  __shared__ Request s_request;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
   uint64_t *q_full = bars, *q_empty = bars + 2, *k_full = bars + 4, *k_empty = k_full + NK, *v_full = k_empty + NK, *v_empty = v_full + NV;
   uint64_t *s_full = v_empty + NV, *p_full = s_full + 2, *o_done = s_full + 4, *o_free = s_full + 6, *seg_done = s_full + 8, *o_full = s_full + 10;
@@ -458,6 +473,13 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const uint32_t tmem_base = *tmem_slot;
   const Stretches deal = stretches_of(p, own_tiles * p.a.kv_heads, own_items * p.a.kv_heads, gridDim.x);
   const bool on_prompt = (int)blockIdx.x < deal.prompt_ctas;
+  const int cta = on_prompt ? blockIdx.x : blockIdx.x - deal.prompt_ctas, per = on_prompt ? deal.per_prompt : deal.per;
+  const int work = on_prompt ? p.prefix_work : deal.own_work;
+  const int lo = (int)min((long long)cta * per, (long long)work), hi = (int)min((long long)(cta + 1) * per, (long long)work);
+  if (!on_prompt)                          // the request in which the stretch begins, by the thread that has scanned it
+    for (int b = threadIdx.x * ((p.a.batch + PA_THREADS - 1) / PA_THREADS), k = 0; k < (p.a.batch + PA_THREADS - 1) / PA_THREADS && b < p.a.batch; ++k, ++b)
+      if (lo >= tiles_before[b] * p.a.kv_heads && lo < tiles_before[b + 1] * p.a.kv_heads) { s_first = b; s_request = request_of(p, b); }
+  __syncthreads();
   const int copies = on_prompt ? p.copies_prompt : p.copies, copy_rows = PA_M / copies;     // 1 and 128, or 4 and 32
 
   // The next entry of the list.  Every warp reads each once, in order, and lets go of it when it has what it needs.
@@ -484,10 +506,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       for (int b = lane; b <= p.a.batch; b += 32) { p.sums[PA_SUMS + b] = tiles_before[b]; p.sums[PA_SUMS + 1 + p.a.batch + b] = items_before[b]; }
     }
     if (lane == 0) {
-      const int cta = on_prompt ? blockIdx.x : blockIdx.x - deal.prompt_ctas, per = on_prompt ? deal.per_prompt : deal.per;
-      const int work = on_prompt ? p.prefix_work : deal.own_work;
-      const int lo = (int)min((long long)cta * per, (long long)work), hi = (int)min((long long)(cta + 1) * per, (long long)work);
       Walk walk(p, tiles_before, items_before, on_prompt, lo, hi);
+      if (!on_prompt && lo < hi) walk.place(s_first, s_request);
       Segment g;
       bool more = true;
       while (more) {
@@ -565,72 +585,90 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
     }
   } else if (warp == 12) {
-    // ---------------------------------------------------------------- products
+    // ---------------------------------------------------------------- products: the next scores or the next P V, whichever has what it needs
     constexpr uint32_t idesc_qk = umma_idesc_bf16(PA_M, PA_N, 0, 0), idesc_pv = umma_idesc_bf16(PA_M, HD, 0, 1);
     const uint64_t q_desc = umma_smem_desc_sw128(smem_u32(smem + Cfg::OFF_Q), 16, 1024), k_desc = umma_smem_desc_sw128(smem_u32(smem + Cfg::OFF_K), 16, 1024);
     const uint64_t v_desc = umma_smem_desc_sw128(smem_u32(smem + Cfg::OFF_V), PA_N * 128, 1024);
-    int ja = 0, na = 0, sqa = -1, ga = 0, la = 0;                 // of the score products, two tiles ahead
-    uint32_t laphase = 0;
-    const auto issue_qk = [&]() -> bool {                         // the next score product, if there is one
-      if (ja == na) {
-        if (!warp_wait(&listed[la], laphase)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
-        const int n = list[la].tiles;
-        if (n == 0) return true;
-        if (++la == PA_LIST) { la = 0; laphase ^= 1; }
-        ja = 0; na = n; ++sqa;
-        if (!warp_wait(&q_full[sqa & 1], (sqa >> 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
-      }
-      const int st = ga % NK;
-      if (!warp_wait(&k_full[st], (ga / NK) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t qd = q_desc + ((sqa & 1) * Cfg::Q_BYTES >> 4), kd = k_desc + (st * Cfg::T_BYTES >> 4);
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
-          const uint32_t off = ((ks >> 2) * (PA_M * 128) + (ks & 3) * 32) >> 4;
-          umma_f16(tmem_base + Cfg::TM_S + (ga & 1) * PA_N, qd + off, kd + off, idesc_qk, ks > 0 ? 1u : 0u);
+    const auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar, parity)); };
+    int gq = 0, jq = 0, nq = 0, sqq = -1, lq = 0;                 // of the score products: tile, tile in the segment, its tiles, segment, list entry
+    uint32_t lqphase = 0;
+    bool q_there = false, q_end = false;
+    int g = 0, sq = 0, j = 0, n = 0;                              // of P V
+    bool o_there = false;
+    uint64_t since = 0;
+    uint32_t idle = 0;
+    for (;;) {
+      bool moved = false;
+      // scores, over P of the tile before the last: behind its product in the pipe
+      if (!q_end && gq < g + 2) {
+        if (jq == nq && ready(&listed[lq], lqphase)) {
+          nq = list[lq].tiles;
+          jq = 0;
+          q_there = false;
+          q_end = nq == 0;
+          if (!q_end) { ++sqq; if (++lq == PA_LIST) { lq = 0; lqphase ^= 1; } }
+          moved = true;
         }
-        umma_commit(&k_empty[st]);
-        umma_commit(&s_full[ga & 1]);
-        if (ja + 1 == na) umma_commit(&q_empty[sqa & 1]);
+        if (jq < nq) {
+          const int st = gq % NK;
+          if (!q_there) q_there = ready(&q_full[sqq & 1], (sqq >> 1) & 1);
+          if (q_there && ready(&k_full[st], (gq / NK) & 1)) {
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t qd = q_desc + ((sqq & 1) * Cfg::Q_BYTES >> 4), kd = k_desc + (st * Cfg::T_BYTES >> 4);
+#pragma unroll
+              for (int ks = 0; ks < HD / 16; ++ks) {
+                const uint32_t off = ((ks >> 2) * (PA_M * 128) + (ks & 3) * 32) >> 4;
+                umma_f16(tmem_base + Cfg::TM_S + (gq & 1) * PA_N, qd + off, kd + off, idesc_qk, ks > 0 ? 1u : 0u);
+              }
+              umma_commit(&k_empty[st]);
+              umma_commit(&s_full[gq & 1]);
+              if (jq + 1 == nq) umma_commit(&q_empty[sqq & 1]);
+            }
+            __syncwarp();
+            ++jq; ++gq;
+            moved = true;
+          }
+        }
       }
-      __syncwarp();
-      ++ja; ++ga;
-      return true;
-    };
-    int g = -2, sq = 0, j = 0, n = 0;                             // g: the tile whose values come next, behind two score products
-#pragma unroll 1
-    while (ok) {
-      if (g >= 0) {
-        if (j == n) {
-          if (!take(s, ok)) break;
+      if (g < gq || (q_end && j == n)) {
+        if (j == n) {                                             // the segment of the next product
+          if (g == gq) break;                                     // there is none
+          if (!take(s, ok)) break;                                // listed already
           let_go();
           n = s.tiles;
           j = 0;
-          ok = warp_wait(&o_free[sq & 1], ((sq >> 1) & 1) ^ 1);   // the result before the last has been read
-          if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); break; }
+          o_there = false;
         }
         const int st = g % NV;
-        ok = warp_wait(&v_full[st], (g / NV) & 1);
-        if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
-        ok = warp_wait(&p_full[g & 1], (g >> 1) & 1);
-        if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); break; }
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t vd = v_desc + (st * Cfg::T_BYTES >> 4);
+        if (!o_there) o_there = ready(&o_free[sq & 1], ((sq >> 1) & 1) ^ 1);      // the result before the last has been read
+        if (o_there && ready(&p_full[g & 1], (g >> 1) & 1) && ready(&v_full[st], (g / NV) & 1)) {
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t vd = v_desc + (st * Cfg::T_BYTES >> 4);
 #pragma unroll
-          for (int ks = 0; ks < PA_N / 16; ++ks)
-            umma_f16_ts(tmem_base + Cfg::TM_O + (sq & 1) * HD, tmem_base + Cfg::TM_S + (g & 1) * PA_N + ks * 8, vd + (ks * 2048 >> 4), idesc_pv,
-                        (j > 0 || ks > 0) ? 1u : 0u);
-          umma_commit(&v_empty[st]);
-          umma_commit(&o_done[g & 1]);
-          if (j + 1 == n) umma_commit(&o_full[sq & 1]);
+            for (int ks = 0; ks < PA_N / 16; ++ks)
+              umma_f16_ts(tmem_base + Cfg::TM_O + (sq & 1) * HD, tmem_base + Cfg::TM_S + (g & 1) * PA_N + ks * 8, vd + (ks * 2048 >> 4), idesc_pv,
+                          (j > 0 || ks > 0) ? 1u : 0u);
+            umma_commit(&v_empty[st]);
+            umma_commit(&o_done[g & 1]);
+            if (j + 1 == n) umma_commit(&o_full[sq & 1]);
+          }
+          __syncwarp();
+          ++g;
+          if (++j == n) ++sq;
+          moved = true;
         }
-        __syncwarp();
-        if (++j == n) ++sq;
       }
-      ok = issue_qk();                                            // over S[g & 1] = P_g: behind its product in the pipe
-      ++g;
+      if (moved) { idle = 0; since = 0; continue; }
+      if (g < gq) mbar_nap(&p_full[g & 1], (g >> 1) & 1, 64);
+      else if (jq < nq) mbar_nap(&k_full[gq % NK], (gq / NK) & 1, 64);
+      else mbar_nap(&listed[lq], lqphase, 64);
+      if ((++idle & 0xff) == 0) {                                 // bounded like every wait: by wall time
+        const uint64_t now = global_timer_ns();
+        if (since == 0) since = now;
+        else if (__any_sync(0xffffffffu, now - since > OA_WAIT_LIMIT_NS)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); break; }
+      }
     }
   } else if (warp < 8) {
     // ---------------------------------------------------------------- softmax: warp w has TMEM lanes 32 (w % 4).. and the keys of half w / 4 of a tile
@@ -954,38 +992,45 @@ struct RowJoin {
   }
 };
 
-// Shared form: every row from the pieces of its prompt item and of its own item.
+// Shared form: every row from the pieces of its prompt item and of its own item.  Block (b, y) has rows 8 y .. of request b, a warp to each, so that
+// all it has to know of the request arrives at once; blocks of b = batch the rows of no request, zeros.
 template <int HD>
 __global__ void __launch_bounds__(256) paged_join_rows_kernel(const __grid_constant__ PagedTcParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= (long long)p.a.tokens * p.a.q_heads) return;
-  const int t = (int)(row / p.a.q_heads), hq = (int)(row - (long long)t * p.a.q_heads), h = hq / p.group, head = hq - h * p.group;
-  const int per_prompt = p.sums[1], per = p.sums[2];
-  RowJoin<HD> join;
-  int b = 0, i = 0;
-  if (find_request(p.a.starts, p.a.batch, t, lane, b, i) && i < p.a.max_fresh) {
-    const int prt = t / p.tpt, p_item = h * p.prefix_row_tiles + prt, pa = p_item * p.prefix_tiles;
-    const int p_first = pa / per_prompt, p_count = (pa + p.prefix_tiles - 1) / per_prompt - p_first + 1;
-    const Request r = request_of(p, b);
-    const int rt = i / p.tpt, tiles = tiles_of(p, r, rt);
-    int first = 0, count = 0, item = 0;
-    if (tiles > 0) {
-      const int before = p.sums[PA_SUMS + b], all = p.sums[PA_SUMS + b + 1] - before;
-      int a = before * p.a.kv_heads + h * all;
-      for (int k = 0; k < rt; ++k) a += tiles_of(p, r, k);
-      item = p.sums[PA_SUMS + 1 + p.a.batch + b] * p.a.kv_heads + h * r.row_tiles + rt;
-      first = a / per;
-      count = (a + tiles - 1) / per - first + 1;
-    }
-    join.add(p, p_count + count, [&](int k) -> long long {
-      return k < p_count ? prompt_row(p, (long long)p_item + p_first + k) + (t - prt * p.tpt) * p.group + head
-                         : own_row(p, (long long)item + first + k - p_count) + (i - rt * p.tpt) * p.group + head;
-    }, lane);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x;
+  if (b == p.a.batch) {
+    const int t0 = p.a.starts[0], t1 = p.a.starts[p.a.batch];
+    for (int t = blockIdx.y * 8 + warp; t < p.a.tokens; t += gridDim.y * 8)
+      if (t < t0 || t >= t1)
+        for (int hq = 0; hq < p.a.q_heads; ++hq) RowJoin<HD>().write(p, t, hq, lane);
+    return;
   }
-  join.write(p, t, hq, lane);
+  const int per_prompt = p.sums[1], per = p.sums[2], before = p.sums[PA_SUMS + b], all = p.sums[PA_SUMS + b + 1] - before;
+  const int items = p.sums[PA_SUMS + 1 + p.a.batch + b];
+  const Request r = request_of(p, b);
+  for (int w = blockIdx.y * 8 + warp; w < r.n * p.a.q_heads; w += gridDim.y * 8) {
+    const int i = w / p.a.q_heads, hq = w - i * p.a.q_heads, t = r.t0 + i, h = hq / p.group, head = hq - h * p.group;
+    if (t < 0 || t >= p.a.tokens) continue;
+    RowJoin<HD> join;
+    if (i < r.fresh) {
+      const int prt = t / p.tpt, p_item = h * p.prefix_row_tiles + prt, pa = p_item * p.prefix_tiles;
+      const int p_first = pa / per_prompt, p_count = (pa + p.prefix_tiles - 1) / per_prompt - p_first + 1;
+      const int rt = i / p.tpt, tiles = tiles_of(p, r, rt), item = items * p.a.kv_heads + h * r.row_tiles + rt;
+      int first = 0, count = 0;
+      if (tiles > 0) {
+        int a = before * p.a.kv_heads + h * all;
+        for (int k = 0; k < rt; ++k) a += tiles_of(p, r, k);
+        first = a / per;
+        count = (a + tiles - 1) / per - first + 1;
+      }
+      join.add(p, p_count + count, [&](int k) -> long long {
+        return k < p_count ? prompt_row(p, (long long)p_item + p_first + k) + (t - prt * p.tpt) * p.group + head
+                           : own_row(p, (long long)item + first + k - p_count) + (i - rt * p.tpt) * p.group + head;
+      }, lane);
+    }
+    join.write(p, t, hq, lane);
+  }
 }
 
 // Joint form: the items that a stretch's end cuts (block c: the one that begins in stretch c and goes beyond it), and zeros for the rows of
@@ -1115,7 +1160,10 @@ static int launch_tc(const PagedAttnParams& a, void* scratch, int* status, cudaS
   if ((rc = make_tmap_box3_bf16(&tk, a.k, dims, ks, box)) || (rc = make_tmap_box3_bf16(&tv, a.v, dims, vs, box))) return rc;
   launch_short(paged_attn_tc_kernel<HD>, dim3((unsigned)c.grid), dim3(PA_THREADS), Cfg::SMEM_BYTES, st, tq, tqo, tk, tv, p);
   if (c.joint) launch_short(paged_join_cuts_kernel<HD>, dim3((unsigned)c.grid), dim3(256), 0, st, p);
-  else launch_short(paged_join_rows_kernel<HD>, dim3((unsigned)(((long long)a.tokens * a.q_heads + 7) / 8)), dim3(256), 0, st, p);
+  else {
+    const long long rows = (long long)(a.max_fresh > 0 ? a.max_fresh : 1) * a.q_heads;           // of a request, at most
+    launch_short(paged_join_rows_kernel<HD>, dim3((unsigned)a.batch + 1, (unsigned)(rows < 8 * 1024 ? (rows + 7) / 8 : 1024)), dim3(256), 0, st, p);
+  }
   return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }
 

@@ -133,55 +133,79 @@ __global__ void __launch_bounds__(128) paged_attn_rows_kernel(const PagedAttnPar
 
 
 // ------------------------------------------------------------------------------------------------ bf16 on the tensor cores
-// A tile of queries is up to 128 rows, the group of query heads that share a key-value head times `tpt` tokens (row = token * group +
-// head), and a tile of keys is 128 keys, one to eight pages.  An item is the work of one query tile on one key-value head:
+// A query tile is the group of query heads that share a key-value head times tokens, row = token * group + head.  An item is the work of one
+// query tile on one key-value head:
 //   shared form   the prompt is read once for the whole batch: its items take tokens of the batch as they come, whatever request they
 //                 belong to, and each request's own keys make items of their own; every row then has two partial results or more;
-//   joint form    where a request's new tokens fill a tile themselves (or there is no prompt) an item sees the prompt's keys and then its own.
-// The key tiles of all items, one after the other, are cut into as many equal stretches as there are CTAs for them (in the shared form some
-// CTAs have the prompt's items and the others the requests'), so that a long prompt for few requests and short histories for many fill the chip
-// alike.  The part of an item in one stretch is a segment.  Segments that are not a whole result leave (o, m, l) in fp32 in scratch, and a
-// second launch joins them.  Where everything goes follows from prefix sums over the batch that each CTA makes for itself; CTA 0 leaves them
-// for the second launch.
+//   joint form    where a request's new tokens fill a tile themselves an item sees the prompt's keys and then its own.
+// The key tiles of all items, one after the other, are cut into equal stretches, so that a long prompt for few requests and short histories
+// for many fill the chip alike.  The part of an item in one stretch is a segment.  Segments that are not a whole result leave (o, m, l) in fp32
+// in scratch, and a second launch joins them.  Where everything goes follows from prefix sums over the batch that each CTA makes for
+// itself; CTA 0 leaves them for the second launch.
 //
-// Inside a CTA, warp 15 works out the segments, one after the other, and leaves them in a list of eight in shared memory (every warp on
-// its own needed so much code that the warps waited for instructions: 32 requests behind 2048 tokens 59 us).  They run through one pipeline of tiles,
-// g = 0, 1, ..:  warps 13 and 14 load Q (two buffers) and K, and V, by TMA, a box for each page;  warp 12 issues S[g & 1] = Q K_g^T two tiles ahead of O[segment & 1] += P_g V_g, P taken from TMEM;  warps 0-7 are the
-// softmax, two threads to a row;  warps 8-11 write a segment's result out while the next one runs.
-//
-// Few rows: a warp reaches only its own quarter of the TMEM lanes, and the two warps of a quarter share a scheduler, so that 32 rows alone
-// would take as long as 128 (0.9 us a tile, where the products need 0.55).  Up to 32 rows therefore lie in the tile four times, and copy c
-// takes a quarter of a tile's keys, its other weights being zeros; the copies' results are joined on the way out.
+// There are two kinds of CTAs.
+//   Many rows (a tile of up to 128, tiles of 128 keys, a stretch to a CTA): tcgen05 with scores, weights and results in TMEM, below.
+//   Few rows (up to 8 or 16, the single tokens of decoding above all; tiles of 16 or 32 keys): what counts is that bytes arrive.  A CTA's
+//   stretch is dealt to eight warps, each with a ring of three tiles that a warp beside it fills by TMA, one box to a page; no warp waits for
+//   another until they join what they have in shared memory.  Scores are K Q^T on mma.sync, keys along M and up to eight rows along N, so
+//   that a row is an eighth of an instruction and not 1/128 of a tile, and stay in registers: their exponentials turn into an operand of
+//   V^T P^T by a transpose among lanes.  128 requests behind 8191 shared keys with 1024 of their own on average, 8 key-value heads of 64, group 8:
+//   own keys arrive at 95 bytes a nanosecond and SM where 72 SMs take them, which is what the memory gives; a tcgen05 tile with 8 of its 128 rows
+//   alive took 3300 instructions and 0.75 us for 128 keys (46 GB/s and SM), and the call 101 us where it now takes 79.
+//   More than 16 rows would need more registers than a thread has.
 //
 // Keys beyond a length are cut off from the scores by a select, and their values are overwritten by zeros before the product: what lies there
 // (the rest of a page, or of the ring) may be anything, NaN included.
-// The product P_g V_g has a barrier for even and one for odd tiles: the scores of tile g + 1 do not wait for it, so that a reader may be two
-// products ahead of one barrier's phase.
+//
+// Many rows.  Warp 15 works out the segments, one after the other, and leaves them in a list of eight in shared memory (every warp on its
+// own needed so much code that the warps waited for instructions).  They run through one pipeline of tiles, g = 0, 1, ..:  warps 13 and 14
+// load Q (two buffers) and K, and V, by TMA, a box for each page;  warp 12 issues S[g & 1] = Q K_g^T two tiles ahead, and O += P_g V_g, P[g & 1] taken from
+// TMEM;  warps 0-3 are the softmax of even tiles, warps 4-7 of odd ones, a thread to a row: the exponentials of one tile run beside the
+// waits of the other.  A row's maximum in use goes from tile to tile through shared memory, ahead of the exponentials, so that both sides
+// share O;  warps 8-11 write a segment's result out while the next one runs.  The product P_g V_g has a barrier for even and one for odd
+// tiles, so that no reader is more than one phase behind.  A tile of 128 x 128 takes 1850 cycles (two threads to a row, all eight warps in the same
+// tile: 2000 and more): each side needs 3500 of them, 1730 for the exponentials, of which the special-function units are busy for 900; the rest are
+// round trips to barriers and TMEM (200 each) that two warps to a scheduler do not hide.
 constexpr int PA_M = 128, PA_N = 128, PA_THREADS = 512, PA_MAX_BATCH = 1024, PA_LIST = 8;
+constexpr int PF_WARPS = 8, PF_STAGES = 3, PF_STAGE_BYTES = 8192, PF_KEPT_BYTES = 664;    // few rows: warps, tiles in a warp's ring, K and V of a tile
+template <int HD> constexpr int PF_KEYS_LOG2 = HD == 64 ? 5 : 4;       // keys of such a tile
+constexpr int PF_ROWS = 16;                                             // and the most rows: what a thread's registers hold
 constexpr float PA_RESCALE = 8.f;          // log2: the running maximum is let be while rows grow by less
 
 template <int HD> struct PaCfg {
   static constexpr int NK = HD == 64 ? 4 : 2, NV = HD == 64 ? 4 : 2;
   static constexpr int Q_BYTES = PA_M * HD * 2, T_BYTES = PA_N * HD * 2;
   static constexpr int OFF_Q = 0, OFF_K = 2 * Q_BYTES, OFF_V = OFF_K + NK * T_BYTES;
-  static constexpr int OFF_X = OFF_V + NV * T_BYTES;             // float[2 parities][2 halves][128]: maxima of a tile's halves
-  static constexpr int OFF_ML = OFF_X + 2 * 2 * PA_M * 4;        // float[2 segments][3][128]: m, and l of either half
-  static constexpr int OFF_STAGE = OFF_ML + 2 * 3 * PA_M * 4;    // float[128][36] (or [32][HD + 8]): results of copies on the way out
-  static constexpr int OFF_BAR = OFF_STAGE + PA_M * 36 * 4, OFF_LIST = OFF_BAR + 512, OFF_SCAN = OFF_LIST + PA_LIST * 48;
-  static constexpr int SMEM_BYTES = OFF_SCAN + 2 * (PA_MAX_BATCH + 1) * 4;
-  static constexpr int TM_S = 0, TM_O = 256;
+  static constexpr int OFF_X = PF_WARPS * PF_STAGES * PF_STAGE_BYTES;         // float[2 parities][128]: maxima in use
+  static constexpr int OFF_ML = OFF_X + 2 * PA_M * 4;            // float[2 segments][even, odd][m, l][128]
+  static constexpr int OFF_BAR = OFF_ML + 2 * 2 * 2 * PA_M * 4, OFF_LIST = OFF_BAR + 512, OFF_SCAN = OFF_LIST + PA_LIST * 48;
+  static constexpr int OFF_FEW = OFF_SCAN + 2 * (PA_MAX_BATCH + 1) * 4;        // FewWarp[8]
+  static constexpr int SMEM_BYTES = OFF_FEW + PF_WARPS * PF_KEPT_BYTES;
+  static_assert(OFF_V + NV * T_BYTES <= OFF_X, "both kinds' rings");
+  static constexpr int TM_S = 0, TM_P = 256, TM_O = 384, SETS = HD == 64 ? 2 : 1;      // S and P of two tiles, O of so many segments
+};
+
+// Where a token's partial results over its own keys are (shared form): those of key-value head h begin at tile pos + h * all, in item + h * row_tiles.
+struct __align__(16) PagedOwn {
+  int pos, all, tiles, item, row_tiles;
+  int inner;                               // the token in its tile; -1: of no request, or beyond those that one may have
+  int pad[2];
 };
 
 struct PagedTcParams {
   PagedAttnParams a;
   int group, group_mul, tpt;               // query heads to a key-value head (and 65536 / group + 1: see token_of), tokens in a tile
   int ts, tb;                              // tokens in a box of an own item, of a prompt's item
-  int copies, copies_prompt;
+  int few, few_prompt;                     // few rows: 8 or 16, the most of an item; or 0
+  int many;                                // some CTA has a tile of more rows
+  int own_log2;                            // keys of a tile of a request's own
   int joint, prefix_tiles, prefix_row_tiles, prefix_work;   // prefix_work: key tiles of all prompt items (shared form)
   float* part;                             // partial o: [prompt slots][tb * group][HD], then [own slots][ts * group][HD]
   float2* ml;                              // their (m, l), m in units of log2
   int* sums;                               // Stretches, tiles before a request [batch + 1], query tiles before a request [batch + 1]
+  PagedOwn* owns;                          // [tokens], shared form
   long long own_slot0, part_rows;          // rows of the prompt's slots, rows in all
+  int ctas;                                // of the first launch: no row has more pieces of one kind
   int* status;
 };
 constexpr int PA_SUMS = 4;                 // ints in front of the prefix sums
@@ -207,7 +231,7 @@ __device__ __forceinline__ int seen_by(const PagedTcParams& p, const Request& r,
 }
 // key tiles of the item: with none at all an item of the joint form takes an empty one, which gives the rows their zeros
 __device__ __forceinline__ int tiles_of(const PagedTcParams& p, const Request& r, int rt) {
-  const int own = (seen_by(p, r, rt) + PA_N - 1) / PA_N;
+  const int own = (seen_by(p, r, rt) + (1 << p.own_log2) - 1) >> p.own_log2;
   return p.joint ? max(p.prefix_tiles + own, 1) : own;
 }
 
@@ -218,22 +242,24 @@ struct Segment {
   int t0, tokens, n, own, seen, i0;        // first token and how many; own items: see Request, i0 = index of the first token in the request
 };
 
-// How the tiles are dealt: CTAs [0, prompt_ctas) have stretches of `per_prompt` of the prompt's, the others of `per` of the requests'.  With
-// both there, in proportion to what they cost: tiles and items of a request's own, tiles of the prompt's by the rows in them.
-// Relative: a full tile waits for its exponentials, one of few rows for its products or its bytes, and an item for its first bytes.
-constexpr float PA_COST_FULL = 1.f, PA_COST_FEW = 0.6f, PA_COST_ITEM = 0.3f;
+// How the tiles are dealt: CTAs [0, prompt_ctas) have stretches of `per_prompt` of the prompt's, the others of `per` of the requests'
+// each.  With both there, in proportion to what they cost, relative to a tile of 128 keys and many rows: 128 keys of few rows, which wait for memory, and
+// what comes with an item (0.2 and 0.45 for the first, 0.1 and 0.2 for the second: up to 15% slower at 32 to 128 requests).
+constexpr float PA_COST_FEW = 0.35f, PA_COST_ITEM = 0.4f;
 struct Stretches { int prompt_ctas, per_prompt, per, own_work; };
+template <int HD>
 __device__ __forceinline__ Stretches stretches_of(const PagedTcParams& p, int own_work, int own_items, int ctas) {
   Stretches d;
   d.own_work = own_work;
   d.prompt_ctas = 0;
+  const float few = PA_COST_FEW * (1 << PF_KEYS_LOG2<HD>) / PA_N;      // of a tile of few rows
   if (p.prefix_work > 0) {
-    const float prompt = (float)p.prefix_work * (p.copies_prompt == 1 ? PA_COST_FULL : PA_COST_FEW);
-    const float own = (float)own_work * (p.copies == 1 ? PA_COST_FULL : PA_COST_FEW) + (float)own_items * PA_COST_ITEM;
+    const float prompt = (float)p.prefix_work * (p.few_prompt ? few : 1.f);
+    const float own = (float)own_work * (p.few ? few : 1.f) + (float)own_items * PA_COST_ITEM;
     d.prompt_ctas = own_work > 0 ? min(max((int)((float)ctas * prompt / (prompt + own) + 0.5f), 1), ctas - 1) : ctas;
   }
   d.per_prompt = max((p.prefix_work + max(d.prompt_ctas, 1) - 1) / max(d.prompt_ctas, 1), 1);
-  d.per = max((own_work + max(ctas - d.prompt_ctas, 1) - 1) / max(ctas - d.prompt_ctas, 1), 1);
+  d.per = max((own_work + ctas - d.prompt_ctas - 1) / max(ctas - d.prompt_ctas, 1), 1);
   return d;
 }
 
@@ -378,62 +404,359 @@ __device__ __forceinline__ void scan_batch(const PagedTcParams& p, int* tiles_be
   all_items = all_i;
 }
 
-// Where a partial result goes.  Shared form: every segment of every item, numbered by item + CTA (a segment begins where an item or a
+// Where a partial result goes.  Shared form: every segment of every item, numbered by item + stretch (a segment begins where an item or a
 // stretch does).  Joint form: only items that a stretch's end cuts, of which a CTA has its first and its last segment.
 __device__ __forceinline__ long long own_row(const PagedTcParams& p, long long slot) { return p.own_slot0 + slot * (p.ts * p.group); }
 __device__ __forceinline__ long long prompt_row(const PagedTcParams& p, long long slot) { return slot * (p.tb * p.group); }
 // Starts that do not rise would make more items than there is room for: their rows stay out of the scratch.
 __device__ __forceinline__ bool has_room(const PagedTcParams& p, long long row) { return row >= 0 && row < p.part_rows; }
 
-// Whether the phase is complete, without waiting for it.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{\n\t.reg .pred P;\n\tmbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\tselp.b32 %0, 1, 0, P;\n\t}\n" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-  return ok != 0;
+// ---- few rows
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// Out of the way until the phase completes, for at most about `ns`: a loop over several barriers that only tests them takes issue slots from
-// the warps beside it.
-__device__ __forceinline__ void mbar_nap(uint64_t* bar, uint32_t parity, uint32_t ns) {
-  asm volatile("{\n\t.reg .pred P;\n\tmbarrier.try_wait.parity.shared::cta.b64 P, [%0], %1, %2;\n\t}\n" ::"r"(smem_u32(bar)), "r"(parity), "r"(ns) : "memory");
+__device__ __forceinline__ void ldmatrix_x4_t(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void softmax_pair_sync(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
-__device__ __forceinline__ void out_sync() { asm volatile("bar.sync 5, 128;" ::: "memory"); }
-// Lanes 0-15 of the quarter, 64 columns: lane l of the warp receives columns 8 k + 2 (l % 4) and the next of row l / 4 in r[4 k], r[4 k + 1], of
-// row 8 + l / 4 in r[4 k + 2], r[4 k + 3].
-__device__ __forceinline__ void tmem_ld_16x256b_x8(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {      // an 8 x 8 matrix of 16 bits, a row to four lanes
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
-               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
+__device__ __forceinline__ void mma_16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// What a warp keeps in shared memory beside its ring.
+struct FewSegment { int tile, tiles, item, h, t0, rows, seen, shift; };          // shift: the row of token i sees own keys before shift + i
+struct FewPart { int rows, goes_on, at; float2 ml[PF_ROWS]; };                   // rows 0: none; `at`: where its o lies in the ring
+struct FewWarp {
+  uint64_t full[PF_STAGES], empty[PF_STAGES], listed[8];
+  FewSegment list[8];                      // of which the warp is in one, and its loads at most five ahead: none is written before it has been read
+  FewPart front, back;                     // what is to be joined with the warp before, and with the warp behind
+  int item;                                // of `back`
+  int pad;
+};
+static_assert(sizeof(FewWarp) == PF_KEPT_BYTES, "what is set aside for it");
+
+__device__ __forceinline__ int few_step(int x, int hole) {        // the next slot of a ring
+  x = x + 1 == PF_STAGES ? 0 : x + 1;
+  if (x == hole) x = x + 1 == PF_STAGES ? 0 : x + 1;
+  return x;
+}
+// The loads of warp `warp`, by a warp beside it: chunks of up to 32 pages of a segment, the pages of the next chunk looked up while this one's
+// tiles are loaded.
+template <int HD>
+__device__ __forceinline__ void few_loads(const PagedTcParams& p, const CUtensorMap* tmK, const CUtensorMap* tmV, uint8_t* ring, FewWarp& mine, int warp,
+                                          const int* tiles_before, const int* items_before, bool prompt, int lo, int hi) {
+  constexpr int UL = PF_KEYS_LOG2<HD>, U = 1 << UL, CHUNKS = HD / 64, KV = U * HD * 2;
+  const int lane = threadIdx.x & 31;
+  const int lg = p.a.page_log2, box = min(1 << lg, U), boxes_log2 = max(UL - lg, 0);         // rows of a box; boxes of a tile
+  const int part = (hi - lo + PF_WARPS - 1) / PF_WARPS, from = min(lo + warp * part, hi), to = min(from + part, hi);
+  struct Chunk { int n, k0, end, h, id; };
+  Walk walk(p, tiles_before, items_before, prompt, from, to);
+  Chunk now{0, 0, 0, 0, 0}, then{0, 0, 0, 0, 0};
+  int seg_h = 0, seg_b = 0, seg_tile = 0, seg_left = 0, seg_end = 0, seg_at = 0, used = 0, st = 0, hole = -1;
+  int keeps = 0;                           // the tile whose slot the warp keeps, counted from 1; 0: none
+  const auto fetch = [&](Chunk& c) {
+    c.n = 0;
+    if (seg_left == 0) {
+      Segment s;
+      if (!walk.next(s)) return;
+      if (lane == 0) {
+        mine.list[seg_at & 7] = FewSegment{s.tile, s.tiles, s.item, s.h, s.t0, s.tokens * p.group, s.seen, s.own - s.n + s.i0 + 1};
+        mbar_arrive(&mine.listed[seg_at & 7]);
+      }
+      if (seg_at == 0 && s.tile > 0 && from > lo && walk.pos < to) keeps = s.tiles;
+      ++seg_at;
+      seg_h = s.h; seg_b = s.b; seg_tile = s.tile; seg_left = s.tiles;
+      seg_end = prompt ? p.a.prefix_len : s.seen;
+      const int t = s.t0 + lane / (p.group * CHUNKS), off = lane % (p.group * CHUNKS) * 64;           // its queries on their way to L2
+      if (lane < s.tokens * p.group * CHUNKS && t >= 0 && t < p.a.tokens)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const __nv_bfloat16*>(p.a.q) + (long long)t * p.a.q_stride + s.h * p.group * HD + off));
+    }
+    c.n = min(seg_left, 32 >> boxes_log2);
+    c.k0 = seg_tile << UL;
+    c.end = seg_end;
+    c.h = seg_h;
+    c.id = -1;
+    if (lane * box < min(c.n << UL, c.end - c.k0)) {
+      const int at = (c.k0 + lane * box) >> lg;
+      c.id = prompt ? p.a.prefix_table[at] : p.a.tables[seg_b * p.a.table_stride + at];
+    }
+    seg_tile += c.n;
+    seg_left -= c.n;
+  };
+  fetch(now);
+  if (now.n > 0) fetch(then);
+  uint32_t phases = (1u << PF_STAGES) - 1;                       // a bit for each slot: free at first
+#pragma unroll 1
+  while (now.n > 0) {
+    const int boxes = (min(U, now.end - now.k0) + box - 1) / box, id = __shfl_sync(0xffffffffu, now.id, (used << boxes_log2) + lane);
+    if (!warp_wait(&mine.empty[st], phases >> st & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); return; }
+    phases ^= 1u << st;
+    if (lane == 0) mbar_expect_tx(&mine.full[st], (uint32_t)(boxes * box * HD * 4));
+    __syncwarp();
+    if (lane < boxes) {
+      uint8_t* at = ring + st * PF_STAGE_BYTES + lane * box * 128;
+      const int y = (now.h << lg) + ((now.k0 + lane * box) & ((1 << lg) - 1));
+#pragma unroll
+      for (int x = 0; x < CHUNKS; ++x) {
+        tma_load_3d(at + x * (U * 128), tmK, &mine.full[st], x * 64, y, id);
+        tma_load_3d(at + KV + x * (U * 128), tmV, &mine.full[st], x * 64, y, id);
+      }
+    }
+    __syncwarp();
+    if (--keeps == 0) hole = st;
+    st = few_step(st, hole);
+    now.k0 += U;
+    ++used;
+    if (--now.n == 0) {
+      now = then;
+      used = 0;
+      if (now.n > 0) fetch(then);
+    }
+  }
+}
+
+// Warp `warp` of eight, NT groups of eight rows.  The CTA's stretch [lo, hi) is cut into a warp's parts.
+template <int HD, int NT>
+__device__ __forceinline__ void few_rows(const PagedTcParams& p, uint8_t* rings, FewWarp* all, bool prompt, int cta, int lo, int hi) {
+  constexpr int UL = PF_KEYS_LOG2<HD>, U = 1 << UL, MT = U / 16, KC = HD / 16, KV = U * HD * 2, PER = HD / 32;
+  static_assert(2 * KV == PF_STAGE_BYTES && NT * 8 * HD * 4 <= PF_STAGE_BYTES, "a tile of K and of V, or results");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, pair = (lane & 3) * 2;
+  const float sl2 = p.a.scale * 1.4426950408889634f;
+  uint8_t* ring = rings + warp * (PF_STAGES * PF_STAGE_BYTES);
+  FewWarp& mine = all[warp];
+  const int part = (hi - lo + PF_WARPS - 1) / PF_WARPS, from = min(lo + warp * part, hi), to = min(from + part, hi);
+  int st = 0, pos = from, sg = 0, hole = -1;
+  uint32_t phases = 0;                     // a bit for each slot
+  bool ok = true;
+  if (lane == 0) mine.front.rows = mine.back.rows = 0;
+#pragma unroll 1
+  while (pos < to && ok) {
+    if (!warp_wait(&mine.listed[sg & 7], sg >> 3 & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+    const FewSegment s = mine.list[sg & 7];
+    ++sg;
+    uint32_t q[KC][NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = n * 8 + quad, i = token_of(p, row), t = s.t0 + i;
+      const bool there = row < s.rows && t >= 0 && t < p.a.tokens;
+      const __nv_bfloat16* at = static_cast<const __nv_bfloat16*>(p.a.q) + (long long)t * p.a.q_stride + (s.h * p.group + row - i * p.group) * HD + pair;
+#pragma unroll
+      for (int k = 0; k < KC; ++k) {
+        q[k][n][0] = there ? *reinterpret_cast<const uint32_t*>(at + k * 16) : 0u;
+        q[k][n][1] = there ? *reinterpret_cast<const uint32_t*>(at + k * 16 + 8) : 0u;
+      }
+    }
+    float o[KC][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; }
+#pragma unroll
+    for (int k = 0; k < KC; ++k)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[k][n][e] = 0.f;
+    const int most = prompt ? p.a.prefix_len : s.seen, least = prompt ? most : min(s.shift, most);
+    const bool front = s.tile > 0 && pos == from && from > lo;                   // begins in a warp before
+    pos += s.tiles;
+#pragma unroll 1
+    for (int j = 0; j < s.tiles; ++j) {
+      const int k0 = (s.tile + j) << UL;
+      if (!warp_wait(&mine.full[st], phases >> st & 1)) {
+        if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL);
+        for (int i = 1; i < PF_STAGES; ++i) {                    // copies that may still be under way
+          st = few_step(st, hole);
+          warp_wait(&mine.full[st], phases >> st & 1);
+        }
+        ok = false;
+        break;
+      }
+      phases ^= 1u << st;
+      const uint32_t kt = smem_u32(ring + st * PF_STAGE_BYTES), vt = kt + KV;
+      float c[MT][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[mt][n][e] = 0.f;
+        const int row = mt * 16 + (lane & 15);
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+          uint32_t a[4];
+          ldmatrix_x4(kt + (k >> 2) * (U * 128) + row * 128 + ((((k & 3) * 2 + (lane >> 4)) ^ (row & 7)) << 4), a);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_16816(c[mt][n], a, q[k][n][0], q[k][n][1]);
+        }
+      }
+      if (k0 + U > least) {                // -inf for what is not seen, zeros over values that no key goes with
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int see = prompt ? most : min(s.shift + token_of(p, n * 8 + pair + e), most);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              if (k0 + mt * 16 + quad >= see) c[mt][n][e] = -INFINITY;
+              if (k0 + mt * 16 + quad + 8 >= see) c[mt][n][e + 2] = -INFINITY;
+            }
+          }
+        if (k0 + U > most) {
+          for (int i = lane; i < (k0 + U - most) * (HD / 8); i += 32) {
+            const int key = most - k0 + i / (HD / 8), x = i % (HD / 8);
+            st_shared_v4(vt + (x >> 3) * (U * 128) + key * 128 + (x & 7) * 16, make_uint4(0, 0, 0, 0));
+          }
+          fence_proxy_async_smem();        // before the copy that comes here next
+          __syncwarp();
+        }
+      }
+      // the running maximum is let be while no row of the warp grows by more than 2^8
+      float top[NT][2];
+      bool grow = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float t = fmaxf(c[0][n][e], c[0][n][e + 2]);
+#pragma unroll
+          for (int mt = 1; mt < MT; ++mt) t = fmax3(t, c[mt][n][e], c[mt][n][e + 2]);
+          top[n][e] = t * sl2;
+          grow |= top[n][e] - m[n][e] > PA_RESCALE;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float t = top[n][e];
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+            if (t > m[n][e]) {
+              const float alpha = fast_exp2(m[n][e] - t);        // 0 from -inf
+              m[n][e] = t;
+              l[n][e] *= alpha;
+#pragma unroll
+              for (int k = 0; k < KC; ++k) { o[k][n][e] *= alpha; o[k][n][e + 2] *= alpha; }
+            }
+          }
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t w[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float base = m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1];     // a row that has seen nothing yet
+            c[mt][n][e] = fast_exp2(fmaf(c[mt][n][e], sl2, -base));
+            l[n][e & 1] += c[mt][n][e];
+          }
+          // weights to bf16, as the products take them; their sum stays fp32
+          w[n][0] = transpose8(pack_bf16x2(c[mt][n][0], c[mt][n][1]));
+          w[n][1] = transpose8(pack_bf16x2(c[mt][n][2], c[mt][n][3]));
+        }
+        const int key = mt * 16 + (lane & 7) + (lane >> 4) * 8;
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+          uint32_t a[4];
+          ldmatrix_x4_t(vt + (k >> 2) * (U * 128) + key * 128 + ((((k & 3) * 2 + ((lane >> 3) & 1)) ^ (key & 7)) << 4), a);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_16816(o[k][n], a, w[n][0], w[n][1]);
+        }
+      }
+      __syncwarp();
+      if (j + 1 == s.tiles && front && pos < to) hole = st;      // this slot keeps the results that another warp joins
+      else if (lane == 0) mbar_arrive(&mine.empty[st]);
+      st = few_step(st, hole);
+    }
+    // Results: a segment that ends where another warp goes on waits for it in shared memory, the others go to scratch.
+    const bool back = pos == to && to < hi && s.tile + s.tiles < (prompt ? p.prefix_tiles : (s.seen + U - 1) >> UL);
+    const long long at = prompt ? prompt_row(p, (long long)s.item + cta) : own_row(p, (long long)s.item + cta);
+    FewPart& kept = front ? mine.front : mine.back;
+    const int slot = front ? (hole >= 0 ? hole : 0) : (hole == 0 ? 1 : 0);       // of the ring, in which nothing is under way
+    if ((front || back) && lane == 0) {
+      kept.rows = s.rows;
+      kept.goes_on = back;
+      kept.at = slot * PF_STAGE_BYTES;
+      mine.item = s.item;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = n * 8 + pair + e;
+        float sum = l[n][e];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        if (row < s.rows) {
+          float* to_o;
+          float2* to_ml;
+          if (front || back) { to_o = reinterpret_cast<float*>(ring + slot * PF_STAGE_BYTES) + row * HD; to_ml = &kept.ml[row]; }
+          else { to_o = p.part + (at + row) * HD; to_ml = p.ml + at + row; }
+          if (front || back || has_room(p, at + row)) {
+            if (quad == 0) *to_ml = make_float2(m[n][e], sum);
+#pragma unroll
+            for (int k = 0; k < KC; ++k) { to_o[k * 16 + quad] = o[k][n][e]; to_o[k * 16 + quad + 8] = o[k][n][e + 2]; }
+          }
+        }
+      }
+  }
+  // Joins what the warps have left, a row to a warp, in the order of the keys.
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll 1
+  for (int w = 0; w < PF_WARPS; ++w) {
+    if (all[w].back.rows == 0) continue;
+    const long long at = prompt ? prompt_row(p, (long long)all[w].item + cta) : own_row(p, (long long)all[w].item + cta);
+#pragma unroll 1
+    for (int row = warp; row < all[w].back.rows; row += PF_WARPS) {
+      float m = -INFINITY, l = 0.f, acc[PER] = {};
+#pragma unroll 1
+      for (int x = w; x < PF_WARPS; ++x) {
+        const FewPart& f = x == w ? all[x].back : all[x].front;
+        if (x > w && f.rows == 0) break;
+        const float2 ml = f.ml[row];
+        const float* o = reinterpret_cast<const float*>(rings + x * (PF_STAGES * PF_STAGE_BYTES) + f.at) + row * HD + lane * PER;
+        if (ml.y != 0.f) {                 // otherwise a part of which this row saw nothing
+          const float top = fmaxf(m, ml.x), a = m == -INFINITY ? 0.f : fast_exp2(m - top), b = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top);
+          l = l * a + ml.y * b;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) acc[e] = acc[e] * a + o[e] * b;
+          m = top;
+        }
+        if (x > w && !f.goes_on) break;
+      }
+      if (!has_room(p, at + row)) continue;
+      if (lane == 0) p.ml[at + row] = make_float2(m, l);
+      float* part_o = p.part + (at + row) * HD + lane * PER;
+      if (PER == 4) *reinterpret_cast<float4*>(part_o) = make_float4(acc[0], acc[1], acc[PER - 2], acc[PER - 1]);
+      else *reinterpret_cast<float2*>(part_o) = make_float2(acc[0], acc[1]);
+    }
+  }
 }
 
 template <int HD>
 __global__ void __launch_bounds__(PA_THREADS, 1)
 paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQown, const __grid_constant__ CUtensorMap tmK,
-                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PagedTcParams p) {
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKfew, const __grid_constant__ CUtensorMap tmVfew,
+                     const __grid_constant__ PagedTcParams p) {
   using Cfg = PaCfg<HD>;
   constexpr int NK = Cfg::NK, NV = Cfg::NV, CHUNKS = HD / 64;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int s_warp_sums[2 * PA_THREADS / 32];
-  __shared__ float s_inv[PA_M];
-  __shared__ int s_fail, s_first;
+  __shared__ int s_first;
   __shared__ Request s_request;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
   uint64_t *q_full = bars, *q_empty = bars + 2, *k_full = bars + 4, *k_empty = k_full + NK, *v_full = k_empty + NK, *v_empty = v_full + NV;
-  uint64_t *s_full = v_empty + NV, *p_full = s_full + 2, *o_done = s_full + 4, *o_free = s_full + 6, *seg_done = s_full + 8, *o_full = s_full + 10;
-  uint64_t *listed = s_full + 12, *list_free = listed + PA_LIST;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(list_free + PA_LIST);
+  uint64_t *s_full = v_empty + NV, *p_full = s_full + 2, *o_done = s_full + 4, *o_free = s_full + 6, *seg_done = s_full + 8, *o_full = s_full + 10, *s_free = s_full + 12, *seg_free = s_full + 14;
+  uint64_t *listed = s_full + 16, *list_free = listed + PA_LIST, *m_there = list_free + PA_LIST;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(m_there + 8);
   const Listed* list = reinterpret_cast<const Listed*>(smem + Cfg::OFF_LIST);
   int* tiles_before = reinterpret_cast<int*>(smem + Cfg::OFF_SCAN);
   int* items_before = tiles_before + p.a.batch + 1;
@@ -444,20 +767,28 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     if (threadIdx.x == 0) report_error(p.status, OA_KERR_BAD_ARG);
     return;
   }
-  if (threadIdx.x == 0) {
+  // `many`: some CTA may have many rows
+  if (p.many && threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 8);
-      mbar_init(&o_done[i], 1); mbar_init(&o_full[i], 1); mbar_init(&o_free[i], 4); mbar_init(&seg_done[i], 8);
+      mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1); mbar_init(&o_full[i], 1); mbar_init(&o_free[i], 4); mbar_init(&seg_done[i], 8); mbar_init(&seg_free[i], 4);
     }
     for (int i = 0; i < NK; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
     for (int i = 0; i < NV; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
+    for (int i = 0; i < 8; ++i) mbar_init(&m_there[i], 1);
     for (int i = 0; i < PA_LIST; ++i) { mbar_init(&listed[i], 1); mbar_init(&list_free[i], 15); }
     mbar_fence_init();
-    s_fail = 0;
   }
-  if (warp == 12) { tmem_alloc<512>(tmem_slot); tmem_relinquish(); }
-  if (warp == 13 && lane == 0) { tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmQown); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); }
-  __syncwarp();
+  if (p.many && warp == 12) { tmem_alloc<512>(tmem_slot); tmem_relinquish(); }
+  if (p.many && warp == 13 && lane == 0) { tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmQown); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); }
+  if (warp >= 16 - PF_WARPS && lane == 0 && (p.few || p.few_prompt)) {           // barriers of the few rows' rings
+    FewWarp& f = reinterpret_cast<FewWarp*>(smem + Cfg::OFF_FEW)[warp - (16 - PF_WARPS)];
+    for (int i = 0; i < PF_STAGES; ++i) { mbar_init(&f.full[i], 1); mbar_init(&f.empty[i], 1); }
+    for (int i = 0; i < 8; ++i) mbar_init(&f.listed[i], 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&tmKfew);
+    tma_prefetch_desc(&tmVfew);
+  }
   pdl_wait();
   {                                        // tables on their way to L2 while the lengths arrive: 128 bytes to a thread
     const int lines = (p.a.width + 31) / 32, at = blockIdx.x * PA_THREADS + threadIdx.x;
@@ -467,20 +798,56 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   }
   int own_tiles, own_items;
   scan_batch(p, tiles_before, items_before, s_warp_sums, own_tiles, own_items);
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  const Stretches deal = stretches_of(p, own_tiles * p.a.kv_heads, own_items * p.a.kv_heads, gridDim.x);
+  const Stretches deal = stretches_of<HD>(p, own_tiles * p.a.kv_heads, own_items * p.a.kv_heads, gridDim.x);
   const bool on_prompt = (int)blockIdx.x < deal.prompt_ctas;
   const int cta = on_prompt ? blockIdx.x : blockIdx.x - deal.prompt_ctas, per = on_prompt ? deal.per_prompt : deal.per;
   const int work = on_prompt ? p.prefix_work : deal.own_work;
+  // for the second launch
+  if (blockIdx.x == 0 && threadIdx.x == 0) { p.sums[0] = deal.prompt_ctas; p.sums[1] = deal.per_prompt; p.sums[2] = deal.per; p.sums[3] = deal.own_work; }
+  if (p.joint) {
+    if (blockIdx.x == 0)
+      for (int b = threadIdx.x; b <= p.a.batch; b += PA_THREADS) { p.sums[PA_SUMS + b] = tiles_before[b]; p.sums[PA_SUMS + 1 + p.a.batch + b] = items_before[b]; }
+  } else {
+    const auto none = [&](int from, int to) {                    // tokens of no request
+      for (int t = max(from, 0) + threadIdx.x; t < min(to, p.a.tokens); t += PA_THREADS) p.owns[t].inner = -1;
+    };
+    for (int b = blockIdx.x; b < p.a.batch; b += gridDim.x) {
+      const Request r = request_of(p, b);
+      if (b == 0) none(0, r.t0);
+      if (b == p.a.batch - 1) none(r.t0 + r.n, p.a.tokens);
+      for (int i = threadIdx.x; i < r.n; i += PA_THREADS) {
+        if (r.t0 + i < 0 || r.t0 + i >= p.a.tokens) continue;
+        const int rt = i / p.tpt;
+        PagedOwn o{tiles_before[b] * p.a.kv_heads, tiles_before[b + 1] - tiles_before[b], tiles_of(p, r, rt), items_before[b] * p.a.kv_heads + rt, r.row_tiles,
+                   i < r.fresh ? i - rt * p.tpt : -1, {0, 0}};
+        for (int k = 0; k < rt; ++k) o.pos += tiles_of(p, r, k);
+        p.owns[r.t0 + i] = o;
+      }
+    }
+  }
+  if (const int few = on_prompt ? p.few_prompt : p.few) {
+    if (p.many && warp == 12) tmem_dealloc<512>(*tmem_slot);
+    const int from = (int)min((long long)cta * per, (long long)work), to = (int)min((long long)(cta + 1) * per, (long long)work);
+    FewWarp* all = reinterpret_cast<FewWarp*>(smem + Cfg::OFF_FEW);
+    if (warp >= PF_WARPS) {
+      few_loads<HD>(p, &tmKfew, &tmVfew, smem + (warp - PF_WARPS) * (PF_STAGES * PF_STAGE_BYTES), all[warp - PF_WARPS], warp - PF_WARPS, tiles_before, items_before,
+                    on_prompt, from, to);
+    } else if (few == 8) {
+      few_rows<HD, 1>(p, smem, all, on_prompt, cta, from, to);
+    } else {
+      few_rows<HD, 2>(p, smem, all, on_prompt, cta, from, to);
+    }
+    return;
+  }
   const int lo = (int)min((long long)cta * per, (long long)work), hi = (int)min((long long)(cta + 1) * per, (long long)work);
   if (!on_prompt)                          // the request in which the stretch begins, by the thread that has scanned it
     for (int b = threadIdx.x * ((p.a.batch + PA_THREADS - 1) / PA_THREADS), k = 0; k < (p.a.batch + PA_THREADS - 1) / PA_THREADS && b < p.a.batch; ++k, ++b)
       if (lo >= tiles_before[b] * p.a.kv_heads && lo < tiles_before[b + 1] * p.a.kv_heads) { s_first = b; s_request = request_of(p, b); }
+  tc_fence_before();
   __syncthreads();
-  const int copies = on_prompt ? p.copies_prompt : p.copies, copy_rows = PA_M / copies;     // 1 and 128, or 4 and 32
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
 
   // The next entry of the list.  Every warp reads each once, in order, and lets go of it when it has what it needs.
   int li = 0;
@@ -501,10 +868,6 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
   if (warp == 15) {
     // ---------------------------------------------------------------- segments
-    if (blockIdx.x == 0) {                 // for the second launch
-      if (lane == 0) { p.sums[0] = deal.prompt_ctas; p.sums[1] = deal.per_prompt; p.sums[2] = deal.per; p.sums[3] = deal.own_work; }
-      for (int b = lane; b <= p.a.batch; b += 32) { p.sums[PA_SUMS + b] = tiles_before[b]; p.sums[PA_SUMS + 1 + p.a.batch + b] = items_before[b]; }
-    }
     if (lane == 0) {
       Walk walk(p, tiles_before, items_before, on_prompt, lo, hi);
       if (!on_prompt && lo < hi) walk.place(s_first, s_request);
@@ -551,12 +914,9 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
         if (elect_one()) {
           const CUtensorMap* mq = (s.flags & 1) ? &tmQ : &tmQown;
-          mbar_expect_tx(&q_full[qb], (uint32_t)(copies * ((s.flags & 1) ? p.tb : p.ts) * p.group * HD * 2));
-#pragma unroll 1
-          for (int c = 0; c < copies; ++c)
+          mbar_expect_tx(&q_full[qb], (uint32_t)(((s.flags & 1) ? p.tb : p.ts) * p.group * HD * 2));
 #pragma unroll
-            for (int x = 0; x < CHUNKS; ++x)
-              tma_load_3d(smem + Cfg::OFF_Q + qb * Cfg::Q_BYTES + x * (PA_M * 128) + c * copy_rows * 128, mq, &q_full[qb], x * 64, h * p.group, s.t0);
+          for (int x = 0; x < CHUNKS; ++x) tma_load_3d(smem + Cfg::OFF_Q + qb * Cfg::Q_BYTES + x * (PA_M * 128), mq, &q_full[qb], x * 64, h * p.group, s.t0);
         }
         __syncwarp();
         ++sq;
@@ -585,191 +945,187 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
     }
   } else if (warp == 12) {
-    // ---------------------------------------------------------------- products: the next scores or the next P V, whichever has what it needs
+    // ---------------------------------------------------------------- products, in the order in which the softmax comes to want them: S of g + 2, P V of g
     constexpr uint32_t idesc_qk = umma_idesc_bf16(PA_M, PA_N, 0, 0), idesc_pv = umma_idesc_bf16(PA_M, HD, 0, 1);
     const uint64_t q_desc = umma_smem_desc_sw128(smem_u32(smem + Cfg::OFF_Q), 16, 1024), k_desc = umma_smem_desc_sw128(smem_u32(smem + Cfg::OFF_K), 16, 1024);
     const uint64_t v_desc = umma_smem_desc_sw128(smem_u32(smem + Cfg::OFF_V), PA_N * 128, 1024);
-    const auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar, parity)); };
     int gq = 0, jq = 0, nq = 0, sqq = -1, lq = 0;                 // of the score products: tile, tile in the segment, its tiles, segment, list entry
     uint32_t lqphase = 0;
-    bool q_there = false, q_end = false;
+    bool q_end = false;
+    const auto product_qk = [&] {
+      if (q_end) return;
+      const int st = gq % NK;
+      bool there = true;
+      if (jq == nq) {
+        there = mbar_wait(&listed[lq], lqphase);
+        nq = there ? list[lq].tiles : 0;
+        jq = 0;
+        if (nq == 0) { q_end = true; ok = __all_sync(0xffffffffu, there) && ok; return; }
+        ++sqq;
+        if (++lq == PA_LIST) { lq = 0; lqphase ^= 1; }
+        there = mbar_wait(&q_full[sqq & 1], (sqq >> 1) & 1);
+      }
+      there = there && mbar_wait(&k_full[st], (gq / NK) & 1) && mbar_wait(&s_free[gq & 1], ((gq >> 1) & 1) ^ 1);
+      ok = __all_sync(0xffffffffu, there) && ok;
+      if (!ok) return;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t qd = q_desc + ((sqq & 1) * Cfg::Q_BYTES >> 4), kd = k_desc + (st * Cfg::T_BYTES >> 4);
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          const uint32_t off = ((ks >> 2) * (PA_M * 128) + (ks & 3) * 32) >> 4;
+          umma_f16(tmem_base + Cfg::TM_S + (gq & 1) * PA_N, qd + off, kd + off, idesc_qk, ks > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[gq & 1]);
+        umma_commit(&k_empty[st]);
+        if (jq + 1 == nq) umma_commit(&q_empty[sqq & 1]);
+      }
+      __syncwarp();
+      ++jq; ++gq;
+    };
     int g = 0, sq = 0, j = 0, n = 0;                              // of P V
-    bool o_there = false;
-    uint64_t since = 0;
-    uint32_t idle = 0;
-    for (;;) {
-      bool moved = false;
-      // scores, over P of the tile before the last: behind its product in the pipe
-      if (!q_end && gq < g + 2) {
-        if (jq == nq && ready(&listed[lq], lqphase)) {
-          nq = list[lq].tiles;
-          jq = 0;
-          q_there = false;
-          q_end = nq == 0;
-          if (!q_end) { ++sqq; if (++lq == PA_LIST) { lq = 0; lqphase ^= 1; } }
-          moved = true;
-        }
-        if (jq < nq) {
-          const int st = gq % NK;
-          if (!q_there) q_there = ready(&q_full[sqq & 1], (sqq >> 1) & 1);
-          if (q_there && ready(&k_full[st], (gq / NK) & 1)) {
-            tc_fence_after();
-            if (elect_one()) {
-              const uint64_t qd = q_desc + ((sqq & 1) * Cfg::Q_BYTES >> 4), kd = k_desc + (st * Cfg::T_BYTES >> 4);
+#pragma unroll 1
+    for (int ahead = 0; ok; ++ahead) {
+      product_qk();
+      if (ahead < 2 && !q_end) continue;                          // two scores before the first P V
+      if (!ok) break;
+      if (j == n) {                                               // the segment of the next product
+        if (!take(s, ok)) break;
+        let_go();
+        n = s.tiles;
+        j = 0;
+      }
+      const int st = g % NV, set = sq % Cfg::SETS;
+      bool there = j > 0 || mbar_wait(&o_free[set], ((sq / Cfg::SETS) & 1) ^ 1);        // the result there before has been read
+      there = there && mbar_wait(&v_full[st], (g / NV) & 1) && mbar_wait(&p_full[g & 1], (g >> 1) & 1);
+      ok = __all_sync(0xffffffffu, there);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t vd = v_desc + (st * Cfg::T_BYTES >> 4);
 #pragma unroll
-              for (int ks = 0; ks < HD / 16; ++ks) {
-                const uint32_t off = ((ks >> 2) * (PA_M * 128) + (ks & 3) * 32) >> 4;
-                umma_f16(tmem_base + Cfg::TM_S + (gq & 1) * PA_N, qd + off, kd + off, idesc_qk, ks > 0 ? 1u : 0u);
-              }
-              umma_commit(&k_empty[st]);
-              umma_commit(&s_full[gq & 1]);
-              if (jq + 1 == nq) umma_commit(&q_empty[sqq & 1]);
-            }
-            __syncwarp();
-            ++jq; ++gq;
-            moved = true;
-          }
-        }
+        for (int ks = 0; ks < PA_N / 16; ++ks)
+          umma_f16_ts(tmem_base + Cfg::TM_O + set * HD, tmem_base + Cfg::TM_P + (g & 1) * 64 + ks * 8, vd + (ks * 2048 >> 4), idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
+        umma_commit(&o_done[g & 1]);
+        umma_commit(&v_empty[st]);
+        if (j + 1 == n) umma_commit(&o_full[sq & 1]);
       }
-      if (g < gq || (q_end && j == n)) {
-        if (j == n) {                                             // the segment of the next product
-          if (g == gq) break;                                     // there is none
-          if (!take(s, ok)) break;                                // listed already
-          let_go();
-          n = s.tiles;
-          j = 0;
-          o_there = false;
-        }
-        const int st = g % NV;
-        if (!o_there) o_there = ready(&o_free[sq & 1], ((sq >> 1) & 1) ^ 1);      // the result before the last has been read
-        if (o_there && ready(&p_full[g & 1], (g >> 1) & 1) && ready(&v_full[st], (g / NV) & 1)) {
-          tc_fence_after();
-          if (elect_one()) {
-            const uint64_t vd = v_desc + (st * Cfg::T_BYTES >> 4);
-#pragma unroll
-            for (int ks = 0; ks < PA_N / 16; ++ks)
-              umma_f16_ts(tmem_base + Cfg::TM_O + (sq & 1) * HD, tmem_base + Cfg::TM_S + (g & 1) * PA_N + ks * 8, vd + (ks * 2048 >> 4), idesc_pv,
-                          (j > 0 || ks > 0) ? 1u : 0u);
-            umma_commit(&v_empty[st]);
-            umma_commit(&o_done[g & 1]);
-            if (j + 1 == n) umma_commit(&o_full[sq & 1]);
-          }
-          __syncwarp();
-          ++g;
-          if (++j == n) ++sq;
-          moved = true;
-        }
-      }
-      if (moved) { idle = 0; since = 0; continue; }
-      if (g < gq) mbar_nap(&p_full[g & 1], (g >> 1) & 1, 64);
-      else if (jq < nq) mbar_nap(&k_full[gq % NK], (gq / NK) & 1, 64);
-      else mbar_nap(&listed[lq], lqphase, 64);
-      if ((++idle & 0xff) == 0) {                                 // bounded like every wait: by wall time
-        const uint64_t now = global_timer_ns();
-        if (since == 0) since = now;
-        else if (__any_sync(0xffffffffu, now - since > OA_WAIT_LIMIT_NS)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); break; }
-      }
+      __syncwarp();
+      ++g;
+      if (++j == n) ++sq;
     }
+    if (!ok && lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX);
   } else if (warp < 8) {
-    // ---------------------------------------------------------------- softmax: warp w has TMEM lanes 32 (w % 4).. and the keys of half w / 4 of a tile
-    constexpr int OC = HD / 2;
-    const int quad = warp & 3, half = warp >> 2, r = quad * 32 + lane;
-    const int copy = copies == 1 ? 0 : quad, row = copies == 1 ? r : lane, i_row = token_of(p, row);      // i_row: token of this row in the tile
-    const uint32_t t_lane = (uint32_t)(quad * 32) << 16;
+    // ---------------------------------------------------------------- softmax: warp w has TMEM lanes 32 (w % 4).. of even (w < 4) or odd tiles
+    const int quad = warp & 3, grp = warp >> 2, r = quad * 32 + lane;
+    const int i_row = token_of(p, r);                             // token of this row in the tile
+    const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16);
+    const uint32_t s_addr = t_lane + Cfg::TM_S + grp * PA_N, p_addr = t_lane + Cfg::TM_P + grp * (PA_N / 2);
     const float sl2 = p.a.scale * 1.4426950408889634f;
     const unsigned long long sl22 = f2_splat(sl2);
-    float* xch = reinterpret_cast<float*>(smem + Cfg::OFF_X);
+    float* xch = reinterpret_cast<float*>(smem + Cfg::OFF_X);     // a row's maximum in use, by the even or odd tile that has set it
     int g = 0, sq = 0;
 #pragma unroll 1
     while (ok && take(s, ok)) {
       let_go();
-      const bool live = copies > 1 || quad * 32 < s.rows;         // of this warp: some row is there
+      const bool live = quad * 32 < s.rows;                       // of this warp: some row is there
       float m_run = -INFINITY, l_run = 0.f;
-      const uint32_t o_addr = tmem_base + t_lane + Cfg::TM_O + (sq & 1) * HD + half * OC;
+      const uint32_t o_addr = t_lane + Cfg::TM_O + sq % Cfg::SETS * HD;
 #pragma unroll 1
       for (int j = 0; j < s.tiles; ++j, ++g) {
+        if ((g & 1) != grp) continue;
         const KeyTile kt = key_tile(p, s.flags, s.seen, s.tile + j);
-        ok = warp_wait(&s_full[g & 1], (g >> 1) & 1);
+        // the scores are there, and P of the tile before the last has been used: its place is free
+        ok = mbar_wait(&s_full[grp], (g >> 1) & 1) && (g < 2 || mbar_wait(&o_done[grp], ((g - 2) >> 1) & 1));
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
         tc_fence_after();
+        // columns up to `last` are seen: the keys that there are, and of a request's own keys those up to the row's token
+        const int last = kt.prompt ? kt.count - 1 : min(kt.count - 1, s.shift + i_row - kt.first);
+        const bool cut = (kt.prompt ? kt.count - 1 : min(kt.count - 1, s.shift - kt.first)) < PA_N - 1;
+        const auto scores = [&](uint32_t* sv, int c0) {           // 64 of them, -inf for those that are not seen
+          tmem_ld32(s_addr + c0, sv);
+          tmem_ld32(s_addr + c0 + 32, sv + 32);
+          tmem_ld_wait();
+          const int lim = last - c0;
+          if (cut && __any_sync(0xffffffffu, lim < 63)) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) sv[i] = i <= lim ? sv[i] : 0xff800000u;
+          }
+        };
+        float mx = -INFINITY;
         if (live) {
-          const uint32_t s_addr = tmem_base + t_lane + Cfg::TM_S + (g & 1) * PA_N;
-          // columns up to `last` are seen: the keys that there are, and of a request's own keys those up to the row's token
-          const int last = kt.prompt ? kt.count - 1 : min(kt.count - 1, s.shift + i_row - kt.first);
-          const bool cut = (kt.prompt ? kt.count - 1 : min(kt.count - 1, s.shift - kt.first)) < PA_N - 1;
-          float alpha = 1.f;
-          bool grow = false;
-          const auto tile = [&](auto copies_of) {                 // 64 / C keys of this thread: half * 64 + copy * W ..
-            constexpr int C = decltype(copies_of)::value, W = 64 / C;
-            uint32_t sv[W];
-            if constexpr (C == 1) { tmem_ld32(s_addr + half * 64, sv); tmem_ld32(s_addr + half * 64 + 32, sv + 32); }
-            else tmem_ld16(s_addr + half * 64 + copy * 16, sv);
-            tmem_ld_wait();
-            if (cut) {
-              const int lim = last - half * 64 - copy * W;
+#pragma unroll 1
+          for (int c0 = 0; c0 < PA_N; c0 += 64) {
+            uint32_t sv[64];
+            scores(sv, c0);
+            float m1 = __uint_as_float(sv[0]);
 #pragma unroll
-              for (int i = 0; i < W; ++i) sv[i] = i <= lim ? sv[i] : 0xff800000u;
-            }
-            float m0 = __uint_as_float(sv[0]), m1 = __uint_as_float(sv[1]);
-#pragma unroll
-            for (int i = 2; i < W - 2; i += 4) {
-              m0 = fmax3(m0, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+            for (int i = 0; i < 64; i += 4) {
+              mx = fmax3(mx, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
               m1 = fmax3(m1, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
             }
-            float mx = fmax3(m0, m1, fmaxf(__uint_as_float(sv[W - 2]), __uint_as_float(sv[W - 1])));
-            float* slots = xch + (g & 1) * (2 * PA_M);
-            slots[(half ^ 1) * PA_M + r] = mx;
-            softmax_pair_sync(quad);                              // both halves are in registers: P may go over S
-            mx = fmaxf(mx, slots[half * PA_M + r]) * sl2;
-            const float m_new = fmaxf(m_run, mx);
-            grow = row < s.rows && (m_new - m_run) > PA_RESCALE;  // the first time: from -inf.  Not for rows that are not there, whose scores are anything
-            const float m_cand = grow ? m_new : m_run;
-            const float m_use = m_cand == -INFINITY ? 0.f : m_cand;       // a row that has seen nothing yet
-            alpha = grow ? fast_exp2(m_run - m_use) : 1.f;
-            m_run = m_cand;
-            const unsigned long long neg_m = f2_splat(-m_use);
-            unsigned long long l01 = 0, l23 = 0;
-            uint32_t pk[W / 2];
+            mx = fmaxf(mx, m1);
+          }
+        }
+        // the maximum in use goes from tile to tile: from the other warps' to this one, and on
+        if (g > 0) ok = warp_wait(&m_there[(grp ^ 1) * 4 + quad], ((g - 1) >> 1) & 1);
+        if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); break; }
+        const float m_old = j == 0 ? -INFINITY : xch[(grp ^ 1) * PA_M + r];
+        const float m_new = fmaxf(m_old, mx * sl2);
+        const bool grow = r < s.rows && (m_new - m_old) > PA_RESCALE;           // the first time: from -inf.  Not for rows that are not there, whose scores are anything
+        const float m_cand = grow ? m_new : m_old;
+        xch[grp * PA_M + r] = m_cand;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m_there[grp * 4 + quad]);
+        if (live) {
+          const float m_use = m_cand == -INFINITY ? 0.f : m_cand; // a row that has seen nothing yet
+          const unsigned long long neg_m = f2_splat(-m_use);
+          unsigned long long l01 = 0, l23 = 0;
+#pragma unroll 1
+          for (int c0 = 0; c0 < PA_N; c0 += 64) {
+            uint32_t sv[64], pk[32];
+            scores(sv, c0);
+            if (c0 + 64 == PA_N) {                                // all have been read
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&s_free[grp]);
+            }
 #pragma unroll
-            for (int i = 0; i < W; i += 4) {
+            for (int i = 0; i < 64; i += 4) {
               const unsigned long long x01 = f2_fma(f2_of(sv[i], sv[i + 1]), sl22, neg_m), x23 = f2_fma(f2_of(sv[i + 2], sv[i + 3]), sl22, neg_m);
-              // one of eight pairs on the multiply-add pipe, where the special-function units are what a full tile waits for
-              const unsigned long long e01 = exp2_mufu2(x01), e23 = C == 1 && (i >> 2) % 4 == 0 ? exp2_fma2(x23) : exp2_mufu2(x23);
+              // one of eight pairs on the multiply-add pipe: the special-function units are what a full tile waits for
+              const unsigned long long e01 = exp2_mufu2(x01), e23 = (i >> 2) % 4 == 0 ? exp2_fma2(x23) : exp2_mufu2(x23);
               l01 = f2_add(l01, e01);
               l23 = f2_add(l23, e23);
               pk[i >> 1] = f2_bf16(e01);                          // weights to bf16, as the tensor cores take them; their sum stays fp32
               pk[(i >> 1) + 1] = f2_bf16(e23);
             }
-            uint32_t a, b;
-            f2_to(f2_add(l01, l23), a, b);
-            l_run = l_run * alpha + (__uint_as_float(a) + __uint_as_float(b));
-            const uint32_t p_addr = s_addr + half * 32;           // this half's 64 keys: the copy's own, zeros elsewhere
-            if constexpr (C == 1) tmem_st32(p_addr, pk);
-            else {
-              uint32_t all[32];
-#pragma unroll
-              for (int i = 0; i < 32; ++i) all[i] = (i >> 3) == copy ? pk[i & 7] : 0u;
-              tmem_st32(p_addr, all);
-            }
-          };
-          if (copies > 1) tile(std::integral_constant<int, 4>());
-          else tile(std::integral_constant<int, 1>());
+            tmem_st32(p_addr + (c0 >> 1), pk);
+          }
+          uint32_t a, b;
+          f2_to(f2_add(l01, l23), a, b);
+          l_run = (m_run == m_cand ? l_run : l_run * fast_exp2(m_run - m_use)) + (__uint_as_float(a) + __uint_as_float(b));
+          m_run = m_cand;
           if (j > 0 && __any_sync(0xffffffffu, grow)) {           // O again to the new maximum, behind the product before
-            ok = warp_wait(&o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
+            const float alpha = grow ? fast_exp2(m_old - m_use) : 1.f;
+            ok = warp_wait(&o_done[grp ^ 1], ((g - 1) >> 1) & 1);
             if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < OC / 32; ++c) {
+            for (int c = 0; c < HD; c += 32) {
               uint32_t o[32];
-              tmem_ld32(o_addr + c * 32, o);
+              tmem_ld32(o_addr + c, o);
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st32(o_addr + c * 32, o);
+              tmem_st32(o_addr + c, o);
             }
           }
           tmem_st_wait();
           tc_fence_before();
+        } else if (lane == 0) {
+          mbar_arrive(&s_free[grp]);
         }
         if (kt.count < PA_N) {                                    // values that no key goes with: zeros, whatever lies there
           const int st = g % NV;
@@ -777,166 +1133,99 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
           const uint32_t base = smem_u32(smem + Cfg::OFF_V + st * Cfg::T_BYTES);
 #pragma unroll 1
-          for (int i = threadIdx.x; i < (PA_N - kt.count) * CHUNKS * 8; i += 256) {
+          for (int i = threadIdx.x & 127; i < (PA_N - kt.count) * CHUNKS * 8; i += 128) {
             const int at = kt.count + i / (CHUNKS * 8), c = i % (CHUNKS * 8);
             st_shared_v4(base + (c >> 3) * (PA_N * 128) + at * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
           }
           fence_proxy_async_smem();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[g & 1]);
+        if (lane == 0) mbar_arrive(&p_full[grp]);
       }
       if (!ok) break;
-      ok = warp_wait(&o_free[sq & 1], ((sq >> 1) & 1) ^ 1);       // m and l of the segment before the last have been read
+      ok = warp_wait(&seg_free[sq & 1], ((sq >> 1) & 1) ^ 1);     // m and l of the segment before the last have been read
       if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); break; }
-      float* ml = s_ml + (sq & 1) * 3 * PA_M;
-      if (half == 0) ml[r] = m_run;
-      ml[(1 + half) * PA_M + r] = l_run;
+      float* ml = s_ml + ((sq & 1) * 2 + grp) * 2 * PA_M;
+      ml[r] = m_run;
+      ml[PA_M + r] = l_run;
       __syncwarp();
       if (lane == 0) mbar_arrive(&seg_done[sq & 1]);
       ++sq;
     }
   } else {
     // ---------------------------------------------------------------- results: warp 8 + q has TMEM lanes 32 q..
-    const int quad = warp & 3, r = quad * 32 + lane, et = threadIdx.x - 256;
-    const int copy = copies == 1 ? 0 : quad, row = copies == 1 ? r : lane, i_row = token_of(p, row);
+    const int quad = warp & 3, r = quad * 32 + lane;
     const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16);
-    float* stage = reinterpret_cast<float*>(smem + Cfg::OFF_STAGE);
     int sq = 0;
-    bool met = false;
 #pragma unroll 1
     while (take(s, ok)) {
       let_go();
       // barriers of segments, of which at most two are under way: this warp may be behind by many tiles
       ok = warp_wait(&seg_done[sq & 1], (sq >> 1) & 1) && warp_wait(&o_full[sq & 1], (sq >> 1) & 1);
-      if (!ok && lane == 0) { report_error(p.status, OA_KERR_WAIT_TMEM_FULL); s_fail = 1; }
-      if (copies > 1) { out_sync(); ok = s_fail == 0; }           // what was staged before has been read; and the four warps leave together
-      if (!ok) { met = true; break; }
+      if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
       tc_fence_after();
-      const float* ml = s_ml + (sq & 1) * 3 * PA_M;
-      const uint32_t o_addr = t_lane + Cfg::TM_O + (sq & 1) * HD;
-      const bool whole = s.flags & 2;                             // nothing to be joined
-      // the row's m, l and the factor of this copy's part
-      float m = ml[r], l = ml[PA_M + r] + ml[2 * PA_M + r], f = 1.f;
-      if (copies > 1) {
-        const float mine = m;
-        float mc[4], sum = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) { mc[c] = ml[c * 32 + lane]; m = fmaxf(m, mc[c]); }
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          sum += (ml[PA_M + c * 32 + lane] + ml[2 * PA_M + c * 32 + lane]) * (mc[c] == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : fast_exp2(mc[c] - m));
-        f = mine == -INFINITY ? 0.f : fast_exp2(mine - m);
-        l = sum;
-      }
-      const float inv = l == 0.f ? 0.f : 1.f / l;                 // NaN stays NaN
-      const int t = s.t0 + i_row;
-      const bool there = row < s.rows && (whole ? t >= 0 && t < p.a.tokens : has_room(p, s.at + row));
-      const long long out_row = (long long)t * p.a.q_heads + s.h * p.group + row - i_row * p.group;
-      if (copy == 0 && there) {
-        if (!whole) p.ml[s.at + row] = make_float2(m, l);
-        else if (p.a.lse) p.a.lse[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-      }
+      const int set = sq % Cfg::SETS;
+      const uint32_t o_addr = t_lane + Cfg::TM_O + set * HD;
+      const float* ml = s_ml + (sq & 1) * 4 * PA_M + r;           // sums of even and odd tiles, each to the maximum that it has seen last; O is to the last of all
+      const float m_even = ml[0], m_odd = ml[2 * PA_M], m = fmaxf(m_even, m_odd);
+      const float l = ml[PA_M] * (m_even == m ? 1.f : fast_exp2(m_even - m)) + ml[3 * PA_M] * (m_odd == m ? 1.f : fast_exp2(m_odd - m));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_free[sq & 1]);
       const auto release = [&] {                                  // all has been read
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&o_free[sq & 1]);
+        if (lane == 0) mbar_arrive(&o_free[set]);
       };
-      if (copies == 1) {                                          // a row to a lane
-        if (quad * 32 < s.rows) {
+      const bool whole = s.flags & 2;                           // nothing to be joined
+      const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;           // NaN stays NaN
+      if (whole) {
+        const int i = token_of(p, r), t = s.t0 + i;
+        if (p.a.lse && r < s.rows && t >= 0 && t < p.a.tokens)
+          p.a.lse[(long long)t * p.a.q_heads + s.h * p.group + r - i * p.group] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      } else if (r < s.rows && has_room(p, s.at + r)) {
+        p.ml[s.at + r] = make_float2(m, l);
+      }
+      if (quad * 32 < s.rows) {
+        const int row0 = quad * 32 + (lane & ~3);               // after an exchange among four lanes a lane has 16 bytes of four rows
 #pragma unroll 1
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + c, o);
-            tmem_ld_wait();
-            const float* x = reinterpret_cast<const float*>(o);
-            if (!there) {
-            } else if (whole) {
-              uint4* to = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.a.out) + out_row * HD + c);
-#pragma unroll
-              for (int k = 0; k < 4; ++k, x += 8)
-                to[k] = make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv), pack_bf16x2(x[6] * inv, x[7] * inv));
-            } else {
-              uint4* to = reinterpret_cast<uint4*>(p.part + (s.at + row) * HD + c);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) to[k] = make_uint4(o[k * 4], o[k * 4 + 1], o[k * 4 + 2], o[k * 4 + 3]);
-            }
-            __syncwarp();
-          }
-        }
-        release();
-      } else {
-        // copies meet in shared memory
-        if (copy == 0) s_inv[row] = inv;
-        const auto emit = [&](int rw, int c, float4 sum) {        // four columns of a row
-          if (!whole) {
-            if (has_room(p, s.at + rw)) *reinterpret_cast<float4*>(p.part + (s.at + rw) * HD + c) = sum;
-            return;
-          }
-          const int i = token_of(p, rw), tr = s.t0 + i;
-          if (tr < 0 || tr >= p.a.tokens) return;
-          const float q = s_inv[rw];
-          *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.a.out) + ((long long)tr * p.a.q_heads + s.h * p.group + rw - i * p.group) * HD + c) =
-              make_uint2(pack_bf16x2(sum.x * q, sum.y * q), pack_bf16x2(sum.z * q, sum.w * q));
-        };
-        if (s.rows <= 8) {
-          // Up to eight rows: a load that gives lane l two neighbouring columns of row l / 4, so that every lane has some of them.  A row to a
-          // lane left 24 lanes or more idle and made a request's single token 1.5 us of it.
-          const float fr = __shfl_sync(0xffffffffu, f, lane >> 2);
-          float* to = stage + (copy * 8 + (lane >> 2)) * (HD + 8) + (lane & 3) * 2;
-          uint32_t o[HD / 2];
-#pragma unroll
-          for (int c = 0; c < HD / 64; ++c) tmem_ld_16x256b_x8(o_addr + c * 64, o + c * 32);
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t x[32];
+          tmem_ld32(o_addr + c, x);
           tmem_ld_wait();
-          release();
+          if (c + 32 == HD) release();
+          if (whole) {
+            uint4 v[4];
 #pragma unroll
-          for (int c = 0; c < HD / 8; ++c)
-            *reinterpret_cast<float2*>(to + c * 8) = fr == 0.f ? make_float2(0.f, 0.f) : make_float2(__uint_as_float(o[c * 4]) * fr, __uint_as_float(o[c * 4 + 1]) * fr);
-          out_sync();
-          constexpr int PER_ROW = HD / 4;
-#pragma unroll 1
-          for (int i = et; i < s.rows * PER_ROW; i += 128) {
-            const int rw = i / PER_ROW, c = (i % PER_ROW) * 4;
-            float4 x[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4*>(stage + (k * 8 + rw) * (HD + 8) + c);
-            emit(rw, c, make_float4((x[0].x + x[1].x) + (x[2].x + x[3].x), (x[0].y + x[1].y) + (x[2].y + x[3].y), (x[0].z + x[1].z) + (x[2].z + x[3].z),
-                                    (x[0].w + x[1].w) + (x[2].w + x[3].w)));
-          }
-        } else {
-#pragma unroll 1
-          for (int c0 = 0; c0 < HD; c0 += 32) {                   // 32 columns at a time
-            if (c0 > 0) out_sync();                               // the columns before have been read
-            uint32_t o[32];
-            tmem_ld32(o_addr + c0, o);
-            tmem_ld_wait();
-            if (c0 + 32 == HD) release();
-            if (row < s.rows) {
-              float4* to = reinterpret_cast<float4*>(stage + r * 36);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const float* x = reinterpret_cast<const float*>(o) + k * 4;
-                to[k] = f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
-              }
+            for (int k = 0; k < 4; ++k) {
+              const auto pair = [&](int i) { return pack_bf16x2(__uint_as_float(x[k * 8 + i]) * inv, __uint_as_float(x[k * 8 + i + 1]) * inv); };
+              v[k] = make_uint4(pair(0), pair(2), pair(4), pair(6));
             }
-            out_sync();
-#pragma unroll 1
-            for (int i = et; i < s.rows * 8; i += 128) {
-              const int rw = i >> 3, c = (i & 7) * 4;
-              float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            exchange4(v, lane);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float4 x = *reinterpret_cast<const float4*>(stage + (k * 32 + rw) * 36 + c);
-                sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
-              }
-              emit(rw, c0 + c, sum);
+            for (int k = 0; k < 4; ++k) {
+              const int row = row0 + k, i = token_of(p, row), t = s.t0 + i;
+              if (row < s.rows && t >= 0 && t < p.a.tokens)
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.a.out) + ((long long)t * p.a.q_heads + s.h * p.group + row - i * p.group) * HD + c + (lane & 3) * 8) = v[k];
+            }
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint4 v[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[k] = make_uint4(x[h * 16 + k * 4], x[h * 16 + k * 4 + 1], x[h * 16 + k * 4 + 2], x[h * 16 + k * 4 + 3]);
+              exchange4(v, lane);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (row0 + k < s.rows && has_room(p, s.at + row0 + k)) *reinterpret_cast<uint4*>(p.part + (s.at + row0 + k) * HD + c + h * 16 + (lane & 3) * 4) = v[k];
             }
           }
+          __syncwarp();
         }
+      } else {
+        release();
       }
       ++sq;
     }
-    if (!ok && copies > 1 && !met) { s_fail = 1; out_sync(); }    // the entry never came: the others, who meet once more, do not wait for this warp
   }
   tc_fence_before();
   __syncthreads();
@@ -948,7 +1237,7 @@ template <int HD>
 struct RowJoin {
   static constexpr int PER = HD / 32;
   float m = -INFINITY, l = 0.f, acc[PER] = {};
-  // `count` pieces, of which row_of(i) is the i-th: the weights of 32 at a time, one to a lane, then their rows, four under way at once
+  // `count` pieces, of which row_of(i) is the i-th: the weights of 32 at a time, one to a lane, then their rows, eight under way at once
   template <typename F>
   __device__ __forceinline__ void add(const PagedTcParams& p, int count, F row_of, int lane) {
     for (int i0 = 0; i0 < count; i0 += 32) {
@@ -963,10 +1252,10 @@ struct RowJoin {
       for (int e = 0; e < PER; ++e) acc[e] *= a;
       m = m_new;
       const int n = min(count - i0, 32);
-      for (int j0 = 0; j0 < n; j0 += 4) {
-        float v[4][PER], wj[4];
+      for (int j0 = 0; j0 < n; j0 += 8) {
+        float v[8][PER], wj[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 8; ++k) {
           const long long row = __shfl_sync(0xffffffffu, mine, min(j0 + k, 31));
           wj[k] = j0 + k < n ? __shfl_sync(0xffffffffu, w, min(j0 + k, 31)) : 0.f;
 #pragma unroll
@@ -977,7 +1266,7 @@ struct RowJoin {
           }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 8; ++k)
 #pragma unroll
           for (int e = 0; e < PER; ++e) acc[e] += v[k][e] * wj[k];
       }
@@ -992,45 +1281,59 @@ struct RowJoin {
   }
 };
 
-// Shared form: every row from the pieces of its prompt item and of its own item.  Block (b, y) has rows 8 y .. of request b, a warp to each, so that
-// all it has to know of the request arrives at once; blocks of b = batch the rows of no request, zeros.
+// Shared form: every row from the pieces of its prompt item and of its own item, HD / 4 lanes to a row.  The first four pieces, of which there are seldom
+// more, are fetched together with their (m, l), before it is known whether they count.
 template <int HD>
 __global__ void __launch_bounds__(256) paged_join_rows_kernel(const __grid_constant__ PagedTcParams p) {
+  constexpr int LANES = HD / 4, AT_ONCE = 4;
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x;
-  if (b == p.a.batch) {
-    const int t0 = p.a.starts[0], t1 = p.a.starts[p.a.batch];
-    for (int t = blockIdx.y * 8 + warp; t < p.a.tokens; t += gridDim.y * 8)
-      if (t < t0 || t >= t1)
-        for (int hq = 0; hq < p.a.q_heads; ++hq) RowJoin<HD>().write(p, t, hq, lane);
-    return;
-  }
-  const int per_prompt = p.sums[1], per = p.sums[2], before = p.sums[PA_SUMS + b], all = p.sums[PA_SUMS + b + 1] - before;
-  const int items = p.sums[PA_SUMS + 1 + p.a.batch + b];
-  const Request r = request_of(p, b);
-  for (int w = blockIdx.y * 8 + warp; w < r.n * p.a.q_heads; w += gridDim.y * 8) {
-    const int i = w / p.a.q_heads, hq = w - i * p.a.q_heads, t = r.t0 + i, h = hq / p.group, head = hq - h * p.group;
-    if (t < 0 || t >= p.a.tokens) continue;
-    RowJoin<HD> join;
-    if (i < r.fresh) {
-      const int prt = t / p.tpt, p_item = h * p.prefix_row_tiles + prt, pa = p_item * p.prefix_tiles;
-      const int p_first = pa / per_prompt, p_count = (pa + p.prefix_tiles - 1) / per_prompt - p_first + 1;
-      const int rt = i / p.tpt, tiles = tiles_of(p, r, rt), item = items * p.a.kv_heads + h * r.row_tiles + rt;
-      int first = 0, count = 0;
-      if (tiles > 0) {
-        int a = before * p.a.kv_heads + h * all;
-        for (int k = 0; k < rt; ++k) a += tiles_of(p, r, k);
-        first = a / per;
-        count = (a + tiles - 1) / per - first + 1;
+  const long long row = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int t = (int)(row / p.a.q_heads), hq = (int)(row - (long long)t * p.a.q_heads), h = hq / p.group, head = hq - h * p.group, x = threadIdx.x % LANES * 4;
+  if (t >= p.a.tokens) return;
+  const PagedOwn own = p.owns[t];
+  const int per_prompt = p.sums[1], per = p.sums[2];
+  const int prt = t / p.tpt, p_item = h * p.prefix_row_tiles + prt, pa = p_item * p.prefix_tiles, p_first = pa / per_prompt;
+  const int p_count = own.inner >= 0 && p.prefix_tiles > 0 ? min((pa + p.prefix_tiles - 1) / per_prompt - p_first + 1, p.ctas) : 0;
+  const int a = own.pos + h * own.all, first = a / per, count = own.inner >= 0 && own.tiles > 0 ? min((a + own.tiles - 1) / per - first + 1, p.ctas) : 0;
+  const long long p_row = prompt_row(p, (long long)p_item + p_first) + (t - prt * p.tpt) * p.group + head;
+  const long long o_row = own_row(p, (long long)own.item + h * own.row_tiles + first) + own.inner * p.group + head;
+  float m = -INFINITY, l = 0.f, acc[4] = {};
+#pragma unroll 1
+  for (int k0 = 0; k0 < p_count + count; k0 += AT_ONCE) {
+    float2 ml[AT_ONCE];
+    float4 v[AT_ONCE];
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const long long at = k0 + k < p_count ? prompt_row(p, k0 + k) + p_row : own_row(p, k0 + k - p_count) - p.own_slot0 + o_row;
+      ml[k] = make_float2(-INFINITY, 0.f);
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k0 + k < p_count + count && has_room(p, at)) {
+        ml[k] = p.ml[at];
+        v[k] = *reinterpret_cast<const float4*>(p.part + at * HD + x);
       }
-      join.add(p, p_count + count, [&](int k) -> long long {
-        return k < p_count ? prompt_row(p, (long long)p_item + p_first + k) + (t - prt * p.tpt) * p.group + head
-                           : own_row(p, (long long)item + first + k - p_count) + (i - rt * p.tpt) * p.group + head;
-      }, lane);
     }
-    join.write(p, t, hq, lane);
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k)
+      if (ml[k].y != 0.f) top = fmaxf(top, ml[k].x);             // otherwise a piece of which this row saw nothing
+    const float keep = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    l *= keep;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= keep;
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      if (ml[k].y == 0.f) continue;
+      const float w = ml[k].x == -INFINITY ? 1.f : fast_exp2(ml[k].x - top);
+      l += ml[k].y * w;
+      acc[0] += v[k].x * w; acc[1] += v[k].y * w; acc[2] += v[k].z * w; acc[3] += v[k].w * w;
+    }
+    m = top;
   }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.a.out) + ((long long)t * p.a.q_heads + hq) * HD + x) =
+      make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+  if (p.a.lse && x == 0) p.a.lse[(long long)t * p.a.q_heads + hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // Joint form: the items that a stretch's end cuts (block c: the one that begins in stretch c and goes beyond it), and zeros for the rows of
@@ -1072,9 +1375,9 @@ using namespace oa;
 
 // The sizes that follow from a call's arguments: which form, how many items there can be, what they need in scratch.
 struct PagedTcPlan {
-  int group, tpt, ts, tb, copies, copies_prompt, joint, prefix_tiles, prefix_row_tiles, grid;
+  int group, tpt, ts, tb, few, few_prompt, own_log2, joint, prefix_tiles, prefix_row_tiles, grid;
   long long prompt_rows, own_rows, items;
-  size_t o_bytes, ml_bytes, bytes;
+  size_t o_bytes, owns_bytes, ml_bytes, bytes;
 };
 static int sm_count() {
   static int sms = 0;
@@ -1090,19 +1393,24 @@ static PagedTcPlan plan_tc(int tokens, int batch, int max_fresh, int q_heads, in
   c.tpt = PA_M / c.group;
   c.ts = max_fresh < c.tpt ? (max_fresh > 0 ? max_fresh : 1) : c.tpt;
   c.tb = tokens < c.tpt ? tokens : c.tpt;
-  c.copies = c.ts * c.group <= 32 ? 4 : 1;
-  c.copies_prompt = c.tb * c.group <= 32 ? 4 : 1;
-  c.prefix_tiles = (prefix_len + PA_N - 1) / PA_N;
+  const int few_log2 = head_dim == 64 ? PF_KEYS_LOG2<64> : PF_KEYS_LOG2<128>;
+  const auto few = [&](int rows) { return rows > PF_ROWS ? 0 : rows <= 8 ? 8 : 16; };
+  c.few = few(c.ts * c.group);
+  c.few_prompt = few(c.tb * c.group);
+  c.own_log2 = c.few ? few_log2 : 7;
   c.prefix_row_tiles = (tokens + c.tpt - 1) / c.tpt;
-  // The prompt for the whole batch at once where that reads it at most half as often as request by request.
-  c.joint = prefix_len == 0 || 2ll * c.prefix_row_tiles > batch;
+  // The prompt for the whole batch at once where that reads it at most half as often as request by request, and always where a request has few rows.
+  c.joint = !c.few && (prefix_len == 0 || 2ll * c.prefix_row_tiles > batch);
+  const int prefix_log2 = c.few_prompt && !c.joint ? few_log2 : 7;
+  c.prefix_tiles = (int)(((long long)prefix_len + (1 << prefix_log2) - 1) >> prefix_log2);
   c.grid = sm_count();
   c.items = ((long long)batch + tokens / c.tpt) * kv_heads;                    // query tiles of single requests, at most
-  c.prompt_rows = c.joint ? 0 : ((long long)c.prefix_row_tiles * kv_heads + c.grid) * (c.tb * c.group);
+  c.prompt_rows = c.joint || prefix_len == 0 ? 0 : ((long long)c.prefix_row_tiles * kv_heads + c.grid) * (c.tb * c.group);
   c.own_rows = (c.joint ? 2ll * c.grid : c.items + c.grid) * (c.ts * c.group);
   c.o_bytes = (size_t)(c.prompt_rows + c.own_rows) * head_dim * sizeof(float);
   c.ml_bytes = (size_t)(c.prompt_rows + c.own_rows) * sizeof(float2);
-  c.bytes = c.o_bytes + c.ml_bytes + (2 * ((size_t)batch + 1) + PA_SUMS) * sizeof(int);
+  c.owns_bytes = c.joint ? 0 : (size_t)tokens * sizeof(PagedOwn);
+  c.bytes = c.o_bytes + c.owns_bytes + c.ml_bytes + (2 * ((size_t)batch + 1) + PA_SUMS) * sizeof(int);
   return c;
 }
 // Which calls the tensor-core kernel takes: bf16, head dims of whole 128-byte rows, a batch whose prefix sums fit in shared memory beside the
@@ -1132,21 +1440,24 @@ static int launch_tc(const PagedAttnParams& a, void* scratch, int* status, cudaS
   }
   const PagedTcPlan c = plan_tc(a.tokens, a.batch, a.max_fresh, a.q_heads, a.kv_heads, HD, a.prefix_len);
   const int ps = 1 << a.page_log2;
-  const long long own_tiles = ((long long)a.width * ps + PA_N - 1) / PA_N;
+  const long long own_tiles = (((long long)a.width * ps) >> c.own_log2) + 1;
   const long long work = (c.joint ? 0 : (long long)a.kv_heads * c.prefix_row_tiles * c.prefix_tiles);
   if (work + c.items * (own_tiles + c.prefix_tiles + 1) > 0x7fffffffll) return OA_ERR_TOO_LARGE;
   PagedTcParams p;
   p.a = a;
   p.group = c.group; p.group_mul = 65536 / c.group + 1; p.tpt = c.tpt; p.ts = c.ts; p.tb = c.tb;
-  p.copies = c.copies; p.copies_prompt = c.copies_prompt;
+  p.few = c.few; p.few_prompt = c.few_prompt; p.own_log2 = c.own_log2;
+  p.many = !c.few || (work > 0 && !c.few_prompt);
   p.joint = c.joint; p.prefix_tiles = c.prefix_tiles; p.prefix_row_tiles = c.prefix_row_tiles; p.prefix_work = (int)work;
   p.part = static_cast<float*>(scratch);
-  p.ml = reinterpret_cast<float2*>(static_cast<char*>(scratch) + c.o_bytes);
-  p.sums = reinterpret_cast<int*>(static_cast<char*>(scratch) + c.o_bytes + c.ml_bytes);
+  p.owns = reinterpret_cast<PagedOwn*>(static_cast<char*>(scratch) + c.o_bytes);
+  p.ml = reinterpret_cast<float2*>(static_cast<char*>(scratch) + c.o_bytes + c.owns_bytes);
+  p.sums = reinterpret_cast<int*>(static_cast<char*>(scratch) + c.o_bytes + c.owns_bytes + c.ml_bytes);
   p.own_slot0 = c.prompt_rows;
   p.part_rows = c.prompt_rows + c.own_rows;
+  p.ctas = c.grid;
   p.status = status;
-  CUtensorMap tq, tqo, tk, tv;
+  CUtensorMap tq, tqo, tk, tv, tkf, tvf;
   int rc;
   {
     const uint64_t dims[3] = {HD, (uint64_t)a.q_heads, (uint64_t)a.tokens}, strides[2] = {HD * 2, (uint64_t)a.q_stride * 2};
@@ -1158,11 +1469,17 @@ static int launch_tc(const PagedAttnParams& a, void* scratch, int* status, cudaS
   const uint32_t box[3] = {64, (uint32_t)ps, 1};
   const uint64_t ks[2] = {HD * 2, (a.pages > 1 ? (uint64_t)a.k_page_stride : packed) * 2}, vs[2] = {HD * 2, (a.pages > 1 ? (uint64_t)a.v_page_stride : packed) * 2};
   if ((rc = make_tmap_box3_bf16(&tk, a.k, dims, ks, box)) || (rc = make_tmap_box3_bf16(&tv, a.v, dims, vs, box))) return rc;
-  launch_short(paged_attn_tc_kernel<HD>, dim3((unsigned)c.grid), dim3(PA_THREADS), Cfg::SMEM_BYTES, st, tq, tqo, tk, tv, p);
+  tkf = tk;
+  tvf = tv;
+  if (ps > 1 << PF_KEYS_LOG2<HD>) {                                // boxes of a tile's keys, where a page has more
+    const uint32_t fewer[3] = {64, 1u << PF_KEYS_LOG2<HD>, 1};
+    if ((rc = make_tmap_box3_bf16(&tkf, a.k, dims, ks, fewer)) || (rc = make_tmap_box3_bf16(&tvf, a.v, dims, vs, fewer))) return rc;
+  }
+  launch_short(paged_attn_tc_kernel<HD>, dim3((unsigned)c.grid), dim3(PA_THREADS), Cfg::SMEM_BYTES, st, tq, tqo, tk, tv, tkf, tvf, p);
   if (c.joint) launch_short(paged_join_cuts_kernel<HD>, dim3((unsigned)c.grid), dim3(256), 0, st, p);
   else {
-    const long long rows = (long long)(a.max_fresh > 0 ? a.max_fresh : 1) * a.q_heads;           // of a request, at most
-    launch_short(paged_join_rows_kernel<HD>, dim3((unsigned)a.batch + 1, (unsigned)(rows < 8 * 1024 ? (rows + 7) / 8 : 1024)), dim3(256), 0, st, p);
+    const long long rows = (long long)a.tokens * a.q_heads, rows_of_block = 1024 / HD;
+    launch_short(paged_join_rows_kernel<HD>, dim3((unsigned)((rows + rows_of_block - 1) / rows_of_block)), dim3(256), 0, st, p);
   }
   return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }

@@ -22,6 +22,23 @@ from ..models.gpt import OaGptModel
 from ..ops import kernels as K
 
 
+def block_tail(b, x: OaMatrix, attn: OaMatrix, few_rows: bool) -> OaMatrix:
+    """What a block does behind its attention: output projection and feed-forward, both added to x."""
+    o = b.Attention.OutProj
+    x = F.Linear(attn, o.Weight.Data, o.Bias.Data if o.Bias else None, residual=x)
+    if b.Moe is not None:
+        return b.Moe.Forward(x)
+    if b.FfnKind == "gelu":
+        hh = b.LnFfn.Forward(x)
+        return FF.FfnGelu(hh, b.Ffn1.Weight.Data, b.Ffn1.Bias.Data if b.Ffn1.Bias else None, b.Ffn2.Weight.Data,
+                          b.Ffn2.Bias.Data if b.Ffn2.Bias else None, residual=x)
+    f = b.Ffn
+    if few_rows and FF.packed_view([f.Gate.Weight.Tensor(), f.Up.Weight.Tensor()]) is None:
+        hh = f.Norm.Forward(x)                        # weights that do not lie side by side: two products rather than a joined copy
+        return F.Linear(F.SiluMul(F.Linear(hh, f.Gate.Weight.Data), F.Linear(hh, f.Up.Weight.Data)), f.Down.Weight.Data, None, residual=x)
+    return f.Forward(x)
+
+
 class OaKvCache:
     """Keys and values of every layer: [layers][batch, heads, max_seq, head_dim] in the model's dtype."""
 
@@ -163,19 +180,7 @@ class OaGptDecoder:
             else:
                 K.kv_append(t[:, D:2 * D], t[:, 2 * D:], self.Cache.K[i], self.Cache.V[i], batch, 1, pos0, pos_dev=pd)
             attn = OaMatrix(K.decode_attn(t[:, :D], self.Cache.K[i], self.Cache.V[i], pos0 + 1, pos_dev=pd))
-        o = a.OutProj
-        x = F.Linear(attn, o.Weight.Data, o.Bias.Data if o.Bias else None, residual=x)
-        if b.Moe is not None:
-            return b.Moe.Forward(x)
-        if b.FfnKind == "gelu":
-            hh = b.LnFfn.Forward(x)
-            return FF.FfnGelu(hh, b.Ffn1.Weight.Data, b.Ffn1.Bias.Data if b.Ffn1.Bias else None, b.Ffn2.Weight.Data,
-                              b.Ffn2.Bias.Data if b.Ffn2.Bias else None, residual=x)
-        f = b.Ffn
-        if s_new == 1 and FF.packed_view([f.Gate.Weight.Tensor(), f.Up.Weight.Tensor()]) is None:
-            hh = f.Norm.Forward(x)                    # weights that do not lie side by side: two products rather than a joined copy
-            return F.Linear(F.SiluMul(F.Linear(hh, f.Gate.Weight.Data), F.Linear(hh, f.Up.Weight.Data)), f.Down.Weight.Data, None, residual=x)
-        return f.Forward(x)
+        return block_tail(b, x, attn, s_new == 1)
 
     def _forward(self, ids: torch.Tensor, x: Optional[torch.Tensor] = None) -> torch.Tensor:
         """ids [B, s_new] int32 -> logits of the last new position [B, vocab]; the cache grows by s_new.  `x`: the rows of the ids,

@@ -430,35 +430,26 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     meet();
     return (int)min(all, (u64)ROW_LIST + 1);
   };
-  // The first n entries of bins into falling order.
+  // The first n entries of bins into falling order, by counting those above each, with four, two or one thread to an entry (64 entries: 0.4 us, by
+  // exchanges 2.0; 256: 1.3 and 4.7; 512 are alike).
   const auto sort_list = [&](int n) {
+    const int lt = n <= ROW_LIST / 4 ? 2 : n <= ROW_LIST / 2 ? 1 : 0, at = tid >> lt, part = tid & ((1 << lt) - 1);
+    if (tid == 0) bins[n] = 0;                                   // entries are read in pairs
     __syncthreads();
-    if (n <= ROW_LIST / 4) {                                     // by counting, four threads to an entry (64 entries: 0.4 us, by exchanges 2.0)
-      const u64 e = (tid >> 2) < n ? bins[tid >> 2] : 0;
-      int above = 0;
-      for (int i = tid & 3; i < n; i += 4) above += bins[i] > e;
-      above += __shfl_xor_sync(0xffffffffu, above, 1);
-      above += __shfl_xor_sync(0xffffffffu, above, 2);
-      __syncthreads();
-      if ((tid & 3) == 0 && (tid >> 2) < n) bins[above] = e;
-      __syncthreads();
-      return;
-    }
-    int size = 64;
-    while (size < n) size <<= 1;
-    if (tid >= n && tid < size) clear_bins();
-    __syncthreads();
-    for (int lk = 1; 1 << lk <= size; ++lk) {
-      for (int lj = lk - 1; lj >= 0; --lj) {
-        if (tid < size / 2) {
-          const int i = ((tid >> lj) << (lj + 1)) | (tid & ((1 << lj) - 1)), o = i + (1 << lj);
-          const u64 u = bins[i], v = bins[o];
-          if ((u < v) == (((i >> lk) & 1) == 0)) { bins[i] = v; bins[o] = u; }
-        }
-        if (lj > 5) __syncthreads(); else __syncwarp();          // up to a distance of 32 a warp's pairs lie in 64 entries of its own
+    u64 e = 0;
+    int above = 0;
+    if (at < n) {
+      e = bins[at];
+#pragma unroll 4
+      for (int i = 2 * part; i < n; i += 2 << lt) {
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(bins + i);
+        above += (o.x > e) + (o.y > e);
       }
-      if (lk >= 6) __syncthreads();
     }
+    if (lt > 0) above += __shfl_xor_sync(0xffffffffu, above, 1);
+    if (lt > 1) above += __shfl_xor_sync(0xffffffffu, above, 2);
+    __syncthreads();
+    if (part == 0 && at < n) bins[above] = e;
     __syncthreads();
   };
   // Sums over a block in thread order: what is before this thread, and all.

@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(128) paged_attn_rows_kernel(const PagedAttnPar
 //   that a row is an eighth of an instruction and not 1/128 of a tile, and stay in registers: their exponentials turn into an operand of
 //   V^T P^T by a transpose among lanes.  128 requests behind 8191 shared keys with 1024 of their own on average, 8 key-value heads of 64, group 8:
 //   own keys arrive at 95 bytes a nanosecond and SM where 72 SMs take them, which is what the memory gives; a tcgen05 tile with 8 of its 128 rows
-//   alive took 3300 instructions and 0.75 us for 128 keys (46 GB/s and SM), and the call 101 us where it now takes 79.
+//   alive took 3300 instructions and 0.75 us for 128 keys (46 bytes a nanosecond and SM), and the call 101 us where this made it 79.
 //   More than 16 rows would need more registers than a thread has.
 //
 // Keys beyond a length are cut off from the scores by a select, and their values are overwritten by zeros before the product: what lies there
@@ -163,9 +163,11 @@ __global__ void __launch_bounds__(128) paged_attn_rows_kernel(const PagedAttnPar
 // TMEM;  warps 0-3 are the softmax of even tiles, warps 4-7 of odd ones, a thread to a row: the exponentials of one tile run beside the
 // waits of the other.  A row's maximum in use goes from tile to tile through shared memory, ahead of the exponentials, so that both sides
 // share O;  warps 8-11 write a segment's result out while the next one runs.  The product P_g V_g has a barrier for even and one for odd
-// tiles, so that no reader is more than one phase behind.  A tile of 128 x 128 takes 1850 cycles (two threads to a row, all eight warps in the same
-// tile: 2000 and more): each side needs 3500 of them, 1730 for the exponentials, of which the special-function units are busy for 900; the rest are
-// round trips to barriers and TMEM (200 each) that two warps to a scheduler do not hide.
+// tiles, so that no reader is more than one phase behind.  Scores are read twice, 32 at a time in loops
+// that are not unrolled: the code has to fit (128 requests behind 8191 shared keys: 73 us; 64 at a time 80; unrolled, the next 32 on their way
+// while these are worked on, 93).  A tile of 128 x 128 takes about 1700 cycles (two threads to a row, all eight warps in the same tile: 2000 and more), of
+// which the exponentials keep the special-function units busy for 1000; the rest are round trips to barriers and TMEM (200 each) that two warps to
+// a scheduler do not hide.
 constexpr int PA_M = 128, PA_N = 128, PA_THREADS = 512, PA_MAX_BATCH = 1024, PA_LIST = 8;
 constexpr int PF_WARPS = 8, PF_STAGES = 3, PF_STAGE_BYTES = 8192, PF_KEPT_BYTES = 664;    // few rows: warps, tiles in a warp's ring, K and V of a tile
 template <int HD> constexpr int PF_KEYS_LOG2 = HD == 64 ? 5 : 4;       // keys of such a tile
@@ -1024,7 +1026,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const float sl2 = p.a.scale * 1.4426950408889634f;
     const unsigned long long sl22 = f2_splat(sl2);
     float* xch = reinterpret_cast<float*>(smem + Cfg::OFF_X);     // a row's maximum in use, by the even or odd tile that has set it
-    int g = 0, sq = 0;
+    int g0 = 0, sq = 0;
 #pragma unroll 1
     while (ok && take(s, ok)) {
       let_go();
@@ -1032,36 +1034,32 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       float m_run = -INFINITY, l_run = 0.f;
       const uint32_t o_addr = t_lane + Cfg::TM_O + sq % Cfg::SETS * HD;
 #pragma unroll 1
-      for (int j = 0; j < s.tiles; ++j, ++g) {
-        if ((g & 1) != grp) continue;
+      for (int j = (g0 ^ grp) & 1; j < s.tiles; j += 2) {
+        const int g = g0 + j;
         const KeyTile kt = key_tile(p, s.flags, s.seen, s.tile + j);
-        // the scores are there, and P of the tile before the last has been used: its place is free
-        ok = mbar_wait(&s_full[grp], (g >> 1) & 1) && (g < 2 || mbar_wait(&o_done[grp], ((g - 2) >> 1) & 1));
-        ok = __all_sync(0xffffffffu, ok);
+        ok = warp_wait(&s_full[grp], (g >> 1) & 1);
         if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
         tc_fence_after();
         // columns up to `last` are seen: the keys that there are, and of a request's own keys those up to the row's token
         const int last = kt.prompt ? kt.count - 1 : min(kt.count - 1, s.shift + i_row - kt.first);
         const bool cut = (kt.prompt ? kt.count - 1 : min(kt.count - 1, s.shift - kt.first)) < PA_N - 1;
-        const auto scores = [&](uint32_t* sv, int c0) {           // 64 of them, -inf for those that are not seen
-          tmem_ld32(s_addr + c0, sv);
-          tmem_ld32(s_addr + c0 + 32, sv + 32);
-          tmem_ld_wait();
-          const int lim = last - c0;
-          if (cut && __any_sync(0xffffffffu, lim < 63)) {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) sv[i] = i <= lim ? sv[i] : 0xff800000u;
-          }
-        };
         float mx = -INFINITY;
         if (live) {
 #pragma unroll 1
-          for (int c0 = 0; c0 < PA_N; c0 += 64) {
-            uint32_t sv[64];
-            scores(sv, c0);
+          for (int c0 = 0; c0 < PA_N; c0 += 32) {
+            uint32_t sv[32];
+            tmem_ld32(s_addr + c0, sv);
+            tmem_ld_wait();
+            if (cut) {                                            // -inf for those that are not seen, here and for the weights
+              const int lim = last - c0;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) sv[i] = i <= lim ? sv[i] : 0xff800000u;
+              tmem_st32(s_addr + c0, sv);
+              tmem_st_wait();
+            }
             float m1 = __uint_as_float(sv[0]);
 #pragma unroll
-            for (int i = 0; i < 64; i += 4) {
+            for (int i = 0; i < 32; i += 4) {
               mx = fmax3(mx, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
               m1 = fmax3(m1, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
             }
@@ -1069,8 +1067,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           }
         }
         // the maximum in use goes from tile to tile: from the other warps' to this one, and on
-        if (g > 0) ok = warp_wait(&m_there[(grp ^ 1) * 4 + quad], ((g - 1) >> 1) & 1);
-        if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); break; }
+        ok = g == 0 || mbar_wait(&m_there[(grp ^ 1) * 4 + quad], ((g - 1) >> 1) & 1);
         const float m_old = j == 0 ? -INFINITY : xch[(grp ^ 1) * PA_M + r];
         const float m_new = fmaxf(m_old, mx * sl2);
         const bool grow = r < s.rows && (m_new - m_old) > PA_RESCALE;           // the first time: from -inf.  Not for rows that are not there, whose scores are anything
@@ -1078,30 +1075,36 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         xch[grp * PA_M + r] = m_cand;
         __syncwarp();
         if (lane == 0) mbar_arrive(&m_there[grp * 4 + quad]);
-        if (live) {
+        // P of the tile before the last has been used: its place is free
+        ok = ok && (g < 2 || mbar_wait(&o_done[grp], ((g - 2) >> 1) & 1));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); break; }
+        tc_fence_after();
+        if (!live) {
+          if (lane == 0) mbar_arrive(&s_free[grp]);
+        } else {
           const float m_use = m_cand == -INFINITY ? 0.f : m_cand; // a row that has seen nothing yet
           const unsigned long long neg_m = f2_splat(-m_use);
           unsigned long long l01 = 0, l23 = 0;
 #pragma unroll 1
-          for (int c0 = 0; c0 < PA_N; c0 += 64) {
-            uint32_t sv[64], pk[32];
-            scores(sv, c0);
-            if (c0 + 64 == PA_N) {                                // all have been read
+          for (int c0 = 0; c0 < PA_N; c0 += 32) {
+            uint32_t sv[32], pk[16];
+            tmem_ld32(s_addr + c0, sv);
+            tmem_ld_wait();
+            if (c0 + 32 == PA_N) {                                // all have been read
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&s_free[grp]);
             }
 #pragma unroll
-            for (int i = 0; i < 64; i += 4) {
-              const unsigned long long x01 = f2_fma(f2_of(sv[i], sv[i + 1]), sl22, neg_m), x23 = f2_fma(f2_of(sv[i + 2], sv[i + 3]), sl22, neg_m);
-              // one of eight pairs on the multiply-add pipe: the special-function units are what a full tile waits for
-              const unsigned long long e01 = exp2_mufu2(x01), e23 = (i >> 2) % 4 == 0 ? exp2_fma2(x23) : exp2_mufu2(x23);
+            for (int i = 0; i < 32; i += 4) {
+              const unsigned long long e01 = exp2_mufu2(f2_fma(f2_of(sv[i], sv[i + 1]), sl22, neg_m)), e23 = exp2_mufu2(f2_fma(f2_of(sv[i + 2], sv[i + 3]), sl22, neg_m));
               l01 = f2_add(l01, e01);
               l23 = f2_add(l23, e23);
               pk[i >> 1] = f2_bf16(e01);                          // weights to bf16, as the tensor cores take them; their sum stays fp32
               pk[(i >> 1) + 1] = f2_bf16(e23);
             }
-            tmem_st32(p_addr + (c0 >> 1), pk);
+            tmem_st16(p_addr + (c0 >> 1), pk);
           }
           uint32_t a, b;
           f2_to(f2_add(l01, l23), a, b);
@@ -1124,8 +1127,6 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           }
           tmem_st_wait();
           tc_fence_before();
-        } else if (lane == 0) {
-          mbar_arrive(&s_free[grp]);
         }
         if (kt.count < PA_N) {                                    // values that no key goes with: zeros, whatever lies there
           const int st = g % NV;
@@ -1151,6 +1152,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       __syncwarp();
       if (lane == 0) mbar_arrive(&seg_done[sq & 1]);
       ++sq;
+      g0 += s.tiles;
     }
   } else {
     // ---------------------------------------------------------------- results: warp 8 + q has TMEM lanes 32 q..

@@ -743,7 +743,8 @@ __device__ __forceinline__ void few_rows(const PagedTcParams& p, uint8_t* rings,
   }
 }
 
-template <int HD>
+// NT: 1, or 2 where some item may have 9 to 16 rows (the registers of which, at head dim 128, spill: 3% of a call that does without)
+template <int HD, int NT>
 __global__ void __launch_bounds__(PA_THREADS, 1)
 paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQown, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKfew, const __grid_constant__ CUtensorMap tmVfew,
@@ -835,10 +836,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     if (warp >= PF_WARPS) {
       few_loads<HD>(p, &tmKfew, &tmVfew, smem + (warp - PF_WARPS) * (PF_STAGES * PF_STAGE_BYTES), all[warp - PF_WARPS], warp - PF_WARPS, tiles_before, items_before,
                     on_prompt, from, to);
-    } else if (few == 8) {
+    } else if (NT == 1 || few == 8) {
       few_rows<HD, 1>(p, smem, all, on_prompt, cta, from, to);
     } else {
-      few_rows<HD, 2>(p, smem, all, on_prompt, cta, from, to);
+      few_rows<HD, NT>(p, smem, all, on_prompt, cta, from, to);
     }
     return;
   }
@@ -1396,9 +1397,10 @@ static PagedTcPlan plan_tc(int tokens, int batch, int max_fresh, int q_heads, in
   c.ts = max_fresh < c.tpt ? (max_fresh > 0 ? max_fresh : 1) : c.tpt;
   c.tb = tokens < c.tpt ? tokens : c.tpt;
   const int few_log2 = head_dim == 64 ? PF_KEYS_LOG2<64> : PF_KEYS_LOG2<128>;
-  const auto few = [&](int rows) { return rows > PF_ROWS ? 0 : rows <= 8 ? 8 : 16; };
+  const auto few = [&](int rows) { return rows > PF_ROWS ? 0 : rows <= 8 ? 8 : 16; };       // own keys, 32 requests of 2048, heads of 128: 22.7 us, 25.6 as tiles
   c.few = few(c.ts * c.group);
-  c.few_prompt = few(c.tb * c.group);
+  // 16 requests, 32 heads of 128, behind 4096 shared keys: 36 us with few rows, 30 without; heads of 64, 4000: 22 and 26
+  c.few_prompt = head_dim == 128 && c.tb * c.group > 8 ? 0 : few(c.tb * c.group);
   c.own_log2 = c.few ? few_log2 : 7;
   c.prefix_row_tiles = (tokens + c.tpt - 1) / c.tpt;
   // The prompt for the whole batch at once where that reads it at most half as often as request by request, and always where a request has few rows.
@@ -1437,7 +1439,9 @@ static int launch_tc(const PagedAttnParams& a, void* scratch, int* status, cudaS
   using Cfg = PaCfg<HD>;
   static bool set = false;
   if (!set) {
-    if (cudaFuncSetAttribute(paged_attn_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES) != cudaSuccess) return OA_ERR_LAUNCH;
+    if (cudaFuncSetAttribute(paged_attn_tc_kernel<HD, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES) != cudaSuccess ||
+        cudaFuncSetAttribute(paged_attn_tc_kernel<HD, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES) != cudaSuccess)
+      return OA_ERR_LAUNCH;
     set = true;
   }
   const PagedTcPlan c = plan_tc(a.tokens, a.batch, a.max_fresh, a.q_heads, a.kv_heads, HD, a.prefix_len);
@@ -1477,7 +1481,8 @@ static int launch_tc(const PagedAttnParams& a, void* scratch, int* status, cudaS
     const uint32_t fewer[3] = {64, 1u << PF_KEYS_LOG2<HD>, 1};
     if ((rc = make_tmap_box3_bf16(&tkf, a.k, dims, ks, fewer)) || (rc = make_tmap_box3_bf16(&tvf, a.v, dims, vs, fewer))) return rc;
   }
-  launch_short(paged_attn_tc_kernel<HD>, dim3((unsigned)c.grid), dim3(PA_THREADS), Cfg::SMEM_BYTES, st, tq, tqo, tk, tv, tkf, tvf, p);
+  const auto kernel = c.few > 8 || (work > 0 && c.few_prompt > 8) ? paged_attn_tc_kernel<HD, 2> : paged_attn_tc_kernel<HD, 1>;
+  launch_short(kernel, dim3((unsigned)c.grid), dim3(PA_THREADS), Cfg::SMEM_BYTES, st, tq, tqo, tk, tv, tkf, tvf, p);
   if (c.joint) launch_short(paged_join_cuts_kernel<HD>, dim3((unsigned)c.grid), dim3(256), 0, st, p);
   else {
     const long long rows = (long long)a.tokens * a.q_heads, rows_of_block = 1024 / HD;

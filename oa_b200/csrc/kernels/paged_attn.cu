@@ -1299,8 +1299,11 @@ __global__ void __launch_bounds__(256) paged_join_rows_kernel(const __grid_const
   const int prt = t / p.tpt, p_item = h * p.prefix_row_tiles + prt, pa = p_item * p.prefix_tiles, p_first = pa / per_prompt;
   const int p_count = own.inner >= 0 && p.prefix_tiles > 0 ? min((pa + p.prefix_tiles - 1) / per_prompt - p_first + 1, p.ctas) : 0;
   const int a = own.pos + h * own.all, first = a / per, count = own.inner >= 0 && own.tiles > 0 ? min((a + own.tiles - 1) / per - first + 1, p.ctas) : 0;
-  const long long p_row = prompt_row(p, (long long)p_item + p_first) + (t - prt * p.tpt) * p.group + head;
-  const long long o_row = own_row(p, (long long)own.item + h * own.row_tiles + first) + own.inner * p.group + head;
+  // rows of the scratch, which is far from 2^31 of them
+  const int p_step = p.tb * p.group, o_step = p.ts * p.group, room = (int)p.part_rows;
+  int at = (p_item + p_first) * p_step + (t - prt * p.tpt) * p.group + head;     // the next piece's row
+  const int o_row = (int)p.own_slot0 + (own.item + h * own.row_tiles + first) * o_step + own.inner * p.group + head;
+  if (p_count == 0) at = o_row;
   float m = -INFINITY, l = 0.f, acc[4] = {};
 #pragma unroll 1
   for (int k0 = 0; k0 < p_count + count; k0 += AT_ONCE) {
@@ -1308,13 +1311,13 @@ __global__ void __launch_bounds__(256) paged_join_rows_kernel(const __grid_const
     float4 v[AT_ONCE];
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k) {
-      const long long at = k0 + k < p_count ? prompt_row(p, k0 + k) + p_row : own_row(p, k0 + k - p_count) - p.own_slot0 + o_row;
       ml[k] = make_float2(-INFINITY, 0.f);
       v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (k0 + k < p_count + count && has_room(p, at)) {
+      if (k0 + k < p_count + count && at >= 0 && at < room) {
         ml[k] = p.ml[at];
-        v[k] = *reinterpret_cast<const float4*>(p.part + at * HD + x);
+        v[k] = *reinterpret_cast<const float4*>(p.part + (long long)at * HD + x);
       }
+      at = k0 + k + 1 == p_count ? o_row : at + (k0 + k + 1 < p_count ? p_step : o_step);
     }
     float top = m;
 #pragma unroll
@@ -1367,7 +1370,8 @@ __global__ void __launch_bounds__(256) paged_join_cuts_kernel(const __grid_const
       for (int hq = warp; hq < p.a.q_heads; hq += 8) RowJoin<HD>().write(p, (int)t, hq, lane);
   };
   for (int b = blockIdx.x; b < p.a.batch; b += gridDim.x) zero((long long)p.a.starts[b] + p.a.max_fresh, p.a.starts[b + 1]);
-  const long long behind = p.a.batch > 0 ? max(p.a.starts[p.a.batch], 0) : 0, rest = max((long long)p.a.tokens - behind, 0ll), share = (rest + gridDim.x - 1) / gridDim.x;
+  const int behind = p.a.batch > 0 ? max(p.a.starts[p.a.batch], 0) : 0;
+  const long long share = ((unsigned)max(p.a.tokens - behind, 0) + gridDim.x - 1) / gridDim.x;
   zero(behind + blockIdx.x * share, behind + (blockIdx.x + 1) * share);
   if (blockIdx.x == 0 && p.a.batch > 0) zero(0, p.a.starts[0]);
 }

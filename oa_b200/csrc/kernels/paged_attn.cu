@@ -1467,23 +1467,22 @@ static int launch_tc(const PagedAttnParams& a, void* scratch, int* status, cudaS
   p.part_rows = c.prompt_rows + c.own_rows;
   p.ctas = c.grid;
   p.status = status;
-  CUtensorMap tq, tqo, tk, tv, tkf, tvf;
+  // descriptors of what the call's kinds of CTAs load; the others' are never used
+  CUtensorMap tq = {}, tqo = {}, tk = {}, tv = {}, tkf = {}, tvf = {};
   int rc;
-  {
-    const uint64_t dims[3] = {HD, (uint64_t)a.q_heads, (uint64_t)a.tokens}, strides[2] = {HD * 2, (uint64_t)a.q_stride * 2};
-    const uint32_t box[3] = {64, (uint32_t)c.group, (uint32_t)c.tb}, own[3] = {64, (uint32_t)c.group, (uint32_t)c.ts};
-    if ((rc = make_tmap_box3_bf16(&tq, a.q, dims, strides, box)) || (rc = make_tmap_box3_bf16(&tqo, a.q, dims, strides, own))) return rc;
-  }
   const uint64_t packed = (uint64_t)a.kv_heads * ps * HD;
   const uint64_t dims[3] = {HD, (uint64_t)a.kv_heads * ps, (uint64_t)a.pages};
-  const uint32_t box[3] = {64, (uint32_t)ps, 1};
   const uint64_t ks[2] = {HD * 2, (a.pages > 1 ? (uint64_t)a.k_page_stride : packed) * 2}, vs[2] = {HD * 2, (a.pages > 1 ? (uint64_t)a.v_page_stride : packed) * 2};
-  if ((rc = make_tmap_box3_bf16(&tk, a.k, dims, ks, box)) || (rc = make_tmap_box3_bf16(&tv, a.v, dims, vs, box))) return rc;
-  tkf = tk;
-  tvf = tv;
-  if (ps > 1 << PF_KEYS_LOG2<HD>) {                                // boxes of a tile's keys, where a page has more
-    const uint32_t fewer[3] = {64, 1u << PF_KEYS_LOG2<HD>, 1};
-    if ((rc = make_tmap_box3_bf16(&tkf, a.k, dims, ks, fewer)) || (rc = make_tmap_box3_bf16(&tvf, a.v, dims, vs, fewer))) return rc;
+  if (p.many) {
+    const uint64_t q_dims[3] = {HD, (uint64_t)a.q_heads, (uint64_t)a.tokens}, strides[2] = {HD * 2, (uint64_t)a.q_stride * 2};
+    const uint32_t box[3] = {64, (uint32_t)c.group, (uint32_t)c.tb}, own[3] = {64, (uint32_t)c.group, (uint32_t)c.ts}, page[3] = {64, (uint32_t)ps, 1};
+    if ((rc = make_tmap_box3_bf16(&tq, a.q, q_dims, strides, box)) || (rc = make_tmap_box3_bf16(&tqo, a.q, q_dims, strides, own)) ||
+        (rc = make_tmap_box3_bf16(&tk, a.k, dims, ks, page)) || (rc = make_tmap_box3_bf16(&tv, a.v, dims, vs, page)))
+      return rc;
+  }
+  if (c.few || c.few_prompt) {                                     // a tile's keys, or a page's where it has fewer
+    const uint32_t box[3] = {64, (uint32_t)(ps < 1 << PF_KEYS_LOG2<HD> ? ps : 1 << PF_KEYS_LOG2<HD>), 1};
+    if ((rc = make_tmap_box3_bf16(&tkf, a.k, dims, ks, box)) || (rc = make_tmap_box3_bf16(&tvf, a.v, dims, vs, box))) return rc;
   }
   const auto kernel = c.few > 8 || (work > 0 && c.few_prompt > 8) ? paged_attn_tc_kernel<HD, 2> : paged_attn_tc_kernel<HD, 1>;
   launch_short(kernel, dim3((unsigned)c.grid), dim3(PA_THREADS), Cfg::SMEM_BYTES, st, tq, tqo, tk, tv, tkf, tvf, p);

@@ -45,10 +45,15 @@ def _int32(what: str, *tensors: torch.Tensor) -> None:
 
 def _table(what: str, tables: torch.Tensor, batch: int):
     """(width, elements between rows) of a table of `batch` rows."""
-    if tables.dtype is not _I32 or tables.dim() != 2:
+    return _table_layout(what, tables.shape, tables.stride(), tables.dtype, batch)
+
+
+@functools.lru_cache(maxsize=256)
+def _table_layout(what: str, shape, stride, dtype, batch: int):
+    if dtype is not _I32 or len(shape) != 2:
         raise ValueError(f"{what}: tables must be int32 [{batch}, width]")
-    rows, width = tables.shape
-    step, unit = tables.stride()
+    rows, width = shape
+    step, unit = stride
     if rows != batch or (width > 1 and unit != 1) or (batch > 1 and step < width):
         raise ValueError(f"{what}: tables must be int32 [{batch}, width] with rows side by side")
     return width, step if batch > 1 else width
@@ -152,15 +157,18 @@ def release(done: torch.Tensor, lens: torch.Tensor, tables: torch.Tensor, free_p
     return now
 
 
-def _pool(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype):
-    """(pages, kv heads, page size, head dim, elements between pages of k, and of v)."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype is not dtype or v_pages.dtype is not dtype:
+# What follows from shapes, strides and types alone is worked out once for each of them: a step makes these calls for every layer, and the checks
+# took longer than the launch.
+@functools.lru_cache(maxsize=256)
+def _pool(what: str, shape, k_stride, v_shape, v_stride, k_dtype, v_dtype, dtype: torch.dtype):
+    """(pages, kv heads, page size, head dim, elements between pages of k, and of v) of a pool."""
+    if len(shape) != 4 or shape != v_shape or k_dtype is not dtype or v_dtype is not dtype:
         raise ValueError(f"{what}: k_pages and v_pages must be [pages, kv_heads, page_size, head_dim] of {dtype}")
-    pages, heads, ps, hd = k_pages.shape
+    pages, heads, ps, hd = shape
     if ps not in PAGE_SIZES:
         raise ValueError(f"{what}: a page holds one of {PAGE_SIZES} tokens, not {ps}")
-    k0, *k_in = k_pages.stride()
-    v0, *v_in = v_pages.stride()
+    k0, *k_in = k_stride
+    v0, *v_in = v_stride
     if k_in != [ps * hd, hd, 1] or v_in != k_in or (pages > 1 and min(k0, v0) < heads * ps * hd):
         raise ValueError(f"{what}: a page must be contiguous and pages must not overlap")
     return pages, heads, ps, hd, k0, v0
@@ -175,7 +183,7 @@ def append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, k_pa
     """New tokens' packed rows [tokens, (q_heads + 2 kv_heads) * head_dim] (row stride allowed): returns q [tokens, q_heads * head_dim], rotated by
     each token's own position (pairs j, j + head_dim / 2; theta <= 0: not rotated), and writes rotated k and v to their slots.  A slot that is
     not in the pool (-1) is left out."""
-    pages, kvh, ps, hd, k_step, v_step = _pool("append", k_pages, v_pages, qkv.dtype)
+    pages, kvh, ps, hd, k_step, v_step = _pool("append", k_pages.shape, k_pages.stride(), v_pages.shape, v_pages.stride(), k_pages.dtype, v_pages.dtype, qkv.dtype)
     tokens, width = qkv.shape if qkv.dim() == 2 else (-1, 0)
     qh = width // hd - 2 * kvh
     if tokens < 0 or width % hd or qh < 1:
@@ -213,23 +221,16 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tab
     starts[b] .. starts[b + 1], at most `max_fresh`) sees the whole shared prompt, `prefix_len` keys in the pages of `prefix_table`, and the
     first lens[b] - n + i + 1 keys of its own pages.  q_heads is a multiple of kv_heads.  Returns [tokens, q_heads * head_dim] and, with
     return_lse, also the natural log-sum-exp [tokens, q_heads] fp32.  Rows that see nothing, and rows of no request, are 0 (-inf)."""
-    pages, kvh, ps, hd, k_step, v_step = _pool("attention", k_pages, v_pages, q.dtype)
-    tokens, cols = q.shape if q.dim() == 2 else (0, 0)
-    if cols == 0 or cols % (hd * kvh):
-        raise ValueError(f"attention: q must be [tokens, q_heads * {hd}] with q_heads a multiple of {kvh}")
-    qh, batch = cols // hd, lens.numel()
-    if starts.numel() != batch + 1 or max_fresh < 0 or prefix_len < 0:
-        raise ValueError("attention: starts has one entry more than lens; max_fresh and prefix_len are not negative")
+    batch = lens.numel()
+    (pages, kvh, ps, hd, k_step, v_step, tokens, cols, qh, width, table_stride, scale, need) = _attention_layout(
+        q.shape, q.dtype, k_pages.shape, k_pages.stride(), v_pages.shape, v_pages.stride(), k_pages.dtype, v_pages.dtype, tables.shape, tables.stride(),
+        tables.dtype, batch, starts.numel(), max_fresh, None if prefix_table is None else prefix_table.numel(), prefix_len, scale, q.is_cuda)
     if prefix_len > 0:
-        if prefix_table is None or prefix_table.numel() * ps < prefix_len:
-            raise ValueError(f"attention: prefix_table holds fewer than {prefix_len} tokens")
         _int32("attention", lens, starts, prefix_table)
         _same_device("attention", q, k_pages, v_pages, tables, lens, starts, prefix_table)
     else:
         _int32("attention", lens, starts)
         _same_device("attention", q, k_pages, v_pages, tables, lens, starts)
-    width, table_stride = _table("attention", tables, batch)
-    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
     if not q.is_cuda:
         return _attention_cpu(q, k_pages, v_pages, tables, lens, starts, max_fresh, prefix_table, prefix_len, scale, return_lse)
     q, q_step = _aligned_rows(q, tokens, cols)
@@ -237,7 +238,6 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tab
     lse = torch.empty_strided((tokens, qh), (qh, 1), dtype=torch.float32, device=q.device) if return_lse else None
     code = K.dt(q)
     # scratch of the call's own: calls on several streams do not meet in it
-    need = _scratch_bytes(code, tokens, batch, max_fresh, qh, kvh, hd, pages, prefix_len, scale)
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     K._launch(N.require().oa_paged_attn(code, q.data_ptr(), q_step, k_pages.data_ptr(), v_pages.data_ptr(), k_step, v_step, tables.data_ptr(), table_stride,
                                         lens.data_ptr(), starts.data_ptr(), N.ptr(prefix_table), prefix_len, out.data_ptr(), N.ptr(lse), tokens, batch,
@@ -247,8 +247,24 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tab
 
 
 @functools.lru_cache(maxsize=256)
-def _scratch_bytes(*sizes) -> int:
-    return N.require().oa_paged_attn_scratch_bytes(*sizes)
+def _attention_layout(q_shape, dtype, k_shape, k_stride, v_shape, v_stride, k_dtype, v_dtype, t_shape, t_stride, t_dtype, batch, n_starts, max_fresh, n_prefix,
+                      prefix_len, scale, cuda):
+    """The checks of `attention`; (.. of the pool, tokens, columns, query heads, table width and row stride, scale, bytes of scratch)."""
+    pool = _pool("attention", k_shape, k_stride, v_shape, v_stride, k_dtype, v_dtype, dtype)
+    pages, kvh, ps, hd = pool[:4]
+    tokens, cols = q_shape if len(q_shape) == 2 else (0, 0)
+    if cols == 0 or cols % (hd * kvh):
+        raise ValueError(f"attention: q must be [tokens, q_heads * {hd}] with q_heads a multiple of {kvh}")
+    if n_starts != batch + 1 or max_fresh < 0 or prefix_len < 0:
+        raise ValueError("attention: starts has one entry more than lens; max_fresh and prefix_len are not negative")
+    if prefix_len > 0 and (n_prefix is None or n_prefix * ps < prefix_len):
+        raise ValueError(f"attention: prefix_table holds fewer than {prefix_len} tokens")
+    width, table_stride = _table_layout("attention", t_shape, t_stride, t_dtype, batch)
+    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+    qh = cols // hd
+    code = K._DT.get(dtype) if cuda else None
+    need = N.require().oa_paged_attn_scratch_bytes(code, tokens, batch, max_fresh, qh, kvh, hd, pages, prefix_len, scale) if code is not None else 0
+    return (*pool, tokens, cols, qh, width, table_stride, scale, need)
 
 
 def _attention_cpu(q, k_pages, v_pages, tables, lens, starts, max_fresh, prefix_table, prefix_len, scale, return_lse):

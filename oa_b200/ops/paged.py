@@ -48,7 +48,6 @@ def _table(what: str, tables: torch.Tensor, batch: int):
     return _table_layout(what, tables.shape, tables.stride(), tables.dtype, batch)
 
 
-@functools.lru_cache(maxsize=256)
 def _table_layout(what: str, shape, stride, dtype, batch: int):
     if dtype is not _I32 or len(shape) != 2:
         raise ValueError(f"{what}: tables must be int32 [{batch}, width]")

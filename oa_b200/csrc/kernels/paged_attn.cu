@@ -1342,8 +1342,8 @@ __global__ void __launch_bounds__(256) paged_join_rows_kernel(const __grid_const
   if (p.a.lse && x == 0) p.a.lse[(long long)t * p.a.q_heads + hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-// Joint form: the items that a stretch's end cuts (block c: the one that begins in stretch c and goes beyond it), and zeros for the rows of
-// no request.
+// Joint form: the items that a stretch's end cuts (blocks (c, y): the one that begins in stretch c and goes beyond it, rows dealt to four blocks: four
+// requests of up to 2048 tokens 88 us, 112 with one), and zeros for the rows of no request.
 template <int HD>
 __global__ void __launch_bounds__(256) paged_join_cuts_kernel(const __grid_constant__ PagedTcParams p) {
   pdl_launch_dependents();
@@ -1355,7 +1355,7 @@ __global__ void __launch_bounds__(256) paged_join_cuts_kernel(const __grid_const
     Segment s;
     if (walk.next(s) && s.tile > 0 && s.tile <= per) {           // begins in this stretch (at its very first tile at the earliest)
       const int a = (int)cut - s.tile, last = (a + s.item_tiles - 1) / per, c0 = blockIdx.x;
-      for (int r = warp; r < s.tokens * p.group; r += 8) {
+      for (int r = blockIdx.y * 8 + warp; r < s.tokens * p.group; r += 8 * gridDim.y) {
         RowJoin<HD> join;
         join.add(p, last - c0 + 1, [&](int k) -> long long {      // the piece is the first of its CTA, but for an item that begins inside
           return own_row(p, 2ll * (c0 + k) + ((long long)(c0 + k) * per >= a ? 0 : 1)) + r;
@@ -1365,6 +1365,7 @@ __global__ void __launch_bounds__(256) paged_join_cuts_kernel(const __grid_const
       }
     }
   }
+  if (blockIdx.y > 0) return;
   const auto zero = [&](long long from, long long to) {
     for (long long t = max(from, 0ll); t < min(to, (long long)p.a.tokens); ++t)
       for (int hq = warp; hq < p.a.q_heads; hq += 8) RowJoin<HD>().write(p, (int)t, hq, lane);
@@ -1407,8 +1408,10 @@ static PagedTcPlan plan_tc(int tokens, int batch, int max_fresh, int q_heads, in
   c.few_prompt = head_dim == 128 && c.tb * c.group > 8 ? 0 : few(c.tb * c.group);
   c.own_log2 = c.few ? few_log2 : 7;
   c.prefix_row_tiles = (tokens + c.tpt - 1) / c.tpt;
-  // The prompt for the whole batch at once where that reads it at most half as often as request by request, and always where a request has few rows.
-  c.joint = !c.few && (prefix_len == 0 || 2ll * c.prefix_row_tiles > batch);
+  // With a prompt, its keys and a request's own in one item only where requests fill many query tiles: results need not be joined then, but the
+  // prompt is read by each request's (4 requests of up to 512 tokens behind 2048: 57 us, 61 apart; 8 of up to 128: 47 and 45; 24 of up to 48
+  // behind 1001: 58 and 52; 64 of up to 16 behind 4000: 141 and 107).
+  c.joint = !c.few && (prefix_len == 0 || c.prefix_row_tiles > 4ll * batch);
   const int prefix_log2 = c.few_prompt && !c.joint ? few_log2 : 7;
   c.prefix_tiles = (int)(((long long)prefix_len + (1 << prefix_log2) - 1) >> prefix_log2);
   c.grid = sm_count();
@@ -1486,7 +1489,7 @@ static int launch_tc(const PagedAttnParams& a, void* scratch, int* status, cudaS
   }
   const auto kernel = c.few > 8 || (work > 0 && c.few_prompt > 8) ? paged_attn_tc_kernel<HD, 2> : paged_attn_tc_kernel<HD, 1>;
   launch_short(kernel, dim3((unsigned)c.grid), dim3(PA_THREADS), Cfg::SMEM_BYTES, st, tq, tqo, tk, tv, tkf, tvf, p);
-  if (c.joint) launch_short(paged_join_cuts_kernel<HD>, dim3((unsigned)c.grid), dim3(256), 0, st, p);
+  if (c.joint) launch_short(paged_join_cuts_kernel<HD>, dim3((unsigned)c.grid, 4), dim3(256), 0, st, p);
   else {
     const long long rows = (long long)a.tokens * a.q_heads, rows_of_block = 1024 / HD;
     launch_short(paged_join_rows_kernel<HD>, dim3((unsigned)((rows + rows_of_block - 1) / rows_of_block)), dim3(256), 0, st, p);

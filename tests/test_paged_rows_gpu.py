@@ -45,3 +45,11 @@ def test_pieces_of_unequal_length_in_both_forms(hd):
         _check_attention("cuda", torch.bfloat16, lens, fresh, 8, 2, hd, 32, prefix)
         _check_attention("cuda", torch.bfloat16, [n % 200 + 24 for n in lens * 4], [f % 24 for f in fresh * 4], 8, 2, hd, 32, prefix)
     K.check_status()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("fresh,lens,prefix", [([700], [700], 0), ([300, 150], [300, 500], 200), ([513], [900], 129), ([260, 0], [260, 0], 1), ([1, 640], [1, 640], 77)])
+def test_long_pieces_of_few_requests(hd, fresh, lens, prefix):
+    _check_attention("cuda", torch.bfloat16, lens, fresh, 8, 2, hd, 16, prefix, room=5)
+    _check_attention("cuda", torch.bfloat16, lens, fresh, 3, 3, hd, 128, prefix)
+    K.check_status()

@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(128) paged_attn_rows_kernel(const PagedAttnPar
 // which the exponentials keep the special-function units busy for 1000; the rest are round trips to barriers and TMEM (200 each) that two warps to
 // a scheduler do not hide.
 constexpr int PA_M = 128, PA_N = 128, PA_THREADS = 512, PA_MAX_BATCH = 1024, PA_LIST = 8;
-constexpr int PF_WARPS = 8, PF_STAGES = 3, PF_STAGE_BYTES = 8192, PF_KEPT_BYTES = 664;    // few rows: warps, tiles in a warp's ring, K and V of a tile
+constexpr int PF_WARPS = 8, PF_STAGES = 3, PF_STAGE_BYTES = 8192, PF_KEPT_BYTES = 792;    // few rows: warps, tiles in a warp's ring, K and V of a tile
 template <int HD> constexpr int PF_KEYS_LOG2 = HD == 64 ? 5 : 4;       // keys of such a tile
 constexpr int PF_ROWS = 16;                                             // and the most rows: what a thread's registers hold
 constexpr float PA_RESCALE = 8.f;          // log2: the running maximum is let be while rows grow by less
@@ -201,6 +201,7 @@ struct PagedTcParams {
   int few, few_prompt;                     // few rows: 8 or 16, the most of an item; or 0
   int many;                                // some CTA has a tile of more rows
   int own_log2;                            // keys of a tile of a request's own
+  int over;                                // what an item of a request's own costs beside its tiles, in tiles
   int joint, prefix_tiles, prefix_row_tiles, prefix_work;   // prefix_work: key tiles of all prompt items (shared form)
   float* part;                             // partial o: [prompt slots][tb * group][HD], then [own slots][ts * group][HD]
   float2* ml;                              // their (m, l), m in units of log2
@@ -237,6 +238,12 @@ __device__ __forceinline__ int tiles_of(const PagedTcParams& p, const Request& r
   return p.joint ? max(p.prefix_tiles + own, 1) : own;
 }
 
+// what the item counts in a stretch: units in front that are no tiles, and its tiles
+__device__ __forceinline__ int units_of(const PagedTcParams& p, const Request& r, int rt) {
+  const int tiles = tiles_of(p, r, rt);
+  return tiles > 0 ? tiles + p.over : 0;
+}
+
 struct Segment {
   int prompt, h, b, rt;                    // of the prompt's items: rt counts tiles of the whole batch
   int tile, tiles;                         // first key tile inside the item, how many
@@ -245,19 +252,20 @@ struct Segment {
 };
 
 // How the tiles are dealt: CTAs [0, prompt_ctas) have stretches of `per_prompt` of the prompt's, the others of `per` of the requests'
-// each.  With both there, in proportion to what they cost, relative to a tile of 128 keys and many rows: 128 keys of few rows, which wait for memory, and
-// what comes with an item (0.2 and 0.45 for the first, 0.1 and 0.2 for the second: up to 15% slower at 32 to 128 requests).
-constexpr float PA_COST_FEW = 0.35f, PA_COST_ITEM = 0.4f;
+// each, in which an item counts some tiles more than it has (`over`) for its beginning and its end (few rows 3, many 1, against none: 32 requests 32.2
+// and 33.6 us, 128 70.8 and 73.9, ragged pieces 37.4 and 39.4).  With both there, CTAs are dealt in proportion to what the tiles cost: 128 keys of few rows,
+// which wait for memory, relative to a tile of 128 keys and many rows (0.31 and 0.4: up to 4% slower at 32 to 128 requests).
+constexpr float PA_COST_FEW = 0.37f;
 struct Stretches { int prompt_ctas, per_prompt, per, own_work; };
 template <int HD>
-__device__ __forceinline__ Stretches stretches_of(const PagedTcParams& p, int own_work, int own_items, int ctas) {
+__device__ __forceinline__ Stretches stretches_of(const PagedTcParams& p, int own_work, int ctas) {
   Stretches d;
   d.own_work = own_work;
   d.prompt_ctas = 0;
   const float few = PA_COST_FEW * (1 << PF_KEYS_LOG2<HD>) / PA_N;      // of a tile of few rows
   if (p.prefix_work > 0) {
     const float prompt = (float)p.prefix_work * (p.few_prompt ? few : 1.f);
-    const float own = (float)own_work * (p.few ? few : 1.f) + (float)own_items * PA_COST_ITEM;
+    const float own = (float)own_work * (p.few ? few : 1.f);
     d.prompt_ctas = own_work > 0 ? min(max((int)((float)ctas * prompt / (prompt + own) + 0.5f), 1), ctas - 1) : ctas;
   }
   d.per_prompt = max((p.prefix_work + max(d.prompt_ctas, 1) - 1) / max(d.prompt_ctas, 1), 1);
@@ -270,11 +278,11 @@ struct Walk {
   const PagedTcParams& p;
   const int *tiles_before, *items_before;
   int pos, end;
-  int b, h, rt, tile;                      // own items: the next one and the tile in it
+  int b, h, rt, unit;                      // own items: the next one and the unit in it
   Request r;
   bool prompt, placed;
   __device__ __forceinline__ Walk(const PagedTcParams& p_, const int* tb, const int* ib, bool prompt_, int pos_, int end_)
-      : p(p_), tiles_before(tb), items_before(ib), pos(pos_), end(end_), b(0), h(0), rt(0), tile(0), prompt(prompt_), placed(false) {}
+      : p(p_), tiles_before(tb), items_before(ib), pos(pos_), end(end_), b(0), h(0), rt(0), unit(0), prompt(prompt_), placed(false) {}
   __device__ __forceinline__ int find() const {      // the last request whose tiles begin at or before pos
     int lo = 0, n = p.a.batch;
     const int per_head = pos / p.a.kv_heads;
@@ -292,8 +300,8 @@ struct Walk {
     h = off / all;
     off -= h * all;
     rt = 0;
-    for (int t = tiles_of(p, r, 0); off >= t && rt + 1 < r.row_tiles; t = tiles_of(p, r, rt)) { off -= t; ++rt; }
-    tile = off;
+    for (int t = units_of(p, r, 0); off >= t && rt + 1 < r.row_tiles; t = units_of(p, r, rt)) { off -= t; ++rt; }
+    unit = off;
     placed = true;
   }
   __device__ __forceinline__ bool next(Segment& s) {
@@ -308,37 +316,40 @@ struct Walk {
       s.t0 = s.rt * p.tpt;
       s.tokens = min(p.tpt, p.a.tokens - s.t0);
       s.b = s.n = s.own = s.seen = s.i0 = 0;
-    } else {
-      if (!placed) { const int at = find(); place(at, request_of(p, at)); }
-      while (rt >= r.row_tiles || tiles_of(p, r, rt) <= tile) {      // on to the next item that has tiles; there is one before `end`
-        tile = 0;
-        if (++rt >= r.row_tiles) {
-          rt = 0;
-          if (++h >= p.a.kv_heads || r.row_tiles == 0) {
-            h = 0;
-            if (++b >= p.a.batch) return false;
-            r = request_of(p, b);
-          }
+      s.tiles = min(s.item_tiles - s.tile, end - pos);
+      pos += s.tiles;
+      return true;
+    }
+    if (!placed) { const int at = find(); place(at, request_of(p, at)); }
+    while (rt >= r.row_tiles || units_of(p, r, rt) <= unit) {        // on to the next item that has tiles; there is one before `end`
+      unit = 0;
+      if (++rt >= r.row_tiles) {
+        rt = 0;
+        if (++h >= p.a.kv_heads || r.row_tiles == 0) {
+          h = 0;
+          if (++b >= p.a.batch) return false;
+          r = request_of(p, b);
         }
       }
-      s.prompt = 0;
-      s.h = h;
-      s.b = b;
-      s.rt = rt;
-      s.tile = tile;
-      s.item_tiles = tiles_of(p, r, rt);
-      s.item = items_before[b] * p.a.kv_heads + h * r.row_tiles + rt;
-      s.i0 = rt * p.tpt;
-      s.t0 = r.t0 + s.i0;
-      s.tokens = min(p.tpt, r.fresh - s.i0);
-      s.n = r.n;
-      s.own = r.own;
-      s.seen = seen_by(p, r, rt);
     }
-    s.tiles = min(s.item_tiles - s.tile, end - pos);
-    pos += s.tiles;
-    if (!s.prompt) tile += s.tiles;
-    return true;
+    s.prompt = 0;
+    s.h = h;
+    s.b = b;
+    s.rt = rt;
+    s.item_tiles = tiles_of(p, r, rt);
+    s.item = items_before[b] * p.a.kv_heads + h * r.row_tiles + rt;
+    s.i0 = rt * p.tpt;
+    s.t0 = r.t0 + s.i0;
+    s.tokens = min(p.tpt, r.fresh - s.i0);
+    s.n = r.n;
+    s.own = r.own;
+    s.seen = seen_by(p, r, rt);
+    const int step = min(s.item_tiles + p.over - unit, end - pos);
+    s.tile = max(unit - p.over, 0);
+    s.tiles = max(unit + step - p.over, 0) - s.tile;
+    pos += step;
+    unit += step;
+    return s.tiles > 0;                    // none: the stretch ends in front of the item's tiles
   }
 };
 
@@ -381,7 +392,7 @@ __device__ __forceinline__ void scan_batch(const PagedTcParams& p, int* tiles_be
     const Request r = request_of(p, b);
     tiles_before[b] = tiles;
     items_before[b] = items;
-    for (int rt = 0; rt < r.row_tiles; ++rt) tiles += tiles_of(p, r, rt);
+    for (int rt = 0; rt < r.row_tiles; ++rt) tiles += units_of(p, r, rt);
     items += r.row_tiles;
   }
   int it = tiles, ii = items;
@@ -432,7 +443,9 @@ __device__ __forceinline__ void mma_16816(float* c, const uint32_t* a, uint32_t 
 }
 
 // What a warp keeps in shared memory beside its ring.
-struct FewSegment { int tile, tiles, item, h, t0, rows, seen, shift; };          // shift: the row of token i sees own keys before shift + i
+// tiles: 0, no more; shift: the row of token i sees own keys before shift + i; flags: 1 begins in a warp before, 2 goes on in the next, 4 the slot of its last tile
+// is kept for its results
+struct FewSegment { int tile, tiles, item, h, t0, rows, seen, shift, flags, pad[3]; };
 struct FewPart { int rows, goes_on, at; float2 ml[PF_ROWS]; };                   // rows 0: none; `at`: where its o lies in the ring
 struct FewWarp {
   uint64_t full[PF_STAGES], empty[PF_STAGES], listed[8];
@@ -448,7 +461,7 @@ __device__ __forceinline__ int few_step(int x, int hole) {        // the next sl
   if (x == hole) x = x + 1 == PF_STAGES ? 0 : x + 1;
   return x;
 }
-// The loads of warp `warp`, by a warp beside it: chunks of up to 32 pages of a segment, the pages of the next chunk looked up while this one's
+// The loads of warp `warp`, whose part of the CTA's stretch [lo, hi) is an eighth, by a warp beside it: chunks of up to 32 pages of a segment, the pages of the next chunk looked up while this one's
 // tiles are loaded.
 template <int HD>
 __device__ __forceinline__ void few_loads(const PagedTcParams& p, const CUtensorMap* tmK, const CUtensorMap* tmV, uint8_t* ring, FewWarp& mine, int warp,
@@ -461,17 +474,21 @@ __device__ __forceinline__ void few_loads(const PagedTcParams& p, const CUtensor
   Walk walk(p, tiles_before, items_before, prompt, from, to);
   Chunk now{0, 0, 0, 0, 0}, then{0, 0, 0, 0, 0};
   int seg_h = 0, seg_b = 0, seg_tile = 0, seg_left = 0, seg_end = 0, seg_at = 0, used = 0, st = 0, hole = -1;
+  bool ended = false;
   int keeps = 0;                           // the tile whose slot the warp keeps, counted from 1; 0: none
   const auto fetch = [&](Chunk& c) {
     c.n = 0;
     if (seg_left == 0) {
-      Segment s;
-      if (!walk.next(s)) return;
+      Segment s{};
+      if (ended) return;
+      ended = !walk.next(s);
+      const bool front = seg_at == 0 && s.tile > 0 && from > lo, back = walk.pos == to && to < hi && s.tile + s.tiles < s.item_tiles, kept = front && walk.pos < to;
       if (lane == 0) {
-        mine.list[seg_at & 7] = FewSegment{s.tile, s.tiles, s.item, s.h, s.t0, s.tokens * p.group, s.seen, s.own - s.n + s.i0 + 1};
+        mine.list[seg_at & 7] = FewSegment{s.tile, ended ? 0 : s.tiles, s.item, s.h, s.t0, s.tokens * p.group, s.seen, s.own - s.n + s.i0 + 1, (front ? 1 : 0) | (back ? 2 : 0) | (kept ? 4 : 0)};
         mbar_arrive(&mine.listed[seg_at & 7]);
       }
-      if (seg_at == 0 && s.tile > 0 && from > lo && walk.pos < to) keeps = s.tiles;
+      if (ended) return;
+      if (kept) keeps = s.tiles;
       ++seg_at;
       seg_h = s.h; seg_b = s.b; seg_tile = s.tile; seg_left = s.tiles;
       seg_end = prompt ? p.a.prefix_len : s.seen;
@@ -523,24 +540,24 @@ __device__ __forceinline__ void few_loads(const PagedTcParams& p, const CUtensor
   }
 }
 
-// Warp `warp` of eight, NT groups of eight rows.  The CTA's stretch [lo, hi) is cut into a warp's parts.
+// Warp `warp` of eight, NT groups of eight rows.
 template <int HD, int NT>
-__device__ __forceinline__ void few_rows(const PagedTcParams& p, uint8_t* rings, FewWarp* all, bool prompt, int cta, int lo, int hi) {
+__device__ __forceinline__ void few_rows(const PagedTcParams& p, uint8_t* rings, FewWarp* all, bool prompt, int cta) {
   constexpr int UL = PF_KEYS_LOG2<HD>, U = 1 << UL, MT = U / 16, KC = HD / 16, KV = U * HD * 2, PER = HD / 32;
   static_assert(2 * KV == PF_STAGE_BYTES && NT * 8 * HD * 4 <= PF_STAGE_BYTES, "a tile of K and of V, or results");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, pair = (lane & 3) * 2;
   const float sl2 = p.a.scale * 1.4426950408889634f;
   uint8_t* ring = rings + warp * (PF_STAGES * PF_STAGE_BYTES);
   FewWarp& mine = all[warp];
-  const int part = (hi - lo + PF_WARPS - 1) / PF_WARPS, from = min(lo + warp * part, hi), to = min(from + part, hi);
-  int st = 0, pos = from, sg = 0, hole = -1;
+  int st = 0, sg = 0, hole = -1;
   uint32_t phases = 0;                     // a bit for each slot
   bool ok = true;
   if (lane == 0) mine.front.rows = mine.back.rows = 0;
 #pragma unroll 1
-  while (pos < to && ok) {
+  while (ok) {
     if (!warp_wait(&mine.listed[sg & 7], sg >> 3 & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
     const FewSegment s = mine.list[sg & 7];
+    if (s.tiles == 0) break;
     ++sg;
     uint32_t q[KC][NT][2];
 #pragma unroll
@@ -566,8 +583,7 @@ __device__ __forceinline__ void few_rows(const PagedTcParams& p, uint8_t* rings,
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[k][n][e] = 0.f;
     const int most = prompt ? p.a.prefix_len : s.seen, least = prompt ? most : min(s.shift, most);
-    const bool front = s.tile > 0 && pos == from && from > lo;                   // begins in a warp before
-    pos += s.tiles;
+    const bool front = s.flags & 1, back = s.flags & 2;
 #pragma unroll 1
     for (int j = 0; j < s.tiles; ++j) {
       const int k0 = (s.tile + j) << UL;
@@ -674,12 +690,11 @@ __device__ __forceinline__ void few_rows(const PagedTcParams& p, uint8_t* rings,
         }
       }
       __syncwarp();
-      if (j + 1 == s.tiles && front && pos < to) hole = st;      // this slot keeps the results that another warp joins
+      if (j + 1 == s.tiles && (s.flags & 4)) hole = st;          // this slot keeps the results that another warp joins
       else if (lane == 0) mbar_arrive(&mine.empty[st]);
       st = few_step(st, hole);
     }
     // Results: a segment that ends where another warp goes on waits for it in shared memory, the others go to scratch.
-    const bool back = pos == to && to < hi && s.tile + s.tiles < (prompt ? p.prefix_tiles : (s.seen + U - 1) >> UL);
     const long long at = prompt ? prompt_row(p, (long long)s.item + cta) : own_row(p, (long long)s.item + cta);
     FewPart& kept = front ? mine.front : mine.back;
     const int slot = front ? (hole >= 0 ? hole : 0) : (hole == 0 ? 1 : 0);       // of the ring, in which nothing is under way
@@ -802,7 +817,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   int own_tiles, own_items;
   scan_batch(p, tiles_before, items_before, s_warp_sums, own_tiles, own_items);
   __syncthreads();
-  const Stretches deal = stretches_of<HD>(p, own_tiles * p.a.kv_heads, own_items * p.a.kv_heads, gridDim.x);
+  const Stretches deal = stretches_of<HD>(p, own_tiles * p.a.kv_heads, gridDim.x);
   const bool on_prompt = (int)blockIdx.x < deal.prompt_ctas;
   const int cta = on_prompt ? blockIdx.x : blockIdx.x - deal.prompt_ctas, per = on_prompt ? deal.per_prompt : deal.per;
   const int work = on_prompt ? p.prefix_work : deal.own_work;
@@ -822,9 +837,9 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       for (int i = threadIdx.x; i < r.n; i += PA_THREADS) {
         if (r.t0 + i < 0 || r.t0 + i >= p.a.tokens) continue;
         const int rt = i / p.tpt;
-        PagedOwn o{tiles_before[b] * p.a.kv_heads, tiles_before[b + 1] - tiles_before[b], tiles_of(p, r, rt), items_before[b] * p.a.kv_heads + rt, r.row_tiles,
+        PagedOwn o{tiles_before[b] * p.a.kv_heads + p.over, tiles_before[b + 1] - tiles_before[b], tiles_of(p, r, rt), items_before[b] * p.a.kv_heads + rt, r.row_tiles,
                    i < r.fresh ? i - rt * p.tpt : -1, {0, 0}};
-        for (int k = 0; k < rt; ++k) o.pos += tiles_of(p, r, k);
+        for (int k = 0; k < rt; ++k) o.pos += units_of(p, r, k);
         p.owns[r.t0 + i] = o;
       }
     }
@@ -837,9 +852,9 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       few_loads<HD>(p, &tmKfew, &tmVfew, smem + (warp - PF_WARPS) * (PF_STAGES * PF_STAGE_BYTES), all[warp - PF_WARPS], warp - PF_WARPS, tiles_before, items_before,
                     on_prompt, from, to);
     } else if (NT == 1 || few == 8) {
-      few_rows<HD, 1>(p, smem, all, on_prompt, cta, from, to);
+      few_rows<HD, 1>(p, smem, all, on_prompt, cta);
     } else {
-      few_rows<HD, NT>(p, smem, all, on_prompt, cta, from, to);
+      few_rows<HD, NT>(p, smem, all, on_prompt, cta);
     }
     return;
   }
@@ -1383,7 +1398,7 @@ using namespace oa;
 
 // The sizes that follow from a call's arguments: which form, how many items there can be, what they need in scratch.
 struct PagedTcPlan {
-  int group, tpt, ts, tb, few, few_prompt, own_log2, joint, prefix_tiles, prefix_row_tiles, grid;
+  int group, tpt, ts, tb, few, few_prompt, own_log2, over, joint, prefix_tiles, prefix_row_tiles, grid;
   long long prompt_rows, own_rows, items;
   size_t o_bytes, owns_bytes, ml_bytes, bytes;
 };
@@ -1412,6 +1427,7 @@ static PagedTcPlan plan_tc(int tokens, int batch, int max_fresh, int q_heads, in
   // prompt is read by each request's (4 requests of up to 512 tokens behind 2048: 57 us, 61 apart; 8 of up to 128: 47 and 45; 24 of up to 48
   // behind 1001: 58 and 52; 64 of up to 16 behind 4000: 141 and 107).
   c.joint = !c.few && (prefix_len == 0 || c.prefix_row_tiles > 4ll * batch);
+  c.over = c.joint ? 0 : c.few ? 3 : 1;
   const int prefix_log2 = c.few_prompt && !c.joint ? few_log2 : 7;
   c.prefix_tiles = (int)(((long long)prefix_len + (1 << prefix_log2) - 1) >> prefix_log2);
   c.grid = sm_count();
@@ -1455,11 +1471,11 @@ static int launch_tc(const PagedAttnParams& a, void* scratch, int* status, cudaS
   const int ps = 1 << a.page_log2;
   const long long own_tiles = (((long long)a.width * ps) >> c.own_log2) + 1;
   const long long work = (c.joint ? 0 : (long long)a.kv_heads * c.prefix_row_tiles * c.prefix_tiles);
-  if (work + c.items * (own_tiles + c.prefix_tiles + 1) > 0x7fffffffll) return OA_ERR_TOO_LARGE;
+  if (work + c.items * (own_tiles + c.over + c.prefix_tiles + 1) > 0x7fffffffll) return OA_ERR_TOO_LARGE;
   PagedTcParams p;
   p.a = a;
   p.group = c.group; p.group_mul = 65536 / c.group + 1; p.tpt = c.tpt; p.ts = c.ts; p.tb = c.tb;
-  p.few = c.few; p.few_prompt = c.few_prompt; p.own_log2 = c.own_log2;
+  p.few = c.few; p.few_prompt = c.few_prompt; p.own_log2 = c.own_log2; p.over = c.over;
   p.many = !c.few || (work > 0 && !c.few_prompt);
   p.joint = c.joint; p.prefix_tiles = c.prefix_tiles; p.prefix_row_tiles = c.prefix_row_tiles; p.prefix_work = (int)work;
   p.part = static_cast<float*>(scratch);

@@ -1426,7 +1426,7 @@ static PagedTcPlan plan_tc(int tokens, int batch, int max_fresh, int q_heads, in
   // With a prompt, its keys and a request's own in one item only where requests fill many query tiles: results need not be joined then, but the
   // prompt is read by each request's (8 requests of up to 1000 tokens behind 500: 141 us, 201 apart; 2 of up to 4000 behind 2048: 178 and 197; 4 of
   // up to 512: 61 and 55; 64 of up to 16 behind 4000: 141 and 92).  Without a prompt always (32 of up to 300: 102 and 129).
-  c.joint = !c.few && (prefix_len == 0 || c.prefix_row_tiles > 10ll * batch);
+  c.joint = !c.few && (prefix_len == 0 || c.prefix_row_tiles > 9ll * batch);
   c.over = c.joint ? 0 : c.few ? 3 : 1;
   const int prefix_log2 = c.few_prompt && !c.joint ? few_log2 : 7;
   c.prefix_tiles = (int)(((long long)prefix_len + (1 << prefix_log2) - 1) >> prefix_log2);

@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(128) paged_attn_rows_kernel(const PagedAttnPar
 //   that a row is an eighth of an instruction and not 1/128 of a tile, and stay in registers: their exponentials turn into an operand of
 //   V^T P^T by a transpose among lanes.  128 requests behind 8191 shared keys with 1024 of their own on average, 8 key-value heads of 64, group 8:
 //   own keys arrive at 95 bytes a nanosecond and SM where 72 SMs take them, which is what the memory gives; a tcgen05 tile with 8 of its 128 rows
-//   alive took 3300 instructions and 0.75 us for 128 keys (46 bytes a nanosecond and SM), and the call 101 us where this made it 79.
+//   alive took 3300 instructions and 0.75 us for 128 keys (46 bytes a nanosecond and SM).  With all items as tiles of many rows: 109 us, 71 so; 32 requests 41.4
+//   and 32.3, 4 requests 22.8 and 19.8.
 //   More than 16 rows would need more registers than a thread has.
 //
 // Keys beyond a length are cut off from the scores by a select, and their values are overwritten by zeros before the product: what lies there
@@ -383,7 +384,7 @@ __device__ __forceinline__ int page_for(const PagedTcParams& p, const Listed& s,
 }
 
 // Prefix sums over the batch (a block of PA_THREADS): key tiles for one key-value head, and query tiles, before each request.
-__device__ __forceinline__ void scan_batch(const PagedTcParams& p, int* tiles_before, int* items_before, int* warp_sums, int& all_tiles, int& all_items) {
+__device__ __forceinline__ void scan_batch(const PagedTcParams& p, int* tiles_before, int* items_before, int* warp_sums, int& all_tiles) {
   constexpr int WARPS = PA_THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.a.batch + PA_THREADS - 1) / PA_THREADS, b0 = min(tid * per, p.a.batch), b1 = min(b0 + per, p.a.batch);
@@ -414,7 +415,6 @@ __device__ __forceinline__ void scan_batch(const PagedTcParams& p, int* tiles_be
   for (int b = b0; b < b1; ++b) { tiles_before[b] += bt; items_before[b] += bi; }
   if (tid == 0) { tiles_before[p.a.batch] = all_t; items_before[p.a.batch] = all_i; }
   all_tiles = all_t;
-  all_items = all_i;
 }
 
 // Where a partial result goes.  Shared form: every segment of every item, numbered by item + stretch (a segment begins where an item or a
@@ -814,8 +814,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       asm volatile("prefetch.global.L2 [%0];" ::"l"(p.a.tables + (long long)(i / lines) * p.a.table_stride + min(i % lines * 32, p.a.width - 1)));
     if (at * 32 < p.a.prefix_len >> p.a.page_log2) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.a.prefix_table + at * 32));
   }
-  int own_tiles, own_items;
-  scan_batch(p, tiles_before, items_before, s_warp_sums, own_tiles, own_items);
+  int own_tiles;
+  scan_batch(p, tiles_before, items_before, s_warp_sums, own_tiles);
   __syncthreads();
   const Stretches deal = stretches_of<HD>(p, own_tiles * p.a.kv_heads, gridDim.x);
   const bool on_prompt = (int)blockIdx.x < deal.prompt_ctas;
@@ -1417,9 +1417,9 @@ static PagedTcPlan plan_tc(int tokens, int batch, int max_fresh, int q_heads, in
   c.ts = max_fresh < c.tpt ? (max_fresh > 0 ? max_fresh : 1) : c.tpt;
   c.tb = tokens < c.tpt ? tokens : c.tpt;
   const int few_log2 = head_dim == 64 ? PF_KEYS_LOG2<64> : PF_KEYS_LOG2<128>;
-  const auto few = [&](int rows) { return rows > PF_ROWS ? 0 : rows <= 8 ? 8 : 16; };       // own keys, 32 requests of 2048, heads of 128: 22.7 us, 25.6 as tiles
+  const auto few = [&](int rows) { return rows > PF_ROWS ? 0 : rows <= 8 ? 8 : 16; };       // 32 requests of 2048, group 16, heads of 128: 19.0 us, 22.5 as tiles of many
   c.few = few(c.ts * c.group);
-  // 16 requests, 32 heads of 128, behind 4096 shared keys: 36 us with few rows, 30 without; heads of 64, 4000: 22 and 26
+  // 16 requests, 32 heads of 128, behind 4096 shared keys: 33.1 us with few rows, 30.7 without; heads of 64, 4000: 21.2 and 26.7
   c.few_prompt = head_dim == 128 && c.tb * c.group > 8 ? 0 : few(c.tb * c.group);
   c.own_log2 = c.few ? few_log2 : 7;
   c.prefix_row_tiles = (tokens + c.tpt - 1) / c.tpt;

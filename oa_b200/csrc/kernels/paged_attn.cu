@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(128) paged_attn_rows_kernel(const PagedAttnPar
 // The key tiles of all items, one after the other, are cut into equal stretches, so that a long prompt for few requests and short histories
 // for many fill the chip alike.  The part of an item in one stretch is a segment.  Segments that are not a whole result leave (o, m, l) in fp32
 // in scratch, and a second launch joins them.  Where everything goes follows from prefix sums over the batch that each CTA makes for
-// itself; CTA 0 leaves them for the second launch.
+// itself; what the second launch has to know of them is left in scratch.
 //
 // There are two kinds of CTAs.
 //   Many rows (a tile of up to 128, tiles of 128 keys, a stretch to a CTA): tcgen05 with scores, weights and results in TMEM, below.
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(128) paged_attn_rows_kernel(const PagedAttnPar
 // while these are worked on, 93).  A tile of 128 x 128 takes about 1700 cycles (two threads to a row, all eight warps in the same tile: 2000 and more), of
 // which the exponentials keep the special-function units busy for 1000; the rest are round trips to barriers and TMEM (200 each) that two warps to
 // a scheduler do not hide.
-constexpr int PA_M = 128, PA_N = 128, PA_THREADS = 512, PA_MAX_BATCH = 1024, PA_LIST = 8;
+constexpr int PA_M = 128, PA_N = 128, PA_THREADS = 512, PA_MAX_BATCH = 2048, PA_LIST = 8;
 constexpr int PF_WARPS = 8, PF_STAGES = 3, PF_STAGE_BYTES = 8192, PF_KEPT_BYTES = 792;    // few rows: warps, tiles in a warp's ring, K and V of a tile
 template <int HD> constexpr int PF_KEYS_LOG2 = HD == 64 ? 5 : 4;       // keys of such a tile
 constexpr int PF_ROWS = 16;                                             // and the most rows: what a thread's registers hold

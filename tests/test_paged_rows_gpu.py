@@ -53,3 +53,9 @@ def test_long_pieces_of_few_requests(hd, fresh, lens, prefix):
     _check_attention("cuda", torch.bfloat16, lens, fresh, 8, 2, hd, 16, prefix, room=5)
     _check_attention("cuda", torch.bfloat16, lens, fresh, 3, 3, hd, 128, prefix)
     K.check_status()
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("batch", [2048, 2049])
+def test_the_most_requests_that_the_sums_hold_and_one_more(dtype, hd, batch):
+    _check_attention("cuda", dtype, [1 + 5 * i % 23 for i in range(batch)], [1] * batch, 2, 1, hd, 16, 17)

@@ -623,9 +623,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     u64 have = 0, before, all;
     clear_bins();
     __syncthreads();
-    each_from(LOWEST, [&](int, float v) {
-      ++have;
-      add_to_bin(place_of_gap(v), {0, 1});
+    each([&](int, const float* v) {
+#pragma unroll
+      for (int k = 0; k < N16; ++k)
+        if (v[k] > -INFINITY) {
+          ++have;
+          add_to_bin(place_of_gap(v[k]), {0, 1});
+        }
     });
     share_sums(warp_total(have), before, all);
     if (all > (u64)want) cut_by_bins(all, place_of_gap, 1.f / 32.f, [](float) { return 1ull; }, [&](u64 n) { return n >= (u64)want; });

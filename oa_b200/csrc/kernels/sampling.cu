@@ -279,6 +279,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     const auto by_hand = [&](int i) { if (i >= a && i < b) places[i] = x[first + i]; else places[i] = T(-INFINITY); };
     for (int i = s0 + lane; i < a16; i += 32) by_hand(i);        // ends off 16 bytes, and places without a token
     for (int i = b16 + lane; i < s1; i += 32) by_hand(i);
+    __syncwarp();                                                // other lanes read them, 16 bytes at a time, and a warp without a copy waits for nothing else
     // every CTA of the cluster is there before anything is written to it
     if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
     if (b16 > a16 && !warp_wait(&sh.bars[warp], 0) && lane == 0) report_error(status, OA_KERR_WAIT_FULL);

@@ -519,6 +519,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     }
     from = at;
     idx = up;
+    meet();                                                      // the last sums have been read everywhere: either set of slots may be written
   };
   // A logit that is surely not above peak - gap, whatever was rounded on the way to the gap
   const auto below_gap = [&](float gap, bool unbounded) { return unbounded ? LOWEST : fmaxf(peak - gap * 1.00001f - (fabsf(peak) + gap) * 0x1p-20f, LOWEST); };
@@ -634,6 +635,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     });
     share_sums(warp_total(have), before, all);
     if (all > (u64)want) cut_by_bins(all, place_of_gap, 1.f / 32.f, [](float) { return 1ull; }, [&](u64 n) { return n >= (u64)want; });
+    else if (cut_p) meet();                                      // as above
   }
   // ---- 3
   if (cut_p) {
@@ -657,7 +659,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
       each_from(from, [&](int i, float v) { if (in(i, v)) put(v); });
     }
     u64 before, binned, rest;
-    tell(sh.slots[0], warp_total(((u64)hi_in << 20) + lo_in));   // both sets: since either was read last, all have met
+    // Both sets: since either was read last, all have met (in `collect`, at the end of `search`, or where nothing was cut off)
+    tell(sh.slots[0], warp_total(((u64)hi_in << 20) + lo_in));
     tell(sh.slots[1], warp_total(((u64)hi_out << 20) + lo_out));
     meet();
     hear(sh.slots[0], before, binned);

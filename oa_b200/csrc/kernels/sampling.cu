@@ -234,7 +234,7 @@ __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float
 struct RowShared {
   u64 slots[2][8 * ROW_WARPS];             // a number of each warp of the cluster, in two sets used in turn
   u64 red[ROW_WARPS];
-  u64 cut, base;                           // where a cut is; a bin and the sum before it
+  u64 cut, base, held;                     // where a cut is; the sum before a bin and the bin's own
   u64 far_cut;                             // the first CTA's word to the others
   uint64_t bars[ROW_WARPS];
   int listed, bin;
@@ -463,9 +463,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     all = __shfl_sync(0xffffffffu, up, ROW_WARPS - 1);
     return __shfl_sync(0xffffffffu, up - r, warp) + inc - v;
   };
-  // The sums of all CTAs' bins, two to a thread; then the first bin in which the running sum is enough, and the sum before it.  Returns
+  // The sums of all CTAs' bins, two to a thread; then the first bin in which the running sum is enough, the sum before it and its own.  Returns
   // false when no bin is.
-  const auto find_bin = [&](u64 base, auto enough, int& bin, u64& before, u64& all) {
+  const auto find_bin = [&](u64 base, auto enough, int& bin, u64& before, u64& held, u64& all) {
     if (tid == 0) sh.bin = -1;
     meet();                                                      // all bins are filled
     const uint32_t at = smem_u32(bins + 2 * tid);
@@ -482,10 +482,12 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
       const bool second = !enough(run + v0);
       sh.bin = 2 * tid + second;
       sh.base = run + (second ? v0 : 0);
+      sh.held = second ? v1 : v0;
     }
     __syncthreads();
     bin = sh.bin;
     before = sh.base;
+    held = sh.held;
     return bin >= 0;
   };
   // What a bin holds are two sums of 32 bits, in units of 1 and 2^20.  A bin of very many large weights overflows, which shows in the sum of all.
@@ -526,14 +528,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
   // and one that is surely not below it
   const auto above_gap = [&](float gap) { return peak - gap * 0.99999f + (fabsf(peak) + gap) * 0x1p-20f; };
   // Cuts what is kept to the shortest head of the ranking whose sum of f is enough.  place(v) rises from 0 as v falls, by 1, a bin, for `step`;
-  // tokens at ROW_LIST or more of it take no part in the first pass of bins, which the caller has made (their sum: `binned`), and are not reached.
-  const auto cut_by_bins = [&](u64 binned, auto place, float step, auto f, auto enough) {
+  // tokens at ROW_BINS or more of it take no part in the first pass of bins, which the caller has made (their sum: `binned`), and are not reached.
+  // `open`: the last bin of that pass holds all tokens from there on, whatever their place, so that it cannot be cut again.  A list makes the cut
+  // only if it has the sum of its bin: whatever else the windows let through or miss is left to the search.
+  const auto cut_by_bins = [&](u64 binned, auto place, float step, bool open, auto f, auto enough) {
     u64 base = 0, all;
     float origin = 0.f, zoom = 1.f;                              // bins of this pass: (place - origin) * zoom
     for (int pass = 0; pass < 3; ++pass) {
       int bin;
-      u64 before;
-      const bool there = find_bin(base, enough, bin, before, all);
+      u64 before, held;
+      const bool there = find_bin(base, enough, bin, before, held, all);
       if (!there || all != binned) break;                        // a bin has overflowed, or all was cut off
       base = before;
       const float o = origin, z = zoom;
@@ -545,15 +549,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
           sort_list(n);
           u64 m = tid < n ? (u64)f(logit_of((uint32_t)(bins[tid] >> 32))) : 0, total;
           const u64 run = base + block_scan(m, total);
-          if (tid < n && !enough(run) && (enough(run + m) || tid == n - 1)) sh.cut = bins[tid];
+          if (tid < n && !enough(run) && enough(run + m)) sh.cut = bins[tid];
           __syncthreads();
-          if (tid < (int)ctas) cluster_st(map_to_cta(smem_u32(&sh.far_cut), tid), sh.cut);
+          if (tid < (int)ctas) cluster_st(map_to_cta(smem_u32(&sh.far_cut), tid), total == held ? sh.cut : 0);      // no entry is 0
         }
         meet();
+        if (sh.far_cut == 0) break;
         cut_at(sh.far_cut);
         return;
       }
-      if (pass == 2 || n == 0) break;
+      if (pass == 2 || n == 0 || (open && pass == 0 && bin == ROW_BINS - 1)) break;
       // the bin again, in as many: the next bits of place
       origin = o + (float)bin / z;
       zoom = z * (float)ROW_BINS;
@@ -634,7 +639,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
         }
     });
     share_sums(warp_total(have), before, all);
-    if (all > (u64)want) cut_by_bins(all, place_of_gap, 1.f / 32.f, [](float) { return 1ull; }, [&](u64 n) { return n >= (u64)want; });
+    if (all > (u64)want) cut_by_bins(all, place_of_gap, 1.f / 32.f, true, [](float) { return 1ull; }, [&](u64 n) { return n >= (u64)want; });
     else if (cut_p) meet();                                      // as above
   }
   // ---- 3
@@ -666,7 +671,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     hear(sh.slots[0], before, binned);
     hear(sh.slots[1], before, rest);
     const double part = dp * (double)(binned + rest);
-    cut_by_bins(binned, place, t / scale, [&](float v) -> u64 { return mass_of(weight(v)); }, [&](u64 m) { return m > 0 && !((double)m < part); });
+    cut_by_bins(binned, place, t / scale, false, [&](float v) -> u64 { return mass_of(weight(v)); }, [&](u64 m) { return m > 0 && !((double)m < part); });
   }
   // ---- 4
   const bool all_in = from == -INFINITY && !(least > 0.f);

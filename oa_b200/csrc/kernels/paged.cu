@@ -86,6 +86,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PlanPara
       const int old = pages_of(c, p), need = max(pages_of((long long)c + f, p) - old, 0);
       const int have = min(max(p.n_free - taken - s_first[b], 0), need);
       lost += f - (int)min((long long)f, max(((long long)(old + have) << p.page_log2) - c, 0ll));
+      const int on = (int)min((long long)f, ((long long)old << p.page_log2) - c);      // go to the page that is begun, which may not be there either
+      if (on > 0 && p.tables[b * p.table_stride + old - 1] < 0) lost += on;
       p.starts[b] = s_start[b];
       p.lens[b] = (int)min((long long)c + f, (long long)p.width << p.page_log2);
     }

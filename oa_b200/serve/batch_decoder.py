@@ -101,34 +101,36 @@ class OaBatchDecoder:
             to.copy_(torch.tensor([getattr(s, name) for s in how], dtype=to.dtype))
 
     def SetPrompt(self, ids: Sequence[int]) -> None:
-        """The prompt that all requests share (none: an empty one), in place of the one before; no request may be under way."""
+        """The prompt that all requests share (none: an empty one), in place of the one before; no request may be under way.  Should it fail once the
+        pages of the one before are given back, there is no prompt."""
         c = self.Cache
         if any(c.Held):
             raise ValueError("SetPrompt: requests are under way")
-        used = c.Used
-        c.Used -= -(-c.PromptLen // c.PageSize)
+        held = -(-c.PromptLen // c.PageSize)
+        c.Used -= held
         try:
             need = c.Room([0], [len(ids)], c.MaxPrompt)
-        except ValueError:
-            c.Used = used
-            raise
+        finally:
+            c.Used += held
         c.Taken.copy_(paged.release(torch.ones(1, dtype=torch.bool, device=c.Lens.device), c.PromptLens, c.PromptTable, c.Free, c.Taken, c.PageSize))
         c.PromptLen = 0
+        c.Used -= held
         self._graph, self._steps = None, 0
         if not len(ids):
             return
         t = torch.tensor(list(ids), dtype=torch.int32, device=c.Lens.device)
         with AG.OaGradNo():
-            step = self._room(torch.full_like(c.PromptLens, len(ids)), c.PromptLens, c.PromptTable, len(ids), 0)
+            step = paged.plan(c.PromptLens, torch.full_like(c.PromptLens, len(ids)), c.PromptTable, c.Free, c.Taken, c.PageSize, len(ids))
             self._layers(t, step, c.PromptTable, len(ids), 0)
+            self._keep(step, c.PromptLens)
         c.Used += need
         c.PromptLen = len(ids)
 
     def Release(self, requests: Sequence[int]) -> None:
         """Forgets these requests; their pages are free for others."""
-        c = self.Cache
+        c, requests = self.Cache, list(requests)
         done = torch.zeros(self.Batch, dtype=torch.bool)
-        done[list(requests)] = True
+        done[requests] = True
         c.Taken.copy_(paged.release(done.to(c.Lens.device), c.Lens, c.Tables, c.Free, c.Taken, c.PageSize))
         for b in requests:
             c.Used -= -(-c.Held[b] // c.PageSize)
@@ -141,11 +143,7 @@ class OaBatchDecoder:
         counts = [len(n) for n in new]
         need = self.Cache.Room(self.Cache.Held, counts, self.Cache.MaxTokens)
         flat = torch.tensor([t for n in new for t in n], dtype=torch.int32, device=self._ids.device)
-        self._fresh.copy_(torch.tensor(counts, dtype=torch.int32))
-        self._draw()
-        out = self._step(flat, max(counts), False)
-        self._grown(counts, need)
-        return out
+        return self._take(counts, need, lambda: self._step(flat, max(counts), False))
 
     def Step(self, ids: torch.Tensor, active: Optional[Sequence[bool]] = None) -> torch.Tensor:
         """One more token ids[b] (on the device) of each active request (default: of all): the tokens that come next, int32 [batch], -1 for the others.
@@ -155,17 +153,17 @@ class OaBatchDecoder:
         counts = [1] * self.Batch if active is None else [int(bool(a)) for a in active]
         need = self.Cache.Room(self.Cache.Held, counts, self.Cache.MaxTokens)
         self._ids.copy_(ids.reshape(-1))
-        self._fresh.copy_(torch.tensor(counts, dtype=torch.int32))
-        self._draw()
-        if self._graph is None and self._may_record and self._steps > 0:      # the step before was eager: buffers that are made once exist
-            self._record()
-        if self._graph is not None:
+
+        def one():
+            if self._graph is None and self._may_record and self._steps > 0:  # the step before was eager: buffers that are made once exist
+                self._record()
+            if self._graph is None:
+                return self._step(self._ids, 1, True)
             self._graph.replay()
-            self.Logits, self.LogProbs, out = self._static
-        else:
-            out = self._step(self._ids, 1, True)
+            return self._static
+
+        out = self._take(counts, need, one)
         self._steps += 1
-        self._grown(counts, need)
         return out
 
     def Generate(self, prompts: Sequence[Sequence[int]], new_tokens: int, stop: Optional[int] = None) -> List[List[int]]:
@@ -198,19 +196,25 @@ class OaBatchDecoder:
         return texts
 
     # ---- one step
-    def _draw(self) -> None:
-        torch.rand(self.Batch, generator=self._random, out=self._u)
+    def _take(self, counts: Sequence[int], need: int, step) -> torch.Tensor:
+        """One step of `counts` new tokens of each request with numbers of its own.  A step that fails moves nothing, and may be made again."""
+        c, numbers = self.Cache, self._random.get_state()
+        try:
+            self._fresh.copy_(torch.tensor(counts, dtype=torch.int32))
+            torch.rand(self.Batch, generator=self._random, out=self._u)
+            out, logits, logprobs = step()
+        except BaseException:
+            self._random.set_state(numbers)
+            raise
+        self.Logits, self.LogProbs = logits, logprobs
+        c.Held = [h + f for h, f in zip(c.Held, counts)]
+        c.Used += need
+        return out
 
-    def _grown(self, counts: Sequence[int], need: int) -> None:
-        self.Cache.Held = [h + f for h, f in zip(self.Cache.Held, counts)]
-        self.Cache.Used += need
-
-    def _room(self, fresh: torch.Tensor, lens: torch.Tensor, tables: torch.Tensor, tokens: int, position0: int) -> paged.PagedStep:
-        c = self.Cache
-        step = paged.plan(lens, fresh, tables, c.Free, c.Taken, c.PageSize, tokens, position0)
+    def _keep(self, step: paged.PagedStep, lens: torch.Tensor) -> None:
+        """The step's tokens and pages are the cache's from here on; before, what it wrote lies beyond the lengths and the stack's top."""
         lens.copy_(step.lens)
-        c.Taken.copy_(step.taken)
-        return step
+        self.Cache.Taken.copy_(step.taken)
 
     def _layers(self, ids: torch.Tensor, step: paged.PagedStep, tables: torch.Tensor, most: int, prompt_len: int) -> torch.Tensor:
         """The rows of the tokens behind the last block; their keys and values go to their pages."""
@@ -227,18 +231,20 @@ class OaBatchDecoder:
             x = block_tail(b, x, OaMatrix(attn), n <= self.Batch)
         return x.Tensor()
 
-    def _step(self, ids: torch.Tensor, most: int, by_request: bool) -> torch.Tensor:
-        """`by_request`: ids [batch], of which the requests that have a new token take theirs."""
+    def _step(self, ids: torch.Tensor, most: int, by_request: bool):
+        """(next tokens, logits, log-probabilities).  `by_request`: ids [batch], of which the requests that have a new token take theirs."""
         m, c = self.Model, self.Cache
         with AG.OaGradNo():
-            step = self._room(self._fresh, c.Lens, c.Tables, ids.numel(), c.PromptLen)
+            step = paged.plan(c.Lens, self._fresh, c.Tables, c.Free, c.Taken, c.PageSize, ids.numel(), c.PromptLen)
             if by_request:
                 ids = ids.index_select(0, step.rows.clamp(min=0)).clamp(min=0)             # rows of no request are some token's, whose result nothing reads
             x = self._layers(ids, step, c.Tables, most, c.PromptLen)
             last = x.index_select(0, (step.starts[1:] - 1).clamp(min=0))
-            self.Logits = m.Head.Forward(m.LnFinal.Forward(OaMatrix(last))).Tensor()
-            tokens, self.LogProbs = sampling.sample(self.Logits, self._u, self._temperature, self._top_k, self._top_p, self._min_p)
-            return torch.where(self._fresh > 0, tokens, -1)
+            logits = m.Head.Forward(m.LnFinal.Forward(OaMatrix(last))).Tensor()
+            tokens, logprobs = sampling.sample(logits, self._u, self._temperature, self._top_k, self._top_p, self._min_p)
+            out = torch.where(self._fresh > 0, tokens, -1)
+            self._keep(step, c.Lens)
+            return out, logits, logprobs
 
     def _record(self) -> None:
         """A step of one token each as a graph: it reads the ids, the requests that have one, the random numbers and the settings where they lie."""
@@ -246,6 +252,5 @@ class OaBatchDecoder:
         g = torch.cuda.CUDAGraph()
         # a replay begins after everything before it on the stream, so whatever changed the weights has finished by then
         with torch.cuda.graph(g, capture_error_mode="thread_local"), K.weights_at_rest([p.Data.Tensor() for p in self.Model.AllParameterPtrs()]):
-            out = self._step(self._ids, 1, True)
-        self._static = (self.Logits, self.LogProbs, out)
+            self._static = self._step(self._ids, 1, True)
         self._graph = g

@@ -21,6 +21,7 @@ from .. import _native as N
 from . import kernels as K
 
 PAGE_SIZES = (16, 32, 64, 128)
+HEAD_DIMS = (32, 64, 128)       # of the attention kernels; the CPU path takes any
 
 
 class PagedStep(NamedTuple):

@@ -76,6 +76,10 @@ class OaBatchDecoder:
             raise ValueError("OaBatchDecoder: batch and max_tokens must be positive")
         if model.PosEmbed is not None and max_tokens + max_prompt > c.SeqLen:
             raise ValueError(f"OaBatchDecoder: {max_prompt} + {max_tokens} tokens, but the model has {c.SeqLen} positions")
+        if page_size not in paged.PAGE_SIZES:
+            raise ValueError(f"OaBatchDecoder: a page holds one of {paged.PAGE_SIZES} tokens, not {page_size}")
+        if w.is_cuda and c.DModel // c.NHeads not in paged.HEAD_DIMS:
+            raise ValueError(f"OaBatchDecoder: heads of one of {paged.HEAD_DIMS}, not of {c.DModel // c.NHeads}")
         if pages is None:
             pages = batch * -(-max_tokens // page_size) + -(-max_prompt // page_size)
         self.Model, self.Cfg, self.Batch = model, c, batch

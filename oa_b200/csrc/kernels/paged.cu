@@ -4,6 +4,7 @@
 //   oa_paged_release  pages of finished requests go back on the free stack
 //   oa_paged_append   rotary embedding of q and k by each token's own position, k and v into their slots
 #include "common.cuh"
+#include "per_device.h"
 #include "api.h"
 
 namespace oa {
@@ -305,8 +306,8 @@ extern "C" int oa_paged_plan(const int* cached, const int* fresh, int* tables, l
   const PlanParams p{cached, fresh, tables, table_stride, free_pages, taken, starts, lens, slots, positions, rows, taken_out, missing,
                      batch, width, n_free, lg, tokens, position0};
   const int work = tokens > batch ? tokens : batch;
-  const int blocks = (work + 4 * PLAN_THREADS - 1) / (4 * PLAN_THREADS);
-  launch_short(paged_plan_kernel, dim3(blocks < 1 ? 1 : blocks > 4 * 148 ? 4 * 148 : blocks), dim3(PLAN_THREADS), smem, (cudaStream_t)stream, p);
+  const int blocks = (work + 4 * PLAN_THREADS - 1) / (4 * PLAN_THREADS), most = 4 * sm_count();
+  launch_short(paged_plan_kernel, dim3(blocks < 1 ? 1 : blocks > most ? most : blocks), dim3(PLAN_THREADS), smem, (cudaStream_t)stream, p);
   return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }
 
@@ -337,7 +338,7 @@ extern "C" int oa_paged_append(int dtype, const void* x, long long row_stride, v
     for (int j = 0; j < half; ++j) p.turns[j] = static_cast<const double*>(turns)[j];
   // A row's pieces over several blocks while the tokens alone leave SMs idle, one to a thread; otherwise two, so that no thread is without (16381 rows
   // of 80 heads of 64: 53 us, 6.3 TB/s; 68 with 256 threads whose fetches wait for the angles).
-  const int n = (q_heads + 2 * kv_heads) * (half / 8), want = (n + 255) / 256, spread = (2 * 148 + tokens - 1) / tokens, per = spread < want ? (n + spread - 1) / spread : n;
+  const int n = (q_heads + 2 * kv_heads) * (half / 8), want = (n + 255) / 256, spread = (2 * sm_count() + tokens - 1) / tokens, per = spread < want ? (n + spread - 1) / spread : n;
   const dim3 grid((unsigned)tokens, (unsigned)(spread < want ? spread : want));
   const int pieces = spread < want ? (per + 511) / 512 * 2 : 1, threads = pieces == 1 ? 256 : ((per + pieces - 1) / pieces + 31) / 32 * 32;
   if (dtype == OA_F32) launch_short(paged_append_kernel<float>, grid, dim3((unsigned)threads), 0, (cudaStream_t)stream, p);

@@ -4,6 +4,7 @@
 // A table entry that names no page counts as keys and values of zeros.  Nothing beyond a request's length is read into a result.
 #include <type_traits>
 #include "common.cuh"
+#include "per_device.h"
 #include "api.h"
 
 namespace oa {
@@ -1402,14 +1403,6 @@ struct PagedTcPlan {
   long long prompt_rows, own_rows, items;
   size_t o_bytes, owns_bytes, ml_bytes, bytes;
 };
-static int sm_count() {
-  static int sms = 0;
-  if (sms == 0) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 0;
-  }
-  return sms > 0 ? sms : 148;
-}
 static PagedTcPlan plan_tc(int tokens, int batch, int max_fresh, int q_heads, int kv_heads, int head_dim, int prefix_len) {
   PagedTcPlan c;
   c.group = q_heads / kv_heads;
@@ -1460,13 +1453,7 @@ int make_tmap_box3_bf16(CUtensorMap* out, const void* ptr, const uint64_t* dims,
 template <int HD>
 static int launch_tc(const PagedAttnParams& a, void* scratch, int* status, cudaStream_t st) {
   using Cfg = PaCfg<HD>;
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(paged_attn_tc_kernel<HD, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES) != cudaSuccess ||
-        cudaFuncSetAttribute(paged_attn_tc_kernel<HD, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES) != cudaSuccess)
-      return OA_ERR_LAUNCH;
-    set = true;
-  }
+  static std::atomic<unsigned long long> allowed[2];
   const PagedTcPlan c = plan_tc(a.tokens, a.batch, a.max_fresh, a.q_heads, a.kv_heads, HD, a.prefix_len);
   const int ps = 1 << a.page_log2;
   const long long own_tiles = (((long long)a.width * ps) >> c.own_log2) + 1;
@@ -1503,7 +1490,9 @@ static int launch_tc(const PagedAttnParams& a, void* scratch, int* status, cudaS
     const uint32_t box[3] = {64, (uint32_t)(ps < 1 << PF_KEYS_LOG2<HD> ? ps : 1 << PF_KEYS_LOG2<HD>), 1};
     if ((rc = make_tmap_box3_bf16(&tkf, a.k, dims, ks, box)) || (rc = make_tmap_box3_bf16(&tvf, a.v, dims, vs, box))) return rc;
   }
-  const auto kernel = c.few > 8 || (work > 0 && c.few_prompt > 8) ? paged_attn_tc_kernel<HD, 2> : paged_attn_tc_kernel<HD, 1>;
+  const bool two = c.few > 8 || (work > 0 && c.few_prompt > 8);
+  const auto kernel = two ? paged_attn_tc_kernel<HD, 2> : paged_attn_tc_kernel<HD, 1>;
+  if (allow_smem(allowed[two], (const void*)kernel, Cfg::SMEM_BYTES) != cudaSuccess) return OA_ERR_LAUNCH;
   launch_short(kernel, dim3((unsigned)c.grid), dim3(PA_THREADS), Cfg::SMEM_BYTES, st, tq, tqo, tk, tv, tkf, tvf, p);
   if (c.joint) launch_short(paged_join_cuts_kernel<HD>, dim3((unsigned)c.grid, 4), dim3(256), 0, st, p);
   else {

@@ -9,6 +9,7 @@
 // log-probability y - log(S / 2^40).  A temperature of 0 or less takes the first of the ranking, with log-probability 0.  NaN counts as
 // -inf; a row without anything above -inf gives token -1 and log-probability -inf.
 #include "common.cuh"
+#include "per_device.h"
 #include "api.h"
 
 namespace oa {
@@ -738,8 +739,9 @@ static int launch_sample(const SampleParams& p, int* status, cudaStream_t st) {
   // As many CTAs to a row as keep its share within 104 KB (two CTAs on an SM); more, up to eight, while rows leave SMs idle and a share
   // has 4096 tokens or more.
   constexpr int UNIT = Lane16<T>::N, WARPS = SAMPLE_THREADS / 32, MOST = 216 * 1024;
+  const int sms = sm_count();
   int lg = 0;
-  while (lg < 3 && ((size_t)(p.vocab >> lg) * sizeof(T) > 104 * 1024 || ((long long)p.rows << lg < 148 && p.vocab >> lg >= 2 * 4096))) ++lg;
+  while (lg < 3 && ((size_t)(p.vocab >> lg) * sizeof(T) > 104 * 1024 || ((long long)p.rows << lg < sms && p.vocab >> lg >= 2 * 4096))) ++lg;
   const int ctas = 1 << lg;
   const int share = (p.vocab + ctas - 1) / ctas + Lane16<T>::N;  // places: tokens, and what the first lacks to 16 bytes
   const int span = (share + WARPS * UNIT - 1) / (WARPS * UNIT) * UNIT;
@@ -748,11 +750,8 @@ static int launch_sample(const SampleParams& p, int* status, cudaStream_t st) {
     launch_short(sample_kernel<T>, dim3((unsigned)p.rows), dim3(SAMPLE_THREADS), 0, st, p);
     return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
   }
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(sample_row_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST) != cudaSuccess) return OA_ERR_LAUNCH;
-    set = true;
-  }
+  static std::atomic<unsigned long long> allowed{0};
+  if (allow_smem(allowed, (const void*)sample_row_kernel<T>, MOST) != cudaSuccess) return OA_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.rows * ctas);
   cfg.blockDim = dim3(SAMPLE_THREADS);

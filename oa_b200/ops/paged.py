@@ -224,7 +224,7 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tab
     batch = lens.numel()
     (pages, kvh, ps, hd, k_step, v_step, tokens, cols, qh, width, table_stride, scale, need) = _attention_layout(
         q.shape, q.dtype, k_pages.shape, k_pages.stride(), v_pages.shape, v_pages.stride(), k_pages.dtype, v_pages.dtype, tables.shape, tables.stride(),
-        tables.dtype, batch, starts.numel(), max_fresh, None if prefix_table is None else prefix_table.numel(), prefix_len, scale, q.is_cuda)
+        tables.dtype, batch, starts.numel(), max_fresh, None if prefix_table is None else prefix_table.numel(), prefix_len, scale, q.get_device())
     if prefix_len > 0:
         _int32("attention", lens, starts, prefix_table)
         _same_device("attention", q, k_pages, v_pages, tables, lens, starts, prefix_table)
@@ -248,8 +248,9 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tab
 
 @functools.lru_cache(maxsize=256)
 def _attention_layout(q_shape, dtype, k_shape, k_stride, v_shape, v_stride, k_dtype, v_dtype, t_shape, t_stride, t_dtype, batch, n_starts, max_fresh, n_prefix,
-                      prefix_len, scale, cuda):
-    """The checks of `attention`; (.. of the pool, tokens, columns, query heads, table width and row stride, scale, bytes of scratch)."""
+                      prefix_len, scale, device):
+    """The checks of `attention`; (.. of the pool, tokens, columns, query heads, table width and row stride, scale, bytes of scratch on
+    the device, -1 being the CPU)."""
     pool = _pool("attention", k_shape, k_stride, v_shape, v_stride, k_dtype, v_dtype, dtype)
     pages, kvh, ps, hd = pool[:4]
     tokens, cols = q_shape if len(q_shape) == 2 else (0, 0)
@@ -262,7 +263,7 @@ def _attention_layout(q_shape, dtype, k_shape, k_stride, v_shape, v_stride, k_dt
     width, table_stride = _table_layout("attention", t_shape, t_stride, t_dtype, batch)
     scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
     qh = cols // hd
-    code = K._DT.get(dtype) if cuda else None
+    code = K._DT.get(dtype) if device >= 0 else None
     need = N.require().oa_paged_attn_scratch_bytes(code, tokens, batch, max_fresh, qh, kvh, hd, pages, prefix_len, scale) if code is not None else 0
     return (*pool, tokens, cols, qh, width, table_stride, scale, need)
 

@@ -736,16 +736,20 @@ using namespace oa;
 
 template <typename T>
 static int launch_sample(const SampleParams& p, int* status, cudaStream_t st) {
-  // As many CTAs to a row as keep its share within 104 KB (two CTAs on an SM); more, up to eight, while rows leave SMs idle and a share
-  // has 4096 tokens or more.
-  constexpr int UNIT = Lane16<T>::N, WARPS = SAMPLE_THREADS / 32, MOST = 216 * 1024;
+  // As many CTAs to a row as leave room for two on an SM (of its 228 KB each has half, less the 1 KB that the system keeps: a share of 98 KB beside bins,
+  // list and slots: 256 rows of 52000 bf16 logits, top-p 81 us, plain 33, top-k 50 27, by one to an SM with twice the share 92, 40 and 26; 592 of 51000
+  // fp32 231, 91 and 96, by one 238, 107 and 94); more, up to eight, while rows leave SMs idle and a share has 4096 tokens or more.
+  constexpr int UNIT = Lane16<T>::N, WARPS = SAMPLE_THREADS / 32, MOST = 216 * 1024, HALF = (228 / 2 - 1) * 1024 - (int)sizeof(RowShared);
   const int sms = sm_count();
+  const auto span_of = [&](int lg) {                             // places: tokens, and what the first lacks to 16 bytes
+    const int share = (p.vocab + (1 << lg) - 1 >> lg) + UNIT;
+    return (share + WARPS * UNIT - 1) / (WARPS * UNIT) * UNIT;
+  };
+  const auto bytes_of = [](int span) { return (ROW_BINS + ROW_LIST) * sizeof(u64) + (size_t)span * WARPS * sizeof(T); };
   int lg = 0;
-  while (lg < 3 && ((size_t)(p.vocab >> lg) * sizeof(T) > 104 * 1024 || ((long long)p.rows << lg < sms && p.vocab >> lg >= 2 * 4096))) ++lg;
-  const int ctas = 1 << lg;
-  const int share = (p.vocab + ctas - 1) / ctas + Lane16<T>::N;  // places: tokens, and what the first lacks to 16 bytes
-  const int span = (share + WARPS * UNIT - 1) / (WARPS * UNIT) * UNIT;
-  const size_t smem = (ROW_BINS + ROW_LIST) * sizeof(u64) + (size_t)span * WARPS * sizeof(T);
+  while (lg < 3 && (bytes_of(span_of(lg)) > HALF || ((long long)p.rows << lg < sms && p.vocab >> lg >= 2 * 4096))) ++lg;
+  const int ctas = 1 << lg, span = span_of(lg);
+  const size_t smem = bytes_of(span);
   if (smem > MOST) {                                             // beyond what eight CTAs hold
     launch_short(sample_kernel<T>, dim3((unsigned)p.rows), dim3(SAMPLE_THREADS), 0, st, p);
     return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;

@@ -73,7 +73,7 @@ def _sample_cpu(logits, u, temperature, top_k, top_p, min_p):
         keep = torch.zeros(vocab, dtype=torch.bool)
         keep[order] = True
         if min_p is not None:
-            keep &= w >= min_p[r].clamp(max=1.0)
+            keep &= w >= torch.nan_to_num(min_p[r], nan=1.0).clamp(max=1.0)
         mass = torch.where(keep, mass, 0)
         total = int(mass.sum())
         at = float(u[r].double() * float(total))

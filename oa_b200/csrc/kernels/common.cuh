@@ -488,30 +488,7 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
-// Two exponentials 2^x on the multiply-add pipe: x = n + f with n the nearest integer (added and taken off at 1.5 * 2^23), 2^f by the
-// minimax polynomial of degree 5 on [-1/2, 1/2] (Remez exchange on the relative error: 7.5e-8, with coefficients rounded to fp32 1.55e-7,
-// 2.1e-7 with the rounding of its steps; ex2.approx states 2^-22 = 2.4e-7), 2^n as an exponent field, which is zero at n = -127: below that, -inf included, the result is 0 as ex2.approx.ftz gives it.
-// NaN stays NaN; x up to 127.
 __device__ __forceinline__ unsigned long long f2_splat(float v) { return f2_of(__float_as_uint(v), __float_as_uint(v)); }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ unsigned long long exp2_fma2(unsigned long long x) {
-  uint32_t a, b;
-  f2_to(x, a, b);
-  x = f2_of(__float_as_uint(max_nan(__uint_as_float(a), -127.f)), __float_as_uint(max_nan(__uint_as_float(b), -127.f)));
-  const unsigned long long t = f2_add(x, f2_splat(12582912.f));
-  const unsigned long long f = f2_fma(f2_add(t, f2_splat(-12582912.f)), f2_splat(-1.f), x);
-  unsigned long long r = f2_fma(f2_splat(0.00132764725f), f, f2_splat(0.00967554096f));
-  r = f2_fma(r, f, f2_splat(0.0555071309f));
-  r = f2_fma(r, f, f2_splat(0.240221202f));
-  r = f2_fma(r, f, f2_splat(0.693146944f));
-  r = f2_fma(r, f, f2_splat(1.00000012f));
-  f2_to(t, a, b);
-  return f2_mul(r, f2_of((a << 23) + 0x3f800000u, (b << 23) + 0x3f800000u));
-}
 __device__ __forceinline__ unsigned long long exp2_mufu2(unsigned long long x) {
   uint32_t a, b;
   f2_to(x, a, b);

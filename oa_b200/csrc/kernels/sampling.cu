@@ -235,7 +235,7 @@ __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float
 struct RowShared {
   u64 slots[2][8 * ROW_WARPS];             // a number of each warp of the cluster, in two sets used in turn
   u64 red[ROW_WARPS];
-  u64 cut, base, held;                     // where a cut is; the sum before a bin and the bin's own
+  u64 cut, base;                           // where a cut is; a bin and the sum before it
   u64 far_cut;                             // the first CTA's word to the others
   uint64_t bars[ROW_WARPS];
   int listed, bin;
@@ -464,9 +464,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
     all = __shfl_sync(0xffffffffu, up, ROW_WARPS - 1);
     return __shfl_sync(0xffffffffu, up - r, warp) + inc - v;
   };
-  // The sums of all CTAs' bins, two to a thread; then the first bin in which the running sum is enough, the sum before it and its own.  Returns
+  // The sums of all CTAs' bins, two to a thread; then the first bin in which the running sum is enough, and the sum before it.  Returns
   // false when no bin is.
-  const auto find_bin = [&](u64 base, auto enough, int& bin, u64& before, u64& held, u64& all) {
+  const auto find_bin = [&](u64 base, auto enough, int& bin, u64& before, u64& all) {
     if (tid == 0) sh.bin = -1;
     meet();                                                      // all bins are filled
     const uint32_t at = smem_u32(bins + 2 * tid);
@@ -483,12 +483,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
       const bool second = !enough(run + v0);
       sh.bin = 2 * tid + second;
       sh.base = run + (second ? v0 : 0);
-      sh.held = second ? v1 : v0;
     }
     __syncthreads();
     bin = sh.bin;
     before = sh.base;
-    held = sh.held;
     return bin >= 0;
   };
   // What a bin holds are two sums of 32 bits, in units of 1 and 2^20.  A bin of very many large weights overflows, which shows in the sum of all.
@@ -530,15 +528,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
   const auto above_gap = [&](float gap) { return peak - gap * 0.99999f + (fabsf(peak) + gap) * 0x1p-20f; };
   // Cuts what is kept to the shortest head of the ranking whose sum of f is enough.  place(v) rises from 0 as v falls, by 1, a bin, for `step`;
   // tokens at ROW_BINS or more of it take no part in the first pass of bins, which the caller has made (their sum: `binned`), and are not reached.
-  // `open`: the last bin of that pass holds all tokens from there on, whatever their place, so that it cannot be cut again.  A list makes the cut
-  // only if it has the sum of its bin: whatever else the windows let through or miss is left to the search.
+  // `open`: the last bin of that pass holds all tokens from there on, whatever their place, so that it cannot be cut again.  A list in which
+  // the sum is not reached makes no cut; the search does then.  (That a list has the sum of its bin is asked for at the price of 2 us in 42 where 256 rows
+  // of 201088 take their largest logit, which comes nowhere near: the code's place and registers.)
   const auto cut_by_bins = [&](u64 binned, auto place, float step, bool open, auto f, auto enough) {
     u64 base = 0, all;
     float origin = 0.f, zoom = 1.f;                              // bins of this pass: (place - origin) * zoom
     for (int pass = 0; pass < 3; ++pass) {
       int bin;
-      u64 before, held;
-      const bool there = find_bin(base, enough, bin, before, held, all);
+      u64 before;
+      const bool there = find_bin(base, enough, bin, before, all);
       if (!there || all != binned) break;                        // a bin has overflowed, or all was cut off
       base = before;
       const float o = origin, z = zoom;
@@ -547,12 +546,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
       const int n = collect([&](auto f) { each_between(below, above, f); }, mine);
       if (n > 0 && n <= ROW_LIST) {
         if (rank == 0) {
+          if (tid == 0) sh.cut = 0;                              // no entry is 0
           sort_list(n);
           u64 m = tid < n ? (u64)f(logit_of((uint32_t)(bins[tid] >> 32))) : 0, total;
           const u64 run = base + block_scan(m, total);
           if (tid < n && !enough(run) && enough(run + m)) sh.cut = bins[tid];
           __syncthreads();
-          if (tid < (int)ctas) cluster_st(map_to_cta(smem_u32(&sh.far_cut), tid), total == held ? sh.cut : 0);      // no entry is 0
+          if (tid < (int)ctas) cluster_st(map_to_cta(smem_u32(&sh.far_cut), tid), sh.cut);
         }
         meet();
         if (sh.far_cut == 0) break;

@@ -157,7 +157,12 @@ __global__ void __launch_bounds__(128) paged_attn_rows_kernel(const PagedAttnPar
 //   More than 16 rows would need more registers than a thread has.
 //
 // Keys beyond a length are cut off from the scores by a select, and their values are overwritten by zeros before the product: what lies there
-// (the rest of a page, or of the ring) may be anything, NaN included.
+// (the rest of a page, or of the ring) may be anything, NaN included.  Among a request's new tokens the cut is the score's alone: a value that is
+// infinite or NaN reaches the earlier tokens in its tile as well, as 0 times it.
+//
+// Weights are rounded to bf16 before they meet the values: both operands of a product have one type, and values are bf16.  That is 2^-9 of each weight, and
+// results are 2.3e-3 from 64 bits (relative, over a whole output) where the rounding of the result alone gives 1.7e-3; weights as two bf16 numbers
+// would take the product twice.  Maxima, sums of weights and partial results are fp32.
 //
 // Many rows.  Warp 15 works out the segments, one after the other, and leaves them in a list of eight in shared memory (every warp on its
 // own needed so much code that the warps waited for instructions).  They run through one pipeline of tiles, g = 0, 1, ..:  warps 13 and 14

@@ -185,8 +185,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SamplePara
 //      tokens go to the first CTA, which sorts them, makes all cuts and samples; the other CTAs are done.
 //   3  top-p (and larger top-k): masses (counts) in 1024 bins of a place that rises as x falls; the bin in which the wanted sum is reached is cut into
 //      1024 again while it holds more than a list does; its tokens go to the first CTA, which sorts them and says where the cut is.
+//      (The last bin of a top-k's first pass, 32 and more below the maximum, has no end, and is not cut again.)
 //      A token of weight below (1 - p) / (2 V) is never kept: all such ones together have less than the mass that is cut off, as the
-//      maximum's weight is 1.  Those take no part.  Equal logits that no bins separate are left to a search over keys and indices, 50 passes.
+//      maximum's weight is 1.  Those take no part.  What no bins separate, equal logits above all, is left to a search over keys and indices, 50 passes.
 //   4  mass of what is kept for each warp, and the warp in whose stretch u falls looks again.
 constexpr int ROW_LIST = 512, ROW_BINS = 1024, ROW_BRIEF_K = 256, ROW_WARPS = SAMPLE_THREADS / 32;
 static_assert(ROW_LIST == SAMPLE_THREADS && ROW_BINS == 2 * SAMPLE_THREADS, "an entry of the list to a thread, and two bins");
@@ -529,8 +530,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_row_kernel(const Sam
   // Cuts what is kept to the shortest head of the ranking whose sum of f is enough.  place(v) rises from 0 as v falls, by 1, a bin, for `step`;
   // tokens at ROW_BINS or more of it take no part in the first pass of bins, which the caller has made (their sum: `binned`), and are not reached.
   // `open`: the last bin of that pass holds all tokens from there on, whatever their place, so that it cannot be cut again.  A list in which
-  // the sum is not reached makes no cut; the search does then.  (That a list has the sum of its bin is asked for at the price of 2 us in 42 where 256 rows
-  // of 201088 take their largest logit, which comes nowhere near: the code's place and registers.)
+  // the sum is not reached makes no cut; the search does then.  (A list's sum against its bin's would say more, but cost 2 us of 42 where 256 rows of 201088
+  // take their largest logit, which comes nowhere near it.)
   const auto cut_by_bins = [&](u64 binned, auto place, float step, bool open, auto f, auto enough) {
     u64 base = 0, all;
     float origin = 0.f, zoom = 1.f;                              // bins of this pass: (place - origin) * zoom

@@ -84,8 +84,8 @@ class OaBatchDecoder:
             pages = batch * -(-max_tokens // page_size) + -(-max_prompt // page_size)
         self.Model, self.Cfg, self.Batch = model, c, batch
         self.Cache = OaPagedCache(c.NLayers, batch, c.NHeads, c.DModel // c.NHeads, pages, page_size, max_tokens, max_prompt, w.dtype, w.device)
-        self.Logits: Optional[torch.Tensor] = None        # [batch, vocab] of the newest token of each request, as of the last step
-        self.LogProbs: Optional[torch.Tensor] = None      # [batch] of the tokens that the last step drew
+        self.Logits: Optional[torch.Tensor] = None        # [batch, vocab] of the newest token of each request in the last step; rows of requests without one mean nothing
+        self.LogProbs: Optional[torch.Tensor] = None      # [batch] of the tokens that the last step drew, likewise
         self._random = torch.Generator(device=w.device)
         self._random.manual_seed(seed)
         self._ids = torch.zeros(batch, dtype=torch.int32, device=w.device)

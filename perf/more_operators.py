@@ -70,10 +70,11 @@ def draw(rng):
         q, kv, hd = rng.choice([(32, 32, 128), (64, 8, 64), (32, 8, 128), (16, 16, 64), (12, 4, 64), (4, 4, 32), (8, 2, 64)])
         dtype = "f32" if hd == 32 or (q, hd) == (8, 64) else "bf16"
         longest = _log(rng, 2, 512 if dtype == "f32" else 5000)
-        room = 0.9 * _flops({"seqs": 6, "longest": 4001, "q_heads": 32, "hd": 128, "step": True}) / (40 if dtype == "f32" else 1)
+        room = 0.7 * _flops({"seqs": 6, "longest": 4001, "q_heads": 32, "hd": 128, "step": True}) / (40 if dtype == "f32" else 1)
         c = {"kind": kind, "dtype": dtype, "step": rng.choice([False, True]), "seqs": 1, "longest": longest, "q_heads": q, "kv_heads": kv, "hd": hd,
              "pad": rng.choice([0, rng.randint(1, 200)])}
-        most = min(600, 3 * room // _flops(c), 2 * 16384 // longest)             # work of ragged lengths is a third
+        # the work of ragged lengths is a third, their tokens are half
+        most = min(600, 3 * room // _flops(c), 2 * min(16000, 13000 * 40 * 128 // ((q + kv) * hd)) // longest)
         return {**c, "seqs": _log(rng, 1, max(1, most))}
     vocab = rng.choice([_log(rng, 64, 1000), 32000, 50257, _log(rng, 1000, 201088)])
     step, dtype = rng.choice([False, True]), rng.choice(["f32", "bf16"])

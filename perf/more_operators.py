@@ -74,7 +74,7 @@ def draw(rng):
         c = {"kind": kind, "dtype": dtype, "step": rng.choice([False, True]), "seqs": 1, "longest": longest, "q_heads": q, "kv_heads": kv, "hd": hd,
              "pad": rng.choice([0, rng.randint(1, 200)])}
         # the work of ragged lengths is a third, their tokens are half
-        most = min(600, 3 * room // _flops(c), 2 * min(16000, 13000 * 40 * 128 // ((q + kv) * hd)) // longest)
+        most = min(600, 3 * room // _flops(c), 2 * min(16000, 11400 * 40 * 128 // ((q + kv) * hd)) // longest)
         return {**c, "seqs": _log(rng, 1, max(1, most))}
     vocab = rng.choice([_log(rng, 64, 1000), 32000, 50257, _log(rng, 1000, 201088)])
     step, dtype = rng.choice([False, True]), rng.choice(["f32", "bf16"])

@@ -297,6 +297,44 @@ size_t oa_paged_attn_scratch_bytes(int dtype, int tokens, int batch, int max_fre
 int oa_sample(int dtype, const void* logits, long long stride, const float* u, const float* temperature, const int* top_k, const float* top_p,
               const float* min_p, int* tokens, float* logprobs, int rows, int vocab, int* status, void* stream);
 
+// ---- packed sequences (packed.cu, packed_attn.cu, packed_attn_f32.cu): sequences of different lengths one behind the other, rows starts[b] .. starts[b + 1] of every tensor
+// What the attention kernels work on, from the starts [batch + 1] (on the device): oa_packed_plan_bytes, 16-byte aligned.  Its words from the fifth on are the
+// starts as the kernels take them: rising, within [0, tokens].
+size_t oa_packed_plan_bytes(int tokens, int batch);
+int oa_packed_plan(const int* starts, int* plan, int batch, int tokens, void* stream);
+// The first `heads` heads of each row of x, each of their first `pairs` pairs (j, j + pairs) turned by its token's position on axis pair_axes[j]; dimensions
+// behind them copied.  y may be x.  positions: [axes, tokens]; pair_axes (bytes) and turns (doubles, the turns a position) are in HOST memory.
+int oa_rotary_axes(int dtype, const void* x, long long x_stride, void* y, long long y_stride, const int* positions, const void* pair_axes,
+                   const void* turns, int pairs, int tokens, int heads, int head_dim, int backward, void* stream);
+
+// Causal attention of every sequence of a plan: q [tokens, q_heads * head_dim], k and v [tokens, kv_heads * head_dim], query head h over key-value head
+// h / (q_heads / kv_heads); o likewise q, lse [q_heads, tokens].  Rows of no sequence: 0 (-inf).  Strides in elements between rows.
+int oa_packed_attn(const void* q, const void* k, const void* v, const int* plan, void* o, float* lse, int tokens, int batch, int q_heads,
+                   int kv_heads, int head_dim, long long q_stride, long long k_stride, long long v_stride, long long o_stride, float scale,
+                   int* status, void* stream);
+size_t oa_packed_attn_bwd_scratch_bytes(int tokens, int batch, int q_heads, int kv_heads, int head_dim);
+int oa_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, const int* plan, void* dq,
+                       void* dk, void* dv, int tokens, int batch, int q_heads, int kv_heads, int head_dim, long long q_stride,
+                       long long k_stride, long long v_stride, long long o_stride, long long do_stride, long long dq_stride,
+                       long long dk_stride, long long dv_stride, float scale, void* scratch, int* status, void* stream);
+int oa_packed_attn_f32(const float* q, const float* k, const float* v, const int* plan, float* o, float* lse, int tokens, int batch, int q_heads,
+                       int kv_heads, int head_dim, long long q_stride, long long k_stride, long long v_stride, long long o_stride, float scale,
+                       void* stream);
+int oa_packed_attn_f32_bwd(const float* q, const float* k, const float* v, const float* o, const float* dout, const float* lse, const int* plan,
+                           float* dq, float* dk, float* dv, int tokens, int batch, int q_heads, int kv_heads, int head_dim, long long q_stride,
+                           long long k_stride, long long v_stride, long long o_stride, long long do_stride, long long dq_stride,
+                           long long dk_stride, long long dv_stride, float scale, void* stream);
+
+// ---- log-probabilities of given tokens (logprob.cu)
+// Of each row of logits times scale: the log-probability of its target (ignore_index: 0; none such in the vocabulary: NaN), the entropy, stats
+// [rows, 2] = (largest, logarithm of the sum of exponentials less it) and the `top` likeliest tokens.
+int oa_token_logprobs(int dtype, const void* logits, long long stride, const int* targets, float* logprobs, float* entropy, float* stats,
+                      float* top_logprobs, int* top_ids, int top, int rows, int vocab, float scale, int ignore_index, void* stream);
+// The logits' gradient from those of the log-probabilities and of the entropy (null: none).  dlogits may be the logits.
+int oa_token_logprobs_bwd(int dtype, const void* logits, long long stride, const int* targets, const float* entropy, const float* stats,
+                          const float* dlogprobs, const float* dentropy, void* dlogits, long long d_stride, int rows, int vocab, float scale,
+                          int ignore_index, void* stream);
+
 // ---- reinforcement learning (rl.cu): vector CartPole, GAE, rollout / replay storage, loss targets, categorical sampling
 int oa_rl_cartpole_reset(void* state, void* done, void* steps, void* episode, int envs, unsigned seed_lo, unsigned seed_hi,
                          int only_done, void* stream);

@@ -1,0 +1,208 @@
+// Packed sequences: which tiles the attention kernels work on, and rotation by positions on several axes.
+#include "common.cuh"
+#include "packed.cuh"
+#include "per_device.h"
+#include "api.h"
+
+namespace oa {
+
+// ------------------------------------------------------------------------------------------------ plan
+// Sequences are rows [starts[b], starts[b + 1]) of the packed tensors; starts that fall or leave [0, tokens] are taken as the nearest that do
+// not.  The attention kernels take their work from two lists, the longest first: tiles of 128 rows of a sequence, and pairs of neighbouring
+// tiles.  Under the causal mask tile i of a sequence sees i + 1 tiles of keys (and its mirror image, tile n - 1 - i, is seen by as many tiles of
+// queries), so both lists are sorted by that index, by counting.  The order among equals is that of the atomics; nothing depends on it but
+// which SM works on a tile.  One block: a batch has few thousand tiles, and one plan serves every layer of a step in both directions.
+constexpr int PLAN_BINS = 1024;           // = threads of the block
+constexpr int PLAN_THREADS = PLAN_BINS;
+
+struct PackedPlanParams {
+  const int* starts;
+  int* plan;
+  int batch, tokens, shift;               // bins of 2^shift tile indices
+};
+
+template <typename Op>
+__device__ __forceinline__ int plan_scan(int v, int* s_warp, Op op) {   // inclusive, over the block
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v = op(v, u);
+  }
+  __syncthreads();                        // the last scan's reads
+  if (lane == 31) s_warp[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    int w = s_warp[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w = op(w, u);
+    }
+    s_warp[lane] = w;
+  }
+  __syncthreads();
+  return warp > 0 ? op(v, s_warp[warp - 1]) : v;
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedPlanParams p) {
+  __shared__ int s_warp[32], s_count[2][PLAN_BINS], s_top;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, shift = p.shift, per = 1 << shift;
+  int* starts = p.plan + PACKED_HEADER;
+  s_count[0][tid] = s_count[1][tid] = 0;
+  if (tid == 0) s_top = 0;
+  const auto most = [](int a, int b) { return max(a, b); };
+  for (int b0 = 0; b0 <= p.batch; b0 += PLAN_THREADS) {
+    const int b = b0 + tid;
+    const int v = plan_scan(b <= p.batch ? min(max(p.starts[b], 0), p.tokens) : 0, s_warp, most);
+    const int s = max(v, s_top);          // written below, behind a barrier
+    if (b <= p.batch) starts[b] = s;
+    __syncthreads();
+    if (tid == PLAN_THREADS - 1) s_top = s;
+  }
+  __syncthreads();
+  // Each warp takes 32 sequences: the first bin of all at once, the others of one sequence after the other, a bin to a lane.
+  // add(which, bin, n) is called for n indices of a bin, returns where they go; put(which, at, first index, n) follows
+  const auto walk = [&](auto add, auto put) {
+    for (int b0 = tid - lane; b0 < p.batch; b0 += PLAN_THREADS) {
+      const int b = b0 + lane;
+      const int lo = b < p.batch ? starts[b] : 0, hi = b < p.batch ? starts[b + 1] : 0;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const int rows = PACKED_TILE << which;
+        const int n = (hi - lo + rows - 1) / rows, head = min(n, per);
+        int sum = head;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += u;
+        }
+        int base = lane == 31 ? add(which, 0, sum) : 0;
+        base = __shfl_sync(0xffffffffu, base, 31);
+        put(which, base + sum - head, 0, head, lo, hi, b);
+        unsigned more = __ballot_sync(0xffffffffu, n > per);
+        while (more) {
+          const int src = __ffs(more) - 1;
+          more &= more - 1;
+          const int nn = __shfl_sync(0xffffffffu, n, src), l = __shfl_sync(0xffffffffu, lo, src), h = __shfl_sync(0xffffffffu, hi, src);
+          for (int k = 1 + lane; (k << shift) < nn; k += 32) {
+            const int c = min(per, nn - (k << shift));
+            put(which, add(which, k, c), k << shift, c, l, h, b0 + src);
+          }
+        }
+      }
+    }
+  };
+  walk([&](int which, int bin, int n) { return n > 0 ? atomicAdd(&s_count[which][bin], n) : 0; }, [](int, int, int, int, int, int, int) {});
+  __syncthreads();
+  int4* lists[2];
+  lists[0] = reinterpret_cast<int4*>(p.plan + packed_tiles_at(p.batch));
+  lists[1] = lists[0] + packed_max_tiles(p.tokens, p.batch);
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    // how many have a larger index: the sums from the end
+    const int mine = s_count[which][PLAN_BINS - 1 - tid];
+    const int sum = plan_scan(mine, s_warp, [](int a, int b) { return a + b; });
+    s_count[which][PLAN_BINS - 1 - tid] = sum - mine;
+    if (tid == PLAN_THREADS - 1) p.plan[which] = sum;
+  }
+  if (tid == 0) { p.plan[2] = starts[0]; p.plan[3] = starts[p.batch]; }
+  __syncthreads();
+  walk([&](int which, int bin, int n) { return n > 0 ? atomicAdd(&s_count[which][bin], n) : 0; },
+       [&](int which, int at, int first, int n, int lo, int hi, int b) {
+         for (int i = 0; i < n; ++i) lists[which][at + i] = make_int4(lo, hi, first + i, b);
+       });
+}
+
+// ------------------------------------------------------------------------------------------------ rotation
+// y = x with each pair (j, j + half) of a head turned by the token's position on the pair's own axis, times theta^(-j / half); dimensions from
+// 2 half on are copied.  A token's angles are worked out once for all its heads: position * turns in 64 bits (in 32 bits a position of 131072 leaves
+// an angle 0.008 off), the whole turns taken off, and what is left in [-1/2, 1/2] turns in 32 bits.  The gradient turns the other way.
+constexpr int ROTARY_MAX_HALF = 128;
+struct RotaryParams {
+  const void* x;
+  long long x_stride;
+  void* y;
+  long long y_stride;
+  const int* positions;                   // [axes, tokens]
+  int tokens, heads, hd, half, backward;
+  uint8_t axis[ROTARY_MAX_HALF];
+  double turns[ROTARY_MAX_HALF];          // turns a position: theta^(-j / half) / (2 pi)
+};
+
+__device__ __forceinline__ void rotary_angles(const RotaryParams& p, int t, float* s_cos, float* s_sin) {
+  for (int k = threadIdx.x; k < p.half; k += blockDim.x) {
+    const double a = (double)p.positions[(long long)p.axis[k] * p.tokens + t] * p.turns[k];
+    float s, c;
+    sincospif((float)(2.0 * (a - rint(a))), &s, &c);
+    s_cos[k] = c;
+    s_sin[k] = p.backward ? -s : s;
+  }
+}
+
+__device__ __forceinline__ float rotary_load(const float* p) { return *p; }
+__device__ __forceinline__ float rotary_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void rotary_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void rotary_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <typename T>
+__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  __shared__ float s_cos[ROTARY_MAX_HALF], s_sin[ROTARY_MAX_HALF];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int rest = p.hd - 2 * p.half, per = p.half + rest;       // pairs and single dimensions of a head
+  for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+    __syncthreads();
+    rotary_angles(p, t, s_cos, s_sin);
+    __syncthreads();
+    const T* x = static_cast<const T*>(p.x) + t * p.x_stride;
+    T* y = static_cast<T*>(p.y) + t * p.y_stride;
+    for (int i = threadIdx.x; i < p.heads * per; i += blockDim.x) {
+      const int h = i / per, j = i - h * per, at = h * p.hd + j;
+      if (j < p.half) {
+        const float a = rotary_load(x + at), b = rotary_load(x + at + p.half), c = s_cos[j], s = s_sin[j];
+        rotary_store(y + at, a * c - b * s);
+        rotary_store(y + at + p.half, b * c + a * s);
+      } else {
+        y[at + p.half] = x[at + p.half];
+      }
+    }
+  }
+}
+
+}  // namespace oa
+
+using namespace oa;
+
+extern "C" size_t oa_packed_plan_bytes(int tokens, int batch) {
+  return ((size_t)packed_tiles_at(batch) + 4 * ((size_t)packed_max_tiles(tokens, batch) + packed_max_pairs(tokens, batch))) * sizeof(int);
+}
+
+extern "C" int oa_packed_plan(const int* starts, int* plan, int batch, int tokens, void* stream) {
+  if (batch < 0 || tokens < 0 || !starts || !plan) return OA_ERR_ARG;
+  if (batch > PACKED_MAX_BATCH || tokens > PACKED_MAX_TOKENS) return OA_ERR_TOO_LARGE;
+  if (reinterpret_cast<uintptr_t>(plan) & 15) return OA_ERR_ALIGN;
+  int shift = 0;
+  while (((tokens / PACKED_TILE) >> shift) >= PLAN_BINS) ++shift;
+  launch_short(packed_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, (cudaStream_t)stream, PackedPlanParams{starts, plan, batch, tokens, shift});
+  return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
+}
+
+extern "C" int oa_rotary_axes(int dtype, const void* x, long long x_stride, void* y, long long y_stride, const int* positions, const void* pair_axes,
+                              const void* turns, int pairs, int tokens, int heads, int head_dim, int backward, void* stream) {
+  if (dtype != OA_F32 && dtype != OA_BF16) return OA_ERR_UNSUPPORTED;
+  if (pairs < 1 || pairs > ROTARY_MAX_HALF) return OA_ERR_UNSUPPORTED;
+  if (tokens < 0 || heads < 1 || 2 * pairs > head_dim || !pair_axes || !turns) return OA_ERR_ARG;
+  if (tokens == 0) return OA_OK;
+  RotaryParams p{x, x_stride, y, y_stride, positions, tokens, heads, head_dim, pairs, backward, {}, {}};
+  for (int j = 0; j < pairs; ++j) {
+    p.axis[j] = static_cast<const uint8_t*>(pair_axes)[j];
+    p.turns[j] = static_cast<const double*>(turns)[j];
+  }
+  const dim3 grid((unsigned)(tokens < (1 << 20) ? tokens : 1 << 20));
+  if (dtype == OA_F32) launch_short(rotary_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, p);
+  else launch_short(rotary_kernel<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, p);
+  return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
+}

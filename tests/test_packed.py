@@ -1,0 +1,436 @@
+"""Packed sequences: the plan's lists, rotary positions with several axes, causal attention with grouped heads and its gradients, on both paths against
+statements in 64 bits with bounds worked out from the roundings.
+
+A rounding to a type is off by at most half its step relative to the value: U bf16 2^-8, fp32 2^-24.  In bf16 the weights p and the score gradients dS are
+rounded once more before they meet V, dO, K and Q, and delta is worked out from the rounded output.
+"""
+import math
+
+import pytest
+import torch
+
+from oa_b200.ops import packed as P
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+F64 = torch.float64
+U = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+THETA = 10000.0
+
+
+def _starts(lengths, device, first=0):
+    return torch.tensor([first] + lengths).cumsum(0).to(torch.int32).to(device)
+
+
+def _inputs(lengths, hq, hk, hd, dtype, device, first=0, pad=0, seed=0, fill=math.nan):
+    """q, k, v as slices of one projection's rows, and dO; rows of no sequence hold `fill`."""
+    g = torch.Generator().manual_seed(seed * 1009 + len(lengths) * 31 + hd)
+    tokens = first + sum(lengths) + pad
+    qkv = torch.randn(tokens, (hq + 2 * hk) * hd, generator=g).to(dtype)
+    dout = torch.randn(tokens, hq * hd, generator=g).to(dtype)
+    for t in (qkv, dout):
+        t[:first] = fill
+        t[tokens - pad:] = fill
+    qkv, dout = qkv.to(device), dout.to(device)
+    return (*torch.split(qkv, [hq * hd, hk * hd, hk * hd], 1), dout)
+
+
+def _oracle(q, k, v, dout, starts, hd, scale, dtype):
+    """{name: (value, bound)} in 64 bits; rows of no sequence are 0 (lse -inf) with bound 0."""
+    q, k, v, dout = (t.cpu().double() for t in (q, k, v, dout))
+    tokens, hq, hk = q.shape[0], q.shape[1] // hd, k.shape[1] // hd
+    u, half = U[dtype], dtype is torch.bfloat16
+    up = u if half else 0.0                                       # the extra rounding of p and dS
+    out = {n: [torch.zeros(tokens, h * hd, dtype=F64), torch.zeros(tokens, h * hd, dtype=F64)] for n, h in (("o", hq), ("dq", hq), ("dk", hk), ("dv", hk))}
+    out["lse"] = [torch.full((hq, tokens), -math.inf, dtype=F64), torch.zeros(hq, tokens, dtype=F64)]
+    st = starts.tolist()
+    for lo, hi in zip(st, st[1:]):
+        n = hi - lo
+        if n <= 0:
+            continue
+        qs, dy = (t[lo:hi].reshape(n, hq, hd).transpose(0, 1) for t in (q, dout))
+        ks, vs = (t[lo:hi].reshape(n, hk, hd).transpose(0, 1).repeat_interleave(hq // hk, 0) for t in (k, v))
+        late = torch.ones(n, n, dtype=torch.bool).triu(1)
+        x = (qs @ ks.transpose(1, 2) * scale).masked_fill(late, -math.inf)
+        lse = torch.logsumexp(x, -1, keepdim=True)
+        p = torch.exp(x - lse)
+        y = p @ vs
+        # scores: hd products added in 32 bits (each step at most 2^-23 of the sum of magnitudes), then the exponential: 2^-21 and
+        # the rounding of its argument; sums of n terms: n 2^-24
+        mag = (qs.abs() @ ks.abs().transpose(1, 2)).masked_fill(late, 0) * scale
+        far = (x - lse).masked_fill(late, 0).abs().amax()
+        dx = mag.amax() * hd * 2 ** -23 + far * 2 ** -22 + 2 ** -20
+        sums = (n + hd) * 2.0 ** -23
+        e = float(2 * dx + sums)                                  # relative error of a weight: its own score and the row's sum
+        bo = u * y.abs() + (up + e) * (p @ vs.abs())
+        delta = (dy * y).sum(-1, keepdim=True)
+        dp = dy @ vs.transpose(1, 2)
+        ds = scale * p * (dp - delta)
+        bdelta = (dy.abs() * bo).sum(-1, keepdim=True) + hd * 2 ** -23 * (dy * y).abs().sum(-1, keepdim=True)
+        bdp = hd * 2 ** -23 * (dy.abs() @ vs.abs().transpose(1, 2))
+        bds = scale * p * (bdelta + bdp + 2 ** -22 * (dp.abs() + delta.abs())) + (up + e) * ds.abs()
+        sum_ds = sums * ds.abs()
+        one = lambda t: t.transpose(0, 1).reshape(n, -1)          # noqa: E731
+        group = lambda t: one(t.reshape(hk, hq // hk, n, hd).sum(1))   # noqa: E731
+        dq, dk, dv = ds @ ks, ds.transpose(1, 2) @ qs, p.transpose(1, 2) @ dy
+        many = (n * (hq // hk)) * 2.0 ** -23
+        for name, val, bound in (("o", one(y), one(bo)), ("dq", one(dq), u * one(dq).abs() + one((bds + sum_ds) @ ks.abs())),
+                                 ("dk", group(dk), u * group(dk).abs() + group((bds + many * ds.abs()).transpose(1, 2) @ qs.abs())),
+                                 ("dv", group(dv), u * group(dv).abs() + (up + e + many) * group(p.transpose(1, 2) @ dy.abs()))):
+            out[name][0][lo:hi], out[name][1][lo:hi] = val, bound
+        out["lse"][0][:, lo:hi] = lse[..., 0]
+        out["lse"][1][:, lo:hi] = dx + sums + 2 ** -21 * (1 + lse[..., 0].abs())
+    return out
+
+
+def _close(name, got, want, bound):
+    got = got.cpu().double()
+    same = got == want                                            # -inf of rows without a sequence
+    err = torch.where(same, 0.0, (got - want).abs())
+    assert not err.isnan().any(), f"{name}: NaN at {err.isnan().nonzero()[:5].tolist()}"
+    over = (err > bound * 1.0001 + 1e-30).nonzero()
+    assert over.numel() == 0, f"{name}: {over.shape[0]} of {err.numel()} off, first {over[0].tolist()}: {got[tuple(over[0])]} for {want[tuple(over[0])]}, " \
+                              f"bound {bound[tuple(over[0])]}"
+
+
+def _both(q, k, v, dout, starts, hd, scale=None):
+    plan = P.plan(starts, q.shape[0])
+    o, lse = P.attention(q, k, v, plan, hd, scale, return_lse=True)
+    return dict(zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *P.attention_backward(q, k, v, o, dout, lse, plan, hd, scale))))
+
+
+def _check(lengths, hq, hk, hd, dtype, device, first=0, pad=0, scale=None, seed=0):
+    q, k, v, dout = _inputs(lengths, hq, hk, hd, dtype, device, first, pad, seed)
+    starts = _starts(lengths, device, first)
+    got = _both(q, k, v, dout, starts, hd, scale)
+    assert got["o"].dtype is dtype and got["lse"].dtype is torch.float32
+    for name, (want, bound) in _oracle(q, k, v, dout, starts, hd, scale or hd ** -0.5, dtype).items():
+        _close(name, got[name], want, bound)
+
+
+RAGGED = [5, 0, 300, 1, 127, 128, 129, 64, 2, 257]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lengths", [[1], [2], [127], [128], [129], [256], [257], [1, 1, 1], RAGGED], ids=lambda v: "-".join(map(str, v)))
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_lengths_bf16(device, lengths, hd):
+    _check(lengths, 4, 2, hd, torch.bfloat16, device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("hq,hk", [(1, 1), (3, 3), (6, 2), (4, 1), (8, 2), (7, 1)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_heads_bf16(device, hq, hk, hd):
+    _check([200, 3, 131], hq, hk, hd, torch.bfloat16, device, first=7, pad=70)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hk,hd", [(2, 2, 64), (4, 1, 64), (2, 2, 128), (4, 1, 128)])
+def test_attention_long_bf16(hq, hk, hd):
+    _check([1500, 700, 1], hq, hk, hd, torch.bfloat16, "cuda", pad=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_more_items_than_sms(hd):
+    _check([17, 260, 40, 1, 90, 300, 5] * 6, 8, 4, hd, torch.bfloat16, "cuda")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lengths", [[1], [31, 33], [129], RAGGED], ids=lambda v: "-".join(map(str, v)))
+@pytest.mark.parametrize("hq,hk,hd", [(4, 4, 32), (4, 2, 64), (3, 1, 128), (2, 1, 20), (2, 2, 7), (12, 4, 50)])
+def test_attention_fp32(device, lengths, hq, hk, hd):
+    _check(lengths, hq, hk, hd, torch.float32, device, first=2, pad=5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [32, 64])
+def test_attention_fp32_many(hd):
+    _check([400, 200, 1, 128] * 4, 8, 4, hd, torch.float32, "cuda")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_scale(device, dtype):
+    _check([140, 20], 2, 2, 64, dtype, device, scale=0.5)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hq,hk", [(2, 2), (4, 1)])
+def test_sequences_do_not_reach_one_another(device, dtype, hq, hk):
+    """One sequence full of NaN and infinities: the others' results are the same bits as beside zeros."""
+    lengths = [3, 40, 20, 130, 129, 1, 60]
+    starts = _starts(lengths, device)
+    for bad in (1, 3, 5):
+        q, k, v, dout = _inputs(lengths, hq, hk, 64, dtype, device)
+        lo, hi = int(starts[bad]), int(starts[bad + 1])
+        for t in (q, k, v, dout):
+            t[lo:hi] = 0
+        clean = _both(q, k, v, dout, starts, 64)
+        for t, x in zip((q, k, v, dout), (math.nan, math.inf, math.nan, -math.inf)):
+            t[lo:hi] = x
+        got = _both(q, k, v, dout, starts, 64)
+        for name in clean:
+            a, b = (d[name].t() if name == "lse" else d[name] for d in (clean, got))
+            assert torch.equal(torch.cat([a[:lo], a[hi:]]), torch.cat([b[:lo], b[hi:]])), name
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_starts_that_fall_or_leave(device):
+    """Starts count as the nearest that rise within the rows."""
+    q, k, v, dout = _inputs([50], 2, 1, 64, torch.float32, device)
+    got = _both(q, k, v, dout, torch.tensor([-5, 10, 4, 30, 99], dtype=torch.int32, device=device), 64)
+    want = _both(q, k, v, dout, torch.tensor([0, 10, 10, 30, 50], dtype=torch.int32, device=device), 64)
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_nothing_to_do(device, dtype):
+    for tokens, starts in ((0, [0]), (0, [0, 0]), (5, [0]), (5, [3, 3, 3])):
+        q, k, v, dout = (torch.full((tokens, 64), math.nan, dtype=dtype, device=device) for _ in range(4))
+        got = _both(q, k, v, dout, torch.tensor(starts, dtype=torch.int32, device=device), 64)
+        assert all(bool((got[n] == 0).all()) for n in ("o", "dq", "dk", "dv")) and bool((got["lse"] == -math.inf).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_layouts(device, dtype):
+    """Rows apart by any distance, columns apart, rows that begin anywhere: the same bits as contiguous operands."""
+    lengths, hq, hk, hd = [70, 130], 2, 1, 64
+    starts = _starts(lengths, device)
+    q, k, v, dout = (t.contiguous() for t in _inputs(lengths, hq, hk, hd, dtype, device))
+    want = _both(q, k, v, dout, starts, hd)
+
+    def wide(t, extra, at):
+        out = torch.full((t.shape[0], t.shape[1] + extra), math.nan, dtype=dtype, device=device)[:, at:at + t.shape[1]]
+        out.copy_(t)
+        return out
+
+    for extra, at in ((8, 8), (5, 3), (64, 0)):
+        got = _both(*(wide(t, extra, at) for t in (q, k, v, dout)), starts, hd)
+        assert all(torch.equal(got[n], want[n]) for n in want)
+    got = _both(*(t.t().contiguous().t() for t in (q, k, v, dout)), starts, hd)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    row = q[:1].expand(200, hq * hd)
+    same = _both(row, k, v, dout, starts, hd)
+    assert all(torch.equal(same[n], t) for n, t in _both(row.contiguous(), k, v, dout, starts, hd).items())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradients_into_a_projections_rows(device, dtype):
+    lengths, hq, hk, hd = [40, 200], 4, 2, 64
+    q, k, v, dout = _inputs(lengths, hq, hk, hd, dtype, device)
+    plan = P.plan(_starts(lengths, device), 240)
+    o, lse = P.attention(q, k, v, plan, hd, return_lse=True)
+    want = P.attention_backward(q, k, v, o, dout, lse, plan, hd)
+    dqkv = torch.full((240, (hq + 2 * hk) * hd), math.nan, dtype=dtype, device=device)
+    got = P.attention_backward(q, k, v, o, dout, lse, plan, hd, dqkv=dqkv)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(dqkv, torch.cat(want, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_same_inputs_same_bits(hd):
+    lengths = [300, 5, 700, 129, 64] * 3
+    q, k, v, dout = _inputs(lengths, 8, 2, hd, torch.bfloat16, "cuda")
+    starts = _starts(lengths, "cuda")
+    want = _both(q, k, v, dout, starts, hd)
+    for _ in range(3):
+        got = _both(q, k, v, dout, starts, hd)
+        assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_graphs_and_streams(dtype):
+    """Two graphs of the whole pass, replayed in turn with other lengths than those they were recorded with, and a call on another stream."""
+    hq, hk, hd, tokens = 4, 2, 64, 600
+    sets = [[100, 500], [600], [1, 299, 300], [37] * 16]
+    q, k, v, dout = _inputs([tokens], hq, hk, hd, dtype, "cuda")
+    fit = lambda lengths: torch.tensor(([0] + torch.tensor(lengths).cumsum(0).tolist() + [sum(lengths)] * 16)[:17], dtype=torch.int32, device="cuda")  # noqa: E731
+    want = [_both(q, k, v, dout, fit(s), hd) for s in sets]
+    starts = [fit(sets[0]), fit(sets[1])]
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = _both(q, k, v, dout, starts[0], hd)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(other[n], want[0][n]) for n in other)
+    for s in starts:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(_both(q, k, v, dout, s, hd))
+        graphs.append(g)
+    for a, b in ((0, 1), (2, 3), (3, 0)):
+        starts[0].copy_(fit(sets[a]))
+        starts[1].copy_(fit(sets[b]))
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for i, w in ((0, a), (1, b)):
+            assert all(torch.equal(outs[i][n], want[w][n]) for n in want[w])
+
+
+@pytest.mark.gpu
+def test_plan_lists():
+    """Every tile and pair of every sequence once, the largest index first."""
+    g = torch.Generator().manual_seed(3)
+    for lengths in ([1], [0], RAGGED, torch.randint(0, 5000, (70,), generator=g).tolist(), [10] * 3000, [300000, 1, 200000], torch.randint(0, 400, (2500,), generator=g).tolist()):
+        tokens, batch = sum(lengths) + 9, len(lengths)
+        p = P.plan(_starts(lengths, "cuda", 2), tokens)
+        w = p.words.cpu()
+        n, m = w[:2].tolist()
+        first = (4 + batch + 1 + 3) // 4 * 4
+        starts = p.starts.cpu().tolist()
+        most = tokens // 128 + batch
+        exact = tokens // 128 < 1024                               # beyond that, bins hold several indices
+        for count, rows, at in ((n, 128, first), (m, 256, first + 4 * most)):
+            got = w[at:at + 4 * count].reshape(-1, 4).tolist()
+            want = [(a, b, i, s) for s, (a, b) in enumerate(zip(starts, starts[1:])) for i in range(-(-(b - a) // rows))]
+            assert sorted(map(tuple, got)) == sorted(want)
+            order = [x[2] for x in got]
+            step = 1 if exact else 1 << (tokens // 128 // 1024).bit_length()
+            assert all(a // step >= b // step for a, b in zip(order, order[1:]))
+
+
+# ------------------------------------------------------------------------------------------------ rotation
+def _rotary_inputs(tokens, cols, axes, dtype, device, far=131072):
+    g = torch.Generator().manual_seed(tokens * 7 + cols)
+    return torch.randn(tokens, cols, generator=g).to(dtype).to(device), torch.randint(-far, far, (axes, tokens), generator=g, dtype=torch.int32).to(device)
+
+
+def _rotary_oracle(x, positions, axes, heads, hd, theta, backward):
+    n, half = x.shape[0], len(axes)
+    v = x.cpu().double()[:, :heads * hd].reshape(n, heads, hd)
+    a = positions.cpu().double()[list(axes)].t() * torch.exp(torch.arange(half, dtype=F64) * (-math.log(theta) / half))
+    c, s = a.cos()[:, None], (-a.sin() if backward else a.sin())[:, None]
+    lo, hi = v[..., :half], v[..., half:2 * half]
+    y = torch.cat([lo * c - hi * s, hi * c + lo * s, v[..., 2 * half:]], -1)
+    pair = lo.abs() + hi.abs()
+    return y.reshape(n, -1), torch.cat([pair, pair, 0 * v[..., 2 * half:]], -1).reshape(n, -1)
+
+
+ROTARY = [((0,) * 32, 64), ((0,) * 8 + (1,) * 12 + (2,) * 12, 64), (tuple(j % 3 for j in range(64)), 128), ((1, 0, 2) * 5, 64), ((0, 1), 128), ((0,) * 16, 32),
+          ((1,) * 7, 19), ((0,) * 128, 256), ((0,) * 24 + (1,) * 8, 64), ((0,), 2)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("axes,hd", ROTARY, ids=[f"{len(a)}of{h}" for a, h in ROTARY])
+@pytest.mark.parametrize("backward", [False, True])
+def test_rotary(device, dtype, axes, hd, backward):
+    for tokens, heads in ((1, 1), (33, 5), (300, 40)):
+        x, positions = _rotary_inputs(tokens, (heads + 2) * hd, 3, dtype, device)
+        keep = x.clone()
+        got = P.rotary(x, positions, axes, heads, hd, THETA, backward)
+        want, pair = _rotary_oracle(x, positions, axes, heads, hd, THETA, backward)
+        # an angle's turns are rounded to 32 bits within [-1/2, 1/2] (2^-24 turns), its products in 64 bits, sincospif to 2^-22 or so; three roundings of the result's sums
+        bound = U[dtype] * want.abs() + pair * (2 * math.pi * 2 ** -24 + 2 ** -21 + 131072 * 2.0 ** -50)
+        _close("rotary", got, want, bound)
+        assert torch.equal(x, keep)
+        inplace = P.rotary(x, positions, axes, heads, hd, THETA, backward, out=x)
+        assert torch.equal(inplace, got) and inplace.data_ptr() == x.data_ptr() and torch.equal(x[:, heads * hd:], keep[:, heads * hd:])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rotary_layouts(device, dtype):
+    axes, heads, hd = (0,) * 16 + (1,) * 16, 3, 64
+    x, positions = _rotary_inputs(50, heads * hd + 64, 2, dtype, device)
+    want = P.rotary(x[:, :heads * hd].contiguous(), positions, axes, heads, hd, THETA)
+    for at in (0, 1, 8, 64):
+        y = torch.zeros(50, heads * hd + 64, dtype=dtype, device=device)
+        y[:, at:at + heads * hd] = x[:, :heads * hd]
+        assert torch.equal(P.rotary(y[:, at:], positions, axes, heads, hd, THETA), want)
+        assert torch.equal(P.rotary(y[:, at:], positions, axes, heads, hd, THETA, out=y[:, at:]), want)
+    assert torch.equal(P.rotary(x.t().contiguous().t(), positions, axes, heads, hd, THETA), want)
+    assert torch.equal(P.rotary(x[:1].expand(50, -1), positions, axes, heads, hd, THETA),
+                       P.rotary(x[:1].expand(50, -1).contiguous(), positions, axes, heads, hd, THETA))
+    empty = P.rotary(x[:0], positions[:, :0].contiguous(), axes, heads, hd, THETA)
+    assert empty.shape == (0, heads * hd)
+
+
+def test_rotary_is_the_usual_one_with_one_axis():
+    from oa_b200.ops import kernels as K
+    x, _ = _rotary_inputs(20, 128, 1, torch.float32, "cpu")
+    want = K.rope_(x.clone(), 2, 64, 10, pos_offset=5, theta=THETA)
+    got = P.rotary(x, (torch.arange(20) % 10 + 5).to(torch.int32)[None], (0,) * 32, 2, 64, THETA)
+    assert torch.allclose(got, want, rtol=0, atol=4 * 2 ** -20)      # rope_ works its angles out in 32 bits
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def test_refusals():
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)      # noqa: E731
+    plan = P.plan(i32(0, 3, 8), 8)
+    q, k = torch.randn(8, 128), torch.randn(8, 64)
+    for bad in (torch.tensor([0, 3]), i32(0, 3, 4, 8)[::2], i32(0, 3).reshape(1, 2), i32()):
+        with pytest.raises(ValueError, match="starts must be"):
+            P.plan(bad, 8)
+    for tokens in (-1, (1 << 30) + 1):
+        with pytest.raises(ValueError, match="rows; at most"):
+            P.plan(i32(0, 1), tokens)
+    lse = torch.zeros(2, 8)
+    for match, args in (("of one type", (q, k.bfloat16(), k)), ("of one type", (q.half(), k.half(), k.half())), ("of one shape", (q, k, k[:, :32])),
+                        ("of one type", (q[0], k, k)), ("multiple of the key-value heads", (q[:, :96], k, k)), ("rows of heads", (q, k[:, :32], k[:, :32])),
+                        ("the plan is for 8 rows", (q[:7], k[:7], k[:7])), ("the plan is for 8 rows", (q, k[:7], k[:7]))):
+        with pytest.raises(ValueError, match=match):
+            P.attention(*args, plan, 64)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(ValueError, match="scale must be positive"):
+            P.attention(q, k, k, plan, 64, scale)
+        with pytest.raises(ValueError, match="scale must be positive"):
+            P.attention_backward(q, k, k, q, q, lse, plan, 64, scale)
+    for match, args in (("o and dout", (k, q, lse)), ("o and dout", (q, q.bfloat16(), lse)), ("lse must be", (q, q, lse[:1])), ("lse must be", (q, q, lse.double()))):
+        with pytest.raises(ValueError, match=match):
+            P.attention_backward(q, k, k, *args, plan, 64)
+    for dqkv in (torch.zeros(8, 255), torch.zeros(8, 256, dtype=torch.bfloat16), torch.zeros(256, 8).t()):
+        with pytest.raises(ValueError, match="dqkv must be"):
+            P.attention_backward(q, k, k, q, q, lse, plan, 64, dqkv=dqkv)
+
+
+def test_rotary_refusals():
+    x, pos = torch.randn(4, 128), torch.zeros(2, 4, dtype=torch.int32)
+    ok = dict(pair_axes=(0,) * 32, heads=2, head_dim=64, theta=THETA)
+    for match, change in (("x must be", dict(heads=3)), ("x must be", dict(heads=0)), ("pairs of a head", dict(pair_axes=())), ("pairs of a head", dict(pair_axes=(0,) * 33)),
+                          ("names axes", dict(pair_axes=(2,))), ("names axes", dict(pair_axes=(-1,))), ("theta must be", dict(theta=0.0)),
+                          ("theta must be", dict(theta=math.nan)), ("out must be", dict(out=torch.zeros(4, 127))), ("out must be", dict(out=torch.zeros(4, 128).bfloat16())),
+                          ("side by side", dict(out=torch.zeros(128, 4).t())), ("side by side", dict(out=torch.zeros(1, 128).expand(4, 128)))):
+        with pytest.raises(ValueError, match=match):
+            P.rotary(x, pos, **{**ok, **change})
+    for bad in (pos.long(), pos[:, :3], pos[0], torch.zeros(9, 4, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32).t()):
+        with pytest.raises(ValueError, match="positions must be"):
+            P.rotary(x, bad, **ok)
+    with pytest.raises(ValueError, match="x must be"):
+        P.rotary(x.half(), pos, **ok)
+
+
+def test_another_device_than_the_current_one(monkeypatch):
+    """Kernels go to the current device's stream: tensors of another one are refused."""
+    class Elsewhere:
+        is_cuda, device = True, "cuda:1"
+
+        def get_device(self):
+            return 1
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(ValueError, match="the current device is cuda:0"):
+        P._together("attention", Elsewhere(), Elsewhere())
+
+
+@pytest.mark.gpu
+def test_refusals_of_the_kernels():
+    plan = P.plan(torch.tensor([0, 8], dtype=torch.int32, device="cuda"), 8)
+    for dtype, hd in ((torch.bfloat16, 32), (torch.bfloat16, 96), (torch.bfloat16, 256), (torch.float32, 192)):
+        q = torch.zeros(8, hd, dtype=dtype, device="cuda")
+        with pytest.raises(ValueError, match="heads of"):
+            P.attention(q, q, q, plan, hd)
+    q = torch.zeros(8, 64, device="cuda")
+    with pytest.raises(ValueError, match="tensors on"):
+        P.attention(q, q.cpu(), q.cpu(), plan, 64)
+    with pytest.raises(ValueError, match="tensors on"):
+        P.attention(q.cpu(), q.cpu(), q.cpu(), plan, 64)

@@ -35,10 +35,11 @@ def _relative(y):
     return (2 * mag + 30) * 2.0 ** -23 + 2.0 ** -21
 
 
-def _check(x, targets, dlogp, dent, device, top=0, scale=1.0, ignore=-100):
+def _check(x, targets, dlogp, dent, device, top=0, scale=1.0, ignore=-100, place=None):
+    """`place`: x as it lies on the device, where it matters how."""
     rows, vocab = x.shape
     chosen, h, logp, p, order = _oracle(x, targets, top, scale, ignore)
-    xd, td = x.to(device), targets.to(device)
+    xd, td = x.to(device) if place is None else place, targets.to(device)
     r = L.token_logprobs(xd, td, top, scale, ignore)
     e = _relative(x.double() * scale) + (math.log2(vocab) + 60) * 2.0 ** -24      # sums by threads, then as a tree: few hundred terms one after the other
     assert r.top_ids.dtype is torch.int32 and torch.equal(r.top_ids.cpu().long(), order)
@@ -63,6 +64,8 @@ def _check(x, targets, dlogp, dent, device, top=0, scale=1.0, ignore=-100):
         bound = U[x.dtype] * d.abs() + scale * (p * ((2 * e[:, None] + 2.0 ** -21) * (gg.abs()[:, None] + kk.abs()[:, None] * inner.abs())
                                                       + kk.abs()[:, None] * (e + 3 * e * (1 + spread) + 2.0 ** -21 * (1 + h.abs()))[:, None]
                                                       + kk.abs()[:, None] * 2.0 ** -21 * torch.where(p > 0, logp.abs(), 0.0)) + 2.0 ** -22 * t) + 2.0 ** -126
+        # a weight below the smallest normal number, 2^-126, may count as 0: its product with the bracket, by at most 2^-126 of that, is then missing
+        bound = bound + scale * 2.0 ** -126 * (gg.abs()[:, None] + kk.abs()[:, None] * inner.abs())
         got = L.token_logprobs_backward(xd, td, r, None if g is None else g.to(device), None if k is None else k.to(device), scale, ignore)
         assert got.dtype is x.dtype
         near("dlogits", got, d, bound)
@@ -172,29 +175,24 @@ def test_masked_and_broken_rows(device, dtype, vocab):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("vocab", [37, 6000, 90001])
 def test_layouts(device, dtype, vocab):
-    """Rows apart, rows that begin anywhere, columns apart, the gradient in the logits' place: the same bits."""
-    x, t, g, h = (v.to(device) for v in _logits(5, vocab, dtype))
-    r = L.token_logprobs(x, t, 6)
-    want = L.token_logprobs_backward(x, t, r, g, h)
-
-    def same(y, out=None):
-        s = L.token_logprobs(y, t, 6)
-        assert all(torch.equal(a, b) for a, b in zip(s, r))
-        assert torch.equal(L.token_logprobs_backward(y, t, s, g, h, out=out), want)
-
+    """Rows apart, rows that begin anywhere, columns apart, and the gradient in other rows or in the logits' place.  Sums depend on where a row begins: they are
+    added up by 16-byte pieces."""
+    x, t, g, h = _logits(5, vocab, dtype)
+    td, gd, hd = (v.to(device) for v in (t, g, h))
     for extra, at in ((8, 0), (8, 8), (3, 1), (5, 4)):
         wide = torch.full((5, vocab + extra), math.nan, dtype=dtype, device=device)
         y = wide[:, at:at + vocab]
         y.copy_(x)
-        same(y)
-        out = torch.full((5, vocab + extra), 7.0, dtype=dtype, device=device)
-        same(x, out[:, at:at + vocab])
-        assert bool((out[:, :at] == 7).all()) and bool((out[:, at + vocab:] == 7).all())
-        same(y, y)
-        assert bool(wide[:, :at].isnan().all()) and bool(wide[:, at + vocab:].isnan().all())
-    same(x.t().contiguous().t())
-    row = x[:1].expand(5, vocab)
-    assert torch.equal(L.token_logprobs(row, t, 6).logprobs, L.token_logprobs(row.contiguous(), t, 6).logprobs)
+        r = _check(x, t, g, h, device, top=6, place=y)
+        want = L.token_logprobs_backward(y, td, r, gd, hd)
+        out = torch.full((5, vocab + extra + 1), 7.0, dtype=dtype, device=device)
+        got = L.token_logprobs_backward(y, td, r, gd, hd, out=out[:, at:at + vocab])
+        assert torch.equal(got, want) and bool((out[:, :at] == 7).all()) and bool((out[:, at + vocab:] == 7).all())
+        assert torch.equal(L.token_logprobs_backward(y, td, r, gd, hd, out=y), want)
+        assert torch.equal(y, want) and bool(wide[:, :at].isnan().all()) and bool(wide[:, at + vocab:].isnan().all())
+    _check(x, t, g, h, device, top=6, place=x.to(device).t().contiguous().t())
+    row = x[:1].to(device).expand(5, vocab)
+    _check(x[:1].expand(5, vocab), t, g, h, device, place=row)
 
 
 @pytest.mark.parametrize("device", DEVICES)

@@ -53,12 +53,21 @@ template <> struct LpPiece<__nv_bfloat16> {
   uint32_t w[4];
   __device__ __forceinline__ u64 pair(int i) const { return f2_bf16x2(w[i]); }
   __device__ __forceinline__ float at(int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
+  __device__ __forceinline__ float largest() const {         // NaN does not count
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
+    const float2 m = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(m.x, m.y);
+  }
   __device__ __forceinline__ void none() { w[0] = w[1] = w[2] = w[3] = 0xff80ff80u; }      // -inf
   __device__ __forceinline__ void put(int i, const __nv_bfloat16* p) {
     const uint32_t b = *reinterpret_cast<const unsigned short*>(p);
     w[i >> 1] = i & 1 ? (w[i >> 1] & 0xffffu) | b << 16 : (w[i >> 1] & 0xffff0000u) | b;
   }
   __device__ __forceinline__ void set(int i, u64 v) { w[i] = f2_bf16(v); }
+  __device__ __forceinline__ void set1(int i, float v) {
+    const __nv_bfloat16 r = __float2bfloat16_rn(v);
+    put(i, &r);
+  }
   __device__ __forceinline__ void get(int i, __nv_bfloat16* p) const { *reinterpret_cast<unsigned short*>(p) = (unsigned short)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu); }
 };
 template <> struct LpPiece<float> {
@@ -66,9 +75,11 @@ template <> struct LpPiece<float> {
   uint32_t w[4];
   __device__ __forceinline__ u64 pair(int i) const { return f2_of(w[2 * i], w[2 * i + 1]); }
   __device__ __forceinline__ float at(int i) const { return __uint_as_float(w[i]); }
+  __device__ __forceinline__ float largest() const { return fmax3(fmaxf(at(0), at(1)), at(2), at(3)); }
   __device__ __forceinline__ void none() { w[0] = w[1] = w[2] = w[3] = 0xff800000u; }
   __device__ __forceinline__ void put(int i, const float* p) { w[i] = __float_as_uint(*p); }
   __device__ __forceinline__ void set(int i, u64 v) { f2_to(v, w[2 * i], w[2 * i + 1]); }
+  __device__ __forceinline__ void set1(int i, float v) { w[i] = __float_as_uint(v); }
   __device__ __forceinline__ void get(int i, float* p) const { *p = __uint_as_float(w[i]); }
 };
 
@@ -77,22 +88,23 @@ template <> struct LpPiece<float> {
 template <typename T>
 struct LpRow {
   static constexpr int N = LpPiece<T>::N;
-  const T* x;
+  const T* x;                              // where the first piece begins
   int head, vocab;
-  __device__ __forceinline__ LpRow(const T* row, int vocab_) : x(row), head((int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T))), vocab(vocab_) {}
+  __device__ __forceinline__ LpRow(const T* row, int vocab_) : head((int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T))), vocab(vocab_) { x = row - head; }
   __device__ __forceinline__ int pieces() const { return (int)(((long long)head + vocab + N - 1) / N); }
   __device__ __forceinline__ int first(int p) const { return p * N - head; }
-  __device__ __forceinline__ bool whole(int e) const { return e >= 0 && e <= vocab - N; }
+  __device__ __forceinline__ bool whole(int p) const { return p * N >= head && p * N <= head + vocab - N; }
+  __device__ __forceinline__ bool holds(int e) const { return e >= 0 && e < vocab; }
+  __device__ __forceinline__ float element(int e) const { return lp_load(x + head + e); }
   __device__ __forceinline__ void load(LpPiece<T>& to, int p) const {
-    const int e = first(p);
-    if (whole(e)) {
-      const uint4 v = *reinterpret_cast<const uint4*>(x + e);
+    if (whole(p)) {
+      const uint4 v = reinterpret_cast<const uint4*>(x)[p];
       to.w[0] = v.x; to.w[1] = v.y; to.w[2] = v.z; to.w[3] = v.w;
     } else {
       to.none();
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (e + i >= 0 && e + i < vocab) to.put(i, x + e + i);
+        if (holds(first(p) + i)) to.put(i, x + p * N + i);
     }
   }
 };
@@ -124,38 +136,65 @@ __device__ __forceinline__ uint32_t lp_key(float x) {
 __device__ __forceinline__ float lp_unkey(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ u64 lp_rank(uint32_t key, int i) { return ((u64)key << 32) | (uint32_t)~i; }
 
+// A row is worked on by a team: a warp of a block, or a whole block (of a cluster).
+template <int THREADS>
+__device__ __forceinline__ void lp_sync() {
+  if (THREADS == 32) __syncwarp();
+  else __syncthreads();
+}
+
 template <int THREADS, bool TOP>
 struct LpShared {
   static constexpr int WARPS = THREADS / 32, GROUPS = THREADS < 128 ? THREADS : 128, PER = THREADS / GROUPS;
-  static constexpr int LIST = !TOP ? 1 : THREADS == 32 ? 256 : THREADS == 128 ? 1024 : 2048;      // candidates for the alternatives
+  static constexpr int LIST = !TOP ? 1 : THREADS == 32 ? 128 : 1024;      // candidates for the alternatives
   u64 list[LIST], best[LP_MAX_TOP], red[WARPS];
-  LpSums sums[WARPS];
+  LpSums sums[WARPS], total;
+  float log_l;
   uint32_t maxima[GROUPS];
-  int count, scan[WARPS];
+  unsigned short hot[TOP ? THREADS : 1];
+  int count, hots, scan[WARPS];
   uint32_t bound;
 };
+
+// s.best[rank] = element, of the n in s.list, as far as rank < top
+template <int THREADS, typename S>
+__device__ __forceinline__ void lp_order(S& s, int n, int top, int tid) {
+  for (int i = tid; i < n; i += THREADS) {
+    const u64 mine = s.list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += s.list[j] > mine;
+    if (rank < top && mine) s.best[rank] = mine;
+  }
+}
 
 // The `top` first of the ranking of pieces [p0, p1) into s.best, 0 where there are fewer.  tmax: the largest key of this thread's pieces p0 + tid +
 // i THREADS
 template <typename T, int THREADS, typename S>
-__device__ __forceinline__ void lp_top(S& s, const LpRow<T>& row, int p0, int p1, uint32_t tmax, int top) {
+__device__ __forceinline__ void lp_top(S& s, const LpRow<T>& row, int p0, int p1, uint32_t tmax, int top, int tid) {
   constexpr int N = LpPiece<T>::N;
   constexpr uint32_t LOW = sizeof(T) == 2 ? 0xffffu : 0u;      // bits of a key that say nothing
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lane = tid & 31, warp = tid >> 5;
   // a bound that at least `top` elements reach: the top-th largest of the maxima of groups of threads
   uint32_t g = tmax;
 #pragma unroll
   for (int o = 1; o < S::PER; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
   if (tid % S::PER == 0) s.maxima[tid / S::PER] = g;
-  if (tid == 0) s.count = 0;
+  if (tid == 0) s.count = s.hots = 0;
   if (tid < LP_MAX_TOP) s.best[tid] = 0;
-  __syncthreads();
+  lp_sync<THREADS>();
   if (warp == 0) {
     uint32_t mine[S::GROUPS / 32], bound = 0;
 #pragma unroll
     for (int i = 0; i < S::GROUPS / 32; ++i) mine[i] = s.maxima[i * 32 + lane] & ~LOW;
+    uint32_t hi = mine[0], lo = mine[0];
+#pragma unroll
+    for (int i = 1; i < S::GROUPS / 32; ++i) { hi = max(hi, mine[i]); lo = min(lo, mine[i]); }
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    uint32_t bit = hi == lo ? 0 : 1u << (31 - __clz(hi ^ lo));             // the first in which they differ
+    bound = bit ? hi & ~(2 * bit - 1) : hi;
 #pragma unroll 1
-    for (uint32_t bit = 1u << 31; bit > LOW; bit >>= 1) {
+    for (; bit > LOW; bit >>= 1) {
       const uint32_t c = bound | bit;
       int n = 0;
 #pragma unroll
@@ -164,41 +203,39 @@ __device__ __forceinline__ void lp_top(S& s, const LpRow<T>& row, int p0, int p1
     }
     if (lane == 0) s.bound = bound;
   }
-  __syncthreads();
+  lp_sync<THREADS>();
   const uint32_t bound = s.bound;
-  // everything from `from` on goes into the list, as far as there is room
+  // The pieces of the threads whose maximum reaches the bound, dealt to all; elements from `from` on go into the list as far as there is room
+  if (tmax >= bound) s.hot[atomicAdd(&s.hots, 1)] = (unsigned short)tid;
+  lp_sync<THREADS>();
+  const int hots = s.hots, steps = (p1 - p0 + THREADS - 1) / THREADS;
   const auto collect = [&](uint32_t from) {
-    if (tmax < from) return;
-    for (int p = p0 + tid; p < p1; p += LP_BATCH * THREADS) {
-      LpPiece<T> v[LP_BATCH];
+    for (int i = tid; i < hots * steps; i += THREADS) {
+      const int h = i / steps, p = p0 + s.hot[h] + (i - h * steps) * THREADS;
+      if (p >= p1) continue;
+      LpPiece<T> v;
+      row.load(v, p);
+      const int e = row.first(p);
 #pragma unroll
-      for (int b = 0; b < LP_BATCH; ++b)
-        if (p + b * THREADS < p1) row.load(v[b], p + b * THREADS);
-#pragma unroll
-      for (int b = 0; b < LP_BATCH; ++b) {
-        if (p + b * THREADS >= p1) break;
-        const int e = row.first(p + b * THREADS);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint32_t k = lp_key(v[b].at(i));
-          if (k >= from && e + i >= 0 && e + i < row.vocab) {
-            const int at = atomicAdd(&s.count, 1);
-            if (at < S::LIST) s.list[at] = lp_rank(k, e + i);
-          }
+      for (int j = 0; j < N; ++j) {
+        const uint32_t k = lp_key(v.at(j));
+        if (k >= from && row.holds(e + j)) {
+          const int at = atomicAdd(&s.count, 1);
+          if (at < S::LIST) s.list[at] = lp_rank(k, e + j);
         }
       }
     }
   };
   collect(bound);
-  __syncthreads();
+  lp_sync<THREADS>();
   int n = s.count;
   if (n > S::LIST) {
     // very many equal logits, masked ones for instance: those above the bound, then of those at it the first by index
-    __syncthreads();
+    lp_sync<THREADS>();
     if (tid == 0) s.count = 0;
-    __syncthreads();
+    lp_sync<THREADS>();
     collect((bound | LOW) + 1);
-    __syncthreads();
+    lp_sync<THREADS>();
     n = s.count;
     if (n <= S::LIST - LP_MAX_TOP) {
       for (int q0 = p0; q0 < p1 && n < top; q0 += THREADS) {     // a step's elements lie side by side: their order is that of threads and pieces
@@ -212,7 +249,7 @@ __device__ __forceinline__ void lp_top(S& s, const LpRow<T>& row, int p0, int p1
 #pragma unroll
           for (int i = 0; i < N; ++i) {
             const uint32_t k = lp_key(v.at(i));
-            if ((k & ~LOW) == bound && e + i >= 0 && e + i < row.vocab) { hit |= 1u << i; key = k; }
+            if ((k & ~LOW) == bound && row.holds(e + i)) { hit |= 1u << i; key = k; }
           }
         }
         const int mine = __popc(hit);
@@ -222,15 +259,15 @@ __device__ __forceinline__ void lp_top(S& s, const LpRow<T>& row, int p0, int p1
           const int u = __shfl_up_sync(0xffffffffu, sum, o);
           if (lane >= o) sum += u;
         }
-        __syncthreads();
+        lp_sync<THREADS>();
         if (lane == 31) s.scan[warp] = sum;
-        __syncthreads();
+        lp_sync<THREADS>();
         int before = n + sum - mine, all = 0;
         for (int w = 0; w < S::WARPS; ++w) { if (w < warp) before += s.scan[w]; all += s.scan[w]; }
         for (; hit && before < top; hit &= hit - 1, ++before) s.list[before] = lp_rank(key, e + __ffs(hit) - 1);
         n = min(n + all, max(top, n));
       }
-      __syncthreads();
+      lp_sync<THREADS>();
     } else {
       // few threads with more than fits above it: one after the other
       u64 last = ~0ull;
@@ -243,158 +280,148 @@ __device__ __forceinline__ void lp_top(S& s, const LpRow<T>& row, int p0, int p1
 #pragma unroll
           for (int i = 0; i < N; ++i) {
             const u64 r = lp_rank(lp_key(v.at(i)), e + i);
-            if (r < last && r > best && e + i >= 0 && e + i < row.vocab) best = r;
+            if (r < last && r > best && row.holds(e + i)) best = r;
           }
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-        __syncthreads();
+        lp_sync<THREADS>();
         if (lane == 0) s.red[warp] = best;
-        __syncthreads();
+        lp_sync<THREADS>();
         for (int w = 0; w < S::WARPS; ++w) best = max(best, s.red[w]);
         last = best;
         if (tid == 0) s.best[k] = best;
       }
-      __syncthreads();
+      lp_sync<THREADS>();
       return;
     }
   }
-  for (int i = tid; i < n; i += THREADS) {
-    const u64 mine = s.list[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += s.list[j] > mine;
-    if (rank < top) s.best[rank] = mine;
-  }
-  __syncthreads();
+  lp_order<THREADS>(s, n, top, tid);
+  lp_sync<THREADS>();
 }
 
-// gridDim.x = rows * CTAs of a cluster; each cluster a row
+__device__ __forceinline__ LpSums lp_warp_join(LpSums a, int lanes = 32) {
+  LpSums to{a.m, 0.f, 0.f};
+  for (int o = lanes >> 1; o > 0; o >>= 1) to.m = fmaxf(to.m, __shfl_xor_sync(0xffffffffu, to.m, o));
+  if (to.m > a.m) a.raise(to.m);
+  for (int o = lanes >> 1; o > 0; o >>= 1) {
+    a.l += __shfl_xor_sync(0xffffffffu, a.l, o);
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+  }
+  return a;
+}
+
+// The sums of a piece's elements, added to l and s; NaN where an element is -inf (0 times infinity) unless FAR, which lets differences end at LP_FAR
+template <bool FAR, typename T>
+__device__ __forceinline__ void lp_add(const LpPiece<T>& v, u64 scale2, u64 neg_m2, u64& l2, u64& s2) {
+#pragma unroll
+  for (int i = 0; i < LpPiece<T>::N / 2; ++i) {
+    u64 d = f2_fma(v.pair(i), scale2, neg_m2);
+    if (FAR) {
+      uint32_t d0, d1;
+      f2_to(d, d0, d1);
+      d = f2_of(__float_as_uint(lp_max_nan(__uint_as_float(d0), LP_FAR)), __float_as_uint(lp_max_nan(__uint_as_float(d1), LP_FAR)));
+    }
+    const u64 e = exp2_mufu2(f2_mul(d, f2_splat(LP_LOG2E)));
+    l2 = f2_add(l2, e);
+    s2 = f2_fma(e, d, s2);
+  }
+}
+__device__ __forceinline__ float lp_both(u64 v) {
+  uint32_t a, b;
+  f2_to(v, a, b);
+  return __uint_as_float(a) + __uint_as_float(b);
+}
+
+// A team of THREADS to a row: 32, eight rows to a block of 256, or a block, gridDim.x = rows * CTAs of a cluster
 template <typename T, int THREADS, bool TOP>
-__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : 1) logprob_kernel(const __grid_constant__ LogprobParams p) {
+__global__ void __launch_bounds__(THREADS == 128 ? 128 : 256, THREADS == 128 ? 8 : 4) logprob_kernel(const __grid_constant__ LogprobParams p) {
   using S = LpShared<THREADS, TOP>;
-  constexpr int N = LpPiece<T>::N;
-  __shared__ S s;
+  constexpr int TEAMS = THREADS == 32 ? 8 : 1;
+  __shared__ S shared[TEAMS];
   pdl_launch_dependents();
   pdl_wait();
-  const cg::cluster_group cluster = cg::this_cluster();
-  const int parts = cluster.num_blocks(), part = cluster.block_rank(), r = blockIdx.x / parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  S& s = shared[TEAMS > 1 ? threadIdx.x >> 5 : 0];
+  int parts = 1, part = 0;
+  if constexpr (TEAMS == 1) {
+    parts = cg::this_cluster().num_blocks();
+    part = cg::this_cluster().block_rank();
+  }
+  const int r = TEAMS > 1 ? blockIdx.x * TEAMS + (threadIdx.x >> 5) : blockIdx.x / parts, tid = threadIdx.x % THREADS, lane = tid & 31, warp = tid >> 5;
+  if (TEAMS > 1 && r >= p.rows) return;
   const LpRow<T> row(static_cast<const T*>(p.x) + r * p.stride, p.vocab);
   const int all = row.pieces(), per = (all + parts - 1) / parts, p0 = min(part * per, all), p1 = min(p0 + per, all);
   LpSums a{-INFINITY, 0.f, 0.f};
   float tmax = -INFINITY;                  // of the logits themselves
-  u64 l2 = 0, s2 = 0;
-  const u64 scale2 = f2_splat(p.scale), log2e2 = f2_splat(LP_LOG2E);
+  const u64 scale2 = f2_splat(p.scale);
   for (int q = p0 + tid; q < p1; q += LP_BATCH * THREADS) {
     LpPiece<T> v[LP_BATCH];
 #pragma unroll
-    for (int b = 0; b < LP_BATCH; ++b) {
+    for (int b = 0; b < LP_BATCH; ++b)
       if (q + b * THREADS < p1) row.load(v[b], q + b * THREADS);
-      else v[b].none();
-    }
-    float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
     for (int b = 0; b < LP_BATCH; ++b)
-#pragma unroll
-      for (int i = 0; i < N; i += 4) {
-        m0 = fmax3(m0, v[b].at(i), v[b].at(i + 1));
-        m1 = fmax3(m1, v[b].at(i + 2), v[b].at(i + 3));
-      }
-    tmax = fmax3(tmax, m0, m1);
+      if (q + b * THREADS < p1) tmax = fmaxf(tmax, v[b].largest());
     const float top = tmax * p.scale;
-    if (top > a.m) {
-      uint32_t u[4];
-      f2_to(l2, u[0], u[1]);
-      f2_to(s2, u[2], u[3]);
-      a.l = __uint_as_float(u[0]) + __uint_as_float(u[1]);
-      a.s = __uint_as_float(u[2]) + __uint_as_float(u[3]);
-      a.raise(top);
-      l2 = f2_of(__float_as_uint(a.l), 0);
-      s2 = f2_of(__float_as_uint(a.s), 0);
-    }
+    if (top > a.m) a.raise(top);
     const u64 neg_m2 = f2_splat(a.m == -INFINITY ? 0.f : -a.m);
+    u64 l2 = 0, s2 = 0;
 #pragma unroll
     for (int b = 0; b < LP_BATCH; ++b)
+      if (q + b * THREADS < p1) lp_add<false>(v[b], scale2, neg_m2, l2, s2);
+    float s1 = lp_both(s2);
+    if (s1 != s1) {
+      l2 = s2 = 0;
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        uint32_t d0, d1;
-        f2_to(f2_fma(v[b].pair(i), scale2, neg_m2), d0, d1);
-        const u64 d = f2_of(__float_as_uint(lp_max_nan(__uint_as_float(d0), LP_FAR)), __float_as_uint(lp_max_nan(__uint_as_float(d1), LP_FAR)));
-        const u64 e = exp2_mufu2(f2_mul(d, log2e2));
-        l2 = f2_add(l2, e);
-        s2 = f2_fma(e, d, s2);
-      }
+      for (int b = 0; b < LP_BATCH; ++b)
+        if (q + b * THREADS < p1) lp_add<true>(v[b], scale2, neg_m2, l2, s2);
+      s1 = lp_both(s2);
+    }
+    a.l += lp_both(l2);
+    a.s += s1;
   }
-  {
-    uint32_t u[4];
-    f2_to(l2, u[0], u[1]);
-    f2_to(s2, u[2], u[3]);
-    a.l = __uint_as_float(u[0]) + __uint_as_float(u[1]);
-    a.s = __uint_as_float(u[2]) + __uint_as_float(u[3]);
+  a = lp_warp_join(a);
+  if (THREADS > 32) {
+    if (lane == 0) s.sums[warp] = a;
+    __syncthreads();
+    if (warp == 0) a = lp_warp_join(lane < S::WARPS ? s.sums[lane] : LpSums{-INFINITY, 0.f, 0.f});
+    if (parts > 1 && tid == 0) s.total = a;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    a.join({__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.l, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
-  if (lane == 0) s.sums[warp] = a;
-  if constexpr (TOP) lp_top<T, THREADS>(s, row, p0, p1, lp_key(tmax), p.top);
-  if (parts > 1) cluster.sync();
-  else __syncthreads();
-  if (part == 0) {
-    if (warp == 0) {
-      // one entry to a lane: the warps of this CTA, then those of the others
-      a = {-INFINITY, 0.f, 0.f};
-      for (int i = lane; i < parts * S::WARPS; i += 32) {
-        const int c = i / S::WARPS, w = i % S::WARPS;
-        const S* from = parts > 1 ? cluster.map_shared_rank(&s, c) : &s;
-        a.join(from->sums[w]);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-        a.join({__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.l, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
-      // +inf leaves NaN in the sums, like NaN itself
-      const bool none = a.m == -INFINITY && a.l == 0.f;
-      if (a.l != a.l) a.m = NAN;
-      const float log_l = none ? 0.f : logf(a.l);
-      const auto logprob = [&](float x) { return none ? -INFINITY : (fmaf(x, p.scale, -a.m)) - log_l; };
-      if (lane == 0) {
-        const int t = p.targets[r];
-        p.logprobs[r] = t == p.ignore ? 0.f : t >= 0 && t < p.vocab ? logprob(lp_load(row.x + t)) : NAN;
-        p.entropy[r] = none ? 0.f : log_l - a.s / a.l;
-        p.stats[2ll * r] = a.m;
-        p.stats[2ll * r + 1] = log_l;
-      }
-      if constexpr (TOP) {
-        const long long out = (long long)r * p.top;
-        const auto write = [&](int rank, u64 v) {
-          p.top_ids[out + rank] = (int)~(uint32_t)v;
-          p.top_logprobs[out + rank] = logprob(lp_unkey((uint32_t)(v >> 32)));
-        };
-        if (parts == 1) {
-          if (lane < p.top) write(lane, s.best[lane]);
-        } else {
-          // the CTAs' lists are in order: an element's rank is the sum of where it would stand in each
-          for (int i = lane; i < parts * p.top; i += 32) {
-            const int c = i / p.top;
-            const u64 mine = cluster.map_shared_rank(&s, c)->best[i % p.top];
-            if (mine == 0) continue;
-            int rank = i % p.top;
-            for (int o = 0; o < parts && rank < p.top; ++o) {
-              if (o == c) continue;
-              const S* from = cluster.map_shared_rank(&s, o);
-              int lo = 0, hi = p.top;
-              while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (from->best[mid] > mine) lo = mid + 1;
-                else hi = mid;
-              }
-              rank += lo;
-            }
-            if (rank < p.top) write(rank, mine);
-          }
+  if constexpr (TOP) lp_top<T, THREADS>(s, row, p0, p1, lp_key(tmax), p.top, tid);
+  if constexpr (TEAMS == 1) {
+    if (parts > 1) {
+      cg::this_cluster().sync();
+      if (part == 0) {
+        if (warp == 0) a = lp_warp_join(lane < parts ? cg::this_cluster().map_shared_rank(&s, lane)->total : LpSums{-INFINITY, 0.f, 0.f});
+        if constexpr (TOP) {
+          for (int i = tid; i < parts * p.top; i += THREADS) s.list[i] = cg::this_cluster().map_shared_rank(&s, i / p.top)->best[i % p.top];
+          __syncthreads();
+          lp_order<THREADS>(s, parts * p.top, p.top, tid);      // the largest of all are at least as many as this CTA's own: every place is written anew
         }
       }
+      cg::this_cluster().sync();           // the others' shared memory has been read
+      if (part != 0) return;
     }
   }
-  if (parts > 1) cluster.sync();           // the others' shared memory has been read
+  if (warp == 0) {
+    // +inf leaves NaN in the sums, like NaN itself
+    const bool none = a.m == -INFINITY && a.l == 0.f;
+    if (a.l != a.l) a.m = NAN;
+    const float log_l = none ? 0.f : logf(a.l);
+    const auto logprob = [&](float x) { return none ? -INFINITY : fmaf(x, p.scale, -a.m) - log_l; };
+    if (lane == 0) {
+      const int t = p.targets[r];
+      p.logprobs[r] = t == p.ignore ? 0.f : t >= 0 && t < p.vocab ? logprob(row.element(t)) : NAN;
+      p.entropy[r] = none ? 0.f : log_l - a.s / a.l;
+      p.stats[2ll * r] = a.m;
+      p.stats[2ll * r + 1] = log_l;
+    }
+    if (TOP && lane < p.top) {
+      const u64 v = s.best[lane];
+      p.top_ids[(long long)r * p.top + lane] = (int)~(uint32_t)v;
+      p.top_logprobs[(long long)r * p.top + lane] = logprob(lp_unkey((uint32_t)(v >> 32)));
+    }
+  }
 }
 
 struct LogprobBwdParams {
@@ -404,64 +431,85 @@ struct LogprobBwdParams {
   const float *entropy, *stats, *dlogprobs, *dentropy;
   void* dx;
   long long d_stride;
-  int rows, vocab, ignore;
+  int rows, vocab, ignore, team_log2;
   float scale;
 };
 
-// blockIdx.y: which part of the row's pieces.  Pieces are those of the logits; where the gradient's rows lie otherwise (`apart`) their elements are written
-// one by one.
-template <typename T>
-__global__ void __launch_bounds__(256) logprob_bwd_kernel(const __grid_constant__ LogprobBwdParams p) {
+// Blocks of 2^team_log2 threads to a row and 256 / 2^team_log2 rows; blockIdx.y: which part of the row's pieces, those of the logits.  Where the gradient's rows
+// lie otherwise (`apart`) their elements are written one by one.  ENTROPY: dentropy is given.
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(256, 5) logprob_bwd_kernel(const __grid_constant__ LogprobBwdParams p) {
   constexpr int N = LpPiece<T>::N;
   pdl_launch_dependents();
   pdl_wait();
-  const int r = blockIdx.x;
+  const int team = 1 << p.team_log2, r = (blockIdx.x << (8 - p.team_log2)) + (threadIdx.x >> p.team_log2);
+  if (r >= p.rows) return;
   const LpRow<T> row(static_cast<const T*>(p.x) + r * p.stride, p.vocab);
-  T* dx = static_cast<T*>(p.dx) + r * p.d_stride;
-  const bool apart = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(row.x)) & 15) != 0;
-  const float m = p.stats[2ll * r], log_l = p.stats[2ll * r + 1], H = p.entropy[r];
-  const int target = p.targets[r];
-  const float g = target == p.ignore || !p.dlogprobs ? 0.f : target >= 0 && target < p.vocab ? p.dlogprobs[r] * p.scale : NAN;
-  const float h = p.dentropy ? p.dentropy[r] * p.scale : 0.f;
-  const bool none = m == -INFINITY;
-  const u64 scale2 = f2_splat(p.scale), neg_m2 = f2_splat(none ? 0.f : -m), neg_l2 = f2_splat(-log_l), log2e2 = f2_splat(LP_LOG2E), h2 = f2_splat(none ? 0.f : h),
-            c2 = f2_splat(none ? 0.f : fmaf(h, H, g)), neg2 = f2_splat(-1.f);
-  const int all = row.pieces(), step = gridDim.y * 256;
-  for (int q = blockIdx.y * 256 + threadIdx.x; q < all; q += LP_BATCH * step) {
-    LpPiece<T> v[LP_BATCH];
+  T* dx = static_cast<T*>(p.dx) + r * p.d_stride - row.head;
+  const bool apart = (reinterpret_cast<uintptr_t>(dx) & 15) != 0;
+  const int all = row.pieces(), step = gridDim.y * team;
+  int q = blockIdx.y * team + (threadIdx.x & (team - 1));
+  LpPiece<T> v[LP_BATCH];
+  const auto fetch = [&] {
 #pragma unroll
     for (int b = 0; b < LP_BATCH; ++b)
       if (q + b * step < all) row.load(v[b], q + b * step);
+  };
+  fetch();                                 // beside the row's own numbers
+  const float m = p.stats[2ll * r], log_l = p.stats[2ll * r + 1];
+  const int target = p.targets[r];
+  const bool none = m == -INFINITY;        // no gradient at all
+  const float g = none || target == p.ignore || !p.dlogprobs ? 0.f : target >= 0 && target < p.vocab ? p.dlogprobs[r] * p.scale : NAN;
+  const float h = ENTROPY && !none ? p.dentropy[r] * p.scale : 0.f;
+  // dx = p_j (-h log p_j - (h H + g)), and g more at the target
+  const u64 scale2 = f2_splat(p.scale), neg_m2 = f2_splat(none ? 0.f : -m), neg_l2 = f2_splat(-log_l), h2 = f2_splat(-h),
+            c2 = f2_splat(-(ENTROPY && !none ? fmaf(h, p.entropy[r], g) : g));
+  while (q < all) {
 #pragma unroll
     for (int b = 0; b < LP_BATCH; ++b) {
-      if (q + b * step >= all) break;
-      const int e = row.first(q + b * step);
+      const int at = q + b * step;
+      if (at >= all) break;
 #pragma unroll
       for (int i = 0; i < N / 2; ++i) {
-        uint32_t d0, d1;
-        f2_to(f2_add(f2_fma(v[b].pair(i), scale2, neg_m2), neg_l2), d0, d1);
-        const u64 d = f2_of(__float_as_uint(lp_max_nan(__uint_as_float(d0), LP_FAR)), __float_as_uint(lp_max_nan(__uint_as_float(d1), LP_FAR)));
-        const u64 w = f2_mul(exp2_mufu2(f2_mul(d, log2e2)), f2_fma(h2, d, c2));
-        u64 out = f2_mul(w, neg2);
-        if (e + 2 * i == target || e + 2 * i + 1 == target) out = f2_add(out, e + 2 * i == target ? f2_of(__float_as_uint(none ? 0.f : g), 0) : f2_of(0, __float_as_uint(none ? 0.f : g)));
-        v[b].set(i, out);
+        u64 d = f2_add(f2_fma(v[b].pair(i), scale2, neg_m2), neg_l2), f = c2;
+        if (ENTROPY) {
+          uint32_t d0, d1;
+          f2_to(d, d0, d1);
+          d = f2_of(__float_as_uint(lp_max_nan(__uint_as_float(d0), LP_FAR)), __float_as_uint(lp_max_nan(__uint_as_float(d1), LP_FAR)));
+          f = f2_fma(h2, d, c2);
+        }
+        v[b].set(i, f2_mul(exp2_mufu2(f2_mul(d, f2_splat(LP_LOG2E))), f));
       }
-      if (row.whole(e) && !apart) {
-        *reinterpret_cast<uint4*>(dx + e) = make_uint4(v[b].w[0], v[b].w[1], v[b].w[2], v[b].w[3]);
+      const int hit = target - row.first(at);
+      if ((unsigned)hit < (unsigned)N && row.holds(target) && !none) {      // its logit still stands where the gradient may go
+        const float d = lp_max_nan(fmaf(row.element(target), p.scale, -m) - log_l, LP_FAR);
+        uint32_t c, unused;
+        f2_to(c2, c, unused);
+        const float w = fmaf(fast_exp2(d * LP_LOG2E), fmaf(-h, d, __uint_as_float(c)), g);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (i == hit) v[b].set1(i, w);
+      }
+      if (row.whole(at) && !apart) {
+        reinterpret_cast<uint4*>(dx)[at] = make_uint4(v[b].w[0], v[b].w[1], v[b].w[2], v[b].w[3]);
       } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          if (e + i >= 0 && e + i < p.vocab) v[b].get(i, dx + e + i);
+          if (row.holds(row.first(at) + i)) v[b].get(i, dx + at * N + i);
       }
     }
+    q += LP_BATCH * step;
+    fetch();
   }
 }
 
 template <typename T, int THREADS>
 static int logprob_launch(const LogprobParams& p, int parts, cudaStream_t st) {
+  const long long blocks = THREADS == 32 ? ((long long)p.rows + 7) / 8 : (long long)p.rows * parts;
+  if (blocks > 0x7fffffffll) return OA_ERR_TOO_LARGE;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((long long)p.rows * parts));
-  cfg.blockDim = dim3(THREADS);
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(THREADS == 32 ? 256 : THREADS);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -470,21 +518,35 @@ static int logprob_launch(const LogprobParams& p, int parts, cudaStream_t st) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_on((long long)p.rows * parts <= PDL_SHORT_BLOCKS) ? 2 : 1;
+  cfg.numAttrs = pdl_on(blocks <= PDL_SHORT_BLOCKS) ? 2 : 1;
   const cudaError_t rc = p.top > 0 ? cudaLaunchKernelEx(&cfg, logprob_kernel<T, THREADS, true>, p) : cudaLaunchKernelEx(&cfg, logprob_kernel<T, THREADS, false>, p);
   return rc == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }
 
 template <typename T>
 static int logprob_run(const LogprobParams& p, cudaStream_t st) {
-  // As many CTAs to a row as leave no SM without one, each with 2048 elements at least; threads by what is left for them
+  // A warp to a row of up to 2048 elements; otherwise as many CTAs to a row as leave no SM without two, each with 2048 elements at least.  Smaller CTAs cover
+  // one another's meetings where there are several waves of them (bf16, five alternatives, threads 128 / 256: 4096 x 32000 66.6 / 74.8 us, 16384 x 8000 98 /
+  // 161), larger ones end sooner where there is one (32 x 201088 12.2 / 11.3, 64 x 50257 9.1 / 8.8) or a thread has many pieces (fp32, twenty alternatives, 4096 x 32000
+  // 143 / 123).
+  if (p.vocab <= 2048) return logprob_launch<T, 32>(p, 1, st);
   int parts = 1;
-  while (parts < 8 && (long long)p.rows * parts * 2 <= 2 * sm_count() && p.vocab / (2 * parts) >= 2048) parts *= 2;
-  const int share = p.vocab / parts;
-  if ((long long)p.rows * parts > 0x7fffffffll) return OA_ERR_TOO_LARGE;
-  if (share <= 1024) return logprob_launch<T, 32>(p, parts, st);
-  if (share <= 8192) return logprob_launch<T, 128>(p, parts, st);
-  return logprob_launch<T, 512>(p, parts, st);
+  while (parts < 8 && (long long)p.rows * parts <= 2 * sm_count() && p.vocab / (2 * parts) >= 2048) parts *= 2;
+  if (p.rows >= 4 * sm_count() && p.vocab / LpPiece<T>::N <= 4200) return logprob_launch<T, 128>(p, parts, st);
+  return logprob_launch<T, 256>(p, parts, st);
+}
+
+template <typename T>
+static int logprob_bwd_run(LogprobBwdParams& p, cudaStream_t st) {
+  // threads to a row that four pieces each fill, and as many blocks side by side as it then still takes
+  const long long pieces = (long long)p.vocab / LpPiece<T>::N + 2;
+  p.team_log2 = 3;
+  while (p.team_log2 < 8 && (LP_BATCH << p.team_log2) < pieces) ++p.team_log2;
+  const long long parts = (pieces + (LP_BATCH << p.team_log2) - 1) / (LP_BATCH << p.team_log2);
+  const dim3 grid((unsigned)(((long long)p.rows + (256 >> p.team_log2) - 1) >> (8 - p.team_log2)), (unsigned)(parts < 65535 ? parts : 65535));
+  if (p.dentropy) launch_short(logprob_bwd_kernel<T, true>, grid, dim3(256), 0, st, p);
+  else launch_short(logprob_bwd_kernel<T, false>, grid, dim3(256), 0, st, p);
+  return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }
 
 }  // namespace oa
@@ -509,11 +571,6 @@ extern "C" int oa_token_logprobs_bwd(int dtype, const void* logits, long long st
   if (rows < 0 || vocab < 1 || stride < 0 || (rows > 1 && d_stride < vocab) || !(scale > 0.f)) return OA_ERR_ARG;
   if (vocab > 0x7ffffff0) return OA_ERR_TOO_LARGE;
   if (rows == 0) return OA_OK;
-  const LogprobBwdParams p{logits, stride, targets, entropy, stats, dlogprobs, dentropy, dlogits, d_stride, rows, vocab, ignore_index, scale};
-  // four pieces to a thread
-  const int n = dtype == OA_F32 ? 4 : 8, per = 256 * LP_BATCH * n, parts = (int)(((long long)vocab + per) / per);
-  const dim3 grid((unsigned)rows, (unsigned)(parts < 65535 ? parts : 65535));
-  if (dtype == OA_F32) launch_short(logprob_bwd_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, p);
-  else launch_short(logprob_bwd_kernel<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, p);
-  return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
+  LogprobBwdParams p{logits, stride, targets, entropy, stats, dlogprobs, dentropy, dlogits, d_stride, rows, vocab, ignore_index, 0, scale};
+  return dtype == OA_F32 ? logprob_bwd_run<float>(p, (cudaStream_t)stream) : logprob_bwd_run<__nv_bfloat16>(p, (cudaStream_t)stream);
 }

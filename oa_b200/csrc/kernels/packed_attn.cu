@@ -20,31 +20,34 @@
 namespace oa {
 
 // A CTA's work items: (tile or pair of tiles, one of `per` heads or pairs of heads), all of the longest tiles first, in snake order over the
-// CTAs (round r: CTA c takes item r G + c, or r G + G - 1 - c when r is odd).  Every warp walks them alike: fetch() sends for the plan's entry of the
-// next item, take() waits for it.
+// CTAs (round r: CTA c takes item r G + c, or r G + G - 1 - c when r is odd).  Every warp walks them alike.  The plan's entries of the first rounds are
+// fetched to shared memory at the start: with a load from L2 for each item, sent for during the one before, the kernels took 6 to 13 % longer.
+constexpr int PACKED_ROUNDS = 128;
 template <bool PAIRS>
 struct PackedWalk {
   const PackedPlan& plan;
+  const int4* kept;
   const int per, n;
   int round, item;
-  int4 ahead;
-  __device__ __forceinline__ PackedWalk(const PackedPlan& p, int heads) : plan(p), per(heads), n((PAIRS ? p.pairs() : p.tiles()) * heads), round(0), item(blockIdx.x) { fetch(); }
-  __device__ __forceinline__ void fetch() {
-    if (item < n) ahead = PAIRS ? plan.pair(item / per) : plan.tile(item / per);
+  __device__ __forceinline__ PackedWalk(const PackedPlan& p, int heads, int4* room)
+      : plan(p), kept(room), per(heads), n((PAIRS ? p.pairs() : p.tiles()) * heads), round(0), item(blockIdx.x) {
+    for (int r = threadIdx.x; r < PACKED_ROUNDS; r += blockDim.x) {
+      const int i = at(r);
+      if (i < n) room[r] = entry_of(i);
+    }
+    __syncthreads();
   }
-  // false: no item left; otherwise the plan's entry and which of the heads
-  __device__ __forceinline__ bool take(int4& entry, int& which) {
-    if (item >= n) return false;
-    entry = ahead;
-    which = item % per;
-    ++round;
+  __device__ __forceinline__ int at(int r) const {
     const int g = gridDim.x;
-    item = round * g + ((round & 1) ? g - 1 - (int)blockIdx.x : (int)blockIdx.x);
-    return true;
+    return r * g + ((r & 1) ? g - 1 - (int)blockIdx.x : (int)blockIdx.x);
   }
+  __device__ __forceinline__ int4 entry_of(int i) const { return PAIRS ? plan.pair(i / per) : plan.tile(i / per); }
+  // false: no item left; otherwise the plan's entry and which of the heads
   __device__ __forceinline__ bool next(int4& entry, int& which) {
-    if (!take(entry, which)) return false;
-    fetch();
+    if (item >= n) return false;
+    entry = round < PACKED_ROUNDS ? kept[round] : entry_of(item);
+    which = item % per;
+    item = at(++round);
     return true;
   }
 };
@@ -88,7 +91,8 @@ struct PackedFwdCfg {
   static constexpr int OFF_K = OFF_Q + 2 * Q_BYTES;
   static constexpr int OFF_V = OFF_K + NS * KV_BYTES;
   static constexpr int OFF_BAR = OFF_V + NS * KV_BYTES;
-  static constexpr int SMEM_BYTES = OFF_BAR + 256;
+  static constexpr int OFF_ITEMS = OFF_BAR + 256;
+  static constexpr int SMEM_BYTES = OFF_ITEMS + PACKED_ROUNDS * 16;
   static constexpr int TMEM_COLS = 512;
   static constexpr int TM_S = 0, TM_P = ALIAS ? 0 : 256, P_STEP = ALIAS ? FA_BN : 64, TM_O = ALIAS ? 256 : 384;   // S: + 128 * tile, O: + HD * tile
   static constexpr int MMA_WARPS = ALIAS ? 1 : 2, TMA_WARP = 8 + MMA_WARPS;   // after 8 softmax warps
@@ -156,12 +160,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();                            // the prologue above ran under the previous kernel's tail; global memory from here on
 
-  const auto waited = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-    const bool ok = warp_wait(bar, parity);
-    if (!ok && lane == 0) report_error(p.status, code);
-    return ok;
-  };
-  PackedWalk<!HEADS> walk(p.plan, HEADS ? p.q_heads >> 1 : p.q_heads);
+  PackedWalk<!HEADS> walk(p.plan, HEADS ? p.q_heads >> 1 : p.q_heads, reinterpret_cast<int4*>(smem + Cfg::OFF_ITEMS));
   int4 entry;
   int which;
 
@@ -172,7 +171,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     while (ok && walk.next(entry, which)) {
       const PackedFwdItem<HEADS> it(p, entry, which);
       const int n_it = max(it.n[0], it.n[1]);
-      if (!waited(q_empty, (itc & 1) ^ 1, OA_KERR_WAIT_EMPTY)) break;
+      if (!warp_wait(q_empty, (itc & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
       if (elect_one()) {
         const int tiles = it.n[1] > 0 ? 2 : 1;
         mbar_expect_tx(q_full, tiles * Cfg::Q_BYTES);
@@ -184,14 +183,14 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       for (int j = 0; j < n_it; ++j, ++blk) {
         const int st = blk % NS, row = it.lo + j * FA_BN;
         const uint32_t ph = (blk / NS) & 1;
-        if (!waited(&k_empty[st], ph ^ 1, OA_KERR_WAIT_EMPTY)) { ok = false; break; }
+        if (!warp_wait(&k_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
         if (elect_one()) {
           mbar_expect_tx(&k_full[st], Cfg::KV_BYTES);
 #pragma unroll
           for (int x = 0; x < HD / 64; ++x)
             tma_load_2d(smem + Cfg::OFF_K + st * Cfg::KV_BYTES + x * (FA_BN * 128), &tmK, &k_full[st], it.kv_head * HD + x * 64, row);
         }
-        if (!waited(&v_empty[st], ph ^ 1, OA_KERR_WAIT_EMPTY)) { ok = false; break; }
+        if (!warp_wait(&v_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
         const bool part = row + FA_BN > it.hi;
         uint8_t* v_tile = smem + Cfg::OFF_V + st * Cfg::KV_BYTES;
         if (elect_one()) {
@@ -202,7 +201,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         __syncwarp();
         if (part) {
-          if (!waited(v_part, parts & 1, OA_KERR_WAIT_FULL)) { ok = false; break; }
+          if (!warp_wait(v_part, parts & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
           ++parts;
           clear_rows<HD>(v_tile, it.hi - row, lane);
           fence_proxy_async_smem();
@@ -223,7 +222,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     // S_t = Q_t K^T of ring block `blk`; `first` / `last`: of the tiles that read it, `end`: nothing reads Q after it
     auto issue_qk = [&](int t, uint32_t blk, bool first, bool last, bool end) -> bool {
       const int st = blk % NS;
-      if (first && !waited(&k_full[st], (blk / NS) & 1, OA_KERR_WAIT_FULL)) return false;
+      if (first && !warp_wait(&k_full[st], (blk / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
       tc_fence_after();
       if (elect_one()) {
         const uint64_t qd = desc_at(q_desc, t * Cfg::Q_BYTES), kd = desc_at(k_desc, st * Cfg::KV_BYTES);
@@ -242,7 +241,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     while (ok && walk.next(entry, which)) {
       const PackedFwdItem<HEADS> item(p, entry, which);
       const int n[2] = {item.n[0], item.n[1]}, n_it = max(n[0], n[1]);
-      if (!waited(q_full, itc & 1, OA_KERR_WAIT_FULL)) break;
+      if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
       // a block's tiles: both, or the one whose row of blocks is longer (tile 1, unless it is absent)
       auto qk = [&](int t, int j) -> bool {
         const bool last = j >= n[1 - t] || t == 1;
@@ -252,13 +251,13 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (ok && n[1] > 0) ok = qk(1, 0);
       for (int j = 0; j < n_it && ok; ++j) {
         const int st = (base + j) % NS;
-        if (!waited(&v_full[st], ((base + j) / NS) & 1, OA_KERR_WAIT_FULL)) { ok = false; break; }
+        if (!warp_wait(&v_full[st], ((base + j) / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (j >= n[t]) continue;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            if (!waited(&p_full[2 * t + half], pc[t] & 1, OA_KERR_WAIT_SOFTMAX)) { ok = false; break; }
+            if (!warp_wait(&p_full[2 * t + half], pc[t] & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
             tc_fence_after();
             if (elect_one()) {
               const uint64_t vd = desc_at(v_desc, st * Cfg::KV_BYTES);
@@ -292,8 +291,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     bool ok = true;
     auto issue_qk = [&](uint32_t blk, bool last) -> bool {       // S_t = Q_t K^T of ring block `blk`
       const int st = blk % NS;
-      if (!waited(&k_full[st], (blk / NS) & 1, OA_KERR_WAIT_FULL)) return false;
-      if (sc > 0 && !waited(&s_empty[t], (sc - 1) & 1, OA_KERR_WAIT_TMEM_EMPTY)) return false;
+      if (!warp_wait(&k_full[st], (blk / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
+      if (sc > 0 && !warp_wait(&s_empty[t], (sc - 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); return false; }
       tc_fence_after();
       if (elect_one()) {
         const uint64_t kd = desc_at(k_desc, st * Cfg::KV_BYTES);
@@ -313,13 +312,13 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     while (ok && walk.next(entry, which)) {
       const PackedFwdItem<HEADS> item(p, entry, which);
       const int n_it = max(item.n[0], item.n[1]), n = t == 0 ? item.n[0] : item.n[1];
-      if (!waited(q_full, itc & 1, OA_KERR_WAIT_FULL)) break;
+      if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
       if (n > 0) ok = issue_qk(base, n == 1);
       for (int j = 0; j < n && ok; ++j) {
         if (j + 1 < n) { ok = issue_qk(base + j + 1, j + 2 == n); if (!ok) break; }
         const int st = (base + j) % NS;
-        if (!waited(&v_full[st], ((base + j) / NS) & 1, OA_KERR_WAIT_FULL)) { ok = false; break; }
-        if (!waited(&p_full[2 * t], pc & 1, OA_KERR_WAIT_SOFTMAX)) { ok = false; break; }
+        if (!warp_wait(&v_full[st], ((base + j) / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+        if (!warp_wait(&p_full[2 * t], pc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
         tc_fence_after();
         if (elect_one()) {
           const uint64_t vd = desc_at(v_desc, st * Cfg::KV_BYTES);
@@ -337,9 +336,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       for (int j = n; j < n_it && ok; ++j) {
         const int st = (base + j) % NS;
         const uint32_t ph = ((base + j) / NS) & 1;
-        if (!waited(&k_full[st], ph, OA_KERR_WAIT_FULL)) { ok = false; break; }
+        if (!warp_wait(&k_full[st], ph)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
         if (lane == 0) mbar_arrive(&k_empty[st]);
-        if (!waited(&v_full[st], ph, OA_KERR_WAIT_FULL)) { ok = false; break; }
+        if (!warp_wait(&v_full[st], ph)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
         if (lane == 0) mbar_arrive(&v_empty[st]);
         __syncwarp();
       }
@@ -366,15 +365,15 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       p.plan.others(blockIdx.x, gridDim.x, [&](int row) {
         for (int h = threadIdx.x; h < p.q_heads; h += 256) p.lse[(long long)h * p.plan.tokens + row] = -INFINITY;
       });
-    while (ok && walk.take(entry, which)) {
+    while (ok && walk.next(entry, which)) {
       const int tile = HEADS ? entry.z : 2 * entry.z + t, head = HEADS ? 2 * which + t : which, hi = entry.y;
       const int q0 = entry.x + tile * FA_BM + quad * 32;    // this warp's first row
-      if (entry.x + tile * FA_BM >= hi) { walk.fetch(); continue; }
+      if (entry.x + tile * FA_BM >= hi) continue;
       const int n = tile + 1;
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = 0; j < n; ++j, ++sc) {
-        ok = waited(&s_full[t], sc & 1, OA_KERR_WAIT_TMEM_FULL);
-        if (!ok) break;
+        ok = warp_wait(&s_full[t], sc & 1);
+        if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
         tc_fence_after();
         uint32_t sv[FA_BN];
 #pragma unroll
@@ -406,8 +405,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         // P_t is free and O_t is complete once the previous P V has finished (head dim 128: s_full already says so, the scores were
         // issued behind it)
         if (!ALIAS && j > 0) {
-          ok = waited(&o_done[t], pc & 1, OA_KERR_WAIT_TMEM_FULL);
-          if (!ok) break;
+          ok = warp_wait(&o_done[t], pc & 1);
+          if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
           ++pc;
           tc_fence_after();
         }
@@ -461,9 +460,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         m_run = m_cand;
       }
       if (!ok) break;
-      walk.fetch();
-      ok = waited(&o_done[t], pc & 1, OA_KERR_WAIT_TMEM_FULL);
-      if (!ok) break;
+      ok = warp_wait(&o_done[t], pc & 1);
+      if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
       ++pc;
       tc_fence_after();
       const float inv = 1.f / l_run;
@@ -544,7 +542,8 @@ struct PackedKvCfg {
   static constexpr int OFF_DO = OFF_Q + NST * T_BYTES;
   static constexpr int OFF_STAT = OFF_DO + NST * T_BYTES;   // float[NST][256]: -lse*log2e | -delta*scale of the query block
   static constexpr int OFF_BAR = OFF_STAT + NST * 256 * 4;
-  static constexpr int SMEM_BYTES = OFF_BAR + 224;
+  static constexpr int OFF_ITEMS = OFF_BAR + 224;
+  static constexpr int SMEM_BYTES = OFF_ITEMS + PACKED_ROUNDS * 16;
   static constexpr int TMEM_COLS = 512;
   static constexpr int TM_S = 0, TM_DP = NS * FA_BN, TM_DV = TM_DP + FA_BN, TM_DK = TM_DV + HD;
 };
@@ -608,12 +607,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();                            // the prologue above ran under the previous kernel's tail; global memory from here on
 
-  const auto waited = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-    const bool ok = warp_wait(bar, parity);
-    if (!ok && lane == 0) report_error(p.status, code);
-    return ok;
-  };
-  PackedWalk<false> walk(p.plan, p.kv_heads);
+  PackedWalk<false> walk(p.plan, p.kv_heads, reinterpret_cast<int4*>(smem + Cfg::OFF_ITEMS));
   int4 entry;
   int which;
 
@@ -623,7 +617,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     bool ok = true;
     while (ok && walk.next(entry, which)) {
       const PackedKvItem it(entry, which);
-      if (!waited(kv_empty, (itc & 1) ^ 1, OA_KERR_WAIT_EMPTY)) break;
+      if (!warp_wait(kv_empty, (itc & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
       if (elect_one()) {
         mbar_expect_tx(kv_full, 2 * Cfg::T_BYTES);
 #pragma unroll
@@ -641,14 +635,14 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           const int qrow = it.lo + it.key0 + i * FA_BM;
           const bool part = qrow + FA_BM > it.hi;
           uint8_t *q_tile = smem + Cfg::OFF_Q + st * Cfg::T_BYTES, *do_tile = smem + Cfg::OFF_DO + st * Cfg::T_BYTES;
-          if (!waited(&q_empty[st], ph ^ 1, OA_KERR_WAIT_EMPTY)) { ok = false; break; }
+          if (!warp_wait(&q_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
           if (elect_one()) {
             uint64_t* bar = part ? part_full : &q_full[st];
             mbar_expect_tx(bar, part ? 2 * Cfg::T_BYTES : Cfg::T_BYTES);
 #pragma unroll
             for (int x = 0; x < HD / 64; ++x) tma_load_2d(q_tile + x * (FA_BM * 128), &tmQ, bar, h * HD + x * 64, qrow);
           }
-          if (!waited(&do_empty[st], ph ^ 1, OA_KERR_WAIT_EMPTY)) { ok = false; break; }
+          if (!warp_wait(&do_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
           if (elect_one()) {
             uint64_t* bar = part ? part_full : &do_full[st];
             if (!part) mbar_expect_tx(bar, Cfg::T_BYTES);
@@ -673,7 +667,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           }
           __syncwarp();
           if (part) {
-            if (!waited(part_full, parts & 1, OA_KERR_WAIT_FULL)) { ok = false; break; }
+            if (!warp_wait(part_full, parts & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
             ++parts;
             clear_rows<HD>(q_tile, it.hi - qrow, lane);
             clear_rows<HD>(do_tile, it.hi - qrow, lane);
@@ -696,7 +690,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     bool ok = true;
     auto issue_s = [&](uint32_t n, bool last) -> bool {
       const int st = n % NST;
-      if (!waited(&q_full[st], (n / NST) & 1, OA_KERR_WAIT_FULL)) return false;
+      if (!warp_wait(&q_full[st], (n / NST) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
       tc_fence_after();
       if (elect_one()) {
         const uint64_t qd = desc_at(q_desc, st * Cfg::T_BYTES);
@@ -714,19 +708,19 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     };
     while (ok && walk.next(entry, which)) {
       const int n_it = PackedKvItem(entry, which).blocks * p.group;
-      if (!waited(kv_full, itc & 1, OA_KERR_WAIT_FULL)) break;
+      if (!warp_wait(kv_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
       ok = issue_s(qc, n_it == 1);
       // the previous item's dV / dK were read by the softmax warps before they produced this item's first P^T, dS^T
       for (int it = 0; it < n_it && ok; ++it, ++qc) {
         if (NS == 2 && it + 1 < n_it) { ok = issue_s(qc + 1, it + 2 == n_it); if (!ok) break; }
         const int st = qc % NST;
-        if (!waited(&do_full[st], (qc / NST) & 1, OA_KERR_WAIT_FULL)) { ok = false; break; }
+        if (!warp_wait(&do_full[st], (qc / NST) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
         const uint64_t bd = desc_at(do_desc, st * Cfg::T_BYTES);
         const uint32_t a_addr = tmem_base + Cfg::TM_S + (qc % NS) * FA_BN;
         for (int half = 0; half < 2; ++half) {
           // an item's first product replaces the accumulator: wait until both halves' warps have read the previous item's
-          if (it == 0 && half == 0) ok = waited(&p_full[(qc % NS) * 2 + 1], (qc / NS) & 1, OA_KERR_WAIT_SOFTMAX);
-          if (!ok || !waited(&p_full[(qc % NS) * 2 + half], (qc / NS) & 1, OA_KERR_WAIT_SOFTMAX)) { ok = false; break; }
+          if (it == 0 && half == 0) ok = warp_wait(&p_full[(qc % NS) * 2 + 1], (qc / NS) & 1);
+          if (!ok || !warp_wait(&p_full[(qc % NS) * 2 + half], (qc / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -758,7 +752,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     bool ok = true;
     auto issue_dp = [&](uint32_t n, bool last) -> bool {
       const int st = n % NST;
-      if (!waited(&do_full[st], (n / NST) & 1, OA_KERR_WAIT_FULL)) return false;
+      if (!warp_wait(&do_full[st], (n / NST) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
       tc_fence_after();
       if (elect_one()) {
         const uint64_t dd = desc_at(do_desc, st * Cfg::T_BYTES);
@@ -776,19 +770,19 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     };
     while (ok && walk.next(entry, which)) {
       const int n_it = PackedKvItem(entry, which).blocks * p.group;
-      if (!waited(kv_full, itc & 1, OA_KERR_WAIT_FULL)) break;
+      if (!warp_wait(kv_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
       ok = issue_dp(qc, n_it == 1);
       for (int it = 0; it < n_it && ok; ++it, ++qc) {
         const int st = qc % NST;
-        if (!waited(&q_full[st], (qc / NST) & 1, OA_KERR_WAIT_FULL)) { ok = false; break; }
+        if (!warp_wait(&q_full[st], (qc / NST) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
         const uint64_t bd = desc_at(q_desc, st * Cfg::T_BYTES);
         if (NS == 1 && it + 1 < n_it) {
-          if (!waited(turn, turns & 1, OA_KERR_WAIT_EMPTY)) { ok = false; break; }
+          if (!warp_wait(turn, turns & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
           ++turns;
         }
         for (int half = 0; half < 2; ++half) {
-          if (it == 0 && half == 0) ok = waited(&ds_full[1], qc & 1, OA_KERR_WAIT_SOFTMAX);   // as for dV
-          if (!ok || !waited(&ds_full[half], qc & 1, OA_KERR_WAIT_SOFTMAX)) { ok = false; break; }
+          if (it == 0 && half == 0) ok = warp_wait(&ds_full[1], qc & 1);   // as for dV
+          if (!ok || !warp_wait(&ds_full[half], qc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -823,9 +817,9 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       for (int it = 0, i = 0; it < n_it; ++it, ++qc, i = i + 1 < item.blocks ? i + 1 : 0) {
         const int st = qc % NST;
         const float* st_cur = stat + st * 256 + half * 64;
-        ok = waited(&q_full[st], (qc / NST) & 1, OA_KERR_WAIT_FULL);   // statistics of this block are staged
-        if (ok) ok = waited(&s_full[qc % NS], (qc / NS) & 1, OA_KERR_WAIT_TMEM_FULL);
-        if (!ok) break;
+        ok = warp_wait(&q_full[st], (qc / NST) & 1);   // statistics of this block are staged
+        if (ok) ok = warp_wait(&s_full[qc % NS], (qc / NS) & 1);
+        if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
         tc_fence_after();
         const uint32_t s_addr = t_lane + Cfg::TM_S + (qc % NS) * FA_BN + half * 64;
         const uint32_t dp_addr = t_lane + Cfg::TM_DP + half * 64;
@@ -857,8 +851,8 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[(qc % NS) * 2 + half]);
-        ok = waited(dp_full, qc & 1, OA_KERR_WAIT_TMEM_FULL);
-        if (!ok) break;
+        ok = warp_wait(dp_full, qc & 1);
+        if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
         tc_fence_after();
         uint32_t dp[64];
         tmem_ld32(dp_addr, dp);
@@ -881,8 +875,8 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (lane == 0) mbar_arrive(&ds_full[half]);
       }
       if (!ok) break;
-      ok = waited(fin_full, itc & 1, OA_KERR_WAIT_TMEM_FULL);
-      if (!ok) break;
+      ok = warp_wait(fin_full, itc & 1);
+      if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
       ++itc;
       tc_fence_after();
       const int k0 = item.lo + item.key0 + quad * 32;   // accumulator rows are keys
@@ -917,7 +911,8 @@ struct PackedQCfg {
   static constexpr int OFF_K = OFF_DO + T_BYTES;
   static constexpr int OFF_V = OFF_K + NK * T_BYTES;
   static constexpr int OFF_BAR = OFF_V + NV * T_BYTES;
-  static constexpr int SMEM_BYTES = OFF_BAR + 224;
+  static constexpr int OFF_ITEMS = OFF_BAR + 224;
+  static constexpr int SMEM_BYTES = OFF_ITEMS + PACKED_ROUNDS * 16;
   static constexpr int TMEM_COLS = 512;
   static constexpr int TM_S = 0, TM_DP = 256, TM_DQ = 384;   // two score buffers; dS over dP
 };
@@ -970,12 +965,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();                            // the prologue above ran under the previous kernel's tail; global memory from here on
 
-  const auto waited = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-    const bool ok = warp_wait(bar, parity);
-    if (!ok && lane == 0) report_error(p.status, code);
-    return ok;
-  };
-  PackedWalk<false> walk(p.plan, p.q_heads);
+  PackedWalk<false> walk(p.plan, p.q_heads, reinterpret_cast<int4*>(smem + Cfg::OFF_ITEMS));
   int4 entry;
   int which;
 
@@ -984,7 +974,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     bool ok = true;
     while (ok && walk.next(entry, which)) {
       const int lo = entry.x, hi = entry.y, n_kv = entry.z + 1, h = which, hk = which / p.group, qrow = lo + entry.z * FA_BM;
-      if (!waited(q_empty, (itc & 1) ^ 1, OA_KERR_WAIT_EMPTY)) break;
+      if (!warp_wait(q_empty, (itc & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
       if (elect_one()) {
         mbar_expect_tx(q_full, 2 * Cfg::T_BYTES);
 #pragma unroll
@@ -997,14 +987,14 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         const int sk = kc % NK, sv = kc % NV, row = lo + j * FA_BN;
         const bool part = row + FA_BN > hi;
         uint8_t *k_tile = smem + Cfg::OFF_K + sk * Cfg::T_BYTES, *v_tile = smem + Cfg::OFF_V + sv * Cfg::T_BYTES;
-        if (!waited(&k_empty[sk], ((kc / NK) & 1) ^ 1, OA_KERR_WAIT_EMPTY)) { ok = false; break; }
+        if (!warp_wait(&k_empty[sk], ((kc / NK) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
         if (elect_one()) {
           uint64_t* bar = part ? part_full : &k_full[sk];
           mbar_expect_tx(bar, part ? 2 * Cfg::T_BYTES : Cfg::T_BYTES);
 #pragma unroll
           for (int x = 0; x < HD / 64; ++x) tma_load_2d(k_tile + x * (FA_BN * 128), &tmK, bar, hk * HD + x * 64, row);
         }
-        if (!waited(&v_empty[sv], ((kc / NV) & 1) ^ 1, OA_KERR_WAIT_EMPTY)) { ok = false; break; }
+        if (!warp_wait(&v_empty[sv], ((kc / NV) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
         if (elect_one()) {
           uint64_t* bar = part ? part_full : &v_full[sv];
           if (!part) mbar_expect_tx(bar, Cfg::T_BYTES);
@@ -1013,7 +1003,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         }
         __syncwarp();
         if (part) {
-          if (!waited(part_full, parts & 1, OA_KERR_WAIT_FULL)) { ok = false; break; }
+          if (!warp_wait(part_full, parts & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
           ++parts;
           clear_rows<HD>(k_tile, hi - row, lane);
           clear_rows<HD>(v_tile, hi - row, lane);
@@ -1033,11 +1023,11 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     bool ok = true;
     while (ok && walk.next(entry, which)) {
       const int n_kv = entry.z + 1;
-      if (!waited(q_full, itc & 1, OA_KERR_WAIT_FULL)) break;
+      if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
       for (int j = 0; j < n_kv; ++j, ++kc) {
         const int st = kc % NK;
-        if (!waited(&k_full[st], (kc / NK) & 1, OA_KERR_WAIT_FULL)) { ok = false; break; }
-        if (kc > 1 && !waited(&s_empty[kc & 1], ((kc >> 1) - 1) & 1, OA_KERR_WAIT_TMEM_EMPTY)) { ok = false; break; }
+        if (!warp_wait(&k_full[st], (kc / NK) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+        if (kc > 1 && !warp_wait(&s_empty[kc & 1], ((kc >> 1) - 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); ok = false; break; }
         tc_fence_after();
         if (elect_one()) {
           const uint64_t kd = desc_at(k_desc, st * Cfg::T_BYTES);
@@ -1063,7 +1053,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     bool ok = true;
     auto issue_dp = [&](uint32_t n, bool last) -> bool {
       const int st = n % NV;
-      if (!waited(&v_full[st], (n / NV) & 1, OA_KERR_WAIT_FULL)) return false;
+      if (!warp_wait(&v_full[st], (n / NV) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
       tc_fence_after();
       if (elect_one()) {
         const uint64_t vd = desc_at(v_desc, st * Cfg::T_BYTES);
@@ -1081,16 +1071,16 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     };
     while (ok && walk.next(entry, which)) {
       const int n_kv = entry.z + 1;
-      if (!waited(q_full, itc & 1, OA_KERR_WAIT_FULL)) break;
+      if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
       ok = issue_dp(kc, n_kv == 1);
       for (int j = 0; j < n_kv && ok; ++j, ++kc) {
         const int st = kc % NK;
-        if (!waited(&k_full[st], (kc / NK) & 1, OA_KERR_WAIT_FULL)) { ok = false; break; }
+        if (!warp_wait(&k_full[st], (kc / NK) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
         const uint64_t kd = desc_at(k_desc, st * Cfg::T_BYTES);
         for (int half = 0; half < 2; ++half) {
           // an item's first product replaces the accumulator: wait until both halves' warps have read the previous item's
-          if (j == 0 && half == 0) ok = waited(&ds_full[1], kc & 1, OA_KERR_WAIT_SOFTMAX);
-          if (!ok || !waited(&ds_full[half], kc & 1, OA_KERR_WAIT_SOFTMAX)) { ok = false; break; }
+          if (j == 0 && half == 0) ok = warp_wait(&ds_full[1], kc & 1);
+          if (!ok || !warp_wait(&ds_full[half], kc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -1124,8 +1114,8 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       const unsigned long long nlse2 = f2_splat(qi < hi ? -p.lse[stat_at] * LOG2E : -INFINITY);
       const unsigned long long ndlt2 = f2_splat(qi < hi ? -p.delta[stat_at] * p.scale : 0.f);
       for (int j = 0; j < n_kv; ++j, ++kc) {
-        ok = waited(&s_full[kc & 1], (kc >> 1) & 1, OA_KERR_WAIT_TMEM_FULL);
-        if (!ok) break;
+        ok = warp_wait(&s_full[kc & 1], (kc >> 1) & 1);
+        if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
         tc_fence_after();
         const uint32_t s_addr = t_lane + Cfg::TM_S + (kc & 1) * FA_BN + half * 64;
         const uint32_t dp_addr = t_lane + Cfg::TM_DP + half * 64;
@@ -1147,8 +1137,8 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll
           for (int i = 0; i < 64; ++i) s[i] = (i <= lim) ? s[i] : 0u;
         }
-        ok = waited(dp_full, kc & 1, OA_KERR_WAIT_TMEM_FULL);
-        if (!ok) break;
+        ok = warp_wait(dp_full, kc & 1);
+        if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
         tc_fence_after();
         uint32_t dp[64];
         tmem_ld32(dp_addr, dp);
@@ -1166,8 +1156,8 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         if (lane == 0) mbar_arrive(&ds_full[half]);
       }
       if (!ok) break;
-      ok = waited(fin_full, itc & 1, OA_KERR_WAIT_TMEM_FULL);
-      if (!ok) break;
+      ok = warp_wait(fin_full, itc & 1);
+      if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
       ++itc;
       tc_fence_after();
       __nv_bfloat16* base = p.dq + q0 * p.dq_stride + h * HD + half * (HD / 2);

@@ -9,7 +9,7 @@
 // dealt to one CTA per SM in snake order; the two tiles of a forward CTA are two heads of one group where groups are even, so that both need the same
 // blocks of keys and values, and neighbouring tiles of one head otherwise; dK and dV of a key-value head stay in TMEM over all query tiles of all
 // heads of its group, so that there is one writer and one order.  A sequence's last block may reach into the next sequence, or into rows that nobody
-// wrote: the loading warp puts zeros in place of those rows (of values forward, of everything that is a product's second operand backward),
+// wrote: a warp of its own puts zeros in place of those rows (of values forward, of everything that is a product's second operand backward),
 // because a weight of 0 times NaN is NaN.
 // Every wait is bounded and reports to a status word.
 #include "attn_tile.cuh"
@@ -95,8 +95,8 @@ struct PackedFwdCfg {
   static constexpr int SMEM_BYTES = OFF_ITEMS + PACKED_ROUNDS * 16;
   static constexpr int TMEM_COLS = 512;
   static constexpr int TM_S = 0, TM_P = ALIAS ? 0 : 256, P_STEP = ALIAS ? FA_BN : 64, TM_O = ALIAS ? 256 : 384;   // S: + 128 * tile, O: + HD * tile
-  static constexpr int MMA_WARPS = ALIAS ? 1 : 2, TMA_WARP = 8 + MMA_WARPS;   // after 8 softmax warps
-  static constexpr int THREADS = (TMA_WARP + 1) * 32;
+  static constexpr int MMA_WARPS = ALIAS ? 1 : 2, TMA_WARP = 8 + MMA_WARPS, CLEAR_WARP = TMA_WARP + 1;   // after 8 softmax warps
+  static constexpr int THREADS = (CLEAR_WARP + 1) * 32;
 };
 
 // What an item of the forward kernel is: up to two tiles of queries and their blocks of keys
@@ -136,8 +136,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* s_empty = s_full + 2;          // [2]   ... and is in registers (4 warps)
   uint64_t* p_full = s_full + 4;           // [2][2]  P_t written, by half of the keys (the first: O_t rescaled if needed) (4 warps)
   uint64_t* o_done = s_full + 8;           // [2]   O_t += P_t V_j finished: P_t may be overwritten, O_t may be rescaled
-  uint64_t* v_part = s_full + 10;          // the values of a sequence's last block are there, and some rows of others
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 11);
+  uint64_t* v_part = s_full + 10;          // [NS]  the values of a sequence's last block are there, and some rows of others
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_part + NS);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -150,7 +150,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     mbar_init(q_empty, Cfg::MMA_WARPS);
     for (int s = 0; s < NS; ++s) { mbar_init(&k_full[s], 1); mbar_init(&v_full[s], 1); mbar_init(&k_empty[s], Cfg::MMA_WARPS); mbar_init(&v_empty[s], Cfg::MMA_WARPS); }
     for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&s_empty[t], 4); mbar_init(&p_full[2 * t], 4); mbar_init(&p_full[2 * t + 1], 4); mbar_init(&o_done[t], 1); }
-    mbar_init(v_part, 1);
+    for (int s = 0; s < NS; ++s) mbar_init(&v_part[s], 1);
     mbar_fence_init();
   }
   if (warp == 8) { tmem_alloc<Cfg::TMEM_COLS>(tmem_slot); tmem_relinquish(); }
@@ -166,7 +166,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   if (warp == Cfg::TMA_WARP) {
     // ------------- producer
-    uint32_t blk = 0, itc = 0, parts = 0;   // K / V blocks and items loaded so far, last blocks with rows of others
+    uint32_t blk = 0, itc = 0;   // K / V blocks and items loaded so far
     bool ok = true;
     while (ok && walk.next(entry, which)) {
       const PackedFwdItem<HEADS> it(p, entry, which);
@@ -191,26 +191,32 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tma_load_2d(smem + Cfg::OFF_K + st * Cfg::KV_BYTES + x * (FA_BN * 128), &tmK, &k_full[st], it.kv_head * HD + x * 64, row);
         }
         if (!warp_wait(&v_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
-        const bool part = row + FA_BN > it.hi;
-        uint8_t* v_tile = smem + Cfg::OFF_V + st * Cfg::KV_BYTES;
         if (elect_one()) {
-          uint64_t* bar = part ? v_part : &v_full[st];
+          uint64_t* bar = row + FA_BN > it.hi ? &v_part[st] : &v_full[st];
           mbar_expect_tx(bar, Cfg::KV_BYTES);
 #pragma unroll
-          for (int x = 0; x < HD / 64; ++x) tma_load_2d(v_tile + x * (FA_BN * 128), &tmV, bar, it.kv_head * HD + x * 64, row);
-        }
-        __syncwarp();
-        if (part) {
-          if (!warp_wait(v_part, parts & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-          ++parts;
-          clear_rows<HD>(v_tile, it.hi - row, lane);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&v_full[st]);
+          for (int x = 0; x < HD / 64; ++x)
+            tma_load_2d(smem + Cfg::OFF_V + st * Cfg::KV_BYTES + x * (FA_BN * 128), &tmV, bar, it.kv_head * HD + x * 64, row);
         }
         __syncwarp();
       }
       ++itc;
+    }
+  } else if (warp == Cfg::CLEAR_WARP) {
+    // ------------- zeros in place of rows behind a sequence, which only an item's last block can have
+    uint32_t blk = 0, phases = 0;
+    while (walk.next(entry, which)) {
+      const PackedFwdItem<HEADS> it(p, entry, which);
+      const int n_it = max(it.n[0], it.n[1]), row = it.lo + (n_it - 1) * FA_BN;
+      blk += n_it;
+      if (row + FA_BN <= it.hi) continue;
+      const int st = (blk - 1) % NS;
+      if (!warp_wait(&v_part[st], (phases >> st) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+      phases ^= 1u << st;
+      clear_rows<HD>(smem + Cfg::OFF_V + st * Cfg::KV_BYTES, it.hi - row, lane);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_full[st]);
     }
   } else if (ALIAS && warp == 8) {
     // ------------- MMA issuer of both tiles, in turn (warp-uniform waits, one lane issues)
@@ -471,7 +477,18 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         uint32_t o[32];
         tmem_ld32(o_addr + c * 32, o);
         tmem_ld_wait();
-        store_rows(op + c * 32, o_stride, hi - q0, o, inv, lane);
+        // At head dim 64 a row's 16 bytes to a lane are the faster (flash_attn.cu)
+        if (ALIAS) store_rows(op + c * 32, o_stride, hi - q0, o, inv, lane);
+        else if (q0 + lane < hi) {
+          __nv_bfloat16* od = op + (long long)lane * o_stride + c * 32;
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint4*>(od + g * 8) = make_uint4(
+                pack_bf16x2(__uint_as_float(o[g * 8]) * inv, __uint_as_float(o[g * 8 + 1]) * inv),
+                pack_bf16x2(__uint_as_float(o[g * 8 + 2]) * inv, __uint_as_float(o[g * 8 + 3]) * inv),
+                pack_bf16x2(__uint_as_float(o[g * 8 + 4]) * inv, __uint_as_float(o[g * 8 + 5]) * inv),
+                pack_bf16x2(__uint_as_float(o[g * 8 + 6]) * inv, __uint_as_float(o[g * 8 + 7]) * inv));
+        }
       }
       if (p.lse && q0 + lane < hi) p.lse[(long long)head * p.plan.tokens + q0 + lane] = (m_run + log2f(l_run)) / LOG2E;
       tc_fence_before();   // the O reads above complete before this warp's next p_full arrival lets the next item's first P V overwrite O
@@ -522,7 +539,7 @@ packed_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __
   if (item < total && sub == 0) delta[(long long)h * tokens + row] = s;
 }
 
-constexpr int PB_THREADS = 352;   // 8 softmax warps + 2 MMA issuer warps + 1 TMA warp
+constexpr int PB_THREADS = 384;   // 8 softmax warps, 2 MMA issuer warps, a TMA warp and one that clears rows
 // Of eight pairs of exponentials, those on the multiply-add pipe (flash_attn.cu)
 template <int HD> constexpr int PB_FMA_PAIRS = HD == 64 ? 2 : 1;
 
@@ -542,7 +559,7 @@ struct PackedKvCfg {
   static constexpr int OFF_DO = OFF_Q + NST * T_BYTES;
   static constexpr int OFF_STAT = OFF_DO + NST * T_BYTES;   // float[NST][256]: -lse*log2e | -delta*scale of the query block
   static constexpr int OFF_BAR = OFF_STAT + NST * 256 * 4;
-  static constexpr int OFF_ITEMS = OFF_BAR + 224;
+  static constexpr int OFF_ITEMS = OFF_BAR + 272;
   static constexpr int SMEM_BYTES = OFF_ITEMS + PACKED_ROUNDS * 16;
   static constexpr int TMEM_COLS = 512;
   static constexpr int TM_S = 0, TM_DP = NS * FA_BN, TM_DV = TM_DP + FA_BN, TM_DK = TM_DV + HD;
@@ -578,8 +595,8 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   uint64_t* ds_full = bars + 21;   // [2]  dS^T, by column half (4 warps each)
   uint64_t* fin_full = bars + 23;  // dV, dK of the item are complete (both issuers arrive)
   uint64_t* turn = bars + 24;      // NS == 1: the next tile's scores are in the pipe, dK and dP may follow (not for an item's last tile)
-  uint64_t* part_full = bars + 25; // Q and dO of a sequence's last block are there, and some rows of others
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+  uint64_t* part_full = bars + 25; // [3]  Q and dO of a sequence's last block are there, and some rows of others
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
   float* stat = reinterpret_cast<float*>(smem + Cfg::OFF_STAT);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -597,7 +614,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     mbar_init(dp_full, 1);
     mbar_init(fin_full, 2);
     mbar_init(turn, 1);
-    mbar_init(part_full, 1);
+    for (int s = 0; s < NST; ++s) mbar_init(&part_full[s], 1);
     mbar_fence_init();
   }
   if (warp == 8) { tmem_alloc<Cfg::TMEM_COLS>(tmem_slot); tmem_relinquish(); }
@@ -613,7 +630,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
   if (warp == 10) {
     // ------------- TMA producer (also stages the per-query statistics of each block)
-    uint32_t itc = 0, qc = 0, parts = 0;       // items and Q / dO blocks loaded so far, last blocks with rows of others
+    uint32_t itc = 0, qc = 0;       // items and Q / dO blocks loaded so far
     bool ok = true;
     while (ok && walk.next(entry, which)) {
       const PackedKvItem it(entry, which);
@@ -637,14 +654,14 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           uint8_t *q_tile = smem + Cfg::OFF_Q + st * Cfg::T_BYTES, *do_tile = smem + Cfg::OFF_DO + st * Cfg::T_BYTES;
           if (!warp_wait(&q_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
           if (elect_one()) {
-            uint64_t* bar = part ? part_full : &q_full[st];
+            uint64_t* bar = part ? &part_full[st] : &q_full[st];
             mbar_expect_tx(bar, part ? 2 * Cfg::T_BYTES : Cfg::T_BYTES);
 #pragma unroll
             for (int x = 0; x < HD / 64; ++x) tma_load_2d(q_tile + x * (FA_BM * 128), &tmQ, bar, h * HD + x * 64, qrow);
           }
           if (!warp_wait(&do_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
           if (elect_one()) {
-            uint64_t* bar = part ? part_full : &do_full[st];
+            uint64_t* bar = part ? &part_full[st] : &do_full[st];
             if (!part) mbar_expect_tx(bar, Cfg::T_BYTES);
 #pragma unroll
             for (int x = 0; x < HD / 64; ++x) tma_load_2d(do_tile + x * (FA_BM * 128), &tmDO, bar, h * HD + x * 64, qrow);
@@ -666,20 +683,31 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             reinterpret_cast<float4*>(dst + 128)[lane] = nd;
           }
           __syncwarp();
-          if (part) {
-            if (!warp_wait(part_full, parts & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-            ++parts;
-            clear_rows<HD>(q_tile, it.hi - qrow, lane);
-            clear_rows<HD>(do_tile, it.hi - qrow, lane);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) { mbar_arrive(&q_full[st]); mbar_arrive(&do_full[st]); }
-          }
           if (lane == 0) mbar_arrive(&q_full[st]);
           __syncwarp();
         }
       }
       ++itc;
+    }
+  } else if (warp == 11) {
+    // ------------- zeros in place of rows behind a sequence, which only a head's last block can have
+    uint32_t qc = 0, phases = 0;
+    bool ok = true;
+    while (ok && walk.next(entry, which)) {
+      const PackedKvItem it(entry, which);
+      const int qrow = it.lo + it.key0 + (it.blocks - 1) * FA_BM;
+      if (qrow + FA_BM <= it.hi) { qc += it.blocks * p.group; continue; }
+      for (int g = 0; g < p.group; ++g) {
+        qc += it.blocks;
+        const int st = (qc - 1) % NST;
+        if (!warp_wait(&part_full[st], (phases >> st) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+        phases ^= 1u << st;
+        clear_rows<HD>(smem + Cfg::OFF_Q + st * Cfg::T_BYTES, it.hi - qrow, lane);
+        clear_rows<HD>(smem + Cfg::OFF_DO + st * Cfg::T_BYTES, it.hi - qrow, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) { mbar_arrive(&q_full[st]); mbar_arrive(&do_full[st]); }
+      }
     }
   } else if (warp == 8) {
     // ------------- MMA issuer A: S^T = K Q^T and dV += P^T dO.  S^T of a tile goes over the P^T that dV read NS tiles ago.
@@ -911,7 +939,7 @@ struct PackedQCfg {
   static constexpr int OFF_K = OFF_DO + T_BYTES;
   static constexpr int OFF_V = OFF_K + NK * T_BYTES;
   static constexpr int OFF_BAR = OFF_V + NV * T_BYTES;
-  static constexpr int OFF_ITEMS = OFF_BAR + 224;
+  static constexpr int OFF_ITEMS = OFF_BAR + 272;
   static constexpr int SMEM_BYTES = OFF_ITEMS + PACKED_ROUNDS * 16;
   static constexpr int TMEM_COLS = 512;
   static constexpr int TM_S = 0, TM_DP = 256, TM_DQ = 384;   // two score buffers; dS over dP
@@ -938,8 +966,9 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint64_t* dp_full = bars + 20;
   uint64_t* ds_full = bars + 21;   // [2]  by column half (4 warps each)
   uint64_t* fin_full = bars + 23;
-  uint64_t* part_full = bars + 24; // K and V of a sequence's last block are there, and some rows of others
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
+  uint64_t* k_part = bars + 24;    // [4]  K, V of a sequence's last block are there, and some rows of others
+  uint64_t* v_part = bars + 28;    // [3]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -955,7 +984,8 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&s_empty[s], 8); mbar_init(&ds_full[s], 4); }
     mbar_init(dp_full, 1);
     mbar_init(fin_full, 1);
-    mbar_init(part_full, 1);
+    for (int s = 0; s < NK; ++s) mbar_init(&k_part[s], 1);
+    for (int s = 0; s < NV; ++s) mbar_init(&v_part[s], 1);
     mbar_fence_init();
   }
   if (warp == 8) { tmem_alloc<Cfg::TMEM_COLS>(tmem_slot); tmem_relinquish(); }
@@ -970,7 +1000,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   int which;
 
   if (warp == 10) {
-    uint32_t itc = 0, kc = 0, parts = 0;
+    uint32_t itc = 0, kc = 0;
     bool ok = true;
     while (ok && walk.next(entry, which)) {
       const int lo = entry.x, hi = entry.y, n_kv = entry.z + 1, h = which, hk = which / p.group, qrow = lo + entry.z * FA_BM;
@@ -989,31 +1019,42 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         uint8_t *k_tile = smem + Cfg::OFF_K + sk * Cfg::T_BYTES, *v_tile = smem + Cfg::OFF_V + sv * Cfg::T_BYTES;
         if (!warp_wait(&k_empty[sk], ((kc / NK) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
         if (elect_one()) {
-          uint64_t* bar = part ? part_full : &k_full[sk];
-          mbar_expect_tx(bar, part ? 2 * Cfg::T_BYTES : Cfg::T_BYTES);
+          uint64_t* bar = part ? &k_part[sk] : &k_full[sk];
+          mbar_expect_tx(bar, Cfg::T_BYTES);
 #pragma unroll
           for (int x = 0; x < HD / 64; ++x) tma_load_2d(k_tile + x * (FA_BN * 128), &tmK, bar, hk * HD + x * 64, row);
         }
         if (!warp_wait(&v_empty[sv], ((kc / NV) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
         if (elect_one()) {
-          uint64_t* bar = part ? part_full : &v_full[sv];
-          if (!part) mbar_expect_tx(bar, Cfg::T_BYTES);
+          uint64_t* bar = part ? &v_part[sv] : &v_full[sv];
+          mbar_expect_tx(bar, Cfg::T_BYTES);
 #pragma unroll
           for (int x = 0; x < HD / 64; ++x) tma_load_2d(v_tile + x * (FA_BN * 128), &tmV, bar, hk * HD + x * 64, row);
         }
         __syncwarp();
-        if (part) {
-          if (!warp_wait(part_full, parts & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-          ++parts;
-          clear_rows<HD>(k_tile, hi - row, lane);
-          clear_rows<HD>(v_tile, hi - row, lane);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) { mbar_arrive(&k_full[sk]); mbar_arrive(&v_full[sv]); }
-          __syncwarp();
-        }
       }
       ++itc;
+    }
+  } else if (warp == 11) {
+    // ------------- zeros in place of rows behind a sequence, which only an item's last block can have
+    uint32_t kc = 0, k_phases = 0, v_phases = 0;
+    while (walk.next(entry, which)) {
+      const int row = entry.x + entry.z * FA_BN, from = entry.y - row;
+      kc += entry.z + 1;
+      if (from >= FA_BN) continue;
+      const int sk = (kc - 1) % NK, sv = (kc - 1) % NV;
+      if (!warp_wait(&k_part[sk], (k_phases >> sk) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+      clear_rows<HD>(smem + Cfg::OFF_K + sk * Cfg::T_BYTES, from, lane);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[sk]);
+      if (!warp_wait(&v_part[sv], (v_phases >> sv) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+      clear_rows<HD>(smem + Cfg::OFF_V + sv * Cfg::T_BYTES, from, lane);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_full[sv]);
+      k_phases ^= 1u << sk;
+      v_phases ^= 1u << sv;
     }
   } else if (warp == 8) {
     // ------------- MMA issuer A: S = Q K_j^T

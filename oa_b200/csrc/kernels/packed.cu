@@ -1,6 +1,7 @@
 // Packed sequences: which tiles the attention kernels work on, and rotation by positions on several axes.
 #include "common.cuh"
 #include "packed.cuh"
+#include "vec8.cuh"
 #include "per_device.h"
 #include "api.h"
 
@@ -120,7 +121,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedP
 // y = x with each pair (j, j + half) of a head turned by the token's position on the pair's own axis, times theta^(-j / half); dimensions from
 // 2 half on are copied.  A token's angles are worked out once for all its heads: position * turns in 64 bits (in 32 bits a position of 131072 leaves
 // an angle 0.008 off), the whole turns taken off, and what is left in [-1/2, 1/2] turns in 32 bits.  The gradient turns the other way.
-constexpr int ROTARY_MAX_HALF = 128;
+//
+// Bound by the bytes: each thread takes 16 bytes of a head's first half and the 16 that belong to them, and has two such pieces on their way before the angles are
+// worked out.  A block works on as many tokens as give its threads a piece each, or on a part of one where tokens alone leave SMs idle.
+constexpr int ROTARY_MAX_HALF = 128, ROTARY_THREADS = 256;
+constexpr int ROTARY_ANGLES = 1024;       // of a block's tokens
 struct RotaryParams {
   const void* x;
   long long x_stride;
@@ -128,34 +133,94 @@ struct RotaryParams {
   long long y_stride;
   const int* positions;                   // [axes, tokens]
   int tokens, heads, hd, half, backward;
+  int group;                              // tokens of a block
+  int per, of_head, turned;               // pieces of a token, of a head, and those of a head that are turned
+  uint32_t per_inv, of_head_inv;          // 2^32 over them, rounded up: quotients of numbers below 2^16 by multiplication
   uint8_t axis[ROTARY_MAX_HALF];
   double turns[ROTARY_MAX_HALF];          // turns a position: theta^(-j / half) / (2 pi)
 };
 
-__device__ __forceinline__ void rotary_angles(const RotaryParams& p, int t, float* s_cos, float* s_sin) {
-  for (int k = threadIdx.x; k < p.half; k += blockDim.x) {
-    const double a = (double)p.positions[(long long)p.axis[k] * p.tokens + t] * p.turns[k];
-    float s, c;
-    sincospif((float)(2.0 * (a - rint(a))), &s, &c);
-    s_cos[k] = c;
-    s_sin[k] = p.backward ? -s : s;
+__device__ __forceinline__ void rotary_angle(const RotaryParams& p, int t, int k, float* s_cos, float* s_sin) {
+  const double a = (double)p.positions[(long long)p.axis[k] * p.tokens + t] * p.turns[k];
+  float s, c;
+  sincospif((float)(2.0 * (a - rint(a))), &s, &c);
+  *s_cos = c;
+  *s_sin = p.backward ? -s : s;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  __shared__ __align__(16) float s_cos[ROTARY_ANGLES], s_sin[ROTARY_ANGLES];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int t0 = blockIdx.x * p.group, here = min(p.group, p.tokens - t0), n = here * p.per, step = gridDim.y * blockDim.x;
+  int i = blockIdx.y * blockDim.x + threadIdx.x;
+  Vec8<T> a[2], b[2];
+  int token[2], off[2], pair[2];          // of a piece: where in its token's row, and its first pair (-1: dimensions that are only copied)
+  const auto over = [](int x, int d, uint32_t inv) { return d == 1 ? x : (int)__umulhi((uint32_t)x, inv); };
+  const auto fetch = [&] {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int at = i + q * step;
+      if (at >= n) continue;
+      token[q] = over(at, p.per, p.per_inv);
+      const int in = at - token[q] * p.per, head = over(in, p.of_head, p.of_head_inv), j = in - head * p.of_head;
+      pair[q] = j < p.turned ? j * 8 : -1;
+      off[q] = head * p.hd + (j < p.turned ? j * 8 : p.half + j * 8);
+      const T* row = static_cast<const T*>(p.x) + (t0 + token[q]) * p.x_stride + off[q];
+      a[q] = *reinterpret_cast<const Vec8<T>*>(row);
+      if (pair[q] >= 0) b[q] = *reinterpret_cast<const Vec8<T>*>(row + p.half);
+    }
+  };
+  fetch();
+  for (int k = threadIdx.x; k < here * p.half; k += blockDim.x) rotary_angle(p, t0 + k / p.half, k % p.half, s_cos + k, s_sin + k);
+  __syncthreads();
+  while (i < n) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if (i + q * step >= n) continue;
+      T* to = static_cast<T*>(p.y) + (t0 + token[q]) * p.y_stride + off[q];
+      if (pair[q] >= 0) {
+        float x[8], y[8], lo[8], hi[8], c[8], s[8];
+        a[q].get(x);
+        b[q].get(y);
+        const int k0 = token[q] * p.half + pair[q];
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) {
+          *reinterpret_cast<float4*>(c + k) = *reinterpret_cast<const float4*>(s_cos + k0 + k);
+          *reinterpret_cast<float4*>(s + k) = *reinterpret_cast<const float4*>(s_sin + k0 + k);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          lo[k] = x[k] * c[k] - y[k] * s[k];
+          hi[k] = y[k] * c[k] + x[k] * s[k];
+        }
+        a[q].set(lo);
+        b[q].set(hi);
+        *reinterpret_cast<Vec8<T>*>(to + p.half) = b[q];
+      }
+      *reinterpret_cast<Vec8<T>*>(to) = a[q];
+    }
+    i += 2 * step;
+    fetch();
   }
 }
 
+// The same element by element: rows that lie anywhere, any number of pairs
 __device__ __forceinline__ float rotary_load(const float* p) { return *p; }
 __device__ __forceinline__ float rotary_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void rotary_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void rotary_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 template <typename T>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(ROTARY_THREADS) rotary_any_kernel(const __grid_constant__ RotaryParams p) {
   __shared__ float s_cos[ROTARY_MAX_HALF], s_sin[ROTARY_MAX_HALF];
   pdl_launch_dependents();
   pdl_wait();
   const int rest = p.hd - 2 * p.half, per = p.half + rest;       // pairs and single dimensions of a head
   for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     __syncthreads();
-    rotary_angles(p, t, s_cos, s_sin);
+    for (int k = threadIdx.x; k < p.half; k += blockDim.x) rotary_angle(p, t, k, s_cos + k, s_sin + k);
     __syncthreads();
     const T* x = static_cast<const T*>(p.x) + t * p.x_stride;
     T* y = static_cast<T*>(p.y) + t * p.y_stride;
@@ -170,6 +235,35 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
       }
     }
   }
+}
+
+template <typename T>
+static int rotary_run(RotaryParams& p, cudaStream_t st) {
+  const int rest = p.hd - 2 * p.half, unit = 16 / (int)sizeof(T);
+  const bool pieces = p.half % 8 == 0 && rest % 8 == 0 && p.x_stride % unit == 0 && p.y_stride % unit == 0 &&
+                      ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.y)) & 15) == 0 && (long long)p.heads * p.hd < (1 << 18);
+  if (!pieces) {
+    const dim3 grid((unsigned)(p.tokens < (1 << 20) ? p.tokens : 1 << 20));
+    launch_short(rotary_any_kernel<T>, grid, dim3(ROTARY_THREADS), 0, st, p);
+    return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
+  }
+  // dimensions that are only copied are left alone where they lie already
+  p.turned = p.half / 8;
+  p.of_head = p.turned + (p.x == p.y && p.x_stride == p.y_stride ? 0 : rest / 8);
+  p.per = p.heads * p.of_head;
+  p.per_inv = (uint32_t)(((1ull << 32) + p.per - 1) / p.per);
+  p.of_head_inv = (uint32_t)(((1ull << 32) + p.of_head - 1) / p.of_head);
+  constexpr int FULL = 2 * ROTARY_THREADS;                       // pieces of a block, two to a thread
+  p.group = p.per >= FULL ? 1 : FULL / p.per;
+  const int few = p.tokens / (2 * sm_count());                   // tokens of a block while every SM has two
+  if (p.group > few) p.group = few > 1 ? few : 1;
+  if (p.group > ROTARY_ANGLES / p.half) p.group = ROTARY_ANGLES / p.half;
+  // a token over several blocks while tokens alone leave SMs idle; the threads that two pieces each keep busy, one each while they are few
+  const int blocks = (p.tokens + p.group - 1) / p.group, n = p.group * p.per, room = (2 * sm_count() + blocks - 1) / blocks, want = (n + ROTARY_THREADS - 1) / ROTARY_THREADS;
+  const int spread = room < want ? room : want, share = (n + spread - 1) / spread, rounds = (share + FULL - 1) / FULL;
+  const int each = blocks >= 2 * sm_count() ? 2 * rounds : (share + ROTARY_THREADS - 1) / ROTARY_THREADS, threads = ((share + each - 1) / each + 31) / 32 * 32;
+  launch_short(rotary_kernel<T>, dim3((unsigned)blocks, (unsigned)spread), dim3((unsigned)threads), 0, st, p);
+  return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }
 
 }  // namespace oa
@@ -196,13 +290,10 @@ extern "C" int oa_rotary_axes(int dtype, const void* x, long long x_stride, void
   if (pairs < 1 || pairs > ROTARY_MAX_HALF) return OA_ERR_UNSUPPORTED;
   if (tokens < 0 || heads < 1 || 2 * pairs > head_dim || !pair_axes || !turns) return OA_ERR_ARG;
   if (tokens == 0) return OA_OK;
-  RotaryParams p{x, x_stride, y, y_stride, positions, tokens, heads, head_dim, pairs, backward, {}, {}};
+  RotaryParams p{x, x_stride, y, y_stride, positions, tokens, heads, head_dim, pairs, backward, 1, 0, 0, 0, 0, 0, {}, {}};
   for (int j = 0; j < pairs; ++j) {
     p.axis[j] = static_cast<const uint8_t*>(pair_axes)[j];
     p.turns[j] = static_cast<const double*>(turns)[j];
   }
-  const dim3 grid((unsigned)(tokens < (1 << 20) ? tokens : 1 << 20));
-  if (dtype == OA_F32) launch_short(rotary_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, p);
-  else launch_short(rotary_kernel<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, p);
-  return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
+  return dtype == OA_F32 ? rotary_run<float>(p, (cudaStream_t)stream) : rotary_run<__nv_bfloat16>(p, (cudaStream_t)stream);
 }

@@ -297,8 +297,8 @@ size_t oa_paged_attn_scratch_bytes(int dtype, int tokens, int batch, int max_fre
 int oa_sample(int dtype, const void* logits, long long stride, const float* u, const float* temperature, const int* top_k, const float* top_p,
               const float* min_p, int* tokens, float* logprobs, int rows, int vocab, int* status, void* stream);
 
-// ---- packed sequences (packed.cu, packed_attn.cu, packed_attn_f32.cu): sequences of different lengths one behind the other, rows starts[b] .. starts[b + 1] of every tensor
-// What the attention kernels work on, from the starts [batch + 1] (on the device): oa_packed_plan_bytes, 16-byte aligned.  Its words from the fifth on are the
+// ---- packed sequences (packed.cu, packed_attn.cu, packed_short.cu, packed_attn_f32.cu): sequences of different lengths one behind the other, rows starts[b] .. starts[b + 1] of every tensor
+// What the attention kernels work on, from the starts [batch + 1] (on the device): oa_packed_plan_bytes, 16-byte aligned.  Its words from the ninth on are the
 // starts as the kernels take them: rising, within [0, tokens].
 size_t oa_packed_plan_bytes(int tokens, int batch);
 int oa_packed_plan(const int* starts, int* plan, int batch, int tokens, void* stream);

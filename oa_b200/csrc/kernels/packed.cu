@@ -9,8 +9,8 @@ namespace oa {
 
 // ------------------------------------------------------------------------------------------------ plan
 // Sequences are rows [starts[b], starts[b + 1]) of the packed tensors; starts that fall or leave [0, tokens] are taken as the nearest that do
-// not.  The attention kernels take their work from two lists, the longest first: tiles of 128 rows of a sequence, and pairs of neighbouring
-// tiles.  Under the causal mask tile i of a sequence sees i + 1 tiles of keys (and its mirror image, tile n - 1 - i, is seen by as many tiles of
+// not.  Sequences of up to 64 rows go on a list of their own; of the others the attention kernels take their work from two lists, the longest first: tiles of 128
+// rows of a sequence, and pairs of neighbouring tiles.  Under the causal mask tile i of a sequence sees i + 1 tiles of keys (and its mirror image, tile n - 1 - i, is seen by as many tiles of
 // queries), so both lists are sorted by that index, by counting.  The order among equals is that of the atomics; nothing depends on it but
 // which SM works on a tile.  One block: a batch has few thousand tiles, and one plan serves every layer of a step in both directions.
 constexpr int PLAN_BINS = 1024;           // = threads of the block
@@ -47,13 +47,13 @@ __device__ __forceinline__ int plan_scan(int v, int* s_warp, Op op) {   // inclu
 }
 
 __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedPlanParams p) {
-  __shared__ int s_warp[32], s_count[2][PLAN_BINS], s_top;
+  __shared__ int s_warp[32], s_count[2][PLAN_BINS], s_top, s_short;
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, shift = p.shift, per = 1 << shift;
   int* starts = p.plan + PACKED_HEADER;
   s_count[0][tid] = s_count[1][tid] = 0;
-  if (tid == 0) s_top = 0;
+  if (tid == 0) s_top = s_short = 0;
   const auto most = [](int a, int b) { return max(a, b); };
   for (int b0 = 0; b0 <= p.batch; b0 += PLAN_THREADS) {
     const int b = b0 + tid;
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedP
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         const int rows = PACKED_TILE << which;
-        const int n = (hi - lo + rows - 1) / rows, head = min(n, per);
+        const int n = hi - lo <= PACKED_SHORT ? 0 : (hi - lo + rows - 1) / rows, head = min(n, per);
         int sum = head;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -98,9 +98,19 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedP
   };
   walk([&](int which, int bin, int n) { return n > 0 ? atomicAdd(&s_count[which][bin], n) : 0; }, [](int, int, int, int, int, int, int) {});
   __syncthreads();
-  int4* lists[2];
+  int4* lists[3];
   lists[0] = reinterpret_cast<int4*>(p.plan + packed_tiles_at(p.batch));
   lists[1] = lists[0] + packed_max_tiles(p.tokens, p.batch);
+  lists[2] = lists[1] + packed_max_pairs(p.tokens, p.batch);
+  for (int b0 = tid - lane; b0 < p.batch; b0 += PLAN_THREADS) {
+    const int b = b0 + lane;
+    const int lo = b < p.batch ? starts[b] : 0, hi = b < p.batch ? starts[b + 1] : 0;
+    const bool brief = hi > lo && hi - lo <= PACKED_SHORT;
+    const unsigned all = __ballot_sync(0xffffffffu, brief);
+    int base = lane == 0 && all ? atomicAdd(&s_short, __popc(all)) : 0;
+    base = __shfl_sync(0xffffffffu, base, 0);
+    if (brief) lists[2][base + __popc(all & ((1u << lane) - 1))] = make_int4(lo, hi, 0, b);
+  }
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     // how many have a larger index: the sums from the end
@@ -109,8 +119,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedP
     s_count[which][PLAN_BINS - 1 - tid] = sum - mine;
     if (tid == PLAN_THREADS - 1) p.plan[which] = sum;
   }
-  if (tid == 0) { p.plan[2] = starts[0]; p.plan[3] = starts[p.batch]; }
   __syncthreads();
+  if (tid == 0) { p.plan[2] = starts[0]; p.plan[3] = starts[p.batch]; p.plan[4] = s_short; }
   walk([&](int which, int bin, int n) { return n > 0 ? atomicAdd(&s_count[which][bin], n) : 0; },
        [&](int which, int at, int first, int n, int lo, int hi, int b) {
          for (int i = 0; i < n; ++i) lists[which][at + i] = make_int4(lo, hi, first + i, b);
@@ -271,7 +281,7 @@ static int rotary_run(RotaryParams& p, cudaStream_t st) {
 using namespace oa;
 
 extern "C" size_t oa_packed_plan_bytes(int tokens, int batch) {
-  return ((size_t)packed_tiles_at(batch) + 4 * ((size_t)packed_max_tiles(tokens, batch) + packed_max_pairs(tokens, batch))) * sizeof(int);
+  return ((size_t)packed_tiles_at(batch) + 4 * ((size_t)packed_max_tiles(tokens, batch) + packed_max_pairs(tokens, batch) + batch)) * sizeof(int);
 }
 
 extern "C" int oa_packed_plan(const int* starts, int* plan, int batch, int tokens, void* stream) {

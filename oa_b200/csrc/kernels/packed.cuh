@@ -1,12 +1,14 @@
-// The plan of a batch of packed sequences, in int32 words: [tiles, pairs, first row, row behind the last, starts.., tiles.., pairs..], where a tile (128
-// rows) or a pair of tiles is (first row of its sequence, row behind it, index in the sequence, sequence), the largest index first.
+// The plan of a batch of packed sequences, in int32 words: [tiles, pairs, first row, row behind the last, short sequences, -, -, -, starts.., tiles.., pairs.., short
+// sequences..].  A tile (128 rows) or a pair of tiles of a sequence of more than 64 rows is (first row of its sequence, row behind it, index in the sequence,
+// sequence), the largest index first; a short sequence is (first row, row behind it, 0, sequence).
 #pragma once
 #include <cuda_runtime.h>
 
 namespace oa {
 
 constexpr int PACKED_TILE = 128;
-constexpr int PACKED_HEADER = 4;
+constexpr int PACKED_SHORT = 64;           // rows of a short sequence, at most
+constexpr int PACKED_HEADER = 8;
 constexpr int PACKED_MAX_BATCH = 1 << 24, PACKED_MAX_TOKENS = 1 << 30;   // numbers of tiles, rows and words stay far below 2^31
 __host__ __device__ inline int packed_tiles_at(int batch) { return (PACKED_HEADER + batch + 1 + 3) & ~3; }
 __host__ __device__ inline int packed_max_tiles(int tokens, int batch) { return tokens / PACKED_TILE + batch; }
@@ -18,9 +20,13 @@ struct PackedPlan {
   int batch, tokens;
   __device__ __forceinline__ int tiles() const { return words[0]; }
   __device__ __forceinline__ int pairs() const { return words[1]; }
+  __device__ __forceinline__ int shorts() const { return words[4]; }
   __device__ __forceinline__ int4 tile(int i) const { return reinterpret_cast<const int4*>(words + packed_tiles_at(batch))[i]; }
   __device__ __forceinline__ int4 pair(int i) const {
     return reinterpret_cast<const int4*>(words + packed_tiles_at(batch))[packed_max_tiles(tokens, batch) + i];
+  }
+  __device__ __forceinline__ int4 brief(int i) const {
+    return reinterpret_cast<const int4*>(words + packed_tiles_at(batch))[packed_max_tiles(tokens, batch) + packed_max_pairs(tokens, batch) + i];
   }
   // f(row) for this worker's share of the rows that belong to no sequence
   template <typename F>

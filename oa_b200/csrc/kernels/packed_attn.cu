@@ -1,4 +1,5 @@
-// Causal attention over packed sequences with grouped heads for sm_100a, forward and backward, bf16 in / fp32 accumulate.
+// Causal attention over packed sequences with grouped heads for sm_100a, forward and backward, bf16 in / fp32 accumulate.  Sequences of up to 64 rows are worked on
+// by packed_short.cu, whose launches stand beside these.
 //
 // Query head h reads key-value head h / group; o_i = sum_j p_ij v_j over the keys j <= i of i's own sequence, p_ij = exp(scale q_i k_j - lse_i).  Backward,
 // with delta_i = dO_i O_i:  dV_j = sum p_ij dO_i,  dS_ij = scale p_ij (dO_i v_j - delta_i),  dQ_i = sum dS_ij k_j,  dK_j = sum dS_ij q_i, where those of a
@@ -13,7 +14,7 @@
 // because a weight of 0 times NaN is NaN.
 // Every wait is bounded and reports to a status word.
 #include "attn_tile.cuh"
-#include "packed.cuh"
+#include "packed_short.h"
 #include "per_device.h"
 #include "api.h"
 
@@ -1272,6 +1273,9 @@ extern "C" int oa_packed_attn(const void* q, const void* k, const void* v, const
   const int group = q_heads / kv_heads;
   const PackedFwdParams p{{plan, batch, tokens}, q_heads, group, scale, (__nv_bfloat16*)o, lse, status};
   cudaStream_t st = (cudaStream_t)stream;
+  const PackedShortFwd brief{p.plan, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (__nv_bfloat16*)o, lse, q_stride, k_stride, v_stride,
+                             o_stride, q_heads, group, scale};
+  if ((rc = packed_short_fwd(brief, head_dim, st))) return rc;
   if (group % 2 == 0) return head_dim == 64 ? packed_fwd<64, true>(tq, tk, tv, p, st) : packed_fwd<128, true>(tq, tk, tv, p, st);
   return head_dim == 64 ? packed_fwd<64, false>(tq, tk, tv, p, st) : packed_fwd<128, false>(tq, tk, tv, p, st);
 }
@@ -1306,5 +1310,8 @@ extern "C" int oa_packed_attn_bwd(const void* q, const void* k, const void* v, c
              (float*)scratch, tokens, q_heads, head_dim, o_stride, do_stride);
   const PackedBwdParams p{{plan, batch, tokens}, q_heads, kv_heads, q_heads / kv_heads, scale, lse, (const float*)scratch, (__nv_bfloat16*)dq,
                           (__nv_bfloat16*)dk, (__nv_bfloat16*)dv, dq_stride, dk_stride, dv_stride, status};
+  const PackedShortBwd brief{p.plan, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (const __nv_bfloat16*)dout, lse, p.delta, p.dq, p.dk, p.dv,
+                             q_stride, k_stride, v_stride, do_stride, dq_stride, dk_stride, dv_stride, kv_heads, p.group, scale};
+  if ((rc = packed_short_bwd(brief, head_dim, st))) return rc;
   return head_dim == 64 ? packed_bwd<64>(tq, tk, tv, tdo, p, st) : packed_bwd<128>(tq, tk, tv, tdo, p, st);
 }

@@ -1,8 +1,8 @@
 // Causal attention over packed sequences in fp32, with grouped heads, forward and backward: the engine's exact precision, and gradient checks.
 //
 // Query head h reads key-value head h / group.  Within a sequence the work is that of attn_f32.cu: a block of 128 threads owns 128 / (DS KS) rows of one
-// head, the other side streams through shared memory 32 rows at a time.  A block finds its rows in the plan's list of tiles (128 rows of a sequence, the
-// longest first): a tile is KS DS blocks.  Rows of other sequences are never read: what a sequence holds does not reach another.  dK and
+// head, the other side streams through shared memory 32 rows at a time.  A block finds its rows in the plan's lists, of tiles (128 rows of a sequence,
+// the longest first) and of short sequences: a tile is KS DS blocks.  Rows of other sequences are never read: what a sequence holds does not reach another.  dK and
 // dV of a key-value head add up over the query heads that share it, one after the other in one block, so that there is one writer and one order.
 #include "attn_f32.cuh"
 #include "packed.cuh"
@@ -26,8 +26,9 @@ template <int ROWS, bool MIRROR>
 __device__ __forceinline__ PackedRows packed_rows(const PackedPlan& plan, int block) {
   constexpr int SUBS = PACKED_TILE / ROWS;
   const int at = block / SUBS, sub = block % SUBS;
-  if (at >= plan.tiles()) return {0, 0, 0};
-  const int4 t = plan.tile(at);
+  const int tiles = plan.tiles();
+  if (at >= tiles + plan.shorts()) return {0, 0, 0};
+  const int4 t = at < tiles ? plan.tile(at) : plan.brief(at - tiles);
   const int n = t.y - t.x, idx = MIRROR ? (n + PACKED_TILE - 1) / PACKED_TILE - 1 - t.z : t.z;
   return {t.x, n, idx * PACKED_TILE + sub * ROWS};
 }

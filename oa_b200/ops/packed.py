@@ -8,7 +8,7 @@ no sequence (behind the last one, say) are neither read nor reach anything, and 
 
 The form for single tokens over a cache is `paged.append` (theta 0, for rows that `rotary` turned) with `paged.attention`.
 
-CUDA tensors run csrc/kernels/packed.cu, packed_attn.cu and packed_attn_f32.cu; CPU tensors the plain statement of the same mathematics.
+CUDA tensors run csrc/kernels/packed.cu, packed_attn.cu, packed_short.cu and packed_attn_f32.cu; CPU tensors the plain statement of the same mathematics.
 """
 from __future__ import annotations
 
@@ -78,7 +78,7 @@ def plan(starts: torch.Tensor, tokens: int) -> PackedPlan:
     _current("plan", starts)
     words = torch.empty(N.require().oa_packed_plan_bytes(tokens, batch) // 4, dtype=torch.int32, device=starts.device)
     K._launch(N.require().oa_packed_plan(starts.data_ptr(), words.data_ptr(), batch, tokens, N.stream()), "oa_packed_plan")
-    return PackedPlan(words[4:4 + batch + 1], words, tokens, batch)
+    return PackedPlan(words[8:8 + batch + 1], words, tokens, batch)
 
 
 @functools.lru_cache(maxsize=64)
@@ -177,7 +177,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPla
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), plan.words.data_ptr(), o.data_ptr(), N.ptr(lse), plan.tokens, plan.batch, hq, hk, head_dim, qs, ks, vs,
             hq * head_dim, scale)
     if half:
-        K._launch(N.require().oa_packed_attn(*args, K.status_word(q.device).data_ptr(), N.stream()), "oa_packed_attn", outputs=(o,))
+        K._launch(N.require().oa_packed_attn(*args, K.status_word(q.device).data_ptr(), N.stream()), "oa_packed_attn", 2, outputs=(o,))
     else:
         K._launch(N.require().oa_packed_attn_f32(*args, N.stream()), "oa_packed_attn_f32", outputs=(o,))
     return (o, lse) if return_lse else o
@@ -240,7 +240,7 @@ def attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: tor
         # scratch of the call's own: calls on several streams, and graphs, do not meet in it
         need = N.require().oa_packed_attn_bwd_scratch_bytes(plan.tokens, plan.batch, hq, hk, head_dim)
         scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-        K._launch(N.require().oa_packed_attn_bwd(*args, scratch.data_ptr(), K.status_word(q.device).data_ptr(), N.stream()), "oa_packed_attn_bwd", 3,
+        K._launch(N.require().oa_packed_attn_bwd(*args, scratch.data_ptr(), K.status_word(q.device).data_ptr(), N.stream()), "oa_packed_attn_bwd", 4,
                   outputs=(dqkv,))
     else:
         K._launch(N.require().oa_packed_attn_f32_bwd(*args, N.stream()), "oa_packed_attn_f32_bwd", outputs=(dqkv,))

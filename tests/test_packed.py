@@ -111,7 +111,7 @@ RAGGED = [5, 0, 300, 1, 127, 128, 129, 64, 2, 257]
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("lengths", [[1], [2], [127], [128], [129], [256], [257], [1, 1, 1], RAGGED], ids=lambda v: "-".join(map(str, v)))
+@pytest.mark.parametrize("lengths", [[1], [2], [15], [16], [17], [33], [48], [63], [64], [65], [127], [128], [129], [256], [257], [1, 1, 1], RAGGED], ids=lambda v: "-".join(map(str, v)))
 @pytest.mark.parametrize("hd", [64, 128])
 def test_attention_lengths_bf16(device, lengths, hd):
     _check(lengths, 4, 2, hd, torch.bfloat16, device)
@@ -128,6 +128,13 @@ def test_attention_heads_bf16(device, hq, hk, hd):
 @pytest.mark.parametrize("hq,hk,hd", [(2, 2, 64), (4, 1, 64), (2, 2, 128), (4, 1, 128)])
 def test_attention_long_bf16(hq, hk, hd):
     _check([1500, 700, 1], hq, hk, hd, torch.bfloat16, "cuda", pad=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hk", [(16, 16), (8, 2), (3, 1)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_many_short(hd, hq, hk):
+    _check([i % 64 + 1 for i in range(150)] + [300], hq, hk, hd, torch.bfloat16, "cuda", pad=2)
 
 
 @pytest.mark.gpu
@@ -278,24 +285,25 @@ def test_graphs_and_streams(dtype):
 
 @pytest.mark.gpu
 def test_plan_lists():
-    """Every tile and pair of every sequence once, the largest index first."""
+    """Every tile and pair of every long sequence once, the largest index first, and every short sequence."""
     g = torch.Generator().manual_seed(3)
     for lengths in ([1], [0], RAGGED, torch.randint(0, 5000, (70,), generator=g).tolist(), [10] * 3000, [300000, 1, 200000], torch.randint(0, 400, (2500,), generator=g).tolist()):
         tokens, batch = sum(lengths) + 9, len(lengths)
         p = P.plan(_starts(lengths, "cuda", 2), tokens)
         w = p.words.cpu()
-        n, m = w[:2].tolist()
-        first = (4 + batch + 1 + 3) // 4 * 4
+        n, m, briefs = w[0].item(), w[1].item(), w[4].item()
+        first = (8 + batch + 1 + 3) // 4 * 4
         starts = p.starts.cpu().tolist()
-        most = tokens // 128 + batch
+        most, pairs = tokens // 128 + batch, tokens // 256 + batch
         exact = tokens // 128 < 1024                               # beyond that, bins hold several indices
-        for count, rows, at in ((n, 128, first), (m, 256, first + 4 * most)):
-            got = w[at:at + 4 * count].reshape(-1, 4).tolist()
-            want = [(a, b, i, s) for s, (a, b) in enumerate(zip(starts, starts[1:])) for i in range(-(-(b - a) // rows))]
-            assert sorted(map(tuple, got)) == sorted(want)
+        lists = [w[at:at + 4 * count].reshape(-1, 4).tolist() for count, at in ((n, first), (m, first + 4 * most), (briefs, first + 4 * (most + pairs)))]
+        long = [(a, b, s) for s, (a, b) in enumerate(zip(starts, starts[1:])) if b - a > 64]
+        for got, rows in zip(lists, (128, 256)):
+            assert sorted(map(tuple, got)) == sorted((a, b, i, s) for a, b, s in long for i in range(-(-(b - a) // rows)))
             order = [x[2] for x in got]
             step = 1 if exact else 1 << (tokens // 128 // 1024).bit_length()
             assert all(a // step >= b // step for a, b in zip(order, order[1:]))
+        assert sorted(map(tuple, lists[2])) == [(a, b, 0, s) for s, (a, b) in enumerate(zip(starts, starts[1:])) if 0 < b - a <= 64]
 
 
 # ------------------------------------------------------------------------------------------------ rotation

@@ -1237,9 +1237,10 @@ template <int HD, bool HEADS>
 static int packed_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PackedFwdParams& p, cudaStream_t st) {
   static std::atomic<unsigned long long> allowed;
   if (allow_smem(allowed, (const void*)packed_fwd_kernel<HD, HEADS>, PackedFwdCfg<HD>::SMEM_BYTES) != cudaSuccess) return OA_ERR_LAUNCH;
+  // starts under the launch for short sequences, which is over at once where there are none
   const long long items = HEADS ? (long long)packed_max_tiles(p.plan.tokens, p.plan.batch) * (p.q_heads / 2)
                                      : (long long)packed_max_pairs(p.plan.tokens, p.plan.batch) * p.q_heads;
-  launch_pdl(packed_fwd_kernel<HD, HEADS>, dim3(packed_ctas(items)), dim3(PackedFwdCfg<HD>::THREADS), PackedFwdCfg<HD>::SMEM_BYTES, st, tq, tk, tv, p);
+  launch_pdl_if(pdl_on(true), packed_fwd_kernel<HD, HEADS>, dim3(packed_ctas(items)), dim3(PackedFwdCfg<HD>::THREADS), PackedFwdCfg<HD>::SMEM_BYTES, st, tq, tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }
 
@@ -1249,7 +1250,7 @@ static int packed_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
   if (allow_smem(allowed_kv, (const void*)packed_bwd_kv_kernel<HD>, PackedKvCfg<HD>::SMEM_BYTES) != cudaSuccess) return OA_ERR_LAUNCH;
   if (allow_smem(allowed_q, (const void*)packed_bwd_q_kernel<HD>, PackedQCfg<HD>::SMEM_BYTES) != cudaSuccess) return OA_ERR_LAUNCH;
   const long long tiles = packed_max_tiles(p.plan.tokens, p.plan.batch);
-  launch_pdl(packed_bwd_kv_kernel<HD>, dim3(packed_ctas(tiles * p.kv_heads)), dim3(PB_THREADS), PackedKvCfg<HD>::SMEM_BYTES, st, tq, tk, tv, tdo, p);
+  launch_pdl_if(pdl_on(true), packed_bwd_kv_kernel<HD>, dim3(packed_ctas(tiles * p.kv_heads)), dim3(PB_THREADS), PackedKvCfg<HD>::SMEM_BYTES, st, tq, tk, tv, tdo, p);
   launch_pdl(packed_bwd_q_kernel<HD>, dim3(packed_ctas(tiles * p.q_heads)), dim3(PB_THREADS), PackedQCfg<HD>::SMEM_BYTES, st, tq, tk, tv, tdo, p);
   return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }

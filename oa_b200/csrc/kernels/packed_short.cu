@@ -1,9 +1,9 @@
 // Causal attention over packed sequences of up to 64 rows, forward and backward, bf16 in / fp32 accumulate: the sequences that a tile of 128 x 128 would be
 // mostly empty for (packed_attn.cu has the mathematics and the longer ones).
 //
-// A block of four warps works on one sequence and one head (backward: one key-value head with its query heads in turn).  Its rows come to shared memory by
-// cp.async, in 16-byte pieces swizzled over eight banks' groups; rows behind the sequence up to the next 16 are zeros.  A warp takes 16 queries (forward, dQ)
-// or 16 keys (dK, dV) and the products run on mma.sync, whose accumulators are the next product's operand as they stand: tiles this small cannot
+// A block of four warps works on one sequence and as many heads as give every warp 16 rows of one (backward: key-value heads, each with its query heads in turn).  The
+// rows come to shared memory by cp.async, in 16-byte pieces swizzled over eight banks' groups; rows behind the sequence up to the next 16 are zeros.  A warp
+// takes 16 queries (forward, dQ) or 16 keys (dK, dV) and the products run on mma.sync, whose accumulators are the next product's operand as they stand: tiles this small cannot
 // fill a tcgen05 instruction.  Backward, scores are worked out twice, with the keys as rows for dK and dV and with the queries as rows for dQ.  Bound by latency: loads,
 // a chain of products and exponentials, stores, one after the other, which as many blocks as fit on an SM cover for one another.
 #include "common.cuh"
@@ -17,36 +17,38 @@ namespace oa {
 constexpr int PS_THREADS = 128;
 constexpr float PS_LOG2E = 1.4426950408889634f;
 
-// [64][HD] bf16 in shared memory
+// [64][HD] bf16 in shared memory, at a multiple of 256 bytes: piece c of row r stands at place c ^ (r & 7).  A lane's address is worked out once for a set of rows;
+// another pair of pieces 2 k, 2 k + 1 of the same rows is that with 32 k exclusive-or'ed into it, 16 rows on are 16 STRIDE.
 template <int HD>
 struct ShortTile {
-  static constexpr int BYTES = PACKED_SHORT * HD * 2, CHUNKS = HD / 8;
-  static __device__ __forceinline__ uint32_t at(uint32_t base, int row, int chunk) { return base + row * (HD * 2) + ((chunk ^ (row & 7)) << 4); }
-  // rows [0, n) from memory, zeros up to `rows`
-  static __device__ __forceinline__ void fetch(uint32_t base, const __nv_bfloat16* from, long long stride, int n, int rows) {
-    for (int i = threadIdx.x; i < rows * CHUNKS; i += PS_THREADS) {
-      const int r = i / CHUNKS, c = i % CHUNKS;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at(base, r, c)), "l"(from + (r < n ? r : 0) * stride + c * 8), "r"(r < n ? 16 : 0) : "memory");
+  static constexpr int STRIDE = HD * 2, BYTES = PACKED_SHORT * STRIDE, CHUNKS = HD / 8;
+  // of a left operand [16 rows x 16 dimensions], and of a right one whose reduction runs along the 16 rows
+  static __device__ __forceinline__ uint32_t rows_first(int lane) { return (lane & 15) * STRIDE + (((lane >> 4) ^ (lane & 7)) << 4); }
+  // of two right operands of 8 columns each, where columns are rows and the reduction runs along dimensions
+  static __device__ __forceinline__ uint32_t columns_first(int lane) { return ((lane & 7) + ((lane >> 4) << 3)) * STRIDE + ((((lane >> 3) & 1) ^ (lane & 7)) << 4); }
+  // rows [0, n) of each of `heads` heads from memory, with zeros up to 16 `tiles` behind each; first(u): where head u's first row begins.  A pass of the
+  // block covers 16 rows (8 at head dim 128), so that its head is one for all threads.
+  template <typename F>
+  static __device__ __forceinline__ void fetch(uint32_t base, long long stride, int n, int tiles, int heads, F first) {
+    constexpr int ROWS = PS_THREADS / CHUNKS;
+    const int r0 = threadIdx.x / CHUNKS, c = threadIdx.x % CHUNKS;
+    uint32_t to = base + r0 * STRIDE + ((c ^ (r0 & 7)) << 4);
+    for (int u = 0; u < heads; ++u) {
+      const __nv_bfloat16* head = first(u) + c * 8;
+      const __nv_bfloat16* src = head + r0 * stride;
+#pragma unroll 2
+      for (int row = r0; row < tiles * 16; row += ROWS, to += ROWS * STRIDE, src += ROWS * stride)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(row < n ? src : head), "r"(row < n ? 16 : 0) : "memory");
     }
-  }
-  // [16 rows x 16 dimensions] as the left operand, rows r0.., dimensions 16 k..
-  static __device__ __forceinline__ void left(uint32_t (&a)[4], uint32_t base, int r0, int k, int lane) {
-    ld4(a, at(base, r0 + (lane & 15), 2 * k + (lane >> 4)));
-  }
-  // the same rows as the right operand of two products of 8 columns each (columns are rows here, the reduction runs along dimensions)
-  static __device__ __forceinline__ void right(uint32_t (&b)[4], uint32_t base, int r0, int k, int lane) {
-    ld4(b, at(base, r0 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
-  }
-  // ... and where the reduction runs along the 16 rows r0.., the columns are dimensions 16 c..
-  static __device__ __forceinline__ void right_t(uint32_t (&b)[4], uint32_t base, int r0, int c, int lane) {
-    const uint32_t p = at(base, r0 + (lane & 15), 2 * c + (lane >> 4));
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "r"(p) : "memory");
-  }
-  static __device__ __forceinline__ void ld4(uint32_t (&a)[4], uint32_t p) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(p) : "memory");
   }
 };
 
+__device__ __forceinline__ void short_ld4(uint32_t (&a)[4], uint32_t p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(p) : "memory");
+}
+__device__ __forceinline__ void short_ld4_t(uint32_t (&a)[4], uint32_t p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(p) : "memory");
+}
 __device__ __forceinline__ void short_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -54,25 +56,27 @@ __device__ __forceinline__ void short_mma(float (&d)[4], const uint32_t (&a)[4],
 __device__ __forceinline__ void short_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void short_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
-// [16 x 16] += rows of x times rows of y, over HD dimensions: d[0], d[1] are the halves of 8 columns
+// [16 x 16] = rows of x (their address as a left operand) times rows of y (as right ones), over HD dimensions: d[0], d[1] are the halves of 8 columns
 template <int HD>
-__device__ __forceinline__ void short_scores(float (&d)[2][4], uint32_t x, int x0, uint32_t y, int y0, int lane) {
+__device__ __forceinline__ void short_scores(float (&d)[2][4], uint32_t x, uint32_t y) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) d[0][u] = d[1][u] = 0.f;
 #pragma unroll
   for (int k = 0; k < HD / 16; ++k) {
     uint32_t a[4], b[4];
-    ShortTile<HD>::left(a, x, x0, k, lane);
-    ShortTile<HD>::right(b, y, y0, k, lane);
+    short_ld4(a, x ^ (k << 5));
+    short_ld4(b, y ^ (k << 5));
     short_mma(d[0], a, b[0], b[1]);
     short_mma(d[1], a, b[2], b[3]);
   }
 }
-// acc[16 x HD] += w[16 x 16] times rows y0.. of y
+// acc[16 x HD] += w[16 x 16] times 16 rows of y
 template <int HD>
-__device__ __forceinline__ void short_weigh(float (&acc)[HD / 8][4], const uint32_t (&w)[4], uint32_t y, int y0, int lane) {
+__device__ __forceinline__ void short_weigh(float (&acc)[HD / 8][4], const uint32_t (&w)[4], uint32_t y) {
 #pragma unroll
   for (int c = 0; c < HD / 16; ++c) {
     uint32_t b[4];
-    ShortTile<HD>::right_t(b, y, y0, c, lane);
+    short_ld4_t(b, y ^ (c << 5));
     short_mma(acc[2 * c], w, b[0], b[1]);
     short_mma(acc[2 * c + 1], w, b[2], b[3]);
   }
@@ -85,65 +89,96 @@ __device__ __forceinline__ void short_operand(uint32_t (&w)[4], const float (&d)
     w[2 * h + 1] = pack_bf16x2(d[h][2], d[h][3]);
   }
 }
-// A warp's 16 rows r0.. of an accumulator, times mul0 / mul1 for its rows lane / 4 and + 8, to memory through the rows of a tile that only this warp uses: those
-// below `n`, in 16-byte pieces
+// A warp's 16 rows of an accumulator, times mul0 / mul1 for its rows lane / 4 and + 8, to memory through 16 rows of a tile (their address) that only this warp
+// uses: the first `n`, in 16-byte pieces
 template <int HD>
-__device__ __forceinline__ void short_store(const float (&acc)[HD / 8][4], float mul0, float mul1, uint8_t* smem, uint32_t base, int r0, int n, __nv_bfloat16* to,
-                                            long long stride, int lane) {
-  const uint32_t off = base - smem_u32(smem);
+__device__ __forceinline__ void short_store(const float (&acc)[HD / 8][4], float mul0, float mul1, uint32_t rows, int n, __nv_bfloat16* to, long long stride, int lane) {
+  constexpr int STRIDE = ShortTile<HD>::STRIDE, CHUNKS = HD / 8;
+  const uint32_t put = rows + (lane >> 2) * STRIDE + (((lane >> 2) & 7) << 4) + (lane & 3) * 4;
 #pragma unroll
-  for (int c = 0; c < HD / 8; ++c) {
-    *reinterpret_cast<uint32_t*>(smem + ShortTile<HD>::at(off, r0 + (lane >> 2), c) + (lane & 3) * 4) = pack_bf16x2(acc[c][0] * mul0, acc[c][1] * mul0);
-    *reinterpret_cast<uint32_t*>(smem + ShortTile<HD>::at(off, r0 + 8 + (lane >> 2), c) + (lane & 3) * 4) = pack_bf16x2(acc[c][2] * mul1, acc[c][3] * mul1);
+  for (int c = 0; c < CHUNKS; ++c) {
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(put ^ (c << 4)), "r"(pack_bf16x2(acc[c][0] * mul0, acc[c][1] * mul0)) : "memory");
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"((put ^ (c << 4)) + 8 * STRIDE), "r"(pack_bf16x2(acc[c][2] * mul1, acc[c][3] * mul1)) : "memory");
   }
   __syncwarp();
+  constexpr int ROWS = 32 / CHUNKS;                                    // of a pass
+  const int r0 = lane / CHUNKS, c = lane % CHUNKS;
+  to += r0 * stride + c * 8;
 #pragma unroll
-  for (int i = lane; i < 16 * HD / 8; i += 32) {
-    const int r = r0 + i / (HD / 8), c = i % (HD / 8);
-    if (r < n) *reinterpret_cast<uint4*>(to + r * stride + c * 8) = *reinterpret_cast<const uint4*>(smem + ShortTile<HD>::at(off, r, c));
+  for (int r = 0; r < 16; r += ROWS, to += ROWS * stride) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(rows + (r + r0) * STRIDE + ((c ^ ((r + r0) & 7)) << 4)) : "memory");
+    if (r + r0 < n) *reinterpret_cast<uint4*>(to) = v;
   }
   __syncwarp();
 }
 
+// A block's task: a sequence and up to four / tiles of its heads, where 16-row tiles of all together are four at most
+struct ShortTask {
+  int lo, n, rows, tiles, head, heads;     // head: the first
+  // task = set of heads * sequences + sequence; false: the sequence has fewer sets
+  __device__ __forceinline__ bool take(const PackedPlan& plan, int shorts, int task, int all_heads) {
+    const int4 e = plan.brief(task % shorts);
+    lo = e.x;
+    n = e.y - e.x;
+    tiles = (n + 15) >> 4;
+    rows = tiles * 16;
+    const int set = tiles == 1 ? 4 : tiles == 2 ? 2 : 1;
+    head = task / shorts * set;
+    heads = min(set, all_heads - head);
+    return heads > 0;
+  }
+};
+
 template <int HD>
-__global__ void __launch_bounds__(PS_THREADS) packed_short_fwd_kernel(const PackedShortFwd p) {
+__global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 5 : 2) packed_short_fwd_kernel(const PackedShortFwd p) {
   using Tile = ShortTile<HD>;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
+  pdl_launch_dependents();
   const uint32_t sq = smem_u32(smem), sk = sq + Tile::BYTES, sv = sk + Tile::BYTES;
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tasks = p.plan.shorts() * p.q_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, shorts = p.plan.shorts(), tasks = shorts * p.q_heads;
   const float sl2 = p.scale * PS_LOG2E;
+  const uint32_t rows_at = Tile::rows_first(lane), columns_at = Tile::columns_first(lane);
   for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
-    const int4 e = p.plan.brief(task / p.q_heads);
-    const int h = task % p.q_heads, hk = h / p.group, n = e.y - e.x, rows = (n + 15) & ~15;
-    Tile::fetch(sq, p.q + e.x * p.qs + h * HD, p.qs, n, rows);
-    Tile::fetch(sk, p.k + e.x * p.ks + hk * HD, p.ks, n, rows);
-    Tile::fetch(sv, p.v + e.x * p.vs + hk * HD, p.vs, n, rows);
+    ShortTask e;
+    if (!e.take(p.plan, shorts, task, p.q_heads)) continue;
+    int kv[4];                               // key-value heads of the query heads
+#pragma unroll
+    for (int u = 0; u < 4; ++u) kv[u] = p.group == 1 ? e.head + u : (e.head + u) / p.group;
+    const auto kv_at = [&](int u) { return (u == 0 ? kv[0] : u == 1 ? kv[1] : u == 2 ? kv[2] : kv[3]) * HD; };
+    Tile::fetch(sq, p.qs, e.n, e.tiles, e.heads, [&](int u) { return p.q + e.lo * p.qs + (e.head + u) * HD; });
+    Tile::fetch(sk, p.ks, e.n, e.tiles, e.heads, [&](int u) { return p.k + e.lo * p.ks + kv_at(u); });
+    Tile::fetch(sv, p.vs, e.n, e.tiles, e.heads, [&](int u) { return p.v + e.lo * p.vs + kv_at(u); });
     short_commit();
     short_wait();
     __syncthreads();
-    const int r0 = warp * 16;
-    if (r0 < n) {
+    const int u = warp / e.tiles, tile = warp - u * e.tiles, base = u * e.rows, r0 = base + tile * 16;      // in shared memory
+    if (u < e.heads) {
       // scores of 16 queries and the keys up to them, at most 64
+      constexpr int STEP = 16 * Tile::STRIDE;
       float s[4][2][4];
-      const int i0 = r0 + (lane >> 2), i1 = i0 + 8;                    // this thread's queries
+      const int i0 = tile * 16 + (lane >> 2), i1 = i0 + 8;             // this thread's queries
       float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        if (t > warp) break;
+        if (t > tile) break;
+        short_scores<HD>(s[t], sq + r0 * Tile::STRIDE + rows_at, sk + base * Tile::STRIDE + t * STEP + columns_at);
+        if (t == tile) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) s[t][c][0] = s[t][c][1] = s[t][c][2] = s[t][c][3] = 0.f;
-        short_scores<HD>(s[t], sq, r0, sk, t * 16, lane);
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+            for (int x = 0; x < 2; ++x) {
+              const int j = t * 16 + c * 8 + (lane & 3) * 2 + x;
+              s[t][c][x] = j <= i0 ? s[t][c][x] : -INFINITY;
+              s[t][c][2 + x] = j <= i1 ? s[t][c][2 + x] : -INFINITY;
+            }
+        }
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int j = t * 16 + c * 8 + (lane & 3) * 2 + u;
-            s[t][c][u] = j <= i0 ? s[t][c][u] : -INFINITY;
-            s[t][c][2 + u] = j <= i1 ? s[t][c][2 + u] : -INFINITY;
-            m0 = fmaxf(m0, s[t][c][u]);
-            m1 = fmaxf(m1, s[t][c][2 + u]);
-          }
+        for (int c = 0; c < 2; ++c) {
+          m0 = fmax3(m0, s[t][c][0], s[t][c][1]);
+          m1 = fmax3(m1, s[t][c][2], s[t][c][3]);
+        }
       }
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) {
@@ -157,7 +192,7 @@ __global__ void __launch_bounds__(PS_THREADS) packed_short_fwd_kernel(const Pack
       for (int c = 0; c < HD / 8; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        if (t > warp) break;
+        if (t > tile) break;
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -167,7 +202,7 @@ __global__ void __launch_bounds__(PS_THREADS) packed_short_fwd_kernel(const Pack
           }
         uint32_t w[4];
         short_operand(w, s[t]);
-        short_weigh<HD>(o, w, sv, t * 16, lane);
+        short_weigh<HD>(o, w, sv + base * Tile::STRIDE + t * STEP + rows_at);
       }
 #pragma unroll
       for (int q = 1; q < 4; q <<= 1) {
@@ -175,108 +210,129 @@ __global__ void __launch_bounds__(PS_THREADS) packed_short_fwd_kernel(const Pack
         l1 += __shfl_xor_sync(0xffffffffu, l1, q);
       }
       if (p.lse && (lane & 3) == 0) {
-        float* to = p.lse + (long long)h * p.plan.tokens + e.x;
-        if (i0 < n) to[i0] = (m0 + log2f(l0)) / PS_LOG2E;
-        if (i1 < n) to[i1] = (m1 + log2f(l1)) / PS_LOG2E;
+        float* to = p.lse + (long long)(e.head + u) * p.plan.tokens + e.lo;
+        if (i0 < e.n) to[i0] = (m0 + log2f(l0)) / PS_LOG2E;
+        if (i1 < e.n) to[i1] = (m1 + log2f(l1)) / PS_LOG2E;
       }
-      short_store<HD>(o, 1.f / l0, 1.f / l1, smem, sq, r0, n, p.o + e.x * p.os + h * HD, p.os, lane);
+      short_store<HD>(o, 1.f / l0, 1.f / l1, sq + r0 * Tile::STRIDE, e.n - tile * 16, p.o + (e.lo + tile * 16) * p.os + (e.head + u) * HD, p.os, lane);
     }
     __syncthreads();                                                   // the tiles are free
   }
 }
 
 template <int HD>
-__global__ void __launch_bounds__(PS_THREADS) packed_short_bwd_kernel(const PackedShortBwd p) {
+__global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd_kernel(const PackedShortBwd p) {
   using Tile = ShortTile<HD>;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
+  pdl_launch_dependents();
   const uint32_t sq = smem_u32(smem), sdo = sq + Tile::BYTES, sk = sdo + Tile::BYTES, sv = sk + Tile::BYTES;
   float* stat = reinterpret_cast<float*>(smem + 4 * Tile::BYTES);      // [2][64]: -lse log2(e), -delta scale
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tasks = p.plan.shorts() * p.kv_heads, r0 = warp * 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, shorts = p.plan.shorts(), tasks = shorts * p.kv_heads;
   const float sl2 = p.scale * PS_LOG2E, scale = p.scale;
+  const uint32_t rows_at = Tile::rows_first(lane), columns_at = Tile::columns_first(lane);
   for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
-    const int4 e = p.plan.brief(task / p.kv_heads);
-    const int hk = task % p.kv_heads, n = e.y - e.x, rows = (n + 15) & ~15;
-    Tile::fetch(sk, p.k + e.x * p.ks + hk * HD, p.ks, n, rows);
-    Tile::fetch(sv, p.v + e.x * p.vs + hk * HD, p.vs, n, rows);
+    ShortTask e;
+    if (!e.take(p.plan, shorts, task, p.kv_heads)) continue;
+    Tile::fetch(sk, p.ks, e.n, e.tiles, e.heads, [&](int u) { return p.k + e.lo * p.ks + (e.head + u) * HD; });
+    Tile::fetch(sv, p.vs, e.n, e.tiles, e.heads, [&](int u) { return p.v + e.lo * p.vs + (e.head + u) * HD; });
+    const int n = e.n, u = warp / e.tiles, tile = warp - u * e.tiles, base = u * e.rows, r0 = base + tile * 16;      // in shared memory
+    const long long row0 = e.lo + tile * 16;
     float dk[HD / 8][4], dv[HD / 8][4];
 #pragma unroll
     for (int c = 0; c < HD / 8; ++c)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) dk[c][u] = dv[c][u] = 0.f;
+      for (int x = 0; x < 4; ++x) dk[c][x] = dv[c][x] = 0.f;
     for (int g = 0; g < p.group; ++g) {
-      const int h = hk * p.group + g;
-      Tile::fetch(sq, p.q + e.x * p.qs + h * HD, p.qs, n, rows);
-      Tile::fetch(sdo, p.dout + e.x * p.dos + h * HD, p.dos, n, rows);
+      // query head g of every key-value head
+      Tile::fetch(sq, p.qs, n, e.tiles, e.heads, [&](int v) { return p.q + e.lo * p.qs + ((e.head + v) * p.group + g) * HD; });
+      Tile::fetch(sdo, p.dos, n, e.tiles, e.heads, [&](int v) { return p.dout + e.lo * p.dos + ((e.head + v) * p.group + g) * HD; });
       short_commit();
-      if (threadIdx.x < PACKED_SHORT) {
-        const bool there = (int)threadIdx.x < n;
-        const long long at = (long long)h * p.plan.tokens + e.x + threadIdx.x;
-        stat[threadIdx.x] = there ? -p.lse[at] * PS_LOG2E : -INFINITY;
-        stat[PACKED_SHORT + threadIdx.x] = there ? -p.delta[at] * scale : 0.f;
+      if (threadIdx.x < e.heads * e.rows) {
+        const int v = e.tiles == 1 ? threadIdx.x >> 4 : e.tiles == 2 ? threadIdx.x >> 5 : 0, in = threadIdx.x - v * e.rows;
+        const long long at = (long long)((e.head + v) * p.group + g) * p.plan.tokens + e.lo + in;
+        stat[threadIdx.x] = in < n ? -p.lse[at] * PS_LOG2E : -INFINITY;
+        stat[PACKED_SHORT + threadIdx.x] = in < n ? -p.delta[at] * scale : 0.f;
       }
       short_wait();
       __syncthreads();
-      if (r0 < n) {
+      if (u < e.heads) {
+        constexpr int STEP = 16 * Tile::STRIDE;
+        const uint32_t mine = r0 * Tile::STRIDE, all = base * Tile::STRIDE;
         // keys as rows: P^T and dS^T, for the queries from them on
-        const int j0 = r0 + (lane >> 2), j1 = j0 + 8;
+        const int j0 = tile * 16 + (lane >> 2), j1 = j0 + 8;
 #pragma unroll 1
-        for (int t = warp; t * 16 < n; ++t) {
-          float s[2][4] = {}, dp[2][4] = {};
-          short_scores<HD>(s, sk, r0, sq, t * 16, lane);
-          short_scores<HD>(dp, sv, r0, sdo, t * 16, lane);
+        for (int t = tile; t < e.tiles; ++t) {
+          float s[2][4], dp[2][4];
+          short_scores<HD>(s, sk + mine + rows_at, sq + all + t * STEP + columns_at);
+          short_scores<HD>(dp, sv + mine + rows_at, sdo + all + t * STEP + columns_at);
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+          for (int c = 0; c < 2; ++c) {
+            const int i = t * 16 + c * 8 + (lane & 3) * 2;
+            const float2 nl = *reinterpret_cast<const float2*>(stat + base + i), nd = *reinterpret_cast<const float2*>(stat + PACKED_SHORT + base + i);
+            s[c][0] = fast_exp2(fmaf(s[c][0], sl2, nl.x));
+            s[c][1] = fast_exp2(fmaf(s[c][1], sl2, nl.y));
+            s[c][2] = fast_exp2(fmaf(s[c][2], sl2, nl.x));
+            s[c][3] = fast_exp2(fmaf(s[c][3], sl2, nl.y));
+            dp[c][0] = s[c][0] * fmaf(dp[c][0], scale, nd.x);
+            dp[c][1] = s[c][1] * fmaf(dp[c][1], scale, nd.y);
+            dp[c][2] = s[c][2] * fmaf(dp[c][2], scale, nd.x);
+            dp[c][3] = s[c][3] * fmaf(dp[c][3], scale, nd.y);
+            if (t == tile || t + 1 == e.tiles) {                       // queries before the key, and behind the sequence
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int i = t * 16 + c * 8 + (lane & 3) * 2 + u;
-              const float nl = stat[i], nd = stat[PACKED_SHORT + i];
-              const bool a0 = j0 <= i && i < n, a1 = j1 <= i && i < n;
-              s[c][u] = a0 ? fast_exp2(fmaf(s[c][u], sl2, nl)) : 0.f;
-              s[c][2 + u] = a1 ? fast_exp2(fmaf(s[c][2 + u], sl2, nl)) : 0.f;
-              dp[c][u] = a0 ? s[c][u] * fmaf(dp[c][u], scale, nd) : 0.f;
-              dp[c][2 + u] = a1 ? s[c][2 + u] * fmaf(dp[c][2 + u], scale, nd) : 0.f;
+              for (int x = 0; x < 2; ++x) {
+                const bool a0 = j0 <= i + x && i + x < n, a1 = j1 <= i + x && i + x < n;
+                s[c][x] = a0 ? s[c][x] : 0.f;
+                s[c][2 + x] = a1 ? s[c][2 + x] : 0.f;
+                dp[c][x] = a0 ? dp[c][x] : 0.f;
+                dp[c][2 + x] = a1 ? dp[c][2 + x] : 0.f;
+              }
             }
+          }
           uint32_t w[4];
           short_operand(w, s);
-          short_weigh<HD>(dv, w, sdo, t * 16, lane);
+          short_weigh<HD>(dv, w, sdo + all + t * STEP + rows_at);
           short_operand(w, dp);
-          short_weigh<HD>(dk, w, sq, t * 16, lane);
+          short_weigh<HD>(dk, w, sq + all + t * STEP + rows_at);
         }
         // queries as rows: dS, for the keys up to them
         float dq[HD / 8][4];
 #pragma unroll
         for (int c = 0; c < HD / 8; ++c) dq[c][0] = dq[c][1] = dq[c][2] = dq[c][3] = 0.f;
-        const float nl0 = stat[j0], nl1 = stat[j1], nd0 = stat[PACKED_SHORT + j0], nd1 = stat[PACKED_SHORT + j1];
+        const float nl0 = stat[base + j0], nl1 = stat[base + j1], nd0 = stat[PACKED_SHORT + base + j0], nd1 = stat[PACKED_SHORT + base + j1];
 #pragma unroll 1
-        for (int t = 0; t <= warp; ++t) {
-          float s[2][4] = {}, dp[2][4] = {};
-          short_scores<HD>(s, sq, r0, sk, t * 16, lane);
-          short_scores<HD>(dp, sdo, r0, sv, t * 16, lane);
+        for (int t = 0; t <= tile; ++t) {
+          float s[2][4], dp[2][4];
+          short_scores<HD>(s, sq + mine + rows_at, sk + all + t * STEP + columns_at);
+          short_scores<HD>(dp, sdo + mine + rows_at, sv + all + t * STEP + columns_at);
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int j = t * 16 + c * 8 + (lane & 3) * 2 + u;
-              dp[c][u] = j <= j0 ? fast_exp2(fmaf(s[c][u], sl2, nl0)) * fmaf(dp[c][u], scale, nd0) : 0.f;
-              dp[c][2 + u] = j <= j1 ? fast_exp2(fmaf(s[c][2 + u], sl2, nl1)) * fmaf(dp[c][2 + u], scale, nd1) : 0.f;
+            for (int x = 0; x < 2; ++x) {
+              dp[c][x] = fast_exp2(fmaf(s[c][x], sl2, nl0)) * fmaf(dp[c][x], scale, nd0);
+              dp[c][2 + x] = fast_exp2(fmaf(s[c][2 + x], sl2, nl1)) * fmaf(dp[c][2 + x], scale, nd1);
+              if (t == tile) {
+                const int j = t * 16 + c * 8 + (lane & 3) * 2 + x;
+                dp[c][x] = j <= j0 ? dp[c][x] : 0.f;
+                dp[c][2 + x] = j <= j1 ? dp[c][2 + x] : 0.f;
+              }
             }
           uint32_t w[4];
           short_operand(w, dp);
-          short_weigh<HD>(dq, w, sk, t * 16, lane);
+          short_weigh<HD>(dq, w, sk + all + t * STEP + rows_at);
         }
         __syncwarp();
         // this warp's rows of dO have other readers, and Q's too: both are done with behind the barrier
         __syncthreads();
-        short_store<HD>(dq, 1.f, 1.f, smem, sq, r0, n, p.dq + e.x * p.dqs + h * HD, p.dqs, lane);
+        short_store<HD>(dq, 1.f, 1.f, sq + r0 * Tile::STRIDE, n - tile * 16, p.dq + row0 * p.dqs + ((e.head + u) * p.group + g) * HD, p.dqs, lane);
       } else {
         __syncthreads();
       }
       __syncthreads();                                                 // Q and dO may be written over
     }
-    if (r0 < n) {
-      short_store<HD>(dk, 1.f, 1.f, smem, sk, r0, n, p.dk + e.x * p.dks + hk * HD, p.dks, lane);
-      short_store<HD>(dv, 1.f, 1.f, smem, sv, r0, n, p.dv + e.x * p.dvs + hk * HD, p.dvs, lane);
+    if (u < e.heads) {
+      short_store<HD>(dk, 1.f, 1.f, sk + r0 * Tile::STRIDE, n - tile * 16, p.dk + row0 * p.dks + (e.head + u) * HD, p.dks, lane);
+      short_store<HD>(dv, 1.f, 1.f, sv + r0 * Tile::STRIDE, n - tile * 16, p.dv + row0 * p.dvs + (e.head + u) * HD, p.dvs, lane);
     }
     __syncthreads();
   }
@@ -287,21 +343,21 @@ template <typename P>
 static int short_launch(void (*kernel)(const P), int smem, std::atomic<unsigned long long>& allowed, int per_sm, long long most, const P& p, cudaStream_t st) {
   if (allow_smem(allowed, (const void*)kernel, smem) != cudaSuccess) return OA_ERR_LAUNCH;
   const long long room = (long long)per_sm * sm_count();
-  launch_pdl(kernel, dim3((unsigned)(most < 1 ? 1 : most < room ? most : room)), dim3(PS_THREADS), smem, st, p);
+  launch_short(kernel, dim3((unsigned)(most < 1 ? 1 : most < room ? most : room)), dim3(PS_THREADS), smem, st, p);
   return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }
 
 int packed_short_fwd(const PackedShortFwd& p, int head_dim, cudaStream_t st) {
   static std::atomic<unsigned long long> a64, a128;
   const long long most = (long long)p.plan.batch * p.q_heads;
-  return head_dim == 64 ? short_launch(packed_short_fwd_kernel<64>, 3 * ShortTile<64>::BYTES, a64, 4, most, p, st)
-                        : short_launch(packed_short_fwd_kernel<128>, 3 * ShortTile<128>::BYTES, a128, 4, most, p, st);
+  return head_dim == 64 ? short_launch(packed_short_fwd_kernel<64>, 3 * ShortTile<64>::BYTES, a64, 5, most, p, st)
+                        : short_launch(packed_short_fwd_kernel<128>, 3 * ShortTile<128>::BYTES, a128, 2, most, p, st);
 }
 
 int packed_short_bwd(const PackedShortBwd& p, int head_dim, cudaStream_t st) {
   static std::atomic<unsigned long long> a64, a128;
   const long long most = (long long)p.plan.batch * p.kv_heads;
-  return head_dim == 64 ? short_launch(packed_short_bwd_kernel<64>, 4 * ShortTile<64>::BYTES + 512, a64, 4, most, p, st)
+  return head_dim == 64 ? short_launch(packed_short_bwd_kernel<64>, 4 * ShortTile<64>::BYTES + 512, a64, 3, most, p, st)
                         : short_launch(packed_short_bwd_kernel<128>, 4 * ShortTile<128>::BYTES + 512, a128, 2, most, p, st);
 }
 

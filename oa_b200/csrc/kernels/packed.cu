@@ -47,13 +47,14 @@ __device__ __forceinline__ int plan_scan(int v, int* s_warp, Op op) {   // inclu
 }
 
 __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedPlanParams p) {
-  __shared__ int s_warp[32], s_count[2][PLAN_BINS], s_top, s_short;
+  __shared__ int s_warp[32], s_count[2][PLAN_BINS], s_top, s_short[3];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, shift = p.shift, per = 1 << shift;
   int* starts = p.plan + PACKED_HEADER;
   s_count[0][tid] = s_count[1][tid] = 0;
-  if (tid == 0) s_top = s_short = 0;
+  if (tid < 3) s_short[tid] = 0;
+  if (tid == 0) s_top = 0;
   const auto most = [](int a, int b) { return max(a, b); };
   for (int b0 = 0; b0 <= p.batch; b0 += PLAN_THREADS) {
     const int b = b0 + tid;
@@ -102,14 +103,28 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedP
   lists[0] = reinterpret_cast<int4*>(p.plan + packed_tiles_at(p.batch));
   lists[1] = lists[0] + packed_max_tiles(p.tokens, p.batch);
   lists[2] = lists[1] + packed_max_pairs(p.tokens, p.batch);
-  for (int b0 = tid - lane; b0 < p.batch; b0 += PLAN_THREADS) {
-    const int b = b0 + lane;
-    const int lo = b < p.batch ? starts[b] : 0, hi = b < p.batch ? starts[b + 1] : 0;
-    const bool brief = hi > lo && hi - lo <= PACKED_SHORT;
-    const unsigned all = __ballot_sync(0xffffffffu, brief);
-    int base = lane == 0 && all ? atomicAdd(&s_short, __popc(all)) : 0;
-    base = __shfl_sync(0xffffffffu, base, 0);
-    if (brief) lists[2][base + __popc(all & ((1u << lane) - 1))] = make_int4(lo, hi, 0, b);
+  // short sequences by their number of 16 rows, most first: counted, then placed
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int b0 = tid - lane; b0 < p.batch; b0 += PLAN_THREADS) {
+      const int b = b0 + lane;
+      const int lo = b < p.batch ? starts[b] : 0, hi = b < p.batch ? starts[b + 1] : 0, n = hi - lo;
+      const int mine = n < 1 || n > PACKED_SHORT ? -1 : n > 32 ? 0 : n > 16 ? 1 : 2;
+#pragma unroll
+      for (int c = 0; c < 3; ++c) {
+        const unsigned all = __ballot_sync(0xffffffffu, mine == c);
+        if (!all) continue;
+        int at = lane == 0 ? atomicAdd(&s_short[c], __popc(all)) : 0;
+        at = __shfl_sync(0xffffffffu, at, 0);
+        if (pass == 1 && mine == c) lists[2][at + __popc(all & ((1u << lane) - 1))] = make_int4(lo, hi, 0, b);
+      }
+    }
+    __syncthreads();
+    if (pass == 0 && tid == 0) {
+      const int n0 = s_short[0], n1 = s_short[1];
+      p.plan[4] = n0; p.plan[5] = n1; p.plan[6] = s_short[2];
+      s_short[0] = 0; s_short[1] = n0; s_short[2] = n0 + n1;
+    }
+    __syncthreads();
   }
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
@@ -120,7 +135,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedP
     if (tid == PLAN_THREADS - 1) p.plan[which] = sum;
   }
   __syncthreads();
-  if (tid == 0) { p.plan[2] = starts[0]; p.plan[3] = starts[p.batch]; p.plan[4] = s_short; }
+  if (tid == 0) { p.plan[2] = starts[0]; p.plan[3] = starts[p.batch]; p.plan[7] = 0; }
   walk([&](int which, int bin, int n) { return n > 0 ? atomicAdd(&s_count[which][bin], n) : 0; },
        [&](int which, int at, int first, int n, int lo, int hi, int b) {
          for (int i = 0; i < n; ++i) lists[which][at + i] = make_int4(lo, hi, first + i, b);

@@ -1,6 +1,7 @@
-// The plan of a batch of packed sequences, in int32 words: [tiles, pairs, first row, row behind the last, short sequences, -, -, -, starts.., tiles.., pairs.., short
-// sequences..].  A tile (128 rows) or a pair of tiles of a sequence of more than 64 rows is (first row of its sequence, row behind it, index in the sequence,
-// sequence), the largest index first; a short sequence is (first row, row behind it, 0, sequence).
+// The plan of a batch of packed sequences, in int32 words: [tiles, pairs, first row, row behind the last, short sequences of 33 to 64 rows, of 17 to 32, of up to 16, -,
+// starts.., tiles.., pairs.., short sequences..].  A tile (128 rows) or a pair of tiles of a sequence of more than 64 rows is (first row of its sequence, row behind it, index in the sequence,
+// sequence), the largest index first; a short sequence is (first row, row behind it, 0, sequence), in the order
+// of the three counts.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -20,7 +21,7 @@ struct PackedPlan {
   int batch, tokens;
   __device__ __forceinline__ int tiles() const { return words[0]; }
   __device__ __forceinline__ int pairs() const { return words[1]; }
-  __device__ __forceinline__ int shorts() const { return words[4]; }
+  __device__ __forceinline__ int shorts() const { return words[4] + words[5] + words[6]; }
   __device__ __forceinline__ int4 tile(int i) const { return reinterpret_cast<const int4*>(words + packed_tiles_at(batch))[i]; }
   __device__ __forceinline__ int4 pair(int i) const {
     return reinterpret_cast<const int4*>(words + packed_tiles_at(batch))[packed_max_tiles(tokens, batch) + i];

@@ -54,7 +54,8 @@ __device__ __forceinline__ void short_mma(float (&d)[4], const uint32_t (&a)[4],
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void short_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void short_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void short_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // [16 x 16] = rows of x (their address as a left operand) times rows of y (as right ones), over HD dimensions: d[0], d[1] are the halves of 8 columns
 template <int HD>
@@ -113,48 +114,63 @@ __device__ __forceinline__ void short_store(const float (&acc)[HD / 8][4], float
   __syncwarp();
 }
 
-// A block's task: a sequence and up to four / tiles of its heads, where 16-row tiles of all together are four at most
+// A block's task: a sequence and as many of its heads as make four 16-row tiles at most.  Tasks with three or four tiles to a head come first, then those with two,
+// then one; sets of heads one after the other.
 struct ShortTask {
-  int lo, n, rows, tiles, head, heads;     // head: the first
-  // task = set of heads * sequences + sequence; false: the sequence has fewer sets
-  __device__ __forceinline__ bool take(const PackedPlan& plan, int shorts, int task, int all_heads) {
-    const int4 e = plan.brief(task % shorts);
-    lo = e.x;
-    n = e.y - e.x;
-    tiles = (n + 15) >> 4;
-    rows = tiles * 16;
-    const int set = tiles == 1 ? 4 : tiles == 2 ? 2 : 1;
-    head = task / shorts * set;
-    heads = min(set, all_heads - head);
-    return heads > 0;
+  int lo, n, tiles, head, heads;           // head: the first
+};
+struct ShortWalk {
+  const PackedPlan& plan;
+  const int all_heads, n0, n1, n2, end0, end1, end;
+  int task;
+  int4 ahead;                              // the next task's entry, on its way
+  __device__ __forceinline__ ShortWalk(const PackedPlan& p, int heads)
+      : plan(p), all_heads(heads), n0(p.words[4]), n1(p.words[5]), n2(p.words[6]), end0(n0 * heads), end1(end0 + n1 * ((heads + 1) >> 1)),
+        end(end1 + n2 * ((heads + 3) >> 2)), task(blockIdx.x) { fetch(); }
+  __device__ __forceinline__ void fetch() {
+    if (task < end) ahead = plan.brief(task < end0 ? task % n0 : task < end1 ? n0 + (task - end0) % n1 : n0 + n1 + (task - end1) % n2);
+  }
+  __device__ __forceinline__ bool next(ShortTask& e) {
+    if (task >= end) return false;
+    e.lo = ahead.x;
+    e.n = ahead.y - ahead.x;
+    e.tiles = (e.n + 15) >> 4;
+    e.head = task < end0 ? task / n0 : task < end1 ? (task - end0) / n1 * 2 : (task - end1) / n2 * 4;
+    e.heads = min(task < end0 ? 1 : task < end1 ? 2 : 4, all_heads - e.head);
+    task += gridDim.x;
+    fetch();
+    return true;
   }
 };
 
 template <int HD>
-__global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 5 : 2) packed_short_fwd_kernel(const PackedShortFwd p) {
+__global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 4 : 2) packed_short_fwd_kernel(const PackedShortFwd p) {
   using Tile = ShortTile<HD>;
-  extern __shared__ __align__(1024) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];      // two stages of Q, K, V
   pdl_launch_dependents();
-  const uint32_t sq = smem_u32(smem), sk = sq + Tile::BYTES, sv = sk + Tile::BYTES;
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, shorts = p.plan.shorts(), tasks = shorts * p.q_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float sl2 = p.scale * PS_LOG2E;
-  const uint32_t rows_at = Tile::rows_first(lane), columns_at = Tile::columns_first(lane);
-  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
-    ShortTask e;
-    if (!e.take(p.plan, shorts, task, p.q_heads)) continue;
-    int kv[4];                               // key-value heads of the query heads
-#pragma unroll
-    for (int u = 0; u < 4; ++u) kv[u] = p.group == 1 ? e.head + u : (e.head + u) / p.group;
-    const auto kv_at = [&](int u) { return (u == 0 ? kv[0] : u == 1 ? kv[1] : u == 2 ? kv[2] : kv[3]) * HD; };
-    Tile::fetch(sq, p.qs, e.n, e.tiles, e.heads, [&](int u) { return p.q + e.lo * p.qs + (e.head + u) * HD; });
-    Tile::fetch(sk, p.ks, e.n, e.tiles, e.heads, [&](int u) { return p.k + e.lo * p.ks + kv_at(u); });
-    Tile::fetch(sv, p.vs, e.n, e.tiles, e.heads, [&](int u) { return p.v + e.lo * p.vs + kv_at(u); });
+  const uint32_t rows_at = Tile::rows_first(lane), columns_at = Tile::columns_first(lane), stages = smem_u32(smem);
+  const auto fetch = [&](uint32_t to, const ShortTask& e) {
+    Tile::fetch(to, p.qs, e.n, e.tiles, e.heads, [&](int u) { return p.q + e.lo * p.qs + (e.head + u) * HD; });
+    Tile::fetch(to + Tile::BYTES, p.ks, e.n, e.tiles, e.heads, [&](int u) { return p.k + e.lo * p.ks + (e.head + u) / p.group * HD; });
+    Tile::fetch(to + 2 * Tile::BYTES, p.vs, e.n, e.tiles, e.heads, [&](int u) { return p.v + e.lo * p.vs + (e.head + u) / p.group * HD; });
+  };
+  ShortWalk walk(p.plan, p.q_heads);
+  ShortTask e, then;
+  if (!walk.next(e)) return;
+  fetch(stages, e);
+  short_commit();
+  for (int stage = 0;; stage ^= 1) {
+    const bool more = walk.next(then);
+    if (more) fetch(stages + (stage ^ 1) * 3 * Tile::BYTES, then);
     short_commit();
-    short_wait();
+    short_wait<1>();
     __syncthreads();
-    const int u = warp / e.tiles, tile = warp - u * e.tiles, base = u * e.rows, r0 = base + tile * 16;      // in shared memory
-    if (u < e.heads) {
+    const uint32_t sq = stages + stage * 3 * Tile::BYTES, sk = sq + Tile::BYTES, sv = sk + Tile::BYTES;
+    const int u = e.tiles == 1 ? warp : e.tiles == 2 ? warp >> 1 : 0, tile = warp - u * e.tiles, base = u * e.tiles * 16, r0 = base + tile * 16;
+    if (u < e.heads && tile < e.tiles) {
       // scores of 16 queries and the keys up to them, at most 64
       constexpr int STEP = 16 * Tile::STRIDE;
       float s[4][2][4];
@@ -216,125 +232,161 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 5 : 2) packed_short_fwd
       }
       short_store<HD>(o, 1.f / l0, 1.f / l1, sq + r0 * Tile::STRIDE, e.n - tile * 16, p.o + (e.lo + tile * 16) * p.os + (e.head + u) * HD, p.os, lane);
     }
-    __syncthreads();                                                   // the tiles are free
+    if (!more) break;
+    __syncthreads();                                                   // the stage is free
+    e = then;
   }
 }
+
+// STAGES: 2 where the next rows are on their way during the work on these
+template <int HD> constexpr int PS_STAGES = HD == 64 ? 2 : 1;
+template <int HD> constexpr int PS_BWD_BYTES = PS_STAGES<HD> * (4 * ShortTile<HD>::BYTES + 2 * PACKED_SHORT * 4);
 
 template <int HD>
 __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd_kernel(const PackedShortBwd p) {
   using Tile = ShortTile<HD>;
-  extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr int STAGES = PS_STAGES<HD>;
+  extern __shared__ __align__(1024) uint8_t smem[];      // stages of Q and dO, of K and V, of log-sum-exp and delta
   pdl_launch_dependents();
-  const uint32_t sq = smem_u32(smem), sdo = sq + Tile::BYTES, sk = sdo + Tile::BYTES, sv = sk + Tile::BYTES;
-  float* stat = reinterpret_cast<float*>(smem + 4 * Tile::BYTES);      // [2][64]: -lse log2(e), -delta scale
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, shorts = p.plan.shorts(), tasks = shorts * p.kv_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float sl2 = p.scale * PS_LOG2E, scale = p.scale;
-  const uint32_t rows_at = Tile::rows_first(lane), columns_at = Tile::columns_first(lane);
-  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
-    ShortTask e;
-    if (!e.take(p.plan, shorts, task, p.kv_heads)) continue;
-    Tile::fetch(sk, p.ks, e.n, e.tiles, e.heads, [&](int u) { return p.k + e.lo * p.ks + (e.head + u) * HD; });
-    Tile::fetch(sv, p.vs, e.n, e.tiles, e.heads, [&](int u) { return p.v + e.lo * p.vs + (e.head + u) * HD; });
-    const int n = e.n, u = warp / e.tiles, tile = warp - u * e.tiles, base = u * e.rows, r0 = base + tile * 16;      // in shared memory
-    const long long row0 = e.lo + tile * 16;
-    float dk[HD / 8][4], dv[HD / 8][4];
-#pragma unroll
-    for (int c = 0; c < HD / 8; ++c)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) dk[c][x] = dv[c][x] = 0.f;
-    for (int g = 0; g < p.group; ++g) {
-      // query head g of every key-value head
-      Tile::fetch(sq, p.qs, n, e.tiles, e.heads, [&](int v) { return p.q + e.lo * p.qs + ((e.head + v) * p.group + g) * HD; });
-      Tile::fetch(sdo, p.dos, n, e.tiles, e.heads, [&](int v) { return p.dout + e.lo * p.dos + ((e.head + v) * p.group + g) * HD; });
-      short_commit();
-      if (threadIdx.x < e.heads * e.rows) {
-        const int v = e.tiles == 1 ? threadIdx.x >> 4 : e.tiles == 2 ? threadIdx.x >> 5 : 0, in = threadIdx.x - v * e.rows;
-        const long long at = (long long)((e.head + v) * p.group + g) * p.plan.tokens + e.lo + in;
-        stat[threadIdx.x] = in < n ? -p.lse[at] * PS_LOG2E : -INFINITY;
-        stat[PACKED_SHORT + threadIdx.x] = in < n ? -p.delta[at] * scale : 0.f;
-      }
-      short_wait();
-      __syncthreads();
-      if (u < e.heads) {
-        constexpr int STEP = 16 * Tile::STRIDE;
-        const uint32_t mine = r0 * Tile::STRIDE, all = base * Tile::STRIDE;
-        // keys as rows: P^T and dS^T, for the queries from them on
-        const int j0 = tile * 16 + (lane >> 2), j1 = j0 + 8;
-#pragma unroll 1
-        for (int t = tile; t < e.tiles; ++t) {
-          float s[2][4], dp[2][4];
-          short_scores<HD>(s, sk + mine + rows_at, sq + all + t * STEP + columns_at);
-          short_scores<HD>(dp, sv + mine + rows_at, sdo + all + t * STEP + columns_at);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int i = t * 16 + c * 8 + (lane & 3) * 2;
-            const float2 nl = *reinterpret_cast<const float2*>(stat + base + i), nd = *reinterpret_cast<const float2*>(stat + PACKED_SHORT + base + i);
-            s[c][0] = fast_exp2(fmaf(s[c][0], sl2, nl.x));
-            s[c][1] = fast_exp2(fmaf(s[c][1], sl2, nl.y));
-            s[c][2] = fast_exp2(fmaf(s[c][2], sl2, nl.x));
-            s[c][3] = fast_exp2(fmaf(s[c][3], sl2, nl.y));
-            dp[c][0] = s[c][0] * fmaf(dp[c][0], scale, nd.x);
-            dp[c][1] = s[c][1] * fmaf(dp[c][1], scale, nd.y);
-            dp[c][2] = s[c][2] * fmaf(dp[c][2], scale, nd.x);
-            dp[c][3] = s[c][3] * fmaf(dp[c][3], scale, nd.y);
-            if (t == tile || t + 1 == e.tiles) {                       // queries before the key, and behind the sequence
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const bool a0 = j0 <= i + x && i + x < n, a1 = j1 <= i + x && i + x < n;
-                s[c][x] = a0 ? s[c][x] : 0.f;
-                s[c][2 + x] = a1 ? s[c][2 + x] : 0.f;
-                dp[c][x] = a0 ? dp[c][x] : 0.f;
-                dp[c][2 + x] = a1 ? dp[c][2 + x] : 0.f;
-              }
-            }
-          }
-          uint32_t w[4];
-          short_operand(w, s);
-          short_weigh<HD>(dv, w, sdo + all + t * STEP + rows_at);
-          short_operand(w, dp);
-          short_weigh<HD>(dk, w, sq + all + t * STEP + rows_at);
-        }
-        // queries as rows: dS, for the keys up to them
-        float dq[HD / 8][4];
-#pragma unroll
-        for (int c = 0; c < HD / 8; ++c) dq[c][0] = dq[c][1] = dq[c][2] = dq[c][3] = 0.f;
-        const float nl0 = stat[base + j0], nl1 = stat[base + j1], nd0 = stat[PACKED_SHORT + base + j0], nd1 = stat[PACKED_SHORT + base + j1];
-#pragma unroll 1
-        for (int t = 0; t <= tile; ++t) {
-          float s[2][4], dp[2][4];
-          short_scores<HD>(s, sq + mine + rows_at, sk + all + t * STEP + columns_at);
-          short_scores<HD>(dp, sdo + mine + rows_at, sv + all + t * STEP + columns_at);
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              dp[c][x] = fast_exp2(fmaf(s[c][x], sl2, nl0)) * fmaf(dp[c][x], scale, nd0);
-              dp[c][2 + x] = fast_exp2(fmaf(s[c][2 + x], sl2, nl1)) * fmaf(dp[c][2 + x], scale, nd1);
-              if (t == tile) {
-                const int j = t * 16 + c * 8 + (lane & 3) * 2 + x;
-                dp[c][x] = j <= j0 ? dp[c][x] : 0.f;
-                dp[c][2 + x] = j <= j1 ? dp[c][2 + x] : 0.f;
-              }
-            }
-          uint32_t w[4];
-          short_operand(w, dp);
-          short_weigh<HD>(dq, w, sk + all + t * STEP + rows_at);
-        }
-        __syncwarp();
-        // this warp's rows of dO have other readers, and Q's too: both are done with behind the barrier
-        __syncthreads();
-        short_store<HD>(dq, 1.f, 1.f, sq + r0 * Tile::STRIDE, n - tile * 16, p.dq + row0 * p.dqs + ((e.head + u) * p.group + g) * HD, p.dqs, lane);
-      } else {
-        __syncthreads();
-      }
-      __syncthreads();                                                 // Q and dO may be written over
+  const uint32_t rows_at = Tile::rows_first(lane), columns_at = Tile::columns_first(lane), stages = smem_u32(smem);
+  const uint32_t kv_stages = stages + STAGES * 2 * Tile::BYTES;
+  float* const stats = reinterpret_cast<float*>(smem + STAGES * 4 * Tile::BYTES);
+  // query head g of every key-value head of a task, and with the first of them the keys and values
+  const auto fetch = [&](int stage, int kv_stage, const ShortTask& e, int g) {
+    const uint32_t sq = stages + stage * 2 * Tile::BYTES;
+    Tile::fetch(sq, p.qs, e.n, e.tiles, e.heads, [&](int v) { return p.q + e.lo * p.qs + ((e.head + v) * p.group + g) * HD; });
+    Tile::fetch(sq + Tile::BYTES, p.dos, e.n, e.tiles, e.heads, [&](int v) { return p.dout + e.lo * p.dos + ((e.head + v) * p.group + g) * HD; });
+    if (g == 0) {
+      const uint32_t sk = kv_stages + kv_stage * 2 * Tile::BYTES;
+      Tile::fetch(sk, p.ks, e.n, e.tiles, e.heads, [&](int v) { return p.k + e.lo * p.ks + (e.head + v) * HD; });
+      Tile::fetch(sk + Tile::BYTES, p.vs, e.n, e.tiles, e.heads, [&](int v) { return p.v + e.lo * p.vs + (e.head + v) * HD; });
     }
-    if (u < e.heads) {
-      short_store<HD>(dk, 1.f, 1.f, sk + r0 * Tile::STRIDE, n - tile * 16, p.dk + row0 * p.dks + (e.head + u) * HD, p.dks, lane);
-      short_store<HD>(dv, 1.f, 1.f, sv + r0 * Tile::STRIDE, n - tile * 16, p.dv + row0 * p.dvs + (e.head + u) * HD, p.dvs, lane);
+    const int row = threadIdx.x & (PACKED_SHORT - 1), v = e.tiles == 1 ? row >> 4 : e.tiles == 2 ? row >> 5 : 0, in = row - v * e.tiles * 16;
+    if (v < e.heads) {
+      const float* from = threadIdx.x < PACKED_SHORT ? p.lse : p.delta;
+      const long long at = (long long)((e.head + v) * p.group + g) * p.plan.tokens + e.lo;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(stats + stage * 2 * PACKED_SHORT + threadIdx.x)), "l"(from + at + (in < e.n ? in : 0)), "r"(in < e.n ? 4 : 0) : "memory");
+    }
+  };
+  ShortWalk walk(p.plan, p.kv_heads);
+  ShortTask e, then;
+  if (!walk.next(e)) return;
+  int g = 0, kv_stage = 0;
+  float dk[HD / 8][4], dv[HD / 8][4];
+  if (STAGES == 2) fetch(0, 0, e, 0);
+  short_commit();
+  for (int stage = 0;; stage ^= STAGES - 1) {
+    const bool last = g + 1 == p.group;
+    bool more = true;
+    if (last) more = walk.next(then);
+    if (STAGES == 2) {
+      if (!last) fetch(stage ^ 1, kv_stage, e, g + 1);
+      else if (more) fetch(stage ^ 1, kv_stage ^ 1, then, 0);
+      short_commit();
+      short_wait<1>();
+    } else {
+      fetch(0, 0, e, g);
+      short_commit();
+      short_wait<0>();
     }
     __syncthreads();
+    const uint32_t sq = stages + stage * 2 * Tile::BYTES, sdo = sq + Tile::BYTES, sk = kv_stages + kv_stage * 2 * Tile::BYTES, sv = sk + Tile::BYTES;
+    const float* stat = stats + stage * 2 * PACKED_SHORT;
+    const int n = e.n, u = e.tiles == 1 ? warp : e.tiles == 2 ? warp >> 1 : 0, tile = warp - u * e.tiles, base = u * e.tiles * 16, r0 = base + tile * 16;
+    const bool mine_too = u < e.heads && tile < e.tiles;
+    const long long row0 = e.lo + tile * 16;
+    float dq[HD / 8][4];
+    if (g == 0) {
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) dk[c][x] = dv[c][x] = 0.f;
+    }
+    if (mine_too) {
+      constexpr int STEP = 16 * Tile::STRIDE;
+      const uint32_t mine = r0 * Tile::STRIDE, all = base * Tile::STRIDE;
+      // keys as rows: P^T and dS^T, for the queries from them on
+      const int j0 = tile * 16 + (lane >> 2), j1 = j0 + 8;
+#pragma unroll 1
+      for (int t = tile; t < e.tiles; ++t) {
+        float s[2][4], dp[2][4];
+        short_scores<HD>(s, sk + mine + rows_at, sq + all + t * STEP + columns_at);
+        short_scores<HD>(dp, sv + mine + rows_at, sdo + all + t * STEP + columns_at);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int i = t * 16 + c * 8 + (lane & 3) * 2;
+          const float2 L = *reinterpret_cast<const float2*>(stat + base + i), D = *reinterpret_cast<const float2*>(stat + PACKED_SHORT + base + i);
+            const float2 nl = make_float2(-L.x * PS_LOG2E, -L.y * PS_LOG2E), nd = make_float2(-D.x * scale, -D.y * scale);
+          s[c][0] = fast_exp2(fmaf(s[c][0], sl2, nl.x));
+          s[c][1] = fast_exp2(fmaf(s[c][1], sl2, nl.y));
+          s[c][2] = fast_exp2(fmaf(s[c][2], sl2, nl.x));
+          s[c][3] = fast_exp2(fmaf(s[c][3], sl2, nl.y));
+          dp[c][0] = s[c][0] * fmaf(dp[c][0], scale, nd.x);
+          dp[c][1] = s[c][1] * fmaf(dp[c][1], scale, nd.y);
+          dp[c][2] = s[c][2] * fmaf(dp[c][2], scale, nd.x);
+          dp[c][3] = s[c][3] * fmaf(dp[c][3], scale, nd.y);
+          if (t == tile || t + 1 == e.tiles) {                       // queries before the key, and behind the sequence
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const bool a0 = j0 <= i + x && i + x < n, a1 = j1 <= i + x && i + x < n;
+              s[c][x] = a0 ? s[c][x] : 0.f;
+              s[c][2 + x] = a1 ? s[c][2 + x] : 0.f;
+              dp[c][x] = a0 ? dp[c][x] : 0.f;
+              dp[c][2 + x] = a1 ? dp[c][2 + x] : 0.f;
+            }
+          }
+        }
+        uint32_t w[4];
+        short_operand(w, s);
+        short_weigh<HD>(dv, w, sdo + all + t * STEP + rows_at);
+        short_operand(w, dp);
+        short_weigh<HD>(dk, w, sq + all + t * STEP + rows_at);
+      }
+      // queries as rows: dS, for the keys up to them
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) dq[c][0] = dq[c][1] = dq[c][2] = dq[c][3] = 0.f;
+      const float nl0 = -stat[base + j0] * PS_LOG2E, nl1 = -stat[base + j1] * PS_LOG2E;
+      const float nd0 = -stat[PACKED_SHORT + base + j0] * scale, nd1 = -stat[PACKED_SHORT + base + j1] * scale;
+#pragma unroll 1
+      for (int t = 0; t <= tile; ++t) {
+        float s[2][4], dp[2][4];
+        short_scores<HD>(s, sq + mine + rows_at, sk + all + t * STEP + columns_at);
+        short_scores<HD>(dp, sdo + mine + rows_at, sv + all + t * STEP + columns_at);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            dp[c][x] = fast_exp2(fmaf(s[c][x], sl2, nl0)) * fmaf(dp[c][x], scale, nd0);
+            dp[c][2 + x] = fast_exp2(fmaf(s[c][2 + x], sl2, nl1)) * fmaf(dp[c][2 + x], scale, nd1);
+            if (t == tile) {
+              const int j = t * 16 + c * 8 + (lane & 3) * 2 + x;
+              dp[c][x] = j <= j0 ? dp[c][x] : 0.f;
+              dp[c][2 + x] = j <= j1 ? dp[c][2 + x] : 0.f;
+            }
+          }
+        uint32_t w[4];
+        short_operand(w, dp);
+        short_weigh<HD>(dq, w, sk + all + t * STEP + rows_at);
+      }
+    }
+    __syncthreads();                                                   // every warp has read what it needs of these rows
+    if (mine_too) {
+      short_store<HD>(dq, 1.f, 1.f, sq + r0 * Tile::STRIDE, n - tile * 16, p.dq + row0 * p.dqs + ((e.head + u) * p.group + g) * HD, p.dqs, lane);
+      if (last) {
+        short_store<HD>(dk, 1.f, 1.f, sk + r0 * Tile::STRIDE, n - tile * 16, p.dk + row0 * p.dks + (e.head + u) * HD, p.dks, lane);
+        short_store<HD>(dv, 1.f, 1.f, sv + r0 * Tile::STRIDE, n - tile * 16, p.dv + row0 * p.dvs + (e.head + u) * HD, p.dvs, lane);
+      }
+    }
+    if (!more) break;
+    __syncthreads();                                                   // the stages may be written over
+    g = last ? 0 : g + 1;
+    if (last) {
+      e = then;
+      kv_stage ^= STAGES - 1;
+    }
   }
 }
 
@@ -350,15 +402,15 @@ static int short_launch(void (*kernel)(const P), int smem, std::atomic<unsigned 
 int packed_short_fwd(const PackedShortFwd& p, int head_dim, cudaStream_t st) {
   static std::atomic<unsigned long long> a64, a128;
   const long long most = (long long)p.plan.batch * p.q_heads;
-  return head_dim == 64 ? short_launch(packed_short_fwd_kernel<64>, 3 * ShortTile<64>::BYTES, a64, 5, most, p, st)
-                        : short_launch(packed_short_fwd_kernel<128>, 3 * ShortTile<128>::BYTES, a128, 2, most, p, st);
+  return head_dim == 64 ? short_launch(packed_short_fwd_kernel<64>, 6 * ShortTile<64>::BYTES, a64, 4, most, p, st)
+                        : short_launch(packed_short_fwd_kernel<128>, 6 * ShortTile<128>::BYTES, a128, 2, most, p, st);
 }
 
 int packed_short_bwd(const PackedShortBwd& p, int head_dim, cudaStream_t st) {
   static std::atomic<unsigned long long> a64, a128;
   const long long most = (long long)p.plan.batch * p.kv_heads;
-  return head_dim == 64 ? short_launch(packed_short_bwd_kernel<64>, 4 * ShortTile<64>::BYTES + 512, a64, 3, most, p, st)
-                        : short_launch(packed_short_bwd_kernel<128>, 4 * ShortTile<128>::BYTES + 512, a128, 2, most, p, st);
+  return head_dim == 64 ? short_launch(packed_short_bwd_kernel<64>, PS_BWD_BYTES<64>, a64, 3, most, p, st)
+                        : short_launch(packed_short_bwd_kernel<128>, PS_BWD_BYTES<128>, a128, 2, most, p, st);
 }
 
 }  // namespace oa

@@ -291,18 +291,21 @@ def test_plan_lists():
         tokens, batch = sum(lengths) + 9, len(lengths)
         p = P.plan(_starts(lengths, "cuda", 2), tokens)
         w = p.words.cpu()
-        n, m, briefs = w[0].item(), w[1].item(), w[4].item()
+        n, m, classes = w[0].item(), w[1].item(), w[4:7].tolist()
         first = (8 + batch + 1 + 3) // 4 * 4
         starts = p.starts.cpu().tolist()
         most, pairs = tokens // 128 + batch, tokens // 256 + batch
         exact = tokens // 128 < 1024                               # beyond that, bins hold several indices
-        lists = [w[at:at + 4 * count].reshape(-1, 4).tolist() for count, at in ((n, first), (m, first + 4 * most), (briefs, first + 4 * (most + pairs)))]
+        lists = [w[at:at + 4 * count].reshape(-1, 4).tolist() for count, at in ((n, first), (m, first + 4 * most), (sum(classes), first + 4 * (most + pairs)))]
         long = [(a, b, s) for s, (a, b) in enumerate(zip(starts, starts[1:])) if b - a > 64]
         for got, rows in zip(lists, (128, 256)):
             assert sorted(map(tuple, got)) == sorted((a, b, i, s) for a, b, s in long for i in range(-(-(b - a) // rows)))
             order = [x[2] for x in got]
             step = 1 if exact else 1 << (tokens // 128 // 1024).bit_length()
             assert all(a // step >= b // step for a, b in zip(order, order[1:]))
+        ends = [b - a for a, b, _, _ in lists[2]]
+        assert classes == [sum(a < e <= b for e in ends) for a, b in ((32, 64), (16, 32), (0, 16))]
+        assert all((-(-a // 16) + 1) // 2 >= (-(-b // 16) + 1) // 2 for a, b in zip(ends, ends[1:]) if a <= 32 or b <= 32)
         assert sorted(map(tuple, lists[2])) == [(a, b, 0, s) for s, (a, b) in enumerate(zip(starts, starts[1:])) if 0 < b - a <= 64]
 
 

@@ -33,12 +33,17 @@ struct ShortTile {
     constexpr int ROWS = PS_THREADS / CHUNKS;
     const int r0 = threadIdx.x / CHUNKS, c = threadIdx.x % CHUNKS;
     uint32_t to = base + r0 * STRIDE + ((c ^ (r0 & 7)) << 4);
+    const long long at = r0 * stride + c * 8;
     for (int u = 0; u < heads; ++u) {
-      const __nv_bfloat16* head = first(u) + c * 8;
-      const __nv_bfloat16* src = head + r0 * stride;
-#pragma unroll 2
-      for (int row = r0; row < tiles * 16; row += ROWS, to += ROWS * STRIDE, src += ROWS * stride)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(row < n ? src : head), "r"(row < n ? 16 : 0) : "memory");
+      const __nv_bfloat16* src = first(u) + at;
+#pragma unroll
+      for (int row = 0; row < PACKED_SHORT; row += ROWS) {
+        if (row >= tiles * 16) break;
+        // a row that is not there is not read: zeros
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(row + r0 < n ? src : first(u)), "r"(row + r0 < n ? 16 : 0) : "memory");
+        to += ROWS * STRIDE;
+        src += ROWS * stride;
+      }
     }
   }
 };
@@ -122,21 +127,25 @@ struct ShortTask {
 struct ShortWalk {
   const PackedPlan& plan;
   const int all_heads, n0, n1, n2, end0, end1, end;
-  int task;
-  int4 ahead;                              // the next task's entry, on its way
+  int task, set, sets;
+  int4 ahead;                              // the next task's entry, on its way; its set of heads, and how many there are to a set
   __device__ __forceinline__ ShortWalk(const PackedPlan& p, int heads)
       : plan(p), all_heads(heads), n0(p.words[4]), n1(p.words[5]), n2(p.words[6]), end0(n0 * heads), end1(end0 + n1 * ((heads + 1) >> 1)),
         end(end1 + n2 * ((heads + 3) >> 2)), task(blockIdx.x) { fetch(); }
   __device__ __forceinline__ void fetch() {
-    if (task < end) ahead = plan.brief(task < end0 ? task % n0 : task < end1 ? n0 + (task - end0) % n1 : n0 + n1 + (task - end1) % n2);
+    if (task >= end) return;
+    const int from = task < end0 ? 0 : task < end1 ? end0 : end1, n = task < end0 ? n0 : task < end1 ? n1 : n2;
+    set = (int)((unsigned)(task - from) / (unsigned)n);
+    ahead = plan.brief((task < end0 ? 0 : task < end1 ? n0 : n0 + n1) + task - from - set * n);
+    sets = task < end0 ? 1 : task < end1 ? 2 : 4;
   }
   __device__ __forceinline__ bool next(ShortTask& e) {
     if (task >= end) return false;
     e.lo = ahead.x;
     e.n = ahead.y - ahead.x;
     e.tiles = (e.n + 15) >> 4;
-    e.head = task < end0 ? task / n0 : task < end1 ? (task - end0) / n1 * 2 : (task - end1) / n2 * 4;
-    e.heads = min(task < end0 ? 1 : task < end1 ? 2 : 4, all_heads - e.head);
+    e.head = set * sets;
+    e.heads = min(sets, all_heads - e.head);
     task += gridDim.x;
     fetch();
     return true;
@@ -153,9 +162,12 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 4 : 2) packed_short_fwd
   const float sl2 = p.scale * PS_LOG2E;
   const uint32_t rows_at = Tile::rows_first(lane), columns_at = Tile::columns_first(lane), stages = smem_u32(smem);
   const auto fetch = [&](uint32_t to, const ShortTask& e) {
-    Tile::fetch(to, p.qs, e.n, e.tiles, e.heads, [&](int u) { return p.q + e.lo * p.qs + (e.head + u) * HD; });
-    Tile::fetch(to + Tile::BYTES, p.ks, e.n, e.tiles, e.heads, [&](int u) { return p.k + e.lo * p.ks + (e.head + u) / p.group * HD; });
-    Tile::fetch(to + 2 * Tile::BYTES, p.vs, e.n, e.tiles, e.heads, [&](int u) { return p.v + e.lo * p.vs + (e.head + u) / p.group * HD; });
+    const __nv_bfloat16* q = p.q + e.lo * p.qs + e.head * HD;
+    Tile::fetch(to, p.qs, e.n, e.tiles, e.heads, [&](int u) { return q + u * HD; });
+    const auto kv = [&](int u) { return (p.group == 1 ? e.head + u : (int)((unsigned)(e.head + u) / (unsigned)p.group)) * HD; };
+    const __nv_bfloat16 *k = p.k + e.lo * p.ks, *v = p.v + e.lo * p.vs;
+    Tile::fetch(to + Tile::BYTES, p.ks, e.n, e.tiles, e.heads, [&](int u) { return k + kv(u); });
+    Tile::fetch(to + 2 * Tile::BYTES, p.vs, e.n, e.tiles, e.heads, [&](int u) { return v + kv(u); });
   };
   ShortWalk walk(p.plan, p.q_heads);
   ShortTask e, then;
@@ -257,12 +269,15 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
   // query head g of every key-value head of a task, and with the first of them the keys and values
   const auto fetch = [&](int stage, int kv_stage, const ShortTask& e, int g) {
     const uint32_t sq = stages + stage * 2 * Tile::BYTES;
-    Tile::fetch(sq, p.qs, e.n, e.tiles, e.heads, [&](int v) { return p.q + e.lo * p.qs + ((e.head + v) * p.group + g) * HD; });
-    Tile::fetch(sq + Tile::BYTES, p.dos, e.n, e.tiles, e.heads, [&](int v) { return p.dout + e.lo * p.dos + ((e.head + v) * p.group + g) * HD; });
+    const int col = (e.head * p.group + g) * HD, apart = p.group * HD;
+    const __nv_bfloat16 *q = p.q + e.lo * p.qs + col, *dout = p.dout + e.lo * p.dos + col;
+    Tile::fetch(sq, p.qs, e.n, e.tiles, e.heads, [&](int u) { return q + u * apart; });
+    Tile::fetch(sq + Tile::BYTES, p.dos, e.n, e.tiles, e.heads, [&](int u) { return dout + u * apart; });
     if (g == 0) {
       const uint32_t sk = kv_stages + kv_stage * 2 * Tile::BYTES;
-      Tile::fetch(sk, p.ks, e.n, e.tiles, e.heads, [&](int v) { return p.k + e.lo * p.ks + (e.head + v) * HD; });
-      Tile::fetch(sk + Tile::BYTES, p.vs, e.n, e.tiles, e.heads, [&](int v) { return p.v + e.lo * p.vs + (e.head + v) * HD; });
+      const __nv_bfloat16 *k = p.k + e.lo * p.ks + e.head * HD, *v = p.v + e.lo * p.vs + e.head * HD;
+      Tile::fetch(sk, p.ks, e.n, e.tiles, e.heads, [&](int u) { return k + u * HD; });
+      Tile::fetch(sk + Tile::BYTES, p.vs, e.n, e.tiles, e.heads, [&](int u) { return v + u * HD; });
     }
     const int row = threadIdx.x & (PACKED_SHORT - 1), v = e.tiles == 1 ? row >> 4 : e.tiles == 2 ? row >> 5 : 0, in = row - v * e.tiles * 16;
     if (v < e.heads) {

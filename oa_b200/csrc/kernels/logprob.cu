@@ -213,6 +213,7 @@ __device__ __forceinline__ void lp_top(S& s, const LpRow<T>& row, int p0, int p1
     for (int i = tid; i < hots * steps; i += THREADS) {
       const int h = i / steps, p = p0 + s.hot[h] + (i - h * steps) * THREADS;
       if (p >= p1) continue;
+      if (*static_cast<volatile int*>(&s.count) > S::LIST) break;          // too many already (a share that is masked as a whole, say)
       LpPiece<T> v;
       row.load(v, p);
       const int e = row.first(p);

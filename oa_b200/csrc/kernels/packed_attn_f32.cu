@@ -180,27 +180,44 @@ __device__ __forceinline__ void packed_f32_bwd_kv(float* sQ, float* sDO, const P
   }
   const int istart = t.i0 / AF_TILE * AF_TILE;               // first query tile that any key of this block is seen by
   for (int h = hk * p.group; h < (hk + 1) * p.group; ++h) {
-    // delta and log-sum-exp of the 32 queries of a tile: four threads to a query.  Tiles alternate between two slots, so that those of the next
-    // tile can be written while the last warps still read this one's.
-    const auto stats = [&](int i0, int slot) {
-      const int r = threadIdx.x >> 2, part = threadIdx.x & 3;
-      float dl = 0.f;
+    // delta and log-sum-exp of the 32 queries of a tile: four threads to a query.  Fetched before a tile is worked on, those of the next one are written behind
+    // it, to the other of two slots: the last warps may still read this one's.
+    const int r = threadIdx.x >> 2, part = threadIdx.x & 3;
+    float delta = 0.f, lse = INFINITY;
+    const auto fetch = [&](int i0) {
+      delta = 0.f;
+      lse = INFINITY;
       if (i0 + r < t.n) {
         const float *pd = p.dout + (t.lo + i0 + r) * p.dos + h * hd, *po = p.o + (t.lo + i0 + r) * p.os + h * hd;
-        for (int d = part; d < hd; d += 4) dl = fmaf(pd[d], po[d], dl);
+        lse = p.lse[(long long)h * p.plan.tokens + t.lo + i0 + r];
+        if (p.vec) {
+#pragma unroll
+          for (int d = part * 4; d < DS * AF_W; d += 16)
+            if (d < hd) {
+              const float4 a = *reinterpret_cast<const float4*>(pd + d), c = *reinterpret_cast<const float4*>(po + d);
+              delta = fmaf(a.x, c.x, fmaf(a.y, c.y, fmaf(a.z, c.z, fmaf(a.w, c.w, delta))));
+            }
+        } else {
+          for (int d = part * 4; d < hd; d += 16)              // in the same order
+            for (int u = 3; u >= 0; --u)
+              if (d + u < hd) delta = fmaf(pd[d + u], po[d + u], delta);
+        }
       }
-      dl += __shfl_xor_sync(0xffffffffu, dl, 1);
-      dl += __shfl_xor_sync(0xffffffffu, dl, 2);
+    };
+    const auto keep = [&](int slot) {
+      delta += __shfl_xor_sync(0xffffffffu, delta, 1);
+      delta += __shfl_xor_sync(0xffffffffu, delta, 2);
       if (part == 0) {
-        sDelta[slot][r] = dl;
-        sL[slot][r] = i0 + r < t.n ? p.lse[(long long)h * p.plan.tokens + t.lo + i0 + r] : INFINITY;
+        sDelta[slot][r] = delta;
+        sL[slot][r] = lse;
       }
     };
     int slot = 0;
     __syncthreads();                                          // the last head's last tile has been read
-    stats(istart, 0);
+    fetch(istart);
+    keep(0);
     af_stream<DS, KS>(sQ, sDO, p.q, p.qs, p.dout, p.dos, t.lo, istart, t.n, t.n, h * hd, hd, p.vec, [&](int i0, const float* tq, const float* td) {
-      if (i0 + AF_TILE < t.n) stats(i0 + AF_TILE, slot ^ 1);
+      fetch(i0 + AF_TILE);
 #pragma unroll 4
       for (int jj = 0; jj < NI; ++jj) {
         const int ii = jj * KS + ks;
@@ -215,6 +232,7 @@ __device__ __forceinline__ void packed_f32_bwd_kv(float* sQ, float* sDO, const P
         af_axpy(accv, e, dorow);
         af_axpy(acck, ds, qrow);
       }
+      keep(slot ^ 1);
       slot ^= 1;
     });
   }

@@ -5,6 +5,7 @@ states the mathematics; CPU tensors the plain statement of it.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple, Optional
 
@@ -12,7 +13,7 @@ import torch
 
 from .. import _native as N
 from . import kernels as K
-from .packed import _together
+from .packed import _copied, _overlap, _step, _stream, _together
 
 MAX_TOP = 32
 
@@ -25,21 +26,21 @@ class TokenLogProbs(NamedTuple):
     top_ids: torch.Tensor           # [rows, top] int32, the likeliest first
 
 
-def _check(what: str, logits: torch.Tensor, targets: torch.Tensor, scale: float) -> None:
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or not 1 <= logits.shape[1] < 1 << 31 or logits.shape[0] >= 1 << 31:
+@functools.lru_cache(maxsize=256)
+def _layout(what, shape, stride, dtype, t_shape, t_stride, t_dtype, scale, top, ignore_index):
+    """The checks that shapes and types allow; elements between the rows of logits, None where they are copied."""
+    if len(shape) != 2 or dtype not in (torch.float32, torch.bfloat16) or not 1 <= shape[1] < 1 << 30 or shape[0] >= 1 << 30:
         raise ValueError(f"{what}: logits must be float32 or bfloat16 [rows, vocab]")
-    if targets.dtype is not torch.int32 or targets.shape != logits.shape[:1] or not targets.is_contiguous():
-        raise ValueError(f"{what}: targets must be a contiguous int32 tensor [{logits.shape[0]}]")
+    rows, vocab = shape
+    if t_dtype is not torch.int32 or t_shape != (rows,) or (rows > 1 and t_stride != (1,)):
+        raise ValueError(f"{what}: targets must be a contiguous int32 tensor [{rows}]")
     if not 0 < scale < math.inf:
         raise ValueError(f"{what}: scale must be positive, not {scale}")
-
-
-def _readable(logits: torch.Tensor):
-    step, unit = logits.stride()
-    rows, vocab = logits.shape
-    if unit != 1 and vocab > 1:
-        return K.contiguous(logits), vocab
-    return logits, step if rows > 1 else vocab
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"{what}: 0 to {min(MAX_TOP, vocab)} alternatives, not {top}")
+    if not -2 ** 31 <= ignore_index < 2 ** 31:
+        raise ValueError(f"{what}: ignore_index is one of the targets' 32 bits, not {ignore_index}")
+    return None if stride[1] != 1 and vocab > 1 else vocab if rows <= 1 else stride[0]
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0, scale: float = 1.0, ignore_index: int = -100) -> TokenLogProbs:
@@ -47,20 +48,20 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0, sc
     the `top` likeliest tokens (at most 32) with theirs; equal logits rank by index.  A target of ignore_index has log-probability 0, any other that is
     no token NaN.  Logits of -inf have probability 0; a row with NaN or +inf is NaN; one without anything above -inf has log-probabilities of
     -inf and entropy 0."""
-    _check("token_logprobs", logits, targets, scale)
-    rows, vocab = logits.shape
-    if not 0 <= top <= min(MAX_TOP, vocab):
-        raise ValueError(f"token_logprobs: 0 to {min(MAX_TOP, vocab)} alternatives, not {top}")
-    _together("token_logprobs", logits, targets)
-    if not logits.is_cuda:
+    step = _layout("token_logprobs", logits.shape, logits.stride(), logits.dtype, targets.shape, targets.stride(), targets.dtype, scale, top, ignore_index)
+    device = _together("token_logprobs", logits, targets)
+    if device < 0:
         return _cpu(logits, targets, top, scale, ignore_index)
-    f32 = dict(dtype=torch.float32, device=logits.device)
-    out = TokenLogProbs(torch.empty(rows, **f32), torch.empty(rows, **f32), torch.empty((rows, 2), **f32), torch.empty((rows, top), **f32),
-                        torch.empty((rows, top), dtype=torch.int32, device=logits.device))
-    logits, step = _readable(logits)
-    K._launch(N.require().oa_token_logprobs(K.dt(logits), logits.data_ptr(), step, targets.data_ptr(), *(t.data_ptr() for t in out), top, rows, vocab,
-                                            float(scale), ignore_index, N.stream()), "oa_token_logprobs", outputs=(out.logprobs, out.entropy))
-    return out
+    rows, vocab = logits.shape
+    if step is None:
+        logits, step = _copied(logits), vocab
+    f32 = torch.empty(rows * (4 + 2 * top), dtype=torch.float32, device=logits.device)
+    logprobs, entropy, stats, top_logprobs, top_ids = torch.unsafe_split_with_sizes(f32, (rows, rows, 2 * rows, top * rows, top * rows))
+    at = f32.data_ptr()
+    K._launch(N.require().oa_token_logprobs(K.dt(logits), logits.data_ptr(), step, targets.data_ptr(), at, at + 4 * rows, at + 8 * rows, at + 16 * rows,
+                                            at + 4 * (4 + top) * rows, top, rows, vocab, scale, ignore_index, _stream(device)),
+              "oa_token_logprobs", outputs=(logprobs, entropy))
+    return TokenLogProbs(logprobs, entropy, stats.view(rows, 2), top_logprobs.view(rows, top), top_ids.view(torch.int32).view(rows, top))
 
 
 def _cpu(logits, targets, top, scale, ignore_index):
@@ -89,24 +90,29 @@ def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, result:
     """The logits' gradient from those of the log-probabilities and of the entropy ([rows] fp32, or None for none), given what `token_logprobs` returned
     for the same logits, targets, scale and ignore_index.  `out` (row stride allowed) may be the logits themselves.  A row whose target is ignore_index
     takes no part in dlogprobs; one with another target that is no token is NaN; one without anything above -inf is 0."""
-    _check("token_logprobs_backward", logits, targets, scale)
+    step = _layout("token_logprobs_backward", logits.shape, logits.stride(), logits.dtype, targets.shape, targets.stride(), targets.dtype, scale, 0, ignore_index)
     rows, vocab = logits.shape
     for name, t, shape in (("dlogprobs", dlogprobs, (rows,)), ("dentropy", dentropy, (rows,)), ("result.entropy", result.entropy, (rows,)),
                            ("result.stats", result.stats, (rows, 2))):
         if t is not None and (t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous()):
             raise ValueError(f"token_logprobs_backward: {name} must be a contiguous float32 tensor {list(shape)}")
+    device = _together("token_logprobs_backward", logits, targets, result.entropy, result.stats, *(t for t in (dlogprobs, dentropy, out) if t is not None))
     if out is None:
         out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
-    elif out.shape != logits.shape or out.dtype is not logits.dtype or (vocab > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < vocab):
-        raise ValueError(f"token_logprobs_backward: out must be {logits.dtype} {list(logits.shape)}, the elements of a row side by side, rows apart")
-    _together("token_logprobs_backward", logits, targets, out, *(t for t in (dlogprobs, dentropy, result.entropy, result.stats) if t is not None))
-    if not logits.is_cuda:
+        to = vocab
+    else:
+        to = _step(out.shape, out.stride()) if out.dim() == 2 else None
+        if out.shape != logits.shape or out.dtype is not logits.dtype or to is None:
+            raise ValueError(f"token_logprobs_backward: out must be {logits.dtype} {list(logits.shape)}, the elements of a row side by side, rows apart")
+        if (out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride()) and _overlap(out, logits):
+            raise ValueError("token_logprobs_backward: out must be the logits or lie apart from them")
+    if device < 0:
         return _backward_cpu(logits, targets, result, dlogprobs, dentropy, scale, ignore_index, out)
-    logits, step = _readable(logits)
+    if step is None:
+        logits, step = _copied(logits), vocab
     K._launch(N.require().oa_token_logprobs_bwd(K.dt(logits), logits.data_ptr(), step, targets.data_ptr(), result.entropy.data_ptr(),
-                                                result.stats.data_ptr(), N.ptr(dlogprobs), N.ptr(dentropy), out.data_ptr(),
-                                                out.stride(0) if rows > 1 else vocab, rows, vocab, float(scale), ignore_index, N.stream()),
-              "oa_token_logprobs_bwd", outputs=(out,))
+                                                result.stats.data_ptr(), N.ptr(dlogprobs), N.ptr(dentropy), out.data_ptr(), to, rows, vocab, scale, ignore_index,
+                                                _stream(device)), "oa_token_logprobs_bwd", outputs=(out,))
     return out
 
 

@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -36,33 +37,51 @@ class PackedPlan(NamedTuple):
     batch: int
 
 
-def _current(what: str, t: torch.Tensor) -> None:
-    if t.is_cuda and t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{what}: tensors on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
-
-
-def _together(what: str, first: torch.Tensor, *tensors: torch.Tensor) -> None:
+def _together(what: str, first: torch.Tensor, *tensors: torch.Tensor) -> int:
+    """The device that all tensors are on (-1: the CPU); a CUDA one has to be the current one, whose stream the kernels go to."""
     at = first.get_device()
     for t in tensors:
         if t.get_device() != at:
             raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
-    _current(what, first)
+    if at >= 0 and at != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensors on {first.device}, but the current device is cuda:{torch.cuda.current_device()}")
+    return at
 
 
-def _rows(t: torch.Tensor, aligned: bool):
-    """(the rows as the kernels read them, elements between rows): elements side by side and, if `aligned`, every row on 16 bytes.  A copy where they
-    are not."""
-    rows, cols = t.shape
-    step, unit = t.stride()
-    if rows <= 1:
-        step = cols                                  # the stride of a single row says nothing
-        if aligned:
-            step += -step % 8
-    if (unit == 1 or cols <= 1) and step >= cols and (not aligned or (step * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0)):
-        return t, step
-    if aligned and cols * t.element_size() % 16:     # rows of whole heads never are
-        raise ValueError(f"packed: rows of {cols} elements do not fill 16-byte pieces")
-    return (t.clone(memory_format=torch.contiguous_format) if t.is_contiguous() else K.contiguous(t)), cols
+def _stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _step(shape, stride) -> Optional[int]:
+    """Elements between the rows of a matrix whose rows have their elements side by side and do not overlap; None otherwise."""
+    rows, cols = shape
+    if cols > 1 and stride[1] != 1:
+        return None
+    return cols if rows <= 1 else stride[0] if stride[0] >= cols else None      # the stride of a single row says nothing
+
+
+def _copied(t: torch.Tensor) -> torch.Tensor:
+    return t.clone(memory_format=torch.contiguous_format) if t.is_contiguous() else K.contiguous(t)
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices share memory (columns of one buffer that lie beside one another do not)."""
+    if not a.numel() or not b.numel():
+        return False
+    size = a.element_size()
+    (lo, hi), (lo2, hi2) = ((t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + (t.shape[1] - 1) * t.stride(1) + 1) * t.element_size()) for t in (a, b))
+    if hi <= lo2 or hi2 <= lo:
+        return False
+    pitch = a.stride(0) * size
+    if a.stride(1) == b.stride(1) == 1 and b.stride(0) * b.element_size() == pitch > 0:
+        at = (lo2 - lo) % pitch
+        return at < a.shape[1] * size or at + b.shape[1] * b.element_size() > pitch
+    return True
+
+
+def _apart(what: str, out: torch.Tensor, *tensors: torch.Tensor) -> None:
+    if any(_overlap(out, t) for t in tensors):
+        raise ValueError(f"{what}: the result's memory is that of an operand")
 
 
 def plan(starts: torch.Tensor, tokens: int) -> PackedPlan:
@@ -75,9 +94,9 @@ def plan(starts: torch.Tensor, tokens: int) -> PackedPlan:
         raise ValueError(f"plan: {batch} sequences in {tokens} rows; at most {1 << 24} in {1 << 30}")
     if not starts.is_cuda:
         return PackedPlan(torch.cummax(starts.clamp(0, tokens), 0).values, None, tokens, batch)
-    _current("plan", starts)
+    device = _together("plan", starts)
     words = torch.empty(N.require().oa_packed_plan_bytes(tokens, batch) // 4, dtype=torch.int32, device=starts.device)
-    K._launch(N.require().oa_packed_plan(starts.data_ptr(), words.data_ptr(), batch, tokens, N.stream()), "oa_packed_plan")
+    K._launch(N.require().oa_packed_plan(starts.data_ptr(), words.data_ptr(), batch, tokens, _stream(device)), "oa_packed_plan")
     return PackedPlan(words[8:8 + batch + 1], words, tokens, batch)
 
 
@@ -92,32 +111,25 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, pair_axes: Sequence[int], h
     """The first `heads` heads of every row of x [tokens, >= heads * head_dim] (row stride allowed) turned by their token's positions [axes, tokens]
     (int32): pair j of a head, dimensions j and j + len(pair_axes), by theta^(-j / len(pair_axes)) times the position on axis pair_axes[j].  Dimensions from
     2 len(pair_axes) on stay as they are.  One axis and half the head's dimensions make the usual rotary embedding.  `backward`: the other way round,
-    which is the gradient.  Returns [tokens, heads * head_dim], `out` if given, which may be x itself or its first columns."""
-    pair_axes = tuple(int(a) for a in pair_axes)
-    if x.dim() != 2 or heads < 1 or head_dim < 2 or x.shape[1] < heads * head_dim or x.dtype not in _FLOATS:
-        raise ValueError(f"rotary: x must be float32 or bfloat16 [tokens, >= {heads} * {head_dim}]")
+    which is the gradient.  Returns [tokens, heads * head_dim], the first columns of `out` if given, which may be x itself but not overlap it otherwise."""
+    if type(pair_axes) is not tuple:
+        pair_axes = tuple(pair_axes)
+    step, axes, turns = _rotary_layout(x.shape, x.stride(), x.dtype, positions.shape, positions.stride(), positions.dtype, pair_axes, heads, head_dim, theta)
     tokens, cols = x.shape[0], heads * head_dim
-    if not 1 <= len(pair_axes) <= min(head_dim // 2, MAX_PAIRS):
-        raise ValueError(f"rotary: 1 to {min(head_dim // 2, MAX_PAIRS)} pairs of a head of {head_dim}, not {len(pair_axes)}")
-    if positions.dtype is not torch.int32 or positions.dim() != 2 or not positions.is_contiguous() or positions.shape[1] != tokens \
-            or not 1 <= positions.shape[0] <= MAX_AXES:
-        raise ValueError(f"rotary: positions must be a contiguous int32 tensor [axes, {tokens}] of at most {MAX_AXES} axes")
-    if min(pair_axes) < 0 or max(pair_axes) >= positions.shape[0]:
-        raise ValueError(f"rotary: pair_axes names axes that positions [{positions.shape[0]}, tokens] do not have")
-    if not 0 < theta < math.inf:
-        raise ValueError(f"rotary: theta must be positive, not {theta}")
-    _together("rotary", x, positions)
     if out is None:
-        out = x.new_empty((tokens, cols))
+        device = _together("rotary", x, positions)
+        out, to = x.new_empty((tokens, cols)), cols
     else:
+        device = _together("rotary", x, positions, out)
         if out.dim() != 2 or out.shape[0] != tokens or out.shape[1] < cols or out.dtype is not x.dtype:
             raise ValueError(f"rotary: out must be {x.dtype} [{tokens}, >= {cols}]")
-        if (out.shape[1] > 1 and out.stride(1) != 1) or (tokens > 1 and out.stride(0) < cols):
-            raise ValueError("rotary: out must have the elements of a row side by side and rows that do not overlap")
-        _together("rotary", x, out)
         out = out[:, :cols]
-    axes, turns = _rotary_tables(pair_axes, float(theta))
-    if not x.is_cuda:
+        to = _step(out.shape, out.stride())
+        if to is None:
+            raise ValueError("rotary: out must have the elements of a row side by side and rows that do not overlap")
+        if x.data_ptr() != out.data_ptr() or (tokens > 1 and x.stride() != out.stride()):
+            _apart("rotary", out, x[:, :cols])
+    if device < 0:
         half = len(pair_axes)
         a = positions.double()[list(pair_axes)].t() * torch.tensor(list(turns), dtype=torch.float64) * (2 * math.pi)
         cos, sin = a.cos().float()[:, None], a.sin().float()[:, None]
@@ -126,36 +138,66 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, pair_axes: Sequence[int], h
         lo, hi = v[..., :half], v[..., half:2 * half]
         out.copy_(torch.cat([lo * cos - hi * sin, hi * cos + lo * sin, v[..., 2 * half:]], -1).reshape(tokens, cols))
         return out
-    x = x[:, :cols]
-    x, step = _rows(x, False)
-    K._launch(N.require().oa_rotary_axes(K.dt(x), x.data_ptr(), step, out.data_ptr(), out.stride(0) if tokens > 1 else cols, positions.data_ptr(),
-                                         ctypes.addressof(axes), ctypes.addressof(turns), len(pair_axes), tokens, heads, head_dim, int(backward),
-                                         N.stream()), "oa_rotary_axes", outputs=(out,))
+    if step is None:
+        x = _copied(x[:, :cols])
+        step = cols
+    K._launch(N.require().oa_rotary_axes(K.dt(x), x.data_ptr(), step, out.data_ptr(), to, positions.data_ptr(), ctypes.addressof(axes), ctypes.addressof(turns),
+                                         len(pair_axes), tokens, heads, head_dim, int(backward), _stream(device)), "oa_rotary_axes", outputs=(out,))
     return out
 
 
-def _heads(what: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPlan, head_dim: int):
-    """The checks of both directions: (query heads, key-value heads)."""
-    if q.dtype not in _FLOATS or k.dtype is not q.dtype or v.dtype is not q.dtype or q.dim() != 2 or k.dim() != 2 or v.shape != k.shape:
+# What follows from shapes, strides and types alone is worked out once for each of them: the checks took longer than a small launch.
+@functools.lru_cache(maxsize=256)
+def _rotary_layout(shape, stride, dtype, p_shape, p_stride, p_dtype, pair_axes, heads, head_dim, theta):
+    """The checks of `rotary`; (elements between the rows of x or None where they are copied, the axes and turns of the pairs)."""
+    if len(shape) != 2 or heads < 1 or head_dim < 2 or shape[1] < heads * head_dim or dtype not in _FLOATS:
+        raise ValueError(f"rotary: x must be float32 or bfloat16 [tokens, >= {heads} * {head_dim}]")
+    if not 1 <= len(pair_axes) <= min(head_dim // 2, MAX_PAIRS):
+        raise ValueError(f"rotary: 1 to {min(head_dim // 2, MAX_PAIRS)} pairs of a head of {head_dim}, not {len(pair_axes)}")
+    if p_dtype is not torch.int32 or len(p_shape) != 2 or p_shape[1] != shape[0] or not 1 <= p_shape[0] <= MAX_AXES \
+            or (p_shape[1] > 1 and p_stride[1] != 1) or (p_shape[0] > 1 and 0 < p_shape[1] != p_stride[0]):
+        raise ValueError(f"rotary: positions must be a contiguous int32 tensor [axes, {shape[0]}] of at most {MAX_AXES} axes")
+    if not all(0 <= operator.index(a) < p_shape[0] for a in pair_axes):
+        raise ValueError(f"rotary: pair_axes names axes that positions [{p_shape[0]}, tokens] do not have")
+    if not 0 < theta < math.inf:
+        raise ValueError(f"rotary: theta must be positive, not {theta}")
+    if shape[0] > 1 << 30 or heads * head_dim > 1 << 30:
+        raise ValueError(f"rotary: {list(shape)} is too large")
+    step = shape[1] if shape[0] <= 1 else stride[0]
+    return (step if stride[1] == 1 else None, *_rotary_tables(pair_axes, float(theta)))
+
+
+@functools.lru_cache(maxsize=256)
+def _layout(what, q_shape, q_stride, k_shape, k_stride, v_shape, v_stride, q_dtype, k_dtype, v_dtype, tokens, head_dim, scale, cuda):
+    """The checks of both directions; (query heads, key-value heads, scale, elements between the rows of q, of k, of v, or None where they are copied)."""
+    if q_dtype not in _FLOATS or k_dtype is not q_dtype or v_dtype is not q_dtype or len(q_shape) != 2 or len(k_shape) != 2 or v_shape != k_shape:
         raise ValueError(f"{what}: q, k and v must be float32 or bfloat16 matrices of one type, k and v of one shape")
-    if head_dim < 1 or q.shape[1] < 1 or k.shape[1] < 1 or k.shape[1] % head_dim or q.shape[1] % k.shape[1]:
-        raise ValueError(f"{what}: rows of heads of {head_dim}, the query heads a multiple of the key-value heads; not {q.shape[1]} and {k.shape[1]} columns")
-    if q.shape[0] != plan.tokens or k.shape[0] != plan.tokens:
-        raise ValueError(f"{what}: the plan is for {plan.tokens} rows, not {q.shape[0]} and {k.shape[0]}")
-    _together(what, q, k, v, plan.starts)
-    if q.is_cuda:
-        if q.dtype is torch.bfloat16 and head_dim not in HEAD_DIMS:
+    if head_dim < 1 or q_shape[1] < 1 or k_shape[1] < 1 or k_shape[1] % head_dim or q_shape[1] % k_shape[1]:
+        raise ValueError(f"{what}: rows of heads of {head_dim}, the query heads a multiple of the key-value heads; not {q_shape[1]} and {k_shape[1]} columns")
+    if q_shape[0] != tokens or k_shape[0] != tokens:
+        raise ValueError(f"{what}: the plan is for {tokens} rows, not {q_shape[0]} and {k_shape[0]}")
+    half = q_dtype is torch.bfloat16
+    if cuda:
+        if half and head_dim not in HEAD_DIMS:
             raise ValueError(f"{what}: bfloat16 heads of one of {HEAD_DIMS}, not of {head_dim}")
         if head_dim > 128:
             raise ValueError(f"{what}: heads of at most 128, not of {head_dim}")
-    return q.shape[1] // head_dim, k.shape[1] // head_dim
-
-
-def _scale(what: str, scale: Optional[float], head_dim: int) -> float:
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
     if not 0 < scale < math.inf:
         raise ValueError(f"{what}: scale must be positive, not {scale}")
-    return scale
+    steps = [_kernel_step(*m, half) for m in ((q_shape, q_stride), (k_shape, k_stride), (v_shape, v_stride))]
+    return (q_shape[1] // head_dim, k_shape[1] // head_dim, scale, *steps)
+
+
+def _kernel_step(shape, stride, half: bool) -> Optional[int]:
+    """As _step; the bf16 kernels also want rows 16 bytes apart."""
+    step = _step(shape, stride)
+    return None if step is not None and half and step % 8 else step
+
+
+def _operands(half: bool, *pairs):
+    """[tensor, elements between rows] of each (tensor, step), copied where the kernels cannot read it as it lies."""
+    return [(t, s) if s is not None and not (half and t.data_ptr() & 15) else (_copied(t), t.shape[1]) for t, s in pairs]
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPlan, head_dim: int, scale: Optional[float] = None, return_lse: bool = False):
@@ -165,21 +207,24 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPla
 
     bf16 (heads of 64 or 128) runs on the tensor cores: weights are rounded to bf16 before they meet the values, sums are fp32.  A value that is not finite
     may reach earlier tokens of its own sequence, as its weight there is 0 times it."""
-    hq, hk = _heads("attention", q, k, v, plan, head_dim)
-    scale = _scale("attention", scale, head_dim)
-    if not q.is_cuda:
+    device = _together("attention", q, k, v, plan.starts)
+    hq, hk, scale, *steps = _layout("attention", q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, plan.tokens, head_dim,
+                                    scale, device >= 0)
+    if device < 0:
         o, lse = _attention_cpu(q, k, v, plan, head_dim, scale)
         return (o.to(q.dtype), lse) if return_lse else o.to(q.dtype)
     half = q.dtype is torch.bfloat16
-    (q, qs), (k, ks), (v, vs) = (_rows(t, half) for t in (q, k, v))
-    o = q.new_empty((plan.tokens, hq * head_dim))
+    (q, qs), (k, ks), (v, vs) = _operands(half, (q, steps[0]), (k, steps[1]), (v, steps[2]))
+    cols = hq * head_dim
+    o = q.new_empty((plan.tokens, cols))
     lse = torch.empty((hq, plan.tokens), dtype=torch.float32, device=q.device) if return_lse else None
-    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), plan.words.data_ptr(), o.data_ptr(), N.ptr(lse), plan.tokens, plan.batch, hq, hk, head_dim, qs, ks, vs,
-            hq * head_dim, scale)
     if half:
-        K._launch(N.require().oa_packed_attn(*args, K.status_word(q.device).data_ptr(), N.stream()), "oa_packed_attn", 2, outputs=(o,))
+        K._launch(N.require().oa_packed_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), plan.words.data_ptr(), o.data_ptr(), N.ptr(lse), plan.tokens, plan.batch, hq, hk,
+                                             head_dim, qs, ks, vs, cols, scale, K.status_word(q.device).data_ptr(), _stream(device)),
+                  "oa_packed_attn", 2, outputs=(o,))
     else:
-        K._launch(N.require().oa_packed_attn_f32(*args, N.stream()), "oa_packed_attn_f32", outputs=(o,))
+        K._launch(N.require().oa_packed_attn_f32(q.data_ptr(), k.data_ptr(), v.data_ptr(), plan.words.data_ptr(), o.data_ptr(), N.ptr(lse), plan.tokens, plan.batch, hq,
+                                                 hk, head_dim, qs, ks, vs, cols, scale, _stream(device)), "oa_packed_attn_f32", outputs=(o,))
     return (o, lse) if return_lse else o
 
 
@@ -207,20 +252,26 @@ def attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: tor
     """The gradients (dq, dk, dv) of `attention` from its inputs, its output and log-sum-exp, and dout [tokens, q_heads * head_dim] (row stride
     allowed).  They are slices of `dqkv` [tokens, (q_heads + 2 kv_heads) * head_dim], a packed projection's gradient.  Those of a key-value head are the
     sums over the query heads that share it, added up in one order: the same inputs give the same bits.  Rows of no sequence are 0."""
-    hq, hk = _heads("attention_backward", q, k, v, plan, head_dim)
-    scale = _scale("attention_backward", scale, head_dim)
+    device = _together("attention_backward", q, k, v, o, dout, lse, plan.starts)
+    hq, hk, scale, *steps = _layout("attention_backward", q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, plan.tokens,
+                                    head_dim, scale, device >= 0)
     if o.shape != q.shape or dout.shape != q.shape or o.dtype is not q.dtype or dout.dtype is not q.dtype:
         raise ValueError(f"attention_backward: o and dout must be {q.dtype} {list(q.shape)}")
     if lse.shape != (hq, plan.tokens) or lse.dtype is not torch.float32 or not lse.is_contiguous():
         raise ValueError(f"attention_backward: lse must be a contiguous float32 tensor [{hq}, {plan.tokens}]")
     cols = [hq * head_dim, hk * head_dim, hk * head_dim]
+    width = sum(cols)
     if dqkv is None:
-        dqkv = q.new_empty((plan.tokens, sum(cols)))
-    elif dqkv.shape != (plan.tokens, sum(cols)) or dqkv.dtype is not q.dtype or not dqkv.is_contiguous():
-        raise ValueError(f"attention_backward: dqkv must be a contiguous {q.dtype} tensor [{plan.tokens}, {sum(cols)}]")
-    _together("attention_backward", q, o, dout, lse, dqkv)
-    grads = torch.split(dqkv, cols, 1)
-    if not q.is_cuda:
+        dqkv = q.new_empty((plan.tokens, width))
+    else:
+        if dqkv.shape != (plan.tokens, width) or dqkv.dtype is not q.dtype or not dqkv.is_contiguous():
+            raise ValueError(f"attention_backward: dqkv must be a contiguous {q.dtype} tensor [{plan.tokens}, {width}]")
+        _together("attention_backward", q, dqkv)
+        _apart("attention_backward", dqkv, q, k, v, o, dout, lse)
+        if device >= 0 and dqkv.data_ptr() & 15:
+            raise ValueError("attention_backward: dqkv must begin on 16 bytes")
+    grads = torch.unsafe_split_with_sizes(dqkv, cols, 1)
+    if device < 0:
         with torch.enable_grad():
             leaves = [t.detach().float().requires_grad_(True) for t in (q, k, v)]
             y, _ = _attention_cpu(*leaves, plan, head_dim, scale)
@@ -229,19 +280,20 @@ def attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: tor
             to.copy_(g) if g is not None else to.zero_()
         return grads
     half = q.dtype is torch.bfloat16
-    (q, qs), (k, ks), (v, vs), (o, os), (dout, dos) = (_rows(t, half) for t in (q, k, v, o, dout))
-    dq, dk, dv = grads
-    if half and dqkv.data_ptr() % 16:
-        raise ValueError("attention_backward: dqkv must begin on 16 bytes")
-    width = dqkv.shape[1]
-    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr(), lse.data_ptr(), plan.words.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-            dv.data_ptr(), plan.tokens, plan.batch, hq, hk, head_dim, qs, ks, vs, os, dos, width, width, width, scale)
+    (q, qs), (k, ks), (v, vs), (o, os), (dout, dos) = _operands(half, (q, steps[0]), (k, steps[1]), (v, steps[2]), (o, _kernel_step(o.shape, o.stride(), half)),
+                                                                (dout, _kernel_step(dout.shape, dout.stride(), half)))
+    at = dqkv.data_ptr()
+    size = dqkv.element_size()
+    dk, dv = at + cols[0] * size, at + (cols[0] + cols[1]) * size
     if half:
         # scratch of the call's own: calls on several streams, and graphs, do not meet in it
         need = N.require().oa_packed_attn_bwd_scratch_bytes(plan.tokens, plan.batch, hq, hk, head_dim)
         scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-        K._launch(N.require().oa_packed_attn_bwd(*args, scratch.data_ptr(), K.status_word(q.device).data_ptr(), N.stream()), "oa_packed_attn_bwd", 4,
-                  outputs=(dqkv,))
+        K._launch(N.require().oa_packed_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr(), lse.data_ptr(), plan.words.data_ptr(), at, dk, dv,
+                                                 plan.tokens, plan.batch, hq, hk, head_dim, qs, ks, vs, os, dos, width, width, width, scale, scratch.data_ptr(),
+                                                 K.status_word(q.device).data_ptr(), _stream(device)), "oa_packed_attn_bwd", 4, outputs=(dqkv,))
     else:
-        K._launch(N.require().oa_packed_attn_f32_bwd(*args, N.stream()), "oa_packed_attn_f32_bwd", outputs=(dqkv,))
+        K._launch(N.require().oa_packed_attn_f32_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr(), lse.data_ptr(), plan.words.data_ptr(), at, dk, dv,
+                                                     plan.tokens, plan.batch, hq, hk, head_dim, qs, ks, vs, os, dos, width, width, width, scale, _stream(device)),
+                  "oa_packed_attn_f32_bwd", outputs=(dqkv,))
     return grads

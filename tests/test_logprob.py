@@ -284,5 +284,11 @@ def test_refusals():
                             ("out must be", (None,), dict(out=torch.zeros(1, 20).expand(3, 20))), ("out must be", (None,), dict(out=x.bfloat16()))):
         with pytest.raises(ValueError, match=match):
             L.token_logprobs_backward(x, t, r, *args, **kw)
+    for ignore in (1 << 31, -(1 << 31) - 1):
+        with pytest.raises(ValueError, match="ignore_index is"):
+            L.token_logprobs(x, t, ignore_index=ignore)
+    both = torch.zeros(3, 21)
+    with pytest.raises(ValueError, match="lie apart"):
+        L.token_logprobs_backward(both[:, 1:], t, r, None, out=both[:, :20])
     with pytest.raises(ValueError, match="result.stats must be"):
         L.token_logprobs_backward(x, t, r._replace(stats=torch.zeros(3)), None)

@@ -433,6 +433,23 @@ def test_another_device_than_the_current_one(monkeypatch):
         P._together("attention", Elsewhere(), Elsewhere())
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_results_in_the_operands_memory(device):
+    """Refused where it would be written before it is read; columns beside one another are no overlap."""
+    plan = P.plan(torch.tensor([0, 6], dtype=torch.int32, device=device), 6)
+    qkv = torch.randn(6, 192, device=device)
+    q, k, v = torch.split(qkv, 64, 1)
+    o, lse = P.attention(q, k, v, plan, 64, return_lse=True)
+    with pytest.raises(ValueError, match="that of an operand"):
+        P.attention_backward(q, k, v, o, o, lse, plan, 64, dqkv=qkv)
+    pos = torch.zeros(1, 6, dtype=torch.int32, device=device)
+    for bad in (qkv.reshape(-1)[64:64 + 5 * 192 + 64].as_strided((6, 64), (192, 1), 32), qkv.reshape(-1).as_strided((6, 64), (64, 1), 0)):
+        with pytest.raises(ValueError, match="that of an operand"):
+            P.rotary(qkv, pos, (0,) * 32, 1, 64, THETA, out=bad)
+    want = P.rotary(qkv[:, :64], pos, (0,) * 32, 1, 64, THETA)
+    assert torch.equal(P.rotary(qkv[:, :64], pos, (0,) * 32, 1, 64, THETA, out=qkv[:, 64:128]), want) and torch.equal(qkv[:, 64:128], want)
+
+
 @pytest.mark.gpu
 def test_refusals_of_the_kernels():
     plan = P.plan(torch.tensor([0, 8], dtype=torch.int32, device="cuda"), 8)

@@ -5,7 +5,10 @@
 // scores, rows ty + 16 i and columns tx + 16 j, so that it takes 8 loads of 16 bytes for 64 multiply-adds and no two rows of a warp's loads meet in a
 // bank; the weights go to shared memory and the second product is dealt out the same way, over the head's dimensions.  The next tile's first operand is on its
 // way (cp.async) while the second product of this one runs.  Rows of other sequences are never read: what a sequence holds does not reach another.  dK and
-// dV of a key-value head add up over the query heads that share it, one after the other in one block: one writer, one order.
+// dV of a key-value head add up over the query heads that share it: up to eight of them are a cluster of blocks, a head to each, whose sums meet in distributed
+// shared memory in the heads' order; more are worked on by one block one after the other.  Either way there is one writer and one order.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "packed.cuh"
 #include "per_device.h"
@@ -13,6 +16,9 @@
 
 namespace oa {
 
+namespace cg = cooperative_groups;
+
+constexpr int PF32_CLUSTER = 8;                        // blocks of a cluster, at most
 constexpr int PF32_THREADS = 256, PF32_ROWS = 64;
 constexpr int PF32_LDW = PF32_ROWS + 4;                // floats between rows of weights
 
@@ -276,15 +282,17 @@ __device__ __forceinline__ void packed_f32_bwd_q(float* sm, const PackedF32Param
   Tile::store(acc, mul, p.dq, p.dqs, t.lo, t.i0, t.n, h * hd, hd, tx, ty);
 }
 
-// dK, dV: rows are keys; the queries of every head of the group stream by with their log-sum-exp and delta = rowsum(dO * O)
+// dK, dV: rows are keys; the queries of the group's heads stream by with their log-sum-exp and delta = rowsum(dO * O).  blockIdx.y: the query head that this block of
+// a cluster works on; without a cluster the first of a group stands for all.
 template <int HD>
 __device__ __forceinline__ void packed_f32_bwd_kv(float* sm, const PackedF32Params& p) {
   using Tile = F32Tile<HD>;
   float *sK = sm, *sV = sK + Tile::FLOATS, *sQ = sV + Tile::FLOATS, *sDO = sQ + Tile::FLOATS, *sW = sDO + Tile::FLOATS;
   __shared__ float sL[PF32_ROWS], sDelta[PF32_ROWS];
-  const int hk = blockIdx.y, hd = p.hd, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  if (hk >= p.kv_heads) return;
-  p.plan.others(blockIdx.x, gridDim.x, [&](int r) {
+  const int hk = blockIdx.y / p.group, first = blockIdx.y % p.group, hd = p.hd, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int parts = p.group <= PF32_CLUSTER ? p.group : 1, heads = p.group / parts;
+  if (first >= parts) return;
+  if (first == 0) p.plan.others(blockIdx.x, gridDim.x, [&](int r) {
     for (int d = threadIdx.x; d < hd; d += PF32_THREADS) p.dk[r * p.dks + hk * hd + d] = p.dv[r * p.dvs + hk * hd + d] = 0.f;
   });
   const PackedRows t = packed_rows<true>(p.plan, blockIdx.x);
@@ -294,16 +302,16 @@ __device__ __forceinline__ void packed_f32_bwd_kv(float* sm, const PackedF32Para
   Tile::fetch(sV, p.v, p.vs, t.lo, t.i0, t.n, hk * hd, hd, vec);
   float dk[4][Tile::WIDE] = {}, dv[4][Tile::WIDE] = {};
   // steps: tiles of queries from the block's own rows on, of one head after the other
-  const int per = (t.n - t.i0 + PF32_ROWS - 1) / PF32_ROWS, steps = per * p.group;
+  const int per = (t.n - t.i0 + PF32_ROWS - 1) / PF32_ROWS, steps = per * heads, h0 = blockIdx.y;
   const auto fetch = [&](int step) {
-    const int h = hk * p.group + step / per, q0 = t.i0 + step % per * PF32_ROWS;
+    const int h = h0 + step / per, q0 = t.i0 + step % per * PF32_ROWS;
     Tile::fetch(sQ, p.q, p.qs, t.lo, q0, t.n, h * hd, hd, vec);
     Tile::fetch(sDO, p.dout, p.dos, t.lo, q0, t.n, h * hd, hd, vec);
     f32_commit();
   };
   fetch(0);
   for (int step = 0; step < steps; ++step) {
-    const int h = hk * p.group + step / per, q0 = t.i0 + step % per * PF32_ROWS;
+    const int h = h0 + step / per, q0 = t.i0 + step % per * PF32_ROWS;
     {                                                         // four threads to a query
       const int r = threadIdx.x >> 2, part = threadIdx.x & 3, row = q0 + r;
       float delta = 0.f, L = INFINITY;
@@ -363,6 +371,29 @@ __device__ __forceinline__ void packed_f32_bwd_kv(float* sm, const PackedF32Para
     __syncthreads();                                          // Q and dO have been read
     if (step + 1 < steps) fetch(step + 1);
   }
+  if (parts > 1) {
+    // every block's sums to its shared memory, in the order of its threads; each then adds up a share of the places over the cluster
+    constexpr int PLACES = 4 * Tile::WIDE;                    // of a thread, for dK and for dV
+    const cg::cluster_group cluster = cg::this_cluster();
+#pragma unroll
+    for (int c = 0; c < PLACES; ++c) {
+      sm[c * PF32_THREADS + threadIdx.x] = dk[c / Tile::WIDE][c % Tile::WIDE];
+      sm[(PLACES + c) * PF32_THREADS + threadIdx.x] = dv[c / Tile::WIDE][c % Tile::WIDE];
+    }
+    cluster.sync();
+    for (int c = first; c < 2 * PLACES; c += parts) {
+      float sum = 0.f;
+      for (int b = 0; b < parts; ++b) sum += cluster.map_shared_rank(sm, b)[c * PF32_THREADS + threadIdx.x];
+      cluster.map_shared_rank(sm, 0)[c * PF32_THREADS + threadIdx.x] = sum;      // nobody else reads this place of any block
+    }
+    cluster.sync();
+    if (first > 0) return;
+#pragma unroll
+    for (int c = 0; c < PLACES; ++c) {
+      dk[c / Tile::WIDE][c % Tile::WIDE] = sm[c * PF32_THREADS + threadIdx.x];
+      dv[c / Tile::WIDE][c % Tile::WIDE] = sm[(PLACES + c) * PF32_THREADS + threadIdx.x];
+    }
+  }
   const float one[4] = {1.f, 1.f, 1.f, 1.f}, mul[4] = {p.scale, p.scale, p.scale, p.scale};
   Tile::store(dk, mul, p.dk, p.dks, t.lo, t.i0, t.n, hk * hd, hd, tx, ty);
   Tile::store(dv, one, p.dv, p.dvs, t.lo, t.i0, t.n, hk * hd, hd, tx, ty);
@@ -388,10 +419,23 @@ template <int HD, bool BWD>
 static int packed_f32_run(const PackedF32Params& p, dim3 grid, cudaStream_t st) {
   static std::atomic<unsigned long long> allowed;
   constexpr int BYTES = ((BWD ? 4 : 3) * F32Tile<HD>::FLOATS + PF32_ROWS * PF32_LDW) * (int)sizeof(float);
+  static_assert(!BWD || BYTES >= 8 * F32Tile<HD>::WIDE * PF32_THREADS * (int)sizeof(float), "a cluster's sums");
   void (*const kernel)(const PackedF32Params) = BWD ? packed_f32_bwd_kernel<HD> : packed_f32_fwd_kernel<HD>;
   if (allow_smem(allowed, (const void*)kernel, BYTES) != cudaSuccess) return OA_ERR_LAUNCH;
-  launch_short(kernel, grid, dim3(PF32_THREADS), BYTES, st, p);
-  return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(PF32_THREADS);
+  cfg.dynamicSmemBytes = BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
+  attr[0].val.clusterDim.y = BWD && p.group <= PF32_CLUSTER ? p.group : 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_on((long long)grid.x * grid.y * grid.z <= PDL_SHORT_BLOCKS) ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }
 
 template <bool BWD>

@@ -145,7 +145,7 @@ def test_attention_more_items_than_sms(hd):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("lengths", [[1], [31, 33], [129], RAGGED], ids=lambda v: "-".join(map(str, v)))
-@pytest.mark.parametrize("hq,hk,hd", [(4, 4, 32), (4, 2, 64), (3, 1, 128), (2, 1, 20), (2, 2, 7), (12, 4, 50)])
+@pytest.mark.parametrize("hq,hk,hd", [(4, 4, 32), (4, 2, 64), (3, 1, 128), (2, 1, 20), (2, 2, 7), (12, 4, 50), (8, 1, 32), (9, 1, 16), (24, 2, 64)])
 def test_attention_fp32(device, lengths, hq, hk, hd):
     _check(lengths, hq, hk, hd, torch.float32, device, first=2, pad=5)
 

@@ -123,7 +123,7 @@ _FN_MATRIX = [n for n in dir(_F) if n[0].isupper()]
 OaFnMatrix = _namespace("OaFnMatrix", "Tensor factories and differentiable operations.", _F, _FN_MATRIX)
 OaFnLoss = _namespace("OaFnLoss", "Loss functions and their explicit backward forms.", _L,
                       ["Bce", "BceBwd", "CrossEntropy", "CrossEntropyBwd", "MaskedCrossEntropy", "L1", "L1Bwd", "Mse", "MseBwd", "SmoothL1",
-                       "SmoothL1Bwd", "LastName"])
+                       "SmoothL1Bwd", "TokenLogProbs", "LastName"])
 for _n in ("PpoClippedPolicy", "PpoClippedPolicyBwd", "Ppo", "Dqn", "SacCritic", "SacActor"):
     setattr(OaFnLoss, _n, getattr(_FRL, _n))
 OaFnLoss.__all__ = OaFnLoss.__all__ + ("PpoClippedPolicy", "PpoClippedPolicyBwd", "Ppo", "Dqn", "SacCritic", "SacActor")

@@ -21,6 +21,7 @@ import torch
 from .. import _native as N
 from ..ml import autograd as AG
 from ..ops import kernels as K
+from ..ops import packed as PK
 from ..runtime import engine as RT
 from .matrix import OaMatrix
 from .types import OaScalarType, to_torch_dtype
@@ -990,6 +991,67 @@ def FlashAttentionCausal(q: OaMatrix, k: OaMatrix, v: OaMatrix, batch: int, seq:
     """q, k, v: [B*S, D] each -> [B*S, D]."""
     D = q.Size(-1)
     return FlashAttentionPacked(Concat([q, k, v], 1), batch, seq, heads, D // heads, causal=True)
+
+
+# ---- sequences of different lengths, packed one behind the other (ops/packed.py)
+class OaPackedSequences:
+    """Which rows of packed tensors are whose: what the attention kernels work on (`Plan`, for every layer in both directions), the rows' positions
+    [axes, tokens] and which axis turns each pair of a head (None: the first axis all of them)."""
+
+    def __init__(self, plan: PK.PackedPlan, positions: torch.Tensor, pair_axes: Optional[Sequence[int]] = None):
+        self.Plan, self.Positions = plan, positions
+        self.PairAxes = None if pair_axes is None else tuple(pair_axes)
+
+    def Tokens(self) -> int:
+        return self.Plan.tokens
+
+    def Axes(self, head_dim: int) -> tuple:
+        return (0,) * (head_dim // 2) if self.PairAxes is None else self.PairAxes
+
+
+def PackedSequences(starts: OaMatrix, tokens: int, positions: Optional[OaMatrix] = None, pair_axes: Optional[Sequence[int]] = None) -> OaPackedSequences:
+    """Sequences in rows starts[b] .. starts[b + 1] (int32 [batch + 1]) of tensors of `tokens` rows.  `positions` [axes, tokens] int32: by default one axis, a
+    row's place in its sequence.  Nothing is read back to the host."""
+    plan = PK.plan(starts.Tensor(), tokens)
+    if positions is not None:
+        return OaPackedSequences(plan, positions.Tensor(), pair_axes)
+    row = torch.arange(tokens, dtype=torch.int32, device=plan.starts.device)
+    first = plan.starts[(torch.searchsorted(plan.starts, row, right=True) - 1).clamp(min=0)]
+    return OaPackedSequences(plan, torch.where((row >= plan.starts[0]) & (row < plan.starts[-1]), row - first, 0)[None].contiguous(), pair_axes)
+
+
+def RotaryAxes(x: OaMatrix, positions: OaMatrix, pair_axes: Sequence[int], heads: int, head_dim: int, theta: float = 10000.0) -> OaMatrix:
+    """Rotary embedding of [tokens, heads*head_dim] rows by their positions [axes, tokens]: pair j of a head turns with axis pair_axes[j]."""
+    _ctx_add("RotaryAxes")
+    t, pos, axes = x.Tensor(), positions.Tensor(), tuple(pair_axes)
+    out = _w(PK.rotary(t, pos, axes, heads, head_dim, theta))
+    return AG.attach("RotaryAxes", out, [x], lambda g: (PK.rotary(_c(g), pos, axes, heads, head_dim, theta, backward=True),))
+
+
+def PackedAttention(qkv: OaMatrix, sequences: OaPackedSequences, heads: int, kv_heads: int, head_dim: int, *, rope_theta: float = 0.0,
+                    consume_input: bool = False) -> OaMatrix:
+    """Causal attention within every packed sequence over a projection output [tokens, (heads + 2*kv_heads)*hd] (q | k | v side by side, heads a multiple of
+    kv_heads); returns [tokens, heads*hd].  With rope_theta > 0 q and k are turned by the sequences' positions in place first (on a copy while autograd
+    records, unless the caller owns the projection output and passes consume_input)."""
+    _ctx_add("PackedAttention")
+    t = qkv.Tensor()
+    turned, axes = heads + kv_heads, sequences.Axes(head_dim)
+    if rope_theta > 0:
+        if (AG.IsEnabled() and qkv.RequiresGrad() and not consume_input) or not t.is_contiguous():
+            t = K.unary("copy", _c(t))
+        PK.rotary(t, sequences.Positions, axes, turned, head_dim, rope_theta, out=t)
+    q, k, v = torch.split(t, [heads * head_dim, kv_heads * head_dim, kv_heads * head_dim], 1)
+    o, lse = PK.attention(q, k, v, sequences.Plan, head_dim, return_lse=True)
+    out = _w(o)
+
+    def back(g):
+        dqkv = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        PK.attention_backward(q, k, v, o, _c(g), lse, sequences.Plan, head_dim, dqkv=dqkv)
+        if rope_theta > 0:
+            PK.rotary(dqkv, sequences.Positions, axes, turned, head_dim, rope_theta, backward=True, out=dqkv)
+        return (dqkv,)
+
+    return AG.attach("PackedAttention", out, [qkv], back)
 
 
 # ======================================================================= embedding

@@ -13,6 +13,7 @@ import torch
 from ..core import fn_matrix as F
 from ..core.matrix import OaMatrix
 from ..ops import kernels as K
+from ..ops import logprob
 from . import autograd as AG
 
 _last_name = ""
@@ -77,6 +78,24 @@ def MaskedCrossEntropy(logits: OaMatrix, targets: OaMatrix, mask: OaMatrix) -> O
     out = OaMatrix((row_loss.sum() / cnt).reshape(1))
     return AG.attach("MaskedCrossEntropy", out, [logits, targets],
                      lambda g: ((dl.float() * (g.reshape(1) / cnt)).to(dl.dtype).reshape(lt.shape), None))
+
+
+def TokenLogProbs(logits: OaMatrix, targets: OaMatrix, scale: float = 1.0, ignore_index: int = -100, in_place_grad: bool = False) -> OaMatrix:
+    """[2, rows] fp32: the log-probability of each row's target in scale * logits [rows, vocab] (0 where it is `ignore_index`) and, below it, the row's
+    entropy; what a policy's loss is made of.  With `in_place_grad` the logits buffer is overwritten by its gradient in the backward pass."""
+    _set("TokenLogProbs")
+    lt = logits.Tensor()
+    l2 = lt.reshape(-1, lt.shape[-1])
+    tg = targets.Tensor().reshape(-1).to(torch.int32).contiguous()
+    r = logprob.token_logprobs(l2, tg, 0, scale, ignore_index)
+    out = OaMatrix(torch.stack([r.logprobs, r.entropy]))
+
+    def back(g):
+        g = g.float().contiguous()
+        d = logprob.token_logprobs_backward(l2, tg, r, g[0], g[1], scale, ignore_index, out=l2 if in_place_grad else None)
+        return (d.reshape(lt.shape), None)
+
+    return AG.attach("TokenLogProbs", out, [logits, targets], back)
 
 
 def CrossEntropyBwd(logits: OaMatrix, targets: OaMatrix) -> OaMatrix:

@@ -198,9 +198,15 @@ class OaMultiHeadAttention(OaModule):
             return False          # the tensor-core kernel is built for head dims 64 and 128; others take the materialised path
         return True
 
-    def Attend(self, qkv: OaMatrix, batch: int, seq: int, pos_offset: int = 0, mask: Optional[OaMatrix] = None) -> OaMatrix:
+    def Attend(self, qkv: OaMatrix, batch: int, seq: int, pos_offset: int = 0, mask: Optional[OaMatrix] = None,
+               packed: Optional[F.OaPackedSequences] = None) -> OaMatrix:
         """`mask`, when given, is an additive [B*H*S, S] (or [S, S]) mask: it takes the materialised path and replaces the
-        causal mask (MultiHeadAttention::ForwardMasked of the reference)."""
+        causal mask (MultiHeadAttention::ForwardMasked of the reference).  `packed`: the rows are sequences of different lengths one behind the
+        other, each of which attends to itself."""
+        if packed is not None:
+            if mask is not None or not self.Causal or pos_offset:
+                raise ValueError("packed sequences are causal, without a mask or a position offset")
+            return F.PackedAttention(qkv, packed, self.NumHeads, self.NumHeads, self.HeadDim, rope_theta=self.RopeTheta, consume_input=True)
         if mask is None and self._use_flash():
             return F.FlashAttentionPacked(qkv, batch, seq, self.NumHeads, self.HeadDim, causal=self.Causal,
                                           rope_theta=self.RopeTheta, pos_offset=pos_offset, consume_input=True)
@@ -221,13 +227,13 @@ class OaMultiHeadAttention(OaModule):
         return self.Forward(x, batch, seq, residual, 0, additive_mask)
 
     def Forward(self, x: OaMatrix, batch: Optional[int] = None, seq: Optional[int] = None, residual: Optional[OaMatrix] = None,
-                pos_offset: int = 0, mask: Optional[OaMatrix] = None) -> OaMatrix:
-        """x: [B*S, D] (pass batch, seq) or [B, S, D]."""
+                pos_offset: int = 0, mask: Optional[OaMatrix] = None, packed: Optional[F.OaPackedSequences] = None) -> OaMatrix:
+        """x: [B*S, D] (pass batch, seq) or [B, S, D]; [tokens, D] with `packed` sequences."""
         shape3 = x.Rank() == 3
         if shape3:
             batch, seq = x.Size(0), x.Size(1)
             x = x.Reshape([batch * seq, self.DModel])
-        a = self.Attend(self.ProjectQkv(x), batch, seq, pos_offset, mask)
+        a = self.Attend(self.ProjectQkv(x), batch, seq, pos_offset, mask, packed)
         o = self.OutProj
         y = F.Linear(a, o.Weight.Data, o.Bias.Data if o.Bias else None, residual=residual)
         return y.Reshape([batch, seq, self.DModel]) if shape3 else y
@@ -356,16 +362,17 @@ class OaTransformerBlock(OaModule):
         return F.Add(x, F.Mul(self._ffn_delta(h), g_f))
 
     def Forward(self, x: OaMatrix, batch: Optional[int] = None, seq: Optional[int] = None, pos_offset: int = 0,
-                mask: Optional[OaMatrix] = None) -> OaMatrix:
+                mask: Optional[OaMatrix] = None, packed: Optional[F.OaPackedSequences] = None) -> OaMatrix:
+        """`packed`: x is [tokens, D], sequences of different lengths one behind the other."""
         shape3 = x.Rank() == 3
         if shape3:
             batch, seq = x.Size(0), x.Size(1)
             x = x.Reshape([batch * seq, self.DModel])
-        if batch is None:
+        if batch is None and packed is None:
             seq = self.SeqLen
             batch = x.Size(0) // seq
         plan = self.BlockPlan()
-        x = self.Attention.Forward(self.LnAttn.Forward(x), batch, seq, residual=x, pos_offset=pos_offset, mask=mask)
+        x = self.Attention.Forward(self.LnAttn.Forward(x), batch, seq, residual=x, pos_offset=pos_offset, mask=mask, packed=packed)
         if self.Moe is not None:
             x = self.Moe.Forward(x)
         elif self.FfnKind == "gelu":

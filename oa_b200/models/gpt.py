@@ -98,6 +98,27 @@ class OaGptModel(OaModule):
         """ids [B, S] int32 -> logits [B*S, vocab]."""
         return self.Head.Forward(self.Hidden(ids))
 
+    def HiddenPacked(self, ids: OaMatrix, sequences: F.OaPackedSequences) -> OaMatrix:
+        """ids [tokens] of sequences of different lengths, one behind the other (`F.PackedSequences`); in bf16 training a multiple of 8 rows, those behind the last
+        sequence belonging to none."""
+        if ids.NumElements() != sequences.Tokens():
+            raise ValueError(f"{ids.NumElements()} tokens, but the sequences are of {sequences.Tokens()} rows")
+        x = F.Embedding(self.Embed.Weight.Data, ids)
+        if self.PosEmbed is not None:
+            x = F.Add(x, F.Embedding(self.PosEmbed.Weight.Data, OaMatrix(sequences.Positions[0])))
+        for b in self.Blocks:
+            x = b.Forward(x, packed=sequences)
+        return self.LnFinal.Forward(x)
+
+    def ForwardPacked(self, ids: OaMatrix, sequences: F.OaPackedSequences) -> OaMatrix:
+        """ids [tokens] int32 -> logits [tokens, vocab]; no sequence sees another."""
+        return self.Head.Forward(self.HiddenPacked(ids, sequences))
+
+    def TokenLogProbs(self, ids: OaMatrix, targets: OaMatrix, sequences: F.OaPackedSequences, scale: float = 1.0) -> OaMatrix:
+        """[2, tokens]: the log-probability of every row's target (-100: none) and the entropy there, for training a policy or scoring texts; the
+        logits buffer is reused for its own gradient."""
+        return L.TokenLogProbs(self.ForwardPacked(ids, sequences), targets, scale=scale, in_place_grad=True)
+
     def Loss(self, ids: OaMatrix, targets: OaMatrix) -> OaMatrix:
         """Mean next-token cross-entropy; the logits buffer is reused for its own gradient."""
         logits = self.Forward(ids)

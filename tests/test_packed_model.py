@@ -1,0 +1,196 @@
+"""A model on packed sequences: rotary positions, attention, log-probabilities and their gradients together, against the same model on one sequence at a
+time, and a training step and scoring of prompts as a program makes them."""
+import pytest
+import torch
+
+from oa_b200.core import fn_matrix as F
+from oa_b200.core.matrix import OaMatrix
+from oa_b200.ml import autograd as AG
+from oa_b200.ml import fn_loss as L
+from oa_b200.ml.optim import OaAdamW
+from oa_b200.models import OaGptConfig, OaGptModel
+from oa_b200.ops import logprob, packed, paged
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+LENGTHS = [5, 1, 70, 0, 33, 129]
+
+
+def _batch(vocab, device, pad=2):
+    g = torch.Generator().manual_seed(1)
+    tokens = sum(LENGTHS) + pad
+    ids = torch.randint(0, vocab, (tokens,), generator=g, dtype=torch.int32)
+    starts = torch.tensor([0] + LENGTHS).cumsum(0).to(torch.int32)
+    targets = ids.roll(-1).clone()
+    targets[starts[1:].long() - 1] = -100                     # nothing follows a sequence's last token
+    targets[sum(LENGTHS) - 1:] = -100
+    weight = torch.randn(2, tokens, generator=g)
+    weight[:, sum(LENGTHS):] = 0
+    return ids.to(device), starts.to(device), targets.to(device), weight.to(device)
+
+
+def _model(rope, device, heads=2, d=64, dtype=torch.float32, **kw):
+    prev = F.GetWeightDtype()
+    F.SetWeightDtype(dtype)
+    try:
+        F.SetRngSeed(3)
+        return OaGptModel(OaGptConfig(104, d, 2, heads, 2 * d, 256, "rms" if rope else "layer", "swiglu" if rope else "gelu", 10000.0 if rope else 0.0, not rope, 1e-5, 0.15, **kw))
+    finally:
+        F.SetWeightDtype(prev)
+
+
+def _grads(model):
+    return [p.Data.GradTensor().float().clone() for p in model.AllParameterPtrs() if p.Data.GradTensor() is not None]
+
+
+def _weighted(out, weight):
+    return F.Sum(F.Mul(out, OaMatrix(weight)))
+
+
+def _run(model, build):
+    for p in model.AllParameterPtrs():
+        p.Data.ZeroGrad()
+    with AG.OaGradientTape() as tape:
+        out, loss = build()
+        tape.Backward(loss)
+    return out, _grads(model)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rope", [False, True])
+def test_packed_is_one_sequence_at_a_time(device, rope):
+    """fp32: each of about 14 products one after the other adds at most 256 terms, 256 2^-24 of the sum of their magnitudes: 14 * 1.5e-5 = 2^-12 of the largest
+    values, and as much on the way back."""
+    model = _model(rope, device)
+    ids, starts, targets, weight = _batch(104, device)
+    seqs = F.PackedSequences(OaMatrix(starts), ids.numel())
+    got, grads = _run(model, lambda: (lambda o: (o, _weighted(o, weight)))(model.TokenLogProbs(OaMatrix(ids), OaMatrix(targets), seqs)))
+    assert got.Tensor().shape == (2, ids.numel()) and bool((got.Tensor()[0][targets == -100] == 0).all())
+
+    def one_by_one():
+        outs, loss = [], None
+        for lo, n in zip(starts.tolist(), LENGTHS):
+            if n:
+                logits = model.Forward(OaMatrix(ids[lo:lo + n].repeat(2, 1)))      # twice, the second time without weight
+                o = L.TokenLogProbs(logits, OaMatrix(targets[lo:lo + n].repeat(2)))
+                part = _weighted(o, torch.cat([weight[:, lo:lo + n], torch.zeros_like(weight[:, lo:lo + n])], 1))
+                outs.append(o.Tensor()[:, :n])
+                loss = part if loss is None else F.Add(loss, part)
+        return torch.cat(outs, 1), loss
+
+    want, want_grads = _run(model, one_by_one)
+    n = sum(LENGTHS)
+    assert float((got.Tensor()[:, :n] - want).abs().max()) <= 2 ** -12 * float(want.abs().max())
+    assert len(grads) == len(want_grads)
+    # A bias of the keys adds one number to all scores of a query: its gradient is 0, and what stands there is what sums of the key weights' terms (rows of unit size
+    # apart) leave when they cancel
+    scale = {id(b.Attention.KProj.Bias): b.Attention.KProj.Weight.Data.GradTensor().abs().max() for b in model.Blocks if b.Attention.KProj.Bias is not None}
+    for p, a, b in zip(model.AllParameterPtrs(), grads, want_grads):
+        assert float((a - b).abs().max()) <= 2 ** -11 * float(scale.get(id(p), b.abs().max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("seq", [40, 200])
+def test_packed_bf16_gradients(hd, seq):
+    """bf16, four sequences of one length, packed and as the batch that the model takes otherwise: the same products with the same roundings, but for the attention
+    kernels, so that against the fp32 model of the same weights the gradients of both are equally far off.  How far roundings of 2^-8 get amplified is the
+    model's affair; over thousands of elements the norms of two such errors are alike, and twice the other's is allowed."""
+    model = _model(True, "cuda", heads=2, d=2 * hd, dtype=torch.bfloat16)
+    ref = _model(True, "cuda", heads=2, d=2 * hd)
+    for a, b in zip(model.AllParameterPtrs(), ref.AllParameterPtrs()):
+        b.Data.Tensor().copy_(a.Data.Tensor().float())
+    g = torch.Generator().manual_seed(2)
+    ids, targets = (torch.randint(0, 104, (4 * seq,), generator=g, dtype=torch.int32).cuda() for _ in range(2))
+    weight = torch.randn(2, 4 * seq, generator=g).cuda()
+    seqs = F.PackedSequences(OaMatrix(torch.arange(0, 5 * seq, seq, dtype=torch.int32, device="cuda")), 4 * seq)
+    dense = lambda m: lambda: (lambda o: (o, _weighted(o, weight)))(L.TokenLogProbs(m.Forward(OaMatrix(ids.reshape(4, seq))), OaMatrix(targets)))      # noqa: E731
+    want = _run(ref, dense(ref))[1]
+    usual = _run(model, dense(model))[1]
+    got = _run(model, lambda: (lambda o: (o, _weighted(o, weight)))(model.TokenLogProbs(OaMatrix(ids), OaMatrix(targets), seqs)))[1]
+    for a, b, w in zip(got, usual, want):
+        assert float((a - w).norm()) <= 2 * float((b - w).norm())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_policy_step(device):
+    """log-probabilities, entropy, gradients and an optimizer step run, and change the weights; rows behind the last sequence take no part."""
+    model = _model(True, device)
+    ids, starts, targets, weight = _batch(104, device)
+    opt = OaAdamW(model.AllParameterPtrs(), 1e-3)
+    seqs = F.PackedSequences(OaMatrix(starts), ids.numel())
+    before = [p.Data.Tensor().clone() for p in model.AllParameterPtrs()]
+    opt.ZeroGrad()
+    with AG.OaGradientTape() as tape:
+        tape.Backward(_weighted(model.TokenLogProbs(OaMatrix(ids), OaMatrix(targets), seqs), weight))
+    grads = _grads(model)
+    opt.Step()
+    assert all(bool(g.isfinite().all()) for g in grads) and any(bool((a != p.Data.Tensor()).any()) for a, p in zip(before, model.AllParameterPtrs()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rotary_attention_logprobs_together(device):
+    """The raw operators as a program for images and text uses them: several axes, grouped heads, alternatives of the last tokens; and the same tokens decoded
+    one by one over pages, turned by `rotary`, appended without a turn."""
+    hq, hk, hd, vocab = 4, 2, 64, 300
+    g = torch.Generator().manual_seed(5)
+    n = 40
+    qkv = torch.randn(n, (hq + 2 * hk) * hd, generator=g).to(device)
+    pos = torch.stack([torch.arange(n), torch.arange(n) // 7, torch.arange(n) % 7]).to(torch.int32).to(device)
+    axes = (0,) * 8 + (1,) * 12 + (2,) * 12
+    starts = torch.tensor([0, 15, n], dtype=torch.int32, device=device)
+    plan = packed.plan(starts, n)
+    turned = qkv.clone()
+    packed.rotary(turned, pos, axes, hq + hk, hd, 10000.0, out=turned)
+    q, k, v = torch.split(turned, [hq * hd, hk * hd, hk * hd], 1)
+    o = packed.attention(q, k, v, plan, hd)
+    table = torch.arange(8, dtype=torch.int32, device=device).reshape(2, 4)
+    k_pages, v_pages = (torch.zeros(8, hk, 16, hd, device=device) for _ in range(2))
+    for b, (lo, hi) in enumerate(((0, 15), (15, n))):
+        for t in range(lo, hi):
+            row = packed.rotary(qkv[t:t + 1], pos[:, t:t + 1].contiguous(), axes, hq + hk, hd, 10000.0)
+            slot = table[b, (t - lo) // 16] * 16 + (t - lo) % 16
+            qs = paged.append(torch.cat([row, qkv[t:t + 1, (hq + hk) * hd:]], 1), torch.zeros(1, dtype=torch.int32, device=device), slot.reshape(1), k_pages, v_pages, 0.0)
+            one = paged.attention(qs, k_pages, v_pages, table[b:b + 1], torch.tensor([t - lo + 1], dtype=torch.int32, device=device),
+                                  torch.tensor([0, 1], dtype=torch.int32, device=device), 1)
+            assert float((one - o[t:t + 1]).abs().max()) <= 2 ** -17      # sums of 64 and 40 terms of magnitude 1 in 32 bits, twice
+    logits = torch.randn(n, vocab, generator=g).to(device)
+    ids = torch.randint(0, vocab, (n,), generator=g, dtype=torch.int32).to(device)
+    r = logprob.token_logprobs(logits, ids, top=3)
+    assert torch.equal(r.top_ids[:, 0].long(), logits.argmax(1)) and bool((r.logprobs <= r.top_logprobs[:, 0] + 1e-6).all())
+
+
+def test_refusals():
+    model = _model(False, "cpu")
+    ids, starts, targets, _ = _batch(104, "cpu")
+    seqs = F.PackedSequences(OaMatrix(starts), ids.numel())
+    with pytest.raises(ValueError, match="tokens, but the sequences"):
+        model.ForwardPacked(OaMatrix(ids[:-1]), seqs)
+    block = model.Blocks[0]
+    x = OaMatrix(torch.zeros(ids.numel(), 64))
+    block.SetAttentionMode(1)
+    with pytest.raises(ValueError, match="packed sequences are causal"):
+        block.Forward(x, packed=seqs)
+    with pytest.raises(ValueError, match="pair_axes names axes"):
+        F.RotaryAxes(x, OaMatrix(seqs.Positions), (1,) * 16, 2, 32)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_default_positions(device):
+    seqs = F.PackedSequences(OaMatrix(torch.tensor([2, 5, 5, 9], dtype=torch.int32, device=device)), 12)
+    assert seqs.Positions.tolist() == [[0, 0, 0, 1, 2, 0, 1, 2, 3, 0, 0, 0]]
+    assert F.PackedSequences(OaMatrix(torch.tensor([0], dtype=torch.int32, device=device)), 0).Positions.shape == (1, 0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradient_of_rotary_axes(device):
+    x = OaMatrix(torch.randn(6, 128, generator=torch.Generator().manual_seed(0)).to(device)).SetRequiresGrad(True)
+    pos = torch.randint(0, 50, (2, 6), generator=torch.Generator().manual_seed(1), dtype=torch.int32).to(device)
+    w = torch.randn(6, 128, generator=torch.Generator().manual_seed(2)).to(device)
+    axes = (0, 1) * 8
+    with AG.OaGradientTape() as tape:
+        tape.Backward(_weighted(F.RotaryAxes(x, OaMatrix(pos), axes, 2, 64), w))
+    assert torch.equal(x.GradTensor(), packed.rotary(w, pos, axes, 2, 64, 10000.0, backward=True))
+    # its transpose: <turn(a), w> = <a, turn back(w)>, sums of 768 terms in 32 bits
+    a = x.Tensor()
+    lhs, rhs = (packed.rotary(a, pos, axes, 2, 64, 10000.0) * w).sum(), (a * x.GradTensor()).sum()
+    assert abs(float(lhs - rhs)) <= 768 * 2.0 ** -23 * float((a.abs() * w.abs()).sum())

@@ -23,7 +23,7 @@ namespace oa {
 // A CTA's work items: (tile or pair of tiles, one of `per` heads or pairs of heads), all of the longest tiles first, in snake order over the
 // CTAs (round r: CTA c takes item r G + c, or r G + G - 1 - c when r is odd).  Every warp walks them alike.  The plan's entries of the first rounds are
 // fetched to shared memory at the start: with a load from L2 for each item, sent for during the one before, the kernels took 6 to 13 % longer.
-constexpr int PACKED_ROUNDS = 128;
+constexpr int PACKED_ROUNDS = 96;
 template <bool PAIRS>
 struct PackedWalk {
   const PackedPlan& plan;
@@ -52,6 +52,19 @@ struct PackedWalk {
     return true;
   }
 };
+
+// The 64 threads of the two warps that share 32 rows
+__device__ __forceinline__ void row_sync(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
+__device__ __forceinline__ float lo_of(unsigned long long v) {
+  uint32_t a, b;
+  f2_to(v, a, b);
+  return __uint_as_float(a);
+}
+__device__ __forceinline__ float f2_sum(unsigned long long v) {
+  uint32_t a, b;
+  f2_to(v, a, b);
+  return __uint_as_float(a) + __uint_as_float(b);
+}
 
 // Zeros in place of rows `from` .. 127 of a tile of 128 rows of HD values that a TMA load has left in shared memory (a row is 128 bytes of each
 // slab of 64 columns, however its pieces are swizzled)
@@ -508,6 +521,7 @@ struct PackedBwdParams {
   float scale;
   const float* lse;      // [q_heads, tokens]
   const float* delta;    // [q_heads, tokens]  sum_d dO * O
+  float* rest;           // [2][q_heads, tokens]  what the sums of dS say is missing from it, times scale
   __nv_bfloat16 *dq, *dk, *dv;
   long long dq_stride, dk_stride, dv_stride;
   int* status;
@@ -632,6 +646,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   if (warp == 10) {
     // ------------- TMA producer (also stages the per-query statistics of each block)
     uint32_t itc = 0, qc = 0;       // items and Q / dO blocks loaded so far
+    const long long all = (long long)p.q_heads * p.plan.tokens;
     bool ok = true;
     while (ok && walk.next(entry, which)) {
       const PackedKvItem it(entry, which);
@@ -677,7 +692,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
               const int qi = qrow + lane * 4 + u;
               const bool okq = qi < it.hi;
               nlp[u] = okq ? -p.lse[stat_base + qi] * LOG2E : -INFINITY;
-              ndp[u] = okq ? -p.delta[stat_base + qi] * p.scale : 0.f;
+              ndp[u] = okq ? -fmaf(p.delta[stat_base + qi], p.scale, p.rest[stat_base + qi] + p.rest[all + stat_base + qi]) : 0.f;
             }
             float* dst = stat + st * 256;
             reinterpret_cast<float4*>(dst)[lane] = nl;
@@ -941,13 +956,19 @@ struct PackedQCfg {
   static constexpr int OFF_V = OFF_K + NK * T_BYTES;
   static constexpr int OFF_BAR = OFF_V + NV * T_BYTES;
   static constexpr int OFF_ITEMS = OFF_BAR + 272;
-  static constexpr int SMEM_BYTES = OFF_ITEMS + PACKED_ROUNDS * 16;
+  static constexpr int OFF_X = OFF_ITEMS + PACKED_ROUNDS * 16;   // float[2 halves][128 rows]
+  static constexpr int SMEM_BYTES = OFF_X + 2 * FA_BM * 4;
   static constexpr int TMEM_COLS = 512;
-  static constexpr int TM_S = 0, TM_DP = 256, TM_DQ = 384;   // two score buffers; dS over dP
+  static constexpr int TM_S = 0, TM_DP = FA_BN, TM_DQ = 3 * FA_BN;   // two buffers of dP, dS over it: 32 columns of each half, its remainder in the next 32
 };
 
 // Items are (tile of queries, query head), the longest rows first; dQ of an item accumulates in TMEM over its key blocks.  P is needed in registers only, so
-// a score buffer is free once it has been read.
+// the one score buffer is free once it has been read; dP has two, so that the next tile's is formed while this one's becomes dS and a product (with two buffers
+// of scores and one of dP, dP -> dS -> dQ -> the next dP stood one behind the other).
+// delta comes from the rounded output of weights that were rounded: what it is off by adds the same multiple of p_ij to a whole row of dS, and rounding dS to bf16
+// adds as much again.  Together 1.6 to 2 times the rounding of the result itself.  So dS goes to the products as two bf16 numbers, its rounding and what that
+// leaves; the rows' sums of dS, which are 0 for the right delta, go to the dK / dV kernel, which then has the right one; and where a row has one block of
+// keys, the right one is there before dS is (shorter rows suffer most).
 template <int HD>
 __global__ void __launch_bounds__(PB_THREADS, 1)
 packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -962,14 +983,14 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint64_t* k_empty = bars + 6;    // [4]  dQ has read K
   uint64_t* v_full = bars + 10;    // [3]
   uint64_t* v_empty = bars + 13;   // [3]
-  uint64_t* s_full = bars + 16;    // [2]
-  uint64_t* s_empty = bars + 18;   // [2]  (8 warps)
-  uint64_t* dp_full = bars + 20;
-  uint64_t* ds_full = bars + 21;   // [2]  by column half (4 warps each)
-  uint64_t* fin_full = bars + 23;
-  uint64_t* k_part = bars + 24;    // [4]  K, V of a sequence's last block are there, and some rows of others
-  uint64_t* v_part = bars + 28;    // [3]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
+  uint64_t* s_full = bars + 16;
+  uint64_t* s_empty = bars + 17;   // (8 warps)
+  uint64_t* dp_full = bars + 18;   // [2]
+  uint64_t* ds_full = bars + 20;   // [2][2]  by buffer and column half (4 warps each)
+  uint64_t* fin_full = bars + 24;
+  uint64_t* k_part = bars + 25;    // [4]  K, V of a sequence's last block are there, and some rows of others
+  uint64_t* v_part = bars + 29;    // [3]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 32);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -982,8 +1003,10 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     mbar_init(q_empty, 2);
     for (int s = 0; s < NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
     for (int s = 0; s < NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&s_empty[s], 8); mbar_init(&ds_full[s], 4); }
-    mbar_init(dp_full, 1);
+    mbar_init(s_full, 1);
+    mbar_init(s_empty, 8);
+    for (int s = 0; s < 2; ++s) mbar_init(&dp_full[s], 1);
+    for (int s = 0; s < 4; ++s) mbar_init(&ds_full[s], 4);
     mbar_init(fin_full, 1);
     for (int s = 0; s < NK; ++s) mbar_init(&k_part[s], 1);
     for (int s = 0; s < NV; ++s) mbar_init(&v_part[s], 1);
@@ -1069,16 +1092,16 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       for (int j = 0; j < n_kv; ++j, ++kc) {
         const int st = kc % NK;
         if (!warp_wait(&k_full[st], (kc / NK) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-        if (kc > 1 && !warp_wait(&s_empty[kc & 1], ((kc >> 1) - 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); ok = false; break; }
+        if (kc > 0 && !warp_wait(s_empty, (kc - 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); ok = false; break; }
         tc_fence_after();
         if (elect_one()) {
           const uint64_t kd = desc_at(k_desc, st * Cfg::T_BYTES);
 #pragma unroll
           for (int ks = 0; ks < HD / 16; ++ks) {
             const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
-            umma_f16(tmem_base + Cfg::TM_S + (kc & 1) * FA_BN, desc_at(q_desc, off), desc_at(kd, off), idesc_s, ks > 0 ? 1u : 0u);
+            umma_f16(tmem_base + Cfg::TM_S, desc_at(q_desc, off), desc_at(kd, off), idesc_s, ks > 0 ? 1u : 0u);
           }
-          umma_commit(&s_full[kc & 1]);
+          umma_commit(s_full);
           if (j + 1 == n_kv) umma_commit(q_empty);
         }
         __syncwarp();
@@ -1090,7 +1113,6 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     constexpr uint32_t idesc_s = umma_idesc_bf16(FA_BM, FA_BN, 0, 0);
     constexpr uint32_t idesc_q = umma_idesc_bf16(FA_BM, HD, 0, 1);   // dQ[q x HD] += dS[q x keys] * K[keys x HD]
     const uint64_t do_desc = desc_k(smem + Cfg::OFF_DO), v_desc = desc_k(smem + Cfg::OFF_V), k_desc = desc_mn(smem + Cfg::OFF_K);
-    const uint32_t dp_tm = tmem_base + Cfg::TM_DP;
     uint32_t itc = 0, kc = 0;
     bool ok = true;
     auto issue_dp = [&](uint32_t n, bool last) -> bool {
@@ -1102,9 +1124,9 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks) {
           const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
-          umma_f16(dp_tm, desc_at(do_desc, off), desc_at(vd, off), idesc_s, ks > 0 ? 1u : 0u);
+          umma_f16(tmem_base + Cfg::TM_DP + (n & 1) * FA_BN, desc_at(do_desc, off), desc_at(vd, off), idesc_s, ks > 0 ? 1u : 0u);
         }
-        umma_commit(dp_full);
+        umma_commit(&dp_full[n & 1]);
         umma_commit(&v_empty[st]);
         if (last) umma_commit(q_empty);
       }
@@ -1115,19 +1137,22 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       const int n_kv = entry.z + 1;
       if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
       ok = issue_dp(kc, n_kv == 1);
+      if (ok && n_kv > 1) ok = issue_dp(kc + 1, n_kv == 2);
       for (int j = 0; j < n_kv && ok; ++j, ++kc) {
         const int st = kc % NK;
         if (!warp_wait(&k_full[st], (kc / NK) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
         const uint64_t kd = desc_at(k_desc, st * Cfg::T_BYTES);
+        const uint32_t ds_tm = tmem_base + Cfg::TM_DP + (kc & 1) * FA_BN;
+        uint64_t* ready = ds_full + (kc & 1) * 2;
         for (int half = 0; half < 2; ++half) {
           // an item's first product replaces the accumulator: wait until both halves' warps have read the previous item's
-          if (j == 0 && half == 0) ok = warp_wait(&ds_full[1], kc & 1);
-          if (!ok || !warp_wait(&ds_full[half], kc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
+          if (j == 0 && half == 0) ok = warp_wait(&ready[1], (kc >> 1) & 1);
+          if (!ok || !warp_wait(&ready[half], (kc >> 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              umma_f16_ts(tmem_base + Cfg::TM_DQ, dp_tm + half * 64 + ks * 8, desc_at(kd, (half * 4 + ks) * 2048),
+            for (int ks = 0; ks < 8; ++ks)           // dS, then its remainder
+              umma_f16_ts(tmem_base + Cfg::TM_DQ, ds_tm + half * 64 + ks * 8, desc_at(kd, (half * 4 + (ks & 3)) * 2048),
                           idesc_q, (j > 0 || half > 0 || ks > 0) ? 1u : 0u);
             if (half == 1) {
               umma_commit(&k_empty[st]);
@@ -1137,7 +1162,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           __syncwarp();
         }
         if (!ok) break;
-        if (j + 1 < n_kv) ok = issue_dp(kc + 1, j + 2 == n_kv);
+        if (j + 2 < n_kv) ok = issue_dp(kc + 2, j + 3 == n_kv);      // over dS_j: ordered after its product by the pipe
       }
       ++itc;
     }
@@ -1149,25 +1174,26 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const unsigned long long sl22 = f2_splat(p.scale * LOG2E), scale2 = f2_splat(p.scale);
     uint32_t itc = 0, kc = 0;
     bool ok = true;
+    float* xch = reinterpret_cast<float*>(smem + Cfg::OFF_X);
     clear_others(p.plan, p.dq, p.dq_stride, p.q_heads * HD, threadIdx.x, 256);
     while (ok && walk.next(entry, which)) {
       const int hi = entry.y, n_kv = entry.z + 1, h = which, q0 = entry.x + entry.z * FA_BM + quad * 32, qi = q0 + lane;
       const long long stat_at = (long long)h * p.plan.tokens + qi;
       const unsigned long long nlse2 = f2_splat(qi < hi ? -p.lse[stat_at] * LOG2E : -INFINITY);
-      const unsigned long long ndlt2 = f2_splat(qi < hi ? -p.delta[stat_at] * p.scale : 0.f);
+      unsigned long long ndlt2 = f2_splat(qi < hi ? -p.delta[stat_at] * p.scale : 0.f), sum2 = 0;
       for (int j = 0; j < n_kv; ++j, ++kc) {
-        ok = warp_wait(&s_full[kc & 1], (kc >> 1) & 1);
+        ok = warp_wait(s_full, kc & 1);
         if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
         tc_fence_after();
-        const uint32_t s_addr = t_lane + Cfg::TM_S + (kc & 1) * FA_BN + half * 64;
-        const uint32_t dp_addr = t_lane + Cfg::TM_DP + half * 64;
+        const uint32_t s_addr = t_lane + Cfg::TM_S + half * 64;
+        const uint32_t dp_addr = t_lane + Cfg::TM_DP + (kc & 1) * FA_BN + half * 64;
         uint32_t s[64];
         tmem_ld32(s_addr, s);
         tmem_ld32(s_addr + 32, s + 32);
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[kc & 1]);
+        if (lane == 0) mbar_arrive(s_empty);
 #pragma unroll
         for (int i = 0; i < 64; i += 4) {
           bwd_prob2(s[i], s[i + 1], sl22, nlse2);
@@ -1179,29 +1205,52 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll
           for (int i = 0; i < 64; ++i) s[i] = (i <= lim) ? s[i] : 0u;
         }
-        ok = warp_wait(dp_full, kc & 1);
+        ok = warp_wait(&dp_full[kc & 1], (kc >> 1) & 1);
         if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
         tc_fence_after();
         uint32_t dp[64];
         tmem_ld32(dp_addr, dp);
         tmem_ld32(dp_addr + 32, dp + 32);
         tmem_ld_wait();
+        if (n_kv == 1) {                           // the whole row is here: delta is its sum of p dP
+          unsigned long long mine2 = 0;
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) mine2 = f2_fma(f2_of(s[i], s[i + 1]), f2_of(dp[i], dp[i + 1]), mine2);
+          xch[half * FA_BM + r] = f2_sum(mine2);
+          row_sync(quad);
+          ndlt2 = f2_splat(-(xch[r] + xch[FA_BM + r]) * p.scale);
+          row_sync(quad);                          // may be written over
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+          uint32_t w[16], rest[16];
 #pragma unroll
-          for (int i = c * 32; i < c * 32 + 32; i += 2) bwd_ds2(s[i], s[i + 1], dp[i], dp[i + 1], scale2, ndlt2);
-          bwd_store16(dp_addr + c * 16, s + c * 32);
+          for (int i = 0; i < 16; ++i) {
+            uint32_t *a = s + c * 32 + 2 * i, *b = dp + c * 32 + 2 * i;
+            bwd_ds2(a[0], a[1], b[0], b[1], scale2, ndlt2);
+            const unsigned long long ds = f2_of(a[0], a[1]);
+            sum2 = f2_add(sum2, ds);
+            w[i] = f2_bf16(ds);
+            rest[i] = f2_bf16(f2_fma(f2_bf16x2(w[i]), f2_splat(-1.f), ds));
+          }
+          tmem_st16(dp_addr + c * 16, w);
+          tmem_st16(dp_addr + 32 + c * 16, rest);
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ds_full[half]);
+        if (lane == 0) mbar_arrive(&ds_full[(kc & 1) * 2 + half]);
       }
       if (!ok) break;
       ok = warp_wait(fin_full, itc & 1);
       if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
       ++itc;
       tc_fence_after();
+      if (qi < hi) {
+        // with a delta of this kernel's own: what the other kernel's is off by, once
+        const float own = n_kv == 1 && half == 0 ? -(lo_of(ndlt2) + p.delta[stat_at] * p.scale) : 0.f;
+        p.rest[half * (long long)p.q_heads * p.plan.tokens + stat_at] = f2_sum(sum2) + own;
+      }
       __nv_bfloat16* base = p.dq + q0 * p.dq_stride + h * HD + half * (HD / 2);
       uint32_t a[HD / 2];
 #pragma unroll
@@ -1250,8 +1299,9 @@ static int packed_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
   if (allow_smem(allowed_kv, (const void*)packed_bwd_kv_kernel<HD>, PackedKvCfg<HD>::SMEM_BYTES) != cudaSuccess) return OA_ERR_LAUNCH;
   if (allow_smem(allowed_q, (const void*)packed_bwd_q_kernel<HD>, PackedQCfg<HD>::SMEM_BYTES) != cudaSuccess) return OA_ERR_LAUNCH;
   const long long tiles = packed_max_tiles(p.plan.tokens, p.plan.batch);
-  launch_pdl_if(pdl_on(true), packed_bwd_kv_kernel<HD>, dim3(packed_ctas(tiles * p.kv_heads)), dim3(PB_THREADS), PackedKvCfg<HD>::SMEM_BYTES, st, tq, tk, tv, tdo, p);
-  launch_pdl(packed_bwd_q_kernel<HD>, dim3(packed_ctas(tiles * p.q_heads)), dim3(PB_THREADS), PackedQCfg<HD>::SMEM_BYTES, st, tq, tk, tv, tdo, p);
+  // dQ first: it works out what delta is off by.  It starts under the launch for short sequences, which is over at once where there are none
+  launch_pdl_if(pdl_on(true), packed_bwd_q_kernel<HD>, dim3(packed_ctas(tiles * p.q_heads)), dim3(PB_THREADS), PackedQCfg<HD>::SMEM_BYTES, st, tq, tk, tv, tdo, p);
+  launch_pdl(packed_bwd_kv_kernel<HD>, dim3(packed_ctas(tiles * p.kv_heads)), dim3(PB_THREADS), PackedKvCfg<HD>::SMEM_BYTES, st, tq, tk, tv, tdo, p);
   return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }
 
@@ -1281,10 +1331,10 @@ extern "C" int oa_packed_attn(const void* q, const void* k, const void* v, const
   return head_dim == 64 ? packed_fwd<64, false>(tq, tk, tv, p, st) : packed_fwd<128, false>(tq, tk, tv, p, st);
 }
 
-// scratch: float[q_heads, tokens] for delta
+// scratch: float[3][q_heads, tokens], delta and what is missing from it
 extern "C" size_t oa_packed_attn_bwd_scratch_bytes(int tokens, int batch, int q_heads, int kv_heads, int head_dim) {
   (void)batch; (void)kv_heads; (void)head_dim;
-  return (size_t)q_heads * tokens * sizeof(float);
+  return 3 * (size_t)q_heads * tokens * sizeof(float);
 }
 
 extern "C" int oa_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, const int* plan, void* dq,
@@ -1309,9 +1359,9 @@ extern "C" int oa_packed_attn_bwd(const void* q, const void* k, const void* v, c
   const long long threads = (long long)tokens * q_heads * (head_dim / 8);
   launch_pdl(packed_delta_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout,
              (float*)scratch, tokens, q_heads, head_dim, o_stride, do_stride);
-  const PackedBwdParams p{{plan, batch, tokens}, q_heads, kv_heads, q_heads / kv_heads, scale, lse, (const float*)scratch, (__nv_bfloat16*)dq,
+  const PackedBwdParams p{{plan, batch, tokens}, q_heads, kv_heads, q_heads / kv_heads, scale, lse, (const float*)scratch, (float*)scratch + (size_t)q_heads * tokens, (__nv_bfloat16*)dq,
                           (__nv_bfloat16*)dk, (__nv_bfloat16*)dv, dq_stride, dk_stride, dv_stride, status};
-  const PackedShortBwd brief{p.plan, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (const __nv_bfloat16*)dout, lse, p.delta, p.dq, p.dk, p.dv,
+  const PackedShortBwd brief{p.plan, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (const __nv_bfloat16*)dout, lse, p.dq, p.dk, p.dv,
                              q_stride, k_stride, v_stride, do_stride, dq_stride, dk_stride, dv_stride, kv_heads, p.group, scale};
   if ((rc = packed_short_bwd(brief, head_dim, st))) return rc;
   return head_dim == 64 ? packed_bwd<64>(tq, tk, tv, tdo, p, st) : packed_bwd<128>(tq, tk, tv, tdo, p, st);

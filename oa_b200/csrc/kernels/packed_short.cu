@@ -279,11 +279,10 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
       Tile::fetch(sk, p.ks, e.n, e.tiles, e.heads, [&](int u) { return k + u * HD; });
       Tile::fetch(sk + Tile::BYTES, p.vs, e.n, e.tiles, e.heads, [&](int u) { return v + u * HD; });
     }
-    const int row = threadIdx.x & (PACKED_SHORT - 1), v = e.tiles == 1 ? row >> 4 : e.tiles == 2 ? row >> 5 : 0, in = row - v * e.tiles * 16;
-    if (v < e.heads) {
-      const float* from = threadIdx.x < PACKED_SHORT ? p.lse : p.delta;
+    const int row = threadIdx.x, v = e.tiles == 1 ? row >> 4 : e.tiles == 2 ? row >> 5 : 0, in = row - v * e.tiles * 16;
+    if (row < PACKED_SHORT && v < e.heads) {
       const long long at = (long long)((e.head + v) * p.group + g) * p.plan.tokens + e.lo;
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(stats + stage * 2 * PACKED_SHORT + threadIdx.x)), "l"(from + at + (in < e.n ? in : 0)), "r"(in < e.n ? 4 : 0) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(stats + stage * 2 * PACKED_SHORT + row)), "l"(p.lse + at + (in < e.n ? in : 0)), "r"(in < e.n ? 4 : 0) : "memory");
     }
   };
   ShortWalk walk(p.plan, p.kv_heads);
@@ -309,7 +308,7 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
     }
     __syncthreads();
     const uint32_t sq = stages + stage * 2 * Tile::BYTES, sdo = sq + Tile::BYTES, sk = kv_stages + kv_stage * 2 * Tile::BYTES, sv = sk + Tile::BYTES;
-    const float* stat = stats + stage * 2 * PACKED_SHORT;
+    float* stat = stats + stage * 2 * PACKED_SHORT;                      // log-sum-exp, and delta from this kernel
     const int n = e.n, u = e.tiles == 1 ? warp : e.tiles == 2 ? warp >> 1 : 0, tile = warp - u * e.tiles, base = u * e.tiles * 16, r0 = base + tile * 16;
     const bool mine_too = u < e.heads && tile < e.tiles;
     const long long row0 = e.lo + tile * 16;
@@ -323,8 +322,66 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
     if (mine_too) {
       constexpr int STEP = 16 * Tile::STRIDE;
       const uint32_t mine = r0 * Tile::STRIDE, all = base * Tile::STRIDE;
-      // keys as rows: P^T and dS^T, for the queries from them on
+      const int j0 = tile * 16 + (lane >> 2), j1 = j0 + 8;                // this thread's queries, then its keys
+      // queries as rows: dS, for the keys up to them
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) dq[c][0] = dq[c][1] = dq[c][2] = dq[c][3] = 0.f;
+      const float nl0 = -stat[base + j0] * PS_LOG2E, nl1 = -stat[base + j1] * PS_LOG2E;
+      // delta = sum p dP, in 32 bits; from the rounded output it would be off by as much as everything else together
+      float nd0 = 0.f, nd1 = 0.f;
+#pragma unroll 1
+      for (int t = 0; t <= tile; ++t) {
+        float s[2][4], dp[2][4];
+        short_scores<HD>(s, sq + mine + rows_at, sk + all + t * STEP + columns_at);
+        short_scores<HD>(dp, sdo + mine + rows_at, sv + all + t * STEP + columns_at);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int j = t * 16 + c * 8 + (lane & 3) * 2 + x;
+            nd0 -= j <= j0 ? fast_exp2(fmaf(s[c][x], sl2, nl0)) * dp[c][x] : 0.f;
+            nd1 -= j <= j1 ? fast_exp2(fmaf(s[c][2 + x], sl2, nl1)) * dp[c][2 + x] : 0.f;
+          }
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        nd0 += __shfl_xor_sync(0xffffffffu, nd0, o);
+        nd1 += __shfl_xor_sync(0xffffffffu, nd1, o);
+      }
+      nd0 *= scale;
+      nd1 *= scale;
+      if ((lane & 3) == 0) {
+        stat[PACKED_SHORT + base + j0] = nd0;
+        stat[PACKED_SHORT + base + j1] = nd1;
+      }
+#pragma unroll 1
+      for (int t = 0; t <= tile; ++t) {
+        float s[2][4], dp[2][4];
+        short_scores<HD>(s, sq + mine + rows_at, sk + all + t * STEP + columns_at);
+        short_scores<HD>(dp, sdo + mine + rows_at, sv + all + t * STEP + columns_at);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            dp[c][x] = fast_exp2(fmaf(s[c][x], sl2, nl0)) * fmaf(dp[c][x], scale, nd0);
+            dp[c][2 + x] = fast_exp2(fmaf(s[c][2 + x], sl2, nl1)) * fmaf(dp[c][2 + x], scale, nd1);
+            if (t == tile) {
+              const int j = t * 16 + c * 8 + (lane & 3) * 2 + x;
+              dp[c][x] = j <= j0 ? dp[c][x] : 0.f;
+              dp[c][2 + x] = j <= j1 ? dp[c][2 + x] : 0.f;
+            }
+          }
+        uint32_t w[4];
+        short_operand(w, dp);
+        short_weigh<HD>(dq, w, sk + all + t * STEP + rows_at);
+      }
+    }
+    __syncthreads();                                                   // delta of every query
+    if (mine_too) {
+      constexpr int STEP = 16 * Tile::STRIDE;
+      const uint32_t mine = r0 * Tile::STRIDE, all = base * Tile::STRIDE;
       const int j0 = tile * 16 + (lane >> 2), j1 = j0 + 8;
+      // keys as rows: P^T and dS^T, for the queries from them on
 #pragma unroll 1
       for (int t = tile; t < e.tiles; ++t) {
         float s[2][4], dp[2][4];
@@ -334,7 +391,7 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
         for (int c = 0; c < 2; ++c) {
           const int i = t * 16 + c * 8 + (lane & 3) * 2;
           const float2 L = *reinterpret_cast<const float2*>(stat + base + i), D = *reinterpret_cast<const float2*>(stat + PACKED_SHORT + base + i);
-            const float2 nl = make_float2(-L.x * PS_LOG2E, -L.y * PS_LOG2E), nd = make_float2(-D.x * scale, -D.y * scale);
+            const float2 nl = make_float2(-L.x * PS_LOG2E, -L.y * PS_LOG2E), nd = D;
           s[c][0] = fast_exp2(fmaf(s[c][0], sl2, nl.x));
           s[c][1] = fast_exp2(fmaf(s[c][1], sl2, nl.y));
           s[c][2] = fast_exp2(fmaf(s[c][2], sl2, nl.x));
@@ -359,32 +416,6 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
         short_weigh<HD>(dv, w, sdo + all + t * STEP + rows_at);
         short_operand(w, dp);
         short_weigh<HD>(dk, w, sq + all + t * STEP + rows_at);
-      }
-      // queries as rows: dS, for the keys up to them
-#pragma unroll
-      for (int c = 0; c < HD / 8; ++c) dq[c][0] = dq[c][1] = dq[c][2] = dq[c][3] = 0.f;
-      const float nl0 = -stat[base + j0] * PS_LOG2E, nl1 = -stat[base + j1] * PS_LOG2E;
-      const float nd0 = -stat[PACKED_SHORT + base + j0] * scale, nd1 = -stat[PACKED_SHORT + base + j1] * scale;
-#pragma unroll 1
-      for (int t = 0; t <= tile; ++t) {
-        float s[2][4], dp[2][4];
-        short_scores<HD>(s, sq + mine + rows_at, sk + all + t * STEP + columns_at);
-        short_scores<HD>(dp, sdo + mine + rows_at, sv + all + t * STEP + columns_at);
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            dp[c][x] = fast_exp2(fmaf(s[c][x], sl2, nl0)) * fmaf(dp[c][x], scale, nd0);
-            dp[c][2 + x] = fast_exp2(fmaf(s[c][2 + x], sl2, nl1)) * fmaf(dp[c][2 + x], scale, nd1);
-            if (t == tile) {
-              const int j = t * 16 + c * 8 + (lane & 3) * 2 + x;
-              dp[c][x] = j <= j0 ? dp[c][x] : 0.f;
-              dp[c][2 + x] = j <= j1 ? dp[c][2 + x] : 0.f;
-            }
-          }
-        uint32_t w[4];
-        short_operand(w, dp);
-        short_weigh<HD>(dq, w, sk + all + t * STEP + rows_at);
       }
     }
     __syncthreads();                                                   // every warp has read what it needs of these rows

@@ -18,7 +18,7 @@ struct PackedShortFwd {
 struct PackedShortBwd {
   PackedPlan plan;
   const __nv_bfloat16 *q, *k, *v, *dout;
-  const float *lse, *delta;                // [q_heads, tokens]
+  const float* lse;                        // [q_heads, tokens]
   __nv_bfloat16 *dq, *dk, *dv;
   long long qs, ks, vs, dos, dqs, dks, dvs;
   int kv_heads, group;

@@ -521,7 +521,7 @@ struct PackedBwdParams {
   float scale;
   const float* lse;      // [q_heads, tokens]
   const float* delta;    // [q_heads, tokens]  sum_d dO * O
-  float* rest;           // [2][q_heads, tokens]  what the sums of dS say is missing from it, times scale
+  float* ndelta;         // [q_heads, tokens]  -scale times the delta that the rows' sums of dS lead to
   __nv_bfloat16 *dq, *dk, *dv;
   long long dq_stride, dk_stride, dv_stride;
   int* status;
@@ -554,7 +554,7 @@ packed_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __
   if (item < total && sub == 0) delta[(long long)h * tokens + row] = s;
 }
 
-constexpr int PB_THREADS = 384;   // 8 softmax warps, 2 MMA issuer warps, a TMA warp and one that clears rows
+constexpr int PB_THREADS = 384;   // 8 softmax warps, 2 MMA issuer warps, a TMA warp and one that clears rows and stages statistics
 // Of eight pairs of exponentials, those on the multiply-add pipe (flash_attn.cu)
 template <int HD> constexpr int PB_FMA_PAIRS = HD == 64 ? 2 : 1;
 
@@ -644,9 +644,8 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   int which;
 
   if (warp == 10) {
-    // ------------- TMA producer (also stages the per-query statistics of each block)
+    // ------------- TMA producer
     uint32_t itc = 0, qc = 0;       // items and Q / dO blocks loaded so far
-    const long long all = (long long)p.q_heads * p.plan.tokens;
     bool ok = true;
     while (ok && walk.next(entry, which)) {
       const PackedKvItem it(entry, which);
@@ -661,7 +660,6 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       for (int g = 0; g < p.group && ok; ++g) {
         const int h = it.kv_head * p.group + g;
-        const long long stat_base = (long long)h * p.plan.tokens;
         for (int i = 0; i < it.blocks; ++i, ++qc) {
           const int st = qc % NST;
           const uint32_t ph = (qc / NST) & 1;
@@ -682,47 +680,47 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
             for (int x = 0; x < HD / 64; ++x) tma_load_2d(do_tile + x * (FA_BM * 128), &tmDO, bar, h * HD + x * 64, qrow);
           }
-          // per-query statistics of this block, negated and pre-scaled: lane l stages queries 4l .. 4l+3
-          {
-            float4 nl, nd;
-            float* nlp = reinterpret_cast<float*>(&nl);
-            float* ndp = reinterpret_cast<float*>(&nd);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int qi = qrow + lane * 4 + u;
-              const bool okq = qi < it.hi;
-              nlp[u] = okq ? -p.lse[stat_base + qi] * LOG2E : -INFINITY;
-              ndp[u] = okq ? -fmaf(p.delta[stat_base + qi], p.scale, p.rest[stat_base + qi] + p.rest[all + stat_base + qi]) : 0.f;
-            }
-            float* dst = stat + st * 256;
-            reinterpret_cast<float4*>(dst)[lane] = nl;
-            reinterpret_cast<float4*>(dst + 128)[lane] = nd;
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&q_full[st]);
           __syncwarp();
         }
       }
       ++itc;
     }
   } else if (warp == 11) {
-    // ------------- zeros in place of rows behind a sequence, which only a head's last block can have
+    // ------------- the per-query statistics of each block, and zeros in place of rows behind a sequence, which only a head's last block can have
     uint32_t qc = 0, phases = 0;
     bool ok = true;
     while (ok && walk.next(entry, which)) {
       const PackedKvItem it(entry, which);
-      const int qrow = it.lo + it.key0 + (it.blocks - 1) * FA_BM;
-      if (qrow + FA_BM <= it.hi) { qc += it.blocks * p.group; continue; }
-      for (int g = 0; g < p.group; ++g) {
-        qc += it.blocks;
-        const int st = (qc - 1) % NST;
-        if (!warp_wait(&part_full[st], (phases >> st) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-        phases ^= 1u << st;
-        clear_rows<HD>(smem + Cfg::OFF_Q + st * Cfg::T_BYTES, it.hi - qrow, lane);
-        clear_rows<HD>(smem + Cfg::OFF_DO + st * Cfg::T_BYTES, it.hi - qrow, lane);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) { mbar_arrive(&q_full[st]); mbar_arrive(&do_full[st]); }
+      for (int g = 0; g < p.group && ok; ++g) {
+        const long long stat_base = (long long)(it.kv_head * p.group + g) * p.plan.tokens;
+        for (int i = 0; i < it.blocks; ++i, ++qc) {
+          const int st = qc % NST, qrow = it.lo + it.key0 + i * FA_BM;
+          // lane l stages queries 4l .. 4l+3; sent for before their place is free
+          float4 nl, nd;
+          float* nlp = reinterpret_cast<float*>(&nl);
+          float* ndp = reinterpret_cast<float*>(&nd);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int qi = qrow + lane * 4 + u;
+            const bool okq = qi < it.hi;
+            nlp[u] = okq ? -p.lse[stat_base + qi] * LOG2E : -INFINITY;
+            ndp[u] = okq ? p.ndelta[stat_base + qi] : 0.f;
+          }
+          if (!warp_wait(&q_empty[st], ((qc / NST) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
+          float* dst = stat + st * 256;
+          reinterpret_cast<float4*>(dst)[lane] = nl;
+          reinterpret_cast<float4*>(dst + 128)[lane] = nd;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_full[st]);
+          if (qrow + FA_BM <= it.hi) continue;
+          if (!warp_wait(&part_full[st], (phases >> st) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+          phases ^= 1u << st;
+          clear_rows<HD>(smem + Cfg::OFF_Q + st * Cfg::T_BYTES, it.hi - qrow, lane);
+          clear_rows<HD>(smem + Cfg::OFF_DO + st * Cfg::T_BYTES, it.hi - qrow, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) { mbar_arrive(&q_full[st]); mbar_arrive(&do_full[st]); }
+        }
       }
     }
   } else if (warp == 8) {
@@ -1246,11 +1244,10 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
       ++itc;
       tc_fence_after();
-      if (qi < hi) {
-        // with a delta of this kernel's own: what the other kernel's is off by, once
-        const float own = n_kv == 1 && half == 0 ? -(lo_of(ndlt2) + p.delta[stat_at] * p.scale) : 0.f;
-        p.rest[half * (long long)p.q_heads * p.plan.tokens + stat_at] = f2_sum(sum2) + own;
-      }
+      if (half == 1) xch[FA_BM + r] = f2_sum(sum2);
+      row_sync(quad);
+      if (half == 0 && qi < hi) p.ndelta[stat_at] = lo_of(ndlt2) - (f2_sum(sum2) + xch[FA_BM + r]);
+      row_sync(quad);                              // may be written over
       __nv_bfloat16* base = p.dq + q0 * p.dq_stride + h * HD + half * (HD / 2);
       uint32_t a[HD / 2];
 #pragma unroll
@@ -1331,10 +1328,10 @@ extern "C" int oa_packed_attn(const void* q, const void* k, const void* v, const
   return head_dim == 64 ? packed_fwd<64, false>(tq, tk, tv, p, st) : packed_fwd<128, false>(tq, tk, tv, p, st);
 }
 
-// scratch: float[3][q_heads, tokens], delta and what is missing from it
+// scratch: float[2][q_heads, tokens], delta from the output and from the rows' sums
 extern "C" size_t oa_packed_attn_bwd_scratch_bytes(int tokens, int batch, int q_heads, int kv_heads, int head_dim) {
   (void)batch; (void)kv_heads; (void)head_dim;
-  return 3 * (size_t)q_heads * tokens * sizeof(float);
+  return 2 * (size_t)q_heads * tokens * sizeof(float);
 }
 
 extern "C" int oa_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, const int* plan, void* dq,

@@ -355,11 +355,11 @@ __global__ void __launch_bounds__(THREADS == 128 ? 128 : 256, THREADS == 128 ? 8
   LpSums a{-INFINITY, 0.f, 0.f};
   float tmax = -INFINITY;                  // of the logits themselves
   const u64 scale2 = f2_splat(p.scale);
-  for (int q = p0 + tid; q < p1; q += LP_BATCH * THREADS) {
-    LpPiece<T> v[LP_BATCH];
+  LpPiece<T> v[LP_BATCH];
 #pragma unroll
-    for (int b = 0; b < LP_BATCH; ++b)
-      if (q + b * THREADS < p1) row.load(v[b], q + b * THREADS);
+  for (int b = 0; b < LP_BATCH; ++b)
+    if (p0 + tid + b * THREADS < p1) row.load(v[b], p0 + tid + b * THREADS);
+  for (int q = p0 + tid; q < p1; q += LP_BATCH * THREADS) {
 #pragma unroll
     for (int b = 0; b < LP_BATCH; ++b)
       if (q + b * THREADS < p1) tmax = fmaxf(tmax, v[b].largest());
@@ -369,13 +369,20 @@ __global__ void __launch_bounds__(THREADS == 128 ? 128 : 256, THREADS == 128 ? 8
     u64 l2 = 0, s2 = 0;
 #pragma unroll
     for (int b = 0; b < LP_BATCH; ++b)
-      if (q + b * THREADS < p1) lp_add<false>(v[b], scale2, neg_m2, l2, s2);
+      if (q + b * THREADS < p1) {
+        lp_add<false>(v[b], scale2, neg_m2, l2, s2);
+        const int next = q + (LP_BATCH + b) * THREADS;      // the place that is free again takes the next step's piece
+        if (next < p1) row.load(v[b], next);
+      }
     float s1 = lp_both(s2);
     if (s1 != s1) {
       l2 = s2 = 0;
-#pragma unroll
-      for (int b = 0; b < LP_BATCH; ++b)
-        if (q + b * THREADS < p1) lp_add<true>(v[b], scale2, neg_m2, l2, s2);
+#pragma unroll 1
+      for (int i = q; i < p1 && i < q + LP_BATCH * THREADS; i += THREADS) {
+        LpPiece<T> again;
+        row.load(again, i);
+        lp_add<true>(again, scale2, neg_m2, l2, s2);
+      }
       s1 = lp_both(s2);
     }
     a.l += lp_both(l2);

@@ -65,29 +65,36 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedP
     if (tid == PLAN_THREADS - 1) s_top = s;
   }
   __syncthreads();
-  // Each warp takes 32 sequences: the first bin of all at once, the others of one sequence after the other, a bin to a lane.
+  // `team` warps to 32 sequences: the first of them takes the first bin of all at once, each the other bins of its share, one sequence after the other, a bin
+  // to a lane.
   // add(which, bin, n) is called for n indices of a bin, returns where they go; put(which, at, first index, n) follows
+  int team = 1;
+  while (team < 32 && team * p.batch <= 16 * 32) team *= 2;
+  const int sub = (tid >> 5) & (team - 1);
   const auto walk = [&](auto add, auto put) {
-    for (int b0 = tid - lane; b0 < p.batch; b0 += PLAN_THREADS) {
+    for (int b0 = (tid >> 5) / team * 32; b0 < p.batch; b0 += PLAN_THREADS / team) {
       const int b = b0 + lane;
       const int lo = b < p.batch ? starts[b] : 0, hi = b < p.batch ? starts[b + 1] : 0;
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         const int rows = PACKED_TILE << which;
         const int n = hi - lo <= PACKED_SHORT ? 0 : (hi - lo + rows - 1) / rows, head = min(n, per);
-        int sum = head;
+        if (sub == 0) {
+          int sum = head;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int u = __shfl_up_sync(0xffffffffu, sum, o);
-          if (lane >= o) sum += u;
+          for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += u;
+          }
+          int base = lane == 31 ? add(which, 0, sum) : 0;
+          base = __shfl_sync(0xffffffffu, base, 31);
+          put(which, base + sum - head, 0, head, lo, hi, b);
         }
-        int base = lane == 31 ? add(which, 0, sum) : 0;
-        base = __shfl_sync(0xffffffffu, base, 31);
-        put(which, base + sum - head, 0, head, lo, hi, b);
         unsigned more = __ballot_sync(0xffffffffu, n > per);
-        while (more) {
+        for (int i = 0; more; ++i) {
           const int src = __ffs(more) - 1;
           more &= more - 1;
+          if ((i & (team - 1)) != sub) continue;
           const int nn = __shfl_sync(0xffffffffu, n, src), l = __shfl_sync(0xffffffffu, lo, src), h = __shfl_sync(0xffffffffu, hi, src);
           for (int k = 1 + lane; (k << shift) < nn; k += 32) {
             const int c = min(per, nn - (k << shift));

@@ -527,31 +527,45 @@ struct PackedBwdParams {
   int* status;
 };
 
-// delta[h, i] = sum_d dO[i, h*hd + d] * O[i, h*hd + d]; hd / 8 lanes per (row, head), 16-byte loads
+// delta[h, i] = sum_d dO[i, h*hd + d] * O[i, h*hd + d]: HD / 8 lanes to a head, each with 16 bytes of four rows under way.  Bound by the bytes.
+constexpr int DELTA_ROWS = 4;
+template <int HD>
 __global__ void __launch_bounds__(256)
-packed_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ dout, float* __restrict__ delta, int tokens, int heads, int hd,
+packed_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ dout, float* __restrict__ delta, int tokens, int heads,
                     long long o_stride, long long do_stride) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lpi = hd >> 3;                                   // lanes per item: 8 (hd 64) or 16 (hd 128)
-  const long long total = (long long)tokens * heads;
-  const long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const long long item = t / lpi;
-  const int sub = (int)(t % lpi);
-  float s = 0.f;
-  int h = 0;
-  long long row = 0;
-  if (item < total) {
-    h = (int)(item % heads);
-    row = item / heads;
-    const uint4 a = *reinterpret_cast<const uint4*>(o + row * o_stride + h * hd + sub * 8);
-    const uint4 b = *reinterpret_cast<const uint4*>(dout + row * do_stride + h * hd + sub * 8);
-    const float2 a0 = unpack_bf16x2(a.x), a1 = unpack_bf16x2(a.y), a2 = unpack_bf16x2(a.z), a3 = unpack_bf16x2(a.w);
-    const float2 b0 = unpack_bf16x2(b.x), b1 = unpack_bf16x2(b.y), b2 = unpack_bf16x2(b.z), b3 = unpack_bf16x2(b.w);
-    s = a0.x * b0.x + a0.y * b0.y + a1.x * b1.x + a1.y * b1.y + a2.x * b2.x + a2.y * b2.y + a3.x * b3.x + a3.y * b3.y;
+  constexpr int LANES = HD / 8;
+  const int row0 = blockIdx.x * DELTA_ROWS, rows = min(DELTA_ROWS, tokens - row0);
+  const int h = (blockIdx.y * 256 + threadIdx.x) / LANES, sub = threadIdx.x % LANES;
+  const bool there = h < heads;
+  uint4 a[DELTA_ROWS], b[DELTA_ROWS];
+#pragma unroll
+  for (int r = 0; r < DELTA_ROWS; ++r) {
+    a[r] = b[r] = make_uint4(0, 0, 0, 0);
+    if (there && r < rows) {
+      a[r] = *reinterpret_cast<const uint4*>(o + (row0 + r) * o_stride + h * HD + sub * 8);
+      b[r] = *reinterpret_cast<const uint4*>(dout + (row0 + r) * do_stride + h * HD + sub * 8);
+    }
   }
-  for (int off = lpi >> 1; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-  if (item < total && sub == 0) delta[(long long)h * tokens + row] = s;
+  float s[DELTA_ROWS];
+#pragma unroll
+  for (int r = 0; r < DELTA_ROWS; ++r) {
+    unsigned long long sum = f2_mul(f2_bf16x2(a[r].x), f2_bf16x2(b[r].x));
+    sum = f2_fma(f2_bf16x2(a[r].y), f2_bf16x2(b[r].y), sum);
+    sum = f2_fma(f2_bf16x2(a[r].z), f2_bf16x2(b[r].z), sum);
+    sum = f2_fma(f2_bf16x2(a[r].w), f2_bf16x2(b[r].w), sum);
+    s[r] = f2_sum(sum);
+#pragma unroll
+    for (int off = LANES >> 1; off > 0; off >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], off);
+  }
+  if (!there || sub != 0) return;
+  float* to = delta + (long long)h * tokens + row0;
+  if (rows == DELTA_ROWS && (tokens & 3) == 0) *reinterpret_cast<float4*>(to) = make_float4(s[0], s[1], s[2], s[3]);
+  else
+#pragma unroll
+    for (int r = 0; r < DELTA_ROWS; ++r)
+      if (r < rows) to[r] = s[r];
 }
 
 constexpr int PB_THREADS = 384;   // 8 softmax warps, 2 MMA issuer warps, a TMA warp and one that clears rows and stages statistics
@@ -1275,7 +1289,7 @@ static int packed_ctas(long long items) {
 static int packed_check(int tokens, int batch, int q_heads, int kv_heads, int head_dim) {
   if (tokens < 0 || batch < 0 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads) return OA_ERR_ARG;
   if (head_dim != 64 && head_dim != 128) return OA_ERR_UNSUPPORTED;
-  if (tokens > PACKED_MAX_TOKENS || batch > PACKED_MAX_BATCH || (long long)packed_max_tiles(tokens, batch) * q_heads > 0x3fffffffll) return OA_ERR_TOO_LARGE;
+  if (tokens > PACKED_MAX_TOKENS || batch > PACKED_MAX_BATCH || (long long)packed_max_tiles(tokens, batch) * q_heads > 0x3fffffffll || q_heads > (1 << 20)) return OA_ERR_TOO_LARGE;
   return OA_OK;
 }
 
@@ -1353,9 +1367,9 @@ extern "C" int oa_packed_attn_bwd(const void* q, const void* k, const void* v, c
   if ((rc = make_tmap_2d_bf16(&tk, k, kv_cols, tokens, (uint64_t)k_stride, 64, FA_BN))) return rc;
   if ((rc = make_tmap_2d_bf16(&tv, v, kv_cols, tokens, (uint64_t)v_stride, 64, FA_BN))) return rc;
   if ((rc = make_tmap_2d_bf16(&tdo, dout, q_cols, tokens, (uint64_t)do_stride, 64, FA_BM))) return rc;
-  const long long threads = (long long)tokens * q_heads * (head_dim / 8);
-  launch_pdl(packed_delta_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout,
-             (float*)scratch, tokens, q_heads, head_dim, o_stride, do_stride);
+  const dim3 grid((unsigned)((tokens + DELTA_ROWS - 1) / DELTA_ROWS), (unsigned)(((long long)q_heads * (head_dim / 8) + 255) / 256));
+  launch_pdl(head_dim == 64 ? packed_delta_kernel<64> : packed_delta_kernel<128>, grid, dim3(256), 0, st, (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout,
+             (float*)scratch, tokens, q_heads, o_stride, do_stride);
   const PackedBwdParams p{{plan, batch, tokens}, q_heads, kv_heads, q_heads / kv_heads, scale, lse, (const float*)scratch, (float*)scratch + (size_t)q_heads * tokens, (__nv_bfloat16*)dq,
                           (__nv_bfloat16*)dk, (__nv_bfloat16*)dv, dq_stride, dk_stride, dv_stride, status};
   const PackedShortBwd brief{p.plan, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (const __nv_bfloat16*)dout, lse, p.dq, p.dk, p.dv,

@@ -53,8 +53,6 @@ struct PackedWalk {
   }
 };
 
-// The 64 threads of the two warps that share 32 rows
-__device__ __forceinline__ void row_sync(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
 __device__ __forceinline__ float lo_of(unsigned long long v) {
   uint32_t a, b;
   f2_to(v, a, b);
@@ -967,7 +965,7 @@ struct PackedQCfg {
   static constexpr int OFF_K = OFF_DO + T_BYTES;
   static constexpr int OFF_V = OFF_K + NK * T_BYTES;
   static constexpr int OFF_BAR = OFF_V + NV * T_BYTES;
-  static constexpr int OFF_ITEMS = OFF_BAR + 272;
+  static constexpr int OFF_ITEMS = OFF_BAR + 304;
   static constexpr int OFF_X = OFF_ITEMS + PACKED_ROUNDS * 16;   // float[2 halves][128 rows]
   static constexpr int SMEM_BYTES = OFF_X + 2 * FA_BM * 4;
   static constexpr int TMEM_COLS = 512;
@@ -1002,7 +1000,8 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint64_t* fin_full = bars + 24;
   uint64_t* k_part = bars + 25;    // [4]  K, V of a sequence's last block are there, and some rows of others
   uint64_t* v_part = bars + 29;    // [3]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 32);
+  uint64_t* x_full = bars + 32;    // [4]  sums of the two warps that share 32 rows are in xch
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 36);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -1013,6 +1012,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); tma_prefetch_desc(&tmDO);
     mbar_init(q_full, 1);
     mbar_init(q_empty, 2);
+    for (int s = 0; s < 4; ++s) mbar_init(&x_full[s], 2);
     for (int s = 0; s < NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
     for (int s = 0; s < NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
     mbar_init(s_full, 1);
@@ -1187,6 +1187,12 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     uint32_t itc = 0, kc = 0;
     bool ok = true;
     float* xch = reinterpret_cast<float*>(smem + Cfg::OFF_X);
+    uint32_t met = 0;
+    const auto rows_met = [&]() -> bool {          // both warps of these 32 rows have written their sums
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&x_full[quad]);
+      return warp_wait(&x_full[quad], met++ & 1);
+    };
     clear_others(p.plan, p.dq, p.dq_stride, p.q_heads * HD, threadIdx.x, 256);
     while (ok && walk.next(entry, which)) {
       const int hi = entry.y, n_kv = entry.z + 1, h = which, q0 = entry.x + entry.z * FA_BM + quad * 32, qi = q0 + lane;
@@ -1229,9 +1235,9 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll
           for (int i = 0; i < 64; i += 2) mine2 = f2_fma(f2_of(s[i], s[i + 1]), f2_of(dp[i], dp[i + 1]), mine2);
           xch[half * FA_BM + r] = f2_sum(mine2);
-          row_sync(quad);
+          ok = rows_met();
+          if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); break; }
           ndlt2 = f2_splat(-(xch[r] + xch[FA_BM + r]) * p.scale);
-          row_sync(quad);                          // may be written over
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -1258,10 +1264,12 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
       ++itc;
       tc_fence_after();
-      if (half == 1) xch[FA_BM + r] = f2_sum(sum2);
-      row_sync(quad);
-      if (half == 0 && qi < hi) p.ndelta[stat_at] = lo_of(ndlt2) - (f2_sum(sum2) + xch[FA_BM + r]);
-      row_sync(quad);                              // may be written over
+      // Into the first half's own place: it has read the second's by now (dQ holds its dS), and the second half writes there again only when dQ holds the
+      // next item's
+      if (half == 1) xch[r] = f2_sum(sum2);
+      ok = rows_met();
+      if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); break; }
+      if (half == 0 && qi < hi) p.ndelta[stat_at] = lo_of(ndlt2) - (f2_sum(sum2) + xch[r]);
       __nv_bfloat16* base = p.dq + q0 * p.dq_stride + h * HD + half * (HD / 2);
       uint32_t a[HD / 2];
 #pragma unroll

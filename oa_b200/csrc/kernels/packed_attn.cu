@@ -22,7 +22,7 @@ namespace oa {
 
 // A CTA's work items: (tile or pair of tiles, one of `per` heads or pairs of heads), all of the longest tiles first, in snake order over the
 // CTAs (round r: CTA c takes item r G + c, or r G + G - 1 - c when r is odd).  Every warp walks them alike.  The plan's entries of the first rounds are
-// fetched to shared memory at the start: with a load from L2 for each item, sent for during the one before, the kernels took 6 to 13 % longer.
+// fetched to shared memory at the start: a load from L2 for each item, sent for during the one before, cost 2 to 3 %.
 constexpr int PACKED_ROUNDS = 96;
 template <bool PAIRS>
 struct PackedWalk {
@@ -78,6 +78,18 @@ __device__ __forceinline__ void clear_others(const PackedPlan& plan, __nv_bfloat
   plan.others(blockIdx.x, gridDim.x, [&](int r) {
     for (int c = tid * 8; c < cols; c += threads * 8) *reinterpret_cast<uint4*>(base + r * stride + c) = make_uint4(0, 0, 0, 0);
   });
+}
+
+// Eight warps of 128 x 128 scores want more than the 168 registers that each of 384 threads can have; the issuing and loading warps do with 104, which leaves
+// 200.  Head dim 64: forward 113 -> 108.5 us, backward 372 -> 363 us for 8 x 2048 rows of 16 heads.  Head dim 128: 119 -> 120 and 450 -> 447 us
+// for 4096 of 32, its MMA warps spill; left alone.
+template <int HD>
+__device__ __forceinline__ void more_registers() {
+  if constexpr (HD == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+}
+template <int HD>
+__device__ __forceinline__ void fewer_registers() {
+  if constexpr (HD == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
 }
 
 struct PackedFwdParams {
@@ -176,196 +188,200 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   int4 entry;
   int which;
 
-  if (warp == Cfg::TMA_WARP) {
-    // ------------- producer
-    uint32_t blk = 0, itc = 0;   // K / V blocks and items loaded so far
-    bool ok = true;
-    while (ok && walk.next(entry, which)) {
-      const PackedFwdItem<HEADS> it(p, entry, which);
-      const int n_it = max(it.n[0], it.n[1]);
-      if (!warp_wait(q_empty, (itc & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
-      if (elect_one()) {
-        const int tiles = it.n[1] > 0 ? 2 : 1;
-        mbar_expect_tx(q_full, tiles * Cfg::Q_BYTES);
-        for (int t = 0; t < tiles; ++t)
-#pragma unroll
-          for (int x = 0; x < HD / 64; ++x)
-            tma_load_2d(smem + Cfg::OFF_Q + t * Cfg::Q_BYTES + x * (FA_BM * 128), &tmQ, q_full, it.head[t] * HD + x * 64, it.lo + it.row[t]);
-      }
-      for (int j = 0; j < n_it; ++j, ++blk) {
-        const int st = blk % NS, row = it.lo + j * FA_BN;
-        const uint32_t ph = (blk / NS) & 1;
-        if (!warp_wait(&k_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
+  if (warp >= 8) {
+    fewer_registers<HD>();
+    if (warp == Cfg::TMA_WARP) {
+      // ------------- producer
+      uint32_t blk = 0, itc = 0;   // K / V blocks and items loaded so far
+      bool ok = true;
+      while (ok && walk.next(entry, which)) {
+        const PackedFwdItem<HEADS> it(p, entry, which);
+        const int n_it = max(it.n[0], it.n[1]);
+        if (!warp_wait(q_empty, (itc & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
         if (elect_one()) {
-          mbar_expect_tx(&k_full[st], Cfg::KV_BYTES);
+          const int tiles = it.n[1] > 0 ? 2 : 1;
+          mbar_expect_tx(q_full, tiles * Cfg::Q_BYTES);
+          for (int t = 0; t < tiles; ++t)
 #pragma unroll
-          for (int x = 0; x < HD / 64; ++x)
-            tma_load_2d(smem + Cfg::OFF_K + st * Cfg::KV_BYTES + x * (FA_BN * 128), &tmK, &k_full[st], it.kv_head * HD + x * 64, row);
+            for (int x = 0; x < HD / 64; ++x)
+              tma_load_2d(smem + Cfg::OFF_Q + t * Cfg::Q_BYTES + x * (FA_BM * 128), &tmQ, q_full, it.head[t] * HD + x * 64, it.lo + it.row[t]);
         }
-        if (!warp_wait(&v_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
-        if (elect_one()) {
-          uint64_t* bar = row + FA_BN > it.hi ? &v_part[st] : &v_full[st];
-          mbar_expect_tx(bar, Cfg::KV_BYTES);
+        for (int j = 0; j < n_it; ++j, ++blk) {
+          const int st = blk % NS, row = it.lo + j * FA_BN;
+          const uint32_t ph = (blk / NS) & 1;
+          if (!warp_wait(&k_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
+          if (elect_one()) {
+            mbar_expect_tx(&k_full[st], Cfg::KV_BYTES);
 #pragma unroll
-          for (int x = 0; x < HD / 64; ++x)
-            tma_load_2d(smem + Cfg::OFF_V + st * Cfg::KV_BYTES + x * (FA_BN * 128), &tmV, bar, it.kv_head * HD + x * 64, row);
-        }
-        __syncwarp();
-      }
-      ++itc;
-    }
-  } else if (warp == Cfg::CLEAR_WARP) {
-    // ------------- zeros in place of rows behind a sequence, which only an item's last block can have
-    uint32_t blk = 0, phases = 0;
-    while (walk.next(entry, which)) {
-      const PackedFwdItem<HEADS> it(p, entry, which);
-      const int n_it = max(it.n[0], it.n[1]), row = it.lo + (n_it - 1) * FA_BN;
-      blk += n_it;
-      if (row + FA_BN <= it.hi) continue;
-      const int st = (blk - 1) % NS;
-      if (!warp_wait(&v_part[st], (phases >> st) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
-      phases ^= 1u << st;
-      clear_rows<HD>(smem + Cfg::OFF_V + st * Cfg::KV_BYTES, it.hi - row, lane);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[st]);
-    }
-  } else if (ALIAS && warp == 8) {
-    // ------------- MMA issuer of both tiles, in turn (warp-uniform waits, one lane issues)
-    constexpr uint32_t idesc_qk = umma_idesc_bf16(FA_BM, FA_BN, 0, 0);
-    constexpr uint32_t idesc_pv = umma_idesc_bf16(FA_BM, HD, 0, 1);
-    uint32_t base = 0, itc = 0, pc[2] = {0, 0};   // K / V blocks before this item, items, P V products of each tile so far
-    bool ok = true;
-    const uint64_t q_desc = desc_k(smem + Cfg::OFF_Q), k_desc = desc_k(smem + Cfg::OFF_K), v_desc = desc_mn(smem + Cfg::OFF_V);
-    // S_t = Q_t K^T of ring block `blk`; `first` / `last`: of the tiles that read it, `end`: nothing reads Q after it
-    auto issue_qk = [&](int t, uint32_t blk, bool first, bool last, bool end) -> bool {
-      const int st = blk % NS;
-      if (first && !warp_wait(&k_full[st], (blk / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t qd = desc_at(q_desc, t * Cfg::Q_BYTES), kd = desc_at(k_desc, st * Cfg::KV_BYTES);
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
-          umma_f16(tmem_base + Cfg::TM_S + t * FA_BN, desc_at(qd, off), desc_at(kd, off), idesc_qk, ks > 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[t]);
-        if (last) umma_commit(&k_empty[st]);
-        if (end) umma_commit(q_empty);
-      }
-      __syncwarp();
-      return true;
-    };
-    while (ok && walk.next(entry, which)) {
-      const PackedFwdItem<HEADS> item(p, entry, which);
-      const int n[2] = {item.n[0], item.n[1]}, n_it = max(n[0], n[1]);
-      if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
-      // a block's tiles: both, or the one whose row of blocks is longer (tile 1, unless it is absent)
-      auto qk = [&](int t, int j) -> bool {
-        const bool last = j >= n[1 - t] || t == 1;
-        return issue_qk(t, base + j, t == 0 || j >= n[0], last, last && j + 1 == n_it);
-      };
-      if (n[0] > 0) ok = qk(0, 0);
-      if (ok && n[1] > 0) ok = qk(1, 0);
-      for (int j = 0; j < n_it && ok; ++j) {
-        const int st = (base + j) % NS;
-        if (!warp_wait(&v_full[st], ((base + j) / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (j >= n[t]) continue;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (!warp_wait(&p_full[2 * t + half], pc[t] & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
-            tc_fence_after();
-            if (elect_one()) {
-              const uint64_t vd = desc_at(v_desc, st * Cfg::KV_BYTES);
-              const uint32_t p_tm = tmem_base + Cfg::TM_P + t * Cfg::P_STEP, o_tm = tmem_base + Cfg::TM_O + t * HD;
-#pragma unroll
-              for (int ks = half * 4; ks < half * 4 + 4; ++ks)
-                umma_f16_ts(o_tm, p_tm + ks * 8, desc_at(vd, ks * 2048), idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
-              if (half == 1) {
-                if (t == 1 || j >= n[1]) umma_commit(&v_empty[st]);
-                if (j + 1 == n[t]) umma_commit(&o_done[t]);
-              }
-            }
-            __syncwarp();
+            for (int x = 0; x < HD / 64; ++x)
+              tma_load_2d(smem + Cfg::OFF_K + st * Cfg::KV_BYTES + x * (FA_BN * 128), &tmK, &k_full[st], it.kv_head * HD + x * 64, row);
           }
-          if (!ok) break;
-          ++pc[t];
-          if (j + 1 < n[t]) { ok = qk(t, j + 1); if (!ok) break; }   // overwrites P_j: ordered after P_j V_j by the pipe
-        }
-      }
-      base += n_it;
-      ++itc;
-    }
-  } else if (!ALIAS && warp >= 8) {
-    // ------------- MMA issuer of tile t (warp-uniform waits, one lane issues)
-    const int t = warp - 8;
-    constexpr uint32_t idesc_qk = umma_idesc_bf16(FA_BM, FA_BN, 0, 0);
-    constexpr uint32_t idesc_pv = umma_idesc_bf16(FA_BM, HD, 0, 1);
-    const uint64_t qd = desc_k(smem + Cfg::OFF_Q + t * Cfg::Q_BYTES), k_desc = desc_k(smem + Cfg::OFF_K), v_desc = desc_mn(smem + Cfg::OFF_V);
-    const uint32_t s_tm = tmem_base + Cfg::TM_S + t * FA_BN, p_tm = tmem_base + Cfg::TM_P + t * Cfg::P_STEP, o_tm = tmem_base + Cfg::TM_O + t * HD;
-    uint32_t base = 0, itc = 0, sc = 0, pc = 0;   // K / V blocks before this item, items, S products and P V products of this tile so far
-    bool ok = true;
-    auto issue_qk = [&](uint32_t blk, bool last) -> bool {       // S_t = Q_t K^T of ring block `blk`
-      const int st = blk % NS;
-      if (!warp_wait(&k_full[st], (blk / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
-      if (sc > 0 && !warp_wait(&s_empty[t], (sc - 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); return false; }
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t kd = desc_at(k_desc, st * Cfg::KV_BYTES);
+          if (!warp_wait(&v_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
+          if (elect_one()) {
+            uint64_t* bar = row + FA_BN > it.hi ? &v_part[st] : &v_full[st];
+            mbar_expect_tx(bar, Cfg::KV_BYTES);
 #pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
-          umma_f16(s_tm, desc_at(qd, off), desc_at(kd, off), idesc_qk, ks > 0 ? 1u : 0u);
+            for (int x = 0; x < HD / 64; ++x)
+              tma_load_2d(smem + Cfg::OFF_V + st * Cfg::KV_BYTES + x * (FA_BN * 128), &tmV, bar, it.kv_head * HD + x * 64, row);
+          }
+          __syncwarp();
         }
-        umma_commit(&k_empty[st]);
-        umma_commit(&s_full[t]);
-        if (last) umma_commit(q_empty);
+        ++itc;
       }
-      __syncwarp();
-      ++sc;
-      return true;
-    };
-    while (ok && walk.next(entry, which)) {
-      const PackedFwdItem<HEADS> item(p, entry, which);
-      const int n_it = max(item.n[0], item.n[1]), n = t == 0 ? item.n[0] : item.n[1];
-      if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
-      if (n > 0) ok = issue_qk(base, n == 1);
-      for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n) { ok = issue_qk(base + j + 1, j + 2 == n); if (!ok) break; }
-        const int st = (base + j) % NS;
-        if (!warp_wait(&v_full[st], ((base + j) / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-        if (!warp_wait(&p_full[2 * t], pc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
+    } else if (warp == Cfg::CLEAR_WARP) {
+      // ------------- zeros in place of rows behind a sequence, which only an item's last block can have
+      uint32_t blk = 0, phases = 0;
+      while (walk.next(entry, which)) {
+        const PackedFwdItem<HEADS> it(p, entry, which);
+        const int n_it = max(it.n[0], it.n[1]), row = it.lo + (n_it - 1) * FA_BN;
+        blk += n_it;
+        if (row + FA_BN <= it.hi) continue;
+        const int st = (blk - 1) % NS;
+        if (!warp_wait(&v_part[st], (phases >> st) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+        phases ^= 1u << st;
+        clear_rows<HD>(smem + Cfg::OFF_V + st * Cfg::KV_BYTES, it.hi - row, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[st]);
+      }
+    } else if (ALIAS && warp == 8) {
+      // ------------- MMA issuer of both tiles, in turn (warp-uniform waits, one lane issues)
+      constexpr uint32_t idesc_qk = umma_idesc_bf16(FA_BM, FA_BN, 0, 0);
+      constexpr uint32_t idesc_pv = umma_idesc_bf16(FA_BM, HD, 0, 1);
+      uint32_t base = 0, itc = 0, pc[2] = {0, 0};   // K / V blocks before this item, items, P V products of each tile so far
+      bool ok = true;
+      const uint64_t q_desc = desc_k(smem + Cfg::OFF_Q), k_desc = desc_k(smem + Cfg::OFF_K), v_desc = desc_mn(smem + Cfg::OFF_V);
+      // S_t = Q_t K^T of ring block `blk`; `first` / `last`: of the tiles that read it, `end`: nothing reads Q after it
+      auto issue_qk = [&](int t, uint32_t blk, bool first, bool last, bool end) -> bool {
+        const int st = blk % NS;
+        if (first && !warp_wait(&k_full[st], (blk / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t vd = desc_at(v_desc, st * Cfg::KV_BYTES);
+          const uint64_t qd = desc_at(q_desc, t * Cfg::Q_BYTES), kd = desc_at(k_desc, st * Cfg::KV_BYTES);
 #pragma unroll
-          for (int ks = 0; ks < FA_BN / 16; ++ks)
-            umma_f16_ts(o_tm, p_tm + ks * 8, desc_at(vd, ks * 2048), idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
-          umma_commit(&v_empty[st]);
-          umma_commit(&o_done[t]);
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
+            umma_f16(tmem_base + Cfg::TM_S + t * FA_BN, desc_at(qd, off), desc_at(kd, off), idesc_qk, ks > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[t]);
+          if (last) umma_commit(&k_empty[st]);
+          if (end) umma_commit(q_empty);
         }
         __syncwarp();
-        ++pc;
+        return true;
+      };
+      while (ok && walk.next(entry, which)) {
+        const PackedFwdItem<HEADS> item(p, entry, which);
+        const int n[2] = {item.n[0], item.n[1]}, n_it = max(n[0], n[1]);
+        if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+        // a block's tiles: both, or the one whose row of blocks is longer (tile 1, unless it is absent)
+        auto qk = [&](int t, int j) -> bool {
+          const bool last = j >= n[1 - t] || t == 1;
+          return issue_qk(t, base + j, t == 0 || j >= n[0], last, last && j + 1 == n_it);
+        };
+        if (n[0] > 0) ok = qk(0, 0);
+        if (ok && n[1] > 0) ok = qk(1, 0);
+        for (int j = 0; j < n_it && ok; ++j) {
+          const int st = (base + j) % NS;
+          if (!warp_wait(&v_full[st], ((base + j) / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= n[t]) continue;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (!warp_wait(&p_full[2 * t + half], pc[t] & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
+              tc_fence_after();
+              if (elect_one()) {
+                const uint64_t vd = desc_at(v_desc, st * Cfg::KV_BYTES);
+                const uint32_t p_tm = tmem_base + Cfg::TM_P + t * Cfg::P_STEP, o_tm = tmem_base + Cfg::TM_O + t * HD;
+#pragma unroll
+                for (int ks = half * 4; ks < half * 4 + 4; ++ks)
+                  umma_f16_ts(o_tm, p_tm + ks * 8, desc_at(vd, ks * 2048), idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
+                if (half == 1) {
+                  if (t == 1 || j >= n[1]) umma_commit(&v_empty[st]);
+                  if (j + 1 == n[t]) umma_commit(&o_done[t]);
+                }
+              }
+              __syncwarp();
+            }
+            if (!ok) break;
+            ++pc[t];
+            if (j + 1 < n[t]) { ok = qk(t, j + 1); if (!ok) break; }   // overwrites P_j: ordered after P_j V_j by the pipe
+          }
+        }
+        base += n_it;
+        ++itc;
       }
-      // blocks of this item that this tile does not use (the last one of the pair's shorter tile, or all of an absent tile):
-      // the rings still expect one arrival per MMA warp, given once the block has landed
-      for (int j = n; j < n_it && ok; ++j) {
-        const int st = (base + j) % NS;
-        const uint32_t ph = ((base + j) / NS) & 1;
-        if (!warp_wait(&k_full[st], ph)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-        if (lane == 0) mbar_arrive(&k_empty[st]);
-        if (!warp_wait(&v_full[st], ph)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-        if (lane == 0) mbar_arrive(&v_empty[st]);
+    } else if (!ALIAS && warp < 8 + Cfg::MMA_WARPS) {
+      // ------------- MMA issuer of tile t (warp-uniform waits, one lane issues)
+      const int t = warp - 8;
+      constexpr uint32_t idesc_qk = umma_idesc_bf16(FA_BM, FA_BN, 0, 0);
+      constexpr uint32_t idesc_pv = umma_idesc_bf16(FA_BM, HD, 0, 1);
+      const uint64_t qd = desc_k(smem + Cfg::OFF_Q + t * Cfg::Q_BYTES), k_desc = desc_k(smem + Cfg::OFF_K), v_desc = desc_mn(smem + Cfg::OFF_V);
+      const uint32_t s_tm = tmem_base + Cfg::TM_S + t * FA_BN, p_tm = tmem_base + Cfg::TM_P + t * Cfg::P_STEP, o_tm = tmem_base + Cfg::TM_O + t * HD;
+      uint32_t base = 0, itc = 0, sc = 0, pc = 0;   // K / V blocks before this item, items, S products and P V products of this tile so far
+      bool ok = true;
+      auto issue_qk = [&](uint32_t blk, bool last) -> bool {       // S_t = Q_t K^T of ring block `blk`
+        const int st = blk % NS;
+        if (!warp_wait(&k_full[st], (blk / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
+        if (sc > 0 && !warp_wait(&s_empty[t], (sc - 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); return false; }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t kd = desc_at(k_desc, st * Cfg::KV_BYTES);
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
+            umma_f16(s_tm, desc_at(qd, off), desc_at(kd, off), idesc_qk, ks > 0 ? 1u : 0u);
+          }
+          umma_commit(&k_empty[st]);
+          umma_commit(&s_full[t]);
+          if (last) umma_commit(q_empty);
+        }
         __syncwarp();
+        ++sc;
+        return true;
+      };
+      while (ok && walk.next(entry, which)) {
+        const PackedFwdItem<HEADS> item(p, entry, which);
+        const int n_it = max(item.n[0], item.n[1]), n = t == 0 ? item.n[0] : item.n[1];
+        if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+        if (n > 0) ok = issue_qk(base, n == 1);
+        for (int j = 0; j < n && ok; ++j) {
+          if (j + 1 < n) { ok = issue_qk(base + j + 1, j + 2 == n); if (!ok) break; }
+          const int st = (base + j) % NS;
+          if (!warp_wait(&v_full[st], ((base + j) / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+          if (!warp_wait(&p_full[2 * t], pc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t vd = desc_at(v_desc, st * Cfg::KV_BYTES);
+#pragma unroll
+            for (int ks = 0; ks < FA_BN / 16; ++ks)
+              umma_f16_ts(o_tm, p_tm + ks * 8, desc_at(vd, ks * 2048), idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
+            umma_commit(&v_empty[st]);
+            umma_commit(&o_done[t]);
+          }
+          __syncwarp();
+          ++pc;
+        }
+        // blocks of this item that this tile does not use (the last one of the pair's shorter tile, or all of an absent tile):
+        // the rings still expect one arrival per MMA warp, given once the block has landed
+        for (int j = n; j < n_it && ok; ++j) {
+          const int st = (base + j) % NS;
+          const uint32_t ph = ((base + j) / NS) & 1;
+          if (!warp_wait(&k_full[st], ph)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+          if (lane == 0) mbar_arrive(&k_empty[st]);
+          if (!warp_wait(&v_full[st], ph)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+          if (lane == 0) mbar_arrive(&v_empty[st]);
+          __syncwarp();
+        }
+        if (n == 0 && ok && lane == 0) mbar_arrive(q_empty);
+        __syncwarp();
+        base += n_it;
+        ++itc;
       }
-      if (n == 0 && ok && lane == 0) mbar_arrive(q_empty);
-      __syncwarp();
-      base += n_it;
-      ++itc;
     }
   } else {
+    more_registers<HD>();
     // ------------- softmax + output of tile t: one thread per query row
     const int t = warp >> 2;
     const int quad = warp & 3;
@@ -655,207 +671,211 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   int4 entry;
   int which;
 
-  if (warp == 10) {
-    // ------------- TMA producer
-    uint32_t itc = 0, qc = 0;       // items and Q / dO blocks loaded so far
-    bool ok = true;
-    while (ok && walk.next(entry, which)) {
-      const PackedKvItem it(entry, which);
-      if (!warp_wait(kv_empty, (itc & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
-      if (elect_one()) {
-        mbar_expect_tx(kv_full, 2 * Cfg::T_BYTES);
+  if (warp >= 8) {
+    fewer_registers<HD>();
+    if (warp == 10) {
+      // ------------- TMA producer
+      uint32_t itc = 0, qc = 0;       // items and Q / dO blocks loaded so far
+      bool ok = true;
+      while (ok && walk.next(entry, which)) {
+        const PackedKvItem it(entry, which);
+        if (!warp_wait(kv_empty, (itc & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
+        if (elect_one()) {
+          mbar_expect_tx(kv_full, 2 * Cfg::T_BYTES);
 #pragma unroll
-        for (int x = 0; x < HD / 64; ++x) {
-          tma_load_2d(smem + Cfg::OFF_K + x * (FA_BN * 128), &tmK, kv_full, it.kv_head * HD + x * 64, it.lo + it.key0);
-          tma_load_2d(smem + Cfg::OFF_V + x * (FA_BN * 128), &tmV, kv_full, it.kv_head * HD + x * 64, it.lo + it.key0);
+          for (int x = 0; x < HD / 64; ++x) {
+            tma_load_2d(smem + Cfg::OFF_K + x * (FA_BN * 128), &tmK, kv_full, it.kv_head * HD + x * 64, it.lo + it.key0);
+            tma_load_2d(smem + Cfg::OFF_V + x * (FA_BN * 128), &tmV, kv_full, it.kv_head * HD + x * 64, it.lo + it.key0);
+          }
+        }
+        for (int g = 0; g < p.group && ok; ++g) {
+          const int h = it.kv_head * p.group + g;
+          for (int i = 0; i < it.blocks; ++i, ++qc) {
+            const int st = qc % NST;
+            const uint32_t ph = (qc / NST) & 1;
+            const int qrow = it.lo + it.key0 + i * FA_BM;
+            const bool part = qrow + FA_BM > it.hi;
+            uint8_t *q_tile = smem + Cfg::OFF_Q + st * Cfg::T_BYTES, *do_tile = smem + Cfg::OFF_DO + st * Cfg::T_BYTES;
+            if (!warp_wait(&q_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
+            if (elect_one()) {
+              uint64_t* bar = part ? &part_full[st] : &q_full[st];
+              mbar_expect_tx(bar, part ? 2 * Cfg::T_BYTES : Cfg::T_BYTES);
+#pragma unroll
+              for (int x = 0; x < HD / 64; ++x) tma_load_2d(q_tile + x * (FA_BM * 128), &tmQ, bar, h * HD + x * 64, qrow);
+            }
+            if (!warp_wait(&do_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
+            if (elect_one()) {
+              uint64_t* bar = part ? &part_full[st] : &do_full[st];
+              if (!part) mbar_expect_tx(bar, Cfg::T_BYTES);
+#pragma unroll
+              for (int x = 0; x < HD / 64; ++x) tma_load_2d(do_tile + x * (FA_BM * 128), &tmDO, bar, h * HD + x * 64, qrow);
+            }
+            __syncwarp();
+          }
+        }
+        ++itc;
+      }
+    } else if (warp == 11) {
+      // ------------- the per-query statistics of each block, and zeros in place of rows behind a sequence, which only a head's last block can have
+      uint32_t qc = 0, phases = 0;
+      bool ok = true;
+      while (ok && walk.next(entry, which)) {
+        const PackedKvItem it(entry, which);
+        for (int g = 0; g < p.group && ok; ++g) {
+          const long long stat_base = (long long)(it.kv_head * p.group + g) * p.plan.tokens;
+          for (int i = 0; i < it.blocks; ++i, ++qc) {
+            const int st = qc % NST, qrow = it.lo + it.key0 + i * FA_BM;
+            // lane l stages queries 4l .. 4l+3; sent for before their place is free
+            float4 nl, nd;
+            float* nlp = reinterpret_cast<float*>(&nl);
+            float* ndp = reinterpret_cast<float*>(&nd);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int qi = qrow + lane * 4 + u;
+              const bool okq = qi < it.hi;
+              nlp[u] = okq ? -p.lse[stat_base + qi] * LOG2E : -INFINITY;
+              ndp[u] = okq ? p.ndelta[stat_base + qi] : 0.f;
+            }
+            if (!warp_wait(&q_empty[st], ((qc / NST) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
+            float* dst = stat + st * 256;
+            reinterpret_cast<float4*>(dst)[lane] = nl;
+            reinterpret_cast<float4*>(dst + 128)[lane] = nd;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[st]);
+            if (qrow + FA_BM <= it.hi) continue;
+            if (!warp_wait(&part_full[st], (phases >> st) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+            phases ^= 1u << st;
+            clear_rows<HD>(smem + Cfg::OFF_Q + st * Cfg::T_BYTES, it.hi - qrow, lane);
+            clear_rows<HD>(smem + Cfg::OFF_DO + st * Cfg::T_BYTES, it.hi - qrow, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(&q_full[st]); mbar_arrive(&do_full[st]); }
+          }
         }
       }
-      for (int g = 0; g < p.group && ok; ++g) {
-        const int h = it.kv_head * p.group + g;
-        for (int i = 0; i < it.blocks; ++i, ++qc) {
+    } else if (warp == 8) {
+      // ------------- MMA issuer A: S^T = K Q^T and dV += P^T dO.  S^T of a tile goes over the P^T that dV read NS tiles ago.
+      constexpr uint32_t idesc_s = umma_idesc_bf16(FA_BN, FA_BM, 0, 0);
+      constexpr uint32_t idesc_g = umma_idesc_bf16(FA_BN, HD, 0, 1);   // [keys x HD] += X^T[keys x q] (TMEM) * Y[q x HD]
+      const uint64_t k_desc = desc_k(smem + Cfg::OFF_K), q_desc = desc_k(smem + Cfg::OFF_Q), do_desc = desc_mn(smem + Cfg::OFF_DO);
+      uint32_t itc = 0, qc = 0;
+      bool ok = true;
+      auto issue_s = [&](uint32_t n, bool last) -> bool {
+        const int st = n % NST;
+        if (!warp_wait(&q_full[st], (n / NST) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t qd = desc_at(q_desc, st * Cfg::T_BYTES);
+          const uint32_t s_tm = tmem_base + Cfg::TM_S + (n % NS) * FA_BN;
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
+            umma_f16(s_tm, desc_at(k_desc, off), desc_at(qd, off), idesc_s, ks > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[n % NS]);
+          if (last) umma_commit(kv_empty);
+        }
+        __syncwarp();
+        return true;
+      };
+      while (ok && walk.next(entry, which)) {
+        const int n_it = PackedKvItem(entry, which).blocks * p.group;
+        if (!warp_wait(kv_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+        ok = issue_s(qc, n_it == 1);
+        // the previous item's dV / dK were read by the softmax warps before they produced this item's first P^T, dS^T
+        for (int it = 0; it < n_it && ok; ++it, ++qc) {
+          if (NS == 2 && it + 1 < n_it) { ok = issue_s(qc + 1, it + 2 == n_it); if (!ok) break; }
           const int st = qc % NST;
-          const uint32_t ph = (qc / NST) & 1;
-          const int qrow = it.lo + it.key0 + i * FA_BM;
-          const bool part = qrow + FA_BM > it.hi;
-          uint8_t *q_tile = smem + Cfg::OFF_Q + st * Cfg::T_BYTES, *do_tile = smem + Cfg::OFF_DO + st * Cfg::T_BYTES;
-          if (!warp_wait(&q_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
-          if (elect_one()) {
-            uint64_t* bar = part ? &part_full[st] : &q_full[st];
-            mbar_expect_tx(bar, part ? 2 * Cfg::T_BYTES : Cfg::T_BYTES);
+          if (!warp_wait(&do_full[st], (qc / NST) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+          const uint64_t bd = desc_at(do_desc, st * Cfg::T_BYTES);
+          const uint32_t a_addr = tmem_base + Cfg::TM_S + (qc % NS) * FA_BN;
+          for (int half = 0; half < 2; ++half) {
+            // an item's first product replaces the accumulator: wait until both halves' warps have read the previous item's
+            if (it == 0 && half == 0) ok = warp_wait(&p_full[(qc % NS) * 2 + 1], (qc / NS) & 1);
+            if (!ok || !warp_wait(&p_full[(qc % NS) * 2 + half], (qc / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int x = 0; x < HD / 64; ++x) tma_load_2d(q_tile + x * (FA_BM * 128), &tmQ, bar, h * HD + x * 64, qrow);
-          }
-          if (!warp_wait(&do_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
-          if (elect_one()) {
-            uint64_t* bar = part ? &part_full[st] : &do_full[st];
-            if (!part) mbar_expect_tx(bar, Cfg::T_BYTES);
-#pragma unroll
-            for (int x = 0; x < HD / 64; ++x) tma_load_2d(do_tile + x * (FA_BM * 128), &tmDO, bar, h * HD + x * 64, qrow);
-          }
-          __syncwarp();
-        }
-      }
-      ++itc;
-    }
-  } else if (warp == 11) {
-    // ------------- the per-query statistics of each block, and zeros in place of rows behind a sequence, which only a head's last block can have
-    uint32_t qc = 0, phases = 0;
-    bool ok = true;
-    while (ok && walk.next(entry, which)) {
-      const PackedKvItem it(entry, which);
-      for (int g = 0; g < p.group && ok; ++g) {
-        const long long stat_base = (long long)(it.kv_head * p.group + g) * p.plan.tokens;
-        for (int i = 0; i < it.blocks; ++i, ++qc) {
-          const int st = qc % NST, qrow = it.lo + it.key0 + i * FA_BM;
-          // lane l stages queries 4l .. 4l+3; sent for before their place is free
-          float4 nl, nd;
-          float* nlp = reinterpret_cast<float*>(&nl);
-          float* ndp = reinterpret_cast<float*>(&nd);
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int qi = qrow + lane * 4 + u;
-            const bool okq = qi < it.hi;
-            nlp[u] = okq ? -p.lse[stat_base + qi] * LOG2E : -INFINITY;
-            ndp[u] = okq ? p.ndelta[stat_base + qi] : 0.f;
-          }
-          if (!warp_wait(&q_empty[st], ((qc / NST) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
-          float* dst = stat + st * 256;
-          reinterpret_cast<float4*>(dst)[lane] = nl;
-          reinterpret_cast<float4*>(dst + 128)[lane] = nd;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&q_full[st]);
-          if (qrow + FA_BM <= it.hi) continue;
-          if (!warp_wait(&part_full[st], (phases >> st) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-          phases ^= 1u << st;
-          clear_rows<HD>(smem + Cfg::OFF_Q + st * Cfg::T_BYTES, it.hi - qrow, lane);
-          clear_rows<HD>(smem + Cfg::OFF_DO + st * Cfg::T_BYTES, it.hi - qrow, lane);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) { mbar_arrive(&q_full[st]); mbar_arrive(&do_full[st]); }
-        }
-      }
-    }
-  } else if (warp == 8) {
-    // ------------- MMA issuer A: S^T = K Q^T and dV += P^T dO.  S^T of a tile goes over the P^T that dV read NS tiles ago.
-    constexpr uint32_t idesc_s = umma_idesc_bf16(FA_BN, FA_BM, 0, 0);
-    constexpr uint32_t idesc_g = umma_idesc_bf16(FA_BN, HD, 0, 1);   // [keys x HD] += X^T[keys x q] (TMEM) * Y[q x HD]
-    const uint64_t k_desc = desc_k(smem + Cfg::OFF_K), q_desc = desc_k(smem + Cfg::OFF_Q), do_desc = desc_mn(smem + Cfg::OFF_DO);
-    uint32_t itc = 0, qc = 0;
-    bool ok = true;
-    auto issue_s = [&](uint32_t n, bool last) -> bool {
-      const int st = n % NST;
-      if (!warp_wait(&q_full[st], (n / NST) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t qd = desc_at(q_desc, st * Cfg::T_BYTES);
-        const uint32_t s_tm = tmem_base + Cfg::TM_S + (n % NS) * FA_BN;
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
-          umma_f16(s_tm, desc_at(k_desc, off), desc_at(qd, off), idesc_s, ks > 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[n % NS]);
-        if (last) umma_commit(kv_empty);
-      }
-      __syncwarp();
-      return true;
-    };
-    while (ok && walk.next(entry, which)) {
-      const int n_it = PackedKvItem(entry, which).blocks * p.group;
-      if (!warp_wait(kv_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
-      ok = issue_s(qc, n_it == 1);
-      // the previous item's dV / dK were read by the softmax warps before they produced this item's first P^T, dS^T
-      for (int it = 0; it < n_it && ok; ++it, ++qc) {
-        if (NS == 2 && it + 1 < n_it) { ok = issue_s(qc + 1, it + 2 == n_it); if (!ok) break; }
-        const int st = qc % NST;
-        if (!warp_wait(&do_full[st], (qc / NST) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-        const uint64_t bd = desc_at(do_desc, st * Cfg::T_BYTES);
-        const uint32_t a_addr = tmem_base + Cfg::TM_S + (qc % NS) * FA_BN;
-        for (int half = 0; half < 2; ++half) {
-          // an item's first product replaces the accumulator: wait until both halves' warps have read the previous item's
-          if (it == 0 && half == 0) ok = warp_wait(&p_full[(qc % NS) * 2 + 1], (qc / NS) & 1);
-          if (!ok || !warp_wait(&p_full[(qc % NS) * 2 + half], (qc / NS) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)    // reduction over the 64 queries of this half
-              umma_f16_ts(tmem_base + Cfg::TM_DV, a_addr + half * 64 + ks * 8, desc_at(bd, (half * 4 + ks) * 2048),
-                          idesc_g, (it > 0 || half > 0 || ks > 0) ? 1u : 0u);
-            if (half == 1) {
-              umma_commit(&do_empty[st]);
-              if (it + 1 == n_it) umma_commit(fin_full);
+              for (int ks = 0; ks < 4; ++ks)    // reduction over the 64 queries of this half
+                umma_f16_ts(tmem_base + Cfg::TM_DV, a_addr + half * 64 + ks * 8, desc_at(bd, (half * 4 + ks) * 2048),
+                            idesc_g, (it > 0 || half > 0 || ks > 0) ? 1u : 0u);
+              if (half == 1) {
+                umma_commit(&do_empty[st]);
+                if (it + 1 == n_it) umma_commit(fin_full);
+              }
             }
+            __syncwarp();
           }
-          __syncwarp();
+          if (!ok) break;
+          if (NS == 1 && it + 1 < n_it) {
+            ok = issue_s(qc + 1, it + 2 == n_it);
+            if (lane == 0) mbar_arrive(turn);
+          }
         }
-        if (!ok) break;
-        if (NS == 1 && it + 1 < n_it) {
-          ok = issue_s(qc + 1, it + 2 == n_it);
-          if (lane == 0) mbar_arrive(turn);
-        }
+        ++itc;
       }
-      ++itc;
-    }
-  } else if (warp == 9) {
-    // ------------- MMA issuer B: dP^T = V dO^T and dK += dS^T Q.  dP^T of a tile goes over the dS^T that dK has read.
-    constexpr uint32_t idesc_s = umma_idesc_bf16(FA_BN, FA_BM, 0, 0);
-    constexpr uint32_t idesc_g = umma_idesc_bf16(FA_BN, HD, 0, 1);
-    const uint64_t v_desc = desc_k(smem + Cfg::OFF_V), do_desc = desc_k(smem + Cfg::OFF_DO), q_desc = desc_mn(smem + Cfg::OFF_Q);
-    const uint32_t dp_tm = tmem_base + Cfg::TM_DP;
-    uint32_t itc = 0, qc = 0, turns = 0;
-    bool ok = true;
-    auto issue_dp = [&](uint32_t n, bool last) -> bool {
-      const int st = n % NST;
-      if (!warp_wait(&do_full[st], (n / NST) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t dd = desc_at(do_desc, st * Cfg::T_BYTES);
+    } else if (warp == 9) {
+      // ------------- MMA issuer B: dP^T = V dO^T and dK += dS^T Q.  dP^T of a tile goes over the dS^T that dK has read.
+      constexpr uint32_t idesc_s = umma_idesc_bf16(FA_BN, FA_BM, 0, 0);
+      constexpr uint32_t idesc_g = umma_idesc_bf16(FA_BN, HD, 0, 1);
+      const uint64_t v_desc = desc_k(smem + Cfg::OFF_V), do_desc = desc_k(smem + Cfg::OFF_DO), q_desc = desc_mn(smem + Cfg::OFF_Q);
+      const uint32_t dp_tm = tmem_base + Cfg::TM_DP;
+      uint32_t itc = 0, qc = 0, turns = 0;
+      bool ok = true;
+      auto issue_dp = [&](uint32_t n, bool last) -> bool {
+        const int st = n % NST;
+        if (!warp_wait(&do_full[st], (n / NST) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t dd = desc_at(do_desc, st * Cfg::T_BYTES);
 #pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
-          umma_f16(dp_tm, desc_at(v_desc, off), desc_at(dd, off), idesc_s, ks > 0 ? 1u : 0u);
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
+            umma_f16(dp_tm, desc_at(v_desc, off), desc_at(dd, off), idesc_s, ks > 0 ? 1u : 0u);
+          }
+          umma_commit(dp_full);
+          umma_commit(&do_empty[st]);
+          if (last) umma_commit(kv_empty);
         }
-        umma_commit(dp_full);
-        umma_commit(&do_empty[st]);
-        if (last) umma_commit(kv_empty);
-      }
-      __syncwarp();
-      return true;
-    };
-    while (ok && walk.next(entry, which)) {
-      const int n_it = PackedKvItem(entry, which).blocks * p.group;
-      if (!warp_wait(kv_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
-      ok = issue_dp(qc, n_it == 1);
-      for (int it = 0; it < n_it && ok; ++it, ++qc) {
-        const int st = qc % NST;
-        if (!warp_wait(&q_full[st], (qc / NST) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-        const uint64_t bd = desc_at(q_desc, st * Cfg::T_BYTES);
-        if (NS == 1 && it + 1 < n_it) {
-          if (!warp_wait(turn, turns & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
-          ++turns;
-        }
-        for (int half = 0; half < 2; ++half) {
-          if (it == 0 && half == 0) ok = warp_wait(&ds_full[1], qc & 1);   // as for dV
-          if (!ok || !warp_wait(&ds_full[half], qc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
-          tc_fence_after();
-          if (elect_one()) {
+        __syncwarp();
+        return true;
+      };
+      while (ok && walk.next(entry, which)) {
+        const int n_it = PackedKvItem(entry, which).blocks * p.group;
+        if (!warp_wait(kv_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+        ok = issue_dp(qc, n_it == 1);
+        for (int it = 0; it < n_it && ok; ++it, ++qc) {
+          const int st = qc % NST;
+          if (!warp_wait(&q_full[st], (qc / NST) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+          const uint64_t bd = desc_at(q_desc, st * Cfg::T_BYTES);
+          if (NS == 1 && it + 1 < n_it) {
+            if (!warp_wait(turn, turns & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
+            ++turns;
+          }
+          for (int half = 0; half < 2; ++half) {
+            if (it == 0 && half == 0) ok = warp_wait(&ds_full[1], qc & 1);   // as for dV
+            if (!ok || !warp_wait(&ds_full[half], qc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              umma_f16_ts(tmem_base + Cfg::TM_DK, dp_tm + half * 64 + ks * 8, desc_at(bd, (half * 4 + ks) * 2048),
-                          idesc_g, (it > 0 || half > 0 || ks > 0) ? 1u : 0u);
-            if (half == 1) {
-              umma_commit(&q_empty[st]);
-              if (it + 1 == n_it) umma_commit(fin_full);
+              for (int ks = 0; ks < 4; ++ks)
+                umma_f16_ts(tmem_base + Cfg::TM_DK, dp_tm + half * 64 + ks * 8, desc_at(bd, (half * 4 + ks) * 2048),
+                            idesc_g, (it > 0 || half > 0 || ks > 0) ? 1u : 0u);
+              if (half == 1) {
+                umma_commit(&q_empty[st]);
+                if (it + 1 == n_it) umma_commit(fin_full);
+              }
             }
+            __syncwarp();
           }
-          __syncwarp();
+          if (!ok) break;
+          if (it + 1 < n_it) ok = issue_dp(qc + 1, it + 2 == n_it);
         }
-        if (!ok) break;
-        if (it + 1 < n_it) ok = issue_dp(qc + 1, it + 2 == n_it);
+        ++itc;
       }
-      ++itc;
     }
   } else {
+    more_registers<HD>();
     const int quad = warp & 3;
     const int half = warp >> 2;                  // this thread owns query columns [64*half, 64*half+64) of the tile
     const int r = quad * 32 + lane;              // key row inside the block = TMEM lane
@@ -1035,150 +1055,154 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   int4 entry;
   int which;
 
-  if (warp == 10) {
-    uint32_t itc = 0, kc = 0;
-    bool ok = true;
-    while (ok && walk.next(entry, which)) {
-      const int lo = entry.x, hi = entry.y, n_kv = entry.z + 1, h = which, hk = which / p.group, qrow = lo + entry.z * FA_BM;
-      if (!warp_wait(q_empty, (itc & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
-      if (elect_one()) {
-        mbar_expect_tx(q_full, 2 * Cfg::T_BYTES);
-#pragma unroll
-        for (int x = 0; x < HD / 64; ++x) {
-          tma_load_2d(smem + Cfg::OFF_Q + x * (FA_BM * 128), &tmQ, q_full, h * HD + x * 64, qrow);
-          tma_load_2d(smem + Cfg::OFF_DO + x * (FA_BM * 128), &tmDO, q_full, h * HD + x * 64, qrow);
-        }
-      }
-      for (int j = 0; j < n_kv; ++j, ++kc) {
-        const int sk = kc % NK, sv = kc % NV, row = lo + j * FA_BN;
-        const bool part = row + FA_BN > hi;
-        uint8_t *k_tile = smem + Cfg::OFF_K + sk * Cfg::T_BYTES, *v_tile = smem + Cfg::OFF_V + sv * Cfg::T_BYTES;
-        if (!warp_wait(&k_empty[sk], ((kc / NK) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
+  if (warp >= 8) {
+    fewer_registers<HD>();
+    if (warp == 10) {
+      uint32_t itc = 0, kc = 0;
+      bool ok = true;
+      while (ok && walk.next(entry, which)) {
+        const int lo = entry.x, hi = entry.y, n_kv = entry.z + 1, h = which, hk = which / p.group, qrow = lo + entry.z * FA_BM;
+        if (!warp_wait(q_empty, (itc & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
         if (elect_one()) {
-          uint64_t* bar = part ? &k_part[sk] : &k_full[sk];
-          mbar_expect_tx(bar, Cfg::T_BYTES);
+          mbar_expect_tx(q_full, 2 * Cfg::T_BYTES);
 #pragma unroll
-          for (int x = 0; x < HD / 64; ++x) tma_load_2d(k_tile + x * (FA_BN * 128), &tmK, bar, hk * HD + x * 64, row);
-        }
-        if (!warp_wait(&v_empty[sv], ((kc / NV) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
-        if (elect_one()) {
-          uint64_t* bar = part ? &v_part[sv] : &v_full[sv];
-          mbar_expect_tx(bar, Cfg::T_BYTES);
-#pragma unroll
-          for (int x = 0; x < HD / 64; ++x) tma_load_2d(v_tile + x * (FA_BN * 128), &tmV, bar, hk * HD + x * 64, row);
-        }
-        __syncwarp();
-      }
-      ++itc;
-    }
-  } else if (warp == 11) {
-    // ------------- zeros in place of rows behind a sequence, which only an item's last block can have
-    uint32_t kc = 0, k_phases = 0, v_phases = 0;
-    while (walk.next(entry, which)) {
-      const int row = entry.x + entry.z * FA_BN, from = entry.y - row;
-      kc += entry.z + 1;
-      if (from >= FA_BN) continue;
-      const int sk = (kc - 1) % NK, sv = (kc - 1) % NV;
-      if (!warp_wait(&k_part[sk], (k_phases >> sk) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
-      clear_rows<HD>(smem + Cfg::OFF_K + sk * Cfg::T_BYTES, from, lane);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&k_full[sk]);
-      if (!warp_wait(&v_part[sv], (v_phases >> sv) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
-      clear_rows<HD>(smem + Cfg::OFF_V + sv * Cfg::T_BYTES, from, lane);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[sv]);
-      k_phases ^= 1u << sk;
-      v_phases ^= 1u << sv;
-    }
-  } else if (warp == 8) {
-    // ------------- MMA issuer A: S = Q K_j^T
-    constexpr uint32_t idesc_s = umma_idesc_bf16(FA_BM, FA_BN, 0, 0);
-    const uint64_t q_desc = desc_k(smem + Cfg::OFF_Q), k_desc = desc_k(smem + Cfg::OFF_K);
-    uint32_t itc = 0, kc = 0;
-    bool ok = true;
-    while (ok && walk.next(entry, which)) {
-      const int n_kv = entry.z + 1;
-      if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
-      for (int j = 0; j < n_kv; ++j, ++kc) {
-        const int st = kc % NK;
-        if (!warp_wait(&k_full[st], (kc / NK) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-        if (kc > 0 && !warp_wait(s_empty, (kc - 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); ok = false; break; }
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t kd = desc_at(k_desc, st * Cfg::T_BYTES);
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) {
-            const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
-            umma_f16(tmem_base + Cfg::TM_S, desc_at(q_desc, off), desc_at(kd, off), idesc_s, ks > 0 ? 1u : 0u);
+          for (int x = 0; x < HD / 64; ++x) {
+            tma_load_2d(smem + Cfg::OFF_Q + x * (FA_BM * 128), &tmQ, q_full, h * HD + x * 64, qrow);
+            tma_load_2d(smem + Cfg::OFF_DO + x * (FA_BM * 128), &tmDO, q_full, h * HD + x * 64, qrow);
           }
-          umma_commit(s_full);
-          if (j + 1 == n_kv) umma_commit(q_empty);
         }
-        __syncwarp();
-      }
-      ++itc;
-    }
-  } else if (warp == 9) {
-    // ------------- MMA issuer B: dP = dO V_j^T and dQ += dS K_j (dS from TMEM, over dP)
-    constexpr uint32_t idesc_s = umma_idesc_bf16(FA_BM, FA_BN, 0, 0);
-    constexpr uint32_t idesc_q = umma_idesc_bf16(FA_BM, HD, 0, 1);   // dQ[q x HD] += dS[q x keys] * K[keys x HD]
-    const uint64_t do_desc = desc_k(smem + Cfg::OFF_DO), v_desc = desc_k(smem + Cfg::OFF_V), k_desc = desc_mn(smem + Cfg::OFF_K);
-    uint32_t itc = 0, kc = 0;
-    bool ok = true;
-    auto issue_dp = [&](uint32_t n, bool last) -> bool {
-      const int st = n % NV;
-      if (!warp_wait(&v_full[st], (n / NV) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t vd = desc_at(v_desc, st * Cfg::T_BYTES);
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
-          umma_f16(tmem_base + Cfg::TM_DP + (n & 1) * FA_BN, desc_at(do_desc, off), desc_at(vd, off), idesc_s, ks > 0 ? 1u : 0u);
-        }
-        umma_commit(&dp_full[n & 1]);
-        umma_commit(&v_empty[st]);
-        if (last) umma_commit(q_empty);
-      }
-      __syncwarp();
-      return true;
-    };
-    while (ok && walk.next(entry, which)) {
-      const int n_kv = entry.z + 1;
-      if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
-      ok = issue_dp(kc, n_kv == 1);
-      if (ok && n_kv > 1) ok = issue_dp(kc + 1, n_kv == 2);
-      for (int j = 0; j < n_kv && ok; ++j, ++kc) {
-        const int st = kc % NK;
-        if (!warp_wait(&k_full[st], (kc / NK) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
-        const uint64_t kd = desc_at(k_desc, st * Cfg::T_BYTES);
-        const uint32_t ds_tm = tmem_base + Cfg::TM_DP + (kc & 1) * FA_BN;
-        uint64_t* ready = ds_full + (kc & 1) * 2;
-        for (int half = 0; half < 2; ++half) {
-          // an item's first product replaces the accumulator: wait until both halves' warps have read the previous item's
-          if (j == 0 && half == 0) ok = warp_wait(&ready[1], (kc >> 1) & 1);
-          if (!ok || !warp_wait(&ready[half], (kc >> 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
-          tc_fence_after();
+        for (int j = 0; j < n_kv; ++j, ++kc) {
+          const int sk = kc % NK, sv = kc % NV, row = lo + j * FA_BN;
+          const bool part = row + FA_BN > hi;
+          uint8_t *k_tile = smem + Cfg::OFF_K + sk * Cfg::T_BYTES, *v_tile = smem + Cfg::OFF_V + sv * Cfg::T_BYTES;
+          if (!warp_wait(&k_empty[sk], ((kc / NK) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
           if (elect_one()) {
+            uint64_t* bar = part ? &k_part[sk] : &k_full[sk];
+            mbar_expect_tx(bar, Cfg::T_BYTES);
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks)           // dS, then its remainder
-              umma_f16_ts(tmem_base + Cfg::TM_DQ, ds_tm + half * 64 + ks * 8, desc_at(kd, (half * 4 + (ks & 3)) * 2048),
-                          idesc_q, (j > 0 || half > 0 || ks > 0) ? 1u : 0u);
-            if (half == 1) {
-              umma_commit(&k_empty[st]);
-              if (j + 1 == n_kv) umma_commit(fin_full);
-            }
+            for (int x = 0; x < HD / 64; ++x) tma_load_2d(k_tile + x * (FA_BN * 128), &tmK, bar, hk * HD + x * 64, row);
+          }
+          if (!warp_wait(&v_empty[sv], ((kc / NV) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
+          if (elect_one()) {
+            uint64_t* bar = part ? &v_part[sv] : &v_full[sv];
+            mbar_expect_tx(bar, Cfg::T_BYTES);
+#pragma unroll
+            for (int x = 0; x < HD / 64; ++x) tma_load_2d(v_tile + x * (FA_BN * 128), &tmV, bar, hk * HD + x * 64, row);
           }
           __syncwarp();
         }
-        if (!ok) break;
-        if (j + 2 < n_kv) ok = issue_dp(kc + 2, j + 3 == n_kv);      // over dS_j: ordered after its product by the pipe
+        ++itc;
       }
-      ++itc;
+    } else if (warp == 11) {
+      // ------------- zeros in place of rows behind a sequence, which only an item's last block can have
+      uint32_t kc = 0, k_phases = 0, v_phases = 0;
+      while (walk.next(entry, which)) {
+        const int row = entry.x + entry.z * FA_BN, from = entry.y - row;
+        kc += entry.z + 1;
+        if (from >= FA_BN) continue;
+        const int sk = (kc - 1) % NK, sv = (kc - 1) % NV;
+        if (!warp_wait(&k_part[sk], (k_phases >> sk) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+        clear_rows<HD>(smem + Cfg::OFF_K + sk * Cfg::T_BYTES, from, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&k_full[sk]);
+        if (!warp_wait(&v_part[sv], (v_phases >> sv) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+        clear_rows<HD>(smem + Cfg::OFF_V + sv * Cfg::T_BYTES, from, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[sv]);
+        k_phases ^= 1u << sk;
+        v_phases ^= 1u << sv;
+      }
+    } else if (warp == 8) {
+      // ------------- MMA issuer A: S = Q K_j^T
+      constexpr uint32_t idesc_s = umma_idesc_bf16(FA_BM, FA_BN, 0, 0);
+      const uint64_t q_desc = desc_k(smem + Cfg::OFF_Q), k_desc = desc_k(smem + Cfg::OFF_K);
+      uint32_t itc = 0, kc = 0;
+      bool ok = true;
+      while (ok && walk.next(entry, which)) {
+        const int n_kv = entry.z + 1;
+        if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+        for (int j = 0; j < n_kv; ++j, ++kc) {
+          const int st = kc % NK;
+          if (!warp_wait(&k_full[st], (kc / NK) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+          if (kc > 0 && !warp_wait(s_empty, (kc - 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_EMPTY); ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t kd = desc_at(k_desc, st * Cfg::T_BYTES);
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks) {
+              const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
+              umma_f16(tmem_base + Cfg::TM_S, desc_at(q_desc, off), desc_at(kd, off), idesc_s, ks > 0 ? 1u : 0u);
+            }
+            umma_commit(s_full);
+            if (j + 1 == n_kv) umma_commit(q_empty);
+          }
+          __syncwarp();
+        }
+        ++itc;
+      }
+    } else if (warp == 9) {
+      // ------------- MMA issuer B: dP = dO V_j^T and dQ += dS K_j (dS from TMEM, over dP)
+      constexpr uint32_t idesc_s = umma_idesc_bf16(FA_BM, FA_BN, 0, 0);
+      constexpr uint32_t idesc_q = umma_idesc_bf16(FA_BM, HD, 0, 1);   // dQ[q x HD] += dS[q x keys] * K[keys x HD]
+      const uint64_t do_desc = desc_k(smem + Cfg::OFF_DO), v_desc = desc_k(smem + Cfg::OFF_V), k_desc = desc_mn(smem + Cfg::OFF_K);
+      uint32_t itc = 0, kc = 0;
+      bool ok = true;
+      auto issue_dp = [&](uint32_t n, bool last) -> bool {
+        const int st = n % NV;
+        if (!warp_wait(&v_full[st], (n / NV) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); return false; }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t vd = desc_at(v_desc, st * Cfg::T_BYTES);
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t off = (ks >> 2) * (FA_BM * 128) + (ks & 3) * 32;
+            umma_f16(tmem_base + Cfg::TM_DP + (n & 1) * FA_BN, desc_at(do_desc, off), desc_at(vd, off), idesc_s, ks > 0 ? 1u : 0u);
+          }
+          umma_commit(&dp_full[n & 1]);
+          umma_commit(&v_empty[st]);
+          if (last) umma_commit(q_empty);
+        }
+        __syncwarp();
+        return true;
+      };
+      while (ok && walk.next(entry, which)) {
+        const int n_kv = entry.z + 1;
+        if (!warp_wait(q_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+        ok = issue_dp(kc, n_kv == 1);
+        if (ok && n_kv > 1) ok = issue_dp(kc + 1, n_kv == 2);
+        for (int j = 0; j < n_kv && ok; ++j, ++kc) {
+          const int st = kc % NK;
+          if (!warp_wait(&k_full[st], (kc / NK) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); ok = false; break; }
+          const uint64_t kd = desc_at(k_desc, st * Cfg::T_BYTES);
+          const uint32_t ds_tm = tmem_base + Cfg::TM_DP + (kc & 1) * FA_BN;
+          uint64_t* ready = ds_full + (kc & 1) * 2;
+          for (int half = 0; half < 2; ++half) {
+            // an item's first product replaces the accumulator: wait until both halves' warps have read the previous item's
+            if (j == 0 && half == 0) ok = warp_wait(&ready[1], (kc >> 1) & 1);
+            if (!ok || !warp_wait(&ready[half], (kc >> 1) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_SOFTMAX); ok = false; break; }
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int ks = 0; ks < 8; ++ks)           // dS, then its remainder
+                umma_f16_ts(tmem_base + Cfg::TM_DQ, ds_tm + half * 64 + ks * 8, desc_at(kd, (half * 4 + (ks & 3)) * 2048),
+                            idesc_q, (j > 0 || half > 0 || ks > 0) ? 1u : 0u);
+              if (half == 1) {
+                umma_commit(&k_empty[st]);
+                if (j + 1 == n_kv) umma_commit(fin_full);
+              }
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+          if (j + 2 < n_kv) ok = issue_dp(kc + 2, j + 3 == n_kv);      // over dS_j: ordered after its product by the pipe
+        }
+        ++itc;
+      }
     }
   } else {
+    more_registers<HD>();
     const int quad = warp & 3;
     const int half = warp >> 2;
     const int r = quad * 32 + lane;

@@ -101,8 +101,9 @@ struct PackedFwdParams {
   int* status;
 };
 
-// How many of eight pairs of exponentials go to the multiply-add pipe (flash_attn.cu)
-constexpr int PF_FMA_PAIRS = 1;
+// How many of eight pairs of exponentials go to the multiply-add pipe.  8 x 2048 rows of 16 heads of 64 with 0 / 1 / 2 / 3: 118 / 109 / 111 / 117 us; 4096 of
+// 32 of 128 with 0 / 1 / 2: 119 / 121.5 / 125.
+template <int HD> constexpr int PF_FMA_PAIRS = HD == 64 ? 1 : 0;
 
 template <int HD_>
 struct PackedFwdCfg {
@@ -471,7 +472,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           for (int i = 0; i < 32; i += 4) {
             const uint32_t* sc4 = sv + c * 32 + i;
             const unsigned long long x01 = f2_fma(f2_of(sc4[0], sc4[1]), sl22, neg_m2), x23 = f2_fma(f2_of(sc4[2], sc4[3]), sl22, neg_m2);
-            const unsigned long long e01 = exp2_mufu2(x01), e23 = (i >> 2) % 4 < PF_FMA_PAIRS ? exp2_fma2(x23) : exp2_mufu2(x23);
+            const unsigned long long e01 = exp2_mufu2(x01), e23 = (i >> 2) % 4 < PF_FMA_PAIRS<HD> ? exp2_fma2(x23) : exp2_mufu2(x23);
             l01 = f2_add(l01, e01);
             l23 = f2_add(l23, e23);
             pk[i >> 1] = f2_bf16(e01);
@@ -583,8 +584,9 @@ packed_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __
 }
 
 constexpr int PB_THREADS = 384;   // 8 softmax warps, 2 MMA issuer warps, a TMA warp and one that clears rows and stages statistics
-// Of eight pairs of exponentials, those on the multiply-add pipe (flash_attn.cu)
-template <int HD> constexpr int PB_FMA_PAIRS = HD == 64 ? 2 : 1;
+// Of eight pairs of exponentials, those on the multiply-add pipe.  The same rows' gradients at head dim 64 with 1 / 2 / 3 / 4: 366 / 362 / 360 / 376 us, at 128
+// with 0 / 1 / 2: 459 / 456 / 462.
+template <int HD> constexpr int PB_FMA_PAIRS = HD == 64 ? 3 : 1;
 
 // The pipeline of both kernels is that of flash_attn.cu, whose comment says why: a tile passes through two phases in the eight softmax warps (two
 // threads per TMEM lane, 64 columns each), scores -> probabilities, then dP -> dS, with barriers of their own; one warp issues the products that hang on
@@ -1321,7 +1323,7 @@ static int packed_ctas(long long items) {
 static int packed_check(int tokens, int batch, int q_heads, int kv_heads, int head_dim) {
   if (tokens < 0 || batch < 0 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads) return OA_ERR_ARG;
   if (head_dim != 64 && head_dim != 128) return OA_ERR_UNSUPPORTED;
-  if (tokens > PACKED_MAX_TOKENS || batch > PACKED_MAX_BATCH || (long long)packed_max_tiles(tokens, batch) * q_heads > 0x3fffffffll || q_heads > (1 << 20)) return OA_ERR_TOO_LARGE;
+  if (tokens > PACKED_MAX_TOKENS || batch > PACKED_MAX_BATCH || (long long)packed_max_tiles(tokens, batch) * q_heads > 0x3fffffffll || q_heads > (1 << 19)) return OA_ERR_TOO_LARGE;
   return OA_OK;
 }
 

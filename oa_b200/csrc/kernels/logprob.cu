@@ -334,27 +334,12 @@ __device__ __forceinline__ float lp_both(u64 v) {
   return __uint_as_float(a) + __uint_as_float(b);
 }
 
-// A team of THREADS to a row: 32, eight rows to a block of 256, or a block, gridDim.x = rows * CTAs of a cluster
-template <typename T, int THREADS, bool TOP>
-__global__ void __launch_bounds__(THREADS == 128 ? 128 : 256, THREADS == 128 ? 8 : 4) logprob_kernel(const __grid_constant__ LogprobParams p) {
-  using S = LpShared<THREADS, TOP>;
-  constexpr int TEAMS = THREADS == 32 ? 8 : 1;
-  __shared__ S shared[TEAMS];
-  pdl_launch_dependents();
-  pdl_wait();
-  S& s = shared[TEAMS > 1 ? threadIdx.x >> 5 : 0];
-  int parts = 1, part = 0;
-  if constexpr (TEAMS == 1) {
-    parts = cg::this_cluster().num_blocks();
-    part = cg::this_cluster().block_rank();
-  }
-  const int r = TEAMS > 1 ? blockIdx.x * TEAMS + (threadIdx.x >> 5) : blockIdx.x / parts, tid = threadIdx.x % THREADS, lane = tid & 31, warp = tid >> 5;
-  if (TEAMS > 1 && r >= p.rows) return;
-  const LpRow<T> row(static_cast<const T*>(p.x) + r * p.stride, p.vocab);
-  const int all = row.pieces(), per = (all + parts - 1) / parts, p0 = min(part * per, all), p1 = min(p0 + per, all);
+// The sums of pieces p0 + tid + i THREADS below p1, and the largest logit there
+template <typename T, int THREADS>
+__device__ __forceinline__ LpSums lp_sums(const LpRow<T>& row, int p0, int p1, int tid, float scale, float& tmax) {
   LpSums a{-INFINITY, 0.f, 0.f};
-  float tmax = -INFINITY;                  // of the logits themselves
-  const u64 scale2 = f2_splat(p.scale);
+  const u64 scale2 = f2_splat(scale);
+  tmax = -INFINITY;
   LpPiece<T> v[LP_BATCH];
 #pragma unroll
   for (int b = 0; b < LP_BATCH; ++b)
@@ -363,7 +348,7 @@ __global__ void __launch_bounds__(THREADS == 128 ? 128 : 256, THREADS == 128 ? 8
 #pragma unroll
     for (int b = 0; b < LP_BATCH; ++b)
       if (q + b * THREADS < p1) tmax = fmaxf(tmax, v[b].largest());
-    const float top = tmax * p.scale;
+    const float top = tmax * scale;
     if (top > a.m) a.raise(top);
     const u64 neg_m2 = f2_splat(a.m == -INFINITY ? 0.f : -a.m);
     u64 l2 = 0, s2 = 0;
@@ -388,6 +373,45 @@ __global__ void __launch_bounds__(THREADS == 128 ? 128 : 256, THREADS == 128 ? 8
     a.l += lp_both(l2);
     a.s += s1;
   }
+  return a;
+}
+
+// +inf leaves NaN in the sums, like NaN itself
+struct LpResult {
+  bool none;
+  float m, log_l, scale;
+  __device__ __forceinline__ LpResult(LpSums a, float scale_) : none(a.m == -INFINITY && a.l == 0.f), m(a.l != a.l ? NAN : a.m), log_l(none ? 0.f : logf(a.l)), scale(scale_) {}
+  __device__ __forceinline__ float logprob(float x) const { return none ? -INFINITY : fmaf(x, scale, -m) - log_l; }
+};
+template <typename T>
+__device__ __forceinline__ void lp_write(const LogprobParams& p, const LpRow<T>& row, int r, const LpSums& a, const LpResult& to) {
+  const int t = p.targets[r];
+  p.logprobs[r] = t == p.ignore ? 0.f : t >= 0 && t < p.vocab ? to.logprob(row.element(t)) : NAN;
+  p.entropy[r] = to.none ? 0.f : to.log_l - a.s / a.l;
+  p.stats[2ll * r] = to.m;
+  p.stats[2ll * r + 1] = to.log_l;
+}
+
+// A team of THREADS to a row: 32, eight rows to a block of 256, or a block, gridDim.x = rows * CTAs of a cluster
+template <typename T, int THREADS, bool TOP>
+__global__ void __launch_bounds__(THREADS == 128 ? 128 : 256, THREADS == 128 ? 8 : 4) logprob_kernel(const __grid_constant__ LogprobParams p) {
+  using S = LpShared<THREADS, TOP>;
+  constexpr int TEAMS = THREADS == 32 ? 8 : 1;
+  __shared__ S shared[TEAMS];
+  pdl_launch_dependents();
+  pdl_wait();
+  S& s = shared[TEAMS > 1 ? threadIdx.x >> 5 : 0];
+  int parts = 1, part = 0;
+  if constexpr (TEAMS == 1) {
+    parts = cg::this_cluster().num_blocks();
+    part = cg::this_cluster().block_rank();
+  }
+  const int r = TEAMS > 1 ? blockIdx.x * TEAMS + (threadIdx.x >> 5) : blockIdx.x / parts, tid = threadIdx.x % THREADS, lane = tid & 31, warp = tid >> 5;
+  if (TEAMS > 1 && r >= p.rows) return;
+  const LpRow<T> row(static_cast<const T*>(p.x) + r * p.stride, p.vocab);
+  const int all = row.pieces(), per = (all + parts - 1) / parts, p0 = min(part * per, all), p1 = min(p0 + per, all);
+  float tmax;                              // of the logits themselves
+  LpSums a = lp_sums<T, THREADS>(row, p0, p1, tid, p.scale, tmax);
   a = lp_warp_join(a);
   if (THREADS > 32) {
     if (lane == 0) s.sums[warp] = a;
@@ -412,24 +436,27 @@ __global__ void __launch_bounds__(THREADS == 128 ? 128 : 256, THREADS == 128 ? 8
     }
   }
   if (warp == 0) {
-    // +inf leaves NaN in the sums, like NaN itself
-    const bool none = a.m == -INFINITY && a.l == 0.f;
-    if (a.l != a.l) a.m = NAN;
-    const float log_l = none ? 0.f : logf(a.l);
-    const auto logprob = [&](float x) { return none ? -INFINITY : fmaf(x, p.scale, -a.m) - log_l; };
-    if (lane == 0) {
-      const int t = p.targets[r];
-      p.logprobs[r] = t == p.ignore ? 0.f : t >= 0 && t < p.vocab ? logprob(row.element(t)) : NAN;
-      p.entropy[r] = none ? 0.f : log_l - a.s / a.l;
-      p.stats[2ll * r] = a.m;
-      p.stats[2ll * r + 1] = log_l;
-    }
+    const LpResult to(a, p.scale);
+    if (lane == 0) lp_write(p, row, r, a, to);
     if (TOP && lane < p.top) {
       const u64 v = s.best[lane];
       p.top_ids[(long long)r * p.top + lane] = (int)~(uint32_t)v;
-      p.top_logprobs[(long long)r * p.top + lane] = logprob(lp_unkey((uint32_t)(v >> 32)));
+      p.top_logprobs[(long long)r * p.top + lane] = to.logprob(lp_unkey((uint32_t)(v >> 32)));
     }
   }
+}
+
+// Short rows without alternatives: eight lanes to a row, so that what a row costs once (the join, the logarithms) is shared by four rows
+constexpr int LP_LANES = 8;
+template <typename T>
+__global__ void __launch_bounds__(256, 4) logprob_short_kernel(const __grid_constant__ LogprobParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int r = blockIdx.x * (256 / LP_LANES) + threadIdx.x / LP_LANES, tid = threadIdx.x % LP_LANES;
+  const LpRow<T> row(static_cast<const T*>(p.x) + (r < p.rows ? r : 0) * p.stride, p.vocab);
+  float tmax;
+  const LpSums a = lp_warp_join(lp_sums<T, LP_LANES>(row, 0, r < p.rows ? row.pieces() : 0, tid, p.scale, tmax), LP_LANES);
+  if (tid == 0 && r < p.rows) lp_write(p, row, r, a, LpResult(a, p.scale));
 }
 
 struct LogprobBwdParams {
@@ -533,10 +560,17 @@ static int logprob_launch(const LogprobParams& p, int parts, cudaStream_t st) {
 
 template <typename T>
 static int logprob_run(const LogprobParams& p, cudaStream_t st) {
-  // A warp to a row of up to 2048 elements; otherwise as many CTAs to a row as leave no SM without two, each with 2048 elements at least.  Smaller CTAs cover
+  // Otherwise a warp to a row of up to 2048 elements; for longer ones as many CTAs to a row as leave no SM without two, each with 2048 elements at least.  Smaller CTAs cover
   // one another's meetings where there are several waves of them (bf16, five alternatives, threads 128 / 256: 4096 x 32000 66.6 / 74.8 us, 16384 x 8000 98 /
   // 161), larger ones end sooner where there is one (32 x 201088 12.2 / 11.3, 64 x 50257 9.1 / 8.8) or a thread has many pieces (fp32, twenty alternatives, 4096 x 32000
   // 143 / 123).
+  // Eight lanes to a row where there are rows enough for every SM's warps, or a row is one 16-byte piece or two to a lane (bf16, eight lanes / a warp to
+  // a row: 200000 x 256 30 / 86 us, 60000 x 1000 28 / 36, 20000 x 2000 20 / 19, 2000 x 128 2.2 / 2.7, 2000 x 500 4.6 / 3.9; fp32, 20000 x 2000 41 / 33).
+  const long long bytes = (long long)p.vocab * sizeof(T);
+  if (p.top == 0 && (bytes <= 256 || (bytes <= 4096 && p.rows >= 64 * sm_count()))) {
+    launch_short(logprob_short_kernel<T>, dim3((unsigned)((p.rows + 256 / LP_LANES - 1) / (256 / LP_LANES))), dim3(256), 0, st, p);
+    return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
+  }
   if (p.vocab <= 2048) return logprob_launch<T, 32>(p, 1, st);
   int parts = 1;
   while (parts < 8 && (long long)p.rows * parts <= 2 * sm_count() && p.vocab / (2 * parts) >= 2048) parts *= 2;

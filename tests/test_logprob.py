@@ -292,3 +292,30 @@ def test_refusals():
         L.token_logprobs_backward(both[:, 1:], t, r, None, out=both[:, :20])
     with pytest.raises(ValueError, match="result.stats must be"):
         L.token_logprobs_backward(x, t, r._replace(stats=torch.zeros(3)), None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [1, 37, 64, 250, 1000, 1024, 2047])
+def test_many_short_rows(vocab, dtype):
+    """Rows enough for eight lanes to each, their number not a multiple of a block's, with rows of every special kind among them."""
+    rows = 64 * torch.cuda.get_device_properties(0).multi_processor_count + 13
+    x, targets, g, h = _logits(rows, vocab, dtype)
+    x[::5, ::2] = -INF
+    x[::5, -1] = 0.0
+    targets[::7] = -100
+    targets[::5] = vocab - 1                 # a target among the masked has log-probability -inf, which no bound is for
+    _check(x, targets, g, h, "cuda")
+    x[3], x[5, 0], x[6, -1] = -INF, math.nan, INF
+    targets[3] = 0
+    r = L.token_logprobs(x.cuda(), targets.cuda())
+    lp, ent = r.logprobs.cpu(), r.entropy.cpu()
+    assert lp[3] == -INF and ent[3] == 0 and ent[5].isnan() and ent[6].isnan() and lp[6].isnan()
+    others = torch.ones(rows, dtype=torch.bool)
+    others[[3, 5, 6]] = False
+    assert lp[others].isfinite().all() and ent[others].isfinite().all()
+    wide = torch.full((rows, vocab + 3), math.nan, dtype=dtype, device="cuda")
+    wide[:, 1:vocab + 1] = x.cuda()
+    odd = L.token_logprobs(wide[:, 1:vocab + 1], targets.cuda())
+    e = _relative(torch.where(others[:, None], x, 0).double()) + (math.log2(vocab) + 60) * 2.0 ** -24
+    _near("logprobs", odd.logprobs[others.cuda()], lp[others].double(), 2 * (e + 2.0 ** -22 * (lp.abs() + 1))[others])

@@ -10,7 +10,11 @@
 // Forward reads a row once, in 16-byte pieces, four to a thread under way: every thread sums below a maximum of its own, and the threads meet at the
 // end.  The alternatives cost no second pass: the k-th largest of the threads' maxima has k elements at or above it, so it is a bound that few others
 // reach, and only the threads whose maximum does read their pieces again, from L2.  Long rows of which there are few are cut over a cluster of CTAs
-// that meet in distributed shared memory.  Backward is one pass.  Bound by the bytes.
+// that meet in distributed shared memory; short ones share a warp.  Backward is one pass.
+//
+// fp32 is bound by the bytes: 4096 x 32000 87.5 us, 6.0 TB/s.  bf16 has an exponential to every two bytes and stays behind them: 52.6 us, 5.0 TB/s (issue slots 58 % busy,
+// the exponentials' unit 57 %), with five alternatives 64.4, the gradient 89.4 (read and written: 5.9 TB/s).  Few rows are latency: 32 x 201088 8 us, with
+// twenty alternatives 13.5.
 #include <cooperative_groups.h>
 
 #include "common.cuh"

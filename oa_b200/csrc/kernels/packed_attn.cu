@@ -12,6 +12,13 @@
 // heads of its group, so that there is one writer and one order.  A sequence's last block may reach into the next sequence, or into rows that nobody
 // wrote: a warp of its own puts zeros in place of those rows (of values forward, of everything that is a product's second operand backward),
 // because a weight of 0 times NaN is NaN.
+//
+// Forward is bound by the softmax warps: about 1700 cycles for a tile of 128 x 128, of which the exponentials need 900 (two warps to a scheduler, each a chain of
+// loads from TMEM, maximum, exponentials, stores).  Backward is two kernels, dQ and then dK and dV, which work out scores and dP twice: seven products for
+// five, but sums of one order, no atomics, and nothing in memory between them but a number to a row.  They too are bound by their softmax warps (issue slots 45 to 50 %
+// busy, tensor pipe 40 % at head dim 64).  Measured: 8 x 2048 rows of 16 heads of 64 108.7 us (633 TFLOP/s of what the mask leaves) and 360 for the gradients
+// (478); 4096 of 32 of 128 120 (1149) and 457 (751); 8192 of 32 over 8 of 128 415 (1326) and 1653 (831).
+//
 // Every wait is bounded and reports to a status word.
 #include "attn_tile.cuh"
 #include "packed_short.h"
@@ -542,45 +549,44 @@ struct PackedBwdParams {
   int* status;
 };
 
-// delta[h, i] = sum_d dO[i, h*hd + d] * O[i, h*hd + d]: HD / 8 lanes to a head, each with 16 bytes of four rows under way.  Bound by the bytes.
-constexpr int DELTA_ROWS = 4;
+// delta[h, i] = sum_d dO[i, h*hd + d] * O[i, h*hd + d] of the rows in tiles (short sequences work out their own): HD / 8 lanes to a head, each with 16 bytes of four
+// rows under way.  Bound by the bytes: 12 us for 16384 rows of 16 heads of 64, 5.6 TB/s.
+constexpr int DELTA_ROWS = 4, DELTA_THREADS = 256;
 template <int HD>
-__global__ void __launch_bounds__(256)
-packed_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ dout, float* __restrict__ delta, int tokens, int heads,
+__global__ void __launch_bounds__(DELTA_THREADS)
+packed_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ dout, float* __restrict__ delta, const PackedPlan plan, int heads,
                     long long o_stride, long long do_stride) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int LANES = HD / 8;
-  const int row0 = blockIdx.x * DELTA_ROWS, rows = min(DELTA_ROWS, tokens - row0);
-  const int h = (blockIdx.y * 256 + threadIdx.x) / LANES, sub = threadIdx.x % LANES;
-  const bool there = h < heads;
-  uint4 a[DELTA_ROWS], b[DELTA_ROWS];
+  constexpr int LANES = HD / 8, GROUPS = FA_BM / DELTA_ROWS;
+  const int per = heads * LANES, chunks = (GROUPS * per + DELTA_THREADS - 1) / DELTA_THREADS;
+  const long long units = (long long)plan.tiles() * chunks;
+  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+    const int tile = (int)(u / chunks), i = (int)(u - (long long)tile * chunks) * DELTA_THREADS + threadIdx.x;
+    const int4 e = plan.tile(tile);
+    const int group = i / per, h = (i - group * per) / LANES, sub = threadIdx.x % LANES;
+    const int row0 = e.x + e.z * FA_BM + group * DELTA_ROWS, rows = group < GROUPS ? min(DELTA_ROWS, e.y - row0) : 0;
+    uint4 a[DELTA_ROWS], b[DELTA_ROWS];
 #pragma unroll
-  for (int r = 0; r < DELTA_ROWS; ++r) {
-    a[r] = b[r] = make_uint4(0, 0, 0, 0);
-    if (there && r < rows) {
-      a[r] = *reinterpret_cast<const uint4*>(o + (row0 + r) * o_stride + h * HD + sub * 8);
-      b[r] = *reinterpret_cast<const uint4*>(dout + (row0 + r) * do_stride + h * HD + sub * 8);
+    for (int r = 0; r < DELTA_ROWS; ++r) {
+      a[r] = b[r] = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        a[r] = *reinterpret_cast<const uint4*>(o + (row0 + r) * o_stride + h * HD + sub * 8);
+        b[r] = *reinterpret_cast<const uint4*>(dout + (row0 + r) * do_stride + h * HD + sub * 8);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < DELTA_ROWS; ++r) {
+      unsigned long long sum = f2_mul(f2_bf16x2(a[r].x), f2_bf16x2(b[r].x));
+      sum = f2_fma(f2_bf16x2(a[r].y), f2_bf16x2(b[r].y), sum);
+      sum = f2_fma(f2_bf16x2(a[r].z), f2_bf16x2(b[r].z), sum);
+      sum = f2_fma(f2_bf16x2(a[r].w), f2_bf16x2(b[r].w), sum);
+      float s = f2_sum(sum);
+#pragma unroll
+      for (int off = LANES >> 1; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+      if (sub == 0 && r < rows) delta[(long long)h * plan.tokens + row0 + r] = s;
     }
   }
-  float s[DELTA_ROWS];
-#pragma unroll
-  for (int r = 0; r < DELTA_ROWS; ++r) {
-    unsigned long long sum = f2_mul(f2_bf16x2(a[r].x), f2_bf16x2(b[r].x));
-    sum = f2_fma(f2_bf16x2(a[r].y), f2_bf16x2(b[r].y), sum);
-    sum = f2_fma(f2_bf16x2(a[r].z), f2_bf16x2(b[r].z), sum);
-    sum = f2_fma(f2_bf16x2(a[r].w), f2_bf16x2(b[r].w), sum);
-    s[r] = f2_sum(sum);
-#pragma unroll
-    for (int off = LANES >> 1; off > 0; off >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], off);
-  }
-  if (!there || sub != 0) return;
-  float* to = delta + (long long)h * tokens + row0;
-  if (rows == DELTA_ROWS && (tokens & 3) == 0) *reinterpret_cast<float4*>(to) = make_float4(s[0], s[1], s[2], s[3]);
-  else
-#pragma unroll
-    for (int r = 0; r < DELTA_ROWS; ++r)
-      if (r < rows) to[r] = s[r];
 }
 
 constexpr int PB_THREADS = 384;   // 8 softmax warps, 2 MMA issuer warps, a TMA warp and one that clears rows and stages statistics
@@ -1401,9 +1407,10 @@ extern "C" int oa_packed_attn_bwd(const void* q, const void* k, const void* v, c
   if ((rc = make_tmap_2d_bf16(&tk, k, kv_cols, tokens, (uint64_t)k_stride, 64, FA_BN))) return rc;
   if ((rc = make_tmap_2d_bf16(&tv, v, kv_cols, tokens, (uint64_t)v_stride, 64, FA_BN))) return rc;
   if ((rc = make_tmap_2d_bf16(&tdo, dout, q_cols, tokens, (uint64_t)do_stride, 64, FA_BM))) return rc;
-  const dim3 grid((unsigned)((tokens + DELTA_ROWS - 1) / DELTA_ROWS), (unsigned)(((long long)q_heads * (head_dim / 8) + 255) / 256));
-  launch_pdl(head_dim == 64 ? packed_delta_kernel<64> : packed_delta_kernel<128>, grid, dim3(256), 0, st, (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout,
-             (float*)scratch, tokens, q_heads, o_stride, do_stride);
+  const long long units = (long long)packed_max_tiles(tokens, batch) * ((FA_BM / DELTA_ROWS * (long long)q_heads * (head_dim / 8) + DELTA_THREADS - 1) / DELTA_THREADS);
+  const int fill = 8 * sm_count();
+  launch_pdl(head_dim == 64 ? packed_delta_kernel<64> : packed_delta_kernel<128>, dim3((unsigned)(units < 1 ? 1 : units < fill ? units : fill)), dim3(DELTA_THREADS), 0, st,
+             (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout, (float*)scratch, PackedPlan{plan, batch, tokens}, q_heads, o_stride, do_stride);
   const PackedBwdParams p{{plan, batch, tokens}, q_heads, kv_heads, q_heads / kv_heads, scale, lse, (const float*)scratch, (float*)scratch + (size_t)q_heads * tokens, (__nv_bfloat16*)dq,
                           (__nv_bfloat16*)dk, (__nv_bfloat16*)dv, dq_stride, dk_stride, dv_stride, status};
   const PackedShortBwd brief{p.plan, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (const __nv_bfloat16*)dout, lse, p.dq, p.dk, p.dv,

@@ -5,7 +5,8 @@
 // rows come to shared memory by cp.async, in 16-byte pieces swizzled over eight banks' groups; rows behind the sequence up to the next 16 are zeros.  A warp
 // takes 16 queries (forward, dQ) or 16 keys (dK, dV) and the products run on mma.sync, whose accumulators are the next product's operand as they stand: tiles this small cannot
 // fill a tcgen05 instruction.  Backward, scores are worked out twice, with the keys as rows for dK and dV and with the queries as rows for dQ.  Bound by latency: loads,
-// a chain of products and exponentials, stores, one after the other, which as many blocks as fit on an SM cover for one another.
+// a chain of products and exponentials, stores, one after the other, which as many blocks as fit on an SM cover for one another (issue slots 56 % busy, memory 35 %).  512 sequences of up to 48 rows, 16 heads of
+// 64: 32 to 37 us, gradients 78 to 90 without delta; the bytes would take 15 and 30.
 #include "common.cuh"
 #include "packed.cuh"
 #include "per_device.h"
@@ -93,6 +94,14 @@ __device__ __forceinline__ void short_operand(uint32_t (&w)[4], const float (&d)
   for (int h = 0; h < 2; ++h) {
     w[2 * h] = pack_bf16x2(d[h][0], d[h][1]);
     w[2 * h + 1] = pack_bf16x2(d[h][2], d[h][3]);
+  }
+}
+// ... and what its rounding leaves
+__device__ __forceinline__ void short_remainder(uint32_t (&w)[4], const float (&d)[2][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float* v = &d[i >> 1][(i & 1) * 2];
+    w[i] = pack_bf16x2(v[0] - __uint_as_float(w[i] << 16), v[1] - __uint_as_float(w[i] & 0xffff0000u));
   }
 }
 // A warp's 16 rows of an accumulator, times mul0 / mul1 for its rows lane / 4 and + 8, to memory through 16 rows of a tile (their address) that only this warp
@@ -311,6 +320,9 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
     float* stat = stats + stage * 2 * PACKED_SHORT;                      // log-sum-exp, and delta from this kernel
     const int n = e.n, u = e.tiles == 1 ? warp : e.tiles == 2 ? warp >> 1 : 0, tile = warp - u * e.tiles, base = u * e.tiles * 16, r0 = base + tile * 16;
     const bool mine_too = u < e.heads && tile < e.tiles;
+    // dS goes to its products rounded, and up to 16 rows, whose few roundings do not even out (gradients of sequences of two tokens up to 1.6 times as far off as by
+    // the rounding of the result alone), what that leaves as well; for all sequences that took 88 us in place of 79
+    const bool few = e.tiles == 1;
     const long long row0 = e.lo + tile * 16;
     float dq[HD / 8][4];
     if (g == 0) {
@@ -328,10 +340,8 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
       for (int c = 0; c < HD / 8; ++c) dq[c][0] = dq[c][1] = dq[c][2] = dq[c][3] = 0.f;
       const float nl0 = -stat[base + j0] * PS_LOG2E, nl1 = -stat[base + j1] * PS_LOG2E;
       // delta = sum p dP, in 32 bits; from the rounded output it would be off by as much as everything else together
-      float nd0 = 0.f, nd1 = 0.f;
-#pragma unroll 1
-      for (int t = 0; t <= tile; ++t) {
-        float s[2][4], dp[2][4];
+      float nd0 = 0.f, nd1 = 0.f, s[2][4], dp[2][4];                      // s: then the weights
+      const auto weights = [&](int t) {
         short_scores<HD>(s, sq + mine + rows_at, sk + all + t * STEP + columns_at);
         short_scores<HD>(dp, sdo + mine + rows_at, sv + all + t * STEP + columns_at);
 #pragma unroll
@@ -339,8 +349,19 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const int j = t * 16 + c * 8 + (lane & 3) * 2 + x;
-            nd0 -= j <= j0 ? fast_exp2(fmaf(s[c][x], sl2, nl0)) * dp[c][x] : 0.f;
-            nd1 -= j <= j1 ? fast_exp2(fmaf(s[c][2 + x], sl2, nl1)) * dp[c][2 + x] : 0.f;
+            s[c][x] = j <= j0 ? fast_exp2(fmaf(s[c][x], sl2, nl0)) : 0.f;
+            s[c][2 + x] = j <= j1 ? fast_exp2(fmaf(s[c][2 + x], sl2, nl1)) : 0.f;
+          }
+      };
+#pragma unroll 1
+      for (int t = 0; t <= tile; ++t) {
+        weights(t);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            nd0 -= s[c][x] * dp[c][x];
+            nd1 -= s[c][2 + x] * dp[c][2 + x];
           }
       }
 #pragma unroll
@@ -355,25 +376,22 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
         stat[PACKED_SHORT + base + j1] = nd1;
       }
 #pragma unroll 1
-      for (int t = 0; t <= tile; ++t) {
-        float s[2][4], dp[2][4];
-        short_scores<HD>(s, sq + mine + rows_at, sk + all + t * STEP + columns_at);
-        short_scores<HD>(dp, sdo + mine + rows_at, sv + all + t * STEP + columns_at);
+      for (int t = tile;; weights(t)) {                                   // the last keys' are still there
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            dp[c][x] = fast_exp2(fmaf(s[c][x], sl2, nl0)) * fmaf(dp[c][x], scale, nd0);
-            dp[c][2 + x] = fast_exp2(fmaf(s[c][2 + x], sl2, nl1)) * fmaf(dp[c][2 + x], scale, nd1);
-            if (t == tile) {
-              const int j = t * 16 + c * 8 + (lane & 3) * 2 + x;
-              dp[c][x] = j <= j0 ? dp[c][x] : 0.f;
-              dp[c][2 + x] = j <= j1 ? dp[c][2 + x] : 0.f;
-            }
+            dp[c][x] = s[c][x] * fmaf(dp[c][x], scale, nd0);
+            dp[c][2 + x] = s[c][2 + x] * fmaf(dp[c][2 + x], scale, nd1);
           }
         uint32_t w[4];
         short_operand(w, dp);
         short_weigh<HD>(dq, w, sk + all + t * STEP + rows_at);
+        if (few) {
+          short_remainder(w, dp);
+          short_weigh<HD>(dq, w, sk + all + t * STEP + rows_at);
+        }
+        if (--t < 0) break;
       }
     }
     __syncthreads();                                                   // delta of every query
@@ -391,7 +409,7 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
         for (int c = 0; c < 2; ++c) {
           const int i = t * 16 + c * 8 + (lane & 3) * 2;
           const float2 L = *reinterpret_cast<const float2*>(stat + base + i), D = *reinterpret_cast<const float2*>(stat + PACKED_SHORT + base + i);
-            const float2 nl = make_float2(-L.x * PS_LOG2E, -L.y * PS_LOG2E), nd = D;
+          const float2 nl = make_float2(-L.x * PS_LOG2E, -L.y * PS_LOG2E), nd = D;
           s[c][0] = fast_exp2(fmaf(s[c][0], sl2, nl.x));
           s[c][1] = fast_exp2(fmaf(s[c][1], sl2, nl.y));
           s[c][2] = fast_exp2(fmaf(s[c][2], sl2, nl.x));
@@ -416,6 +434,10 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
         short_weigh<HD>(dv, w, sdo + all + t * STEP + rows_at);
         short_operand(w, dp);
         short_weigh<HD>(dk, w, sq + all + t * STEP + rows_at);
+        if (few) {
+          short_remainder(w, dp);
+          short_weigh<HD>(dk, w, sq + all + t * STEP + rows_at);
+        }
       }
     }
     __syncthreads();                                                   // every warp has read what it needs of these rows

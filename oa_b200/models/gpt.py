@@ -100,7 +100,7 @@ class OaGptModel(OaModule):
 
     def HiddenPacked(self, ids: OaMatrix, sequences: F.OaPackedSequences) -> OaMatrix:
         """ids [tokens] of sequences of different lengths, one behind the other (`F.PackedSequences`); in bf16 training a multiple of 8 rows, those behind the last
-        sequence belonging to none."""
+        sequence belonging to none (any token of the vocabulary, no target)."""
         if ids.NumElements() != sequences.Tokens():
             raise ValueError(f"{ids.NumElements()} tokens, but the sequences are of {sequences.Tokens()} rows")
         x = F.Embedding(self.Embed.Weight.Data, ids)

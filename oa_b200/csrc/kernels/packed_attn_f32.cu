@@ -7,8 +7,8 @@
 // way (cp.async) while the second product of this one runs.  Rows of other sequences are never read: what a sequence holds does not reach another.  dK and
 // dV of a key-value head add up over the query heads that share it: up to eight of them are a cluster of blocks, a head to each, whose sums meet in distributed
 // shared memory in the heads' order; more are worked on by one block one after the other.  Either way there is one writer and one order.
-// Bound by the loads from shared memory: 16 x 512 rows of 4 heads of 32 64 us (17 TFLOP/s) and 175 for the gradients (15), 512 of 8 heads over 2 of 64 47 and 108;
-// 16 of up to 128 of 4 of 32, a few tiles to an SM, 12 and 23, a chain of loads and products.
+// 16 x 512 rows of 4 heads of 32 take 63 us (17 TFLOP/s) and 175 for the gradients (15), 512 of 8 heads over 2 of 64 46 and 109; 16 of up to 128 of 4 of 32, a few
+// tiles to an SM, 12 and 23.  There what the warps wait for is shared memory and one another (issue slots 43 % busy, multiply-add pipe 26 %).
 #include <cooperative_groups.h>
 
 #include "common.cuh"

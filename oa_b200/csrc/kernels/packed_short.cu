@@ -6,7 +6,7 @@
 // takes 16 queries (forward, dQ) or 16 keys (dK, dV) and the products run on mma.sync, whose accumulators are the next product's operand as they stand: tiles this small cannot
 // fill a tcgen05 instruction.  Backward, scores are worked out twice, with the keys as rows for dK and dV and with the queries as rows for dQ.  Bound by latency: loads,
 // a chain of products and exponentials, stores, one after the other, which as many blocks as fit on an SM cover for one another (issue slots 56 % busy, memory 35 %).  512 sequences of up to 48 rows, 16 heads of
-// 64: 32 to 37 us, gradients 78 to 90 without delta; the bytes would take 15 and 30.
+// 64: 31 us, gradients 77; the bytes would take 15 and 30.
 #include "common.cuh"
 #include "packed.cuh"
 #include "per_device.h"
@@ -320,9 +320,9 @@ __global__ void __launch_bounds__(PS_THREADS, HD == 64 ? 3 : 2) packed_short_bwd
     float* stat = stats + stage * 2 * PACKED_SHORT;                      // log-sum-exp, and delta from this kernel
     const int n = e.n, u = e.tiles == 1 ? warp : e.tiles == 2 ? warp >> 1 : 0, tile = warp - u * e.tiles, base = u * e.tiles * 16, r0 = base + tile * 16;
     const bool mine_too = u < e.heads && tile < e.tiles;
-    // dS goes to its products rounded, and up to 16 rows, whose few roundings do not even out (gradients of sequences of two tokens up to 1.6 times as far off as by
-    // the rounding of the result alone), what that leaves as well; for all sequences that took 88 us in place of 79
-    const bool few = e.tiles == 1;
+    // dS goes to its products rounded, and up to 32 rows, whose roundings are too few to even out (gradients of sequences of two tokens up to 1.6 times as far off as
+    // by the rounding of the result alone), what that leaves as well: 512 sequences of up to 48 rows take 76.8 us, with it for all of them 80.9
+    const bool few = e.tiles <= 2;
     const long long row0 = e.lo + tile * 16;
     float dq[HD / 8][4];
     if (g == 0) {

@@ -36,9 +36,9 @@ struct PackedWalk {
   const PackedPlan& plan;
   const int4* kept;
   const int per, n;
-  int round, item;
+  int round, item, index;                 // index: of the entry last handed out
   __device__ __forceinline__ PackedWalk(const PackedPlan& p, int heads, int4* room)
-      : plan(p), kept(room), per(heads), n((PAIRS ? p.pairs() : p.tiles()) * heads), round(0), item(blockIdx.x) {
+      : plan(p), kept(room), per(heads), n((PAIRS ? p.pairs() : p.tiles()) * heads), round(0), item(blockIdx.x), index(0) {
     for (int r = threadIdx.x; r < PACKED_ROUNDS; r += blockDim.x) {
       const int i = at(r);
       if (i < n) room[r] = entry_of(i);
@@ -54,7 +54,8 @@ struct PackedWalk {
   __device__ __forceinline__ bool next(int4& entry, int& which) {
     if (item >= n) return false;
     entry = round < PACKED_ROUNDS ? kept[round] : entry_of(item);
-    which = item % per;
+    index = item / per;
+    which = item - index * per;
     item = at(++round);
     return true;
   }
@@ -547,6 +548,11 @@ struct PackedBwdParams {
   __nv_bfloat16 *dq, *dk, *dv;
   long long dq_stride, dk_stride, dv_stride;
   int* status;
+  int parts, heads;      // CTAs that share the query heads of a key-value head's tile, and how many each takes
+  float4* partial;       // [parts][tiles, at most][kv_heads][dV, dK][HD / 4][128 rows], where there are several
+  __device__ __forceinline__ long long partial_at(int part, int tile, int kv_head, int w, int hd) const {
+    return ((((long long)part * packed_max_tiles(plan.tokens, plan.batch) + tile) * kv_heads + kv_head) * 2 + w) * (hd / 4 * FA_BM);
+  }
 };
 
 // delta[h, i] = sum_d dO[i, h*hd + d] * O[i, h*hd + d] of the rows in tiles (short sequences work out their own): HD / 8 lanes to a head, each with 16 bytes of four
@@ -618,15 +624,21 @@ struct PackedKvCfg {
 
 // An item of the dK/dV kernel: a tile of keys of one key-value head, and how many tiles of queries see it, of each of the group's heads.  The list has the
 // tiles of queries with the longest rows first; tiles of keys are their mirror images.
+template <bool SPLIT>
 struct PackedKvItem {
-  int lo, hi, key0, blocks, kv_head;
-  __device__ __forceinline__ PackedKvItem(const int4& e, int which) : lo(e.x), hi(e.y), kv_head(which) {
+  int lo, hi, key0, blocks, kv_head, part, head0, heads;      // the query heads: `heads` from head0 on
+  __device__ __forceinline__ PackedKvItem(const PackedBwdParams& p, const int4& e, int which) : lo(e.x), hi(e.y) {
+    kv_head = SPLIT ? which / p.parts : which;
+    part = SPLIT ? which - kv_head * p.parts : 0;
+    heads = SPLIT ? p.heads : p.group;
+    head0 = which * heads;
     blocks = e.z + 1;
     key0 = ((e.y - e.x + FA_BN - 1) / FA_BN - blocks) * FA_BN;
   }
 };
 
-template <int HD>
+// SPLIT: the group's heads are several CTAs' (a template, because the code for it cost the others 2 %)
+template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(PB_THREADS, 1)
 packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const __grid_constant__ CUtensorMap tmDO, const PackedBwdParams p) {
@@ -675,7 +687,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();                            // the prologue above ran under the previous kernel's tail; global memory from here on
 
-  PackedWalk<false> walk(p.plan, p.kv_heads, reinterpret_cast<int4*>(smem + Cfg::OFF_ITEMS));
+  PackedWalk<false> walk(p.plan, SPLIT ? p.kv_heads * p.parts : p.kv_heads, reinterpret_cast<int4*>(smem + Cfg::OFF_ITEMS));
   int4 entry;
   int which;
 
@@ -686,7 +698,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       uint32_t itc = 0, qc = 0;       // items and Q / dO blocks loaded so far
       bool ok = true;
       while (ok && walk.next(entry, which)) {
-        const PackedKvItem it(entry, which);
+        const PackedKvItem<SPLIT> it(p, entry, which);
         if (!warp_wait(kv_empty, (itc & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); break; }
         if (elect_one()) {
           mbar_expect_tx(kv_full, 2 * Cfg::T_BYTES);
@@ -696,8 +708,8 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             tma_load_2d(smem + Cfg::OFF_V + x * (FA_BN * 128), &tmV, kv_full, it.kv_head * HD + x * 64, it.lo + it.key0);
           }
         }
-        for (int g = 0; g < p.group && ok; ++g) {
-          const int h = it.kv_head * p.group + g;
+        for (int g = 0; g < it.heads && ok; ++g) {
+          const int h = it.head0 + g;
           for (int i = 0; i < it.blocks; ++i, ++qc) {
             const int st = qc % NST;
             const uint32_t ph = (qc / NST) & 1;
@@ -728,9 +740,9 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       uint32_t qc = 0, phases = 0;
       bool ok = true;
       while (ok && walk.next(entry, which)) {
-        const PackedKvItem it(entry, which);
-        for (int g = 0; g < p.group && ok; ++g) {
-          const long long stat_base = (long long)(it.kv_head * p.group + g) * p.plan.tokens;
+        const PackedKvItem<SPLIT> it(p, entry, which);
+        for (int g = 0; g < it.heads && ok; ++g) {
+          const long long stat_base = (long long)(it.head0 + g) * p.plan.tokens;
           for (int i = 0; i < it.blocks; ++i, ++qc) {
             const int st = qc % NST, qrow = it.lo + it.key0 + i * FA_BM;
             // lane l stages queries 4l .. 4l+3; sent for before their place is free
@@ -787,7 +799,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         return true;
       };
       while (ok && walk.next(entry, which)) {
-        const int n_it = PackedKvItem(entry, which).blocks * p.group;
+        const int n_it = (entry.z + 1) * (SPLIT ? p.heads : p.group);
         if (!warp_wait(kv_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
         ok = issue_s(qc, n_it == 1);
         // the previous item's dV / dK were read by the softmax warps before they produced this item's first P^T, dS^T
@@ -849,7 +861,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         return true;
       };
       while (ok && walk.next(entry, which)) {
-        const int n_it = PackedKvItem(entry, which).blocks * p.group;
+        const int n_it = (entry.z + 1) * (SPLIT ? p.heads : p.group);
         if (!warp_wait(kv_full, itc & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
         ok = issue_dp(qc, n_it == 1);
         for (int it = 0; it < n_it && ok; ++it, ++qc) {
@@ -894,8 +906,8 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     clear_others(p.plan, p.dk, p.dk_stride, p.kv_heads * HD, threadIdx.x, 256);
     clear_others(p.plan, p.dv, p.dv_stride, p.kv_heads * HD, threadIdx.x, 256);
     while (ok && walk.next(entry, which)) {
-      const PackedKvItem item(entry, which);
-      const int n_it = item.blocks * p.group;
+      const PackedKvItem<SPLIT> item(p, entry, which);
+      const int n_it = item.blocks * item.heads;
       for (int it = 0, i = 0; it < n_it; ++it, ++qc, i = i + 1 < item.blocks ? i + 1 : 0) {
         const int st = qc % NST;
         const float* st_cur = stat + st * 256 + half * 64;
@@ -971,8 +983,14 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c) tmem_ld32(tcol + c * 32, a + c * 32);
         tmem_ld_wait();
+        if constexpr (SPLIT) {                       // a row to a lane, side by side
+          float4* to = p.partial + p.partial_at(item.part, walk.index, item.kv_head, w, HD) + half * (HD / 8) * FA_BM + r;
 #pragma unroll
-        for (int c = 0; c < HD / 64; ++c) store_rows(base + c * 32, stride, item.hi - k0, a + c * 32, 1.f, lane);
+          for (int c = 0; c < HD / 8; ++c) to[c * FA_BM] = *reinterpret_cast<const float4*>(a + 4 * c);
+        } else {
+#pragma unroll
+          for (int c = 0; c < HD / 64; ++c) store_rows(base + c * 32, stride, item.hi - k0, a + c * 32, 1.f, lane);
+        }
       }
       tc_fence_before();   // dV / dK are read before this warp's next p_full / ds_full arrivals let the next item's products overwrite them
     }
@@ -1318,6 +1336,34 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   if (warp == 8) { tc_fence_after(); tmem_dealloc<Cfg::TMEM_COLS>(tmem_base); }
 }
 
+// dK and dV of the tiles whose query heads several CTAs shared: their sums added up in order.  A warp takes four rows of 64 columns
+constexpr int JOIN_THREADS = 256;
+template <int HD>
+__global__ void __launch_bounds__(JOIN_THREADS) packed_join_kernel(const PackedBwdParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int CHUNKS = FA_BM * HD / 8 / JOIN_THREADS;       // of dK or dV of a tile and head, 8 columns to a thread
+  const long long units = (long long)p.plan.tiles() * p.kv_heads * 2 * CHUNKS;
+  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+    const int chunk = (int)(u % CHUNKS), w = (int)(u / CHUNKS) & 1;
+    const long long at = u / (2 * CHUNKS);
+    const int tile = (int)(at / p.kv_heads), kv_head = (int)(at - (long long)tile * p.kv_heads);
+    const PackedKvItem<true> item(p, p.plan.tile(tile), kv_head * p.parts);
+    const int i = chunk * JOIN_THREADS + threadIdx.x, col = (i & 7) + i / (8 * FA_BM) * 8, row = i / 8 % FA_BM;
+    float v[8] = {};
+    for (int part = 0; part < p.parts; ++part) {
+      const float4* from = p.partial + p.partial_at(part, tile, kv_head, w, HD) + 2 * col * FA_BM + row;
+      const float4 a = from[0], b = from[FA_BM];
+      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+      v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    }
+    const int key = item.lo + item.key0 + row;
+    if (key >= item.hi) continue;
+    __nv_bfloat16* to = (w == 0 ? p.dv + key * p.dv_stride : p.dk + key * p.dk_stride) + kv_head * HD + col * 8;
+    *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  }
+}
+
 int make_tmap_2d_bf16(CUtensorMap* out, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld,
                       uint32_t box_inner, uint32_t box_outer);
 
@@ -1325,6 +1371,18 @@ static int packed_ctas(long long items) {
   const int sms = sm_count();
   return (int)(items < 1 ? 1 : items < sms ? items : sms);      // persistent: one CTA per SM walks its items
 }
+
+// Over how many CTAs the query heads of a key-value head go.  A tile of keys is as long as all the queries behind it times the group, and with few tiles the first
+// ones are most of the kernel: as many as bring the longest item down to an SM's share, were the sequences equally long.  With it / without: one sequence of 1000
+// rows of 64 heads over 8 of 64 69 / 112 us, of 2000 188 / 253, of 2048 of 32 over 8 of 128 146 / 180, 100 + 1700 + 300 + 900 of 64 over 8 238 / 254; 4 of 500 97 / 92.
+static int packed_parts(int tokens, int batch, int kv_heads, int group) {
+  const long long seqs = batch > 0 ? batch : 1, n = tokens / (FA_BM * seqs) + 1;
+  int parts = 1;
+  for (int d = 2; tokens > PACKED_SHORT && d <= group && d <= 64 && 5 * parts * kv_heads * seqs * (n + 1) < 8 * sm_count(); ++d)
+    if (group % d == 0) parts = d;
+  return parts;
+}
+static size_t packed_delta_floats(int tokens, int q_heads) { return (2 * (size_t)q_heads * tokens + 3) & ~(size_t)3; }
 
 static int packed_check(int tokens, int batch, int q_heads, int kv_heads, int head_dim) {
   if (tokens < 0 || batch < 0 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads) return OA_ERR_ARG;
@@ -1346,13 +1404,18 @@ static int packed_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
 
 template <int HD>
 static int packed_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo, const PackedBwdParams& p, cudaStream_t st) {
-  static std::atomic<unsigned long long> allowed_kv, allowed_q;
-  if (allow_smem(allowed_kv, (const void*)packed_bwd_kv_kernel<HD>, PackedKvCfg<HD>::SMEM_BYTES) != cudaSuccess) return OA_ERR_LAUNCH;
+  static std::atomic<unsigned long long> allowed_kv, allowed_split, allowed_q;
+  const auto kv_kernel = p.parts > 1 ? packed_bwd_kv_kernel<HD, true> : packed_bwd_kv_kernel<HD, false>;
+  if (allow_smem(p.parts > 1 ? allowed_split : allowed_kv, (const void*)kv_kernel, PackedKvCfg<HD>::SMEM_BYTES) != cudaSuccess) return OA_ERR_LAUNCH;
   if (allow_smem(allowed_q, (const void*)packed_bwd_q_kernel<HD>, PackedQCfg<HD>::SMEM_BYTES) != cudaSuccess) return OA_ERR_LAUNCH;
   const long long tiles = packed_max_tiles(p.plan.tokens, p.plan.batch);
   // dQ first: it works out what delta is off by.  It starts under the launch for short sequences, which is over at once where there are none
   launch_pdl_if(pdl_on(true), packed_bwd_q_kernel<HD>, dim3(packed_ctas(tiles * p.q_heads)), dim3(PB_THREADS), PackedQCfg<HD>::SMEM_BYTES, st, tq, tk, tv, tdo, p);
-  launch_pdl(packed_bwd_kv_kernel<HD>, dim3(packed_ctas(tiles * p.kv_heads)), dim3(PB_THREADS), PackedKvCfg<HD>::SMEM_BYTES, st, tq, tk, tv, tdo, p);
+  launch_pdl(kv_kernel, dim3(packed_ctas(tiles * p.kv_heads * p.parts)), dim3(PB_THREADS), PackedKvCfg<HD>::SMEM_BYTES, st, tq, tk, tv, tdo, p);
+  if (p.parts > 1) {
+    const long long units = tiles * p.kv_heads * 2 * (FA_BM * HD / 8 / JOIN_THREADS);
+    launch_short(packed_join_kernel<HD>, dim3((unsigned)(units < 8 * sm_count() ? units : 8 * sm_count())), dim3(JOIN_THREADS), 0, st, p);
+  }
   return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }
 
@@ -1382,10 +1445,12 @@ extern "C" int oa_packed_attn(const void* q, const void* k, const void* v, const
   return head_dim == 64 ? packed_fwd<64, false>(tq, tk, tv, p, st) : packed_fwd<128, false>(tq, tk, tv, p, st);
 }
 
-// scratch: float[2][q_heads, tokens], delta from the output and from the rows' sums
+// scratch: float[2][q_heads, tokens], delta from the output and from the rows' sums; then what CTAs that share a group's heads add up to
 extern "C" size_t oa_packed_attn_bwd_scratch_bytes(int tokens, int batch, int q_heads, int kv_heads, int head_dim) {
-  (void)batch; (void)kv_heads; (void)head_dim;
-  return 2 * (size_t)q_heads * tokens * sizeof(float);
+  if (packed_check(tokens, batch, q_heads, kv_heads, head_dim)) return 0;
+  const int parts = packed_parts(tokens, batch, kv_heads, q_heads / kv_heads);
+  const size_t sums = parts > 1 ? (size_t)parts * packed_max_tiles(tokens, batch) * kv_heads * 2 * FA_BM * head_dim : 0;
+  return (packed_delta_floats(tokens, q_heads) + sums) * sizeof(float);
 }
 
 extern "C" int oa_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, const int* plan, void* dq,
@@ -1396,7 +1461,7 @@ extern "C" int oa_packed_attn_bwd(const void* q, const void* k, const void* v, c
   if (!(scale > 0.f)) return OA_ERR_ARG;
   if (((dq_stride | dk_stride | dv_stride | o_stride | do_stride) & 7) ||
       ((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(o) |
-        reinterpret_cast<uintptr_t>(dout)) & 15))
+        reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(scratch)) & 15))
     return OA_ERR_ALIGN;
   if (tokens == 0) return OA_OK;
   cudaStream_t st = (cudaStream_t)stream;
@@ -1411,8 +1476,10 @@ extern "C" int oa_packed_attn_bwd(const void* q, const void* k, const void* v, c
   const int fill = 8 * sm_count();
   launch_pdl(head_dim == 64 ? packed_delta_kernel<64> : packed_delta_kernel<128>, dim3((unsigned)(units < 1 ? 1 : units < fill ? units : fill)), dim3(DELTA_THREADS), 0, st,
              (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout, (float*)scratch, PackedPlan{plan, batch, tokens}, q_heads, o_stride, do_stride);
+  const int parts = packed_parts(tokens, batch, kv_heads, q_heads / kv_heads);
   const PackedBwdParams p{{plan, batch, tokens}, q_heads, kv_heads, q_heads / kv_heads, scale, lse, (const float*)scratch, (float*)scratch + (size_t)q_heads * tokens, (__nv_bfloat16*)dq,
-                          (__nv_bfloat16*)dk, (__nv_bfloat16*)dv, dq_stride, dk_stride, dv_stride, status};
+                          (__nv_bfloat16*)dk, (__nv_bfloat16*)dv, dq_stride, dk_stride, dv_stride, status, parts, q_heads / kv_heads / parts,
+                          reinterpret_cast<float4*>((float*)scratch + packed_delta_floats(tokens, q_heads))};
   const PackedShortBwd brief{p.plan, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (const __nv_bfloat16*)dout, lse, p.dq, p.dk, p.dv,
                              q_stride, k_stride, v_stride, do_stride, dq_stride, dk_stride, dv_stride, kv_heads, p.group, scale};
   if ((rc = packed_short_bwd(brief, head_dim, st))) return rc;

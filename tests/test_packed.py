@@ -135,6 +135,17 @@ def test_few_rows_round_only_the_result(lengths, hq, hk, hd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths,hq,hk,hd", [([200, 1, 130], 64, 1, 64), ([1000], 12, 4, 64), ([300, 65], 7, 1, 128), ([900, 40], 16, 2, 128), ([64, 65, 128], 10, 2, 64), ([129] * 3, 70, 1, 64)])
+def test_heads_of_a_group_on_several_blocks(lengths, hq, hk, hd):
+    """Few tiles: a group's heads are dealt out and their sums joined, in one order."""
+    _check(lengths, hq, hk, hd, torch.bfloat16, "cuda", first=3, pad=150)
+    q, k, v, dout = _inputs(lengths, hq, hk, hd, torch.bfloat16, "cuda", 3, 150)
+    starts = _starts(lengths, "cuda", 3)
+    one, two = (_both(q, k, v, dout, starts, hd) for _ in range(2))
+    assert all(torch.equal(one[n], two[n]) for n in one)
+
+
+@pytest.mark.gpu
 def test_backward_leaves_short_sequences_beside_long_ones():
     """delta's own launch goes over the tiles of longer sequences; scratch of earlier calls, NaN here, reaches no result."""
     lengths = [3, 200, 64, 65, 1, 128, 500, 17]

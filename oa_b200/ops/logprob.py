@@ -43,6 +43,12 @@ def _layout(what, shape, stride, dtype, t_shape, t_stride, t_dtype, scale, top, 
     return None if stride[1] != 1 and vocab > 1 else vocab if rows <= 1 else stride[0]
 
 
+@functools.lru_cache(maxsize=64)
+def _no_alternatives(rows, device):
+    """Tensors without elements: making them took a fifth of a small call."""
+    return torch.empty((rows, 0), dtype=torch.float32, device=device), torch.empty((rows, 0), dtype=torch.int32, device=device)
+
+
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0, scale: float = 1.0, ignore_index: int = -100) -> TokenLogProbs:
     """Of every row of scale * logits [rows, vocab] (row stride allowed; scale is 1 / temperature): the log-probability of its target, the entropy, and
     the `top` likeliest tokens (at most 32) with theirs; equal logits rank by index.  A target of ignore_index has log-probability 0, any other that is
@@ -56,12 +62,17 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0, sc
     if step is None:
         logits, step = _copied(logits), vocab
     f32 = torch.empty(rows * (4 + 2 * top), dtype=torch.float32, device=logits.device)
-    logprobs, entropy, stats, top_logprobs, top_ids = torch.unsafe_split_with_sizes(f32, (rows, rows, 2 * rows, top * rows, top * rows))
+    if top:
+        logprobs, entropy, stats, top_logprobs, top_ids = torch.unsafe_split_with_sizes(f32, (rows, rows, 2 * rows, top * rows, top * rows))
+        top_logprobs, top_ids = top_logprobs.view(rows, top), top_ids.view(torch.int32).view(rows, top)
+    else:
+        logprobs, entropy, stats = torch.unsafe_split_with_sizes(f32, (rows, rows, 2 * rows))
+        top_logprobs, top_ids = _no_alternatives(rows, logits.device)
     at = f32.data_ptr()
     K._launch(N.require().oa_token_logprobs(K.dt(logits), logits.data_ptr(), step, targets.data_ptr(), at, at + 4 * rows, at + 8 * rows, at + 16 * rows,
                                             at + 4 * (4 + top) * rows, top, rows, vocab, scale, ignore_index, _stream(device)),
               "oa_token_logprobs", outputs=(logprobs, entropy))
-    return TokenLogProbs(logprobs, entropy, stats.view(rows, 2), top_logprobs.view(rows, top), top_ids.view(torch.int32).view(rows, top))
+    return TokenLogProbs(logprobs, entropy, stats.view(rows, 2), top_logprobs, top_ids)
 
 
 def _cpu(logits, targets, top, scale, ignore_index):

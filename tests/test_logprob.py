@@ -319,3 +319,25 @@ def test_many_short_rows(vocab, dtype):
     odd = L.token_logprobs(wide[:, 1:vocab + 1], targets.cuda())
     e = _relative(torch.where(others[:, None], x, 0).double()) + (math.log2(vocab) + 60) * 2.0 ** -24
     _near("logprobs", odd.logprobs[others.cuda()], lp[others].double(), 2 * (e + 2.0 ** -22 * (lp.abs() + 1))[others])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [250, 32000])
+def test_rows_beyond_32_bits(vocab):
+    """The last rows of more than 2^31 logits: the bits of a small tensor's, forward and in place backward."""
+    n = 64 * torch.cuda.get_device_properties(0).multi_processor_count if vocab == 250 else 704      # enough for the same form, a multiple of 8
+    rows = 2 ** 31 // vocab // 8 * 8 + 96 + n                        # so that those rows lie on 16 bytes as in a tensor of their own: how a row is cut depends on it
+    x = torch.empty(rows, vocab, dtype=torch.bfloat16, device="cuda")
+    for part in x.split(1 << 18):
+        part.normal_(std=3.0)
+    first = rows - n
+    targets = torch.randint(0, vocab, (rows,), dtype=torch.int32, device="cuda")
+    g, h = torch.randn(rows, device="cuda"), torch.randn(rows, device="cuda")
+    tail = x[first:].clone()
+    r = L.token_logprobs(x, targets)
+    s = L.token_logprobs(tail, targets[first:].clone())
+    for name in ("logprobs", "entropy", "stats"):
+        assert torch.equal(getattr(r, name)[first:], getattr(s, name)), name
+    want = L.token_logprobs_backward(tail, targets[first:].clone(), s, g[first:].clone(), h[first:].clone())
+    L.token_logprobs_backward(x, targets, r, g, h, out=x)
+    assert torch.equal(x[first:], want)

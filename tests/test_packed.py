@@ -187,6 +187,21 @@ def test_attention_more_items_than_sms(hd):
     _check([17, 260, 40, 1, 90, 300, 5] * 6, 8, 4, hd, torch.bfloat16, "cuda")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,hq,hk", [(64, 84, 84), (64, 168, 84), (128, 84, 84)])
+def test_attention_more_items_than_are_kept(hd, hq, hk):
+    """A CTA's first rounds are kept in shared memory, the others are fetched: the same bits as from calls with fewer heads, which need no others."""
+    lengths = [65 + i % 60 for i in range(190)]                      # 190 tiles times 84 heads are more than 96 rounds of 148 CTAs
+    q, k, v, dout = _inputs(lengths, hq, hk, hd, torch.bfloat16, "cuda", pad=9, fill=0.0)
+    starts = _starts(lengths, "cuda")
+    whole = _both(q, k, v, dout, starts, hd)
+    for at in range(0, hk, 28):
+        mine = lambda t, h: t[:, at * (h // hk) * hd:(at + 28) * (h // hk) * hd]       # noqa: E731
+        some = _both(mine(q, hq), mine(k, hk), mine(v, hk), mine(dout, hq), starts, hd)
+        for n, h in (("o", hq), ("dq", hq), ("dk", hk), ("dv", hk)):
+            assert torch.equal(mine(whole[n], h), some[n]), n
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("lengths", [[1], [31, 33], [129], RAGGED], ids=lambda v: "-".join(map(str, v)))
 @pytest.mark.parametrize("hq,hk,hd", [(4, 4, 32), (4, 2, 64), (3, 1, 128), (2, 1, 20), (2, 2, 7), (12, 4, 50), (8, 1, 32), (9, 1, 16), (24, 2, 64)])
@@ -506,3 +521,30 @@ def test_refusals_of_the_kernels():
         P.attention(q, q.cpu(), q.cpu(), plan, 64)
     with pytest.raises(ValueError, match="tensors on"):
         P.attention(q.cpu(), q.cpu(), q.cpu(), plan, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_beyond_32_bits(dtype):
+    """Sequences at the end of tensors of more than 2^31 elements: the bits of small ones."""
+    hd, heads, lengths = 128, 16, [200, 30, 64, 300]
+    width, n = 3 * heads * hd, sum(lengths)
+    tokens = 2 ** 31 // width + n + 50
+    q, k, v, dout = _inputs(lengths, heads, heads, hd, dtype, "cuda")
+    small = torch.cat([q, k, v], 1)
+    far = torch.full((tokens, width), math.nan, dtype=dtype, device="cuda")
+    dfar = torch.full((tokens, heads * hd), math.nan, dtype=dtype, device="cuda")
+    far[tokens - n:], dfar[tokens - n:] = small, dout
+    starts, positions = _starts(lengths, "cuda"), torch.arange(tokens, dtype=torch.int32, device="cuda")[None]
+    axes = (0,) * (hd // 2)
+    P.rotary(far, positions, axes, 2 * heads, hd, THETA, out=far)
+    small = torch.cat([P.rotary(small, positions[:, tokens - n:], axes, 2 * heads, hd, THETA), v], 1)
+    assert torch.equal(far[tokens - n:], small)
+    cols = [heads * hd] * 3
+    want = _both(*torch.split(small, cols, 1), dout, starts, hd)
+    got = _both(*torch.split(far, cols, 1), dfar, starts + (tokens - n), hd)
+    for name, w in want.items():
+        g = got[name]
+        assert torch.equal(g[:, tokens - n:] if name == "lse" else g[tokens - n:], w), name
+        rest = g[:, :tokens - n] if name == "lse" else g[:tokens - n]
+        assert all((part == (-math.inf if name == "lse" else 0)).all() for part in rest.split(1 << 16)), name

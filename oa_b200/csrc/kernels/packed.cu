@@ -12,10 +12,9 @@ namespace oa {
 // not.  Sequences of up to 64 rows go on a list of their own; of the others the attention kernels take their work from two lists, the longest first: tiles of 128
 // rows of a sequence, and pairs of neighbouring tiles.  Under the causal mask tile i of a sequence sees i + 1 tiles of keys (and its mirror image, tile n - 1 - i, is seen by as many tiles of
 // queries), so both lists are sorted by that index, by counting.  The order among equals is that of the atomics; nothing depends on it but
-// which SM works on a tile.  One block: a batch has few thousand tiles, and one plan serves every layer of a step in both directions.  Latency: 6.5 us
-// for one sequence of 4096, 8 for 8 of 2048, 12 for 64 of up to 300.
-constexpr int PLAN_BINS = 1024;           // = threads of the block
-constexpr int PLAN_THREADS = PLAN_BINS;
+// which SM works on a tile.  One block: a batch has few thousand tiles, and one plan serves every layer of a step in both directions.  Latency: 5 us
+// for one sequence of 4096, 6 for 8 of 2048, 11 for 64 of up to 300.
+constexpr int PLAN_KEPT = 1024;           // sequences whose starts are kept in shared memory, at most
 
 struct PackedPlanParams {
   const int* starts;
@@ -23,7 +22,7 @@ struct PackedPlanParams {
   int batch, tokens, shift;               // bins of 2^shift tile indices
 };
 
-template <typename Op>
+template <int THREADS, typename Op>
 __device__ __forceinline__ int plan_scan(int v, int* s_warp, Op op) {   // inclusive, over the block
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -34,46 +33,50 @@ __device__ __forceinline__ int plan_scan(int v, int* s_warp, Op op) {   // inclu
   __syncthreads();                        // the last scan's reads
   if (lane == 31) s_warp[warp] = v;
   __syncthreads();
-  if (warp == 0) {
-    int w = s_warp[lane];
+  int w = s_warp[lane < THREADS / 32 ? lane : 0];            // by every warp for itself
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w = op(w, u);
-    }
-    s_warp[lane] = w;
+  for (int o = 1; o < THREADS / 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w = op(w, u);
   }
-  __syncthreads();
-  return warp > 0 ? op(v, s_warp[warp - 1]) : v;
+  const int before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+  return warp > 0 ? op(v, before) : v;
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedPlanParams p) {
-  __shared__ int s_warp[32], s_count[2][PLAN_BINS], s_top, s_short[3];
+// THREADS: of the block, and bins
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) packed_plan_kernel(const PackedPlanParams p) {
+  __shared__ int s_warp[32], s_count[2][THREADS], s_top, s_short[3], s_starts[PLAN_KEPT + 1];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, shift = p.shift, per = 1 << shift;
-  int* starts = p.plan + PACKED_HEADER;
+  int* const out = p.plan + PACKED_HEADER;
+  const bool kept = p.batch <= PLAN_KEPT;
+  const int* const starts = kept ? s_starts : out;
   s_count[0][tid] = s_count[1][tid] = 0;
   if (tid < 3) s_short[tid] = 0;
   if (tid == 0) s_top = 0;
   const auto most = [](int a, int b) { return max(a, b); };
-  for (int b0 = 0; b0 <= p.batch; b0 += PLAN_THREADS) {
+  for (int b0 = 0; b0 <= p.batch; b0 += THREADS) {
     const int b = b0 + tid;
-    const int v = plan_scan(b <= p.batch ? min(max(p.starts[b], 0), p.tokens) : 0, s_warp, most);
+    const int v = plan_scan<THREADS>(b <= p.batch ? min(max(p.starts[b], 0), p.tokens) : 0, s_warp, most);
     const int s = max(v, s_top);          // written below, behind a barrier
-    if (b <= p.batch) starts[b] = s;
+    if (b <= p.batch) {
+      out[b] = s;
+      if (kept) s_starts[b] = s;
+    }
     __syncthreads();
-    if (tid == PLAN_THREADS - 1) s_top = s;
+    if (tid == THREADS - 1) s_top = s;
   }
   __syncthreads();
   // `team` warps to 32 sequences: the first of them takes the first bin of all at once, each the other bins of its share, one sequence after the other, a bin
   // to a lane.
   // add(which, bin, n) is called for n indices of a bin, returns where they go; put(which, at, first index, n) follows
   int team = 1;
-  while (team < 32 && team * p.batch <= 16 * 32) team *= 2;
+  while (team < THREADS / 32 && team * p.batch <= THREADS / 2) team *= 2;
   const int sub = (tid >> 5) & (team - 1);
   const auto walk = [&](auto add, auto put) {
-    for (int b0 = (tid >> 5) / team * 32; b0 < p.batch; b0 += PLAN_THREADS / team) {
+    for (int b0 = (tid >> 5) / team * 32; b0 < p.batch; b0 += THREADS / team) {
       const int b = b0 + lane;
       const int lo = b < p.batch ? starts[b] : 0, hi = b < p.batch ? starts[b + 1] : 0;
 #pragma unroll
@@ -113,7 +116,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedP
   lists[2] = lists[1] + packed_max_pairs(p.tokens, p.batch);
   // short sequences by their number of 16 rows, most first: counted, then placed
   for (int pass = 0; pass < 2; ++pass) {
-    for (int b0 = tid - lane; b0 < p.batch; b0 += PLAN_THREADS) {
+    for (int b0 = tid - lane; b0 < p.batch; b0 += THREADS) {
       const int b = b0 + lane;
       const int lo = b < p.batch ? starts[b] : 0, hi = b < p.batch ? starts[b + 1] : 0, n = hi - lo;
       const int mine = n < 1 || n > PACKED_SHORT ? -1 : n > 32 ? 0 : n > 16 ? 1 : 2;
@@ -137,10 +140,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const PackedP
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     // how many have a larger index: the sums from the end
-    const int mine = s_count[which][PLAN_BINS - 1 - tid];
-    const int sum = plan_scan(mine, s_warp, [](int a, int b) { return a + b; });
-    s_count[which][PLAN_BINS - 1 - tid] = sum - mine;
-    if (tid == PLAN_THREADS - 1) p.plan[which] = sum;
+    const int mine = s_count[which][THREADS - 1 - tid];
+    const int sum = plan_scan<THREADS>(mine, s_warp, [](int a, int b) { return a + b; });
+    s_count[which][THREADS - 1 - tid] = sum - mine;
+    if (tid == THREADS - 1) p.plan[which] = sum;
   }
   __syncthreads();
   if (tid == 0) { p.plan[2] = starts[0]; p.plan[3] = starts[p.batch]; p.plan[7] = 0; }
@@ -312,9 +315,13 @@ extern "C" int oa_packed_plan(const int* starts, int* plan, int batch, int token
   if (batch < 0 || tokens < 0 || !starts || !plan) return OA_ERR_ARG;
   if (batch > PACKED_MAX_BATCH || tokens > PACKED_MAX_TOKENS) return OA_ERR_TOO_LARGE;
   if (reinterpret_cast<uintptr_t>(plan) & 15) return OA_ERR_ALIGN;
+  // the smaller block where a bin to an index is not more than it has threads, for it gets through its barriers sooner
+  const bool small = batch <= 256 && tokens / PACKED_TILE < 256;
+  const int bins = small ? 256 : 1024;
   int shift = 0;
-  while (((tokens / PACKED_TILE) >> shift) >= PLAN_BINS) ++shift;
-  launch_short(packed_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, (cudaStream_t)stream, PackedPlanParams{starts, plan, batch, tokens, shift});
+  while (((tokens / PACKED_TILE) >> shift) >= bins) ++shift;
+  launch_short(small ? packed_plan_kernel<256> : packed_plan_kernel<1024>, dim3(1), dim3(bins), 0, (cudaStream_t)stream,
+               PackedPlanParams{starts, plan, batch, tokens, shift});
   return cudaGetLastError() == cudaSuccess ? OA_OK : OA_ERR_LAUNCH;
 }
 

@@ -13,8 +13,9 @@ namespace oa {
 // rows of a sequence, and pairs of neighbouring tiles.  Under the causal mask tile i of a sequence sees i + 1 tiles of keys (and its mirror image, tile n - 1 - i, is seen by as many tiles of
 // queries), so both lists are sorted by that index, by counting.  The order among equals is that of the atomics; nothing depends on it but
 // which SM works on a tile.  One block: a batch has few thousand tiles, and one plan serves every layer of a step in both directions.  Latency: 5 us
-// for one sequence of 4096, 6 for 8 of 2048, 11 for 64 of up to 300.
+// for one sequence of 4096 and for 16 of up to 2048, 5.6 for 64 of up to 300, 6.5 for 512 of up to 48.
 constexpr int PLAN_KEPT = 1024;           // sequences whose starts are kept in shared memory, at most
+constexpr int PLAN_FEW = 8;               // bins taken for 32 sequences at once
 
 struct PackedPlanParams {
   const int* starts;
@@ -69,8 +70,8 @@ __global__ void __launch_bounds__(THREADS) packed_plan_kernel(const PackedPlanPa
     if (tid == THREADS - 1) s_top = s;
   }
   __syncthreads();
-  // `team` warps to 32 sequences: the first of them takes the first bin of all at once, each the other bins of its share, one sequence after the other, a bin
-  // to a lane.
+  // `team` warps to 32 sequences.  The first bins are taken for all of them at once, each by one of the warps; the others of one sequence after the other, a bin to
+  // a lane, each warp its share of the sequences.
   // add(which, bin, n) is called for n indices of a bin, returns where they go; put(which, at, first index, n) follows
   int team = 1;
   while (team < THREADS / 32 && team * p.batch <= THREADS / 2) team *= 2;
@@ -82,25 +83,31 @@ __global__ void __launch_bounds__(THREADS) packed_plan_kernel(const PackedPlanPa
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         const int rows = PACKED_TILE << which;
-        const int n = hi - lo <= PACKED_SHORT ? 0 : (hi - lo + rows - 1) / rows, head = min(n, per);
-        if (sub == 0) {
-          int sum = head;
+        const int n = hi - lo <= PACKED_SHORT ? 0 : (hi - lo + rows - 1) / rows;
+        for (int k = sub; k < PLAN_FEW; k += team) {
+          const int c = min(max(n - (k << shift), 0), per);
+          const unsigned any = __ballot_sync(0xffffffffu, c > 0);
+          if (!any) break;
+          int sum = __popc(any & 0xffffffffu >> (31 - lane));              // of the lanes up to this one
+          if (per > 1) {
+            sum = c;
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += u;
+            for (int o = 1; o < 32; o <<= 1) {
+              const int u = __shfl_up_sync(0xffffffffu, sum, o);
+              if (lane >= o) sum += u;
+            }
           }
-          int base = lane == 31 ? add(which, 0, sum) : 0;
+          int base = lane == 31 ? add(which, k, sum) : 0;
           base = __shfl_sync(0xffffffffu, base, 31);
-          put(which, base + sum - head, 0, head, lo, hi, b);
+          put(which, base + sum - c, k << shift, c, lo, hi, b);
         }
-        unsigned more = __ballot_sync(0xffffffffu, n > per);
+        unsigned more = __ballot_sync(0xffffffffu, n > PLAN_FEW << shift);
         for (int i = 0; more; ++i) {
           const int src = __ffs(more) - 1;
           more &= more - 1;
           if ((i & (team - 1)) != sub) continue;
           const int nn = __shfl_sync(0xffffffffu, n, src), l = __shfl_sync(0xffffffffu, lo, src), h = __shfl_sync(0xffffffffu, hi, src);
-          for (int k = 1 + lane; (k << shift) < nn; k += 32) {
+          for (int k = PLAN_FEW + lane; (k << shift) < nn; k += 32) {
             const int c = min(per, nn - (k << shift));
             put(which, add(which, k, c), k << shift, c, l, h, b0 + src);
           }

@@ -64,24 +64,34 @@ def _copied(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format) if t.is_contiguous() else K.contiguous(t)
 
 
+def _end(t: torch.Tensor) -> int:
+    """The address behind a matrix's last element."""
+    (rows, cols), (down, right) = t.shape, t.stride()
+    return t.data_ptr() + ((rows - 1) * down + (cols - 1) * right + 1) * t.element_size()
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two matrices share memory (columns of one buffer that lie beside one another do not)."""
     if not a.numel() or not b.numel():
         return False
-    size = a.element_size()
-    (lo, hi), (lo2, hi2) = ((t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + (t.shape[1] - 1) * t.stride(1) + 1) * t.element_size()) for t in (a, b))
-    if hi <= lo2 or hi2 <= lo:
+    lo, lo2 = a.data_ptr(), b.data_ptr()
+    if (lo2 >= _end(a)) if lo <= lo2 else (lo >= _end(b)):
         return False
-    pitch = a.stride(0) * size
+    pitch = a.stride(0) * a.element_size()
     if a.stride(1) == b.stride(1) == 1 and b.stride(0) * b.element_size() == pitch > 0:
         at = (lo2 - lo) % pitch
-        return at < a.shape[1] * size or at + b.shape[1] * b.element_size() > pitch
+        return at < a.shape[1] * a.element_size() or at + b.shape[1] * b.element_size() > pitch
     return True
 
 
 def _apart(what: str, out: torch.Tensor, *tensors: torch.Tensor) -> None:
-    if any(_overlap(out, t) for t in tensors):
-        raise ValueError(f"{what}: the result's memory is that of an operand")
+    if not out.numel():
+        return
+    lo, hi = out.data_ptr(), _end(out)
+    for t in tensors:
+        at = t.data_ptr()
+        if at < hi and (at >= lo or _end(t) > lo) and _overlap(out, t):
+            raise ValueError(f"{what}: the result's memory is that of an operand")
 
 
 def plan(starts: torch.Tensor, tokens: int) -> PackedPlan:
@@ -189,6 +199,23 @@ def _layout(what, q_shape, q_stride, k_shape, k_stride, v_shape, v_stride, q_dty
     return (q_shape[1] // head_dim, k_shape[1] // head_dim, scale, *steps)
 
 
+@functools.lru_cache(maxsize=256)
+def _backward_layout(forward, o_shape, o_stride, o_dtype, d_shape, d_stride, d_dtype, lse_shape, lse_dtype, lse_side_by_side, batch, device):
+    """The checks of the gradients; (query heads, key-value heads, scale, elements between the rows of q, k, v, o and dout or None, columns of dq, dk and
+    dv, their sum, bytes of scratch)."""
+    q_shape, q_dtype, tokens, head_dim = forward[0], forward[6], forward[9], forward[10]
+    hq, hk, scale, *steps = _layout("attention_backward", *forward)
+    if o_shape != q_shape or d_shape != q_shape or o_dtype is not q_dtype or d_dtype is not q_dtype:
+        raise ValueError(f"attention_backward: o and dout must be {q_dtype} {list(q_shape)}")
+    if lse_shape != (hq, tokens) or lse_dtype is not torch.float32 or not lse_side_by_side:
+        raise ValueError(f"attention_backward: lse must be a contiguous float32 tensor [{hq}, {tokens}]")
+    half = q_dtype is torch.bfloat16
+    steps += [_kernel_step(o_shape, o_stride, half), _kernel_step(d_shape, d_stride, half)]
+    cols = [hq * head_dim, hk * head_dim, hk * head_dim]
+    need = N.require().oa_packed_attn_bwd_scratch_bytes(tokens, batch, hq, hk, head_dim) if half and device >= 0 else 0
+    return hq, hk, scale, steps, cols, sum(cols), need
+
+
 def _kernel_step(shape, stride, half: bool) -> Optional[int]:
     """As _step; the bf16 kernels also want rows 16 bytes apart."""
     step = _step(shape, stride)
@@ -253,14 +280,9 @@ def attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: tor
     allowed).  They are slices of `dqkv` [tokens, (q_heads + 2 kv_heads) * head_dim], a packed projection's gradient.  Those of a key-value head are the
     sums over the query heads that share it, added up in one order: the same inputs give the same bits.  Rows of no sequence are 0."""
     device = _together("attention_backward", q, k, v, o, dout, lse, plan.starts)
-    hq, hk, scale, *steps = _layout("attention_backward", q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, plan.tokens,
-                                    head_dim, scale, device >= 0)
-    if o.shape != q.shape or dout.shape != q.shape or o.dtype is not q.dtype or dout.dtype is not q.dtype:
-        raise ValueError(f"attention_backward: o and dout must be {q.dtype} {list(q.shape)}")
-    if lse.shape != (hq, plan.tokens) or lse.dtype is not torch.float32 or not lse.is_contiguous():
-        raise ValueError(f"attention_backward: lse must be a contiguous float32 tensor [{hq}, {plan.tokens}]")
-    cols = [hq * head_dim, hk * head_dim, hk * head_dim]
-    width = sum(cols)
+    hq, hk, scale, steps, cols, width, need = _backward_layout(
+        (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, plan.tokens, head_dim, scale, device >= 0),
+        o.shape, o.stride(), o.dtype, dout.shape, dout.stride(), dout.dtype, lse.shape, lse.dtype, lse.is_contiguous(), plan.batch, device)
     if dqkv is None:
         dqkv = q.new_empty((plan.tokens, width))
     else:
@@ -280,18 +302,17 @@ def attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: tor
             to.copy_(g) if g is not None else to.zero_()
         return grads
     half = q.dtype is torch.bfloat16
-    (q, qs), (k, ks), (v, vs), (o, os), (dout, dos) = _operands(half, (q, steps[0]), (k, steps[1]), (v, steps[2]), (o, _kernel_step(o.shape, o.stride(), half)),
-                                                                (dout, _kernel_step(dout.shape, dout.stride(), half)))
+    (q, qs), (k, ks), (v, vs), (o, os), (dout, dos) = _operands(half, (q, steps[0]), (k, steps[1]), (v, steps[2]), (o, steps[3]), (dout, steps[4]))
     at = dqkv.data_ptr()
     size = dqkv.element_size()
     dk, dv = at + cols[0] * size, at + (cols[0] + cols[1]) * size
     if half:
         # scratch of the call's own: calls on several streams, and graphs, do not meet in it
-        need = N.require().oa_packed_attn_bwd_scratch_bytes(plan.tokens, plan.batch, hq, hk, head_dim)
         scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
         K._launch(N.require().oa_packed_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr(), lse.data_ptr(), plan.words.data_ptr(), at, dk, dv,
                                                  plan.tokens, plan.batch, hq, hk, head_dim, qs, ks, vs, os, dos, width, width, width, scale, scratch.data_ptr(),
-                                                 K.status_word(q.device).data_ptr(), _stream(device)), "oa_packed_attn_bwd", 4, outputs=(dqkv,))
+                                                 K.status_word(q.device).data_ptr(), _stream(device)), "oa_packed_attn_bwd",
+                  5 if need > 8 * hq * plan.tokens + 12 else 4, outputs=(dqkv,))      # a fifth where partial sums are joined
     else:
         K._launch(N.require().oa_packed_attn_f32_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr(), lse.data_ptr(), plan.words.data_ptr(), at, dk, dv,
                                                      plan.tokens, plan.batch, hq, hk, head_dim, qs, ks, vs, os, dos, width, width, width, scale, _stream(device)),

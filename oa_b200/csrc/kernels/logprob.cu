@@ -7,14 +7,14 @@
 // A logit of -inf has probability 0 and adds nothing anywhere.  A row with NaN or +inf is NaN; a row without anything above -inf has
 // log-probability -inf, entropy 0 and no gradient.
 //
-// Forward reads a row once, in 16-byte pieces, four to a thread under way: every thread sums below a maximum of its own, and the threads meet at the
+// Forward reads a row once, in 16-byte pieces, four to eight to a thread under way: every thread sums below a maximum of its own, and the threads meet at the
 // end.  The alternatives cost no second pass: the k-th largest of the threads' maxima has k elements at or above it, so it is a bound that few others
 // reach, and only the threads whose maximum does read their pieces again, from L2.  Long rows of which there are few are cut over a cluster of CTAs
 // that meet in distributed shared memory; short ones share a warp.  Backward is one pass.
 //
-// fp32 is bound by the bytes: 4096 x 32000 87.5 us, 6.0 TB/s.  bf16 has an exponential to every two bytes and stays behind them: 52.6 us, 5.0 TB/s (issue slots 58 % busy,
-// the exponentials' unit 57 %), with five alternatives 64.4, the gradient 89.4 (read and written: 5.9 TB/s).  Few rows are latency: 32 x 201088 8 us, with
-// twenty alternatives 13.5.
+// fp32 is bound by the bytes: 16384 x 32000 297 us, 7.1 TB/s.  bf16 has an exponential to every two bytes and stays behind them: 187 us, 5.6 TB/s (issue slots 58 % busy,
+// the exponentials' unit 57 %), with five alternatives 226, the gradient 350 (read and written: 6.0 TB/s).  Few rows are latency: 32 x 201088 8.5 us, with
+// twenty alternatives 13.8.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -338,36 +338,39 @@ __device__ __forceinline__ float lp_both(u64 v) {
   return __uint_as_float(a) + __uint_as_float(b);
 }
 
-// The sums of pieces p0 + tid + i THREADS below p1, and the largest logit there
-template <typename T, int THREADS>
+// Teams of a block have more on its way, as far as registers go.  16384 x 32000 with 4 / 5 / 6 / 8: fp32 322 / 315 / 309 / 297 us, with five alternatives 393 / 385 / 374 / 369 (but
+// 32 x 201088 12.5 / 12.7 / 12.8 / 13.7), bf16 189 / 187 / 187 / 186 and 230 / 227 / 226 / 282, which spills.
+template <typename T, int THREADS, bool TOP> constexpr int LP_DEEP = THREADS < 128 ? LP_BATCH : sizeof(T) == 4 && !TOP ? 8 : 6;
+// The sums of pieces p0 + tid + i THREADS below p1, and the largest logit there; BATCH: pieces of a thread under way
+template <typename T, int THREADS, int BATCH>
 __device__ __forceinline__ LpSums lp_sums(const LpRow<T>& row, int p0, int p1, int tid, float scale, float& tmax) {
   LpSums a{-INFINITY, 0.f, 0.f};
   const u64 scale2 = f2_splat(scale);
   tmax = -INFINITY;
-  LpPiece<T> v[LP_BATCH];
+  LpPiece<T> v[BATCH];
 #pragma unroll
-  for (int b = 0; b < LP_BATCH; ++b)
+  for (int b = 0; b < BATCH; ++b)
     if (p0 + tid + b * THREADS < p1) row.load(v[b], p0 + tid + b * THREADS);
-  for (int q = p0 + tid; q < p1; q += LP_BATCH * THREADS) {
+  for (int q = p0 + tid; q < p1; q += BATCH * THREADS) {
 #pragma unroll
-    for (int b = 0; b < LP_BATCH; ++b)
+    for (int b = 0; b < BATCH; ++b)
       if (q + b * THREADS < p1) tmax = fmaxf(tmax, v[b].largest());
     const float top = tmax * scale;
     if (top > a.m) a.raise(top);
     const u64 neg_m2 = f2_splat(a.m == -INFINITY ? 0.f : -a.m);
     u64 l2 = 0, s2 = 0;
 #pragma unroll
-    for (int b = 0; b < LP_BATCH; ++b)
+    for (int b = 0; b < BATCH; ++b)
       if (q + b * THREADS < p1) {
         lp_add<false>(v[b], scale2, neg_m2, l2, s2);
-        const int next = q + (LP_BATCH + b) * THREADS;      // the place that is free again takes the next step's piece
+        const int next = q + (BATCH + b) * THREADS;      // the place that is free again takes the next step's piece
         if (next < p1) row.load(v[b], next);
       }
     float s1 = lp_both(s2);
     if (s1 != s1) {
       l2 = s2 = 0;
 #pragma unroll 1
-      for (int i = q; i < p1 && i < q + LP_BATCH * THREADS; i += THREADS) {
+      for (int i = q; i < p1 && i < q + BATCH * THREADS; i += THREADS) {
         LpPiece<T> again;
         row.load(again, i);
         lp_add<true>(again, scale2, neg_m2, l2, s2);
@@ -415,7 +418,7 @@ __global__ void __launch_bounds__(THREADS == 128 ? 128 : 256, THREADS == 128 ? 8
   const LpRow<T> row(static_cast<const T*>(p.x) + r * p.stride, p.vocab);
   const int all = row.pieces(), per = (all + parts - 1) / parts, p0 = min(part * per, all), p1 = min(p0 + per, all);
   float tmax;                              // of the logits themselves
-  LpSums a = lp_sums<T, THREADS>(row, p0, p1, tid, p.scale, tmax);
+  LpSums a = lp_sums<T, THREADS, LP_DEEP<T, THREADS, TOP>>(row, p0, p1, tid, p.scale, tmax);
   a = lp_warp_join(a);
   if (THREADS > 32) {
     if (lane == 0) s.sums[warp] = a;
@@ -459,7 +462,7 @@ __global__ void __launch_bounds__(256, 4) logprob_short_kernel(const __grid_cons
   const int r = blockIdx.x * (256 / LP_LANES) + threadIdx.x / LP_LANES, tid = threadIdx.x % LP_LANES;
   const LpRow<T> row(static_cast<const T*>(p.x) + (r < p.rows ? r : 0) * p.stride, p.vocab);
   float tmax;
-  const LpSums a = lp_warp_join(lp_sums<T, LP_LANES>(row, 0, r < p.rows ? row.pieces() : 0, tid, p.scale, tmax), LP_LANES);
+  const LpSums a = lp_warp_join(lp_sums<T, LP_LANES, LP_BATCH>(row, 0, r < p.rows ? row.pieces() : 0, tid, p.scale, tmax), LP_LANES);
   if (tid == 0 && r < p.rows) lp_write(p, row, r, a, LpResult(a, p.scale));
 }
 

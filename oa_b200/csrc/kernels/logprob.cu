@@ -13,7 +13,7 @@
 // that meet in distributed shared memory; short ones share a warp.  Backward is one pass.
 //
 // fp32 is bound by the bytes: 16384 x 32000 297 us, 7.1 TB/s.  bf16 has an exponential to every two bytes and stays behind them: 187 us, 5.6 TB/s (issue slots 58 % busy,
-// the exponentials' unit 57 %), with five alternatives 226, the gradient 350 (read and written: 6.0 TB/s).  Few rows are latency: 32 x 201088 8.5 us, with
+// the exponentials' unit 57 %), with five alternatives 225, the gradient 350 (read and written: 6.0 TB/s).  Few rows are latency: 32 x 201088 8.5 us, with
 // twenty alternatives 13.8.
 #include <cooperative_groups.h>
 
@@ -195,7 +195,7 @@ __device__ __forceinline__ void lp_top(S& s, const LpRow<T>& row, int p0, int p1
     for (int i = 1; i < S::GROUPS / 32; ++i) { hi = max(hi, mine[i]); lo = min(lo, mine[i]); }
     hi = __reduce_max_sync(0xffffffffu, hi);
     lo = __reduce_min_sync(0xffffffffu, lo);
-    uint32_t bit = hi == lo ? 0 : 1u << (31 - __clz(hi ^ lo));             // the first in which they differ
+    uint32_t bit = top == 1 || hi == lo ? 0 : 1u << (31 - __clz(hi ^ lo));       // the first in which they differ; one alternative is at the largest maximum
     bound = bit ? hi & ~(2 * bit - 1) : hi;
 #pragma unroll 1
     for (; bit > LOW; bit >>= 1) {
@@ -204,6 +204,7 @@ __device__ __forceinline__ void lp_top(S& s, const LpRow<T>& row, int p0, int p1
 #pragma unroll
       for (int i = 0; i < S::GROUPS / 32; ++i) n += __popc(__ballot_sync(0xffffffffu, mine[i] >= c));
       if (n >= top) bound = c;
+      if (n == top) break;                 // a closer one would leave out little more
     }
     if (lane == 0) s.bound = bound;
   }

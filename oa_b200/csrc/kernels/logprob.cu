@@ -588,8 +588,9 @@ static int logprob_run(const LogprobParams& p, cudaStream_t st) {
 
 template <typename T>
 static int logprob_bwd_run(LogprobBwdParams& p, cudaStream_t st) {
-  // threads to a row that four pieces each fill, and as many blocks side by side as it then still takes
-  const long long pieces = (long long)p.vocab / LpPiece<T>::N + 2;
+  // threads to a row that four pieces each fill, and as many blocks side by side as it then still takes; a row that does not begin on 16 bytes has a piece more, for
+  // which the loop goes round again (200000 x 256 in bf16, with threads for that piece too / without: 55 / 43 us)
+  const long long pieces = ((long long)p.vocab + LpPiece<T>::N - 1) / LpPiece<T>::N;
   p.team_log2 = 3;
   while (p.team_log2 < 8 && (LP_BATCH << p.team_log2) < pieces) ++p.team_log2;
   const long long parts = (pieces + (LP_BATCH << p.team_log2) - 1) / (LP_BATCH << p.team_log2);

@@ -12,9 +12,9 @@
 // reach, and only the threads whose maximum does read their pieces again, from L2.  Long rows of which there are few are cut over a cluster of CTAs
 // that meet in distributed shared memory; short ones share a warp.  Backward is one pass.
 //
-// fp32 is bound by the bytes: 16384 x 32000 297 us, 7.1 TB/s.  bf16 has an exponential to every two bytes and stays behind them: 187 us, 5.6 TB/s (issue slots 58 % busy,
-// the exponentials' unit 57 %), with five alternatives 225, the gradient 350 (read and written: 6.0 TB/s).  Few rows are latency: 32 x 201088 8.5 us, with
-// twenty alternatives 13.8.
+// fp32 is bound by the bytes: 16384 x 32000 297 us, 7.1 TB/s.  bf16 has an exponential to every two bytes and stays behind them: 189 us, 5.6 TB/s (issue slots 58 % busy,
+// the exponentials' unit 57 %), with five alternatives 229, the gradient 343 (read and written: 6.1 TB/s).  Few rows are latency: 32 x 201088 8.2 us, with
+// twenty alternatives 13.5.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -339,9 +339,10 @@ __device__ __forceinline__ float lp_both(u64 v) {
   return __uint_as_float(a) + __uint_as_float(b);
 }
 
-// Teams of a block have more on its way, as far as registers go.  16384 x 32000 with 4 / 5 / 6 / 8: fp32 322 / 315 / 309 / 297 us, with five alternatives 393 / 385 / 374 / 369 (but
-// 32 x 201088 12.5 / 12.7 / 12.8 / 13.7), bf16 189 / 187 / 187 / 186 and 230 / 227 / 226 / 282, which spills.
-template <typename T, int THREADS, bool TOP> constexpr int LP_DEEP = THREADS < 128 ? LP_BATCH : sizeof(T) == 4 && !TOP ? 8 : 6;
+// fp32 teams of a block have more under way, as far as registers go: 16384 x 32000 with 4 / 5 / 6 / 8 322 / 315 / 309 / 297 us, with five alternatives 393 / 385 / 374 / 369 (but
+// 32 x 201088 12.5 / 12.7 / 12.8 / 13.7).  bf16 with 4 / 6: one call after the other on the same logits 189 / 187 and 230 / 226, on others each time, out of memory, 4096 x 32000 with
+// five alternatives 68.1 / 69.5 and 16384 x 32000 with its gradient 592 / 600.
+template <typename T, int THREADS, bool TOP> constexpr int LP_DEEP = sizeof(T) == 2 || THREADS < 128 ? LP_BATCH : TOP ? 6 : 8;
 // The sums of pieces p0 + tid + i THREADS below p1, and the largest logit there; BATCH: pieces of a thread under way
 template <typename T, int THREADS, int BATCH>
 __device__ __forceinline__ LpSums lp_sums(const LpRow<T>& row, int p0, int p1, int tid, float scale, float& tmax) {

@@ -82,6 +82,18 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int lane) {
     for (int i = from * 8 + lane; i < FA_BM * 8; i += 32) reinterpret_cast<uint4*>(tile + x * (FA_BM * 128))[i] = make_uint4(0, 0, 0, 0);
 }
 
+// A wait that spans other warps' work on whole items (their blocks may be so many that it outlasts the limit of a wait for one): the limit runs anew
+// as long as `pulse`, in shared memory, moves with the blocks that the loading warp sends for.  Its own waits are for one block each, so this one ends too.
+__device__ __forceinline__ bool idle_wait(uint64_t* bar, uint32_t parity, const volatile uint32_t* pulse) {
+  uint32_t seen = __shfl_sync(0xffffffffu, *pulse, 0);
+  while (!warp_wait(bar, parity)) {
+    const uint32_t now = __shfl_sync(0xffffffffu, *pulse, 0);
+    if (now == seen) return false;
+    seen = now;
+  }
+  return true;
+}
+
 // Rows that belong to no sequence become zeros: `cols` bf16, a multiple of 8, by `threads` threads of every CTA
 __device__ __forceinline__ void clear_others(const PackedPlan& plan, __nv_bfloat16* base, long long stride, int cols, int tid, int threads) {
   plan.others(blockIdx.x, gridDim.x, [&](int r) {
@@ -172,6 +184,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* o_done = s_full + 8;           // [2]   O_t += P_t V_j finished: P_t may be overwritten, O_t may be rescaled
   uint64_t* v_part = s_full + 10;          // [NS]  the values of a sequence's last block are there, and some rows of others
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_part + NS);
+  volatile uint32_t* pulse = tmem_slot + 1;   // blocks sent for
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -185,6 +198,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     for (int s = 0; s < NS; ++s) { mbar_init(&k_full[s], 1); mbar_init(&v_full[s], 1); mbar_init(&k_empty[s], Cfg::MMA_WARPS); mbar_init(&v_empty[s], Cfg::MMA_WARPS); }
     for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&s_empty[t], 4); mbar_init(&p_full[2 * t], 4); mbar_init(&p_full[2 * t + 1], 4); mbar_init(&o_done[t], 1); }
     for (int s = 0; s < NS; ++s) mbar_init(&v_part[s], 1);
+    *pulse = 0;
     mbar_fence_init();
   }
   if (warp == 8) { tmem_alloc<Cfg::TMEM_COLS>(tmem_slot); tmem_relinquish(); }
@@ -229,6 +243,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (!warp_wait(&v_empty[st], ph ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
           if (elect_one()) {
             uint64_t* bar = row + FA_BN > it.hi ? &v_part[st] : &v_full[st];
+            *pulse = blk + 1;
             mbar_expect_tx(bar, Cfg::KV_BYTES);
 #pragma unroll
             for (int x = 0; x < HD / 64; ++x)
@@ -247,7 +262,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         blk += n_it;
         if (row + FA_BN <= it.hi) continue;
         const int st = (blk - 1) % NS;
-        if (!warp_wait(&v_part[st], (phases >> st) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+        // from the last such item to this one's last block
+        if (!idle_wait(&v_part[st], (phases >> st) & 1, pulse)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
         phases ^= 1u << st;
         clear_rows<HD>(smem + Cfg::OFF_V + st * Cfg::KV_BYTES, it.hi - row, lane);
         fence_proxy_async_smem();
@@ -403,7 +419,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const float sl2 = p.scale * LOG2E;
     const int o_stride = p.q_heads * HD;
     uint32_t sc = 0, pc = 0;     // score tiles consumed and P V completions awaited so far
-    bool ok = true;
+    bool ok = true, idle = false;
     clear_others(p.plan, p.o, o_stride, o_stride, threadIdx.x, 256);
     if (p.lse)
       p.plan.others(blockIdx.x, gridDim.x, [&](int row) {
@@ -412,7 +428,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     while (ok && walk.next(entry, which)) {
       const int tile = HEADS ? entry.z : 2 * entry.z + t, head = HEADS ? 2 * which + t : which, hi = entry.y;
       const int q0 = entry.x + tile * FA_BM + quad * 32;    // this warp's first row
-      if (entry.x + tile * FA_BM >= hi) continue;
+      if (entry.x + tile * FA_BM >= hi) { idle = true; continue; }
+      if (!HEADS && idle) {          // the other tile alone has been worked on since
+        idle = false;
+        ok = idle_wait(&s_full[t], sc & 1, pulse);
+        if (!ok) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_TMEM_FULL); break; }
+      }
       const int n = tile + 1;
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = 0; j < n; ++j, ++sc) {
@@ -1049,6 +1070,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint64_t* v_part = bars + 29;    // [3]
   uint64_t* x_full = bars + 32;    // [4]  sums of the two warps that share 32 rows are in xch
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 36);
+  volatile uint32_t* pulse = tmem_slot + 1;   // blocks sent for
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -1069,6 +1091,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     mbar_init(fin_full, 1);
     for (int s = 0; s < NK; ++s) mbar_init(&k_part[s], 1);
     for (int s = 0; s < NV; ++s) mbar_init(&v_part[s], 1);
+    *pulse = 0;
     mbar_fence_init();
   }
   if (warp == 8) { tmem_alloc<Cfg::TMEM_COLS>(tmem_slot); tmem_relinquish(); }
@@ -1105,6 +1128,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (!warp_wait(&k_empty[sk], ((kc / NK) & 1) ^ 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_EMPTY); ok = false; break; }
           if (elect_one()) {
             uint64_t* bar = part ? &k_part[sk] : &k_full[sk];
+            *pulse = kc + 1;
             mbar_expect_tx(bar, Cfg::T_BYTES);
 #pragma unroll
             for (int x = 0; x < HD / 64; ++x) tma_load_2d(k_tile + x * (FA_BN * 128), &tmK, bar, hk * HD + x * 64, row);
@@ -1128,7 +1152,8 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         kc += entry.z + 1;
         if (from >= FA_BN) continue;
         const int sk = (kc - 1) % NK, sv = (kc - 1) % NV;
-        if (!warp_wait(&k_part[sk], (k_phases >> sk) & 1)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
+        // from the last such item to this one's last block
+        if (!idle_wait(&k_part[sk], (k_phases >> sk) & 1, pulse)) { if (lane == 0) report_error(p.status, OA_KERR_WAIT_FULL); break; }
         clear_rows<HD>(smem + Cfg::OFF_K + sk * Cfg::T_BYTES, from, lane);
         fence_proxy_async_smem();
         __syncwarp();

@@ -9,6 +9,7 @@ import math
 import pytest
 import torch
 
+from oa_b200.ops import kernels as K
 from oa_b200.ops import packed as P
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -548,3 +549,43 @@ def test_rows_beyond_32_bits(dtype):
         assert torch.equal(g[:, tokens - n:] if name == "lse" else g[tokens - n:], w), name
         rest = g[:, :tokens - n] if name == "lse" else g[:tokens - n]
         assert all((part == (-math.inf if name == "lse" else 0)).all() for part in rest.split(1 << 16)), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,hq,tiles,back", [(64, 1, 34001, True), (128, 2, 22001, False)])
+def test_waits_for_a_sequence_that_takes_seconds(hd, hq, tiles, back):
+    """A ragged sequence behind one of whole tiles that every CTA works on for longer than the 2 s that a wait for one block may take: the ragged one has the bits
+    that it has alone, and the long one's last rows are those of the definition."""
+    K.check_status()
+    n, m = 128 * tiles, 200
+    g = torch.Generator(device="cuda").manual_seed(7)
+    qkv = torch.randn(n + m, (hq + 2) * hd, generator=g, device="cuda").bfloat16()
+    q, k, v = torch.split(qkv, [hq * hd, hd, hd], 1)
+    v += 1                                                        # so that the means of millions of them are not 0
+    plan, alone = P.plan(_starts([n, m], "cuda"), n + m), P.plan(_starts([m], "cuda"), m)
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    begin.record()
+    o, lse = P.attention(q, k, v, plan, hd, return_lse=True)
+    end.record()
+    end.synchronize()
+    K.check_status()
+    assert begin.elapsed_time(end) > 2000
+    short = [t[n:].contiguous() for t in (q, k, v)]
+    want, want_lse = P.attention(*short, alone, hd, return_lse=True)
+    assert torch.equal(o[n:], want) and torch.equal(lse[:, n:], want_lse)
+    for i in (n - 1, n - 128, n - 129):
+        x = (k[:i + 1].double() @ q[i].double().reshape(hq, hd).t()).t() * hd ** -0.5
+        p = torch.softmax(x, -1)
+        y = p @ v[:i + 1].double()
+        # the result's rounding and the weights'; products added up in 32 bits sixteen keys at a time, 8 additions to a tile that may be cut off (2^-23), and the
+        # weights a tile at a time
+        bound = 2.0 ** -8 * y.abs() + (2.0 ** -8 + (128 + 17 * tiles) * 2.0 ** -24 + 2.0 ** -15) * (p @ v[:i + 1].double().abs())
+        _close("o", o[i].reshape(hq, hd), y.cpu(), bound.cpu())
+    if not back:
+        return
+    dout = torch.randn(n + m, hq * hd, generator=g, device="cuda").bfloat16()
+    dqkv = torch.full_like(qkv, math.nan)
+    P.attention_backward(q, k, v, o, dout, lse, plan, hd, dqkv=dqkv)
+    K.check_status()
+    assert bool(dqkv.isfinite().all())
+    assert torch.equal(dqkv[n:], torch.cat(P.attention_backward(*short, want, dout[n:].contiguous(), want_lse, alone, hd), 1))

@@ -1021,11 +1021,18 @@ def PackedSequences(starts: OaMatrix, tokens: int, positions: Optional[OaMatrix]
 
 
 def RotaryAxes(x: OaMatrix, positions: OaMatrix, pair_axes: Sequence[int], heads: int, head_dim: int, theta: float = 10000.0) -> OaMatrix:
-    """Rotary embedding of [tokens, heads*head_dim] rows by their positions [axes, tokens]: pair j of a head turns with axis pair_axes[j]."""
+    """Rotary embedding of the first `heads` heads of [tokens, >= heads*head_dim] rows by their positions [axes, tokens]: pair j of a head turns with axis
+    pair_axes[j].  Returns [tokens, heads*head_dim]; columns behind those heads are not in it."""
     _ctx_add("RotaryAxes")
     t, pos, axes = x.Tensor(), positions.Tensor(), tuple(pair_axes)
     out = _w(PK.rotary(t, pos, axes, heads, head_dim, theta))
-    return AG.attach("RotaryAxes", out, [x], lambda g: (PK.rotary(_c(g), pos, axes, heads, head_dim, theta, backward=True),))
+
+    def back(g):
+        wide = None if t.shape[1] == heads * head_dim else torch.zeros(t.shape, dtype=t.dtype, device=t.device)
+        d = PK.rotary(_c(g), pos, axes, heads, head_dim, theta, backward=True, out=wide)
+        return (d if wide is None else wide,)
+
+    return AG.attach("RotaryAxes", out, [x], back)
 
 
 def PackedAttention(qkv: OaMatrix, sequences: OaPackedSequences, heads: int, kv_heads: int, head_dim: int, *, rope_theta: float = 0.0,

@@ -194,3 +194,20 @@ def test_gradient_of_rotary_axes(device):
     a = x.Tensor()
     lhs, rhs = (packed.rotary(a, pos, axes, 2, 64, 10000.0) * w).sum(), (a * x.GradTensor()).sum()
     assert abs(float(lhs - rhs)) <= 768 * 2.0 ** -23 * float((a.abs() * w.abs()).sum())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradient_of_rotary_axes_over_the_first_columns(device, dtype):
+    """Rows wider than the heads that are turned: the other columns are not in the result, and their gradient is 0."""
+    g = torch.Generator().manual_seed(0)
+    x = OaMatrix(torch.randn(6, 200, generator=g).to(dtype).to(device)).SetRequiresGrad(True)
+    pos = torch.randint(0, 50, (1, 6), generator=g, dtype=torch.int32).to(device)
+    w = torch.randn(6, 128, generator=g).to(dtype).to(device)
+    with AG.OaGradientTape() as tape:
+        y = F.RotaryAxes(x, OaMatrix(pos), (0,) * 32, 2, 64)
+        assert y.Tensor().shape == (6, 128)
+        tape.Backward(_weighted(y, w))
+    got = x.GradTensor()
+    assert got.shape == (6, 200) and bool((got[:, 128:] == 0).all())
+    assert torch.equal(got[:, :128], packed.rotary(w, pos, (0,) * 32, 2, 64, 10000.0, backward=True))

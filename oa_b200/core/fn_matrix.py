@@ -1000,7 +1000,7 @@ class OaPackedSequences:
 
     def __init__(self, plan: PK.PackedPlan, positions: torch.Tensor, pair_axes: Optional[Sequence[int]] = None):
         self.Plan, self.Positions = plan, positions
-        self.PairAxes = None if pair_axes is None else tuple(pair_axes)
+        self.PairAxes = None if pair_axes is None else tuple(map(int, pair_axes))
 
     def Tokens(self) -> int:
         return self.Plan.tokens
@@ -1024,7 +1024,7 @@ def RotaryAxes(x: OaMatrix, positions: OaMatrix, pair_axes: Sequence[int], heads
     """Rotary embedding of the first `heads` heads of [tokens, >= heads*head_dim] rows by their positions [axes, tokens]: pair j of a head turns with axis
     pair_axes[j].  Returns [tokens, heads*head_dim]; columns behind those heads are not in it."""
     _ctx_add("RotaryAxes")
-    t, pos, axes = x.Tensor(), positions.Tensor(), tuple(pair_axes)
+    t, pos, axes = x.Tensor(), positions.Tensor(), tuple(map(int, pair_axes))
     out = _w(PK.rotary(t, pos, axes, heads, head_dim, theta))
 
     def back(g):

@@ -13,7 +13,7 @@ import torch
 
 from .. import _native as N
 from . import kernels as K
-from .packed import _copied, _overlap, _step, _stream, _together
+from .packed import _copied, _overlap, _step, _stream, _together, _whole
 
 MAX_TOP = 32
 
@@ -54,6 +54,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0, sc
     the `top` likeliest tokens (at most 32) with theirs; equal logits rank by index.  A target of ignore_index has log-probability 0, any other that is
     no token NaN.  Logits of -inf have probability 0; a row with NaN or +inf is NaN; one without anything above -inf has log-probabilities of
     -inf and entropy 0."""
+    scale, top, ignore_index = float(scale), _whole(top), _whole(ignore_index)
     step = _layout("token_logprobs", logits.shape, logits.stride(), logits.dtype, targets.shape, targets.stride(), targets.dtype, scale, top, ignore_index)
     device = _together("token_logprobs", logits, targets)
     if device < 0:
@@ -101,6 +102,7 @@ def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, result:
     """The logits' gradient from those of the log-probabilities and of the entropy ([rows] fp32, or None for none), given what `token_logprobs` returned
     for the same logits, targets, scale and ignore_index.  `out` (row stride allowed) may be the logits themselves.  A row whose target is ignore_index
     takes no part in dlogprobs; one with another target that is no token is NaN; one without anything above -inf is 0."""
+    scale, ignore_index = float(scale), _whole(ignore_index)
     step = _layout("token_logprobs_backward", logits.shape, logits.stride(), logits.dtype, targets.shape, targets.stride(), targets.dtype, scale, 0, ignore_index)
     rows, vocab = logits.shape
     for name, t, shape in (("dlogprobs", dlogprobs, (rows,)), ("dentropy", dentropy, (rows,)), ("result.entropy", result.entropy, (rows,)),

@@ -48,6 +48,11 @@ def _together(what: str, first: torch.Tensor, *tensors: torch.Tensor) -> int:
     return at
 
 
+def _whole(x) -> int:
+    """What the checks below are remembered by has to be plain numbers: a tensor is the same key whatever it holds by now."""
+    return x if type(x) is int else operator.index(x)
+
+
 def _stream(device: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
@@ -97,6 +102,7 @@ def _apart(what: str, out: torch.Tensor, *tensors: torch.Tensor) -> None:
 def plan(starts: torch.Tensor, tokens: int) -> PackedPlan:
     """What `attention` needs to know about sequences whose rows begin at `starts` [batch + 1] (int32; the last entry is the end of the last one) in
     tensors of `tokens` rows.  Starts that fall, or leave [0, tokens], count as the nearest ones that do not.  Nothing is read back to the host."""
+    tokens = _whole(tokens)
     if starts.dtype is not torch.int32 or starts.dim() != 1 or not starts.is_contiguous() or starts.numel() < 1:
         raise ValueError("plan: starts must be a contiguous int32 tensor [batch + 1]")
     batch = starts.numel() - 1
@@ -123,7 +129,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, pair_axes: Sequence[int], h
     2 len(pair_axes) on stay as they are.  One axis and half the head's dimensions make the usual rotary embedding.  `backward`: the other way round,
     which is the gradient.  Returns [tokens, heads * head_dim], the first columns of `out` if given, which may be x itself but not overlap it otherwise."""
     if type(pair_axes) is not tuple:
-        pair_axes = tuple(pair_axes)
+        pair_axes = tuple(map(operator.index, pair_axes))
+    heads, head_dim, theta = _whole(heads), _whole(head_dim), float(theta)
     step, axes, turns = _rotary_layout(x.shape, x.stride(), x.dtype, positions.shape, positions.stride(), positions.dtype, pair_axes, heads, head_dim, theta)
     tokens, cols = x.shape[0], heads * head_dim
     if out is None:
@@ -167,6 +174,8 @@ def _rotary_layout(shape, stride, dtype, p_shape, p_stride, p_dtype, pair_axes, 
     if p_dtype is not torch.int32 or len(p_shape) != 2 or p_shape[1] != shape[0] or not 1 <= p_shape[0] <= MAX_AXES \
             or (p_shape[1] > 1 and p_stride[1] != 1) or (p_shape[0] > 1 and 0 < p_shape[1] != p_stride[0]):
         raise ValueError(f"rotary: positions must be a contiguous int32 tensor [axes, {shape[0]}] of at most {MAX_AXES} axes")
+    if any(isinstance(a, torch.Tensor) for a in pair_axes):
+        raise ValueError("rotary: pair_axes must be whole numbers, not tensors")
     if not all(0 <= operator.index(a) < p_shape[0] for a in pair_axes):
         raise ValueError(f"rotary: pair_axes names axes that positions [{p_shape[0]}, tokens] do not have")
     if not 0 < theta < math.inf:
@@ -174,7 +183,7 @@ def _rotary_layout(shape, stride, dtype, p_shape, p_stride, p_dtype, pair_axes, 
     if shape[0] > 1 << 30 or heads * head_dim > 1 << 30:
         raise ValueError(f"rotary: {list(shape)} is too large")
     step = shape[1] if shape[0] <= 1 else stride[0]
-    return (step if stride[1] == 1 else None, *_rotary_tables(pair_axes, float(theta)))
+    return (step if stride[1] == 1 else None, *_rotary_tables(pair_axes, theta))
 
 
 @functools.lru_cache(maxsize=256)
@@ -192,7 +201,7 @@ def _layout(what, q_shape, q_stride, k_shape, k_stride, v_shape, v_stride, q_dty
             raise ValueError(f"{what}: bfloat16 heads of one of {HEAD_DIMS}, not of {head_dim}")
         if head_dim > 128:
             raise ValueError(f"{what}: heads of at most 128, not of {head_dim}")
-    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
     if not 0 < scale < math.inf:
         raise ValueError(f"{what}: scale must be positive, not {scale}")
     steps = [_kernel_step(*m, half) for m in ((q_shape, q_stride), (k_shape, k_stride), (v_shape, v_stride))]
@@ -235,6 +244,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPla
     bf16 (heads of 64 or 128) runs on the tensor cores: weights are rounded to bf16 before they meet the values, sums are fp32.  A value that is not finite
     may reach earlier tokens of its own sequence, as its weight there is 0 times it."""
     device = _together("attention", q, k, v, plan.starts)
+    head_dim, scale = _whole(head_dim), None if scale is None else float(scale)
     hq, hk, scale, *steps = _layout("attention", q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, plan.tokens, head_dim,
                                     scale, device >= 0)
     if device < 0:
@@ -280,6 +290,7 @@ def attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: tor
     allowed).  They are slices of `dqkv` [tokens, (q_heads + 2 kv_heads) * head_dim], a packed projection's gradient.  Those of a key-value head are the
     sums over the query heads that share it, added up in one order: the same inputs give the same bits.  Rows of no sequence are 0."""
     device = _together("attention_backward", q, k, v, o, dout, lse, plan.starts)
+    head_dim, scale = _whole(head_dim), None if scale is None else float(scale)
     hq, hk, scale, steps, cols, width, need = _backward_layout(
         (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, plan.tokens, head_dim, scale, device >= 0),
         o.shape, o.stride(), o.dtype, dout.shape, dout.stride(), dout.dtype, lse.shape, lse.dtype, lse.is_contiguous(), plan.batch, device)

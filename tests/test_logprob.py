@@ -341,3 +341,21 @@ def test_rows_beyond_32_bits(vocab):
     want = L.token_logprobs_backward(tail, targets[first:].clone(), s, g[first:].clone(), h[first:].clone())
     L.token_logprobs_backward(x, targets, r, g, h, out=x)
     assert torch.equal(x[first:], want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_scale_given_as_a_tensor(device):
+    """It is read at every call, not remembered by which tensor it was."""
+    x, t, g, h = (v.to(device) for v in _logits(3, 50, torch.float32))
+    scale = torch.tensor(1.0)
+    for s in (1.0, 0.25):
+        scale.fill_(s)
+        got, want = L.token_logprobs(x, t, 2, scale), L.token_logprobs(x, t, 2, s)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(L.token_logprobs_backward(x, t, got, g, h, scale), L.token_logprobs_backward(x, t, want, g, h, s))
+    for bad in (0.0, -1.0, INF):
+        scale.fill_(bad)
+        with pytest.raises(ValueError, match="scale must be positive"):
+            L.token_logprobs(x, t, 2, scale)
+        with pytest.raises(ValueError, match="scale must be positive"):
+            L.token_logprobs_backward(x, t, want, g, h, scale)

@@ -589,3 +589,28 @@ def test_waits_for_a_sequence_that_takes_seconds(hd, hq, tiles, back):
     K.check_status()
     assert bool(dqkv.isfinite().all())
     assert torch.equal(dqkv[n:], torch.cat(P.attention_backward(*short, want, dout[n:].contiguous(), want_lse, alone, hd), 1))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_numbers_given_as_tensors(device):
+    """A scale and a theta that are tensors are read at every call, not remembered by which tensor it was."""
+    q, k, v, dout = _inputs([9, 3], 2, 1, 64, torch.float32, device)
+    plan, pos = P.plan(_starts([9, 3], device), 12), torch.arange(12, dtype=torch.int32, device=device)[None]
+    scale, theta = torch.tensor(0.125), torch.tensor(10000.0)
+    for s, t in ((0.125, 10000.0), (0.5, 500.0)):
+        scale.fill_(s), theta.fill_(t)
+        o, lse = P.attention(q, k, v, plan, 64, scale, return_lse=True)
+        want, want_lse = P.attention(q, k, v, plan, 64, s, return_lse=True)
+        assert torch.equal(o, want) and torch.equal(lse, want_lse)
+        for a, b in zip(P.attention_backward(q, k, v, o, dout, lse, plan, 64, scale), P.attention_backward(q, k, v, o, dout, lse, plan, 64, s)):
+            assert torch.equal(a, b)
+        assert torch.equal(P.rotary(q, pos, (0,) * 32, 2, 64, theta), P.rotary(q, pos, (0,) * 32, 2, 64, t))
+    for bad in (0.0, -1.0, math.inf, math.nan):
+        scale.fill_(bad), theta.fill_(bad)
+        with pytest.raises(ValueError, match="scale must be positive"):
+            P.attention(q, k, v, plan, 64, scale)
+        with pytest.raises(ValueError, match="theta must be positive"):
+            P.rotary(q, pos, (0,) * 32, 2, 64, theta)
+    assert torch.equal(P.rotary(q, pos, torch.zeros(32, dtype=torch.int64), 2, 64, 500.0), P.rotary(q, pos, (0,) * 32, 2, 64, 500.0))
+    with pytest.raises(ValueError, match="whole numbers"):
+        P.rotary(q, pos, tuple(torch.zeros(32, dtype=torch.int64)), 2, 64, 500.0)

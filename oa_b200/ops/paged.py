@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 from typing import NamedTuple, Optional
 
 import torch
@@ -183,6 +184,7 @@ def append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, k_pa
     """New tokens' packed rows [tokens, (q_heads + 2 kv_heads) * head_dim] (row stride allowed): returns q [tokens, q_heads * head_dim], rotated by
     each token's own position (pairs j, j + head_dim / 2; theta <= 0: not rotated), and writes rotated k and v to their slots.  A slot that is
     not in the pool (-1) is left out."""
+    theta = float(theta)                    # what is worked out once is remembered by numbers: a tensor is the same key whatever it holds by now
     pages, kvh, ps, hd, k_step, v_step = _pool("append", k_pages.shape, k_pages.stride(), v_pages.shape, v_pages.stride(), k_pages.dtype, v_pages.dtype, qkv.dtype)
     tokens, width = qkv.shape if qkv.dim() == 2 else (-1, 0)
     qh = width // hd - 2 * kvh
@@ -224,7 +226,7 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tab
 
     bf16 with heads of 64 or 128, up to 2048 requests, runs on the tensor cores: weights are rounded to bf16 before they meet the values, sums are
     fp32, and a value of a request's new tokens that is not finite may reach its earlier new tokens too.  All else takes a block to a row."""
-    batch = lens.numel()
+    batch, max_fresh, prefix_len, scale = lens.numel(), operator.index(max_fresh), operator.index(prefix_len), None if scale is None else float(scale)
     (pages, kvh, ps, hd, k_step, v_step, tokens, cols, qh, width, table_stride, scale, need) = _attention_layout(
         q.shape, q.dtype, k_pages.shape, k_pages.stride(), v_pages.shape, v_pages.stride(), k_pages.dtype, v_pages.dtype, tables.shape, tables.stride(),
         tables.dtype, batch, starts.numel(), max_fresh, None if prefix_table is None else prefix_table.numel(), prefix_len, scale, q.get_device())
@@ -264,7 +266,7 @@ def _attention_layout(q_shape, dtype, k_shape, k_stride, v_shape, v_stride, k_dt
     if prefix_len > 0 and (n_prefix is None or n_prefix * ps < prefix_len):
         raise ValueError(f"attention: prefix_table holds fewer than {prefix_len} tokens")
     width, table_stride = _table_layout("attention", t_shape, t_stride, t_dtype, batch)
-    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(hd) if scale is None else scale
     qh = cols // hd
     code = K._DT.get(dtype) if device >= 0 else None
     need = N.require().oa_paged_attn_scratch_bytes(code, tokens, batch, max_fresh, qh, kvh, hd, pages, prefix_len, scale) if code is not None else 0

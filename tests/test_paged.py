@@ -392,3 +392,21 @@ def test_refusals_of_the_kernels():
     pool = z(4, 2, 16, 256, dtype=torch.bfloat16)
     with pytest.raises(N.OaKernelError):
         P.append(z(3, 8 * 256, dtype=torch.bfloat16), z(3), z(3), pool, pool, 1e4)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_numbers_given_as_tensors(device):
+    """A scale, a theta and lengths that are tensors are read at every call, not remembered by which tensor it was."""
+    g = torch.Generator().manual_seed(11)
+    k, v = (torch.randn(4, 1, 16, 64, generator=g).to(device) for _ in range(2))
+    q, table, lens, starts = torch.randn(2, 128, generator=g).to(device), _i32([[0, 1]], device), _i32([20], device), _i32([0, 2], device)
+    prefix = _i32([2, 3], device)
+    scale, theta, shared, fresh = torch.tensor(0.1), torch.tensor(10000.0), torch.tensor(0), torch.tensor(0)
+    for s, t, n, f in ((0.1, 10000.0, 17, 2), (0.4, 0.0, 30, 3), (0.2, 100.0, 5, 2)):
+        for a, b in ((scale, s), (theta, t), (shared, n), (fresh, f)):
+            a.fill_(b)
+        got, want = (P.attention(q, k, v, table, lens, starts, *a) for a in ((fresh, prefix, shared, scale), (f, prefix, n, s)))
+        assert torch.equal(got, want)
+        rows = torch.randn(2, 256, generator=g).to(device)
+        got, want = (P.append(rows, _i32([3, 70], device), _i32([5, -1], device), k.clone(), v.clone(), a) for a in (theta, t))
+        assert torch.equal(got, want)

@@ -1005,6 +1005,11 @@ class OaPackedSequences:
     def Tokens(self) -> int:
         return self.Plan.tokens
 
+    def Rows(self) -> torch.Tensor:
+        """[tokens] bool: the rows that belong to a sequence."""
+        row, starts = torch.arange(self.Plan.tokens, dtype=torch.int32, device=self.Plan.starts.device), self.Plan.starts
+        return (row >= starts[0]) & (row < starts[-1])
+
     def Axes(self, head_dim: int) -> tuple:
         return (0,) * (head_dim // 2) if self.PairAxes is None else self.PairAxes
 

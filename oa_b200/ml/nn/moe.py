@@ -138,8 +138,11 @@ class OaMoE(OaModule):
     def AuxLoss(self) -> OaMatrix: return self.LastAuxLoss
 
     # ---- forward
-    def Forward(self, x: OaMatrix) -> OaMatrix:
-        """x [T, D] -> x + routed experts + shared experts (pre-norm inside)."""
+    def Forward(self, x: OaMatrix, rows: Optional[torch.Tensor] = None) -> OaMatrix:
+        """x [T, D] -> x + routed experts + shared experts (pre-norm inside).  `rows` [T] bool: which rows the balancing losses and the load count, where
+        some only fill up a batch (None: all).  Those go through the experts too, but move nothing."""
+        if rows is not None and self.Dispatcher is not None and (self.AuxAlpha > 0 or self.ZBeta > 0 or self.BalanceGamma > 0):
+            raise ValueError("OaMoE: rows that only fill up a batch cannot be told apart in the load over expert-parallel ranks; switch the balancing losses off")
         normed = self.Norm.Forward(x)
         logits = self.Router.Forward(normed)
         sel_bias = self.RoutingBias.Tensor().reshape(-1) if self.BalanceGamma > 0 else None
@@ -148,14 +151,17 @@ class OaMoE(OaModule):
         if self.SparseExecution and (not tn.is_cuda or tn.dtype == torch.bfloat16):
             out = _routed_experts(normed, logits, self.GateUpW.Data, self.GateUpB.Data if self.GateUpB else None, self.DownW.Data,
                                   self.DownB.Data if self.DownB else None, self.ExpertsPerToken, sel_bias, x, self)
+            if rows is not None and self.Dispatcher is None:
+                probs, idx, w, _ = self._last
+                self._last = (probs, idx, w, (torch.zeros_like(probs).scatter_(1, idx.long(), 1.0) * rows[:, None]).sum(0))
         else:
-            out = F.Add(x, self._dense_oracle(normed, logits, sel_bias))
+            out = F.Add(x, self._dense_oracle(normed, logits, sel_bias, rows))
         for se in self.SharedExperts:
             out = se.Forward(normed, residual=out)
-        self.LastAuxLoss = self._aux_loss(logits)
+        self.LastAuxLoss = self._aux_loss(logits, rows)
         return out
 
-    def _dense_oracle(self, normed: OaMatrix, logits: OaMatrix, sel_bias) -> OaMatrix:
+    def _dense_oracle(self, normed: OaMatrix, logits: OaMatrix, sel_bias, rows: Optional[torch.Tensor] = None) -> OaMatrix:
         """Independent dense reference: every expert on every token, gated by the masked renormalised probabilities."""
         E, Kk = self.NumExperts, self.ExpertsPerToken
         probs = F.Softmax(logits)
@@ -163,7 +169,8 @@ class OaMoE(OaModule):
         mask = F.TopKMask(sel, Kk)
         gate_un = F.Mul(probs, mask)
         gate = F.Div(gate_un, F.Reshape(F.Sum(gate_un, 1), [normed.Size(0), 1]))
-        self._last = (probs.Tensor().float(), None, None, mask.Tensor().float().sum(0))
+        took = mask.Tensor().float()
+        self._last = (probs.Tensor().float(), None, None, (took if rows is None else took * rows[:, None]).sum(0))
         acc = None
         for e in range(E):
             # slices of leaves: gradients flow back through explicit Slice nodes
@@ -176,35 +183,41 @@ class OaMoE(OaModule):
             acc = y if acc is None else F.Add(acc, y)
         return acc
 
-    def _aux_loss(self, logits: OaMatrix) -> OaMatrix:
-        """alpha * (E/K) * sum_e f_e * P_e (+ beta * mean(LSE^2)); f = dispatch fraction (constant), P = mean probability."""
+    def _aux_loss(self, logits: OaMatrix, rows: Optional[torch.Tensor] = None) -> OaMatrix:
+        """alpha * (E/K) * sum_e f_e * P_e (+ beta * mean(LSE^2)); f = dispatch fraction (constant), P = mean probability, over `rows` where given."""
         if self.AuxAlpha <= 0.0 and self.ZBeta <= 0.0 or self._last is None:
             return OaMatrix(torch.zeros(1, dtype=torch.float32, device=logits.Tensor().device))
         probs, idx, w, counts = self._last
         T, E = probs.shape
+        if rows is not None:
+            rows = rows[:, None].float()
+            T = rows.sum().clamp(min=1.0)
         Kk = self.ExpertsPerToken
         fe = counts.float() / T
         coef = self.AuxAlpha * E / Kk
-        pe = K.col_sum(probs).float() / T
+        pe = K.col_sum(probs if rows is None else probs * rows).float() / T
         val = (fe * pe).sum().reshape(1) * coef
         tl = logits.Tensor()
         zb = self.ZBeta
         lse = None
         if zb > 0.0:
             lse = torch.logsumexp(tl.float(), -1)
-            val = val + zb * (lse * lse).mean().reshape(1)
+            val = val + zb * ((lse * lse).mean() if rows is None else (lse * lse * rows[:, 0]).sum() / T).reshape(1)
         out = OaMatrix(val)
 
         def back(g):
             gs = g.reshape(1).float()
             if idx is not None:
                 zeros = torch.zeros_like(w)
-                dl = M.router_bwd(probs, idx, w, zeros, fe * gs, coef / T, torch.float32)
+                dl = M.router_bwd(probs, idx, w, zeros, fe * gs, coef / T, torch.float32) if rows is None else \
+                    M.router_bwd(probs, idx, w, zeros, fe * gs / T, coef, torch.float32)
             else:
-                dp = (fe * gs * coef / T).reshape(1, E).expand(T, E)
+                dp = (fe * gs * coef / T).reshape(1, E).expand(probs.shape)
                 dl = probs * (dp - (dp * probs).sum(-1, keepdim=True))
             if zb > 0.0:
                 dl = dl + (2.0 * zb / T) * gs * lse[:, None] * probs
+            if rows is not None:
+                dl = dl * rows
             return (dl.to(tl.dtype),)
 
         return AG.attach("MoeAuxLoss", out, [logits], back)

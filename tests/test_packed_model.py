@@ -211,3 +211,93 @@ def test_gradient_of_rotary_axes_over_the_first_columns(device, dtype):
     got = x.GradTensor()
     assert got.shape == (6, 200) and bool((got[:, 128:] == 0).all())
     assert torch.equal(got[:, :128], packed.rotary(w, pos, (0,) * 32, 2, 64, 10000.0, backward=True))
+
+
+def _aux(model):
+    loss = None
+    for b in model.Blocks:
+        if b.Moe is not None:
+            loss = b.Moe.AuxLoss() if loss is None else F.Add(loss, b.Moe.AuxLoss())
+    return loss
+
+
+def _step(model, ids, starts, targets, weight, tokens):
+    """(log-probabilities and entropy, balancing loss, gradients, shares of the experts) of the first `tokens` rows' batch."""
+    seqs = F.PackedSequences(OaMatrix(starts), tokens)
+
+    def build():
+        out = model.TokenLogProbs(OaMatrix(ids[:tokens].clone()), OaMatrix(targets[:tokens].clone()), seqs)
+        loss, aux = _weighted(out, weight[:, :tokens].contiguous()), _aux(model)
+        return (out, aux), loss if aux is None else F.Add(loss, aux)
+
+    (out, aux), grads = _run(model, build)
+    return out.Tensor().clone(), None if aux is None else aux.Tensor().clone(), grads, [b.Moe.LastLoadFraction() for b in model.Blocks if b.Moe is not None]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("experts", [0, 4])
+def test_rows_of_no_sequence_take_no_part(device, experts):
+    """fp32: whatever tokens stand behind the last sequence, and whether any do, the real rows' results, the gradients, the experts' shares and their balancing losses are
+    those of the sequences.  Sums may be added up in another order: the bounds of test_packed_is_one_sequence_at_a_time."""
+    model = _model(True, device, **({"NumExperts": experts, "TopK": 2, "ExpertFf": 48, "AuxAlpha": 0.3} if experts else {}))
+    for b in model.Blocks:
+        if b.Moe is not None:
+            b.Moe.SetZLossBeta(0.2)
+    ids, starts, targets, weight = _batch(104, device, pad=90)
+    n = sum(LENGTHS)
+    want, want_aux, want_grads, want_shares = _step(model, ids, starts, targets, weight, n)
+    for fill in (0, 1, 103):
+        ids[n:] = fill
+        got, aux, grads, shares = _step(model, ids, starts, targets, weight, n + 90)
+        assert float((got[:, :n] - want).abs().max()) <= 2 ** -12 * float(want.abs().max())
+        assert len(grads) == len(want_grads) and all(float((a - b).abs().max()) <= 2 ** -11 * float(b.abs().max()) for a, b in zip(grads, want_grads))
+        assert shares == want_shares
+        if experts:
+            assert abs(float(aux) - float(want_aux)) <= 2 ** -12 * float(want_aux)
+
+
+@pytest.mark.gpu
+def test_rows_of_no_sequence_take_no_part_bf16():
+    """Same number of rows, other tokens behind the last sequence: a row's products do not depend on other rows, so the sequences' results are the same bits, and
+    the experts' shares the same counts."""
+    model = _model(True, "cuda", d=128, dtype=torch.bfloat16, NumExperts=8, TopK=2, ExpertFf=64, AuxAlpha=0.3)
+    ids, starts, targets, weight = _batch(104, "cuda", pad=90)
+    n = sum(LENGTHS)
+    want = None
+    for fill in (0, 1, 103):
+        ids[n:] = fill
+        got, aux, _, shares = _step(model, ids, starts, targets, weight, n + 90)
+        want = want or (got, aux, shares)
+        assert torch.equal(got[:, :n], want[0][:, :n]) and shares == want[2]
+        # 8 products of shares and mean probabilities, which are sums of 238 and 90 zeros
+        assert abs(float(aux) - float(want[1])) <= 2.0 ** -16 * float(want[1])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_step_moves_what_has_a_gradient(device):
+    model = _model(True, device)
+    ids, starts, targets, weight = _batch(104, device)
+    params = model.AllParameterPtrs()
+    opt = OaAdamW(params, 1e-3)
+    opt.ZeroGrad()
+    _, _, grads, _ = _step(model, ids, starts, targets, weight, ids.numel())
+    before = [p.Data.Tensor().clone() for p in params]
+    opt.Step()
+    assert len(grads) == len(params)
+    for p, a, g in zip(params, before, grads):
+        assert bool(g.abs().max() > 0) and bool((p.Data.Tensor() != a)[g.abs() > 1e-3 * g.abs().max()].all())
+
+
+def test_load_over_ranks_is_refused():
+    """Where the load is counted over expert-parallel ranks, rows of no sequence cannot be left out of what is balanced by it."""
+    model = _model(True, "cpu", NumExperts=4, TopK=2, ExpertFf=48, AuxAlpha=0.3)
+    ids, starts, _, _ = _batch(104, "cpu")
+    model.Blocks[0].Moe.Dispatcher = object()
+    with pytest.raises(ValueError, match="over expert-parallel ranks"):
+        model.ForwardPacked(OaMatrix(ids), F.PackedSequences(OaMatrix(starts), ids.numel()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_of_sequences(device):
+    seqs = F.PackedSequences(OaMatrix(torch.tensor([2, 5, 5, 9], dtype=torch.int32, device=device)), 12)
+    assert seqs.Rows().tolist() == [2 <= i < 9 for i in range(12)]

@@ -1382,7 +1382,8 @@ extern "C" int oa_gemm_bf16_batched(const void* A, const void* B, void* out, int
                                     long long sb_batch, long long sc_batch, long long sr_batch, long long saux_batch,
                                     long long sbias_batch, int* status, void* stream) {
   if (M <= 0 || N <= 0 || K <= 0 || batch <= 0) return OA_ERR_ARG;
-  if ((N & 7) || (K & 7) || (a_mn && (M & 7))) return OA_ERR_ALIGN;
+  // a row of an operand whose rows run along K is whole 16 bytes; where both lie the other way (a weight's gradient, K rows of tokens) any K will do
+  if ((N & 7) || ((K & 7) && !(a_mn && b_mn)) || (a_mn && (M & 7))) return OA_ERR_ALIGN;
   if ((ldc & (out_f32 ? 3 : 7)) || (residual && (ldr & 7)) || ((aux_out || aux_in) && (ldaux & 7))) return OA_ERR_ALIGN;
   if (batch > 1 && ((sc_batch & 7) || (sr_batch & 7) || (saux_batch & 7) || (sbias_batch & 7))) return OA_ERR_ALIGN;
   // A handful of rows against a large weight: the kernel that streams the weight (gemm_skinny.cu).  It adds the products up in another

@@ -99,8 +99,8 @@ class OaGptModel(OaModule):
         return self.Head.Forward(self.Hidden(ids))
 
     def HiddenPacked(self, ids: OaMatrix, sequences: F.OaPackedSequences) -> OaMatrix:
-        """ids [tokens] of sequences of different lengths, one behind the other (`F.PackedSequences`); in bf16 training a multiple of 8 rows, those behind the last
-        sequence belonging to none (any token of the vocabulary, no target)."""
+        """ids [tokens] of sequences of different lengths, one behind the other (`F.PackedSequences`), any number of rows.  Rows behind the last sequence belong to
+        none: any token of the vocabulary, no target."""
         if ids.NumElements() != sequences.Tokens():
             raise ValueError(f"{ids.NumElements()} tokens, but the sequences are of {sequences.Tokens()} rows")
         x = F.Embedding(self.Embed.Weight.Data, ids)

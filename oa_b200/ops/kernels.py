@@ -253,7 +253,7 @@ def gemm(a: torch.Tensor, b: torch.Tensor, *, a_mn: bool = False, b_mn: bool = F
                     V.OA_VALIDATE(t.stride(0) * t.element_size() % 16 == 0, V.OaValidationSeverity.Error, "Kernel",
                                   "%s: row pitch %d bytes is not a multiple of 16", nm, t.stride(0) * t.element_size())
             V.ValidateTensor("gemm.bias", bias, dtype=torch.bfloat16, cuda=True)
-            V.OA_VALIDATE(Nn % 8 == 0 and K % 8 == 0, V.OaValidationSeverity.Error, "Kernel", "gemm: N=%d and K=%d must be multiples of 8", Nn, K)
+            V.OA_VALIDATE(Nn % 8 == 0 and (K % 8 == 0 or (a_mn and b_mn)), V.OaValidationSeverity.Error, "Kernel", "gemm: N=%d and K=%d must be multiples of 8", Nn, K)
             if force_bn == 0 and (M < 128 or Nn < 128):
                 V.OaValidation.Report(V.OaValidationSeverity.Info, "Kernel", "gemm M=%d N=%d K=%d: tile larger than the problem", M, Nn, K)
         resting = getattr(_weights_at_rest, "storages", ())

@@ -301,3 +301,21 @@ def test_load_over_ranks_is_refused():
 def test_rows_of_sequences(device):
     seqs = F.PackedSequences(OaMatrix(torch.tensor([2, 5, 5, 9], dtype=torch.int32, device=device)), 12)
     assert seqs.Rows().tolist() == [2 <= i < 9 for i in range(12)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,experts", [(64, 0), (128, 0), (64, 8)])
+def test_bf16_training_on_any_number_of_rows(hd, experts):
+    """238 rows as they come and with two or ten of no sequence behind them: the same products and zeros, so that gradients differ by the order of sums in 32 bits, then a
+    rounding to bf16 on either side."""
+    model = _model(True, "cuda", heads=2, d=2 * hd, dtype=torch.bfloat16, **({"NumExperts": experts, "TopK": 2, "ExpertFf": 64} if experts else {}))
+    ids, starts, targets, weight = _batch(104, "cuda", pad=10)
+    n = sum(LENGTHS)
+    assert n % 8
+    want = None
+    for tokens in (n + 2, n, n + 10, n + 1):
+        out, _, grads, _ = _step(model, ids, starts, targets, weight, tokens)
+        want = want or (out, grads)
+        assert torch.equal(out[:, :n], want[0][:, :n]) and len(grads) == len(want[1])
+        for a, b in zip(grads, want[1]):
+            assert float((a - b).abs().max()) <= 2.0 ** -7 * float(b.abs().max())

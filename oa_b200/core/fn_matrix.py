@@ -1049,7 +1049,7 @@ def PackedAttention(qkv: OaMatrix, sequences: OaPackedSequences, heads: int, kv_
     t = qkv.Tensor()
     turned, axes = heads + kv_heads, sequences.Axes(head_dim)
     if rope_theta > 0:
-        if (AG.IsEnabled() and qkv.RequiresGrad() and not consume_input) or not t.is_contiguous():
+        if (AG.IsEnabled() and not consume_input) or not t.is_contiguous():
             t = K.unary("copy", _c(t))
         PK.rotary(t, sequences.Positions, axes, turned, head_dim, rope_theta, out=t)
     q, k, v = torch.split(t, [heads * head_dim, kv_heads * head_dim, kv_heads * head_dim], 1)

@@ -319,3 +319,19 @@ def test_bf16_training_on_any_number_of_rows(hd, experts):
         assert torch.equal(out[:, :n], want[0][:, :n]) and len(grads) == len(want[1])
         for a, b in zip(grads, want[1]):
             assert float((a - b).abs().max()) <= 2.0 ** -7 * float(b.abs().max())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_attention_leaves_its_input_alone_while_autograd_records(device):
+    """Whether or not the projection asks for a gradient; given to be consumed, or without recording, it is turned in place."""
+    qkv = torch.randn(12, 3 * 64, generator=torch.Generator().manual_seed(3)).to(device)
+    seqs = F.PackedSequences(OaMatrix(torch.tensor([0, 5, 12], dtype=torch.int32, device=device)), 12)
+    for wants in (False, True):
+        x = OaMatrix(qkv.clone()).SetRequiresGrad(wants)
+        with AG.OaGradientTape():
+            first = F.PackedAttention(x, seqs, 1, 1, 64, rope_theta=100.0).Tensor()
+            assert torch.equal(x.Tensor(), qkv)
+            assert torch.equal(F.PackedAttention(x, seqs, 1, 1, 64, rope_theta=100.0).Tensor(), first)
+            given = OaMatrix(qkv.clone()).SetRequiresGrad(wants)
+            assert torch.equal(F.PackedAttention(given, seqs, 1, 1, 64, rope_theta=100.0, consume_input=True).Tensor(), first)
+            assert not torch.equal(given.Tensor(), qkv)

@@ -76,6 +76,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0, sc
     return TokenLogProbs(logprobs, entropy, stats.view(rows, 2), top_logprobs, top_ids)
 
 
+@torch.no_grad()
 def _cpu(logits, targets, top, scale, ignore_index):
     rows, vocab = logits.shape
     logits = logits.contiguous()
@@ -129,6 +130,7 @@ def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, result:
     return out
 
 
+@torch.no_grad()
 def _backward_cpu(logits, targets, result, dlogprobs, dentropy, scale, ignore_index, out):
     rows, vocab = logits.shape
     m, log_l = result.stats[:, :1], result.stats[:, 1:]

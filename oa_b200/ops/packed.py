@@ -147,13 +147,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, pair_axes: Sequence[int], h
         if x.data_ptr() != out.data_ptr() or (tokens > 1 and x.stride() != out.stride()):
             _apart("rotary", out, x[:, :cols])
     if device < 0:
-        half = len(pair_axes)
-        a = positions.double()[list(pair_axes)].t() * torch.tensor(list(turns), dtype=torch.float64) * (2 * math.pi)
-        cos, sin = a.cos().float()[:, None], a.sin().float()[:, None]
-        sin = -sin if backward else sin
-        v = x[:, :cols].float().reshape(tokens, heads, head_dim)
-        lo, hi = v[..., :half], v[..., half:2 * half]
-        out.copy_(torch.cat([lo * cos - hi * sin, hi * cos + lo * sin, v[..., 2 * half:]], -1).reshape(tokens, cols))
+        _rotary_cpu(x[:, :cols].reshape(tokens, heads, head_dim), positions, pair_axes, turns, backward, out)
         return out
     if step is None:
         x = _copied(x[:, :cols])
@@ -161,6 +155,17 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, pair_axes: Sequence[int], h
     K._launch(N.require().oa_rotary_axes(K.dt(x), x.data_ptr(), step, out.data_ptr(), to, positions.data_ptr(), ctypes.addressof(axes), ctypes.addressof(turns),
                                          len(pair_axes), tokens, heads, head_dim, int(backward), _stream(device)), "oa_rotary_axes", outputs=(out,))
     return out
+
+
+@torch.no_grad()
+def _rotary_cpu(x, positions, pair_axes, turns, backward, out):
+    half = len(pair_axes)
+    a = positions.double()[list(pair_axes)].t() * torch.tensor(list(turns), dtype=torch.float64) * (2 * math.pi)
+    cos, sin = a.cos().float()[:, None], a.sin().float()[:, None]
+    sin = -sin if backward else sin
+    v = x.float()
+    lo, hi = v[..., :half], v[..., half:2 * half]
+    out.copy_(torch.cat([lo * cos - hi * sin, hi * cos + lo * sin, v[..., 2 * half:]], -1).reshape(out.shape))
 
 
 # What follows from shapes, strides and types alone is worked out once for each of them: the checks took longer than a small launch.
@@ -248,7 +253,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPla
     hq, hk, scale, *steps = _layout("attention", q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, plan.tokens, head_dim,
                                     scale, device >= 0)
     if device < 0:
-        o, lse = _attention_cpu(q, k, v, plan, head_dim, scale)
+        with torch.no_grad():
+            o, lse = _attention_cpu(q, k, v, plan, head_dim, scale)
         return (o.to(q.dtype), lse) if return_lse else o.to(q.dtype)
     half = q.dtype is torch.bfloat16
     (q, qs), (k, ks), (v, vs) = _operands(half, (q, steps[0]), (k, steps[1]), (v, steps[2]))

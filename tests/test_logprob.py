@@ -359,3 +359,14 @@ def test_a_scale_given_as_a_tensor(device):
             L.token_logprobs(x, t, 2, scale)
         with pytest.raises(ValueError, match="scale must be positive"):
             L.token_logprobs_backward(x, t, want, g, h, scale)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_results_carry_no_graph(device):
+    x, t, g, h = (v.to(device) for v in _logits(3, 50, torch.float32))
+    for v in (x, g, h):
+        v.requires_grad_(True)
+    r = L.token_logprobs(x, t, 2)
+    d = L.token_logprobs_backward(x, t, r, g, h)
+    for v in (*r, d):
+        assert not v.requires_grad and v.grad_fn is None

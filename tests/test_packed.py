@@ -614,3 +614,17 @@ def test_numbers_given_as_tensors(device):
     assert torch.equal(P.rotary(q, pos, torch.zeros(32, dtype=torch.int64), 2, 64, 500.0), P.rotary(q, pos, (0,) * 32, 2, 64, 500.0))
     with pytest.raises(ValueError, match="whole numbers"):
         P.rotary(q, pos, tuple(torch.zeros(32, dtype=torch.int64)), 2, 64, 500.0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_results_carry_no_graph(device):
+    """Gradients are calls of their own: what the operators give back of tensors that ask for one has no history, on either path, and can be written in place."""
+    q, k, v, dout = (t.detach().clone().requires_grad_(True) for t in _inputs([9, 3], 2, 1, 64, torch.float32, device))
+    plan, pos = P.plan(_starts([9, 3], device), 12), torch.arange(12, dtype=torch.int32, device=device)[None]
+    o, lse = P.attention(q, k, v, plan, 64, return_lse=True)
+    turned = P.rotary(q, pos, (0,) * 32, 2, 64, THETA)
+    grads = P.attention_backward(q, k, v, o, dout, lse, plan, 64)
+    into = P.rotary(q, pos, (0,) * 32, 2, 64, THETA, out=torch.empty(12, 128, device=device))
+    for t in (o, lse, turned, into, *grads):
+        assert not t.requires_grad and t.grad_fn is None
+    assert torch.equal(into, turned)

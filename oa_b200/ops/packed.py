@@ -311,8 +311,8 @@ def attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: tor
             raise ValueError("attention_backward: dqkv must begin on 16 bytes")
     grads = torch.unsafe_split_with_sizes(dqkv, cols, 1)
     if device < 0:
-        with torch.enable_grad():
-            leaves = [t.detach().float().requires_grad_(True) for t in (q, k, v)]
+        with torch.inference_mode(False), torch.enable_grad():        # inference mode records nothing, and its tensors cannot be recorded: copies
+            leaves = [t.detach().to(torch.float32, copy=True).requires_grad_(True) for t in (q, k, v)]
             y, _ = _attention_cpu(*leaves, plan, head_dim, scale)
             got = torch.autograd.grad(y, leaves, dout.float(), allow_unused=True) if y.requires_grad else (None,) * 3
         for to, g in zip(grads, got):

@@ -370,3 +370,20 @@ def test_results_carry_no_graph(device):
     d = L.token_logprobs_backward(x, t, r, g, h)
     for v in (*r, d):
         assert not v.requires_grad and v.grad_fn is None
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("top", [0, 2])
+def test_inference_mode(device, top):
+    """Calls within inference mode give what they give elsewhere, and leave nothing of it to calls outside; what one call gives back is that call's alone."""
+    x, t, g, h = (v.to(device) for v in _logits(7, 53, torch.float32))
+    with torch.inference_mode():
+        within = L.token_logprobs(x, t, top)
+        grad = L.token_logprobs_backward(x, t, within, g, h)
+    outside, again = L.token_logprobs(x, t, top), L.token_logprobs(x, t, top)
+    assert all(torch.equal(a, b) for a, b in zip(within, outside)) and torch.equal(grad, L.token_logprobs_backward(x, t, outside, g, h))
+    for a, b in zip(outside, again):
+        assert not a.is_inference() and a is not b
+        if a.dtype.is_floating_point:
+            a.requires_grad_(True)
+            assert not b.requires_grad and not L.token_logprobs(x, t, top).top_logprobs.requires_grad

@@ -628,3 +628,19 @@ def test_results_carry_no_graph(device):
     for t in (o, lse, turned, into, *grads):
         assert not t.requires_grad and t.grad_fn is None
     assert torch.equal(into, turned)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("within", [False, True])
+def test_inference_mode(device, within):
+    """Calls within inference mode, on tensors made there or before, give what they give elsewhere."""
+    lengths = [9, 0, 70]
+    q, k, v, dout = _inputs(lengths, 2, 1, 64, torch.float32, device)
+    starts = _starts(lengths, device)
+    want = _both(q, k, v, dout, starts, 64)
+    with torch.inference_mode():
+        args = [t.clone() for t in (q, k, v, dout, starts)] if within else [q, k, v, dout, starts]
+        got = _both(*args, 64)
+        assert all(torch.equal(got[n], want[n]) for n in want)
+    got = _both(*args, 64)                                           # tensors of inference mode outside it
+    assert all(torch.equal(got[n], want[n]) for n in want)

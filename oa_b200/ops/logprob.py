@@ -43,12 +43,6 @@ def _layout(what, shape, stride, dtype, t_shape, t_stride, t_dtype, scale, top, 
     return None if stride[1] != 1 and vocab > 1 else vocab if rows <= 1 else stride[0]
 
 
-@functools.lru_cache(maxsize=64)
-def _no_alternatives(rows, device):
-    """Tensors without elements: making them took a fifth of a small call."""
-    return torch.empty((rows, 0), dtype=torch.float32, device=device), torch.empty((rows, 0), dtype=torch.int32, device=device)
-
-
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0, scale: float = 1.0, ignore_index: int = -100) -> TokenLogProbs:
     """Of every row of scale * logits [rows, vocab] (row stride allowed; scale is 1 / temperature): the log-probability of its target, the entropy, and
     the `top` likeliest tokens (at most 32) with theirs; equal logits rank by index.  A target of ignore_index has log-probability 0, any other that is
@@ -68,7 +62,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0, sc
         top_logprobs, top_ids = top_logprobs.view(rows, top), top_ids.view(torch.int32).view(rows, top)
     else:
         logprobs, entropy, stats = torch.unsafe_split_with_sizes(f32, (rows, rows, 2 * rows))
-        top_logprobs, top_ids = _no_alternatives(rows, logits.device)
+        top_logprobs = f32.as_strided((rows, 0), (1, 1))         # without elements: not worth two allocations
+        top_ids = top_logprobs.view(torch.int32)
     at = f32.data_ptr()
     K._launch(N.require().oa_token_logprobs(K.dt(logits), logits.data_ptr(), step, targets.data_ptr(), at, at + 4 * rows, at + 8 * rows, at + 16 * rows,
                                             at + 4 * (4 + top) * rows, top, rows, vocab, scale, ignore_index, _stream(device)),

@@ -246,8 +246,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPla
     multiple of kv_heads.  Returns [tokens, q_heads * head_dim] and, with return_lse, also the natural log-sum-exp [q_heads, tokens] fp32, which the
     gradients need.  `scale` defaults to head_dim^-1/2.  Rows of no sequence are 0 (-inf).
 
-    bf16 (heads of 64 or 128) runs on the tensor cores: weights are rounded to bf16 before they meet the values, sums are fp32.  A value that is not finite
-    may reach earlier tokens of its own sequence, as its weight there is 0 times it."""
+    bf16 (heads of 64 or 128) runs on the tensor cores: weights are rounded to bf16 before they meet the values, sums are fp32.  A query or key that is not finite
+    reaches no earlier token.  A value (a row of v) that is not finite may reach earlier tokens of its own sequence, in every type and on the CPU: its weight
+    there is 0, and 0 times it is NaN."""
     device = _together("attention", q, k, v, plan.starts)
     head_dim, scale = _whole(head_dim), None if scale is None else float(scale)
     hq, hk, scale, *steps = _layout("attention", q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, plan.tokens, head_dim,
@@ -294,7 +295,11 @@ def attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: tor
                        head_dim: int, scale: Optional[float] = None, dqkv: Optional[torch.Tensor] = None):
     """The gradients (dq, dk, dv) of `attention` from its inputs, its output and log-sum-exp, and dout [tokens, q_heads * head_dim] (row stride
     allowed).  They are slices of `dqkv` [tokens, (q_heads + 2 kv_heads) * head_dim], a packed projection's gradient.  Those of a key-value head are the
-    sums over the query heads that share it, added up in one order: the same inputs give the same bits.  Rows of no sequence are 0."""
+    sums over the query heads that share it, added up in one order: the same inputs give the same bits.  Rows of no sequence are 0.
+
+    bf16: dv takes the weights rounded to bf16.  The score gradients dS go to dq's product as two bf16 numbers and to dk's rounded to one; in sequences of up to 32
+    rows to both as two, of 33 to 64 to both as one.  Delta, the row's sum of weights times dP that is taken off in dS, is summed in 32 bits, but for dq of a sequence's
+    129th row and on, where it comes from o and dout as they are.  What is not finite may reach the gradients of every token of its sequence."""
     device = _together("attention_backward", q, k, v, o, dout, lse, plan.starts)
     head_dim, scale = _whole(head_dim), None if scale is None else float(scale)
     hq, hk, scale, steps, cols, width, need = _backward_layout(

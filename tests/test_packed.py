@@ -644,3 +644,27 @@ def test_inference_mode(device, within):
         assert all(torch.equal(got[n], want[n]) for n in want)
     got = _both(*args, 64)                                           # tensors of inference mode outside it
     assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,at", [(8, 5), (60, 33), (200, 70), (300, 299)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_not_finite_within_a_sequence(device, dtype, n, at, bad):
+    """A query or a key that is not finite leaves the results of earlier tokens as they are; a value may reach any token of its sequence and always reaches its own, but
+    none of another sequence."""
+    q, k, v, _ = _inputs([4, n, 7], 2, 1, 64, dtype, device)
+    plan = P.plan(_starts([4, n, 7], device), n + 11)
+    want, want_lse = P.attention(q, k, v, plan, 64, return_lse=True)
+    assert bool(want.isfinite().all())
+    row = 4 + at
+    for which in range(3):
+        args = [t.clone() for t in (q, k, v)]
+        args[which][row] = bad
+        got, lse = P.attention(*args, plan, 64, return_lse=True)
+        assert not bool(got[row].isfinite().any()) if which == 2 else not bool(got[row].isfinite().all())
+        same = [slice(0, 4), slice(4 + n, None)] + ([slice(4, row)] if which < 2 else [])
+        assert all(torch.equal(got[s], want[s]) for s in same)
+        assert torch.equal(lse if which == 2 else lse[:, :row], want_lse if which == 2 else want_lse[:, :row])
+        if which == 0:
+            assert torch.equal(got[row + 1:], want[row + 1:])

@@ -387,3 +387,65 @@ def test_inference_mode(device, top):
         if a.dtype.is_floating_point:
             a.requires_grad_(True)
             assert not b.requires_grad and not L.token_logprobs(x, t, top).top_logprobs.requires_grad
+
+
+def _many():
+    """Rows enough for blocks of 128 threads where the vocabulary allows, not a multiple of anything."""
+    return 4 * torch.cuda.get_device_properties(0).multi_processor_count + 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,vocab", [(torch.bfloat16, 2049), (torch.bfloat16, 8191), (torch.bfloat16, 32000), (torch.bfloat16, 33600), (torch.bfloat16, 33607),
+                                         (torch.float32, 2049), (torch.float32, 8191), (torch.float32, 16800), (torch.float32, 16803)])
+@pytest.mark.parametrize("top", [0, 1, 5, 32])
+def test_many_long_rows(dtype, vocab, top):
+    _check(*_logits(_many(), vocab, dtype), "cuda", top=top)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [2500, 8192, 16001])
+@pytest.mark.parametrize("top", [1, 20, 32])
+def test_orders_and_ties_of_many_rows(dtype, vocab, top):
+    x = torch.stack(list(_order_cases(vocab).values())).to(dtype)
+    order = torch.sort(x.float(), dim=1, descending=True, stable=True).indices[:, :top]
+    logp = (x.double() - torch.logsumexp(x.double(), 1, keepdim=True)).gather(1, order)
+    n, many = x.shape[0], _many()
+    at = torch.arange(many) % n
+    r = L.token_logprobs(x.cuda()[at.cuda()], torch.zeros(many, dtype=torch.int32, device="cuda"), top)
+    assert torch.equal(r.top_ids.cpu().long(), order[at])
+    _near("top", r.top_logprobs, logp[at], 2.0 ** -17 + 2.0 ** -22 * logp[at].abs().nan_to_num(posinf=0.0))      # as in test_orders_and_ties
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [2050, 9001])
+@pytest.mark.parametrize("top", [0, 5])
+def test_masked_and_broken_rows_among_many(dtype, vocab, top):
+    """Few such rows and many: the same where they are 0, infinite or NaN, the same alternatives, and values as near as either is to the definition."""
+    x, t, g, h = _logits(8, vocab, dtype)
+    t[:] = torch.tensor([vocab - 1, 0, 3, 3, 3, -100, vocab, -1])
+    x[0, :vocab - 1] = -INF
+    x[1, 1:] = torch.finfo(dtype).min
+    x[2] = -INF
+    x[3, vocab // 2] = math.nan
+    x[4, vocab // 3] = INF
+    x[5, ::2] = -INF
+    few = [v.cuda() for v in (x, t, g, h)]
+    at = torch.arange(_many(), device="cuda") % 8
+    many = [v[at] for v in few]
+    got = []
+    for a in (few, many):
+        r = L.token_logprobs(a[0], a[1], top)
+        got.append([*r, L.token_logprobs_backward(a[0], a[1], r, a[2], a[3])])
+    # |y| to 15: (30 + 30) 2^-23 and the sums, either way; a gradient up to 6 such errors with g, h and log p to 16, then rounded
+    e = 2 * 2.0 ** -16
+    for name, a, b in zip(("logprobs", "entropy", "stats", "top_logprobs", "top_ids", "dlogits"), *got):
+        a = a[at]
+        same = (a == b) | (a.isnan() & b.isnan()) if a.is_floating_point() else a == b
+        if name == "top_ids":
+            assert bool(same.all())
+        else:
+            d = (a.double() - b.double()).abs().masked_fill(same, 0)
+            bound = e + 2.0 ** -22 * a.double().abs() if name != "dlogits" else 16 * 6 * e * a.double().abs() + 2 * U[dtype] * a.double().abs() + 2.0 ** -100
+            assert bool((same | (d <= bound)).all()), name             # the bound of a NaN is NaN: those are the same, or differ by NaN

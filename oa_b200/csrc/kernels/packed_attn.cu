@@ -1399,12 +1399,16 @@ static int packed_ctas(long long items) {
 }
 
 // Over how many CTAs the query heads of a key-value head go.  A tile of keys is as long as all the queries behind it times the group, and with few tiles the first
-// ones are most of the kernel: as many as bring the longest item down to an SM's share, were the sequences equally long.  With it / without: one sequence of 1000
-// rows of 64 heads over 8 of 64 69 / 112 us, of 2000 188 / 253, of 2048 of 32 over 8 of 128 146 / 180, 100 + 1700 + 300 + 900 of 64 over 8 238 / 254; 4 of 500 97 / 92.
-static int packed_parts(int tokens, int batch, int kv_heads, int group) {
+// ones are most of the kernel: more as long as the longest item, were the sequences equally long, is more than 5/4 of an SM's share, at head dim 128, where
+// partial sums are twice as many, 8/5.  Gradients of 64 heads over 8 of 64 with 1 / 2 / 4 CTAs: one sequence of 1000 rows 111 / 81 / 68 us, of 2000 251 / 187 / 196, of 3000 417 / 378;
+// 4 of 375 (2.3 shares) 72 / 66 / 73, of 500 (1.9) 95 / 96, of 750 (1.3) 147 / 155, of rising lengths up to 1200 197 / 192, 1800 beside 3 of 400 262 / 239.  Of 32 over 8 of 128: one of 1500 131 /
+// 109 / 115, of 3000 (1.5) 295 / 287; 2 of 750 97 / 80 / 90; 8 of 250 (1.5) 52 / 69, of rising lengths up to 444 115 / 136, 1200 beside 7 of 114 116 / 107.
+// The host knows the number of sequences, not their lengths: where one is much longer than the others, or many are empty, more would be better than it takes.
+static int packed_parts(int tokens, int batch, int kv_heads, int group, int head_dim) {
   const long long seqs = batch > 0 ? batch : 1, n = tokens / (FA_BM * seqs) + 1;
+  const long long share = head_dim == 64 ? 32 : 25;                  // 2 / (5/4), 2 / (8/5), in twentieths
   int parts = 1;
-  for (int d = 2; tokens > PACKED_SHORT && d <= group && d <= 64 && 5 * parts * kv_heads * seqs * (n + 1) < 8 * sm_count(); ++d)
+  for (int d = 2; tokens > PACKED_SHORT && d <= group && d <= 64 && 20 * parts * kv_heads * seqs * (n + 1) < share * sm_count(); ++d)
     if (group % d == 0) parts = d;
   return parts;
 }
@@ -1474,7 +1478,7 @@ extern "C" int oa_packed_attn(const void* q, const void* k, const void* v, const
 // scratch: float[2][q_heads, tokens], delta from the output and from the rows' sums; then what CTAs that share a group's heads add up to
 extern "C" size_t oa_packed_attn_bwd_scratch_bytes(int tokens, int batch, int q_heads, int kv_heads, int head_dim) {
   if (packed_check(tokens, batch, q_heads, kv_heads, head_dim)) return 0;
-  const int parts = packed_parts(tokens, batch, kv_heads, q_heads / kv_heads);
+  const int parts = packed_parts(tokens, batch, kv_heads, q_heads / kv_heads, head_dim);
   const size_t sums = parts > 1 ? (size_t)parts * packed_max_tiles(tokens, batch) * kv_heads * 2 * FA_BM * head_dim : 0;
   return (packed_delta_floats(tokens, q_heads) + sums) * sizeof(float);
 }
@@ -1502,7 +1506,7 @@ extern "C" int oa_packed_attn_bwd(const void* q, const void* k, const void* v, c
   const int fill = 8 * sm_count();
   launch_pdl(head_dim == 64 ? packed_delta_kernel<64> : packed_delta_kernel<128>, dim3((unsigned)(units < 1 ? 1 : units < fill ? units : fill)), dim3(DELTA_THREADS), 0, st,
              (const __nv_bfloat16*)o, (const __nv_bfloat16*)dout, (float*)scratch, PackedPlan{plan, batch, tokens}, q_heads, o_stride, do_stride);
-  const int parts = packed_parts(tokens, batch, kv_heads, q_heads / kv_heads);
+  const int parts = packed_parts(tokens, batch, kv_heads, q_heads / kv_heads, head_dim);
   const PackedBwdParams p{{plan, batch, tokens}, q_heads, kv_heads, q_heads / kv_heads, scale, lse, (const float*)scratch, (float*)scratch + (size_t)q_heads * tokens, (__nv_bfloat16*)dq,
                           (__nv_bfloat16*)dk, (__nv_bfloat16*)dv, dq_stride, dk_stride, dv_stride, status, parts, q_heads / kv_heads / parts,
                           reinterpret_cast<float4*>((float*)scratch + packed_delta_floats(tokens, q_heads))};

@@ -570,9 +570,10 @@ static int logprob_launch(const LogprobParams& p, int parts, cudaStream_t st) {
 template <typename T>
 static int logprob_run(const LogprobParams& p, cudaStream_t st) {
   // Otherwise a warp to a row of up to 2048 elements; for longer ones as many CTAs to a row as leave no SM without two, each with 2048 elements at least.  Smaller CTAs cover
-  // one another's meetings where there are several waves of them (bf16, five alternatives, threads 128 / 256: 4096 x 32000 66.6 / 74.8 us, 16384 x 8000 98 /
-  // 161), larger ones end sooner where there is one (32 x 201088 12.2 / 11.3, 64 x 50257 9.1 / 8.8) or a thread has many pieces (fp32, twenty alternatives, 4096 x 32000
-  // 143 / 123).
+  // one another's meetings where there are several waves of them, larger ones end sooner where there is one (bf16, five alternatives, threads 128 / 256: 32 x 201088 12.2 / 11.3
+  // us, 64 x 50257 9.1 / 8.8) or a thread has many pieces, which its second look pays for by the alternatives.  4096 rows of 4000 pieces, bf16 x 32000 and fp32 x 16000, with
+  // five 65 / 73 and 58 / 63, with twenty 80 / 83 and 68 / 70; of 5000 and 6000, bf16 x 40000 and fp32 x 24001, five 78 / 84 and 79 / 84, twenty 98 / 94 and 100 / 93; of 8100, five
+  // 118 / 118 and 101 / 100, none 99 / 102 and 84 / 81.  Two waves, bf16 1800 x 40000, five 40 / 43; one, 600 rows of 4000 and 5000, 18.5 / 18.1 and 22 / 20.
   // Eight lanes to a row where there are rows enough for every SM's warps, or a row is one 16-byte piece or two to a lane (bf16, eight lanes / a warp to
   // a row: 200000 x 256 30 / 86 us, 60000 x 1000 28 / 36, 20000 x 2000 20 / 19, 2000 x 128 2.2 / 2.7, 2000 x 500 4.6 / 3.9; fp32, 20000 x 2000 41 / 33).
   const long long bytes = (long long)p.vocab * sizeof(T);
@@ -583,7 +584,7 @@ static int logprob_run(const LogprobParams& p, cudaStream_t st) {
   if (p.vocab <= 2048) return logprob_launch<T, 32>(p, 1, st);
   int parts = 1;
   while (parts < 8 && (long long)p.rows * parts <= 2 * sm_count() && p.vocab / (2 * parts) >= 2048) parts *= 2;
-  if (p.rows >= 4 * sm_count() && p.vocab / LpPiece<T>::N <= 4200) return logprob_launch<T, 128>(p, parts, st);
+  if (p.rows >= 4 * sm_count() && p.vocab / LpPiece<T>::N <= (p.top <= 8 && p.rows >= 12 * sm_count() ? 7000 : 4200)) return logprob_launch<T, 128>(p, parts, st);
   return logprob_launch<T, 256>(p, parts, st);
 }
 

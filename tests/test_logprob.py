@@ -449,3 +449,10 @@ def test_masked_and_broken_rows_among_many(dtype, vocab, top):
             d = (a.double() - b.double()).abs().masked_fill(same, 0)
             bound = e + 2.0 ** -22 * a.double().abs() if name != "dlogits" else 16 * 6 * e * a.double().abs() + 2 * U[dtype] * a.double().abs() + 2.0 ** -100
             assert bool((same | (d <= bound)).all()), name             # the bound of a NaN is NaN: those are the same, or differ by NaN
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("top", [5, 9])
+def test_several_waves_of_longer_rows(top):
+    """Twelve rows to an SM and more of over 4200 pieces: blocks of 128 threads up to eight alternatives, of 256 beyond."""
+    _check(*_logits(12 * torch.cuda.get_device_properties(0).multi_processor_count + 3, 17201, torch.float32), "cuda", top=top)

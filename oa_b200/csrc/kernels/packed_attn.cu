@@ -15,7 +15,8 @@
 //
 // Forward is bound by the softmax warps: about 1700 cycles for a tile of 128 x 128, of which the exponentials need 900 (two warps to a scheduler, each a chain of
 // loads from TMEM, maximum, exponentials, stores).  Backward is two kernels, dQ and then dK and dV, which work out scores and dP twice: seven products for
-// five, but sums of one order, no atomics, and nothing in memory between them but a number to a row.  They too are bound by their softmax warps (issue slots 45 to 50 %
+// five, but sums of one order, no atomics, and little in memory between them: two numbers to a row (delta, and delta put right), and where the heads of a group go over
+// several CTAs their fp32 sums of dK and dV.  They too are bound by their softmax warps (issue slots 45 to 50 %
 // busy, tensor pipe 40 % at head dim 64).  Measured: 8 x 2048 rows of 16 heads of 64 109 us (630 TFLOP/s of what the mask leaves) and 353 for the gradients
 // (487); 4096 of 32 of 128 120 (1149) and 457 (751); 8192 of 32 over 8 of 128 415 (1326) and 1653 (831).  Where tiles are few the heads of a group go over several CTAs
 // whose dK and dV are joined by a third kernel.

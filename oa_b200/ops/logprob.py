@@ -47,7 +47,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0, sc
     """Of every row of scale * logits [rows, vocab] (row stride allowed; scale is 1 / temperature): the log-probability of its target, the entropy, and
     the `top` likeliest tokens (at most 32) with theirs; equal logits rank by index.  A target of ignore_index has log-probability 0, any other that is
     no token NaN.  Logits of -inf have probability 0; a row with NaN or +inf is NaN; one without anything above -inf has log-probabilities of
-    -inf and entropy 0."""
+    -inf and entropy 0.  The same call gives the same bits; the last bits of a row depend on the order of its sums, which goes by where it begins (from a
+    multiple of 16 bytes or not), `top` and the number of rows."""
     scale, top, ignore_index = float(scale), _whole(top), _whole(ignore_index)
     step = _layout("token_logprobs", logits.shape, logits.stride(), logits.dtype, targets.shape, targets.stride(), targets.dtype, scale, top, ignore_index)
     device = _together("token_logprobs", logits, targets)

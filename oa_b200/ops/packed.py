@@ -295,7 +295,7 @@ def attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: tor
                        head_dim: int, scale: Optional[float] = None, dqkv: Optional[torch.Tensor] = None):
     """The gradients (dq, dk, dv) of `attention` from its inputs, its output and log-sum-exp, and dout [tokens, q_heads * head_dim] (row stride
     allowed).  They are slices of `dqkv` [tokens, (q_heads + 2 kv_heads) * head_dim], a packed projection's gradient.  Those of a key-value head are the
-    sums over the query heads that share it, added up in one order: the same inputs give the same bits.  Rows of no sequence are 0.
+    sums over the query heads that share it, added up in one order: the same call gives the same bits, while the order goes by the number of rows and of sequences.  Rows of no sequence are 0.
 
     bf16: dv takes the weights rounded to bf16.  The score gradients dS go to dq's product as two bf16 numbers and to dk's rounded to one; in sequences of up to 32
     rows to both as two, of 33 to 64 to both as one.  Delta, the row's sum of weights times dP that is taken off in dS, is summed in 32 bits, but for dq of a sequence's

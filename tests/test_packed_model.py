@@ -335,3 +335,41 @@ def test_attention_leaves_its_input_alone_while_autograd_records(device):
             given = OaMatrix(qkv.clone()).SetRequiresGrad(wants)
             assert torch.equal(F.PackedAttention(given, seqs, 1, 1, 64, rope_theta=100.0, consume_input=True).Tensor(), first)
             assert not torch.equal(given.Tensor(), qkv)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hk,hd", [(4, 4, 64), (8, 2, 64), (8, 2, 128)])
+def test_single_tokens_bf16(hq, hk, hd):
+    """Tokens decoded one by one over pages, turned by `rotary`, appended without a turn, against the whole sequences: each side rounds its weights before they meet the values
+    and its result once, 2^-8 of the magnitudes for either, and sums of at most 200 terms in 32 bits."""
+    lengths = [70, 200]
+    n, ps = sum(lengths), 16
+    g = torch.Generator().manual_seed(6)
+    qkv = torch.randn(n, (hq + 2 * hk) * hd, generator=g).bfloat16().cuda()
+    pos = torch.stack([torch.arange(n), torch.arange(n) // 7]).to(torch.int32).cuda()
+    axes = (0, 1) * (hd // 4)
+    starts = torch.tensor([0, 70, n], dtype=torch.int32, device="cuda")
+    turned = packed.rotary(qkv, pos, axes, hq + hk, hd, 10000.0)
+    q, k = torch.split(turned, [hq * hd, hk * hd], 1)
+    v = qkv[:, (hq + hk) * hd:]
+    o = packed.attention(q, k, v, packed.plan(starts, n), hd)
+    table = torch.arange(26, dtype=torch.int32, device="cuda").reshape(2, 13)
+    k_pages, v_pages = (torch.zeros(26, hk, ps, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    one = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    got = torch.empty_like(o)
+    for b, (lo, hi) in enumerate(((0, 70), (70, n))):
+        for t in range(lo, hi):
+            row = packed.rotary(qkv[t:t + 1], pos[:, t:t + 1].contiguous(), axes, hq + hk, hd, 10000.0)
+            assert torch.equal(row, turned[t:t + 1])
+            slot = table[b, (t - lo) // ps] * ps + (t - lo) % ps
+            qs = paged.append(torch.cat([row, v[t:t + 1]], 1), torch.zeros(1, dtype=torch.int32, device="cuda"), slot.reshape(1), k_pages, v_pages, 0.0)
+            got[t] = paged.attention(qs, k_pages, v_pages, table[b:b + 1], torch.tensor([t - lo + 1], dtype=torch.int32, device="cuda"), one, 1)[0]
+    for lo, hi in ((0, 70), (70, n)):
+        m = hi - lo
+        qd = q[lo:hi].double().reshape(m, hq, hd)
+        kd, vd = (x[lo:hi].double().reshape(m, hk, hd).repeat_interleave(hq // hk, 1) for x in (k, v))
+        p = torch.softmax((torch.einsum("ihd,jhd->hij", qd, kd) * hd ** -0.5).masked_fill(torch.ones(m, m, dtype=torch.bool, device="cuda").triu(1), float("-inf")), -1)
+        y, mag = (torch.einsum("hij,jhd->ihd", p, x).reshape(m, hq * hd) for x in (vd, vd.abs()))
+        bound = 2.0 ** -8 * y.abs() + (2.0 ** -8 + 2.0 ** -13) * mag
+        for side in (o, got):
+            assert bool(((side[lo:hi].double() - y).abs() <= bound).all())

@@ -374,7 +374,7 @@ class OaTransformerBlock(OaModule):
         plan = self.BlockPlan()
         x = self.Attention.Forward(self.LnAttn.Forward(x), batch, seq, residual=x, pos_offset=pos_offset, mask=mask, packed=packed)
         if self.Moe is not None:
-            x = self.Moe.Forward(x, None if packed is None else packed.Rows())
+            x = self.Moe.Forward(x) if packed is None else self.Moe.Forward(x, packed.Rows())
         elif self.FfnKind == "gelu":
             h = self.LnFfn.Forward(x)
             x = _ffn_gelu(plan, h, self.Ffn1.Weight.Data, self.Ffn1.Bias.Data if self.Ffn1.Bias else None, self.Ffn2.Weight.Data,

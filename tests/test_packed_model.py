@@ -373,3 +373,22 @@ def test_single_tokens_bf16(hq, hk, hd):
         bound = 2.0 ** -8 * y.abs() + (2.0 ** -8 + 2.0 ** -13) * mag
         for side in (o, got):
             assert bool(((side[lo:hi].double() - y).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+def test_bf16_training_on_any_number_of_rows_with_biases():
+    """As above, for the model with layer norms, GELU, biases and learned positions.  A gradient that sums of many terms leave when they cancel (the key bias's is 0) is as near as
+    the sums: 2^-8 of the largest term's products, taken from the weight that the bias belongs to."""
+    model = _model(False, "cuda", heads=2, d=128, dtype=torch.bfloat16)
+    ids, starts, targets, weight = _batch(104, "cuda", pad=10)
+    n = sum(LENGTHS)
+    scale = {}
+    want = None
+    for tokens in (n + 2, n, n + 9):
+        out, _, grads, _ = _step(model, ids, starts, targets, weight, tokens)
+        if want is None:
+            want = (out, grads)
+            scale = {id(b.Attention.KProj.Bias): b.Attention.KProj.Weight.Data.GradTensor().float().abs().max() for b in model.Blocks if b.Attention.KProj.Bias is not None}
+        assert torch.equal(out[:, :n], want[0][:, :n]) and len(grads) == len(want[1])
+        for p, a, b in zip(model.AllParameterPtrs(), grads, want[1]):
+            assert float((a - b).abs().max()) <= 2.0 ** -7 * float(scale.get(id(p), b.abs().max()))

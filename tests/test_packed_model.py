@@ -392,3 +392,34 @@ def test_bf16_training_on_any_number_of_rows_with_biases():
         assert torch.equal(out[:, :n], want[0][:, :n]) and len(grads) == len(want[1])
         for p, a, b in zip(model.AllParameterPtrs(), grads, want[1]):
             assert float((a - b).abs().max()) <= 2.0 ** -7 * float(scale.get(id(p), b.abs().max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("experts", [0, 8])
+def test_scoring_in_a_graph(experts):
+    """The plan, positions, rows and all layers recorded once and replayed on other sequences: the bits of calls made one by one, the experts' balancing loss too."""
+    model = _model(True, "cuda", d=128, dtype=torch.bfloat16, **({"NumExperts": experts, "TopK": 2, "ExpertFf": 64, "AuxAlpha": 0.3} if experts else {}))
+    ids, starts, targets, _ = _batch(104, "cuda", pad=90)
+    n = ids.numel()
+
+    def score():
+        out = model.TokenLogProbs(OaMatrix(ids), OaMatrix(targets), F.PackedSequences(OaMatrix(starts), n)).Tensor()
+        return out, _aux(model).Tensor() if experts else None
+
+    sets = [starts.clone(), torch.tensor([3, 3, 100, 101, 250, 299, 299], dtype=torch.int32, device="cuda"), torch.zeros_like(starts)]
+    want = []
+    for s in sets:
+        starts.copy_(s)
+        want.append([None if t is None else t.clone() for t in score()])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = score()
+    for i in (0, 1, 2, 1):
+        starts.copy_(sets[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        rows = slice(int(sets[i][0]), int(sets[i][-1]))
+        assert torch.equal(got[0][:, rows], want[i][0][:, rows])
+        if experts:
+            assert torch.equal(got[1], want[i][1])

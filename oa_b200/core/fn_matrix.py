@@ -13,6 +13,7 @@ and friends live in `OaFnLoss`.
 from __future__ import annotations
 
 import math
+import operator
 import struct
 from typing import Optional, Sequence
 
@@ -1000,7 +1001,7 @@ class OaPackedSequences:
 
     def __init__(self, plan: PK.PackedPlan, positions: torch.Tensor, pair_axes: Optional[Sequence[int]] = None):
         self.Plan, self.Positions = plan, positions
-        self.PairAxes = None if pair_axes is None else tuple(map(int, pair_axes))
+        self.PairAxes = None if pair_axes is None else tuple(map(operator.index, pair_axes))
 
     def Tokens(self) -> int:
         return self.Plan.tokens
@@ -1029,7 +1030,7 @@ def RotaryAxes(x: OaMatrix, positions: OaMatrix, pair_axes: Sequence[int], heads
     """Rotary embedding of the first `heads` heads of [tokens, >= heads*head_dim] rows by their positions [axes, tokens]: pair j of a head turns with axis
     pair_axes[j].  Returns [tokens, heads*head_dim]; columns behind those heads are not in it."""
     _ctx_add("RotaryAxes")
-    t, pos, axes = x.Tensor(), positions.Tensor(), tuple(map(int, pair_axes))
+    t, pos, axes = x.Tensor(), positions.Tensor(), tuple(map(operator.index, pair_axes))
     out = _w(PK.rotary(t, pos, axes, heads, head_dim, theta))
 
     def back(g):

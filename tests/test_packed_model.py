@@ -423,3 +423,14 @@ def test_scoring_in_a_graph(experts):
         assert torch.equal(got[0][:, rows], want[i][0][:, rows])
         if experts:
             assert torch.equal(got[1], want[i][1])
+
+
+def test_axes_are_whole_numbers():
+    x, pos = OaMatrix(torch.ones(3, 64)), OaMatrix(torch.ones(2, 3, dtype=torch.int32))
+    want = F.RotaryAxes(x, pos, (0, 1) * 16, 1, 64).Tensor()
+    assert torch.equal(F.RotaryAxes(x, pos, torch.tensor([0, 1] * 16), 1, 64).Tensor(), want)
+    for bad in ((0.5,) * 32, ("0",) * 32):
+        with pytest.raises(TypeError):
+            F.RotaryAxes(x, pos, bad, 1, 64)
+        with pytest.raises(TypeError):
+            F.PackedSequences(OaMatrix(torch.tensor([0, 3], dtype=torch.int32)), 3, pos, bad)
